@@ -323,6 +323,151 @@ int mimir_cross_attention_bwd(mimir_ctx* ctx, const float* query_input, int64_t 
                               float* grad_query, int accumulate_query, float* grad_kv, int accumulate_kv);
 
 /* ---------------------------------------------------------------------------
+ * Serving: rotary positions per token, a cache of keys and values in pages, and
+ * attention of new tokens over it.  No counterpart in the reference, whose
+ * attention layers take whole sequences of one length.  Activations are fp32;
+ * device pointers, stream order.
+ * ------------------------------------------------------------------------- */
+
+/* How positions past those a model was trained on are scaled: with f_i =
+ * theta^(-2i/rot_dim), the angle of position p and pair i is p * f'_i and
+ * cos / sin are multiplied by `magnitude`.
+ *   NONE      f' = f
+ *   LINEAR    f' = f / factor (position interpolation)
+ *   BASE      f' = f of theta * factor^(rot_dim / (rot_dim - 2)); rot_dim > 2
+ *   BY_PARTS  r = original_len f / 2pi turns over the original length,
+ *             g = clamp((r - low) / (high - low), 0, 1),
+ *             f' = (1 - g) f / factor + g f; low < high */
+#define MIMIR_ROPE_SCALE_NONE 0
+#define MIMIR_ROPE_SCALE_LINEAR 1
+#define MIMIR_ROPE_SCALE_BASE 2
+#define MIMIR_ROPE_SCALE_BY_PARTS 3
+typedef struct mimir_rope_scaling {
+    int32_t kind;        /* MIMIR_ROPE_SCALE_* */
+    double factor;       /* > 0; read by every kind but NONE */
+    double original_len; /* BY_PARTS: > 0 */
+    double low, high;    /* BY_PARTS */
+    double magnitude;    /* finite; 1 leaves cos / sin as they are */
+} mimir_rope_scaling;
+
+/* mimir_rope_table with scaled frequencies, for positions first .. first + rows - 1:
+ * cos_tab / sin_tab are HOST arrays of rows * rot_dim / 2 floats, each value
+ * computed in double and rounded once.  scaling NULL: NONE with magnitude 1. */
+int mimir_rope_table_scaled(int64_t first, int64_t rows, int64_t rot_dim, double theta,
+                            const mimir_rope_scaling* scaling, float* cos_tab, float* sin_tab);
+
+/* Which dimensions of a head are rotated, and the DEVICE tables [table_rows x
+ * rot_dim / 2] of its positions. */
+typedef struct mimir_rope {
+    const float* cos_tab;
+    const float* sin_tab;
+    int64_t table_rows;
+    int32_t rot_dim;     /* even, 0 < rot_dim <= head_dim; the dimensions from rot_dim on are copied */
+    int32_t interleaved; /* 0: pairs (i, i + rot_dim / 2); 1: pairs (2i, 2i + 1) */
+} mimir_rope;
+
+/* RoPE of packed tokens, each at its own position: row t of q (stride ld_q
+ * floats) holds q_heads heads of head_dim, row t of k (ld_k) k_heads of them, and
+ * token t stands at positions[t] (DEVICE).  For each pair (x0, x1):
+ *   y0 = x0 cos - x1 sin,  y1 = x1 cos + x0 sin
+ * each computed in double and rounded once.  A position outside [0, table_rows)
+ * gives a row of zeros (as the gather's ids do).  q or k may be NULL.  q_out may
+ * be q with the same stride (in place), and k_out k; other overlaps of inputs and
+ * outputs are not allowed.  Any head_dim, stride (>= heads * head_dim) and 4-byte
+ * alignment; multiples of 16 bytes are faster. */
+int mimir_rope_rows_fwd(mimir_ctx* ctx, const float* q, int64_t ld_q, float* q_out, int64_t ld_q_out, int64_t q_heads,
+                        const float* k, int64_t ld_k, float* k_out, int64_t ld_k_out, int64_t k_heads, int64_t tokens,
+                        int64_t head_dim, const int32_t* positions, const mimir_rope* rope);
+/* Its gradient: dq_in (+)= the transposed rotation of dq (cos and sin as they
+ * are, magnitude included), and dk_in of dk; rows of positions outside the table
+ * get zeros (accumulate: nothing).  `accumulate` as for the other backward
+ * entry points.  In place as the forward (without accumulate). */
+int mimir_rope_rows_bwd(mimir_ctx* ctx, const float* dq, int64_t ld_dq, float* dq_in, int64_t ld_dq_in, int64_t q_heads,
+                        const float* dk, int64_t ld_dk, float* dk_in, int64_t ld_dk_in, int64_t k_heads, int64_t tokens,
+                        int64_t head_dim, const int32_t* positions, const mimir_rope* rope, int accumulate);
+
+/* A cache of keys and values in pages of page_size tokens.  k and v are
+ * [pages][kv_heads][page_size][stride] elements, stride = head_dim rounded up to
+ * a multiple of 16; the padding is written as zeros with each row and has to be
+ * finite where a program fills a page by other means.
+ *   MIMIR_KV_F32   4 bytes, the values
+ *   MIMIR_KV_BF16  2 bytes, rounded to nearest even
+ *   MIMIR_KV_I8    1 byte, codes -127 .. 127 that stand for code * scale, with
+ *                  one fp32 scale per token and head in k_scale / v_scale
+ *                  [pages][kv_heads][page_size]: scale = max|x| / 127 of the
+ *                  row, code = x * 127 / max|x| rounded to nearest even (of the
+ *                  exact quotient).  A row of zeros has scale 0; a row with a
+ *                  NaN or an infinity has scale NaN and reads back as NaN. */
+#define MIMIR_KV_F32 0
+#define MIMIR_KV_BF16 1
+#define MIMIR_KV_I8 2
+typedef struct mimir_kv_cache {
+    int32_t dtype;     /* MIMIR_KV_* */
+    int32_t page_size; /* a multiple of 16 */
+    int64_t pages;
+    int32_t kv_heads;
+    int32_t head_dim;  /* 1 .. 256 */
+    void* k;           /* DEVICE, 16-byte aligned, as the other three */
+    void* v;
+    float* k_scale;    /* MIMIR_KV_I8 only */
+    float* v_scale;
+} mimir_kv_cache;
+
+/* Bytes of k (v takes the same) and of k_scale (likewise; 0 without scales). */
+int mimir_kv_cache_bytes(const mimir_kv_cache* cache, size_t* kv_bytes, size_t* scale_bytes);
+
+/* New tokens of several sequences, packed: sequence s has rows token_start[s] ..
+ * token_start[s + 1] - 1 of the activations and kv_len[s] cached tokens, the new
+ * ones included, so that its row i of n stands at position kv_len[s] - n + i.
+ * Position p lies in slot p % page_size of page page_table[s * ld_pages + p /
+ * page_size].  The arrays are DEVICE int32: they may change between two replays
+ * of a captured graph, within the bounds that the call was made with.  No call
+ * reads or writes outside the given buffers, whatever they hold: rows from
+ * token_start[sequences] on are left as they are, tokens past max_new or
+ * max_len are passed over, and a page outside [0, pages) holds no tokens (it is
+ * not written; its keys are not attended; it reads as zeros), nor does a
+ * position below 0.  A slot that two tokens of one call share is left with
+ * either's row or a mixture. */
+typedef struct mimir_kv_batch {
+    int64_t sequences;
+    int64_t tokens;             /* rows of the activations */
+    const int32_t* token_start; /* [sequences + 1], rising from 0 */
+    const int32_t* kv_len;      /* [sequences] */
+    const int32_t* page_table;  /* [sequences][ld_pages] */
+    int64_t ld_pages;
+    int64_t max_new;            /* no sequence has more new tokens */
+    int64_t max_len;            /* nor more cached ones; <= ld_pages * page_size */
+} mimir_kv_batch;
+
+/* Writes the new tokens' keys and values into their pages: row t of k and of v
+ * (stride ld_kv floats) holds kv_heads heads of head_dim.  With `rope` the keys
+ * are rotated on the way, and q (q_heads heads; NULL: none), whose rotation goes
+ * to q_out (rows at positions below 0 get zeros), as mimir_rope_rows_fwd does at
+ * the tokens' positions; max_len <= table_rows.  Without rope, q must be NULL.
+ * q_out may be q with the same stride. */
+int mimir_kv_append(mimir_ctx* ctx, const mimir_kv_cache* cache, const mimir_kv_batch* batch, const float* k,
+                    const float* v, int64_t ld_kv, const mimir_rope* rope, const float* q, int64_t ld_q, float* q_out,
+                    int64_t ld_q_out, int64_t q_heads);
+
+/* Reads them back: row t of k_out / v_out (either may be NULL; stride ld_out)
+ * gets the cached key / value of token t, as fp32.  A batch whose sequences have
+ * kv_len[s] rows each reads whole sequences. */
+int mimir_kv_read(mimir_ctx* ctx, const mimir_kv_cache* cache, const mimir_kv_batch* batch, float* k_out, float* v_out,
+                  int64_t ld_out);
+
+/* mimir_attention_fwd's core for new tokens over their sequences' pages: row t of
+ * q (stride ld_q) and out (ld_out) holds q_heads heads, a multiple of kv_heads; q
+ * head h attends with key / value head h / (q_heads / kv_heads).  Causal: a token
+ * sees the keys up to its own position; else all kv_len[s].  The new tokens'
+ * keys are in the cache already (mimir_kv_append).  fp32 precision as
+ * mimir_attention_fwd, of the values that the cache's entries stand for.  A token
+ * without keys gets zeros; what stands in keys that a token does not see does not
+ * reach it.  out must not overlap q.  Uses the context's 33 MiB workspace
+ * as mimir_attention_fwd does. */
+int mimir_attention_paged_fwd(mimir_ctx* ctx, const mimir_kv_cache* cache, const mimir_kv_batch* batch, const float* q,
+                              int64_t ld_q, float* out, int64_t ld_out, int64_t q_heads, float scale, int causal);
+
+/* ---------------------------------------------------------------------------
  * Backward of the path's ops: the branches of the reference's
  * Model::backwardPass (Model.cpp:7305-9153).  Device pointers, stream order.
  *

@@ -29,6 +29,9 @@ LAYER_TYPES = {"LayerNorm": 1, "RMSNorm": 2, "Softmax": 3, "LogSoftmax": 4, "GEL
 # The reference's BranchType and MergeOperation (Layers.hpp:59-80), in order.
 BRANCH_TYPES = ("NONE", "RESIDUAL", "SKIP_CONNECTION", "DENSE_CONNECTION", "ATTENTION_BRANCH", "MULTI_SCALE",
                 "GATE", "SPLIT", "MERGE")
+# MIMIR_KV_* (element types of a key/value cache) and MIMIR_ROPE_SCALE_*, in order.
+KV_TYPES = ("f32", "bf16", "i8")
+ROPE_SCALINGS = ("none", "linear", "base", "by_parts")
 MERGE_OPS = ("ADD", "MULTIPLY", "CONCATENATE", "MAX", "AVERAGE", "GATED", "ATTENTION_WEIGHTED")
 
 
@@ -68,6 +71,30 @@ class Layer_C(Structure):
                 ("padding_idx", c_int32), ("seq_len", c_int32), ("grad_weights", c_void_p),
                 ("branch_type", c_int32), ("merge_op", c_int32), ("branch_sources", POINTER(c_int32)),
                 ("n_branch_sources", c_int32), ("num_heads", c_int32), ("head_dim", c_int32), ("causal", c_int32)]
+
+
+class RopeScaling_C(Structure):
+    """struct mimir_rope_scaling."""
+    _fields_ = [("kind", c_int32), ("factor", c_double), ("original_len", c_double), ("low", c_double),
+                ("high", c_double), ("magnitude", c_double)]
+
+
+class Rope_C(Structure):
+    """struct mimir_rope."""
+    _fields_ = [("cos_tab", c_void_p), ("sin_tab", c_void_p), ("table_rows", c_int64), ("rot_dim", c_int32),
+                ("interleaved", c_int32)]
+
+
+class KVCache_C(Structure):
+    """struct mimir_kv_cache."""
+    _fields_ = [("dtype", c_int32), ("page_size", c_int32), ("pages", c_int64), ("kv_heads", c_int32),
+                ("head_dim", c_int32), ("k", c_void_p), ("v", c_void_p), ("k_scale", c_void_p), ("v_scale", c_void_p)]
+
+
+class KVBatch_C(Structure):
+    """struct mimir_kv_batch."""
+    _fields_ = [("sequences", c_int64), ("tokens", c_int64), ("token_start", c_void_p), ("kv_len", c_void_p),
+                ("page_table", c_void_p), ("ld_pages", c_int64), ("max_new", c_int64), ("max_len", c_int64)]
 
 
 # name -> (restype, argtypes); mirrors include/mimir_hip.h one to one.
@@ -111,6 +138,17 @@ SIGNATURES = {
                                     c_int64, c_int64, c_float, c_int]),
     "mimir_self_attention_fwd": (c_int, [_P, _P, c_int64, c_int64, c_int64, c_int, _P, c_int64, _P]),
     "mimir_cross_attention_fwd": (c_int, [_P, _P, c_int64, _P, c_int64, c_int64, c_int64, c_int, _P, c_int64, _P]),
+    "mimir_rope_table_scaled": (c_int, [c_int64, c_int64, c_int64, c_double, POINTER(RopeScaling_C), _P, _P]),
+    "mimir_rope_rows_fwd": (c_int, [_P, _P, c_int64, _P, c_int64, c_int64, _P, c_int64, _P, c_int64, c_int64, c_int64,
+                                    c_int64, _P, POINTER(Rope_C)]),
+    "mimir_rope_rows_bwd": (c_int, [_P, _P, c_int64, _P, c_int64, c_int64, _P, c_int64, _P, c_int64, c_int64, c_int64,
+                                    c_int64, _P, POINTER(Rope_C), c_int]),
+    "mimir_kv_cache_bytes": (c_int, [POINTER(KVCache_C), POINTER(c_size_t), POINTER(c_size_t)]),
+    "mimir_kv_append": (c_int, [_P, POINTER(KVCache_C), POINTER(KVBatch_C), _P, _P, c_int64, POINTER(Rope_C), _P, c_int64,
+                                _P, c_int64, c_int64]),
+    "mimir_kv_read": (c_int, [_P, POINTER(KVCache_C), POINTER(KVBatch_C), _P, _P, c_int64]),
+    "mimir_attention_paged_fwd": (c_int, [_P, POINTER(KVCache_C), POINTER(KVBatch_C), _P, c_int64, _P, c_int64, c_int64,
+                                          c_float, c_int]),
     "mimir_attention_bwd": (c_int, [_P, _P, c_int64, _P, _P, c_int64, _P, c_int64, _P, c_int64, _P, _P, c_int64,
                                     c_int64, c_int64, c_int64, c_int64, c_int64, c_float, c_int]),
     "mimir_self_attention_bwd": (c_int, [_P, _P, _P, c_int64, c_int64, c_int64, c_int, _P, c_int64, _P, _P, c_int]),

@@ -230,6 +230,48 @@ class Context:
                                                       num_heads, int(bool(causal)), _ptr(weights), weights_len,
                                                       _ptr(out)))
 
+    # -- serving: positions per token, a paged cache, attention over it --------
+
+    def rope_rows(self, q, q_out, q_heads, k, k_out, k_heads, tokens, head_dim, positions, rope: "Rope", ld_q=None,
+                  ld_k=None, ld_q_out=None, ld_k_out=None):
+        """mimir_rope_rows_fwd: each token of q and k (either may be None) rotated
+        at its own position; the row strides default to heads * head_dim."""
+        wq, wk = q_heads * head_dim, k_heads * head_dim
+        self.check(self.lib.mimir_rope_rows_fwd(self.handle, _ptr(q), ld_q or wq, _ptr(q_out), ld_q_out or wq, q_heads,
+                                                _ptr(k), ld_k or wk, _ptr(k_out), ld_k_out or wk, k_heads, tokens,
+                                                head_dim, _ptr(positions), rope.c))
+
+    def rope_rows_bwd(self, dq, dq_in, q_heads, dk, dk_in, k_heads, tokens, head_dim, positions, rope: "Rope", ld_q=None,
+                      ld_k=None, ld_q_out=None, ld_k_out=None, accumulate=False):
+        """mimir_rope_rows_bwd: the transposed rotation of dq and dk."""
+        wq, wk = q_heads * head_dim, k_heads * head_dim
+        self.check(self.lib.mimir_rope_rows_bwd(self.handle, _ptr(dq), ld_q or wq, _ptr(dq_in), ld_q_out or wq, q_heads,
+                                                _ptr(dk), ld_k or wk, _ptr(dk_in), ld_k_out or wk, k_heads, tokens,
+                                                head_dim, _ptr(positions), rope.c, int(bool(accumulate))))
+
+    def kv_append(self, cache: "KVCache", batch: "KVBatch", k, v, ld_kv=None, rope: "Rope" = None, q=None, q_out=None,
+                  heads=0, ld_q=None, ld_q_out=None):
+        """mimir_kv_append: the batch's new keys and values into their pages; with
+        `rope` the keys are rotated on the way, and q (`heads` heads) into q_out."""
+        wk, wq = cache.kv_heads * cache.head_dim, heads * cache.head_dim
+        self.check(self.lib.mimir_kv_append(self.handle, cache.c, batch.c, _ptr(k), _ptr(v), ld_kv or wk,
+                                            rope.c if rope is not None else None, _ptr(q), ld_q or wq, _ptr(q_out),
+                                            ld_q_out or wq, heads))
+
+    def kv_read(self, cache: "KVCache", batch: "KVBatch", k_out, v_out, ld_out=None):
+        """mimir_kv_read: the batch's cached keys and values as fp32 (either output may be None)."""
+        self.check(self.lib.mimir_kv_read(self.handle, cache.c, batch.c, _ptr(k_out), _ptr(v_out),
+                                          ld_out or cache.kv_heads * cache.head_dim))
+
+    def attention_paged(self, cache: "KVCache", batch: "KVBatch", q, out, heads, causal=True, scale=None, ld_q=None,
+                        ld_out=None):
+        """mimir_attention_paged_fwd: the batch's new tokens attend over their
+        sequences' pages; scale defaults to 1 / sqrt(head_dim) as attention()'s."""
+        width = heads * cache.head_dim
+        self.check(self.lib.mimir_attention_paged_fwd(self.handle, cache.c, batch.c, _ptr(q), ld_q or width, _ptr(out),
+                                                      ld_out or width, heads, cache.scale if scale is None else float(scale),
+                                                      int(bool(causal))))
+
     # -- backward (Model::backwardPass branches) -------------------------------
 
     def attention_bwd(self, q, k, v, dout, dq, dk, dv, batch, q_len, kv_len, heads, head_dim, causal=False,
@@ -321,6 +363,81 @@ def rope_table(rows, head_dim, theta=10000.0):
     if st != OK:
         raise MimirError(st, "mimir_rope_table: invalid argument")
     return c, s
+
+
+def rope_table_scaled(rows, rot_dim, theta=10000.0, kind="none", factor=1.0, original_len=1.0, low=1.0, high=32.0,
+                      magnitude=1.0, first=0):
+    """Host cos/sin tables [rows x rot_dim/2] of positions first .. first + rows - 1
+    from mimir_rope_table_scaled; kind: "none", "linear", "base" or "by_parts"."""
+    lib = _lib.load()
+    c = np.empty((rows, rot_dim // 2), np.float32)
+    s = np.empty((rows, rot_dim // 2), np.float32)
+    z = _lib.RopeScaling_C(_lib.ROPE_SCALINGS.index(kind), factor, original_len, low, high, magnitude)
+    st = lib.mimir_rope_table_scaled(first, rows, rot_dim, float(theta), byref(z), c.ctypes.data_as(c_void_p),
+                                     s.ctypes.data_as(c_void_p))
+    if st != OK:
+        raise MimirError(st, "mimir_rope_table_scaled: invalid argument")
+    return c, s
+
+
+def _address(x):
+    p = _ptr(x)
+    return p.value if p is not None else None
+
+
+class Rope:
+    """Which dimensions of a head are rotated, and the device tables of its
+    positions [table_rows x rot_dim/2] (``mimir_rope``).  Keeps its arguments alive."""
+
+    def __init__(self, cos_tab, sin_tab, table_rows, rot_dim, interleaved=False):
+        self._held = (cos_tab, sin_tab)
+        self.c = _lib.Rope_C(_address(cos_tab), _address(sin_tab), table_rows, rot_dim, int(bool(interleaved)))
+
+
+class KVCache:
+    """A cache of keys and values in pages (``mimir_kv_cache``): given buffers
+    (DeviceArrays or device addresses, [pages][kv_heads][page_size][stride] elements,
+    and [pages][kv_heads][page_size] scales for "i8"), or, with k None, buffers of
+    its own, which close() frees.  dtype: "f32", "bf16" or "i8"."""
+
+    def __init__(self, ctx, dtype, pages, page_size, kv_heads, head_dim, k=None, v=None, k_scale=None, v_scale=None):
+        self.ctx, self.dtype, self.kv_heads, self.head_dim = ctx, dtype, int(kv_heads), int(head_dim)
+        self.stride = (self.head_dim + 15) // 16 * 16
+        self.scale = float(np.float32(1.0) / np.sqrt(np.float32(max(self.head_dim, 1))))  # LayerOps.hpp:1047
+        self._own = []
+        kind = _lib.KV_TYPES.index(dtype)
+        self.c = _lib.KVCache_C(kind, page_size, pages, kv_heads, head_dim)
+        if k is None:
+            kv, scale = ctypes.c_size_t(), ctypes.c_size_t()
+            if ctx.lib.mimir_kv_cache_bytes(self.c, byref(kv), byref(scale)) != OK:
+                raise MimirError(EINVAL, f"KV cache: page_size {page_size}, kv_heads {kv_heads}, head_dim {head_dim}")
+            rows = (pages, kv_heads, page_size)
+            np_type = (np.float32, np.uint16, np.int8)[kind]
+            self._own = [ctx.empty(rows + (self.stride,), np_type) for _ in range(2)]
+            if kind == 2:
+                self._own += [ctx.empty(rows) for _ in range(2)]
+            k, v, k_scale, v_scale = (self._own + [None, None])[:4]
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        if dtype != "i8":
+            k_scale = v_scale = None
+        self.c.k, self.c.v = _address(k), _address(v)
+        self.c.k_scale, self.c.v_scale = _address(k_scale), _address(v_scale)
+
+    def close(self):
+        for b in self._own:
+            b.free()
+        self._own = []
+
+
+class KVBatch:
+    """New tokens of several sequences and their page tables (``mimir_kv_batch``):
+    device int32 arrays token_start [sequences + 1], kv_len [sequences] and
+    page_table [sequences][ld_pages].  Keeps its arguments alive."""
+
+    def __init__(self, token_start, kv_len, page_table, sequences, tokens, ld_pages, max_new, max_len):
+        self._held = (token_start, kv_len, page_table)
+        self.c = _lib.KVBatch_C(sequences, tokens, _address(token_start), _address(kv_len), _address(page_table), ld_pages,
+                                max_new, max_len)
 
 
 class Store:

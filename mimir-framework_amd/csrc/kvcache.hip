@@ -2,10 +2,9 @@
 // into their pages (keys and queries rotated on the way), and read back.
 //
 // Bound by HBM: q, k and v are read once and written once, in the cache's type.
-// LPR lanes hold a head row, eight elements each (two 16-byte vectors: a rotated
-// part's first and second elements, or two side by side), so that the largest
-// absolute value of an 8-bit row is a few lane exchanges away and nothing is read
-// twice.  A workgroup takes rows of one token, whose sequence its waves search in
+// LPR lanes hold a head row, eight elements each (two vectors, kvcache.hpp
+// unit_place), so that the largest absolute value of an 8-bit row is a few lane
+// exchanges away and nothing is read twice.  A workgroup takes rows of one token, whose sequence its waves search in
 // token_start while the row is on its way.
 //
 // Numerics.  Rotation in double, rounded once (rotate_pair).  An 8-bit code is the
@@ -79,166 +78,124 @@ __device__ __forceinline__ void put(char* row, int at, const float* x) {
 }
 
 // W: elements per vector, 4 where every row of q, k, v and q_out is whole 16-byte
-// vectors; UN units of 2 W elements per lane; ROWS head rows per lane group.
-template <int DT, int LPR, int W, int ROWS>
+// vectors; UN units of 2 W elements per lane; T tokens, the same row of each.
+template <int DT, int LPR, int W, int T>
 __global__ __launch_bounds__(kBlock) void kv_append(AppendArgs a) {
     constexpr int UN = 4 / W;  // 8 elements a lane
     constexpr int kGroups = kBlock / LPR;
-    const uint32_t t = blockIdx.x / a.parts, part = blockIdx.x % a.parts;
+    const uint32_t t0 = blockIdx.x / a.parts * T, part = blockIdx.x % a.parts;
     const int lane = threadIdx.x % LPR, group = threadIdx.x / LPR;
-    const int rows = a.q_heads + 2 * a.c.kv_heads, d = a.c.head_dim;
-    float lo[ROWS][UN][W], hi[ROWS][UN][W];
-    int row[ROWS];
-    // Where a unit's vectors stand in a row.  Values are not rotated: their units
-    // lie side by side.
-    const auto place = [&](int u, bool turned, int* d0, int* d1) {
-        const bool split = turned && u * W < a.half && !a.interleaved;
-        *d0 = split ? u * W : 2 * u * W;
-        *d1 = split ? a.half + u * W : 2 * u * W + W;
-    };
-#pragma unroll
-    for (int j = 0; j < ROWS; ++j) {
-        row[j] = (static_cast<int>(part) * ROWS + j) * kGroups + group;
-        const bool is_q = row[j] < a.q_heads, is_k = !is_q && row[j] < a.q_heads + a.c.kv_heads;
-        const int head = is_q ? row[j] : row[j] - a.q_heads - (is_k ? 0 : a.c.kv_heads);
-        const float* x = is_q ? a.q + t * a.ld_q : (is_k ? a.k : a.v) + t * a.ld_kv;
-        x += static_cast<int64_t>(head) * d;
-#pragma unroll
-        for (int n = 0; n < UN; ++n) {
-            int d0, d1;
-            place(lane + n * LPR, is_q || is_k, &d0, &d1);
-#pragma unroll
-            for (int e = 0; e < W; ++e) lo[j][n][e] = hi[j][n][e] = 0.f;
-            if (row[j] >= rows) continue;
-            if constexpr (W == 4) {
-                if (d0 < d) {
-                    const f4 v = ld4<true>(x + d0);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) lo[j][n][e] = v[e];
-                }
-                if (d1 < d) {
-                    const f4 v = ld4<true>(x + d1);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) hi[j][n][e] = v[e];
-                }
-            } else {
-                if (d0 < d) lo[j][n][0] = x[d0];
-                if (d1 < d) hi[j][n][0] = x[d1];
-            }
-        }
-    }
-
-    const int s = kv_sequence_of(a.b, static_cast<int>(t));
-    if (s < 0) return;
-    const KvSequence seq = kv_sequence(a.b, s);
-    const int i = static_cast<int>(t) - seq.first;
-    if (i < 0 || i >= seq.n) return;
-    const int pos = seq.len - seq.n + i;
-    // Page and slot of the token; a negative page: nothing is written.
-    const auto [page, slot] = kv_slot(a.b, a.c.pages, a.c.page_div, s, pos);
-    float c[UN][W], sn[UN][W];
+    const int d = a.c.head_dim, row = static_cast<int>(part) * kGroups + group;
+    const bool is_q = row < a.q_heads, is_k = !is_q && row < a.q_heads + a.c.kv_heads;
+    const bool mine = row < a.q_heads + 2 * a.c.kv_heads;
+    const int head = is_q ? row : row - a.q_heads - (is_k ? 0 : a.c.kv_heads);
+    const int half = is_q || is_k ? a.half : 0;  // values are not rotated
+    const int64_t ld = is_q ? a.ld_q : a.ld_kv;
+    const float* x = (is_q ? a.q : is_k ? a.k : a.v) + t0 * ld + static_cast<int64_t>(head) * d;
+    float lo[T][UN][W], hi[T][UN][W];
+    UnitPlace at[UN];
 #pragma unroll
     for (int n = 0; n < UN; ++n) {
-        const int p = (lane + n * LPR) * W;
-        const bool in = pos >= 0 && p < a.half;
-        const int64_t at = static_cast<int64_t>(pos) * a.half + p;
+        at[n] = unit_place<W>(lane + n * LPR, half, a.interleaved, a.c.stride);
 #pragma unroll
-        for (int e = 0; e < W; ++e) {
-            c[n][e] = in ? a.cos_tab[at + e] : 1.f;
-            sn[n][e] = in ? a.sin_tab[at + e] : 0.f;
+        for (int i = 0; i < T; ++i) {
+#pragma unroll
+            for (int e = 0; e < W; ++e) lo[i][n][e] = hi[i][n][e] = 0.f;
+            if (!mine || static_cast<int64_t>(t0) + i >= a.b.tokens) continue;
+            if constexpr (W == 4) {
+                if (at[n].d0 < d) {
+                    const f4 v = ld4<true>(x + i * ld + at[n].d0);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) lo[i][n][e] = v[e];
+                }
+                if (at[n].d1 < d) {
+                    const f4 v = ld4<true>(x + i * ld + at[n].d1);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) hi[i][n][e] = v[e];
+                }
+            } else {
+                if (at[n].d0 < d) lo[i][n][0] = x[i * ld + at[n].d0];
+                if (at[n].d1 < d) hi[i][n][0] = x[i * ld + at[n].d1];
+            }
         }
     }
 
+    int s[T];
+    KvToken tok[T];
+    kv_sequences_of<T>(a.b, static_cast<int>(t0), s);
 #pragma unroll
-    for (int j = 0; j < ROWS; ++j) {
-        const bool is_q = row[j] < a.q_heads, is_k = !is_q && row[j] < a.q_heads + a.c.kv_heads;
-        if (is_q || is_k) {
+    for (int i = 0; i < T; ++i) tok[i] = kv_token(a.b, a.c, s[i], static_cast<int>(t0) + i);
+    float c[T][UN][W], sn[T][UN][W];
 #pragma unroll
-            for (int n = 0; n < UN; ++n) {
-                if ((lane + n * LPR) * W >= a.half) continue;
-                if (a.interleaved) {
-                    float x[2 * W];
+    for (int i = 0; i < T; ++i)
 #pragma unroll
-                    for (int e = 0; e < W; ++e) {
-                        x[e] = lo[j][n][e];
-                        x[W + e] = hi[j][n][e];
-                    }
+        for (int n = 0; n < UN; ++n)
+            if (at[n].turned && tok[i].position >= 0)
+                unit_turns<W>(a.cos_tab, a.sin_tab, static_cast<int64_t>(tok[i].position) * a.half, lane + n * LPR, a.half,
+                              a.interleaved, c[i][n], sn[i][n]);
+
 #pragma unroll
-                    for (int e = 0; e < W; ++e) rotate_pair(x[2 * e], x[2 * e + 1], c[n][e], sn[n][e]);
+    for (int i = 0; i < T; ++i) {
+        if (!tok[i].in) continue;
 #pragma unroll
-                    for (int e = 0; e < W; ++e) {
-                        lo[j][n][e] = x[e];
-                        hi[j][n][e] = x[W + e];
-                    }
-                } else {
-#pragma unroll
-                    for (int e = 0; e < W; ++e) rotate_pair(lo[j][n][e], hi[j][n][e], c[n][e], sn[n][e]);
-                }
-            }
-        }
+        for (int n = 0; n < UN; ++n)
+            if (at[n].turned && tok[i].position >= 0) unit_rotate<W>(lo[i][n], hi[i][n], c[i][n], sn[i][n], a.interleaved);
         if (is_q) {
-            float* y = a.q_out + t * a.ld_q_out + static_cast<int64_t>(row[j]) * d;
+            char* y = reinterpret_cast<char*>(a.q_out + (t0 + i) * a.ld_q_out + static_cast<int64_t>(head) * d);
 #pragma unroll
             for (int n = 0; n < UN; ++n) {
-                int d0, d1;
-                place(lane + n * LPR, true, &d0, &d1);
-                if (pos < 0) {
+                if (tok[i].position < 0) {
 #pragma unroll
-                    for (int e = 0; e < W; ++e) lo[j][n][e] = hi[j][n][e] = 0.f;
+                    for (int e = 0; e < W; ++e) lo[i][n][e] = hi[i][n][e] = 0.f;
                 }
-                if (d0 < d) put<MIMIR_KV_F32, W>(reinterpret_cast<char*>(y), d0, lo[j][n]);
-                if (d1 < d) put<MIMIR_KV_F32, W>(reinterpret_cast<char*>(y), d1, hi[j][n]);
+                if (at[n].d0 < d) put<MIMIR_KV_F32, W>(y, at[n].d0, lo[i][n]);
+                if (at[n].d1 < d) put<MIMIR_KV_F32, W>(y, at[n].d1, hi[i][n]);
             }
             continue;
         }
-        const bool mine = row[j] < rows && page >= 0;
-        const int head = row[j] - a.q_heads - (is_k ? 0 : a.c.kv_heads);
-        const int64_t at = mine ? (static_cast<int64_t>(page) * a.c.kv_heads + head) * a.c.page_size + slot : 0;
+        const bool held = mine && tok[i].page >= 0;
+        const int64_t slot = held ? (static_cast<int64_t>(tok[i].page) * a.c.kv_heads + head) * a.c.page_size + tok[i].slot : 0;
         if constexpr (DT == MIMIR_KV_I8) {
             uint32_t bits = 0;  // all lanes of the group come here together
 #pragma unroll
             for (int n = 0; n < UN; ++n)
 #pragma unroll
                 for (int e = 0; e < W; ++e) {
-                    bits = max(bits, __builtin_bit_cast(uint32_t, lo[j][n][e]) & 0x7fffffffu);
-                    bits = max(bits, __builtin_bit_cast(uint32_t, hi[j][n][e]) & 0x7fffffffu);
+                    bits = max(bits, __builtin_bit_cast(uint32_t, lo[i][n][e]) & 0x7fffffffu);
+                    bits = max(bits, __builtin_bit_cast(uint32_t, hi[i][n][e]) & 0x7fffffffu);
                 }
             bits = lanes_max<LPR>(bits);
-            if (!mine) continue;
+            if (!held) continue;
             const bool finite = bits < 0x7f800000u;
             const float most = __builtin_bit_cast(float, bits), inv = 127.f / most;
-            char* out = (is_k ? a.c.k : a.c.v) + at * a.c.stride;
-            if (lane == 0) (is_k ? a.c.k_scale : a.c.v_scale)[at] = finite ? most / 127.f : __builtin_nanf("");
+            char* out = (is_k ? a.c.k : a.c.v) + slot * a.c.stride;
+            if (lane == 0) (is_k ? a.c.k_scale : a.c.v_scale)[slot] = finite ? most / 127.f : __builtin_nanf("");
             const bool codes = finite && bits > 0;
 #pragma unroll
             for (int n = 0; n < UN; ++n) {
-                int d0, d1;
-                place(lane + n * LPR, is_k, &d0, &d1);
                 uint32_t l = 0, h = 0;
                 if (codes) {
 #pragma unroll
                     for (int e = 0; e < W; ++e) {
-                        l |= static_cast<uint32_t>(code_of(lo[j][n][e], most, inv) & 0xff) << (8 * e);
-                        h |= static_cast<uint32_t>(code_of(hi[j][n][e], most, inv) & 0xff) << (8 * e);
+                        l |= static_cast<uint32_t>(code_of(lo[i][n][e], most, inv) & 0xff) << (8 * e);
+                        h |= static_cast<uint32_t>(code_of(hi[i][n][e], most, inv) & 0xff) << (8 * e);
                     }
                 }
                 if constexpr (W == 4) {
-                    if (d0 < a.c.stride) *reinterpret_cast<uint32_t*>(out + d0) = l;
-                    if (d1 < a.c.stride) *reinterpret_cast<uint32_t*>(out + d1) = h;
+                    if (at[n].d0 < a.c.stride) *reinterpret_cast<uint32_t*>(out + at[n].d0) = l;
+                    if (at[n].d1 < a.c.stride) *reinterpret_cast<uint32_t*>(out + at[n].d1) = h;
                 } else {
-                    if (d0 < a.c.stride) out[d0] = static_cast<char>(l);
-                    if (d1 < a.c.stride) out[d1] = static_cast<char>(h);
+                    if (at[n].d0 < a.c.stride) out[at[n].d0] = static_cast<char>(l);
+                    if (at[n].d1 < a.c.stride) out[at[n].d1] = static_cast<char>(h);
                 }
             }
         } else {
-            if (!mine) continue;
-            char* out = (is_k ? a.c.k : a.c.v) + at * a.c.stride * (DT == MIMIR_KV_F32 ? 4 : 2);
+            if (!held) continue;
+            char* out = (is_k ? a.c.k : a.c.v) + slot * a.c.stride * (DT == MIMIR_KV_F32 ? 4 : 2);
 #pragma unroll
             for (int n = 0; n < UN; ++n) {
-                int d0, d1;
-                place(lane + n * LPR, is_k, &d0, &d1);
-                if (d0 < a.c.stride) put<DT, W>(out, d0, lo[j][n]);
-                if (d1 < a.c.stride) put<DT, W>(out, d1, hi[j][n]);
+                if (at[n].d0 < a.c.stride) put<DT, W>(out, at[n].d0, lo[i][n]);
+                if (at[n].d1 < a.c.stride) put<DT, W>(out, at[n].d1, hi[i][n]);
             }
         }
     }
@@ -254,55 +211,75 @@ struct ReadArgs {
     uint32_t parts;  // workgroups per token
 };
 
-// LPR lanes per row, eight elements each.  VEC: 16-byte stores.
-template <int DT, int LPR, bool VEC>
+// Four elements of a cache row, as the type's bits.
+template <int DT>
+__device__ __forceinline__ u4 get(const char* row, int at) {
+    if constexpr (DT == MIMIR_KV_F32) return *reinterpret_cast<const u4*>(row + 4 * at);
+    else if constexpr (DT == MIMIR_KV_BF16) {
+        const uint64_t w = *reinterpret_cast<const uint64_t*>(row + 2 * at);
+        return u4{static_cast<uint32_t>(w), static_cast<uint32_t>(w >> 32), 0, 0};
+    } else return u4{*reinterpret_cast<const uint32_t*>(row + at), 0, 0, 0};
+}
+
+template <int DT>
+__device__ __forceinline__ f4 value_of(u4 w, float scale) {
+    if constexpr (DT == MIMIR_KV_F32) return __builtin_bit_cast(f4, w);
+    else if constexpr (DT == MIMIR_KV_BF16)
+        return __builtin_bit_cast(f4, u4{w[0] << 16, w[0] & 0xffff0000u, w[1] << 16, w[1] & 0xffff0000u});
+    else {
+        f4 x;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = static_cast<float>(static_cast<int8_t>(w[0] >> (8 * e))) * scale;
+        return x;
+    }
+}
+
+// LPR lanes per row, two vectors of four elements each (unit_place); T tokens, the
+// same row of each.  VEC: 16-byte stores.
+template <int DT, int LPR, bool VEC, int T>
 __global__ __launch_bounds__(kBlock) void kv_read(ReadArgs a) {
     constexpr int kGroups = kBlock / LPR;
-    const uint32_t t = blockIdx.x / a.parts, part = blockIdx.x % a.parts;
+    const uint32_t t0 = blockIdx.x / a.parts * T, part = blockIdx.x % a.parts;
     const int lane = threadIdx.x % LPR, group = threadIdx.x / LPR;
-    const int s = kv_sequence_of(a.b, static_cast<int>(t));
-    if (s < 0) return;
-    const KvSequence seq = kv_sequence(a.b, s);
-    const int i = static_cast<int>(t) - seq.first;
-    if (i < 0 || i >= seq.n) return;
-    const int pos = seq.len - seq.n + i;
-    const auto [page, slot] = kv_slot(a.b, a.c.pages, a.c.page_div, s, pos);
+    int s[T];
+    KvToken tok[T];
+    kv_sequences_of<T>(a.b, static_cast<int>(t0), s);
+#pragma unroll
+    for (int i = 0; i < T; ++i) tok[i] = kv_token(a.b, a.c, s[i], static_cast<int>(t0) + i);
     const int row = static_cast<int>(part) * kGroups + group;
     if (row >= a.kinds * a.c.kv_heads) return;
     const bool is_k = a.k_out && row < a.c.kv_heads;
-    const int head = row % a.c.kv_heads, d0 = 8 * lane;
-    if (d0 >= a.c.head_dim) return;
-    float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (page >= 0) {
-        const int64_t at = (static_cast<int64_t>(page) * a.c.kv_heads + head) * a.c.page_size + slot;
-        const char* in = (is_k ? a.c.k : a.c.v) + (at * a.c.stride + d0) * (DT == MIMIR_KV_F32 ? 4 : DT == MIMIR_KV_BF16 ? 2 : 1);
-        if constexpr (DT == MIMIR_KV_F32) {
-            const f4 l = ld4<true>(reinterpret_cast<const float*>(in)), h = ld4<true>(reinterpret_cast<const float*>(in) + 4);
+    const int head = row % a.c.kv_heads;
+    const auto [d0, d1, turned] = unit_place<4>(lane, 0, false, a.c.stride);
+    if (d1 >= a.c.stride) return;
+    u4 lo[T], hi[T];
+    float scale[T];
+#pragma unroll
+    for (int i = 0; i < T; ++i) {
+        lo[i] = hi[i] = u4{0, 0, 0, 0};
+        scale[i] = 0.f;
+        if (tok[i].page < 0) continue;
+        const int64_t at = (static_cast<int64_t>(tok[i].page) * a.c.kv_heads + head) * a.c.page_size + tok[i].slot;
+        const char* in = (is_k ? a.c.k : a.c.v) + at * a.c.stride * (DT == MIMIR_KV_F32 ? 4 : DT == MIMIR_KV_BF16 ? 2 : 1);
+        lo[i] = get<DT>(in, d0);
+        hi[i] = get<DT>(in, d1);
+        if constexpr (DT == MIMIR_KV_I8) scale[i] = (is_k ? a.c.k_scale : a.c.v_scale)[at];
+    }
+#pragma unroll
+    for (int i = 0; i < T; ++i) {
+        if (!tok[i].in) continue;
+        float* y = (is_k ? a.k_out : a.v_out) + (t0 + i) * a.ld_out + static_cast<int64_t>(head) * a.c.head_dim;
+        const f4 l = value_of<DT>(lo[i], scale[i]), h = value_of<DT>(hi[i], scale[i]);
+        if constexpr (VEC) {
+            if (d0 < a.c.head_dim) st_stream(y + d0, l);
+            if (d1 < a.c.head_dim) st_stream(y + d1, h);
+        } else {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                x[e] = l[e];
-                x[4 + e] = h[e];
+                if (d0 + e < a.c.head_dim) y[d0 + e] = l[e];
+                if (d1 + e < a.c.head_dim) y[d1 + e] = h[e];
             }
-        } else if constexpr (DT == MIMIR_KV_BF16) {
-            const u4 w = *reinterpret_cast<const u4*>(in);
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-                x[e] = __builtin_bit_cast(float, e % 2 ? w[e / 2] & 0xffff0000u : w[e / 2] << 16);
-        } else {
-            const uint64_t w = *reinterpret_cast<const uint64_t*>(in);
-            const float scale = (is_k ? a.c.k_scale : a.c.v_scale)[at];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = static_cast<float>(static_cast<int8_t>(w >> (8 * e))) * scale;
         }
-    }
-    float* y = (is_k ? a.k_out : a.v_out) + t * a.ld_out + static_cast<int64_t>(head) * a.c.head_dim + d0;
-    if constexpr (VEC) {
-        st_stream(y, f4{x[0], x[1], x[2], x[3]});
-        if (d0 + 4 < a.c.head_dim) st_stream(y + 4, f4{x[4], x[5], x[6], x[7]});
-    } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-            if (d0 + e < a.c.head_dim) y[e] = x[e];
     }
 }
 
@@ -313,6 +290,10 @@ int with_lanes(int stride, Fn&& f) {
     if (stride <= 128) return f(std::integral_constant<int, 16>{});
     return f(std::integral_constant<int, 32>{});
 }
+
+// Tokens of a workgroup where there are enough for the GPU.
+constexpr int kTokens = 4;
+bool several_tokens(int64_t tokens, int64_t parts) { return tokens / kTokens * parts >= 2048; }
 
 template <class Fn>
 int with_type(int dtype, Fn&& f) {
@@ -418,11 +399,15 @@ int mimir_kv_append(mimir_ctx* ctx, const mimir_kv_cache* cache, const mimir_kv_
             constexpr int LPR = decltype(lpr)::value, DT = decltype(dt)::value;
             constexpr int64_t kGroups = kBlock / LPR;
             a.parts = static_cast<uint32_t>((rows + kGroups - 1) / kGroups);
-            const int64_t blocks = batch->tokens * a.parts;
+            const bool many = several_tokens(batch->tokens, a.parts);
+            const int64_t blocks = (many ? (batch->tokens + kTokens - 1) / kTokens : batch->tokens) * a.parts;
             MIMIR_REQUIRE(ctx, dispatch_fits(blocks, kBlock), "%s: grid of %lld workgroups exceeds the limit", what,
                           (long long)blocks);
-            if (vec) kv_append<DT, LPR, 4, 1><<<static_cast<unsigned>(blocks), kBlock, 0, ctx->stream>>>(a);
-            else kv_append<DT, LPR, 1, 1><<<static_cast<unsigned>(blocks), kBlock, 0, ctx->stream>>>(a);
+            const auto grid = static_cast<unsigned>(blocks);
+            if (vec && many) kv_append<DT, LPR, 4, kTokens><<<grid, kBlock, 0, ctx->stream>>>(a);
+            else if (vec) kv_append<DT, LPR, 4, 1><<<grid, kBlock, 0, ctx->stream>>>(a);
+            else if (many) kv_append<DT, LPR, 1, kTokens><<<grid, kBlock, 0, ctx->stream>>>(a);
+            else kv_append<DT, LPR, 1, 1><<<grid, kBlock, 0, ctx->stream>>>(a);
             return launched(ctx, "kv_append");
         });
     });
@@ -449,11 +434,15 @@ int mimir_kv_read(mimir_ctx* ctx, const mimir_kv_cache* cache, const mimir_kv_ba
             constexpr int LPR = decltype(lpr)::value, DT = decltype(dt)::value;
             constexpr int64_t kGroups = kBlock / LPR;
             a.parts = static_cast<uint32_t>((static_cast<int64_t>(a.kinds) * cache->kv_heads + kGroups - 1) / kGroups);
-            const int64_t blocks = batch->tokens * a.parts;
+            const bool many = several_tokens(batch->tokens, a.parts);
+            const int64_t blocks = (many ? (batch->tokens + kTokens - 1) / kTokens : batch->tokens) * a.parts;
             MIMIR_REQUIRE(ctx, dispatch_fits(blocks, kBlock), "%s: grid of %lld workgroups exceeds the limit", what,
                           (long long)blocks);
-            if (vec) kv_read<DT, LPR, true><<<static_cast<unsigned>(blocks), kBlock, 0, ctx->stream>>>(a);
-            else kv_read<DT, LPR, false><<<static_cast<unsigned>(blocks), kBlock, 0, ctx->stream>>>(a);
+            const auto grid = static_cast<unsigned>(blocks);
+            if (vec && many) kv_read<DT, LPR, true, kTokens><<<grid, kBlock, 0, ctx->stream>>>(a);
+            else if (vec) kv_read<DT, LPR, true, 1><<<grid, kBlock, 0, ctx->stream>>>(a);
+            else if (many) kv_read<DT, LPR, false, kTokens><<<grid, kBlock, 0, ctx->stream>>>(a);
+            else kv_read<DT, LPR, false, 1><<<grid, kBlock, 0, ctx->stream>>>(a);
             return launched(ctx, "kv_read");
         });
     });

@@ -24,17 +24,37 @@ struct KvView {
     FastDiv page_div;
 };
 
-// Which sequence has row t, searched by a whole wave (every lane gets the
-// answer): the last one that starts at or before t.  -1: none has it.
-__device__ __forceinline__ int kv_sequence_of(const KvBatch& b, int t) {
-    int below = 0;  // starts at or before t
+// Which sequences have rows t .. t + T - 1, searched by a whole wave (every lane gets
+// the answers): the last one that starts at or before each.  -1: none has it.
+template <int T>
+__device__ __forceinline__ void kv_sequences_of(const KvBatch& b, int t, int* found) {
+#pragma unroll
+    for (int i = 0; i < T; ++i) found[i] = 0;  // starts at or before t + i
     for (int s = threadIdx.x & (kWave - 1); __any(s <= b.sequences); s += kWave) {
-        const bool in = s <= b.sequences && b.token_start[min(s, b.sequences)] <= t;
-        const int n = __popcll(__ballot(in));
-        below += n;
-        if (n < kWave) break;
+        const bool in = s <= b.sequences;
+        const int start = b.token_start[min(s, b.sequences)];
+#pragma unroll
+        for (int i = 0; i < T; ++i) found[i] += __popcll(__ballot(in && start <= t + i));
+        if (!__all(in && start <= t + T - 1)) break;
     }
-    return below >= 1 && below <= b.sequences ? below - 1 : -1;
+#pragma unroll
+    for (int i = 0; i < T; ++i) found[i] = found[i] >= 1 && found[i] <= b.sequences ? found[i] - 1 : -1;
+}
+
+// Where token t of sequence s (kv_sequences_of) stands: its position (below 0 for
+// tokens that the cache has no room for), page and slot.  Not `in`: no token.
+struct KvToken {
+    bool in;
+    int32_t position, page, slot;
+};
+
+__device__ __forceinline__ KvToken kv_token(const KvBatch& b, const KvView& c, int s, int t) {
+    if (s < 0) return KvToken{false, -1, -1, 0};
+    const KvSequence q = kv_sequence(b, s);
+    const int i = t - q.first, position = q.len - q.n + i;
+    if (i < 0 || i >= q.n) return KvToken{false, -1, -1, 0};
+    const KvSlot at = kv_slot(b, c.pages, c.page_div, s, position);
+    return KvToken{true, position, at.page, at.slot};
 }
 
 inline int kv_element_bytes(int dtype) { return dtype == MIMIR_KV_F32 ? 4 : dtype == MIMIR_KV_BF16 ? 2 : 1; }
@@ -53,6 +73,49 @@ __device__ __forceinline__ void rotate_pair(float& x0, float& x1, float c, float
     const double a = x0, b = x1, cd = c, sd = s;
     x0 = static_cast<float>(a * cd - b * sd);
     x1 = static_cast<float>(b * cd + a * sd);
+}
+
+// A unit: two vectors of W elements of a head row, for one lane.  Unit u of the
+// rotated part holds vectors u and u + (half of the part), which for pairs half the
+// part apart are the pairs' two elements, and otherwise W / 2 pairs each (W = 1: the
+// pair itself); the rest of the row is halved the same way.  So lanes side by side
+// read and write one run of memory with each vector.
+struct UnitPlace {
+    int d0, d1;  // first elements
+    bool turned;
+};
+
+template <int W>
+__device__ __forceinline__ UnitPlace unit_place(int u, int half, bool interleaved, int width) {
+    if (u * W < half) return W == 1 && interleaved ? UnitPlace{2 * u, 2 * u + 1, true} : UnitPlace{u * W, half + u * W, true};
+    const int rest = (width - 2 * half) / W, d = 2 * half + (u - half / W) * W;
+    return UnitPlace{d, d + (rest + 1) / 2 * W, false};
+}
+
+// cos and sin of a turned unit's W pairs; `row`: the position's first pair.
+template <int W>
+__device__ __forceinline__ void unit_turns(const float* cos_tab, const float* sin_tab, int64_t row, int u, int half,
+                                           bool interleaved, float* c, float* s) {
+#pragma unroll
+    for (int e = 0; e < W; ++e) {
+        const int pair = W == 1 || !interleaved ? u * W + e : (e < W / 2 ? 0 : half / 2) + u * W / 2 + e % ((W + 1) / 2);
+        c[e] = cos_tab[row + pair];
+        s[e] = sin_tab[row + pair];
+    }
+}
+
+template <int W>
+__device__ __forceinline__ void unit_rotate(float* lo, float* hi, const float* c, const float* s, bool interleaved) {
+    if (W > 1 && interleaved) {
+#pragma unroll
+        for (int e = 0; e < W / 2; ++e) {
+            rotate_pair(lo[2 * e], lo[2 * e + 1], c[e], s[e]);
+            rotate_pair(hi[2 * e], hi[2 * e + 1], c[W / 2 + e], s[W / 2 + e]);
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < W; ++e) rotate_pair(lo[e], hi[e], c[e], s[e]);
+    }
 }
 
 // MIMIR_OK, or why these tables do not fit heads of head_dim.

@@ -7,9 +7,9 @@
 //
 // Bound by HBM: every element is read once and written once; the positions and
 // their table rows are shared by the heads of a token and stay in L2.  A "slot" is
-// two vectors of one head row: four pairs (their first and second elements, or two
-// vectors side by side), or eight dimensions that are copied.  Each thread handles
-// kSlots of them a workgroup apart, all loads ahead of the first store.  The
+// two vectors of one head row (kvcache.hpp unit_place): four pairs, or eight
+// dimensions that are copied.  Each thread handles kSlots of them a workgroup
+// apart, all loads ahead of the first store.  The
 // products are taken in double (kvcache.hpp rotate_pair): 8 operations on pairs
 // that cost 32 bytes of HBM, a tenth of the time those take.
 #include "common.hpp"
@@ -93,9 +93,7 @@ __global__ __launch_bounds__(kBlock) void rope_rows(RowsArgs a) {
         const FastDiv& heads = is_q ? a.q_div : a.k_div;
         const uint32_t t = fastdiv(row, heads);
         const int64_t col = static_cast<int64_t>(row - t * heads.d) * a.head_dim;
-        const bool pairs = unit * W < a.half;
-        const int d0 = pairs && !a.interleaved ? unit * W : 2 * unit * W;
-        const int d1 = pairs && !a.interleaved ? a.half + unit * W : 2 * unit * W + W;
+        const auto [d0, d1, pairs] = unit_place<W>(unit, a.half, a.interleaved, a.head_dim);
         const float* x = (is_q ? a.q + t * a.ld_q : a.k + t * a.ld_k) + col;
         float* y = (is_q ? a.q_out + t * a.ld_q_out : a.k_out + t * a.ld_k_out) + col;
         lo[j].load(x + d0, true);
@@ -105,13 +103,9 @@ __global__ __launch_bounds__(kBlock) void rope_rows(RowsArgs a) {
         const int64_t p = a.positions[t];
         turn[j] = p < 0 || p >= a.table_rows ? 3 : pairs ? 2 : 1;
         if (turn[j] == 2) {
-            const float* ct = a.cos_tab + p * a.half + unit * W;
-            const float* st = a.sin_tab + p * a.half + unit * W;
+            unit_turns<W>(a.cos_tab, a.sin_tab, p * a.half, unit, a.half, a.interleaved, c[j], s[j]);
 #pragma unroll
-            for (int e = 0; e < W; ++e) {
-                c[j][e] = ct[e];
-                s[j][e] = st[e] * a.sign;
-            }
+            for (int e = 0; e < W; ++e) s[j][e] *= a.sign;
         }
     }
 #pragma unroll
@@ -122,25 +116,7 @@ __global__ __launch_bounds__(kBlock) void rope_rows(RowsArgs a) {
 #pragma unroll
             for (int e = 0; e < W; ++e) lo[j].x[e] = hi[j].x[e] = 0.f;
         } else if (turn[j] == 2) {
-            if (a.interleaved) {
-                // The 2 W floats in a row: element 2i of pair i, then 2i + 1.
-                float x[2 * W];
-#pragma unroll
-                for (int e = 0; e < W; ++e) {
-                    x[e] = lo[j].x[e];
-                    x[W + e] = hi[j].x[e];
-                }
-#pragma unroll
-                for (int e = 0; e < W; ++e) rotate_pair(x[2 * e], x[2 * e + 1], c[j][e], s[j][e]);
-#pragma unroll
-                for (int e = 0; e < W; ++e) {
-                    lo[j].x[e] = x[e];
-                    hi[j].x[e] = x[W + e];
-                }
-            } else {
-#pragma unroll
-                for (int e = 0; e < W; ++e) rotate_pair(lo[j].x[e], hi[j].x[e], c[j][e], s[j][e]);
-            }
+            unit_rotate<W>(lo[j].x, hi[j].x, c[j], s[j], a.interleaved);
         }
         lo[j].template store<KEEP, ACC>(out_lo[j], true);
         hi[j].template store<KEEP, ACC>(out_hi[j], out_hi[j] != nullptr);

@@ -87,6 +87,9 @@ __device__ __forceinline__ void row_over_keys(const PagedArgs& a, int s, int kv_
 
 typedef float f4r __attribute__((ext_vector_type(4)));
 
+// Memory that a kernel only reads, at addresses that a wave shares.
+typedef const __attribute__((address_space(4))) int32_t* scalar_i32;
+
 constexpr int kRows = 16;     // query rows of a tile: (token, head of the group) pairs
 constexpr int kKeys = 32;     // keys of a step: two halves of 16, each inside one page
 constexpr int kStreamWaves = 4;
@@ -217,7 +220,8 @@ struct Values {
 
 struct StreamArgs {
     PagedArgs p;
-    float* part;       // [workgroup][row][max, sum, head_dim sums], null: one split
+    float* part;       // [block][split][row][max, sum, head_dim sums], null: one split
+    uint32_t blocks;   // sequences x key / value heads x row blocks
     int32_t row_blocks;
     int32_t rows;      // rows of a block that are kept in `part`
     int32_t splits, span;  // splits of a sequence's keys, keys of each (a multiple of 128)
@@ -251,21 +255,20 @@ __device__ __forceinline__ int row_end(const PagedArgs& a, const KvSequence& q, 
 }
 
 template <int DT, int DP>
-__global__ __launch_bounds__(kStreamWaves * kWave, DP == 256 ? 1 : 2) void paged_stream(StreamArgs a) {
+__global__ __launch_bounds__(kStreamWaves * kWave, DP == 256 ? 1 : DT == MIMIR_KV_F32 ? (DP == 128 ? 2 : 3) : DP == 128 ? 3 : 4) void paged_stream(StreamArgs a) {
     using K = Kind<DT, DP>;
     constexpr int ND = DP / 16, kSteps = DP / 32;
-    // Wide heads keep their queries' terms in LDS: with fp32 keys and values the
-    // registers of one wave per SIMD would not hold them.
-    constexpr bool kQueriesInLds = DP * K::kBytes > 256;
     typedef float Share[kRows][DP + 2];
     __shared__ __attribute__((aligned(16))) char lds[sizeof(Share) * kStreamWaves];
     Share* const share = reinterpret_cast<Share*>(lds);  // after the keys
     u4* const q_lds = reinterpret_cast<u4*>(lds);        // [step][term][lane], during them
-    static_assert(!kQueriesInLds || kSteps * 3 * kWave * sizeof(u4) <= sizeof lds, "the queries fit");
+    static_assert(kSteps * 3 * kWave * sizeof(u4) <= sizeof lds, "the queries fit");
     __shared__ uint32_t bad;
     const PagedArgs& p = a.p;
-    const uint32_t split = blockIdx.x % static_cast<uint32_t>(a.splits);
-    const StreamWork w = stream_work(a, blockIdx.x / static_cast<uint32_t>(a.splits));
+    // The XCDs take workgroups in turn: blocks first, so that each gets whole splits'
+    // worth of them, the splits that every sequence has ahead of those few have.
+    const uint32_t split = blockIdx.x / a.blocks, block = blockIdx.x % a.blocks;
+    const StreamWork w = stream_work(a, block);
     const int k0 = static_cast<int>(split) * a.span, k1 = min(w.end, k0 + a.span);
     if (w.rows <= 0 || (split > 0 && k0 >= w.end)) return;
     const bool whole = a.part == nullptr || w.end <= a.span;  // no other split has keys
@@ -288,48 +291,35 @@ __global__ __launch_bounds__(kStreamWaves * kWave, DP == 256 ? 1 : 2) void paged
         }
         return split8(x);
     };
-    Split8 q_reg[kQueriesInLds ? 1 : kSteps];
-    if constexpr (kQueriesInLds) {
-        const float* row = q_row(my_row);
-        for (int c = wave; c < kSteps; c += kStreamWaves) {
-            const Split8 x = query(row, c);
-            q_lds[(3 * c) * kWave + lane] = x.h;
-            q_lds[(3 * c + 1) * kWave + lane] = x.m;
-            q_lds[(3 * c + 2) * kWave + lane] = x.l;
-        }
-        __syncthreads();
-    } else {
-        const float* row = q_row(my_row);
-#pragma unroll
-        for (int c = 0; c < kSteps; ++c) q_reg[c] = query(row, c);
+    for (int c = wave; c < kSteps; c += kStreamWaves) {
+        const Split8 x = query(q_row(my_row), c);
+        q_lds[(3 * c) * kWave + lane] = x.h;
+        q_lds[(3 * c + 1) * kWave + lane] = x.m;
+        q_lds[(3 * c + 2) * kWave + lane] = x.l;
     }
-    const auto q_at = [&](int c) {
-        if constexpr (kQueriesInLds)
-            return Split8{q_lds[(3 * c) * kWave + lane], q_lds[(3 * c + 1) * kWave + lane], q_lds[(3 * c + 2) * kWave + lane]};
-        else return q_reg[c];
-    };
+    __syncthreads();
 
     // Where the two halves of a step stand; a half without a page (or past the
-    // keys) borrows the other's address, and its keys count as unseen.
+    // keys) takes the first page's address, and its keys count as unseen.
     struct Step {
         int64_t at[2];  // rows of the cache
         bool has[2];
     };
+    // The table through scalar loads: a vector load's wait would be one for the keys
+    // and values in flight before it too.
+    const scalar_i32 table = (scalar_i32)(p.b.page_table + w.s * p.b.ld_pages);
     const auto find = [&](int key) {
         Step st;
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
             const int j = key + 16 * u;
-            st.has[u] = false;
-            st.at[u] = 0;
-            if (j < k1) {
-                const auto [page, slot] = kv_slot(p.b, p.c.pages, p.c.page_div, w.s, j);
-                st.has[u] = page >= 0;
-                st.at[u] = (static_cast<int64_t>(page) * p.c.kv_heads + w.head) * p.c.page_size + slot;
-            }
+            const int i = min(j, (k1 - 1) & -16);
+            const uint32_t entry = fastdiv(static_cast<uint32_t>(i), p.c.page_div);
+            const int page = table[entry];
+            st.has[u] = j < k1 && page >= 0 && page < p.c.pages;
+            st.at[u] = (static_cast<int64_t>(st.has[u] ? page : 0) * p.c.kv_heads + w.head) * p.c.page_size + i -
+                       static_cast<int>(entry) * p.c.page_size;
         }
-        if (!st.has[0]) st.at[0] = st.at[1];
-        if (!st.has[1]) st.at[1] = st.at[0];
         return st;
     };
     const int64_t row_bytes = static_cast<int64_t>(p.c.stride) * K::kBytes;
@@ -368,29 +358,24 @@ __global__ __launch_bounds__(kStreamWaves * kWave, DP == 256 ? 1 : 2) void paged
 
     constexpr int kStep = kKeys * kStreamWaves;
     int key = k0 + wave * kKeys;
-    // Steps without any page are passed over.
-    const auto next = [&](int from, Step* st) {
-        for (; from < k1; from += kStep) {
-            *st = find(from);
-            if (st->has[0] || st->has[1]) break;
-        }
-        return from;
-    };
-    Step st;
-    key = next(key, &st);
+    Step st{}, nx{};  // this step's, and the next one's, found a step ahead of its loads
     if (key < k1) {
+        st = find(key);
         load_k(st);
         load_v(st);
+        nx = find(key + kStep);
     }
-    while (key < k1) {
-        const int at = key;
-        const Step now = st;
-        key = next(key + kStep, &st);
-
+    // One step.  more: the next one's loads are issued in between, K's once the scores
+    // have read this one's, V's at the end; compiled apart from the last step, so that
+    // the waits for loads in flight count them.
+    const auto step = [&](auto more) {
+        int at = lane;
+        asm volatile("" : "+v"(at));  // read here in each step, not held in registers across them
+        const u4* const mine = q_lds + at;
         f4r s[2] = {f4r{0.f, 0.f, 0.f, 0.f}, f4r{0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
         for (int c = 0; c < kSteps; ++c) {
-            const Split8 q = q_at(c);
+            const Split8 q{mine[(3 * c) * kWave], mine[(3 * c + 1) * kWave], mine[(3 * c + 2) * kWave]};
 #pragma unroll
             for (int u = 0; u < 2; ++u) s[u] = mfma16_split(K::operand(kr[u], c), q, s[u]);
         }
@@ -399,7 +384,7 @@ __global__ __launch_bounds__(kStreamWaves * kWave, DP == 256 ? 1 : 2) void paged
             scale[0] = ks[0];
             scale[1] = ks[1];
         }
-        if (key < k1) load_k(st);
+        if constexpr (decltype(more)::value) load_k(nx);
 
         float x[8];
 #pragma unroll
@@ -409,15 +394,15 @@ __global__ __launch_bounds__(kStreamWaves * kWave, DP == 256 ? 1 : 2) void paged
         // Rows whose keys end inside the step, and halves that are not there: the
         // weights are 0 and, where no row of the tile sees a key, so are its values
         // (what is stored there may be anything).
-        const bool edge = !now.has[0] || !now.has[1] || __any(at + kKeys > my_end);
+        const bool edge = !st.has[0] || !st.has[1] || __any(key + kKeys > my_end);
         if (edge) {
 #pragma unroll
             for (int u = 0; u < 2; ++u)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const int j = at + 16 * u + 4 * hg + r;
-                    x[4 * u + r] = now.has[u] && j < my_end ? x[4 * u + r] : -INFINITY;
-                    if (!now.has[u] || j >= k1) {
+                    const int j = key + 16 * u + 4 * hg + r;
+                    x[4 * u + r] = st.has[u] && j < my_end ? x[4 * u + r] : -INFINITY;
+                    if (!st.has[u] || j >= k1) {
                         vr.clear(4 * u + r);
                         if constexpr (DT == MIMIR_KV_I8) vs[u][r] = 0.f;
                     }
@@ -443,11 +428,18 @@ __global__ __launch_bounds__(kStreamWaves * kWave, DP == 256 ? 1 : 2) void paged
         const Split8 pw = split8(x);
 #pragma unroll
         for (int t = 0; t < ND; ++t) o[t] = mfma16_split(vr.operand(t), pw, o[t]);
-        if (key < k1) load_v(st);
+        if constexpr (decltype(more)::value) load_v(nx);
+    };
+    for (; key + kStep < k1; key += kStep) {
+        const Step after = find(key + 2 * kStep);
+        step(std::true_type{});
+        st = nx;
+        nx = after;
     }
+    if (key < k1) step(std::false_type{});
 
     // The waves' shares of the rows.  Lane (li, hg) holds dimensions (4 hg + r) ND + t.
-    if constexpr (kQueriesInLds) __syncthreads();
+    __syncthreads();
     l_run += __shfl_xor(l_run, 16);
     l_run += __shfl_xor(l_run, 32);
 #pragma unroll
@@ -464,7 +456,7 @@ __global__ __launch_bounds__(kStreamWaves * kWave, DP == 256 ? 1 : 2) void paged
         return p.out + (w.seq.first + r / p.group) * p.ld_out + static_cast<int64_t>(w.head * p.group + r % p.group) * p.c.head_dim;
     };
     const auto part_row = [&](int row) {
-        return a.part + (static_cast<int64_t>(blockIdx.x) * a.rows + row) * (p.c.head_dim + 2);
+        return a.part + ((static_cast<int64_t>(block) * a.splits + split) * a.rows + row) * (p.c.head_dim + 2);
     };
     for (int x = threadIdx.x; x < w.rows * p.c.head_dim; x += kStreamWaves * kWave) {
         const int row = x / p.c.head_dim, d = x % p.c.head_dim;
@@ -512,13 +504,12 @@ __global__ __launch_bounds__(kStreamWaves * kWave, DP == 256 ? 1 : 2) void paged
     }
 }
 
-// The splits of one row, a wave per row: brought to one max and divided.
+// The splits of one row: brought to one max, added up by four waves and divided.
 __global__ __launch_bounds__(kBlock) void paged_join(StreamArgs a) {
-    const int64_t at = static_cast<int64_t>(blockIdx.x) * (kBlock / kWave) + threadIdx.x / kWave;
-    const int64_t blocks = static_cast<int64_t>(a.p.b.sequences) * a.p.c.kv_heads * a.row_blocks;
-    if (at / a.rows >= blocks) return;
-    const auto block = static_cast<uint32_t>(at / a.rows);
-    const int row = static_cast<int>(at % a.rows), lane = threadIdx.x % kWave;
+    __shared__ float share[kBlock / kWave][kKvMaxDim];
+    const auto block = blockIdx.x / static_cast<uint32_t>(a.rows);
+    const int row = static_cast<int>(blockIdx.x % static_cast<uint32_t>(a.rows));
+    const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
     const StreamWork w = stream_work(a, block);
     if (row >= w.rows || w.end <= a.span) return;
     const int d = a.p.c.head_dim, n = (w.end + a.span - 1) / a.span;
@@ -531,20 +522,23 @@ __global__ __launch_bounds__(kBlock) void paged_join(StreamArgs a) {
     l = wave_sum(l);
 #pragma unroll
     for (int c = 0; c < kRowChunks; ++c) acc[c] = 0.f;
-    for (int s = 0; s < n; ++s) {
+#pragma unroll 4
+    for (int s = wave; s < n; s += kBlock / kWave) {
         const float f = __builtin_amdgcn_exp2f(part[s * step] - m);
 #pragma unroll
         for (int c = 0; c < kRowChunks; ++c)
             if (lane + c * kWave < d) acc[c] += part[s * step + 2 + lane + c * kWave] * f;
     }
-    const float inv = 1.0f / (l + 1e-9f);
-    const int r = w.row0 + row;
-    float* out = a.p.out + (w.seq.first + r / a.p.group) * a.p.ld_out +
-                 static_cast<int64_t>(w.head * a.p.group + r % a.p.group) * d;
 #pragma unroll
-    for (int c = 0; c < kRowChunks; ++c)
-        if (lane + c * kWave < d) out[lane + c * kWave] = acc[c] * inv;
+    for (int c = 0; c < kRowChunks; ++c) share[wave][lane + c * kWave] = acc[c];
+    __syncthreads();
+    const int x = static_cast<int>(threadIdx.x);
+    if (x >= d) return;
+    const int r = w.row0 + row;
+    a.p.out[(w.seq.first + r / a.p.group) * a.p.ld_out + static_cast<int64_t>(w.head * a.p.group + r % a.p.group) * d + x] =
+        ((share[0][x] + share[1][x]) + (share[2][x] + share[3][x])) * (1.0f / (l + 1e-9f));
 }
+static_assert(kKvMaxDim <= kBlock && kBlock / kWave == 4, "a thread per dimension, four waves");
 
 template <int DT>
 void launch_stream_dim(const StreamArgs& a, unsigned grid, hipStream_t s) {
@@ -573,15 +567,16 @@ int launch_stream(mimir_ctx* ctx, const PagedArgs& p, int dtype, int64_t most_ro
     a.span = static_cast<int32_t>((grains + splits - 1) / splits * kGrain);
     a.splits = static_cast<int32_t>((grains * kGrain + a.span - 1) / a.span);
     if (a.splits == 1) a.part = nullptr;
-    MIMIR_REQUIRE(ctx, dispatch_fits(blocks * a.splits, kStreamWaves * kWave) && dispatch_fits((blocks * a.rows + 3) / 4, kBlock),
+    MIMIR_REQUIRE(ctx, dispatch_fits(blocks * a.splits, kStreamWaves * kWave) && dispatch_fits(blocks * a.rows, kBlock),
                   "paged attention: grid of %lld workgroups exceeds the limit", (long long)(blocks * a.splits));
+    a.blocks = static_cast<uint32_t>(blocks);
     const auto grid = static_cast<unsigned>(blocks * a.splits);
     if (dtype == MIMIR_KV_F32) launch_stream_dim<MIMIR_KV_F32>(a, grid, ctx->stream);
     else if (dtype == MIMIR_KV_BF16) launch_stream_dim<MIMIR_KV_BF16>(a, grid, ctx->stream);
     else launch_stream_dim<MIMIR_KV_I8>(a, grid, ctx->stream);
     if (int st = launched(ctx, "paged_stream")) return st;
     if (!a.part) return MIMIR_OK;
-    paged_join<<<static_cast<unsigned>((blocks * a.rows + 3) / 4), kBlock, 0, ctx->stream>>>(a);
+    paged_join<<<static_cast<unsigned>(blocks * a.rows), kBlock, 0, ctx->stream>>>(a);
     return launched(ctx, "paged_join");
 }
 
@@ -602,6 +597,7 @@ extern "C" int mimir_attention_paged_fwd(mimir_ctx* ctx, const mimir_kv_cache* c
                   (long long)ld_q, (long long)ld_out, (long long)width);
     MIMIR_REQUIRE(ctx, std::isfinite(scale), "%s: scale must be finite", what);
     if (batch->tokens == 0 || batch->sequences == 0 || batch->max_new == 0) return MIMIR_OK;
+    if (cache->pages == 0) a.b.max_len = 0;  // no keys, and no memory to point at
     MIMIR_REQUIRE(ctx, q && out, "%s: null pointer", what);
     MIMIR_ENTER(ctx);
     a.q = q;

@@ -91,7 +91,8 @@ typedef float f4r __attribute__((ext_vector_type(4)));
 typedef const __attribute__((address_space(4))) int32_t* scalar_i32;
 
 constexpr int kRows = 16;     // query rows of a tile: (token, head of the group) pairs
-constexpr int kKeys = 32;     // keys of a step: two halves of 16, each inside one page
+constexpr int kHalf = 16;     // keys that stand in one page
+constexpr int kNt = 2;        // a buffer load's non-temporal bit
 constexpr int kStreamWaves = 4;
 constexpr float kMaxSlack = 8.0f;  // as attention.hip: the running max may lag by this many base-2 units
 
@@ -140,6 +141,7 @@ struct Kind;
 
 template <int DP>
 struct Kind<MIMIR_KV_F32, DP> {
+    static constexpr int kHalves = 2;  // of a step
     static constexpr int kBytes = 4, kVecs = DP / 16;  // K vectors of a lane per half
     typedef Split8 Operand;
     static __device__ __forceinline__ int first(int v, int hg) { return 16 * v + 4 * hg; }
@@ -152,6 +154,7 @@ struct Kind<MIMIR_KV_F32, DP> {
 };
 template <int DP>
 struct Kind<MIMIR_KV_BF16, DP> {
+    static constexpr int kHalves = 2;  // of a step
     static constexpr int kBytes = 2, kVecs = DP / 32;
     typedef u4 Operand;
     static __device__ __forceinline__ int first(int v, int hg) { return 32 * v + 8 * hg; }
@@ -160,6 +163,7 @@ struct Kind<MIMIR_KV_BF16, DP> {
 };
 template <int DP>
 struct Kind<MIMIR_KV_I8, DP> {
+    static constexpr int kHalves = 2;  // of a step
     static constexpr int kBytes = 1, kVecs = DP / 64;
     typedef u4 Operand;
     static __device__ __forceinline__ int first(int v, int hg) { return 64 * v + 16 * hg; }
@@ -177,21 +181,21 @@ struct Values {
     static constexpr int kBytes = DT == MIMIR_KV_F32 ? 4 : DT == MIMIR_KV_BF16 ? 2 : 1;
     static constexpr int kWords = ND * kBytes / 4;
     uint32_t w[8][kWords];
-    __device__ __forceinline__ void load(int key, const char* p) {
+    __device__ __forceinline__ void load(int key, __amdgpu_buffer_rsrc_t rows, uint32_t off, uint32_t row) {
         if constexpr (kWords % 4 == 0) {
 #pragma unroll
             for (int i = 0; i < kWords / 4; ++i) {
-                const u4 x = reinterpret_cast<const u4*>(p)[i];
+                const u4 x = __builtin_amdgcn_raw_buffer_load_b128(rows, off + 16 * i, row, kNt);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) w[key][4 * i + e] = x[e];
             }
         } else if constexpr (kWords == 2) {
-            const u2 x = *reinterpret_cast<const u2*>(p);
+            const u2 x = __builtin_amdgcn_raw_buffer_load_b64(rows, off, row, kNt);
             w[key][0] = x[0];
             w[key][1] = x[1];
         } else {
             static_assert(kWords == 1, "one word, two or whole vectors");
-            w[key][0] = *reinterpret_cast<const uint32_t*>(p);
+            w[key][0] = __builtin_amdgcn_raw_buffer_load_b32(rows, off, row, kNt);
         }
     }
     __device__ __forceinline__ void clear(int key) {
@@ -220,32 +224,96 @@ struct Values {
 
 struct StreamArgs {
     PagedArgs p;
-    float* part;       // [block][split][row][max, sum, head_dim sums], null: one split
-    uint32_t blocks;   // sequences x key / value heads x row blocks
-    int32_t row_blocks;
-    int32_t rows;      // rows of a block that are kept in `part`
-    int32_t splits, span;  // splits of a sequence's keys, keys of each (a multiple of 128)
-    int32_t most_rows; // sequences with more query rows than this are another kernel's
+    // Blocks that several workgroups have keys of: which (first workgroup, number of
+    // them; by sequence, head and rows), and their sums, [workgroup][2][row][max, sum,
+    // head_dim sums].  Null: blocks are not divided.
+    int2* shared;
+    float* part;
+    uint32_t grain;     // keys that are not divided among workgroups
+    uint32_t extra;     // what a block costs besides its keys, in grains
+    uint32_t groups;    // workgroups
+    int32_t row_blocks; // of the sequence with the most rows
+    int32_t rows;       // rows of a block that are kept in `part`
+    int32_t most_rows;  // sequences with more query rows than this are another kernel's
 };
 
-// What a workgroup of the stream kernel (and its part of the join) has to do.
-struct StreamWork {
+// The work: a block is 16 query rows of one key / value head of a sequence against
+// its keys, and costs its keys' grains and `extra`; all blocks' costs in order
+// (sequence, head, rows) are dealt to the workgroups in equal runs, so that sequences
+// of any lengths fill the GPU evenly.  A run may begin and end inside a block.  Every
+// wave works out its run from the sequences' lengths, 64 of them at a time.
+struct StreamChunk {
+    int base;         // its first sequence
+    uint32_t before;  // costs of those ahead
+    KvSequence seq;   // the lane's sequence: its part of the batch, a block's cost, its
+    uint32_t cost, blocks, sum;  // blocks, the costs up to it
+};
+
+__device__ __forceinline__ uint32_t lane_of(uint32_t v, int lane) {
+    return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), lane));
+}
+
+// Cost of a block of a sequence, and its blocks (0: another kernel's, or none).
+__device__ __forceinline__ uint32_t stream_cost(const StreamArgs& a, const KvSequence& q, uint32_t* blocks) {
+    const int64_t rows = static_cast<int64_t>(q.n) * a.p.group;
+    *blocks = rows > 0 && rows <= a.most_rows
+                  ? static_cast<uint32_t>((rows + kRows - 1) / kRows) * static_cast<uint32_t>(a.p.c.kv_heads)
+                  : 0;
+    return a.extra + max(1u, (static_cast<uint32_t>(q.len) + a.grain - 1) / a.grain);
+}
+
+__device__ __forceinline__ StreamChunk stream_chunk(const StreamArgs& a, int base, uint32_t before) {
+    const int lane = static_cast<int>(threadIdx.x % kWave);
+    StreamChunk c{base, before, KvSequence{0, 0, 0}, 0, 0, 0};
+    if (base + lane < a.p.b.sequences) {
+        c.seq = kv_sequence(a.p.b, base + lane);
+        c.cost = stream_cost(a, c.seq, &c.blocks);
+    }
+    c.sum = c.cost * c.blocks;
+#pragma unroll
+    for (int x = 1; x < kWave; x *= 2) {
+        const uint32_t y = static_cast<uint32_t>(__shfl_up(static_cast<int>(c.sum), x));
+        if (lane >= x) c.sum += y;
+    }
+    return c;
+}
+
+struct StreamBlock {
     int s, head, row0, rows;  // sequence, key / value head, first row and rows of the block
     int end;                  // keys that some row of it sees
+    uint32_t index;           // of its sequence's blocks
+    uint32_t first, cost;     // its run of all costs
     KvSequence seq;
 };
 
-__device__ __forceinline__ StreamWork stream_work(const StreamArgs& a, uint32_t block) {
-    StreamWork w;
-    const uint32_t rb = block % static_cast<uint32_t>(a.row_blocks), sh = block / static_cast<uint32_t>(a.row_blocks);
-    w.s = static_cast<int>(sh / static_cast<uint32_t>(a.p.c.kv_heads));
-    w.head = static_cast<int>(sh % static_cast<uint32_t>(a.p.c.kv_heads));
-    w.seq = kv_sequence(a.p.b, w.s);
-    const int64_t all = static_cast<int64_t>(w.seq.n) * a.p.group;
-    w.row0 = static_cast<int>(rb) * kRows;
-    w.rows = all > a.most_rows ? 0 : static_cast<int>(min(all - w.row0, static_cast<int64_t>(kRows)));
-    const int last = (w.row0 + max(w.rows, 1) - 1) / a.p.group;
-    w.end = a.p.causal ? min(max(w.seq.len - w.seq.n + last + 1, 0), w.seq.len) : w.seq.len;
+__device__ __forceinline__ void stream_rows(const StreamArgs& a, uint32_t blocks, StreamBlock* w) {
+    const uint32_t row_blocks = max(1u, blocks / static_cast<uint32_t>(a.p.c.kv_heads));
+    w->head = static_cast<int>(w->index / row_blocks);
+    w->row0 = static_cast<int>(w->index % row_blocks) * kRows;
+    w->rows = w->index < blocks ? min(w->seq.n * a.p.group - w->row0, kRows) : 0;
+    const int last = (w->row0 + max(w->rows, 1) - 1) / a.p.group;
+    w->end = a.p.causal ? min(max(w->seq.len - w->seq.n + last + 1, 0), w->seq.len) : w->seq.len;
+}
+
+// The block that x (below the total) falls in; `c` moves on to its chunk.
+__device__ __forceinline__ StreamBlock stream_locate(const StreamArgs& a, uint32_t x, StreamChunk* c) {
+    for (;;) {
+        const uint32_t to = c->before + lane_of(c->sum, kWave - 1);
+        if (x < to || c->base + kWave >= a.p.b.sequences) break;
+        *c = stream_chunk(a, c->base + kWave, to);
+    }
+    const uint64_t above = __ballot(c->before + c->sum > x);
+    const int lane = above ? __builtin_ctzll(above) : kWave - 1;
+    StreamBlock w;
+    w.s = c->base + lane;
+    w.seq = KvSequence{static_cast<int>(lane_of(c->seq.first, lane)), static_cast<int>(lane_of(c->seq.n, lane)),
+                       static_cast<int>(lane_of(c->seq.len, lane))};
+    w.cost = lane_of(c->cost, lane);
+    const uint32_t blocks = lane_of(c->blocks, lane);
+    const uint32_t start = c->before + lane_of(c->sum, lane) - w.cost * blocks;
+    w.index = (x - start) / w.cost;
+    w.first = start + w.index * w.cost;
+    stream_rows(a, blocks, &w);
     return w;
 }
 
@@ -254,10 +322,16 @@ __device__ __forceinline__ int row_end(const PagedArgs& a, const KvSequence& q, 
     return a.causal ? min(max(q.len - q.n + row / a.group + 1, 0), q.len) : q.len;
 }
 
+// Where a workgroup keeps the sums of a block that it shares with others: the block
+// that its run begins in (0) or the one that it ends in (1).
+__device__ __forceinline__ float* stream_part(const StreamArgs& a, uint32_t group, bool ends, int row) {
+    return a.part + ((static_cast<int64_t>(group) * 2 + (ends ? 1 : 0)) * a.rows + row) * (a.p.c.head_dim + 2);
+}
+
 template <int DT, int DP>
 __global__ __launch_bounds__(kStreamWaves * kWave, DP == 256 ? 1 : DT == MIMIR_KV_F32 ? (DP == 128 ? 2 : 3) : DP == 128 ? 3 : 4) void paged_stream(StreamArgs a) {
     using K = Kind<DT, DP>;
-    constexpr int ND = DP / 16, kSteps = DP / 32;
+    constexpr int ND = DP / 16, kSteps = DP / 32, H = K::kHalves;
     typedef float Share[kRows][DP + 2];
     __shared__ __attribute__((aligned(16))) char lds[sizeof(Share) * kStreamWaves];
     Share* const share = reinterpret_cast<Share*>(lds);  // after the keys
@@ -265,45 +339,55 @@ __global__ __launch_bounds__(kStreamWaves * kWave, DP == 256 ? 1 : DT == MIMIR_K
     static_assert(kSteps * 3 * kWave * sizeof(u4) <= sizeof lds, "the queries fit");
     __shared__ uint32_t bad;
     const PagedArgs& p = a.p;
-    // The XCDs take workgroups in turn: blocks first, so that each gets whole splits'
-    // worth of them, the splits that every sequence has ahead of those few have.
-    const uint32_t split = blockIdx.x / a.blocks, block = blockIdx.x % a.blocks;
-    const StreamWork w = stream_work(a, block);
-    const int k0 = static_cast<int>(split) * a.span, k1 = min(w.end, k0 + a.span);
-    if (w.rows <= 0 || (split > 0 && k0 >= w.end)) return;
-    const bool whole = a.part == nullptr || w.end <= a.span;  // no other split has keys
-
-    const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave), lane = threadIdx.x % kWave;
-    const int li = lane % 16, hg = lane / 16;
-    if (threadIdx.x == 0) bad = 0;
+    StreamChunk chunk = stream_chunk(a, 0, 0);
+    uint32_t total = lane_of(chunk.sum, kWave - 1);
+    for (int base = kWave; base < p.b.sequences; base += kWave)
+        total += lane_of(stream_chunk(a, base, 0).sum, kWave - 1);
+    const uint32_t run = (total + a.groups - 1) / a.groups;
+    const auto end = static_cast<uint32_t>(min(static_cast<uint64_t>(total), (static_cast<uint64_t>(blockIdx.x) + 1) * run));
+    const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave);
+    for (uint64_t from = static_cast<uint64_t>(blockIdx.x) * run; from < end;) {
+    int tid = static_cast<int>(threadIdx.x);
+    asm volatile("" : "+v"(tid));  // what follows from it is computed for each block, not held in registers across them
+    const int lane = tid % kWave, li = lane % 16, hg = lane / 16;
+    const StreamBlock w = stream_locate(a, static_cast<uint32_t>(from), &chunk);
+    const uint32_t x0 = static_cast<uint32_t>(from) - w.first, x1 = min(w.cost, end - w.first);
+    from = w.first + x1;
+    const bool whole = x0 == 0 && x1 == w.cost;  // no other workgroup has keys of the block
+    const auto keys_to = [&](uint32_t x) {
+        return static_cast<int>(min(static_cast<uint64_t>(x > a.extra ? x - a.extra : 0) * a.grain, static_cast<uint64_t>(w.end)));
+    };
+    const int k0 = keys_to(x0), k1 = keys_to(x1);
+    if (a.part && x0 == 0 && tid == 0)
+        a.shared[static_cast<int64_t>(w.s) * a.row_blocks * p.c.kv_heads + w.index] =
+            int2{static_cast<int>(blockIdx.x), static_cast<int>((w.first + w.cost - 1) / run - blockIdx.x) + 1};
     const int my_row = w.row0 + min(li, w.rows - 1);
     const int my_end = min(row_end(p, w.seq, my_row), k1);
     const auto q_row = [&](int row) {
         return p.q + (w.seq.first + row / p.group) * p.ld_q + static_cast<int64_t>(w.head * p.group + row % p.group) * p.c.head_dim;
     };
-
-    const auto query = [&](const float* row, int c) {
-        float x[8];
+    // The queries' loads go out ahead of the first keys', their terms follow those.
+    constexpr int kOwn = (kSteps + kStreamWaves - 1) / kStreamWaves;
+    float qx[kOwn][8];
+#pragma unroll
+    for (int i = 0; i < kOwn; ++i) {
+        const float* row = q_row(my_row);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            const int d = K::dim(c, hg, e);
-            x[e] = d < p.c.head_dim ? row[d] * p.qscale : 0.f;
+            const int d = K::dim(wave + i * kStreamWaves, hg, e);
+            qx[i][e] = d < p.c.head_dim ? row[d] : 0.f;
         }
-        return split8(x);
-    };
-    for (int c = wave; c < kSteps; c += kStreamWaves) {
-        const Split8 x = query(q_row(my_row), c);
-        q_lds[(3 * c) * kWave + lane] = x.h;
-        q_lds[(3 * c + 1) * kWave + lane] = x.m;
-        q_lds[(3 * c + 2) * kWave + lane] = x.l;
     }
-    __syncthreads();
 
-    // Where the two halves of a step stand; a half without a page (or past the
-    // keys) takes the first page's address, and its keys count as unseen.
+    // Where the halves of a step stand; one without a page (or past the keys) takes
+    // the first page's address, and its keys count as unseen.
     struct Step {
-        int64_t at[2];  // rows of the cache
-        bool has[2];
+        int page[H], slot[H];
+        __device__ __forceinline__ bool has(int u, const KvView& c) const { return page[u] >= 0 && page[u] < c.pages; }
+        // Row of the cache.
+        __device__ __forceinline__ int64_t at(int u, const KvView& c, int head) const {
+            return (static_cast<int64_t>(has(u, c) ? page[u] : 0) * c.kv_heads + head) * c.page_size + slot[u];
+        }
     };
     // The table through scalar loads: a vector load's wait would be one for the keys
     // and values in flight before it too.
@@ -311,43 +395,46 @@ __global__ __launch_bounds__(kStreamWaves * kWave, DP == 256 ? 1 : DT == MIMIR_K
     const auto find = [&](int key) {
         Step st;
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            const int j = key + 16 * u;
-            const int i = min(j, (k1 - 1) & -16);
+        for (int u = 0; u < H; ++u) {
+            const int j = key + kHalf * u;
+            const int i = min(j, (k1 - 1) & -kHalf);
             const uint32_t entry = fastdiv(static_cast<uint32_t>(i), p.c.page_div);
-            const int page = table[entry];
-            st.has[u] = j < k1 && page >= 0 && page < p.c.pages;
-            st.at[u] = (static_cast<int64_t>(st.has[u] ? page : 0) * p.c.kv_heads + w.head) * p.c.page_size + i -
-                       static_cast<int>(entry) * p.c.page_size;
+            st.page[u] = j < k1 ? table[entry] : -1;
+            st.slot[u] = i - static_cast<int>(entry) * p.c.page_size;
         }
         return st;
     };
-    const int64_t row_bytes = static_cast<int64_t>(p.c.stride) * K::kBytes;
-    uint32_t k_off[K::kVecs], v_off;
+    const int row_bytes = p.c.stride * K::kBytes;
+    const auto half_rows = [&](const char* base, int64_t at) {
+        return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base) + at * row_bytes, 0, kHalf * row_bytes, kBufferWord3);
+    };
+    uint32_t k_off[K::kVecs];
 #pragma unroll
     for (int v = 0; v < K::kVecs; ++v)
         k_off[v] = static_cast<uint32_t>((li * p.c.stride + min(K::first(v, hg), p.c.stride - 16 / K::kBytes)) * K::kBytes);
-    v_off = static_cast<uint32_t>((4 * hg * p.c.stride + min(li * ND, p.c.stride - ND)) * K::kBytes);
+    const uint32_t v_off = static_cast<uint32_t>((4 * hg * p.c.stride + min(li * ND, p.c.stride - ND)) * K::kBytes);
 
-    u4 kr[2][K::kVecs];
-    Values<DT, ND> vr;
-    f4 ks[2], vs[2];
+    u4 kr[H][K::kVecs];
+    Values<DT, ND> vr[H / 2];
+    f4 ks[H], vs[H];
     const auto load_k = [&](const Step& st) {
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            const char* base = p.c.k + st.at[u] * row_bytes;
+        for (int u = 0; u < H; ++u) {
+            const int64_t at = st.at(u, p.c, w.head);
+            const __amdgpu_buffer_rsrc_t rows = half_rows(p.c.k, at);
 #pragma unroll
-            for (int v = 0; v < K::kVecs; ++v) kr[u][v] = *reinterpret_cast<const u4*>(base + k_off[v]);
-            if constexpr (DT == MIMIR_KV_I8) ks[u] = *reinterpret_cast<const f4*>(p.c.k_scale + st.at[u] + 4 * hg);
+            for (int v = 0; v < K::kVecs; ++v) kr[u][v] = __builtin_amdgcn_raw_buffer_load_b128(rows, k_off[v], 0, kNt);
+            if constexpr (DT == MIMIR_KV_I8) ks[u] = *reinterpret_cast<const f4*>(p.c.k_scale + at + 4 * hg);
         }
     };
     const auto load_v = [&](const Step& st) {
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            const char* base = p.c.v + st.at[u] * row_bytes;
+        for (int u = 0; u < H; ++u) {
+            const int64_t at = st.at(u, p.c, w.head);
+            const __amdgpu_buffer_rsrc_t rows = half_rows(p.c.v, at);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) vr.load(4 * u + e, base + v_off + e * row_bytes);
-            if constexpr (DT == MIMIR_KV_I8) vs[u] = *reinterpret_cast<const f4*>(p.c.v_scale + st.at[u] + 4 * hg);
+            for (int e = 0; e < 4; ++e) vr[u / 2].load(4 * (u % 2) + e, rows, v_off, e * row_bytes);
+            if constexpr (DT == MIMIR_KV_I8) vs[u] = *reinterpret_cast<const f4*>(p.c.v_scale + at + 4 * hg);
         }
     };
 
@@ -356,15 +443,29 @@ __global__ __launch_bounds__(kStreamWaves * kWave, DP == 256 ? 1 : DT == MIMIR_K
     for (int t = 0; t < ND; ++t) o[t] = f4r{0.f, 0.f, 0.f, 0.f};
     float m_run = -1e30f, l_run = 0.f;  // the max is the row's, the sum this lane's share
 
-    constexpr int kStep = kKeys * kStreamWaves;
+    constexpr int kKeys = kHalf * H, kStep = kKeys * kStreamWaves;
     int key = k0 + wave * kKeys;
-    Step st{}, nx{};  // this step's, and the next one's, found a step ahead of its loads
+    Step st{}, nx{}, after{};  // this step's, and the next two's, found a step ahead of their loads
     if (key < k1) {
         st = find(key);
         load_k(st);
         load_v(st);
         nx = find(key + kStep);
     }
+    __syncthreads();  // the last block's sums and flags are read
+    if (tid == 0) bad = 0;
+#pragma unroll
+    for (int i = 0; i < kOwn; ++i) {
+        const int c = wave + i * kStreamWaves;
+        if (c >= kSteps) break;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) qx[i][e] *= p.qscale;
+        const Split8 x = split8(qx[i]);
+        q_lds[(3 * c) * kWave + lane] = x.h;
+        q_lds[(3 * c + 1) * kWave + lane] = x.m;
+        q_lds[(3 * c + 2) * kWave + lane] = x.l;
+    }
+    __syncthreads();
     // One step.  more: the next one's loads are issued in between, K's once the scores
     // have read this one's, V's at the end; compiled apart from the last step, so that
     // the waits for loads in flight count them.
@@ -372,43 +473,50 @@ __global__ __launch_bounds__(kStreamWaves * kWave, DP == 256 ? 1 : DT == MIMIR_K
         int at = lane;
         asm volatile("" : "+v"(at));  // read here in each step, not held in registers across them
         const u4* const mine = q_lds + at;
-        f4r s[2] = {f4r{0.f, 0.f, 0.f, 0.f}, f4r{0.f, 0.f, 0.f, 0.f}};
+        f4r s[H];
+#pragma unroll
+        for (int u = 0; u < H; ++u) s[u] = f4r{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int c = 0; c < kSteps; ++c) {
             const Split8 q{mine[(3 * c) * kWave], mine[(3 * c + 1) * kWave], mine[(3 * c + 2) * kWave]};
 #pragma unroll
-            for (int u = 0; u < 2; ++u) s[u] = mfma16_split(K::operand(kr[u], c), q, s[u]);
+            for (int u = 0; u < H; ++u) s[u] = mfma16_split(K::operand(kr[u], c), q, s[u]);
+            if constexpr (DT == MIMIR_KV_F32) __builtin_amdgcn_sched_barrier(0);  // few terms at a time
         }
-        f4 scale[2];
         if constexpr (DT == MIMIR_KV_I8) {
-            scale[0] = ks[0];
-            scale[1] = ks[1];
+#pragma unroll
+            for (int u = 0; u < H; ++u)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) s[u][r] *= ks[u][r];
         }
-        if constexpr (decltype(more)::value) load_k(nx);
+        if constexpr (decltype(more)::value) {
+            load_k(nx);
+            after = find(key + 2 * kStep);  // here, where no LDS read waits for it
+        }
 
-        float x[8];
+        float x[4 * H];
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) x[4 * u + r] = DT == MIMIR_KV_I8 ? s[u][r] * scale[u][r] : s[u][r];
+        for (int e = 0; e < 4 * H; ++e) x[e] = s[e / 4][e % 4];
         // Rows whose keys end inside the step, and halves that are not there: the
         // weights are 0 and, where no row of the tile sees a key, so are its values
         // (what is stored there may be anything).
-        const bool edge = !st.has[0] || !st.has[1] || __any(key + kKeys > my_end);
+        bool edge = __any(key + kKeys > my_end);
+#pragma unroll
+        for (int u = 0; u < H; ++u) edge = edge || !st.has(u, p.c);
         if (edge) {
 #pragma unroll
-            for (int u = 0; u < 2; ++u)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int j = key + 16 * u + 4 * hg + r;
-                    x[4 * u + r] = st.has[u] && j < my_end ? x[4 * u + r] : -INFINITY;
-                    if (!st.has[u] || j >= k1) {
-                        vr.clear(4 * u + r);
-                        if constexpr (DT == MIMIR_KV_I8) vs[u][r] = 0.f;
-                    }
+            for (int e = 0; e < 4 * H; ++e) {
+                const int u = e / 4, j = key + kHalf * u + 4 * hg + e % 4;
+                x[e] = st.has(u, p.c) && j < my_end ? x[e] : -INFINITY;
+                if (!st.has(u, p.c) || j >= k1) {
+                    vr[u / 2].clear(e % 8);
+                    if constexpr (DT == MIMIR_KV_I8) vs[u][e % 4] = 0.f;
                 }
+            }
         }
-        float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+        float top = x[0];
+#pragma unroll
+        for (int e = 1; e < 4 * H; ++e) top = fmaxf(top, x[e]);
         if (__any(top > m_run + kMaxSlack)) {
             top = fmaxf(top, __shfl_xor(top, 16));
             top = fmaxf(top, __shfl_xor(top, 32));
@@ -420,18 +528,24 @@ __global__ __launch_bounds__(kStreamWaves * kWave, DP == 256 ? 1 : DT == MIMIR_K
             for (int t = 0; t < ND; ++t) o[t] *= f;
         }
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
+        for (int e = 0; e < 4 * H; ++e) {
             x[e] = __builtin_amdgcn_exp2f(x[e] - m_run);
             l_run += x[e];
             if constexpr (DT == MIMIR_KV_I8) x[e] *= vs[e / 4][e % 4];
         }
-        const Split8 pw = split8(x);
 #pragma unroll
-        for (int t = 0; t < ND; ++t) o[t] = mfma16_split(vr.operand(t), pw, o[t]);
+        for (int h = 0; h < H / 2; ++h) {
+            const Split8 pw = split8(x + 8 * h);
+#pragma unroll
+            for (int t = 0; t < ND; ++t) {
+                o[t] = mfma16_split(vr[h].operand(t), pw, o[t]);
+                if constexpr (DT == MIMIR_KV_F32)
+                    if (t % 2 == 1) __builtin_amdgcn_sched_barrier(0);
+            }
+        }
         if constexpr (decltype(more)::value) load_v(nx);
     };
     for (; key + kStep < k1; key += kStep) {
-        const Step after = find(key + 2 * kStep);
         step(std::true_type{});
         st = nx;
         nx = after;
@@ -455,10 +569,8 @@ __global__ __launch_bounds__(kStreamWaves * kWave, DP == 256 ? 1 : DT == MIMIR_K
         const int r = w.row0 + row;
         return p.out + (w.seq.first + r / p.group) * p.ld_out + static_cast<int64_t>(w.head * p.group + r % p.group) * p.c.head_dim;
     };
-    const auto part_row = [&](int row) {
-        return a.part + ((static_cast<int64_t>(block) * a.splits + split) * a.rows + row) * (p.c.head_dim + 2);
-    };
-    for (int x = threadIdx.x; x < w.rows * p.c.head_dim; x += kStreamWaves * kWave) {
+    const auto part_row = [&](int row) { return stream_part(a, blockIdx.x, x0 == 0, row); };
+    for (int x = tid; x < w.rows * p.c.head_dim; x += kStreamWaves * kWave) {
         const int row = x / p.c.head_dim, d = x % p.c.head_dim;
         float m = share[0][row][DP];
 #pragma unroll
@@ -485,7 +597,7 @@ __global__ __launch_bounds__(kStreamWaves * kWave, DP == 256 ? 1 : DT == MIMIR_K
     __syncthreads();
     // Rows that came out NaN or infinite, again in fp32: an operand had no bf16 split
     // (split.hpp), or a value that the row does not see is not finite.
-    if (bad == 0) return;
+    if (bad == 0) continue;
     for (int row = wave; row < w.rows; row += kStreamWaves) {
         if (!(bad >> row & 1)) continue;
         float acc[kRowChunks], m, l;
@@ -502,43 +614,88 @@ __global__ __launch_bounds__(kStreamWaves * kWave, DP == 256 ? 1 : DT == MIMIR_K
             out[-1] = l;
         }
     }
+    }
 }
 
-// The splits of one row: brought to one max, added up by four waves and divided.
+// The shares of one row of a block that several workgroups had keys of: brought to
+// one max, added up by four waves and divided.
 __global__ __launch_bounds__(kBlock) void paged_join(StreamArgs a) {
-    __shared__ float share[kBlock / kWave][kKvMaxDim];
-    const auto block = blockIdx.x / static_cast<uint32_t>(a.rows);
+    constexpr int kWaves = kBlock / kWave, kAhead = 4;
+    __shared__ float share[kWaves][kKvMaxDim + 2];
     const int row = static_cast<int>(blockIdx.x % static_cast<uint32_t>(a.rows));
-    const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-    const StreamWork w = stream_work(a, block);
-    if (row >= w.rows || w.end <= a.span) return;
-    const int d = a.p.c.head_dim, n = (w.end + a.span - 1) / a.span;
-    const float* part = a.part + (static_cast<int64_t>(block) * a.splits * a.rows + row) * (d + 2);
-    const int64_t step = static_cast<int64_t>(a.rows) * (d + 2);
+    const uint32_t rest = blockIdx.x / static_cast<uint32_t>(a.rows);
+    const uint32_t most = static_cast<uint32_t>(a.row_blocks) * static_cast<uint32_t>(a.p.c.kv_heads);
+    const int2 run = a.shared[rest];  // means nothing where the sequence has no such block
+    StreamBlock w;
+    w.s = static_cast<int>(rest / most);
+    w.index = rest % most;
+    w.seq = kv_sequence(a.p.b, w.s);
+    uint32_t blocks;
+    stream_cost(a, w.seq, &blocks);
+    stream_rows(a, blocks, &w);
+    if (row >= w.rows || run.y <= 1) return;
+    const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, d = a.p.c.head_dim;
     float m = -1e30f, l = 0.f, acc[kRowChunks];
-    for (int s = lane; s < n; s += kWave) m = fmaxf(m, part[s * step]);
-    m = wave_max(m);
-    for (int s = lane; s < n; s += kWave) l += part[s * step + 1] * __builtin_amdgcn_exp2f(part[s * step] - m);
-    l = wave_sum(l);
 #pragma unroll
     for (int c = 0; c < kRowChunks; ++c) acc[c] = 0.f;
-#pragma unroll 4
-    for (int s = wave; s < n; s += kBlock / kWave) {
-        const float f = __builtin_amdgcn_exp2f(part[s * step] - m);
+    for (int i = wave; i < run.y; i += kAhead * kWaves) {
+        float ms[kAhead], ls[kAhead], x[kAhead][kRowChunks];
 #pragma unroll
-        for (int c = 0; c < kRowChunks; ++c)
-            if (lane + c * kWave < d) acc[c] += part[s * step + 2 + lane + c * kWave] * f;
+        for (int u = 0; u < kAhead; ++u) {
+            const int j = i + u * kWaves;
+            ms[u] = -1e30f;
+            ls[u] = 0.f;
+#pragma unroll
+            for (int c = 0; c < kRowChunks; ++c) x[u][c] = 0.f;
+            if (j >= run.y) continue;
+            // The first workgroup's run ends in the block, the others' begin.
+            const float* part = stream_part(a, static_cast<uint32_t>(run.x + j), j == 0, row);
+            ms[u] = part[0];
+            ls[u] = part[1];
+#pragma unroll
+            for (int c = 0; c < kRowChunks; ++c)
+                if (lane + c * kWave < d) x[u][c] = part[2 + lane + c * kWave];
+        }
+        float m_new = m;
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) m_new = fmaxf(m_new, ms[u]);
+        const float f = __builtin_amdgcn_exp2f(m - m_new);
+        m = m_new;
+        l *= f;
+#pragma unroll
+        for (int c = 0; c < kRowChunks; ++c) acc[c] *= f;
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            const float g = __builtin_amdgcn_exp2f(ms[u] - m);
+            l += ls[u] * g;
+#pragma unroll
+            for (int c = 0; c < kRowChunks; ++c) acc[c] += x[u][c] * g;
+        }
     }
 #pragma unroll
     for (int c = 0; c < kRowChunks; ++c) share[wave][lane + c * kWave] = acc[c];
+    if (lane == 0) {
+        share[wave][kKvMaxDim] = m;
+        share[wave][kKvMaxDim + 1] = l;
+    }
     __syncthreads();
     const int x = static_cast<int>(threadIdx.x);
     if (x >= d) return;
+    float top = share[0][kKvMaxDim];
+#pragma unroll
+    for (int v = 1; v < kWaves; ++v) top = fmaxf(top, share[v][kKvMaxDim]);
+    float sum = 0.f, all = 0.f;
+#pragma unroll
+    for (int v = 0; v < kWaves; ++v) {
+        const float f = __builtin_amdgcn_exp2f(share[v][kKvMaxDim] - top);
+        sum += share[v][x] * f;
+        all += share[v][kKvMaxDim + 1] * f;
+    }
     const int r = w.row0 + row;
     a.p.out[(w.seq.first + r / a.p.group) * a.p.ld_out + static_cast<int64_t>(w.head * a.p.group + r % a.p.group) * d + x] =
-        ((share[0][x] + share[1][x]) + (share[2][x] + share[3][x])) * (1.0f / (l + 1e-9f));
+        sum * (1.0f / (all + 1e-9f));
 }
-static_assert(kKvMaxDim <= kBlock && kBlock / kWave == 4, "a thread per dimension, four waves");
+static_assert(kKvMaxDim <= kBlock, "a thread per dimension");
 
 template <int DT>
 void launch_stream_dim(const StreamArgs& a, unsigned grid, hipStream_t s) {
@@ -546,6 +703,17 @@ void launch_stream_dim(const StreamArgs& a, unsigned grid, hipStream_t s) {
     if (a.p.c.stride <= 64) paged_stream<DT, 64><<<grid, kThreads, 0, s>>>(a);
     else if (a.p.c.stride <= 128) paged_stream<DT, 128><<<grid, kThreads, 0, s>>>(a);
     else paged_stream<DT, 256><<<grid, kThreads, 0, s>>>(a);
+}
+
+// What a block costs a workgroup besides its keys (its queries, the first keys' way
+// in, the sums' way out), in steps of 128 keys.
+constexpr int64_t kStreamExtra = 2;
+
+// Workgroups that the GPU holds at once.
+int64_t stream_resident(int dtype, int stride) {
+    if (stride > 128) return 256;
+    if (dtype == MIMIR_KV_F32) return stride > 64 ? 512 : 768;
+    return stride > 64 ? 768 : 1024;
 }
 
 int launch_stream(mimir_ctx* ctx, const PagedArgs& p, int dtype, int64_t most_rows) {
@@ -556,24 +724,31 @@ int launch_stream(mimir_ctx* ctx, const PagedArgs& p, int dtype, int64_t most_ro
     a.row_blocks = static_cast<int32_t>((rows + kRows - 1) / kRows);
     a.rows = static_cast<int32_t>(std::min<int64_t>(rows, kRows));
     const int64_t blocks = static_cast<int64_t>(p.b.sequences) * p.c.kv_heads * a.row_blocks;
-    constexpr int64_t kGrain = kKeys * kStreamWaves, kTarget = 2048;
-    const int64_t grains = std::max<int64_t>(1, (p.b.max_len + kGrain - 1) / kGrain);
-    int64_t splits = std::min(grains, std::max<int64_t>(1, kTarget / blocks));
-    if (ctx->tune.decode_splits > 0) splits = std::min<int64_t>(grains, ctx->tune.decode_splits);
-    const int64_t floats = blocks * a.rows * (p.c.head_dim + 2);
-    splits = std::max<int64_t>(1, std::min<int64_t>(splits, kFixedWorkBytes / 4 / floats));
-    a.part = splits > 1 ? fixed_work(ctx) : nullptr;
-    if (!a.part) splits = 1;
-    a.span = static_cast<int32_t>((grains + splits - 1) / splits * kGrain);
-    a.splits = static_cast<int32_t>((grains * kGrain + a.span - 1) / a.span);
-    if (a.splits == 1) a.part = nullptr;
-    MIMIR_REQUIRE(ctx, dispatch_fits(blocks * a.splits, kStreamWaves * kWave) && dispatch_fits(blocks * a.rows, kBlock),
-                  "paged attention: grid of %lld workgroups exceeds the limit", (long long)(blocks * a.splits));
-    a.blocks = static_cast<uint32_t>(blocks);
-    const auto grid = static_cast<unsigned>(blocks * a.splits);
-    if (dtype == MIMIR_KV_F32) launch_stream_dim<MIMIR_KV_F32>(a, grid, ctx->stream);
-    else if (dtype == MIMIR_KV_BF16) launch_stream_dim<MIMIR_KV_BF16>(a, grid, ctx->stream);
-    else launch_stream_dim<MIMIR_KV_I8>(a, grid, ctx->stream);
+    a.groups = static_cast<uint32_t>(ctx->tune.decode_splits > 0 ? ctx->tune.decode_splits : stream_resident(dtype, p.c.stride));
+    // A grain is a step of the four waves, or as many as keep the sum of all in 31 bits.
+    const int64_t len = std::max<int64_t>(p.b.max_len, 1);
+    int64_t grain = 2 * kHalf * kStreamWaves;
+    const auto grains = [&] { return (len + grain - 1) / grain; };
+    // Blocks of up to two steps are not worth a join.
+    const int64_t words = 2 * blocks + static_cast<int64_t>(a.groups) * 2 * a.rows * (p.c.head_dim + 2);
+    float* work = grains() > 2 && words * 4 <= static_cast<int64_t>(kFixedWorkBytes) ? fixed_work(ctx) : nullptr;
+    int64_t grid = blocks;
+    if (work) {
+        a.extra = kStreamExtra;
+        while ((grains() + kStreamExtra) * blocks >= (int64_t{1} << 31) && grains() > 1) grain *= 2;
+        a.shared = reinterpret_cast<int2*>(work);
+        a.part = work + 2 * blocks;
+        grid = std::min<int64_t>(a.groups, blocks * (grains() + kStreamExtra));
+    } else {  // a workgroup per block
+        grain *= grains();
+        a.groups = static_cast<uint32_t>(std::min<int64_t>(blocks, INT32_MAX));
+    }
+    a.grain = static_cast<uint32_t>(grain);
+    MIMIR_REQUIRE(ctx, dispatch_fits(grid, kStreamWaves * kWave) && dispatch_fits(blocks * a.rows, kBlock),
+                  "paged attention: grid of %lld workgroups exceeds the limit", (long long)blocks);
+    if (dtype == MIMIR_KV_F32) launch_stream_dim<MIMIR_KV_F32>(a, static_cast<unsigned>(grid), ctx->stream);
+    else if (dtype == MIMIR_KV_BF16) launch_stream_dim<MIMIR_KV_BF16>(a, static_cast<unsigned>(grid), ctx->stream);
+    else launch_stream_dim<MIMIR_KV_I8>(a, static_cast<unsigned>(grid), ctx->stream);
     if (int st = launched(ctx, "paged_stream")) return st;
     if (!a.part) return MIMIR_OK;
     paged_join<<<static_cast<unsigned>(blocks * a.rows), kBlock, 0, ctx->stream>>>(a);

@@ -1,0 +1,314 @@
+// attention_paged.hpp -- what the kernels of attention over a paged cache share:
+// their arguments, how the work is dealt to workgroups, the conversion of cache
+// entries, and one query row in plain fp32.
+#pragma once
+
+#include "kvcache.hpp"
+#include "split.hpp"
+
+namespace mimir {
+
+constexpr float kPagedLog2e = 1.4426950408889634f;
+// As attention.hip: the running max may lag by this many base-2 units.
+constexpr float kPagedSlack = 8.0f;
+constexpr int kHalf = 16;  // keys in a row that surely stand in one page
+
+struct PagedArgs {
+    KvView c;
+    KvBatch b;
+    const float* q;
+    float* out;
+    int64_t ld_q, ld_out;
+    int32_t heads, group;  // query heads, those that share a key / value head
+    FastDiv group_div;
+    float qscale;          // scale * log2(e)
+    int32_t causal;
+};
+
+// Memory that a kernel only reads, at addresses that a wave shares: scalar loads.
+typedef const __attribute__((address_space(4))) int32_t* scalar_i32;
+
+// --- the work --------------------------------------------------------------------
+// A block is `block_rows` query rows ((token, head of the group) pairs) of one key /
+// value head of a sequence, against the keys that its last row sees.  It costs those
+// keys and `extra`.  All blocks' costs, in order of sequence, head and rows, are dealt
+// to the workgroups in equal runs, so that sequences of any lengths fill the GPU
+// evenly; a run may begin and end inside a block, whose parts paged_join adds up.
+// Every wave works out its run from the sequences' lengths, 64 of them at a time.
+
+// A block that a run begins and others go on with.
+struct PagedShared {
+    int32_t runs;                      // how many have keys of it; 0: none but this one
+    int32_t first, row0, rows, head;   // its sequence's first token, its rows, its key / value head
+    int32_t pad[3];
+};
+
+struct PagedRuns {
+    // Blocks that several runs have keys of, by the run that begins them, and their
+    // sums, [run][2][row][max, sum, head_dim sums].  Null: a run is one whole block.
+    PagedShared* shared;
+    float* part;
+    uint32_t runs;
+    uint32_t extra;      // what a block costs besides its keys, in keys
+    uint32_t grain;      // blocks are cut at multiples of this many keys
+    int32_t block_rows;
+    int32_t part_rows;   // rows of a block that `part` has room for
+    int32_t least_rows, most_rows;  // of a sequence's; those with fewer or more are another kernel's
+};
+
+__device__ __forceinline__ uint32_t lane_of(uint32_t v, int lane) {
+    return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), lane));
+}
+__device__ __forceinline__ uint64_t lane_of(uint64_t v, int lane) {
+    return static_cast<uint64_t>(lane_of(static_cast<uint32_t>(v >> 32), lane)) << 32 | lane_of(static_cast<uint32_t>(v), lane);
+}
+
+// Costs of a sequence's row blocks, the same for each of its heads: row block i costs
+// base + slope (i + 1), since a causal block's keys end `slope` later than the one
+// before it (at the sequence's end at the latest; the last one's cost is too high by
+// what it lacks).
+struct PagedCost {
+    uint32_t base, slope, blocks;
+    __device__ __forceinline__ uint64_t ahead(uint32_t i) const {
+        return static_cast<uint64_t>(i) * base + static_cast<uint64_t>(slope) * i * (i + 1) / 2;
+    }
+};
+
+__device__ __forceinline__ PagedCost paged_cost(const PagedArgs& p, const PagedRuns& a, const KvSequence& q) {
+    const int64_t rows = static_cast<int64_t>(q.n) * p.group;
+    PagedCost c{1, 0, 0};
+    if (rows > 0 && rows >= a.least_rows && rows <= a.most_rows)
+        c.blocks = static_cast<uint32_t>((rows + a.block_rows - 1) / a.block_rows);
+    if (!a.part) return c;
+    c.base = a.extra + static_cast<uint32_t>(p.causal ? max(q.len - q.n, 0) : q.len);
+    c.slope = p.causal ? static_cast<uint32_t>((a.block_rows + p.group - 1) / p.group) : 0;
+    return c;
+}
+
+// 64 sequences in LDS, one a lane.
+struct PagedChunk {
+    uint64_t sum[kWave];  // costs up to the sequence, of this chunk's
+    KvSequence seq[kWave];
+    PagedCost cost[kWave];
+};
+
+// The costs of the sequences from `base` on up to the lane's; wave 0 writes them down.
+__device__ __forceinline__ uint64_t paged_chunk(const PagedArgs& p, const PagedRuns& a, int base, PagedChunk* chunk) {
+    const int lane = static_cast<int>(threadIdx.x % kWave);
+    KvSequence seq{0, 0, 0};
+    PagedCost cost{1, 0, 0};
+    if (base + lane < p.b.sequences) {
+        seq = kv_sequence(p.b, base + lane);
+        cost = paged_cost(p, a, seq);
+    }
+    uint64_t sum = cost.ahead(cost.blocks) * static_cast<uint32_t>(p.c.kv_heads);
+#pragma unroll
+    for (int x = 1; x < kWave; x *= 2) {
+        const auto y = static_cast<uint64_t>(__shfl_up(static_cast<unsigned long long>(sum), x));
+        if (lane >= x) sum += y;
+    }
+    if (chunk && threadIdx.x < kWave) {
+        chunk->sum[lane] = sum;
+        chunk->seq[lane] = seq;
+        chunk->cost[lane] = cost;
+    }
+    return sum;
+}
+
+// Keys that row `row` (of all its sequence's) sees.
+__device__ __forceinline__ int row_end(const PagedArgs& p, const KvSequence& q, int row) {
+    return p.causal ? min(max(q.len - q.n + static_cast<int>(fastdiv(static_cast<uint32_t>(row), p.group_div)) + 1, 0), q.len) : q.len;
+}
+
+// A run's part of a block.
+struct PagedPiece {
+    int s, head, row0, rows;  // sequence, key / value head, first row and rows of the block
+    KvSequence seq;
+    int k0, k1;               // keys
+    bool whole, begins;       // all of the block's keys; the first of them
+};
+
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ uint32_t uniform(uint32_t x) {
+    return static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(x)));
+}
+
+__device__ __forceinline__ uint64_t uniform(uint64_t x) {
+    return static_cast<uint64_t>(uniform(static_cast<uint32_t>(x >> 32))) << 32 | uniform(static_cast<uint32_t>(x));
+}
+
+// The pieces of one run, in order.  All waves of the workgroup walk together.
+struct PagedWalk {
+    PagedChunk* chunk;
+    int base;                  // of the chunk: its first sequence, the costs ahead of it
+    uint64_t before;
+    uint64_t from, end, run;   // what is left of the run, the length of all runs
+    uint32_t index;
+
+    __device__ __forceinline__ PagedWalk(const PagedArgs& p, const PagedRuns& a, uint32_t index_, PagedChunk* chunk_)
+        : chunk(chunk_), base(0), before(0), index(index_) {
+        uint64_t total = lane_of(paged_chunk(p, a, 0, chunk), kWave - 1);
+        for (int b = kWave; b < p.b.sequences; b += kWave) total += lane_of(paged_chunk(p, a, b, nullptr), kWave - 1);
+        run = uniform(a.part ? max((total + a.runs - 1) / a.runs, static_cast<uint64_t>(a.extra + a.grain)) : uint64_t{1});
+        from = uniform(min(total, run * index));
+        end = uniform(min(total, from + run));
+        // A run of nothing begins no block; the others say so as they end.
+        if (a.part && from >= end && threadIdx.x == 0) a.shared[index].runs = 0;
+        __syncthreads();
+    }
+    __device__ __forceinline__ bool more() const { return from < end; }
+
+    __device__ __forceinline__ PagedPiece next(const PagedArgs& p, const PagedRuns& a) {
+        const int mine = static_cast<int>(threadIdx.x % kWave);
+        uint64_t sum;
+        for (;;) {
+            sum = chunk->sum[mine];
+            const uint64_t to = before + lane_of(sum, kWave - 1);
+            if (from < to || base + kWave >= p.b.sequences) break;
+            __syncthreads();  // all waves have read it
+            base += kWave;
+            before = uniform(to);
+            paged_chunk(p, a, base, chunk);
+            __syncthreads();
+        }
+        const uint64_t above = __ballot(before + sum > from);
+        const int lane = above ? __builtin_ctzll(above) : 0;
+        PagedPiece w;
+        w.s = base + lane;
+        w.seq = KvSequence{uniform(chunk->seq[lane].first), uniform(chunk->seq[lane].n), uniform(chunk->seq[lane].len)};
+        const PagedCost cost{uniform(chunk->cost[lane].base), uniform(chunk->cost[lane].slope), uniform(chunk->cost[lane].blocks)};
+        const uint64_t head_cost = cost.ahead(cost.blocks);
+        uint64_t first = before + lane_of(sum, lane) - head_cost * static_cast<uint32_t>(p.c.kv_heads);
+        w.head = uniform(static_cast<int>((from - first) / head_cost));
+        first += head_cost * static_cast<uint32_t>(w.head);
+        uint32_t lo = 0, hi = cost.blocks;  // row block lo begins at or before `from`, hi after it
+        while (hi - lo > 1) {
+            const uint32_t mid = (lo + hi) / 2;
+            if (first + cost.ahead(mid) <= from) lo = mid;
+            else hi = mid;
+        }
+        lo = uniform(lo);
+        first = uniform(first + cost.ahead(lo));
+        w.row0 = static_cast<int>(lo) * a.block_rows;
+        w.rows = min(w.seq.n * p.group - w.row0, a.block_rows);
+        const int keys = row_end(p, w.seq, w.row0 + w.rows - 1);
+        const uint64_t all = static_cast<uint64_t>(cost.base) + static_cast<uint64_t>(cost.slope) * (lo + 1);
+        const uint64_t x0 = from - first, x1 = min(all, end - first);
+        const auto cut = [&](uint64_t x) {
+            return x >= all ? keys : static_cast<int>(static_cast<uint64_t>(keys) * x / all / a.grain * a.grain);
+        };
+        w.k0 = uniform(cut(x0));
+        w.k1 = uniform(cut(x1));
+        w.begins = x0 == 0;
+        w.whole = w.begins && x1 == all;
+        if (a.part && threadIdx.x == 0 && w.begins && !w.whole)
+            a.shared[index] = PagedShared{static_cast<int32_t>((first + all - 1) / run - index) + 1, w.seq.first, w.row0, w.rows, w.head, {}};
+        from = uniform(first + x1);
+        // None that a later run goes on with.
+        if (a.part && threadIdx.x == 0 && from >= end && (w.whole || !w.begins)) a.shared[index].runs = 0;
+        return w;
+    }
+};
+
+// Where a run keeps the sums of a block that it shares with others: the one that it
+// begins (1) or goes on with (0).
+__device__ __forceinline__ float* paged_part(const PagedRuns& a, int head_dim, uint32_t run, bool begins, int row) {
+    return a.part + ((static_cast<int64_t>(run) * 2 + (begins ? 1 : 0)) * a.part_rows + row) * (head_dim + 2);
+}
+
+// Row `row` of a sequence's (token, head) rows in q and out.
+__device__ __forceinline__ int64_t paged_row(const PagedArgs& p, int64_t ld, int first, int head, int row) {
+    const auto t = static_cast<int>(fastdiv(static_cast<uint32_t>(row), p.group_div));
+    return (first + static_cast<int64_t>(t)) * ld + static_cast<int64_t>(head * p.group + row - t * p.group) * p.c.head_dim;
+}
+
+// --- entries ---------------------------------------------------------------------
+
+// The two's complement bytes of a dword as floats, and pairs of small whole numbers
+// (exact in bf16, so their floats' upper halves) packed.
+__device__ __forceinline__ float byte_float(uint32_t w, int i) {
+    return static_cast<float>(static_cast<int32_t>(w << (24 - 8 * i)) >> 24);
+}
+__device__ __forceinline__ uint32_t pack_high(float a, float b) {
+    return __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, b), __builtin_bit_cast(uint32_t, a), 0x07060302u);
+}
+__device__ __forceinline__ u4 bytes_bf16(uint32_t lo, uint32_t hi) {
+    u4 r;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        r[i] = pack_high(byte_float(lo, 2 * i), byte_float(lo, 2 * i + 1));
+        r[2 + i] = pack_high(byte_float(hi, 2 * i), byte_float(hi, 2 * i + 1));
+    }
+    return r;
+}
+
+// Element d of a cache row (index `at` among the rows of the type's buffer).
+template <int DT>
+__device__ __forceinline__ float element(const char* base, int64_t at, int stride, int d) {
+    const int64_t i = at * stride + d;
+    if constexpr (DT == MIMIR_KV_F32) return reinterpret_cast<const float*>(base)[i];
+    else if constexpr (DT == MIMIR_KV_BF16)
+        return __builtin_bit_cast(float, static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(base)[i]) << 16);
+    else return static_cast<float>(reinterpret_cast<const int8_t*>(base)[i]);
+}
+
+constexpr int kRowChunks = kKvMaxDim / kWave;
+
+// One query row over keys j0 .. j1 - 1 by one wave, lane l holding dimensions l + 64 c.
+// Leaves the sums (without the division) and the running max (base-2 units) and sum.
+template <int DT>
+__device__ __forceinline__ void row_over_keys(const PagedArgs& a, int s, int kv_head, const float* q, int j0, int j1,
+                                              float* acc, float* m_out, float* l_out) {
+    const int lane = threadIdx.x % kWave;
+    float x[kRowChunks];
+#pragma unroll
+    for (int c = 0; c < kRowChunks; ++c) {
+        const int d = lane + c * kWave;
+        x[c] = d < a.c.head_dim ? q[d] * a.qscale : 0.f;
+        acc[c] = 0.f;
+    }
+    float m = -1e30f, l = 0.f;
+    for (int j = j0; j < j1; ++j) {
+        const auto [page, slot] = kv_slot(a.b, a.c.pages, a.c.page_div, s, j);
+        if (page < 0) continue;
+        const int64_t at = (static_cast<int64_t>(page) * a.c.kv_heads + kv_head) * a.c.page_size + slot;
+        float part = 0.f;
+#pragma unroll
+        for (int c = 0; c < kRowChunks; ++c) {
+            const int d = lane + c * kWave;
+            if (d < a.c.head_dim) part += x[c] * element<DT>(a.c.k, at, a.c.stride, d);
+        }
+        float score = wave_sum(part);
+        if constexpr (DT == MIMIR_KV_I8) score *= a.c.k_scale[at];
+        const float m_new = fmaxf(m, score);
+        const float alpha = __builtin_amdgcn_exp2f(m - m_new);
+        const float p = __builtin_amdgcn_exp2f(score - m_new);
+        m = m_new;
+        l = l * alpha + p;
+        const float w = DT == MIMIR_KV_I8 ? p * a.c.v_scale[at] : p;
+#pragma unroll
+        for (int c = 0; c < kRowChunks; ++c) {
+            const int d = lane + c * kWave;
+            if (d < a.c.head_dim) acc[c] = acc[c] * alpha + w * element<DT>(a.c.v, at, a.c.stride, d);
+        }
+    }
+    *m_out = m;
+    *l_out = l;
+}
+
+// The host's side (attention_paged_stream.hip, attention_paged_block.hip): sequences
+// of up to `most_rows` query rows a key / value head, and of `least_rows` on.
+int paged_stream_launch(mimir_ctx* ctx, const PagedArgs& p, int dtype, int64_t most_rows);
+int paged_block_launch(mimir_ctx* ctx, const PagedArgs& p, int dtype, int64_t least_rows);
+
+// The widest heads (padded) of the block kernel: its queries' terms are registers.
+constexpr int kPagedBlockStride = 128;
+
+// Joins the blocks that several runs had keys of.
+int paged_join_launch(mimir_ctx* ctx, const PagedArgs& p, const PagedRuns& a);
+
+// Sets up `a` for at most `runs` workgroups in the workspace, or for one per block
+// (`blocks` of them) where that is not to be had or `split` says not to; the grid.
+int64_t paged_runs(mimir_ctx* ctx, const PagedArgs& p, PagedRuns* a, int64_t runs, int64_t blocks, bool split);
+
+}  // namespace mimir

@@ -36,6 +36,8 @@ struct mimir_ctx {
     // dealt to several workgroups (attention.hip, attention_decode.hip), in stream
     // order.  Made by the first call that deals them (fixed_work), kept.
     void* fixed_work = nullptr;
+    // The same for attention over a paged cache (attention_paged.hip), kPagedWorkBytes.
+    void* paged_work = nullptr;
     // This GPU's columns of 1.0f then -0.0f (mimir::kUnitCols each), the
     // weights of a row kernel's absent scale / bias (norm.hip).
     const float* unit_weights = nullptr;
@@ -146,6 +148,10 @@ constexpr size_t kFixedWorkBytes = sizeof(float) * 256 * 256 * 130;
 // The workspace, null where there is no memory for it: the call then runs on one
 // workgroup per query block.
 float* fixed_work(mimir_ctx* ctx);
+// What attention over a paged cache keeps of blocks that two workgroups share: two of
+// 256 rows of 128 dimensions for each of 256, and which they are.
+constexpr size_t kPagedWorkBytes = sizeof(float) * 256 * 2 * 256 * 130 + 64 * 1024;
+char* paged_work(mimir_ctx* ctx);
 bool attention_decode_applies(int64_t bh, int64_t q_len, int64_t kv_len, int64_t head_dim, bool causal);
 int attention_decode_launch(mimir_ctx* ctx, const float* q, int64_t ld_q, const float* k, const float* v, int64_t ld_kv,
                             float* out, int64_t ld_out, int64_t batch, int64_t q_len, int64_t kv_len, int64_t heads,

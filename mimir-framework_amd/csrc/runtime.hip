@@ -108,20 +108,28 @@ int mimir::ensure_scratch(mimir_ctx* ctx, size_t bytes, void** out) {
     return MIMIR_OK;
 }
 
-float* mimir::fixed_work(mimir_ctx* ctx) {
-    if (!ctx->fixed_work) {
+namespace {
+
+// A workspace that the first call makes and the context keeps.
+void* kept_work(void** work, size_t bytes) {
+    if (!*work) {
         // A stream may be capturing, this context's or another thread's: the
         // allocation is no part of the graph.
         hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
         if (hipThreadExchangeStreamCaptureMode(&mode) != hipSuccess) return nullptr;
-        if (hipMalloc(&ctx->fixed_work, kFixedWorkBytes) != hipSuccess) {
+        if (hipMalloc(work, bytes) != hipSuccess) {
             (void)hipGetLastError();
-            ctx->fixed_work = nullptr;
+            *work = nullptr;
         }
         (void)hipThreadExchangeStreamCaptureMode(&mode);
     }
-    return static_cast<float*>(ctx->fixed_work);
+    return *work;
 }
+
+}  // namespace
+
+float* mimir::fixed_work(mimir_ctx* ctx) { return static_cast<float*>(kept_work(&ctx->fixed_work, kFixedWorkBytes)); }
+char* mimir::paged_work(mimir_ctx* ctx) { return static_cast<char*>(kept_work(&ctx->paged_work, kPagedWorkBytes)); }
 
 extern "C" {
 
@@ -161,6 +169,7 @@ int mimir_ctx_destroy(mimir_ctx* ctx) {
         for (auto& kv : ctx->allocs) (void)hipFree(kv.first);
         if (ctx->scratch) (void)hipFree(ctx->scratch);
         if (ctx->fixed_work) (void)hipFree(ctx->fixed_work);
+        if (ctx->paged_work) (void)hipFree(ctx->paged_work);
         for (void* p : ctx->retired) (void)hipFree(p);
         (void)hipStreamDestroy(ctx->own_stream);
     }

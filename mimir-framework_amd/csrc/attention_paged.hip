@@ -17,88 +17,87 @@ namespace {
 
 constexpr int64_t kStreamRows = 32;
 
-// The shares of one row: brought to one max, added up and divided.  WAVES waves a
-// row; the block's first run (this descriptor's) kept what it begins, the others what
-// they go on with.
-template <int WAVES>
+// The shares of one row: brought to one max, added up and divided.  LPR lanes hold a
+// row, four dimensions each.  ONE: the whole workgroup takes one row, its groups of
+// lanes every so many of the runs (a long sequence's row may have dozens); else each
+// group a row of its own.  The block's first run, whose descriptor this is, kept what
+// it begins, the others what they go on with.
+template <int LPR, bool ONE>
 __global__ __launch_bounds__(kBlock) void paged_join(PagedArgs p, PagedRuns a) {
-    constexpr int kAhead = 4, kRowsOf = kBlock / kWave / WAVES;
-    __shared__ float share[kBlock / kWave][kKvMaxDim + 2];
-    const uint32_t groups = static_cast<uint32_t>((a.part_rows + kRowsOf - 1) / kRowsOf);
-    const uint32_t first = blockIdx.x / groups;
+    constexpr int kAhead = 4, kGroups = kBlock / LPR, kEach = ONE ? kGroups : 1, kRowsOf = ONE ? 1 : kGroups;
+    __shared__ f4 share[kGroups][LPR];
+    __shared__ f2 stats[kGroups];
+    const uint32_t parts = static_cast<uint32_t>((a.part_rows + kRowsOf - 1) / kRowsOf);
+    const uint32_t first = blockIdx.x / parts;
     const PagedShared s = a.shared[first];
-    const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, d = p.c.head_dim;
-    const int row = static_cast<int>(blockIdx.x % groups) * kRowsOf + wave / WAVES;
     if (s.runs <= 1) return;
+    const int lane = threadIdx.x % LPR, group = threadIdx.x / LPR, d = p.c.head_dim;
+    const int row = static_cast<int>(blockIdx.x % parts) * kRowsOf + (ONE ? 0 : group);
+    if (ONE && row >= s.rows) return;  // the whole workgroup
     const bool mine = row < s.rows;
-    float m = -1e30f, l = 0.f, acc[kRowChunks];
-#pragma unroll
-    for (int c = 0; c < kRowChunks; ++c) acc[c] = 0.f;
-    for (int i = wave % WAVES; mine && i < s.runs; i += kAhead * WAVES) {
-        float ms[kAhead], ls[kAhead], x[kAhead][kRowChunks];
+    float m = -1e30f, l = 0.f;
+    f4 acc{0.f, 0.f, 0.f, 0.f};
+    for (int i = ONE ? group : 0; mine && i < s.runs; i += kAhead * kEach) {
+        f2 st[kAhead];
+        f4 x[kAhead];
 #pragma unroll
         for (int u = 0; u < kAhead; ++u) {
-            const int j = i + u * WAVES;
-            ms[u] = -1e30f;
-            ls[u] = 0.f;
-#pragma unroll
-            for (int c = 0; c < kRowChunks; ++c) x[u][c] = 0.f;
+            const int j = i + u * kEach;
+            st[u] = f2{-1e30f, 0.f};
+            x[u] = f4{0.f, 0.f, 0.f, 0.f};
             if (j >= s.runs) continue;
-            const float* part = paged_part(a, d, first + static_cast<uint32_t>(j), j == 0, row);
-            ms[u] = part[0];
-            ls[u] = part[1];
-#pragma unroll
-            for (int c = 0; c < kRowChunks; ++c)
-                if (lane + c * kWave < d) x[u][c] = part[2 + lane + c * kWave];
+            const PagedPart part(a, d, first + static_cast<uint32_t>(j), j == 0);
+            st[u] = *part.stat(row);
+            if (4 * lane < d) x[u] = *reinterpret_cast<const f4*>(part.sums(row) + 4 * lane);
         }
         float m_new = m;
 #pragma unroll
-        for (int u = 0; u < kAhead; ++u) m_new = fmaxf(m_new, ms[u]);
+        for (int u = 0; u < kAhead; ++u) m_new = fmaxf(m_new, st[u][0]);
         const float f = __builtin_amdgcn_exp2f(m - m_new);
         m = m_new;
         l *= f;
-#pragma unroll
-        for (int c = 0; c < kRowChunks; ++c) acc[c] *= f;
+        acc *= f;
 #pragma unroll
         for (int u = 0; u < kAhead; ++u) {
-            const float g = __builtin_amdgcn_exp2f(ms[u] - m);
-            l += ls[u] * g;
-#pragma unroll
-            for (int c = 0; c < kRowChunks; ++c) acc[c] += x[u][c] * g;
+            const float g = __builtin_amdgcn_exp2f(st[u][0] - m);
+            l += st[u][1] * g;
+            acc += x[u] * g;
         }
     }
-    if constexpr (WAVES > 1) {
-#pragma unroll
-        for (int c = 0; c < kRowChunks; ++c) share[wave][lane + c * kWave] = acc[c];
-        if (lane == 0) {
-            share[wave][kKvMaxDim] = m;
-            share[wave][kKvMaxDim + 1] = l;
-        }
+    if constexpr (ONE) {
+        share[group][lane] = acc;
+        if (lane == 0) stats[group] = f2{m, l};
         __syncthreads();
-        const int w0 = wave / WAVES * WAVES;
-        if (wave != w0) return;
+        if (group > 0) return;
 #pragma unroll
-        for (int v = 1; v < WAVES; ++v) {
-            const float mv = share[w0 + v][kKvMaxDim], m_new = fmaxf(m, mv);
-            const float f = __builtin_amdgcn_exp2f(m - m_new), g = __builtin_amdgcn_exp2f(mv - m_new);
+        for (int v = 1; v < kGroups; ++v) {
+            const f2 st = stats[v];
+            const float m_new = fmaxf(m, st[0]);
+            const float f = __builtin_amdgcn_exp2f(m - m_new), g = __builtin_amdgcn_exp2f(st[0] - m_new);
             m = m_new;
-            l = l * f + share[w0 + v][kKvMaxDim + 1] * g;
-#pragma unroll
-            for (int c = 0; c < kRowChunks; ++c) acc[c] = acc[c] * f + share[w0 + v][lane + c * kWave] * g;
+            l = l * f + st[1] * g;
+            acc = acc * f + share[v][lane] * g;
         }
     }
     if (!mine) return;
     const float inv = 1.0f / (l + 1e-9f);
     float* out = p.out + paged_row(p, p.ld_out, s.first, s.head, s.row0 + row);
 #pragma unroll
-    for (int c = 0; c < kRowChunks; ++c)
-        if (lane + c * kWave < d) out[lane + c * kWave] = acc[c] * inv;
+    for (int e = 0; e < 4; ++e)  // a row's sums may be followed by what nothing wrote
+        if (4 * lane + e < d) out[4 * lane + e] = acc[e] * inv;
+}
+
+template <int LPR>
+void launch_join(const PagedArgs& p, const PagedRuns& a, hipStream_t s) {
+    constexpr int kRowsOf = kBlock / LPR;
+    if (a.part_rows <= 16) paged_join<LPR, true><<<a.runs * static_cast<unsigned>(a.part_rows), kBlock, 0, s>>>(p, a);
+    else paged_join<LPR, false><<<a.runs * static_cast<unsigned>((a.part_rows + kRowsOf - 1) / kRowsOf), kBlock, 0, s>>>(p, a);
 }
 
 }  // namespace
 
 int64_t mimir::paged_runs(mimir_ctx* ctx, const PagedArgs& p, PagedRuns* a, int64_t runs, int64_t blocks, bool split) {
-    const int64_t floats = runs * 2 * a->part_rows * (p.c.head_dim + 2);
+    const int64_t floats = runs * 2 * paged_part_floats(a->part_rows, p.c.head_dim);
     const int64_t bytes = runs * static_cast<int64_t>(sizeof(PagedShared)) + floats * 4;
     char* work = split && bytes <= static_cast<int64_t>(kPagedWorkBytes) ? paged_work(ctx) : nullptr;
     if (!work) return blocks;
@@ -110,9 +109,8 @@ int64_t mimir::paged_runs(mimir_ctx* ctx, const PagedArgs& p, PagedRuns* a, int6
 
 int mimir::paged_join_launch(mimir_ctx* ctx, const PagedArgs& p, const PagedRuns& a) {
     if (!a.part) return MIMIR_OK;
-    // Few rows: four waves each, as many runs may have shared a long sequence.
-    if (a.part_rows <= 16) paged_join<4><<<a.runs * static_cast<unsigned>(a.part_rows), kBlock, 0, ctx->stream>>>(p, a);
-    else paged_join<1><<<a.runs * static_cast<unsigned>((a.part_rows + 3) / 4), kBlock, 0, ctx->stream>>>(p, a);
+    if (p.c.head_dim <= 128) launch_join<32>(p, a, ctx->stream);
+    else launch_join<64>(p, a, ctx->stream);
     return launched(ctx, "paged_join");
 }
 

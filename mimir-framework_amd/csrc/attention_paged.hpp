@@ -45,7 +45,7 @@ struct PagedShared {
 
 struct PagedRuns {
     // Blocks that several runs have keys of, by the run that begins them, and their
-    // sums, [run][2][row][max, sum, head_dim sums].  Null: a run is one whole block.
+    // sums (PagedPart).  Null: a run is one whole block.
     PagedShared* shared;
     float* part;
     uint32_t runs;
@@ -210,11 +210,24 @@ struct PagedWalk {
     }
 };
 
-// Where a run keeps the sums of a block that it shares with others: the one that it
-// begins (1) or goes on with (0).
-__device__ __forceinline__ float* paged_part(const PagedRuns& a, int head_dim, uint32_t run, bool begins, int row) {
-    return a.part + ((static_cast<int64_t>(run) * 2 + (begins ? 1 : 0)) * a.part_rows + row) * (head_dim + 2);
+// Where a run keeps the sums of a block that it shares with others, the one that it
+// begins or goes on with: a max and a sum per row, then rows of head_dim sums from
+// 16-byte boundaries on.
+__host__ __device__ inline int64_t paged_part_stats(int part_rows) { return (2 * static_cast<int64_t>(part_rows) + 3) & ~int64_t{3}; }
+__host__ __device__ inline int64_t paged_part_stride(int head_dim) { return (head_dim + 3) & ~3; }
+__host__ __device__ inline int64_t paged_part_floats(int part_rows, int head_dim) {
+    return paged_part_stats(part_rows) + part_rows * paged_part_stride(head_dim);
 }
+struct PagedPart {
+    float* at;
+    int32_t rows;
+    int64_t stride;
+    __device__ __forceinline__ PagedPart(const PagedRuns& a, int head_dim, uint32_t run, bool begins)
+        : at(a.part + (static_cast<int64_t>(run) * 2 + (begins ? 1 : 0)) * paged_part_floats(a.part_rows, head_dim)),
+          rows(a.part_rows), stride(paged_part_stride(head_dim)) {}
+    __device__ __forceinline__ f2* stat(int row) const { return reinterpret_cast<f2*>(at) + row; }
+    __device__ __forceinline__ float* sums(int row) const { return at + paged_part_stats(rows) + row * stride; }
+};
 
 // Row `row` of a sequence's (token, head) rows in q and out.
 __device__ __forceinline__ int64_t paged_row(const PagedArgs& p, int64_t ld, int first, int head, int row) {

@@ -27,9 +27,9 @@ struct BlockTile {
     static constexpr int kValueRow = DP % 64 == 32 ? 2 * DP : 2 * DP + 64;
     static_assert(kValueRow / 4 % 32 == 16, "four rows' reads in different banks");
     static constexpr int kKeyPlane = kTile * kKeyRow, kValuePlane = kTile * kValueRow;
-    static constexpr int kValuesAt = kPlanes * kKeyPlane;
-    static constexpr int kScalesAt = kValuesAt + kPlanes * kValuePlane;  // 8-bit: 32 of the keys, 32 of the values
-    static constexpr int kBytes = kScalesAt + (DT == MIMIR_KV_I8 ? 2 * kTile * 4 : 0);
+    static constexpr int kScalesAt = kPlanes * kKeyPlane;  // 8-bit: 32 of the keys, 32 of the values, beside the keys
+    static constexpr int kKeyBytes = kScalesAt + (DT == MIMIR_KV_I8 ? 2 * kTile * 4 : 0);
+    static constexpr int kValueBytes = kPlanes * kValuePlane;
 };
 
 // Eight elements of a row on their way from memory to LDS.
@@ -37,18 +37,14 @@ template <int DT>
 struct RowItem {
     static constexpr int kVecs = DT == MIMIR_KV_F32 ? 2 : 1;
     u4 v[kVecs];
-    __device__ __forceinline__ void load(const char* p) {
+    __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t rows, uint32_t off) {
         if constexpr (DT == MIMIR_KV_I8) {
-            const u2 x = *reinterpret_cast<const u2*>(p);
+            const u2 x = __builtin_amdgcn_raw_buffer_load_b64(rows, off, 0, 0);
             v[0] = u4{x[0], x[1], 0, 0};
         } else {
 #pragma unroll
-            for (int i = 0; i < kVecs; ++i) v[i] = reinterpret_cast<const u4*>(p)[i];
+            for (int i = 0; i < kVecs; ++i) v[i] = __builtin_amdgcn_raw_buffer_load_b128(rows, off + 16 * i, 0, 0);
         }
-    }
-    __device__ __forceinline__ void clear() {
-#pragma unroll
-        for (int i = 0; i < kVecs; ++i) v[i] = u4{0, 0, 0, 0};
     }
     __device__ __forceinline__ void stash(char* lds, int plane) const {
         if constexpr (DT == MIMIR_KV_F32) {
@@ -80,8 +76,13 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void paged_block(PagedArgs p, Pag
     using Tile = BlockTile<DT, DP>;
     constexpr int kThreads = WAVES * kWave, kC = DP / 16, kDb = DP / 32;
     constexpr int kElement = DT == MIMIR_KV_F32 ? 4 : DT == MIMIR_KV_BF16 ? 2 : 1;
-    constexpr int kItems = (kTile * (DP / 8) + kThreads - 1) / kThreads;
-    __shared__ __attribute__((aligned(16))) char lds[2 * Tile::kBytes];
+    // Eight waves: the second four, which share the SIMDs with the first, multiply a
+    // tile's values one tile later, so that one's softmax runs beside the other's products;
+    // the values stay that much longer.
+    constexpr bool kStagger = WAVES == 8;
+    constexpr int kValueBufs = kStagger ? 3 : 2;
+    __shared__ __attribute__((aligned(16))) char lds[2 * Tile::kKeyBytes + kValueBufs * Tile::kValueBytes];
+    char* const values = lds + 2 * Tile::kKeyBytes;
     __shared__ PagedChunk chunk;
 
     // Each XCD takes runs that follow each other, whose keys it has in its L2.
@@ -100,10 +101,11 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void paged_block(PagedArgs p, Pag
     const int my_end = min(row_end(p, w.seq, min(my_row, w.row0 + w.rows - 1)), k1);
     const int wave_end = wave_rows > 0 ? min(k1, row_end(p, w.seq, w.row0 + wave * kTile + wave_rows - 1)) : k0;
     const auto q_row = [&](int row) { return p.q + paged_row(p, p.ld_q, w.seq.first, w.head, row); };
+    const PagedPart part(a, p.c.head_dim, walk.index, w.begins);
     // Row of the block: its output, or where its sums are kept.
     const auto out_row = [&](int row) {
         return w.whole ? p.out + paged_row(p, p.ld_out, w.seq.first, w.head, w.row0 + row)
-                       : paged_part(a, p.c.head_dim, walk.index, w.begins, row) + 2;
+                       : part.sums(row);
     };
 
     // This lane's query values, times scale * log2(e).
@@ -126,8 +128,10 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void paged_block(PagedArgs p, Pag
     const int tiles = (k1 - k0 + kTile - 1) / kTile;
     const scalar_i32 table = (scalar_i32)(p.b.page_table + w.s * p.b.ld_pages);
     const int row_bytes = p.c.stride * kElement;
+    // Where a tile's halves stand, and how many of their keys are there (none of one
+    // without a page).
     struct Pages {
-        int page[2], slot[2];
+        int page[2], slot[2], keys[2];
     };
     const auto find = [&](int t) {
         Pages g;
@@ -135,50 +139,57 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void paged_block(PagedArgs p, Pag
         for (int u = 0; u < 2; ++u) {
             const int j = k0 + t * kTile + kHalf * u, i = max(min(j, (k1 - 1) & -kHalf), 0);
             const uint32_t entry = fastdiv(static_cast<uint32_t>(i), p.c.page_div);
-            const int page = j < k1 ? table[entry] : -1;
-            g.page[u] = page < p.c.pages ? page : -1;
+            g.page[u] = j < k1 ? table[entry] : -1;
             g.slot[u] = i - static_cast<int>(entry) * p.c.page_size;
+            g.keys[u] = min(k1 - j, kHalf);
         }
         return g;
     };
-    const auto cache_row = [&](const Pages& g, int u) {
-        return (static_cast<int64_t>(max(g.page[u], 0)) * p.c.kv_heads + w.head) * p.c.page_size + g.slot[u];
-    };
+    const auto pages = static_cast<uint32_t>(p.c.pages);
+    const auto there = [&](const Pages& g, int u) { return static_cast<uint32_t>(g.page[u]) < pages; };
+    // A thread's items: eight dimensions of a row.  The rows of a wave are of one half.
+    // What lies past a row's dimensions or the half's keys reads as zeros.
+    constexpr int kLanes = DP == 64 ? 8 : 16;
+    constexpr int kItems = (kTile * kLanes + kThreads - 1) / kThreads;
+    static_assert(kWave / kLanes <= kHalf && kHalf % (kWave / kLanes) == 0, "a wave's rows in one half");
+    const int d_mine = 8 * (tid % kLanes);
+    const auto row_of = [&](int n) { return (tid + n * kThreads) / kLanes; };
     RowItem<DT> ki[kItems], vi[kItems];
     float scale = 0.f;
-    const auto load = [&](int t, const Pages& g) {
-        const int64_t r0 = cache_row(g, 0), r1 = cache_row(g, 1);
+    const auto load = [&](const Pages& g) {
 #pragma unroll
         for (int n = 0; n < kItems; ++n) {
-            const int id = tid + n * kThreads, row = id / (DP / 8), d = 8 * (id % (DP / 8));
-            if (row >= kTile) continue;
-            const int u = row / kHalf;
-            const int64_t off = ((u ? r1 : r0) + row % kHalf) * row_bytes + min(d, p.c.stride - 8) * kElement;
-            ki[n].load(p.c.k + off);
-            vi[n].load(p.c.v + off);
-            // Dimensions past the row, and values of keys that are not there.
-            if (d >= p.c.stride) ki[n].clear();
-            if (d >= p.c.stride || k0 + t * kTile + row >= k1 || (u ? g.page[1] : g.page[0]) < 0) vi[n].clear();
+            const int u = uniform(row_of(n)) / kHalf;
+            if (u > 1) continue;
+            const bool has = u ? there(g, 1) : there(g, 0);
+            const int64_t row = (static_cast<int64_t>(has ? (u ? g.page[1] : g.page[0]) : 0) * p.c.kv_heads + w.head) * p.c.page_size +
+                                (u ? g.slot[1] : g.slot[0]);
+            const int bytes = has ? (u ? g.keys[1] : g.keys[0]) * row_bytes : 0;
+            const uint32_t off = d_mine < p.c.stride ? static_cast<uint32_t>(row_of(n) % kHalf * row_bytes + d_mine * kElement) : kOutside;
+            ki[n].load(__builtin_amdgcn_make_buffer_rsrc(p.c.k + row * row_bytes, 0, bytes, kBufferWord3), off);
+            vi[n].load(__builtin_amdgcn_make_buffer_rsrc(p.c.v + row * row_bytes, 0, bytes, kBufferWord3), off);
         }
         if constexpr (DT == MIMIR_KV_I8) {
-            if (tid < 2 * kTile) {
-                const int row = tid % kTile, u = row / kHalf;
-                const int64_t at = (u ? r1 : r0) + row % kHalf;
-                scale = (tid < kTile ? p.c.k_scale : p.c.v_scale)[at];
-                if (k0 + t * kTile + row >= k1 || (u ? g.page[1] : g.page[0]) < 0) scale = 0.f;
+            if (wave < 4) {  // the keys' of both halves, then the values'
+                const int u = wave % 2;
+                const bool has = u ? there(g, 1) : there(g, 0);
+                const int64_t row = (static_cast<int64_t>(has ? (u ? g.page[1] : g.page[0]) : 0) * p.c.kv_heads + w.head) * p.c.page_size +
+                                    (u ? g.slot[1] : g.slot[0]);
+                const int bytes = has ? 4 * (u ? g.keys[1] : g.keys[0]) : 0;
+                scale = buffer_f1(buffer_of((wave < 2 ? p.c.k_scale : p.c.v_scale) + row, bytes), static_cast<uint32_t>(4 * (lane % kHalf)));
             }
         }
     };
-    const auto stash = [&](char* buf) {
+    const auto stash = [&](char* key_buf, char* value_buf) {
 #pragma unroll
         for (int n = 0; n < kItems; ++n) {
-            const int id = tid + n * kThreads, row = id / (DP / 8), at = 16 * (id % (DP / 8));
-            if (row >= kTile) continue;
-            ki[n].stash(buf + row * Tile::kKeyRow + at, Tile::kKeyPlane);
-            vi[n].stash(buf + Tile::kValuesAt + row * Tile::kValueRow + at, Tile::kValuePlane);
+            const int row = row_of(n);
+            if (row >= kTile || d_mine >= DP) continue;
+            ki[n].stash(key_buf + row * Tile::kKeyRow + 2 * d_mine, Tile::kKeyPlane);
+            vi[n].stash(value_buf + row * Tile::kValueRow + 2 * d_mine, Tile::kValuePlane);
         }
         if constexpr (DT == MIMIR_KV_I8)
-            if (tid < 2 * kTile) reinterpret_cast<float*>(buf + Tile::kScalesAt)[tid] = scale;
+            if (wave < 4 && lane < kHalf) reinterpret_cast<float*>(key_buf + Tile::kScalesAt)[wave * kHalf + lane] = scale;
     };
 
     f16v o[kDb];
@@ -189,35 +200,100 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void paged_block(PagedArgs p, Pag
     Pages g0{}, g1{}, g2{};  // of the tile in LDS, the one in registers, the next
     if (tiles > 0) {
         g0 = find(0);
-        load(0, g0);
+        load(g0);
         g1 = find(1);
-        stash(lds);
-        load(1, g1);
+        stash(lds, values);
+        load(g1);
         g2 = find(2);
     }
     __syncthreads();
     // A lane's part of a transposed read: key 4 hf + (lane % 16) / 4, dimensions
     // 16 (lane / 16 % 2) + 4 (lane % 4) on.
     const int v_lane = (4 * hf + lane % 16 / 4) * Tile::kValueRow + (lane / 16 % 2 * 16 + 4 * (lane % 4)) * 2;
-    for (int t = 0; t < tiles; ++t) {
-        const char* cur = lds + (t & 1) * Tile::kBytes;
-        char* const next = lds + ((t + 1) & 1) * Tile::kBytes;
-        const int key = k0 + t * kTile;
-        if (key < wave_end) {
-            f16v s = f16v{};
-            __builtin_amdgcn_s_setprio(1);
+    f16v s;  // scores of a tile, then its weights
+    // o += V^T P^T over a tile's keys.  Values are read one operand ahead of their
+    // products, and the second half's weights are split beside the first half's.
+    const auto weigh = [&](const char* buf) {
+        const auto read = [&](int i, u4* v) {
+            const char* const at = buf + v_lane + 16 * (i / kDb) * Tile::kValueRow + 64 * (i % kDb);
 #pragma unroll
-            for (int c = 0; c < kC; ++c) {
-                u4 k[Tile::kPlanes];
+            for (int n = 0; n < Tile::kPlanes; ++n) {
+                const u2 x0 = __builtin_bit_cast(u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(at + n * Tile::kValuePlane)));
+                const u2 x1 = __builtin_bit_cast(
+                    u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(at + n * Tile::kValuePlane + 8 * Tile::kValueRow)));
+                v[n] = u4{x0[0], x0[1], x1[0], x1[1]};
+            }
+        };
+        const auto split = [&](int c) {
+            float x[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = s[8 * c + e];
+            return split8(x);
+        };
+        __builtin_amdgcn_s_setprio(1);
+        u4 v[2][Tile::kPlanes];
+        read(0, v[0]);
+        Split8 pw = split(0), pn;
+#pragma unroll
+        for (int i = 0; i < 2 * kDb; ++i) {
+            if (i + 1 < 2 * kDb) read(i + 1, v[(i + 1) % 2]);
+            if (i == 0) pn = split(1);
+            if (i == kDb) pw = pn;
+            o[i % kDb] = mfma_planes<Tile::kPlanes>(v[i % 2], pw, o[i % kDb]);
+        }
+        if constexpr (Tile::kPlanes == 1) {
+            __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+            __builtin_amdgcn_sched_group_barrier(0x002, 44, 0);
+#pragma unroll
+            for (int i = 0; i < 2 * kDb; ++i) {
+                __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+#pragma unroll
+                for (int n = 0; n < 3; ++n) {
+                    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                    if (i < kDb) __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);
+                }
+            }
+        }
+        __builtin_amdgcn_s_setprio(0);
+    };
+    const bool late = kStagger && wave >= WAVES / 2;
+    char *v_old = values, *v_cur = values, *v_next = values + Tile::kValueBytes;
+    for (int t = 0; t < tiles + (kStagger ? 1 : 0); ++t) {
+        const char* cur = lds + (t & 1) * Tile::kKeyBytes;
+        char* const next = lds + ((t + 1) & 1) * Tile::kKeyBytes;
+        const int key = k0 + t * kTile;
+        if (kStagger && late && t > 0 && key - kTile < wave_end) weigh(v_old);
+        const bool active = key < wave_end;
+        if (active) {
+            const auto read = [&](int c, u4* k) {
 #pragma unroll
                 for (int n = 0; n < Tile::kPlanes; ++n)
                     k[n] = *reinterpret_cast<const u4*>(cur + n * Tile::kKeyPlane + li * Tile::kKeyRow + 32 * c + 16 * hf);
-                s = mfma_planes<Tile::kPlanes>(k, q[c], s);
+            };
+            s = f16v{};
+            __builtin_amdgcn_s_setprio(1);
+            u4 k[2][Tile::kPlanes];
+            read(0, k[0]);
+#pragma unroll
+            for (int c = 0; c < kC; ++c) {
+                if (c + 1 < kC) read(c + 1, k[(c + 1) % 2]);
+                s = mfma_planes<Tile::kPlanes>(k[c % 2], q[c], s);
             }
-            // Past the last tile the stash rewrites a buffer that is not read again.
-            stash(next);
+            if constexpr (Tile::kPlanes == 1) {
+                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+#pragma unroll
+                for (int c = 0; c < kC; ++c) {
+                    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x008, 3, 0);
+                }
+            }
             __builtin_amdgcn_s_setprio(0);
-            load(t + 2, g2);
+        }
+        if (t < tiles) {  // past the last tile the stash rewrites buffers that are not read again
+            stash(next, v_next);
+            load(g2);
+        }
+        if (active) {
             if constexpr (DT == MIMIR_KV_I8) {
 #pragma unroll
                 for (int r = 0; r < 16; r += 4) {
@@ -226,11 +302,11 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void paged_block(PagedArgs p, Pag
                     for (int e = 0; e < 4; ++e) s[r + e] *= x[e];
                 }
             }
-            if (g0.page[0] < 0 || g0.page[1] < 0 || __any(key + kTile > my_end)) {
+            if (!there(g0, 0) || !there(g0, 1) || __any(key + kTile > my_end)) {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
                     const int j = key + 8 * (r / 4) + 4 * hf + r % 4;
-                    s[r] = j < my_end && g0.page[r / 8] >= 0 ? s[r] : -INFINITY;
+                    s[r] = j < my_end && there(g0, r / 8) ? s[r] : -INFINITY;
                 }
             }
             float top = s[0];
@@ -259,34 +335,15 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void paged_block(PagedArgs p, Pag
                     for (int e = 0; e < 4; ++e) s[r + e] *= x[e];
                 }
             }
-            __builtin_amdgcn_s_setprio(1);
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                float x[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) x[e] = s[8 * c + e];
-                const Split8 pw = split8(x);
-#pragma unroll
-                for (int d = 0; d < kDb; ++d) {
-                    u4 v[Tile::kPlanes];
-#pragma unroll
-                    for (int n = 0; n < Tile::kPlanes; ++n) {
-                        const char* at = cur + Tile::kValuesAt + n * Tile::kValuePlane + v_lane + 16 * c * Tile::kValueRow + 64 * d;
-                        const u2 x0 = __builtin_bit_cast(u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)at));
-                        const u2 x1 = __builtin_bit_cast(u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(at + 8 * Tile::kValueRow)));
-                        v[n] = u4{x0[0], x0[1], x1[0], x1[1]};
-                    }
-                    o[d] = mfma_planes<Tile::kPlanes>(v, pw, o[d]);
-                }
-            }
-            __builtin_amdgcn_s_setprio(0);
-        } else {
-            stash(next);
-            load(t + 2, g2);
+            if (!late) weigh(v_cur);
         }
         g0 = g1;
         g1 = g2;
         g2 = find(t + 3);
+        char* const v_free = kStagger ? v_old : v_cur;
+        v_old = v_cur;
+        v_cur = v_next;
+        v_next = kStagger && t == 0 ? values + 2 * Tile::kValueBytes : v_free;
         __syncthreads();
     }
 
@@ -296,7 +353,7 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void paged_block(PagedArgs p, Pag
     const int row = my_row - w.row0, d_all = p.c.head_dim;
     float* const out = out_row(row);
     const float inv = w.whole ? 1.0f / (l_tot + 1e-9f) : 1.0f;
-    const bool vec = w.whole && d_all % 4 == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15) == 0 && p.ld_out % 4 == 0;
+    const bool vec = d_all % 4 == 0 && (!w.whole || ((reinterpret_cast<uintptr_t>(p.out) & 15) == 0 && p.ld_out % 4 == 0));
     float check = l_tot - l_tot;
 #pragma unroll
     for (int d = 0; d < kDb; ++d)
@@ -315,10 +372,7 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void paged_block(PagedArgs p, Pag
                     if (d0 + e < d_all) out[d0 + e] = x[e];
             }
         }
-    if (!w.whole && in && hf == 0) {
-        out[-2] = m_run;
-        out[-1] = l_tot;
-    }
+    if (!w.whole && in && hf == 0) *part.stat(row) = f2{m_run, l_tot};
     // Rows that came out NaN or infinite, again in fp32 (as paged_stream).
     const uint64_t ballot = __ballot(check != check && in);
     for (uint32_t bad = static_cast<uint32_t>(ballot | ballot >> 32); bad; bad &= bad - 1) {
@@ -330,10 +384,7 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void paged_block(PagedArgs p, Pag
 #pragma unroll
         for (int c = 0; c < kRowChunks; ++c)
             if (lane + c * kWave < d_all) to[lane + c * kWave] = acc[c] * f;
-        if (!w.whole && lane == 0) {
-            to[-2] = m;
-            to[-1] = l;
-        }
+        if (!w.whole && lane == 0) *part.stat(r) = f2{m, l};
     }
     }
 }

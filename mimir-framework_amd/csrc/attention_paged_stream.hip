@@ -101,10 +101,6 @@ struct Values {
             w[key][0] = __builtin_amdgcn_raw_buffer_load_b32(rows, off, row, kNt);
         }
     }
-    __device__ __forceinline__ void clear(int key) {
-#pragma unroll
-        for (int i = 0; i < kWords; ++i) w[key][i] = 0;
-    }
     __device__ __forceinline__ auto operand(int t) const {
         if constexpr (DT == MIMIR_KV_F32) {
             float x[8];
@@ -190,8 +186,9 @@ __global__ __launch_bounds__(kStreamWaves * kWave, stream_waves(DT, DP)) void pa
         return st;
     };
     const int row_bytes = p.c.stride * K::kBytes;
-    const auto half_rows = [&](const char* base, int64_t at) {
-        return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base) + at * row_bytes, 0, kHalf * row_bytes, kBufferWord3);
+    // A half's rows; `keys` of them are there, the others read as zeros.
+    const auto half_rows = [&](char* base, int64_t at, int keys) {
+        return __builtin_amdgcn_make_buffer_rsrc(base + at * row_bytes, 0, keys * row_bytes, kBufferWord3);
     };
     uint32_t k_off[K::kVecs];
 #pragma unroll
@@ -206,20 +203,21 @@ __global__ __launch_bounds__(kStreamWaves * kWave, stream_waves(DT, DP)) void pa
 #pragma unroll
         for (int u = 0; u < H; ++u) {
             const int64_t at = st.at(u, p.c, w.head);
-            const __amdgpu_buffer_rsrc_t rows = half_rows(p.c.k, at);
+            const __amdgpu_buffer_rsrc_t rows = half_rows(p.c.k, at, kHalf);
 #pragma unroll
             for (int v = 0; v < K::kVecs; ++v) kr[u][v] = __builtin_amdgcn_raw_buffer_load_b128(rows, k_off[v], 0, kNt);
             if constexpr (DT == MIMIR_KV_I8) ks[u] = *reinterpret_cast<const f4*>(p.c.k_scale + at + 4 * hg);
         }
     };
-    const auto load_v = [&](const Step& st) {
+    const auto load_v = [&](const Step& st, int key_of) {
 #pragma unroll
         for (int u = 0; u < H; ++u) {
             const int64_t at = st.at(u, p.c, w.head);
-            const __amdgpu_buffer_rsrc_t rows = half_rows(p.c.v, at);
+            const int keys = st.has(u, p.c) ? min(k1 - (key_of + kHalf * u), kHalf) : 0;
+            const __amdgpu_buffer_rsrc_t rows = half_rows(p.c.v, at, keys);
 #pragma unroll
             for (int e = 0; e < 4; ++e) vr[u / 2].load(4 * (u % 2) + e, rows, v_off, e * row_bytes);
-            if constexpr (DT == MIMIR_KV_I8) vs[u] = *reinterpret_cast<const f4*>(p.c.v_scale + at + 4 * hg);
+            if constexpr (DT == MIMIR_KV_I8) vs[u] = buffer_f4(buffer_of(p.c.v_scale + at, 4 * keys), static_cast<uint32_t>(16 * hg));
         }
     };
 
@@ -234,7 +232,7 @@ __global__ __launch_bounds__(kStreamWaves * kWave, stream_waves(DT, DP)) void pa
     if (key < k1) {
         st = find(key);
         load_k(st);
-        load_v(st);
+        load_v(st, key);
         nx = find(key + kStep);
     }
     __syncthreads();  // the last block's sums and flags are read
@@ -283,8 +281,7 @@ __global__ __launch_bounds__(kStreamWaves * kWave, stream_waves(DT, DP)) void pa
 #pragma unroll
         for (int e = 0; e < 4 * H; ++e) x[e] = s[e / 4][e % 4];
         // Rows whose keys end inside the step, and halves that are not there: the
-        // weights are 0 and, where no row of the tile sees a key, so are its values
-        // (what is stored there may be anything).
+        // weights are 0 (and values of keys that no row sees were read as zeros).
         bool edge = __any(key + kKeys > my_end);
 #pragma unroll
         for (int u = 0; u < H; ++u) edge = edge || !st.has(u, p.c);
@@ -293,10 +290,6 @@ __global__ __launch_bounds__(kStreamWaves * kWave, stream_waves(DT, DP)) void pa
             for (int e = 0; e < 4 * H; ++e) {
                 const int u = e / 4, j = key + kHalf * u + 4 * hg + e % 4;
                 x[e] = st.has(u, p.c) && j < my_end ? x[e] : -INFINITY;
-                if (!st.has(u, p.c) || j >= k1) {
-                    vr[u / 2].clear(e % 8);
-                    if constexpr (DT == MIMIR_KV_I8) vs[u][e % 4] = 0.f;
-                }
             }
         }
         float top = x[0];
@@ -328,7 +321,7 @@ __global__ __launch_bounds__(kStreamWaves * kWave, stream_waves(DT, DP)) void pa
                     if (t % 2 == 1) __builtin_amdgcn_sched_barrier(0);
             }
         }
-        if constexpr (decltype(more)::value) load_v(nx);
+        if constexpr (decltype(more)::value) load_v(nx, key + kStep);
     };
     for (; key + kStep < k1; key += kStep) {
         step(std::true_type{});
@@ -351,7 +344,7 @@ __global__ __launch_bounds__(kStreamWaves * kWave, stream_waves(DT, DP)) void pa
     }
     __syncthreads();
     const auto out_row = [&](int row) { return p.out + paged_row(p, p.ld_out, w.seq.first, w.head, w.row0 + row); };
-    const auto part_row = [&](int row) { return paged_part(a, p.c.head_dim, walk.index, w.begins, row); };
+    const PagedPart part(a, p.c.head_dim, walk.index, w.begins);
     for (int x = tid; x < w.rows * p.c.head_dim; x += kStreamWaves * kWave) {
         const int row = x / p.c.head_dim, d = x % p.c.head_dim;
         float m = share[0][row][DP];
@@ -368,12 +361,8 @@ __global__ __launch_bounds__(kStreamWaves * kWave, stream_waves(DT, DP)) void pa
         if (w.whole) {
             out_row(row)[d] = sum * (1.0f / (l + 1e-9f));
         } else {
-            float* part = part_row(row);
-            part[2 + d] = sum;
-            if (d == 0) {
-                part[0] = m;
-                part[1] = l;
-            }
+            part.sums(row)[d] = sum;
+            if (d == 0) *part.stat(row) = f2{m, l};
         }
     }
     __syncthreads();
@@ -385,16 +374,13 @@ __global__ __launch_bounds__(kStreamWaves * kWave, stream_waves(DT, DP)) void pa
         float acc[kRowChunks], m, l;
         row_over_keys<DT>(p, w.s, w.head, q_row(w.row0 + row), k0, min(k1, row_end(p, w.seq, w.row0 + row)), acc, &m, &l);
         const float inv = w.whole ? 1.0f / (l + 1e-9f) : 1.0f;
-        float* out = w.whole ? out_row(row) : part_row(row) + 2;
+        float* out = w.whole ? out_row(row) : part.sums(row);
 #pragma unroll
         for (int c = 0; c < kRowChunks; ++c) {
             const int d = lane + c * kWave;
             if (d < p.c.head_dim) out[d] = acc[c] * inv;
         }
-        if (!w.whole && lane == 0) {
-            out[-2] = m;
-            out[-1] = l;
-        }
+        if (!w.whole && lane == 0) *part.stat(row) = f2{m, l};
     }
     }
 }

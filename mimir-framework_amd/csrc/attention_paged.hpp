@@ -54,6 +54,7 @@ struct PagedRuns {
     int32_t block_rows;
     int32_t part_rows;   // rows of a block that `part` has room for
     int32_t least_rows, most_rows;  // of a sequence's; those with fewer or more are another kernel's
+    int32_t row_blocks;  // of a sequence with as many rows as the host allows
 };
 
 __device__ __forceinline__ uint32_t lane_of(uint32_t v, int lane) {
@@ -76,10 +77,9 @@ struct PagedCost {
 
 __device__ __forceinline__ PagedCost paged_cost(const PagedArgs& p, const PagedRuns& a, const KvSequence& q) {
     const int64_t rows = static_cast<int64_t>(q.n) * p.group;
-    PagedCost c{1, 0, 0};
+    PagedCost c{1, 0, 0};  // base of a sequence without blocks
     if (rows > 0 && rows >= a.least_rows && rows <= a.most_rows)
         c.blocks = static_cast<uint32_t>((rows + a.block_rows - 1) / a.block_rows);
-    if (!a.part) return c;
     c.base = a.extra + static_cast<uint32_t>(p.causal ? max(q.len - q.n, 0) : q.len);
     c.slope = p.causal ? static_cast<uint32_t>((a.block_rows + p.group - 1) / p.group) : 0;
     return c;
@@ -147,18 +147,39 @@ struct PagedWalk {
 
     __device__ __forceinline__ PagedWalk(const PagedArgs& p, const PagedRuns& a, uint32_t index_, PagedChunk* chunk_)
         : chunk(chunk_), base(0), before(0), index(index_) {
+        if (!a.part) {  // one block, found without the lengths of the others
+            from = 0;
+            end = run = 1;
+            return;
+        }
         uint64_t total = lane_of(paged_chunk(p, a, 0, chunk), kWave - 1);
         for (int b = kWave; b < p.b.sequences; b += kWave) total += lane_of(paged_chunk(p, a, b, nullptr), kWave - 1);
-        run = uniform(a.part ? max((total + a.runs - 1) / a.runs, static_cast<uint64_t>(a.extra + a.grain)) : uint64_t{1});
+        run = uniform(max((total + a.runs - 1) / a.runs, static_cast<uint64_t>(a.extra + a.grain)));
         from = uniform(min(total, run * index));
         end = uniform(min(total, from + run));
         // A run of nothing begins no block; the others say so as they end.
-        if (a.part && from >= end && threadIdx.x == 0) a.shared[index].runs = 0;
+        if (from >= end && threadIdx.x == 0) a.shared[index].runs = 0;
         __syncthreads();
     }
     __device__ __forceinline__ bool more() const { return from < end; }
 
+    // A piece without rows has nothing to do.
     __device__ __forceinline__ PagedPiece next(const PagedArgs& p, const PagedRuns& a) {
+        if (!a.part) {
+            from = end;
+            PagedPiece w;
+            const uint32_t pair = index / static_cast<uint32_t>(a.row_blocks), heads = static_cast<uint32_t>(p.c.kv_heads);
+            w.s = static_cast<int>(pair / heads);
+            w.head = static_cast<int>(pair % heads);
+            w.seq = kv_sequence(p.b, w.s);
+            w.row0 = static_cast<int>(index % static_cast<uint32_t>(a.row_blocks)) * a.block_rows;
+            const int64_t all = static_cast<int64_t>(w.seq.n) * p.group;
+            w.rows = all >= a.least_rows && all <= a.most_rows ? static_cast<int>(min(all - w.row0, static_cast<int64_t>(a.block_rows))) : 0;
+            w.k0 = 0;
+            w.k1 = w.rows > 0 ? row_end(p, w.seq, w.row0 + w.rows - 1) : 0;
+            w.whole = w.begins = true;
+            return w;
+        }
         const int mine = static_cast<int>(threadIdx.x % kWave);
         uint64_t sum;
         for (;;) {
@@ -201,11 +222,11 @@ struct PagedWalk {
         w.k1 = uniform(cut(x1));
         w.begins = x0 == 0;
         w.whole = w.begins && x1 == all;
-        if (a.part && threadIdx.x == 0 && w.begins && !w.whole)
+        if (threadIdx.x == 0 && w.begins && !w.whole)
             a.shared[index] = PagedShared{static_cast<int32_t>((first + all - 1) / run - index) + 1, w.seq.first, w.row0, w.rows, w.head, {}};
         from = uniform(first + x1);
         // None that a later run goes on with.
-        if (a.part && threadIdx.x == 0 && from >= end && (w.whole || !w.begins)) a.shared[index].runs = 0;
+        if (threadIdx.x == 0 && from >= end && (w.whole || !w.begins)) a.shared[index].runs = 0;
         return w;
     }
 };

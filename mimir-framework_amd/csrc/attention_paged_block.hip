@@ -93,6 +93,7 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void paged_block(PagedArgs p, Pag
     asm volatile("" : "+v"(tid));  // what follows from it is computed for each block, not held in registers across them
     const int lane = tid % kWave;
     const PagedPiece w = walk.next(p, a);
+    if (w.rows <= 0) return;
     const int k0 = w.k0, k1 = w.k1;
     const int li = lane % 32, hf = lane / 32;
     const int wave_rows = min(w.rows - wave * kTile, kTile);  // below 1: a wave that only moves tiles
@@ -393,7 +394,8 @@ template <int DT, int DP, int WAVES>
 int launch(mimir_ctx* ctx, const PagedArgs& p, PagedRuns a) {
     a.block_rows = a.part_rows = WAVES * kTile;
     const int64_t rows = static_cast<int64_t>(p.b.max_new) * p.group;
-    const int64_t blocks = static_cast<int64_t>(p.b.sequences) * p.c.kv_heads * ((rows + a.block_rows - 1) / a.block_rows);
+    a.row_blocks = static_cast<int32_t>((rows + a.block_rows - 1) / a.block_rows);
+    const int64_t blocks = static_cast<int64_t>(p.b.sequences) * p.c.kv_heads * a.row_blocks;
     const int64_t runs = ctx->tune.attn_splits > 0 ? ctx->tune.attn_splits : 2048 / WAVES;
     const int64_t grid = paged_runs(ctx, p, &a, runs, blocks, true);
     MIMIR_REQUIRE(ctx, dispatch_fits(grid, WAVES * kWave), "paged attention: grid of %lld workgroups exceeds the limit",

@@ -143,6 +143,7 @@ __global__ __launch_bounds__(kStreamWaves * kWave, stream_waves(DT, DP)) void pa
     asm volatile("" : "+v"(tid));  // what follows from it is computed for each block, not held in registers across them
     const int lane = tid % kWave, li = lane % 16, hg = lane / 16;
     const PagedPiece w = walk.next(p, a);
+    if (w.rows <= 0) return;
     const int k0 = w.k0, k1 = w.k1;
     const int my_row = w.row0 + min(li, w.rows - 1);
     const int my_end = min(row_end(p, w.seq, my_row), k1);
@@ -413,7 +414,8 @@ int mimir::paged_stream_launch(mimir_ctx* ctx, const PagedArgs& p, int dtype, in
     a.most_rows = static_cast<int32_t>(most_rows);
     const int64_t rows = std::min(static_cast<int64_t>(p.b.max_new) * p.group, most_rows);
     a.part_rows = static_cast<int32_t>(std::min<int64_t>(rows, kRows));
-    const int64_t blocks = static_cast<int64_t>(p.b.sequences) * p.c.kv_heads * ((rows + kRows - 1) / kRows);
+    a.row_blocks = static_cast<int32_t>((rows + kRows - 1) / kRows);
+    const int64_t blocks = static_cast<int64_t>(p.b.sequences) * p.c.kv_heads * a.row_blocks;
     const int64_t runs = ctx->tune.decode_splits > 0 ? ctx->tune.decode_splits : stream_resident(dtype, p.c.stride);
     // Blocks of up to two steps are not worth a join.
     const int64_t grid = paged_runs(ctx, p, &a, runs, blocks, p.b.max_len > static_cast<int64_t>(2 * kStep));

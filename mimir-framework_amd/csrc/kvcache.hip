@@ -78,125 +78,122 @@ __device__ __forceinline__ void put(char* row, int at, const float* x) {
 }
 
 // W: elements per vector, 4 where every row of q, k, v and q_out is whole 16-byte
-// vectors; UN units of 2 W elements per lane; T tokens, the same row of each.
-template <int DT, int LPR, int W, int T>
+// vectors; UN units of 2 W elements per lane.  A workgroup has rows of one token:
+// several tokens each kept fewer loads in flight (prompts of 9270 tokens x 48 heads of
+// 128, 8-bit: 91 us written and read back, with two 94, four 101, eight 123).
+template <int DT, int LPR, int W, bool KEEP>
 __global__ __launch_bounds__(kBlock) void kv_append(AppendArgs a) {
     constexpr int UN = 4 / W;  // 8 elements a lane
-    constexpr int kGroups = kBlock / LPR;
-    const uint32_t t0 = blockIdx.x / a.parts * T, part = blockIdx.x % a.parts;
+    const uint32_t t = blockIdx.x / a.parts, part = blockIdx.x % a.parts;
     const int lane = threadIdx.x % LPR, group = threadIdx.x / LPR;
-    const int d = a.c.head_dim, row = static_cast<int>(part) * kGroups + group;
+    const int d = a.c.head_dim, row = static_cast<int>(part * (blockDim.x / LPR)) + group;
     const bool is_q = row < a.q_heads, is_k = !is_q && row < a.q_heads + a.c.kv_heads;
     const bool mine = row < a.q_heads + 2 * a.c.kv_heads;
     const int head = is_q ? row : row - a.q_heads - (is_k ? 0 : a.c.kv_heads);
     const int half = is_q || is_k ? a.half : 0;  // values are not rotated
     const int64_t ld = is_q ? a.ld_q : a.ld_kv;
-    const float* x = (is_q ? a.q : is_k ? a.k : a.v) + t0 * ld + static_cast<int64_t>(head) * d;
-    float lo[T][UN][W], hi[T][UN][W];
+    const float* x = (is_q ? a.q : is_k ? a.k : a.v) + t * ld + static_cast<int64_t>(head) * d;
+    float lo[UN][W], hi[UN][W];
     UnitPlace at[UN];
 #pragma unroll
     for (int n = 0; n < UN; ++n) {
         at[n] = unit_place<W>(lane + n * LPR, half, a.interleaved, a.c.stride);
 #pragma unroll
-        for (int i = 0; i < T; ++i) {
-#pragma unroll
-            for (int e = 0; e < W; ++e) lo[i][n][e] = hi[i][n][e] = 0.f;
-            if (!mine || static_cast<int64_t>(t0) + i >= a.b.tokens) continue;
+        for (int e = 0; e < W; ++e) lo[n][e] = hi[n][e] = 0.f;
+        if (mine) {
             if constexpr (W == 4) {
                 if (at[n].d0 < d) {
-                    const f4 v = ld4<true>(x + i * ld + at[n].d0);
+                    const f4 v = ld4<true>(x + at[n].d0);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) lo[i][n][e] = v[e];
+                    for (int e = 0; e < 4; ++e) lo[n][e] = v[e];
                 }
                 if (at[n].d1 < d) {
-                    const f4 v = ld4<true>(x + i * ld + at[n].d1);
+                    const f4 v = ld4<true>(x + at[n].d1);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) hi[i][n][e] = v[e];
+                    for (int e = 0; e < 4; ++e) hi[n][e] = v[e];
                 }
             } else {
-                if (at[n].d0 < d) lo[i][n][0] = x[i * ld + at[n].d0];
-                if (at[n].d1 < d) hi[i][n][0] = x[i * ld + at[n].d1];
+                if (at[n].d0 < d) lo[n][0] = x[at[n].d0];
+                if (at[n].d1 < d) hi[n][0] = x[at[n].d1];
             }
         }
     }
 
-    int s[T];
-    KvToken tok[T];
-    kv_sequences_of<T>(a.b, static_cast<int>(t0), s);
+    int s;
+    kv_sequences_of<1>(a.b, static_cast<int>(t), &s);
+    const KvToken tok = kv_token(a.b, a.c, s, static_cast<int>(t));
+    if (!tok.in) return;  // the whole workgroup
 #pragma unroll
-    for (int i = 0; i < T; ++i) tok[i] = kv_token(a.b, a.c, s[i], static_cast<int>(t0) + i);
-    float c[T][UN][W], sn[T][UN][W];
+    for (int n = 0; n < UN; ++n) {
+        if (!at[n].turned || tok.position < 0) continue;
+        float c[W], sn[W];
+        unit_turns<W>(a.cos_tab, a.sin_tab, static_cast<int64_t>(tok.position) * a.half, lane + n * LPR, a.half, a.interleaved,
+                      c, sn);
+        unit_rotate<W>(lo[n], hi[n], c, sn, a.interleaved);
+    }
+    if (is_q) {
+        float* y = a.q_out + t * a.ld_q_out + static_cast<int64_t>(head) * d;
 #pragma unroll
-    for (int i = 0; i < T; ++i)
+        for (int n = 0; n < UN; ++n) {
+            if (tok.position < 0) {
 #pragma unroll
-        for (int n = 0; n < UN; ++n)
-            if (at[n].turned && tok[i].position >= 0)
-                unit_turns<W>(a.cos_tab, a.sin_tab, static_cast<int64_t>(tok[i].position) * a.half, lane + n * LPR, a.half,
-                              a.interleaved, c[i][n], sn[i][n]);
-
-#pragma unroll
-    for (int i = 0; i < T; ++i) {
-        if (!tok[i].in) continue;
-#pragma unroll
-        for (int n = 0; n < UN; ++n)
-            if (at[n].turned && tok[i].position >= 0) unit_rotate<W>(lo[i][n], hi[i][n], c[i][n], sn[i][n], a.interleaved);
-        if (is_q) {
-            char* y = reinterpret_cast<char*>(a.q_out + (t0 + i) * a.ld_q_out + static_cast<int64_t>(head) * d);
-#pragma unroll
-            for (int n = 0; n < UN; ++n) {
-                if (tok[i].position < 0) {
-#pragma unroll
-                    for (int e = 0; e < W; ++e) lo[i][n][e] = hi[i][n][e] = 0.f;
-                }
-                if (at[n].d0 < d) put<MIMIR_KV_F32, W>(y, at[n].d0, lo[i][n]);
-                if (at[n].d1 < d) put<MIMIR_KV_F32, W>(y, at[n].d1, hi[i][n]);
+                for (int e = 0; e < W; ++e) lo[n][e] = hi[n][e] = 0.f;
             }
-            continue;
+            // Written through (85 us for prompts of 9270 tokens, plain stores 91), or kept
+            // (mimir_ctx_set_output_caching).
+            if constexpr (W == 4) {
+                if (at[n].d0 < d) st_out<KEEP, kStoreThrough>(y + at[n].d0, f4{lo[n][0], lo[n][1], lo[n][2], lo[n][3]});
+                if (at[n].d1 < d) st_out<KEEP, kStoreThrough>(y + at[n].d1, f4{hi[n][0], hi[n][1], hi[n][2], hi[n][3]});
+            } else {
+                if (at[n].d0 < d) y[at[n].d0] = lo[n][0];
+                if (at[n].d1 < d) y[at[n].d1] = hi[n][0];
+            }
         }
-        const bool held = mine && tok[i].page >= 0;
-        const int64_t slot = held ? (static_cast<int64_t>(tok[i].page) * a.c.kv_heads + head) * a.c.page_size + tok[i].slot : 0;
-        if constexpr (DT == MIMIR_KV_I8) {
-            uint32_t bits = 0;  // all lanes of the group come here together
+        return;
+    }
+    const bool held = mine && tok.page >= 0;
+    const int64_t slot = held ? (static_cast<int64_t>(tok.page) * a.c.kv_heads + head) * a.c.page_size + tok.slot : 0;
+    if constexpr (DT == MIMIR_KV_I8) {
+        uint32_t bits = 0;  // all lanes of the group come here together
 #pragma unroll
-            for (int n = 0; n < UN; ++n)
+        for (int n = 0; n < UN; ++n)
+#pragma unroll
+            for (int e = 0; e < W; ++e) {
+                bits = max(bits, __builtin_bit_cast(uint32_t, lo[n][e]) & 0x7fffffffu);
+                bits = max(bits, __builtin_bit_cast(uint32_t, hi[n][e]) & 0x7fffffffu);
+            }
+        bits = lanes_max<LPR>(bits);
+        if (!held) return;
+        const bool finite = bits < 0x7f800000u;
+        const float most = __builtin_bit_cast(float, bits), inv = 127.f / most;
+        char* out = (is_k ? a.c.k : a.c.v) + slot * a.c.stride;
+        if (lane == 0) (is_k ? a.c.k_scale : a.c.v_scale)[slot] = finite ? most / 127.f : __builtin_nanf("");
+        const bool codes = finite && bits > 0;
+#pragma unroll
+        for (int n = 0; n < UN; ++n) {
+            uint32_t l = 0, h = 0;
+            if (codes) {
 #pragma unroll
                 for (int e = 0; e < W; ++e) {
-                    bits = max(bits, __builtin_bit_cast(uint32_t, lo[i][n][e]) & 0x7fffffffu);
-                    bits = max(bits, __builtin_bit_cast(uint32_t, hi[i][n][e]) & 0x7fffffffu);
-                }
-            bits = lanes_max<LPR>(bits);
-            if (!held) continue;
-            const bool finite = bits < 0x7f800000u;
-            const float most = __builtin_bit_cast(float, bits), inv = 127.f / most;
-            char* out = (is_k ? a.c.k : a.c.v) + slot * a.c.stride;
-            if (lane == 0) (is_k ? a.c.k_scale : a.c.v_scale)[slot] = finite ? most / 127.f : __builtin_nanf("");
-            const bool codes = finite && bits > 0;
-#pragma unroll
-            for (int n = 0; n < UN; ++n) {
-                uint32_t l = 0, h = 0;
-                if (codes) {
-#pragma unroll
-                    for (int e = 0; e < W; ++e) {
-                        l |= static_cast<uint32_t>(code_of(lo[i][n][e], most, inv) & 0xff) << (8 * e);
-                        h |= static_cast<uint32_t>(code_of(hi[i][n][e], most, inv) & 0xff) << (8 * e);
-                    }
-                }
-                if constexpr (W == 4) {
-                    if (at[n].d0 < a.c.stride) *reinterpret_cast<uint32_t*>(out + at[n].d0) = l;
-                    if (at[n].d1 < a.c.stride) *reinterpret_cast<uint32_t*>(out + at[n].d1) = h;
-                } else {
-                    if (at[n].d0 < a.c.stride) out[at[n].d0] = static_cast<char>(l);
-                    if (at[n].d1 < a.c.stride) out[at[n].d1] = static_cast<char>(h);
+                    l |= static_cast<uint32_t>(code_of(lo[n][e], most, inv) & 0xff) << (8 * e);
+                    h |= static_cast<uint32_t>(code_of(hi[n][e], most, inv) & 0xff) << (8 * e);
                 }
             }
-        } else {
-            if (!held) continue;
-            char* out = (is_k ? a.c.k : a.c.v) + slot * a.c.stride * (DT == MIMIR_KV_F32 ? 4 : 2);
-#pragma unroll
-            for (int n = 0; n < UN; ++n) {
-                if (at[n].d0 < a.c.stride) put<DT, W>(out, at[n].d0, lo[i][n]);
-                if (at[n].d1 < a.c.stride) put<DT, W>(out, at[n].d1, hi[i][n]);
+            if constexpr (W == 4) {
+                if (at[n].d0 < a.c.stride) *reinterpret_cast<uint32_t*>(out + at[n].d0) = l;
+                if (at[n].d1 < a.c.stride) *reinterpret_cast<uint32_t*>(out + at[n].d1) = h;
+            } else {
+                if (at[n].d0 < a.c.stride) out[at[n].d0] = static_cast<char>(l);
+                if (at[n].d1 < a.c.stride) out[at[n].d1] = static_cast<char>(h);
             }
+        }
+    } else {
+        if (!held) return;
+        char* out = (is_k ? a.c.k : a.c.v) + slot * a.c.stride * (DT == MIMIR_KV_F32 ? 4 : 2);
+#pragma unroll
+        for (int n = 0; n < UN; ++n) {
+            if (at[n].d0 < a.c.stride) put<DT, W>(out, at[n].d0, lo[n]);
+            if (at[n].d1 < a.c.stride) put<DT, W>(out, at[n].d1, hi[n]);
         }
     }
 }
@@ -397,17 +394,19 @@ int mimir_kv_append(mimir_ctx* ctx, const mimir_kv_cache* cache, const mimir_kv_
     return with_type(cache->dtype, [&](auto dt) {
         return with_lanes(a.c.stride, [&](auto lpr) {
             constexpr int LPR = decltype(lpr)::value, DT = decltype(dt)::value;
+            // Half the threads where they leave fewer without a row.
             constexpr int64_t kGroups = kBlock / LPR;
-            a.parts = static_cast<uint32_t>((rows + kGroups - 1) / kGroups);
-            const bool many = several_tokens(batch->tokens, a.parts);
-            const int64_t blocks = (many ? (batch->tokens + kTokens - 1) / kTokens : batch->tokens) * a.parts;
-            MIMIR_REQUIRE(ctx, dispatch_fits(blocks, kBlock), "%s: grid of %lld workgroups exceeds the limit", what,
+            const auto parts_of = [&](int64_t groups) { return (rows + groups - 1) / groups; };
+            const bool small = parts_of(kGroups / 2) < 2 * parts_of(kGroups);
+            a.parts = static_cast<uint32_t>(parts_of(small ? kGroups / 2 : kGroups));
+            const int threads = small ? kBlock / 2 : kBlock;
+            const int64_t blocks = batch->tokens * a.parts;
+            MIMIR_REQUIRE(ctx, dispatch_fits(blocks, threads), "%s: grid of %lld workgroups exceeds the limit", what,
                           (long long)blocks);
             const auto grid = static_cast<unsigned>(blocks);
-            if (vec && many) kv_append<DT, LPR, 4, kTokens><<<grid, kBlock, 0, ctx->stream>>>(a);
-            else if (vec) kv_append<DT, LPR, 4, 1><<<grid, kBlock, 0, ctx->stream>>>(a);
-            else if (many) kv_append<DT, LPR, 1, kTokens><<<grid, kBlock, 0, ctx->stream>>>(a);
-            else kv_append<DT, LPR, 1, 1><<<grid, kBlock, 0, ctx->stream>>>(a);
+            if (vec && ctx->keep_outputs) kv_append<DT, LPR, 4, true><<<grid, threads, 0, ctx->stream>>>(a);
+            else if (vec) kv_append<DT, LPR, 4, false><<<grid, threads, 0, ctx->stream>>>(a);
+            else kv_append<DT, LPR, 1, true><<<grid, threads, 0, ctx->stream>>>(a);
             return launched(ctx, "kv_append");
         });
     });

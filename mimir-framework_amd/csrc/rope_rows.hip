@@ -8,8 +8,7 @@
 // Bound by HBM: every element is read once and written once; the positions and
 // their table rows are shared by the heads of a token and stay in L2.  A "slot" is
 // two vectors of one head row (kvcache.hpp unit_place): four pairs, or eight
-// dimensions that are copied.  Each thread handles kSlots of them a workgroup
-// apart, all loads ahead of the first store.  The
+// dimensions that are copied.  The
 // products are taken in double (kvcache.hpp rotate_pair): 8 operations on pairs
 // that cost 32 bytes of HBM, a tenth of the time those take.
 #include "common.hpp"
@@ -48,7 +47,7 @@ struct Half {
     __device__ __forceinline__ void load(const float* p, bool in) {
         if (!in) return;
         if constexpr (W == 4) {
-            const f4 v = ld4<true>(p);
+            const f4 v = *reinterpret_cast<const f4*>(p);
 #pragma unroll
             for (int e = 0; e < 4; ++e) x[e] = v[e];
         } else {
@@ -71,62 +70,49 @@ struct Half {
     }
 };
 
-constexpr int kSlots = 4;
-
-// W: elements per half of a slot, 4 where every row is whole 16-byte vectors.
+// W: elements per half of a slot, 4 where every row is whole 16-byte vectors.  A
+// thread has one slot: 8192 tokens x 40 heads of 128 take 58 us = 5.8 TB/s (a copy of
+// as many bytes 53), with two slots a thread 61, four 61, eight 89.  The loads leave
+// their lines in the caches, where the projection before may have put them (4099
+// tokens x 32 heads: 22 us, non-temporal 26; the larger case 58 and 57).
 template <int W, bool KEEP, bool ACC>
 __global__ __launch_bounds__(kBlock) void rope_rows(RowsArgs a) {
-    Half<W> lo[kSlots], hi[kSlots];
-    float *out_lo[kSlots], *out_hi[kSlots], c[kSlots][W], s[kSlots][W];
-    int turn[kSlots];  // 0 no slot, 1 copied, 2 rotated, 3 zeros
+    const uint32_t slot = blockIdx.x * kBlock + threadIdx.x;
+    if (slot >= a.slots) return;
+    const bool is_q = slot < a.q_slots;
+    const uint32_t local = is_q ? slot : slot - a.q_slots;
+    const uint32_t row = fastdiv(local, a.unit_div);
+    const int unit = static_cast<int>(local - row * a.unit_div.d);
+    const FastDiv& heads = is_q ? a.q_div : a.k_div;
+    const uint32_t t = fastdiv(row, heads);
+    const int64_t col = static_cast<int64_t>(row - t * heads.d) * a.head_dim;
+    const auto [d0, d1, pairs] = unit_place<W>(unit, a.half, a.interleaved, a.head_dim);
+    const float* x = (is_q ? a.q + t * a.ld_q : a.k + t * a.ld_k) + col;
+    float* y = (is_q ? a.q_out + t * a.ld_q_out : a.k_out + t * a.ld_k_out) + col;
+    const bool two = d1 < a.head_dim;
+    Half<W> lo, hi;
+    lo.load(x + d0, true);
+    hi.load(x + d1, two);
+    const int64_t p = a.positions[t];
+    if (p < 0 || p >= a.table_rows) {
+        if constexpr (ACC) return;
 #pragma unroll
-    for (int j = 0; j < kSlots; ++j) {
-        const int64_t at = static_cast<int64_t>(blockIdx.x) * kSlots * kBlock + j * kBlock + threadIdx.x;
-        turn[j] = 0;
-        out_lo[j] = out_hi[j] = nullptr;
-        if (at >= a.slots) continue;
-        const uint32_t slot = static_cast<uint32_t>(at);
-        const bool is_q = slot < a.q_slots;
-        const uint32_t local = is_q ? slot : slot - a.q_slots;
-        const uint32_t row = fastdiv(local, a.unit_div);
-        const int unit = static_cast<int>(local - row * a.unit_div.d);
-        const FastDiv& heads = is_q ? a.q_div : a.k_div;
-        const uint32_t t = fastdiv(row, heads);
-        const int64_t col = static_cast<int64_t>(row - t * heads.d) * a.head_dim;
-        const auto [d0, d1, pairs] = unit_place<W>(unit, a.half, a.interleaved, a.head_dim);
-        const float* x = (is_q ? a.q + t * a.ld_q : a.k + t * a.ld_k) + col;
-        float* y = (is_q ? a.q_out + t * a.ld_q_out : a.k_out + t * a.ld_k_out) + col;
-        lo[j].load(x + d0, true);
-        hi[j].load(x + d1, d1 < a.head_dim);
-        out_lo[j] = y + d0;
-        if (d1 < a.head_dim) out_hi[j] = y + d1;
-        const int64_t p = a.positions[t];
-        turn[j] = p < 0 || p >= a.table_rows ? 3 : pairs ? 2 : 1;
-        if (turn[j] == 2) {
-            unit_turns<W>(a.cos_tab, a.sin_tab, p * a.half, unit, a.half, a.interleaved, c[j], s[j]);
+        for (int e = 0; e < W; ++e) lo.x[e] = hi.x[e] = 0.f;
+    } else if (pairs) {
+        float c[W], s[W];
+        unit_turns<W>(a.cos_tab, a.sin_tab, p * a.half, unit, a.half, a.interleaved, c, s);
 #pragma unroll
-            for (int e = 0; e < W; ++e) s[j][e] *= a.sign;
-        }
+        for (int e = 0; e < W; ++e) s[e] *= a.sign;
+        unit_rotate<W>(lo.x, hi.x, c, s, a.interleaved);
     }
-#pragma unroll
-    for (int j = 0; j < kSlots; ++j) {
-        if (!turn[j]) continue;
-        if (turn[j] == 3) {
-            if constexpr (ACC) continue;
-#pragma unroll
-            for (int e = 0; e < W; ++e) lo[j].x[e] = hi[j].x[e] = 0.f;
-        } else if (turn[j] == 2) {
-            unit_rotate<W>(lo[j].x, hi[j].x, c[j], s[j], a.interleaved);
-        }
-        lo[j].template store<KEEP, ACC>(out_lo[j], true);
-        hi[j].template store<KEEP, ACC>(out_hi[j], out_hi[j] != nullptr);
-    }
+    lo.template store<KEEP, ACC>(y + d0, true);
+    hi.template store<KEEP, ACC>(y + d1, two);
 }
 
 template <int W, bool ACC>
 int launch(mimir_ctx* ctx, const RowsArgs& a) {
     unsigned blocks;
-    if (!grid_for(a.slots, kSlots * kBlock, kBlock, &blocks)) return fail(ctx, MIMIR_EINVAL, "RoPE: grid exceeds the limit");
+    if (!grid_for(a.slots, kBlock, kBlock, &blocks)) return fail(ctx, MIMIR_EINVAL, "RoPE: grid exceeds the limit");
     if (ctx->keep_outputs) rope_rows<W, true, ACC><<<blocks, kBlock, 0, ctx->stream>>>(a);
     else rope_rows<W, false, ACC><<<blocks, kBlock, 0, ctx->stream>>>(a);
     return launched(ctx, "rope_rows");

@@ -15,88 +15,106 @@ using namespace mimir;
 
 namespace {
 
-constexpr int64_t kStreamRows = 32;
+// Query rows of a key / value head that the stream kernel takes, of all sequences or of
+// those beside longer ones.  Where the block kernel would take as long (40 to 64 rows,
+// stream / block, us): 32 sequences x 3000 keys x 4 heads of 128, bf16 90-98 / 86-88,
+// 8-bit 76-82 / 92-93, fp32 162-167 / 181-185; one of 30000 x 8 heads, 64 rows, bf16
+// 62 / 86, 8-bit 58 / 88, fp32 111 / 141.  Beside longer ones it has 16 rows a block.
+constexpr int64_t kStreamRows = 64, kStreamBeside = 32;
 
-// The shares of one row: brought to one max, added up and divided.  LPR lanes hold a
-// row, four dimensions each.  ONE: the whole workgroup takes one row, its groups of
-// lanes every so many of the runs (a long sequence's row may have dozens); else each
-// group a row of its own.  The block's first run, whose descriptor this is, kept what
-// it begins, the others what they go on with.
+// The shares of a block's rows: each brought to one max, added up and divided.  LPR
+// lanes hold a row, four dimensions each.  ONE: the whole workgroup takes a row at a
+// time, its groups of lanes every so many of the runs (a long sequence's block may have
+// hundreds); else each group a row of its own.  The block's first run, whose descriptor
+// this is, kept what it begins, the others what they go on with.  `parts` workgroups
+// for each descriptor.
 template <int LPR, bool ONE>
-__global__ __launch_bounds__(kBlock) void paged_join(PagedArgs p, PagedRuns a) {
+__global__ __launch_bounds__(kBlock) void paged_join(PagedArgs p, PagedRuns a, uint32_t parts) {
     constexpr int kAhead = 4, kGroups = kBlock / LPR, kEach = ONE ? kGroups : 1, kRowsOf = ONE ? 1 : kGroups;
     __shared__ f4 share[kGroups][LPR];
     __shared__ f2 stats[kGroups];
-    const uint32_t parts = static_cast<uint32_t>((a.part_rows + kRowsOf - 1) / kRowsOf);
     const uint32_t first = blockIdx.x / parts;
     const PagedShared s = a.shared[first];
     if (s.runs <= 1) return;
     const int lane = threadIdx.x % LPR, group = threadIdx.x / LPR, d = p.c.head_dim;
-    const int row = static_cast<int>(blockIdx.x % parts) * kRowsOf + (ONE ? 0 : group);
-    if (ONE && row >= s.rows) return;  // the whole workgroup
-    const bool mine = row < s.rows;
-    float m = -1e30f, l = 0.f;
-    f4 acc{0.f, 0.f, 0.f, 0.f};
-    for (int i = ONE ? group : 0; mine && i < s.runs; i += kAhead * kEach) {
-        f2 st[kAhead];
-        f4 x[kAhead];
+    for (int row0 = static_cast<int>(blockIdx.x % parts) * kRowsOf; row0 < s.rows; row0 += static_cast<int>(parts) * kRowsOf) {
+        const int row = row0 + (ONE ? 0 : group);
+        const bool mine = row < s.rows;
+        float m = -1e30f, l = 0.f;
+        f4 acc{0.f, 0.f, 0.f, 0.f};
+        for (int i = ONE ? group : 0; mine && i < s.runs; i += kAhead * kEach) {
+            f2 st[kAhead];
+            f4 x[kAhead];
 #pragma unroll
-        for (int u = 0; u < kAhead; ++u) {
-            const int j = i + u * kEach;
-            st[u] = f2{-1e30f, 0.f};
-            x[u] = f4{0.f, 0.f, 0.f, 0.f};
-            if (j >= s.runs) continue;
-            const PagedPart part(a, d, first + static_cast<uint32_t>(j), j == 0);
-            st[u] = *part.stat(row);
-            if (4 * lane < d) x[u] = *reinterpret_cast<const f4*>(part.sums(row) + 4 * lane);
-        }
-        float m_new = m;
+            for (int u = 0; u < kAhead; ++u) {
+                const int j = i + u * kEach;
+                st[u] = f2{-1e30f, 0.f};
+                x[u] = f4{0.f, 0.f, 0.f, 0.f};
+                if (j >= s.runs) continue;
+                const PagedPart part(a, d, first + static_cast<uint32_t>(j), j == 0);
+                st[u] = *part.stat(row);
+                if (4 * lane < d) x[u] = *reinterpret_cast<const f4*>(part.sums(row) + 4 * lane);
+            }
+            float m_new = m;
 #pragma unroll
-        for (int u = 0; u < kAhead; ++u) m_new = fmaxf(m_new, st[u][0]);
-        const float f = __builtin_amdgcn_exp2f(m - m_new);
-        m = m_new;
-        l *= f;
-        acc *= f;
-#pragma unroll
-        for (int u = 0; u < kAhead; ++u) {
-            const float g = __builtin_amdgcn_exp2f(st[u][0] - m);
-            l += st[u][1] * g;
-            acc += x[u] * g;
-        }
-    }
-    if constexpr (ONE) {
-        share[group][lane] = acc;
-        if (lane == 0) stats[group] = f2{m, l};
-        __syncthreads();
-        if (group > 0) return;
-#pragma unroll
-        for (int v = 1; v < kGroups; ++v) {
-            const f2 st = stats[v];
-            const float m_new = fmaxf(m, st[0]);
-            const float f = __builtin_amdgcn_exp2f(m - m_new), g = __builtin_amdgcn_exp2f(st[0] - m_new);
+            for (int u = 0; u < kAhead; ++u) m_new = fmaxf(m_new, st[u][0]);
+            const float f = __builtin_amdgcn_exp2f(m - m_new);
             m = m_new;
-            l = l * f + st[1] * g;
-            acc = acc * f + share[v][lane] * g;
-        }
-    }
-    if (!mine) return;
-    const float inv = 1.0f / (l + 1e-9f);
-    float* out = p.out + paged_row(p, p.ld_out, s.first, s.head, s.row0 + row);
+            l *= f;
+            acc *= f;
 #pragma unroll
-    for (int e = 0; e < 4; ++e)  // a row's sums may be followed by what nothing wrote
-        if (4 * lane + e < d) out[4 * lane + e] = acc[e] * inv;
+            for (int u = 0; u < kAhead; ++u) {
+                const float g = __builtin_amdgcn_exp2f(st[u][0] - m);
+                l += st[u][1] * g;
+                acc += x[u] * g;
+            }
+        }
+        if constexpr (ONE) {
+            share[group][lane] = acc;
+            if (lane == 0) stats[group] = f2{m, l};
+            __syncthreads();
+            if (group == 0) {
+#pragma unroll
+                for (int v = 1; v < kGroups; ++v) {
+                    const f2 st = stats[v];
+                    const float m_new = fmaxf(m, st[0]);
+                    const float f = __builtin_amdgcn_exp2f(m - m_new), g = __builtin_amdgcn_exp2f(st[0] - m_new);
+                    m = m_new;
+                    l = l * f + st[1] * g;
+                    acc = acc * f + share[v][lane] * g;
+                }
+            }
+            __syncthreads();  // the next row's shares
+        }
+        if (!mine || (ONE && group > 0)) continue;
+        const float inv = 1.0f / (l + 1e-9f);
+        float* out = p.out + paged_row(p, p.ld_out, s.first, s.head, s.row0 + row);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)  // a row's sums may be followed by what nothing wrote
+            if (4 * lane + e < d) out[4 * lane + e] = acc[e] * inv;
+    }
 }
 
 template <int LPR>
 void launch_join(const PagedArgs& p, const PagedRuns& a, hipStream_t s) {
     constexpr int kRowsOf = kBlock / LPR;
-    if (a.part_rows <= 16) paged_join<LPR, true><<<a.runs * static_cast<unsigned>(a.part_rows), kBlock, 0, s>>>(p, a);
-    else paged_join<LPR, false><<<a.runs * static_cast<unsigned>((a.part_rows + kRowsOf - 1) / kRowsOf), kBlock, 0, s>>>(p, a);
+    if (a.many) {
+        const unsigned parts = static_cast<unsigned>(std::min(a.part_rows, 8));
+        paged_join<LPR, true><<<a.runs * parts, kBlock, 0, s>>>(p, a, parts);
+    } else {
+        const unsigned parts = static_cast<unsigned>((a.part_rows + kRowsOf - 1) / kRowsOf);
+        paged_join<LPR, false><<<a.runs * parts, kBlock, 0, s>>>(p, a, parts);
+    }
 }
 
 }  // namespace
 
 int64_t mimir::paged_runs(mimir_ctx* ctx, const PagedArgs& p, PagedRuns* a, int64_t runs, int64_t blocks, bool split) {
+    // No more than keep to the least length of a run (PagedWalk), by the longest costs.
+    const int64_t cost = a->extra + static_cast<int64_t>(p.b.max_len) + (p.causal ? (a->block_rows + p.group - 1) / p.group : 0);
+    runs = std::max<int64_t>(1, std::min(runs, blocks * cost / (a->extra + a->grain) + 1));
+    a->apart = a->row_blocks == 1 && p.b.sequences <= kWave && 2 * blocks <= runs && p.b.max_len < 1 << 30;
+    a->many = a->part_rows <= 32 && runs > 4 * blocks;
     const int64_t floats = runs * 2 * paged_part_floats(a->part_rows, p.c.head_dim);
     const int64_t bytes = runs * static_cast<int64_t>(sizeof(PagedShared)) + floats * 4;
     char* work = split && bytes <= static_cast<int64_t>(kPagedWorkBytes) ? paged_work(ctx) : nullptr;
@@ -141,15 +159,13 @@ extern "C" int mimir_attention_paged_fwd(mimir_ctx* ctx, const mimir_kv_cache* c
     a.qscale = scale * kPagedLog2e;
     a.causal = causal ? 1 : 0;
     a.group_div = make_fastdiv(static_cast<uint32_t>(a.group));
+    // Sequences with few query rows of a key / value head stream their keys, the others'
+    // keys go through LDS, by a launch each.  A batch whose sequences all have max_new
+    // tokens (or whose rows would suffice for that) has the second alone, which takes any.
     const int64_t rows = static_cast<int64_t>(a.b.max_new) * a.group;
     MIMIR_REQUIRE(ctx, rows <= INT32_MAX, "%s: %lld query rows of a head", what, (long long)rows);
-    // Sequences with up to kStreamRows query rows of a key / value head stream their
-    // keys, the others' keys go through LDS.  A batch whose sequences all have the
-    // same number needs one of the two.
-    const bool even = a.b.sequences * static_cast<int64_t>(a.b.max_new) == a.b.tokens;
-    if (a.c.stride > kPagedBlockStride) return paged_stream_launch(ctx, a, cache->dtype, INT32_MAX);
-    if (rows <= kStreamRows || !even)
-        if (int st = paged_stream_launch(ctx, a, cache->dtype, kStreamRows)) return st;
-    if (rows <= kStreamRows) return MIMIR_OK;
-    return paged_block_launch(ctx, a, cache->dtype, kStreamRows + 1);
+    if (rows <= kStreamRows || a.c.stride > kPagedBlockStride) return paged_stream_launch(ctx, a, cache->dtype, INT32_MAX);
+    if (a.b.sequences * static_cast<int64_t>(a.b.max_new) <= a.b.tokens) return paged_block_launch(ctx, a, cache->dtype, 1);
+    if (int st = paged_stream_launch(ctx, a, cache->dtype, kStreamBeside)) return st;
+    return paged_block_launch(ctx, a, cache->dtype, kStreamBeside + 1);
 }

@@ -50,10 +50,12 @@ struct PagedRuns {
     float* part;
     uint32_t runs;
     uint32_t extra;      // what a block costs besides its keys, in keys
-    uint32_t grain;      // blocks are cut at multiples of this many keys
+    uint32_t grain;      // blocks are cut at multiples of this many keys, a power of two
     int32_t block_rows;
     int32_t part_rows;   // rows of a block that `part` has room for
     int32_t least_rows, most_rows;  // of a sequence's; those with fewer or more are another kernel's
+    int32_t many;        // a block may have many runs (paged_join)
+    int32_t apart;       // no run need have parts of two blocks (PagedWalk)
     int32_t row_blocks;  // of a sequence with as many rows as the host allows
 };
 
@@ -92,25 +94,32 @@ struct PagedChunk {
     PagedCost cost[kWave];
 };
 
-// The costs of the sequences from `base` on up to the lane's; wave 0 writes them down.
-__device__ __forceinline__ uint64_t paged_chunk(const PagedArgs& p, const PagedRuns& a, int base, PagedChunk* chunk) {
+// The lanes' sums up to each.
+__device__ __forceinline__ uint64_t lanes_up_to(uint64_t sum) {
     const int lane = static_cast<int>(threadIdx.x % kWave);
-    KvSequence seq{0, 0, 0};
-    PagedCost cost{1, 0, 0};
-    if (base + lane < p.b.sequences) {
-        seq = kv_sequence(p.b, base + lane);
-        cost = paged_cost(p, a, seq);
-    }
-    uint64_t sum = cost.ahead(cost.blocks) * static_cast<uint32_t>(p.c.kv_heads);
 #pragma unroll
     for (int x = 1; x < kWave; x *= 2) {
         const auto y = static_cast<uint64_t>(__shfl_up(static_cast<unsigned long long>(sum), x));
         if (lane >= x) sum += y;
     }
+    return sum;
+}
+
+// The costs of the sequences from `base` on up to the lane's; wave 0 writes them down.
+// The lane's own is left in `cost`.
+__device__ __forceinline__ uint64_t paged_chunk(const PagedArgs& p, const PagedRuns& a, int base, PagedChunk* chunk, PagedCost* cost) {
+    const int lane = static_cast<int>(threadIdx.x % kWave);
+    KvSequence seq{0, 0, 0};
+    *cost = PagedCost{1, 0, 0};
+    if (base + lane < p.b.sequences) {
+        seq = kv_sequence(p.b, base + lane);
+        *cost = paged_cost(p, a, seq);
+    }
+    const uint64_t sum = lanes_up_to(cost->ahead(cost->blocks) * static_cast<uint32_t>(p.c.kv_heads));
     if (chunk && threadIdx.x < kWave) {
         chunk->sum[lane] = sum;
         chunk->seq[lane] = seq;
-        chunk->cost[lane] = cost;
+        chunk->cost[lane] = *cost;
     }
     return sum;
 }
@@ -137,6 +146,15 @@ __device__ __forceinline__ uint64_t uniform(uint64_t x) {
     return static_cast<uint64_t>(uniform(static_cast<uint32_t>(x >> 32))) << 32 | uniform(static_cast<uint32_t>(x));
 }
 
+// x / y without the long way of a 64-bit division: its rounding is put right by the
+// remainder (a quotient of up to 53 bits is off by 1 at most).
+__device__ __forceinline__ uint64_t quotient(uint64_t x, uint64_t y) {
+    auto q = static_cast<uint64_t>(static_cast<double>(x) / static_cast<double>(y));
+    if (q * y > x) --q;
+    else if (x - q * y >= y) ++q;
+    return q;
+}
+
 // The pieces of one run, in order.  All waves of the workgroup walk together.
 struct PagedWalk {
     PagedChunk* chunk;
@@ -152,14 +170,40 @@ struct PagedWalk {
             end = run = 1;
             return;
         }
-        uint64_t total = lane_of(paged_chunk(p, a, 0, chunk), kWave - 1);
-        for (int b = kWave; b < p.b.sequences; b += kWave) total += lane_of(paged_chunk(p, a, b, nullptr), kWave - 1);
-        run = uniform(max((total + a.runs - 1) / a.runs, static_cast<uint64_t>(a.extra + a.grain)));
+        PagedCost cost, other;
+        uint64_t total = lane_of(paged_chunk(p, a, 0, chunk, &cost), kWave - 1);
+        for (int b = kWave; b < p.b.sequences; b += kWave) total += lane_of(paged_chunk(p, a, b, nullptr, &other), kWave - 1);
+        run = uniform(max(quotient(total + a.runs - 1, a.runs), static_cast<uint64_t>(a.extra + a.grain)));
+        if (a.apart) total = set_apart(p, a, total, cost);
         from = uniform(min(total, run * index));
         end = uniform(min(total, from + run));
         // A run of nothing begins no block; the others say so as they end.
         if (from >= end && threadIdx.x == 0) a.shared[index].runs = 0;
         __syncthreads();
+    }
+    // With fewer blocks than half the runs, a block's cost may be rounded up to whole
+    // runs: a second part costs its run a way in and out.  With these runs if there are
+    // enough, or somewhat longer ones, if that is not longer than such a part.  The total.
+    __device__ __forceinline__ uint64_t set_apart(const PagedArgs& p, const PagedRuns& a, uint64_t total, PagedCost cost) {
+        const int lane = static_cast<int>(threadIdx.x % kWave);
+        const uint64_t each = cost.ahead(1);  // a sequence has one block for each head, or none
+        const uint32_t count = cost.blocks * static_cast<uint32_t>(p.c.kv_heads);
+        const uint32_t left = a.runs - static_cast<uint32_t>(p.b.sequences * p.c.kv_heads);
+        const uint64_t longer = max(uniform(quotient(total + left - 1, left)), run);
+        uint64_t whole = quotient(each + run - 1, run);
+        if (lane_of(lanes_up_to(whole * count), kWave - 1) > a.runs) {
+            if (longer > run + a.extra) return total;
+            run = longer;
+            whole = quotient(each + run - 1, run);
+        }
+        cost.slope = 0;
+        cost.base = static_cast<uint32_t>(whole * run);
+        const uint64_t sum = lanes_up_to(whole * run * count);
+        if (threadIdx.x < kWave) {
+            chunk->sum[lane] = sum;
+            chunk->cost[lane] = cost;
+        }
+        return lane_of(sum, kWave - 1);
     }
     __device__ __forceinline__ bool more() const { return from < end; }
 
@@ -189,7 +233,8 @@ struct PagedWalk {
             __syncthreads();  // all waves have read it
             base += kWave;
             before = uniform(to);
-            paged_chunk(p, a, base, chunk);
+            PagedCost cost;
+            paged_chunk(p, a, base, chunk, &cost);
             __syncthreads();
         }
         const uint64_t above = __ballot(before + sum > from);
@@ -200,7 +245,7 @@ struct PagedWalk {
         const PagedCost cost{uniform(chunk->cost[lane].base), uniform(chunk->cost[lane].slope), uniform(chunk->cost[lane].blocks)};
         const uint64_t head_cost = cost.ahead(cost.blocks);
         uint64_t first = before + lane_of(sum, lane) - head_cost * static_cast<uint32_t>(p.c.kv_heads);
-        w.head = uniform(static_cast<int>((from - first) / head_cost));
+        w.head = uniform(static_cast<int>(quotient(from - first, head_cost)));
         first += head_cost * static_cast<uint32_t>(w.head);
         uint32_t lo = 0, hi = cost.blocks;  // row block lo begins at or before `from`, hi after it
         while (hi - lo > 1) {
@@ -215,15 +260,17 @@ struct PagedWalk {
         const int keys = row_end(p, w.seq, w.row0 + w.rows - 1);
         const uint64_t all = static_cast<uint64_t>(cost.base) + static_cast<uint64_t>(cost.slope) * (lo + 1);
         const uint64_t x0 = from - first, x1 = min(all, end - first);
+        // The same for the run that ends here and the one that begins, and never less for more.
         const auto cut = [&](uint64_t x) {
-            return x >= all ? keys : static_cast<int>(static_cast<uint64_t>(keys) * x / all / a.grain * a.grain);
+            const auto at = static_cast<uint32_t>(keys * (static_cast<double>(x) / static_cast<double>(all)));
+            return x >= all ? keys : min(keys, static_cast<int>((at + a.grain / 2) & -a.grain));
         };
         w.k0 = uniform(cut(x0));
         w.k1 = uniform(cut(x1));
         w.begins = x0 == 0;
         w.whole = w.begins && x1 == all;
         if (threadIdx.x == 0 && w.begins && !w.whole)
-            a.shared[index] = PagedShared{static_cast<int32_t>((first + all - 1) / run - index) + 1, w.seq.first, w.row0, w.rows, w.head, {}};
+            a.shared[index] = PagedShared{static_cast<int32_t>(quotient(first + all - 1, run) - index) + 1, w.seq.first, w.row0, w.rows, w.head, {}};
         from = uniform(first + x1);
         // None that a later run goes on with.
         if (threadIdx.x == 0 && from >= end && (w.whole || !w.begins)) a.shared[index].runs = 0;

@@ -71,17 +71,27 @@ __device__ __forceinline__ f16v mfma_planes(const u4* a, const Split8& b, f16v c
     return mfma_bf16(a[0], b.h, c);
 }
 
+// Value buffers of a workgroup, and workgroups of a CU: one of eight waves, or two of
+// four where the tiles leave room.
 template <int DT, int DP, int WAVES>
-__global__ __launch_bounds__(WAVES * kWave, 2) void paged_block(PagedArgs p, PagedRuns a) {
+struct BlockShape {
     using Tile = BlockTile<DT, DP>;
+    static constexpr int kValueBufs = WAVES == 8 ? 3 : 2;
+    static constexpr int kBytes = 2 * Tile::kKeyBytes + kValueBufs * Tile::kValueBytes;
+    static constexpr int kResident = WAVES == 8 || kBytes + sizeof(PagedChunk) > 80 * 1024 ? 1 : 2;
+};
+
+template <int DT, int DP, int WAVES>
+__global__ __launch_bounds__(WAVES * kWave, (WAVES / 4 * BlockShape<DT, DP, WAVES>::kResident)) void paged_block(PagedArgs p, PagedRuns a) {
+    using Tile = BlockTile<DT, DP>;
+    using Shape = BlockShape<DT, DP, WAVES>;
     constexpr int kThreads = WAVES * kWave, kC = DP / 16, kDb = DP / 32;
     constexpr int kElement = DT == MIMIR_KV_F32 ? 4 : DT == MIMIR_KV_BF16 ? 2 : 1;
     // Eight waves: the second four, which share the SIMDs with the first, multiply a
     // tile's values one tile later, so that one's softmax runs beside the other's products;
     // the values stay that much longer.
     constexpr bool kStagger = WAVES == 8;
-    constexpr int kValueBufs = kStagger ? 3 : 2;
-    __shared__ __attribute__((aligned(16))) char lds[2 * Tile::kKeyBytes + kValueBufs * Tile::kValueBytes];
+    __shared__ __attribute__((aligned(16))) char lds[Shape::kBytes];
     char* const values = lds + 2 * Tile::kKeyBytes;
     __shared__ PagedChunk chunk;
 
@@ -396,7 +406,7 @@ int launch(mimir_ctx* ctx, const PagedArgs& p, PagedRuns a) {
     const int64_t rows = static_cast<int64_t>(p.b.max_new) * p.group;
     a.row_blocks = static_cast<int32_t>((rows + a.block_rows - 1) / a.block_rows);
     const int64_t blocks = static_cast<int64_t>(p.b.sequences) * p.c.kv_heads * a.row_blocks;
-    const int64_t runs = ctx->tune.attn_splits > 0 ? ctx->tune.attn_splits : 2048 / WAVES;
+    const int64_t runs = ctx->tune.paged_runs > 0 ? ctx->tune.paged_runs : 256 * BlockShape<DT, DP, WAVES>::kResident;
     const int64_t grid = paged_runs(ctx, p, &a, runs, blocks, true);
     MIMIR_REQUIRE(ctx, dispatch_fits(grid, WAVES * kWave), "paged attention: grid of %lld workgroups exceeds the limit",
                   (long long)grid);

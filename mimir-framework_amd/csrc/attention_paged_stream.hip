@@ -122,19 +122,20 @@ struct Values {
 };
 
 // Waves of a SIMD.
-constexpr int stream_waves(int dtype, int dp) {
-    return dp == 256 ? 1 : dtype == MIMIR_KV_F32 ? (dp == 128 ? 1 : 2) : dp == 128 ? 2 : 4;
+constexpr int stream_waves(int dtype, int dp, int tiles) {
+    return dp == 256 ? 1 : dtype == MIMIR_KV_F32 ? (dp == 128 ? 1 : 2) : dp == 128 || tiles == 2 ? 2 : 4;
 }
 
-template <int DT, int DP>
-__global__ __launch_bounds__(kStreamWaves * kWave, stream_waves(DT, DP)) void paged_stream(PagedArgs p, PagedRuns a) {
+// TILES: of 16 rows, that share the keys' and values' way in.
+template <int DT, int DP, int TILES>
+__global__ __launch_bounds__(kStreamWaves * kWave, stream_waves(DT, DP, TILES)) void paged_stream(PagedArgs p, PagedRuns a) {
     using K = Kind<DT, DP>;
-    constexpr int ND = DP / 16, kSteps = DP / 32, H = K::kHalves;
-    typedef float Share[kRows][DP + 2];
+    constexpr int ND = DP / 16, kSteps = DP / 32, H = K::kHalves, R = TILES;
+    typedef float Share[kRows * R][DP + 2];
     __shared__ __attribute__((aligned(16))) char lds[sizeof(Share) * kStreamWaves];
     Share* const share = reinterpret_cast<Share*>(lds);  // after the keys
-    u4* const q_lds = reinterpret_cast<u4*>(lds);        // [step][term][lane], during them
-    static_assert(kSteps * 3 * kWave * sizeof(u4) <= sizeof lds, "the queries fit");
+    u4* const q_lds = reinterpret_cast<u4*>(lds);        // [tile][step][term][lane], during them
+    static_assert(R * kSteps * 3 * kWave * sizeof(u4) <= sizeof lds, "the queries fit");
     __shared__ uint32_t bad;
     __shared__ PagedChunk chunk;
     const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave);
@@ -145,20 +146,26 @@ __global__ __launch_bounds__(kStreamWaves * kWave, stream_waves(DT, DP)) void pa
     const PagedPiece w = walk.next(p, a);
     if (w.rows <= 0) return;
     const int k0 = w.k0, k1 = w.k1;
-    const int my_row = w.row0 + min(li, w.rows - 1);
-    const int my_end = min(row_end(p, w.seq, my_row), k1);
+    int my_row[R], my_end[R];
+#pragma unroll
+    for (int n = 0; n < R; ++n) {
+        my_row[n] = w.row0 + min(kRows * n + li, w.rows - 1);
+        my_end[n] = min(row_end(p, w.seq, my_row[n]), k1);
+    }
     const auto q_row = [&](int row) { return p.q + paged_row(p, p.ld_q, w.seq.first, w.head, row); };
     // The queries' loads go out ahead of the first keys', their terms follow those.
     constexpr int kOwn = (kSteps + kStreamWaves - 1) / kStreamWaves;
-    float qx[kOwn][8];
+    float qx[R][kOwn][8];
 #pragma unroll
-    for (int i = 0; i < kOwn; ++i) {
-        const float* row = q_row(my_row);
+    for (int n = 0; n < R; ++n) {
+        const float* row = q_row(my_row[n]);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const int d = K::dim(wave + i * kStreamWaves, hg, e);
-            qx[i][e] = d < p.c.head_dim ? row[d] : 0.f;
-        }
+        for (int i = 0; i < kOwn; ++i)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int d = K::dim(wave + i * kStreamWaves, hg, e);
+                qx[n][i][e] = d < p.c.head_dim ? row[d] : 0.f;
+            }
     }
 
     // Where the halves of a step stand; one without a page (or past the keys) takes
@@ -222,10 +229,15 @@ __global__ __launch_bounds__(kStreamWaves * kWave, stream_waves(DT, DP)) void pa
         }
     };
 
-    f4r o[ND];
+    f4r o[R][ND];
+    float m_run[R], l_run[R];  // the max is the row's, the sum this lane's share
 #pragma unroll
-    for (int t = 0; t < ND; ++t) o[t] = f4r{0.f, 0.f, 0.f, 0.f};
-    float m_run = -1e30f, l_run = 0.f;  // the max is the row's, the sum this lane's share
+    for (int n = 0; n < R; ++n) {
+        m_run[n] = -1e30f;
+        l_run[n] = 0.f;
+#pragma unroll
+        for (int t = 0; t < ND; ++t) o[n][t] = f4r{0.f, 0.f, 0.f, 0.f};
+    }
 
     constexpr int kKeys = kHalf * H, kStep = kKeys * kStreamWaves;
     int key = k0 + wave * kKeys;
@@ -243,11 +255,15 @@ __global__ __launch_bounds__(kStreamWaves * kWave, stream_waves(DT, DP)) void pa
         const int c = wave + i * kStreamWaves;
         if (c >= kSteps) break;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) qx[i][e] *= p.qscale;
-        const Split8 x = split8(qx[i]);
-        q_lds[(3 * c) * kWave + lane] = x.h;
-        q_lds[(3 * c + 1) * kWave + lane] = x.m;
-        q_lds[(3 * c + 2) * kWave + lane] = x.l;
+        for (int n = 0; n < R; ++n) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) qx[n][i][e] *= p.qscale;
+            const Split8 x = split8(qx[n][i]);
+            u4* const to = q_lds + 3 * (n * kSteps + c) * kWave + lane;
+            to[0] = x.h;
+            to[kWave] = x.m;
+            to[2 * kWave] = x.l;
+        }
     }
     __syncthreads();
     // One step.  more: the next one's loads are issued in between, K's once the scores
@@ -257,71 +273,88 @@ __global__ __launch_bounds__(kStreamWaves * kWave, stream_waves(DT, DP)) void pa
         int at = lane;
         asm volatile("" : "+v"(at));  // read here in each step, not held in registers across them
         const u4* const mine = q_lds + at;
-        f4r s[H];
+        f4r s[R][H];
 #pragma unroll
-        for (int u = 0; u < H; ++u) s[u] = f4r{0.f, 0.f, 0.f, 0.f};
+        for (int n = 0; n < R; ++n)
+#pragma unroll
+            for (int u = 0; u < H; ++u) s[n][u] = f4r{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int c = 0; c < kSteps; ++c) {
-            const Split8 q{mine[(3 * c) * kWave], mine[(3 * c + 1) * kWave], mine[(3 * c + 2) * kWave]};
+            typename K::Operand k[H];
 #pragma unroll
-            for (int u = 0; u < H; ++u) s[u] = mfma16_split(K::operand(kr[u], c), q, s[u]);
+            for (int u = 0; u < H; ++u) k[u] = K::operand(kr[u], c);
+#pragma unroll
+            for (int n = 0; n < R; ++n) {
+                const u4* const x = mine + 3 * (n * kSteps + c) * kWave;
+                const Split8 q{x[0], x[kWave], x[2 * kWave]};
+#pragma unroll
+                for (int u = 0; u < H; ++u) s[n][u] = mfma16_split(k[u], q, s[n][u]);
+            }
             if constexpr (DT == MIMIR_KV_F32) __builtin_amdgcn_sched_barrier(0);  // few terms at a time
         }
         if constexpr (DT == MIMIR_KV_I8) {
 #pragma unroll
-            for (int u = 0; u < H; ++u)
+            for (int n = 0; n < R; ++n)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) s[u][r] *= ks[u][r];
+                for (int u = 0; u < H; ++u)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) s[n][u][r] *= ks[u][r];
         }
         if constexpr (decltype(more)::value) {
             load_k(nx);
             after = find(key + 2 * kStep);  // here, where no LDS read waits for it
         }
 
-        float x[4 * H];
+        bool holes = false;
 #pragma unroll
-        for (int e = 0; e < 4 * H; ++e) x[e] = s[e / 4][e % 4];
-        // Rows whose keys end inside the step, and halves that are not there: the
-        // weights are 0 (and values of keys that no row sees were read as zeros).
-        bool edge = __any(key + kKeys > my_end);
+        for (int u = 0; u < H; ++u) holes = holes || !st.has(u, p.c);
+        Split8 pw[R][H / 2];
 #pragma unroll
-        for (int u = 0; u < H; ++u) edge = edge || !st.has(u, p.c);
-        if (edge) {
+        for (int n = 0; n < R; ++n) {
+            float x[4 * H];
+#pragma unroll
+            for (int e = 0; e < 4 * H; ++e) x[e] = s[n][e / 4][e % 4];
+            // Rows whose keys end inside the step, and halves that are not there: the
+            // weights are 0 (and values of keys that no row sees were read as zeros).
+            if (holes || __any(key + kKeys > my_end[n])) {
+#pragma unroll
+                for (int e = 0; e < 4 * H; ++e) {
+                    const int u = e / 4, j = key + kHalf * u + 4 * hg + e % 4;
+                    x[e] = st.has(u, p.c) && j < my_end[n] ? x[e] : -INFINITY;
+                }
+            }
+            float top = x[0];
+#pragma unroll
+            for (int e = 1; e < 4 * H; ++e) top = fmaxf(top, x[e]);
+            if (__any(top > m_run[n] + kPagedSlack)) {
+                top = fmaxf(top, __shfl_xor(top, 16));
+                top = fmaxf(top, __shfl_xor(top, 32));
+                const float m_new = fmaxf(m_run[n], top);
+                const float f = __builtin_amdgcn_exp2f(m_run[n] - m_new);
+                m_run[n] = m_new;
+                l_run[n] *= f;
+#pragma unroll
+                for (int t = 0; t < ND; ++t) o[n][t] *= f;
+            }
 #pragma unroll
             for (int e = 0; e < 4 * H; ++e) {
-                const int u = e / 4, j = key + kHalf * u + 4 * hg + e % 4;
-                x[e] = st.has(u, p.c) && j < my_end ? x[e] : -INFINITY;
+                x[e] = __builtin_amdgcn_exp2f(x[e] - m_run[n]);
+                l_run[n] += x[e];
+                if constexpr (DT == MIMIR_KV_I8) x[e] *= vs[e / 4][e % 4];
             }
-        }
-        float top = x[0];
 #pragma unroll
-        for (int e = 1; e < 4 * H; ++e) top = fmaxf(top, x[e]);
-        if (__any(top > m_run + kPagedSlack)) {
-            top = fmaxf(top, __shfl_xor(top, 16));
-            top = fmaxf(top, __shfl_xor(top, 32));
-            const float m_new = fmaxf(m_run, top);
-            const float f = __builtin_amdgcn_exp2f(m_run - m_new);
-            m_run = m_new;
-            l_run *= f;
-#pragma unroll
-            for (int t = 0; t < ND; ++t) o[t] *= f;
+            for (int h = 0; h < H / 2; ++h) pw[n][h] = split8(x + 8 * h);
         }
 #pragma unroll
-        for (int e = 0; e < 4 * H; ++e) {
-            x[e] = __builtin_amdgcn_exp2f(x[e] - m_run);
-            l_run += x[e];
-            if constexpr (DT == MIMIR_KV_I8) x[e] *= vs[e / 4][e % 4];
-        }
-#pragma unroll
-        for (int h = 0; h < H / 2; ++h) {
-            const Split8 pw = split8(x + 8 * h);
+        for (int h = 0; h < H / 2; ++h)
 #pragma unroll
             for (int t = 0; t < ND; ++t) {
-                o[t] = mfma16_split(vr[h].operand(t), pw, o[t]);
+                const auto v = vr[h].operand(t);
+#pragma unroll
+                for (int n = 0; n < R; ++n) o[n][t] = mfma16_split(v, pw[n][h], o[n][t]);
                 if constexpr (DT == MIMIR_KV_F32)
                     if (t % 2 == 1) __builtin_amdgcn_sched_barrier(0);
             }
-        }
         if constexpr (decltype(more)::value) load_v(nx, key + kStep);
     };
     for (; key + kStep < k1; key += kStep) {
@@ -333,15 +366,19 @@ __global__ __launch_bounds__(kStreamWaves * kWave, stream_waves(DT, DP)) void pa
 
     // The waves' shares of the rows.  Lane (li, hg) holds dimensions (4 hg + r) ND + t.
     __syncthreads();
-    l_run += __shfl_xor(l_run, 16);
-    l_run += __shfl_xor(l_run, 32);
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
+    for (int n = 0; n < R; ++n) {
+        l_run[n] += __shfl_xor(l_run[n], 16);
+        l_run[n] += __shfl_xor(l_run[n], 32);
+        float* const to = share[wave][kRows * n + li];
 #pragma unroll
-        for (int t = 0; t < ND; ++t) share[wave][li][(4 * hg + r) * ND + t] = o[t][r];
-    if (hg == 0) {
-        share[wave][li][DP] = m_run;
-        share[wave][li][DP + 1] = l_run;
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int t = 0; t < ND; ++t) to[(4 * hg + r) * ND + t] = o[n][t][r];
+        if (hg == 0) {
+            to[DP] = m_run[n];
+            to[DP + 1] = l_run[n];
+        }
     }
     __syncthreads();
     const auto out_row = [&](int row) { return p.out + paged_row(p, p.ld_out, w.seq.first, w.head, w.row0 + row); };
@@ -386,44 +423,55 @@ __global__ __launch_bounds__(kStreamWaves * kWave, stream_waves(DT, DP)) void pa
     }
 }
 
-template <int DT>
+template <int DT, int TILES>
 void launch_dim(const PagedArgs& p, const PagedRuns& a, unsigned grid, hipStream_t s) {
     constexpr int kThreads = kStreamWaves * kWave;
-    if (p.c.stride <= 64) paged_stream<DT, 64><<<grid, kThreads, 0, s>>>(p, a);
-    else if (p.c.stride <= 128) paged_stream<DT, 128><<<grid, kThreads, 0, s>>>(p, a);
-    else paged_stream<DT, 256><<<grid, kThreads, 0, s>>>(p, a);
+    if (p.c.stride <= 64) paged_stream<DT, 64, TILES><<<grid, kThreads, 0, s>>>(p, a);
+    else if (p.c.stride <= 128) paged_stream<DT, 128, TILES><<<grid, kThreads, 0, s>>>(p, a);
+    else if constexpr (!(DT == MIMIR_KV_F32 && TILES == 2)) paged_stream<DT, 256, TILES><<<grid, kThreads, 0, s>>>(p, a);
+}
+template <int DT>
+void launch_tiles(const PagedArgs& p, const PagedRuns& a, int tiles, unsigned grid, hipStream_t s) {
+    if (tiles == 1) launch_dim<DT, 1>(p, a, grid, s);
+    else launch_dim<DT, 2>(p, a, grid, s);
 }
 
 // Workgroups that the GPU holds at once.
-int64_t stream_resident(int dtype, int stride) {
+int64_t stream_resident(int dtype, int stride, int tiles) {
     // Two a compute unit where registers allow them: measured (256 / 512 / 1024 workgroups, us), 64 sequences x
     // 4096 keys x 8 heads x 128: 8-bit 112 / 99 / 105, bf16 168 / 162 / 170; heads of 64: 8-bit 76 / 60 / 60, bf16
     // 88 / 87 / 92, fp32 183 / 168 / 174; heads of 256, one a unit: bf16 120 / 131 / 145.
-    return 256 * std::min(2, stream_waves(dtype, stride <= 64 ? 64 : stride <= 128 ? 128 : 256));
+    return 256 * std::min(2, stream_waves(dtype, stride <= 64 ? 64 : stride <= 128 ? 128 : 256, tiles));
 }
 
 }  // namespace
 
 int mimir::paged_stream_launch(mimir_ctx* ctx, const PagedArgs& p, int dtype, int64_t most_rows) {
     constexpr uint32_t kStep = 2 * kHalf * kStreamWaves;
+    const int64_t rows = std::min(static_cast<int64_t>(p.b.max_new) * p.group, most_rows);
+    // A sequence's second tile shares the first one's keys, unless other sequences have more rows
+    // than this kernel takes: then single tokens are what most have.  (For wide fp32
+    // heads two tiles are more than the registers hold.)
+    const bool wide = dtype == MIMIR_KV_F32 && p.c.stride > 128;
+    const int tiles = rows > kRows && !wide && rows == static_cast<int64_t>(p.b.max_new) * p.group ? 2 : 1;
     PagedRuns a{};
     a.extra = 2 * kStep;  // the queries, the first keys' way in, the sums' way out
     a.grain = kStep;
-    a.block_rows = kRows;
+    a.block_rows = kRows * tiles;
     a.least_rows = 1;
     a.most_rows = static_cast<int32_t>(most_rows);
-    const int64_t rows = std::min(static_cast<int64_t>(p.b.max_new) * p.group, most_rows);
-    a.part_rows = static_cast<int32_t>(std::min<int64_t>(rows, kRows));
-    a.row_blocks = static_cast<int32_t>((rows + kRows - 1) / kRows);
+    a.part_rows = static_cast<int32_t>(std::min<int64_t>(rows, a.block_rows));
+    a.row_blocks = static_cast<int32_t>((rows + a.block_rows - 1) / a.block_rows);
     const int64_t blocks = static_cast<int64_t>(p.b.sequences) * p.c.kv_heads * a.row_blocks;
-    const int64_t runs = ctx->tune.decode_splits > 0 ? ctx->tune.decode_splits : stream_resident(dtype, p.c.stride);
-    // Blocks of up to two steps are not worth a join.
-    const int64_t grid = paged_runs(ctx, p, &a, runs, blocks, p.b.max_len > static_cast<int64_t>(2 * kStep));
+    const int64_t runs = ctx->tune.paged_runs > 0 ? ctx->tune.paged_runs : stream_resident(dtype, p.c.stride, tiles);
+    // Blocks of up to eight steps are not worth a join: 500 and 1000 keys x 8 heads of one sequence whole / cut, us:
+    // 10 / 16, 14 / 17; 2000, 29 / 18.
+    const int64_t grid = paged_runs(ctx, p, &a, runs, blocks, p.b.max_len > static_cast<int64_t>(8 * kStep));
     MIMIR_REQUIRE(ctx, dispatch_fits(grid, kStreamWaves * kWave), "paged attention: grid of %lld workgroups exceeds the limit",
                   (long long)grid);
-    if (dtype == MIMIR_KV_F32) launch_dim<MIMIR_KV_F32>(p, a, static_cast<unsigned>(grid), ctx->stream);
-    else if (dtype == MIMIR_KV_BF16) launch_dim<MIMIR_KV_BF16>(p, a, static_cast<unsigned>(grid), ctx->stream);
-    else launch_dim<MIMIR_KV_I8>(p, a, static_cast<unsigned>(grid), ctx->stream);
+    if (dtype == MIMIR_KV_F32) launch_tiles<MIMIR_KV_F32>(p, a, tiles, static_cast<unsigned>(grid), ctx->stream);
+    else if (dtype == MIMIR_KV_BF16) launch_tiles<MIMIR_KV_BF16>(p, a, tiles, static_cast<unsigned>(grid), ctx->stream);
+    else launch_tiles<MIMIR_KV_I8>(p, a, tiles, static_cast<unsigned>(grid), ctx->stream);
     if (int st = launched(ctx, "paged_stream")) return st;
     return paged_join_launch(ctx, p, a);
 }

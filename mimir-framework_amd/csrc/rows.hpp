@@ -67,6 +67,7 @@ struct Tuning {
     int attn_waves = 0;       // attention forward: waves per workgroup (4, 8; 0: measured default)
     int attn_splits = 0;      // attention forward: splits of the keys (0: measured default)
     int decode_splits = 0;    // attention_decode: workgroups per (sequence, head) (0: measured default)
+    int paged_runs = 0;       // paged attention: workgroups that the work is dealt to (0: measured default)
     int attn_bwd_heads = 0;   // attention backward: (sequence, head) pairs per group (0: what 512 MiB of dS, or, heads
                               // over 128, 1 GiB of P and dS hold)
     int attn_bwd_blocks = 0;  // causal attention backward: query / key blocks of the products (0: default)
@@ -122,6 +123,7 @@ inline Tuning read_tuning() {
         else if (!std::strcmp(k, "attnwaves")) t.attn_waves = std::atoi(v);
         else if (!std::strcmp(k, "attnsplits")) t.attn_splits = std::atoi(v);
         else if (!std::strcmp(k, "decode")) t.decode_splits = std::atoi(v);
+        else if (!std::strcmp(k, "paged")) t.paged_runs = std::atoi(v);
         else if (!std::strcmp(k, "attnbwd_heads")) t.attn_bwd_heads = std::atoi(v);
         else if (!std::strcmp(k, "attnbwd_blocks")) t.attn_bwd_blocks = std::atoi(v);
         else if (!std::strcmp(k, "embsort")) t.embed_bwd_sort = std::atoi(v);

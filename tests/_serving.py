@@ -1,5 +1,7 @@
 """Plain 64-bit forms of the serving operators (rotary positions per token, the
 paged key/value cache, attention over it) and the batches their tests use."""
+import ctypes
+
 import numpy as np
 
 import mimir_hip as M
@@ -157,3 +159,53 @@ def attention64(q, k, v, first, causal, scale):
             score = (4 * np.sqrt(d) + 8) * sa[i, :m].max()
             tol[i, h] = U * mag * (2 * score + 8 + 2 * (4 * np.sqrt(m) + 8)) + 1e-37
     return out, tol
+
+
+# --- contexts and graphs -----------------------------------------------------
+
+def tuned_context(tune):
+    """A context of its own with MIMIR_TUNE set."""
+    import os
+    old = os.environ.get("MIMIR_TUNE")
+    os.environ["MIMIR_TUNE"] = tune
+    try:
+        return M.Context(0)
+    finally:
+        if old is None:
+            del os.environ["MIMIR_TUNE"]
+        else:
+            os.environ["MIMIR_TUNE"] = old
+
+
+class Hip:
+    """The runtime's own stream and graph calls, through the library that links it."""
+
+    def __init__(self, ctx):
+        self.lib = ctypes.CDLL(M._lib.LIB_PATH)
+
+    def __call__(self, name, *args):
+        st = getattr(self.lib, name)(*args)
+        assert st == 0, f"{name}: {st}"
+
+
+class Graph:
+    """What `calls` enqueues on the context's stream, captured."""
+
+    def __init__(self, ctx, calls):
+        self.ctx, self.hip = ctx, Hip(ctx)
+        ctx.lib.mimir_ctx_stream.restype = ctypes.c_void_p
+        self.stream = ctypes.c_void_p(ctx.lib.mimir_ctx_stream(ctx.handle))
+        graph, self.exe = ctypes.c_void_p(), ctypes.c_void_p()
+        self.hip("hipStreamBeginCapture", self.stream, 1)  # thread local
+        try:
+            calls()
+        finally:
+            self.hip("hipStreamEndCapture", self.stream, ctypes.byref(graph))
+        self.hip("hipGraphInstantiate", ctypes.byref(self.exe), graph, None, None, ctypes.c_size_t(0))
+        self.hip("hipGraphDestroy", graph)
+
+    def launch(self):
+        self.hip("hipGraphLaunch", self.exe, self.stream)
+
+    def close(self):
+        self.hip("hipGraphExecDestroy", self.exe)

@@ -103,6 +103,52 @@ def test_append_and_read(ctx, dtype, lens, kh, d, page):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d,heads,kh,ld_extra", [(32, 3, 2, 0), (128, 4, 1, 0), (7, 2, 2, 1)])
+def test_many_tokens(ctx, dtype, d, heads, kh, ld_extra):
+    """Enough for several a workgroup, whose last one is not full; sequences that end
+    inside one, some without new tokens."""
+    lens = [(4000, 4000), (1, 9), (0, 0), (1, 1), (1, 1), (0, 5), (4998, 5010)]
+    p = Paged(ctx, dtype, lens, kh, d, 64, seed=d)
+    k, v, q = rand_rows(d + 1, (p.tokens, kh, d), (p.tokens, kh, d), (p.tokens, heads, d))
+    rot = d // 2 * 2
+    c, s = M.rope_table_scaled(5010, rot)
+    rope = M.Rope(ctx.to_device(c), ctx.to_device(s), 5010, rot, False)
+    pos = np.concatenate([np.arange(m - n, m) for n, m in lens])
+    cache, batch, got = append(ctx, p, k, v, q, rope, ld_extra=ld_extra)
+    np.testing.assert_array_equal(got, rotate(q, pos, c, s, rot, False))
+    turned = rotate(k, pos, c, s, rot, False)
+    assert_cache(p, cache, expected(p, turned, v))
+    ld = kh * d + ld_extra
+    ko, vo = (ctx.to_device(np.full((p.tokens, ld), -4.0, np.float32)) for _ in range(2))
+    ctx.kv_read(cache, batch, ko, vo, ld_out=ld)
+    for out, x in ((ko, turned), (vo, v)):
+        o = out.numpy()
+        np.testing.assert_array_equal(o[:, :kh * d].reshape(x.shape), held(x, dtype))
+        assert (o[:, kh * d:] == -4).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_kept_outputs_have_the_same_bits(ctx, dtype):
+    """Queries and rows read back written with plain stores."""
+    lens, d = [(30, 40), (1, 2)], 64
+    p = Paged(ctx, dtype, lens, 2, d, 16)
+    k, v, q = rand_rows(8, (31, 2, d), (31, 2, d), (31, 4, d))
+    c, s = M.rope_table_scaled(40, d)
+    rope = M.Rope(ctx.to_device(c), ctx.to_device(s), 40, d, False)
+    pos = np.concatenate([np.arange(m - n, m) for n, m in lens])
+    ctx.set_output_caching(True)
+    try:
+        cache, batch, got = append(ctx, p, k, v, q, rope)
+        ko = ctx.empty((31, 2, d))
+        ctx.kv_read(cache, batch, ko, None)
+        ko = ko.numpy()
+    finally:
+        ctx.set_output_caching(False)
+    np.testing.assert_array_equal(got, rotate(q, pos, c, s, d, False))
+    np.testing.assert_array_equal(ko, held(rotate(k, pos, c, s, d, False), dtype))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("d,rot,interleaved", [(128, 128, False), (64, 32, True), (80, 16, False), (256, 256, True), (10, 6, False),
                                                (6, 6, True), (37, 20, True), (48, 4, False)])
 def test_append_rotated(ctx, dtype, d, rot, interleaved):

@@ -113,7 +113,7 @@ int64_t mimir::paged_runs(mimir_ctx* ctx, const PagedArgs& p, PagedRuns* a, int6
     // No more than keep to the least length of a run (PagedWalk), by the longest costs.
     const int64_t cost = a->extra + static_cast<int64_t>(p.b.max_len) + (p.causal ? (a->block_rows + p.group - 1) / p.group : 0);
     runs = std::max<int64_t>(1, std::min(runs, blocks * cost / (a->extra + a->grain) + 1));
-    a->apart = a->row_blocks == 1 && p.b.sequences <= kWave && 2 * blocks <= runs && p.b.max_len < 1 << 30;
+    a->apart = p.b.sequences <= kWave;
     a->many = a->part_rows <= 32 && runs > 4 * blocks;
     const int64_t floats = runs * 2 * paged_part_floats(a->part_rows, p.c.head_dim);
     const int64_t bytes = runs * static_cast<int64_t>(sizeof(PagedShared)) + floats * 4;

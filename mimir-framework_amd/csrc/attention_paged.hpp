@@ -186,14 +186,16 @@ struct PagedWalk {
     // enough, or somewhat longer ones, if that is not longer than such a part.  The total.
     __device__ __forceinline__ uint64_t set_apart(const PagedArgs& p, const PagedRuns& a, uint64_t total, PagedCost cost) {
         const int lane = static_cast<int>(threadIdx.x % kWave);
-        const uint64_t each = cost.ahead(1);  // a sequence has one block for each head, or none
-        const uint32_t count = cost.blocks * static_cast<uint32_t>(p.c.kv_heads);
-        const uint32_t left = a.runs - static_cast<uint32_t>(p.b.sequences * p.c.kv_heads);
-        const uint64_t longer = max(uniform(quotient(total + left - 1, left)), run);
+        const uint64_t each = cost.base + static_cast<uint64_t>(cost.slope) * cost.blocks;  // the sequence's last block's
+        const uint64_t count = static_cast<uint64_t>(cost.blocks) * static_cast<uint32_t>(p.c.kv_heads);
+        const uint64_t all = lane_of(lanes_up_to(count), kWave - 1);
+        if (2 * all > a.runs || all == 0) return total;
         uint64_t whole = quotient(each + run - 1, run);
         if (lane_of(lanes_up_to(whole * count), kWave - 1) > a.runs) {
+            const uint64_t most = lane_of(lanes_up_to(each * count), kWave - 1), left = a.runs - all;
+            const uint64_t longer = uniform(quotient(most + left - 1, left));
             if (longer > run + a.extra) return total;
-            run = longer;
+            run = max(run, longer);
             whole = quotient(each + run - 1, run);
         }
         cost.slope = 0;

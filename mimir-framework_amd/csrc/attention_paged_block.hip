@@ -110,6 +110,7 @@ __global__ __launch_bounds__(WAVES * kWave, (WAVES / 4 * BlockShape<DT, DP, WAVE
     const bool in = li < wave_rows;
     const int my_row = w.row0 + wave * kTile + max(0, min(li, wave_rows - 1));
     const int my_end = min(row_end(p, w.seq, min(my_row, w.row0 + w.rows - 1)), k1);
+    const int first_end = uniform(my_end);  // the wave's first row's, none sees fewer
     const int wave_end = wave_rows > 0 ? min(k1, row_end(p, w.seq, w.row0 + wave * kTile + wave_rows - 1)) : k0;
     const auto q_row = [&](int row) { return p.q + paged_row(p, p.ld_q, w.seq.first, w.head, row); };
     const PagedPart part(a, p.c.head_dim, walk.index, w.begins);
@@ -119,103 +120,127 @@ __global__ __launch_bounds__(WAVES * kWave, (WAVES / 4 * BlockShape<DT, DP, WAVE
                        : part.sums(row);
     };
 
-    // This lane's query values, times scale * log2(e).
-    Split8 q[kC];
-    {
-        const float* row = q_row(min(my_row, w.row0 + w.rows - 1));
-#pragma unroll
-        for (int c = 0; c < kC; ++c) {
-            float x[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const int d = 16 * c + 8 * hf + e;
-                x[e] = d < p.c.head_dim ? row[d] * p.qscale : 0.f;
-            }
-            q[c] = split8(x);
-        }
-    }
-
     // Tiles in, one item (eight dimensions of a key) at a time.
     const int tiles = (k1 - k0 + kTile - 1) / kTile;
     const scalar_i32 table = (scalar_i32)(p.b.page_table + w.s * p.b.ld_pages);
     const int row_bytes = p.c.stride * kElement;
-    // Where a tile's halves stand, and how many of their keys are there (none of one
-    // without a page).
-    struct Pages {
-        int page[2], slot[2], keys[2];
-    };
-    const auto find = [&](int t) {
-        Pages g;
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            const int j = k0 + t * kTile + kHalf * u, i = max(min(j, (k1 - 1) & -kHalf), 0);
-            const uint32_t entry = fastdiv(static_cast<uint32_t>(i), p.c.page_div);
-            g.page[u] = j < k1 ? table[entry] : -1;
-            g.slot[u] = i - static_cast<int>(entry) * p.c.page_size;
-            g.keys[u] = min(k1 - j, kHalf);
-        }
-        return g;
-    };
     const auto pages = static_cast<uint32_t>(p.c.pages);
-    const auto there = [&](const Pages& g, int u) { return static_cast<uint32_t>(g.page[u]) < pages; };
-    // A thread's items: eight dimensions of a row.  The rows of a wave are of one half.
-    // What lies past a row's dimensions or the half's keys reads as zeros.
+    const auto entry_of = [&](int j) { return fastdiv(static_cast<uint32_t>(max(min(j, (k1 - 1) & -kHalf), 0)), p.c.page_div); };
+    const auto there = [&](int j) { return static_cast<uint32_t>(table[entry_of(j)]) < pages; };
+    // Whether a page of these keys is none.
+    bool holes = false;
+    if (tiles > 0) {
+        const int32_t* entries = p.b.page_table + w.s * p.b.ld_pages;
+        const auto last = static_cast<int>(fastdiv(static_cast<uint32_t>(k1 - 1), p.c.page_div));
+        for (int e = static_cast<int>(fastdiv(static_cast<uint32_t>(k0), p.c.page_div)) + lane; e <= last; e += kWave)
+            holes = holes || static_cast<uint32_t>(entries[e]) >= pages;
+        holes = __any(holes);
+    }
+    // A thread's items: eight dimensions of a row.  An item's rows are, for a wave, of
+    // one half of the tile; what lies past a row's dimensions or the half's keys reads
+    // as zeros.
     constexpr int kLanes = DP == 64 ? 8 : 16;
     constexpr int kItems = (kTile * kLanes + kThreads - 1) / kThreads;
     static_assert(kWave / kLanes <= kHalf && kHalf % (kWave / kLanes) == 0, "a wave's rows in one half");
+    static_assert(kItems == 1 || (kItems == 2 && kThreads == kHalf * kLanes), "an item a half");
+    constexpr int kMovers = kItems == 2 ? WAVES : kHalf * kLanes / kWave;  // waves that share a half
     const int d_mine = 8 * (tid % kLanes);
     const auto row_of = [&](int n) { return (tid + n * kThreads) / kLanes; };
-    RowItem<DT> ki[kItems], vi[kItems];
-    float scale = 0.f;
-    const auto load = [&](const Pages& g) {
+    const auto half_of = [&](int n) { return kItems == 2 ? n : wave / kMovers; };
+    const uint32_t off = d_mine < p.c.stride ? static_cast<uint32_t>(row_of(0) % kHalf * row_bytes + d_mine * kElement) : kOutside;
+    const int64_t page_rows = static_cast<int64_t>(p.c.kv_heads) * p.c.page_size, head_rows = static_cast<int64_t>(w.head) * p.c.page_size;
+    const bool mover = kItems == 2 || half_of(0) < 2;
+    // Where an item's half stands, and how many of its keys are there.
+    struct Halves {
+        int page[kItems], slot[kItems], keys[kItems];
+    };
+    const auto find = [&](int t) {
+        Halves g;
 #pragma unroll
         for (int n = 0; n < kItems; ++n) {
-            const int u = uniform(row_of(n)) / kHalf;
-            if (u > 1) continue;
-            const bool has = u ? there(g, 1) : there(g, 0);
-            const int64_t row = (static_cast<int64_t>(has ? (u ? g.page[1] : g.page[0]) : 0) * p.c.kv_heads + w.head) * p.c.page_size +
-                                (u ? g.slot[1] : g.slot[0]);
-            const int bytes = has ? (u ? g.keys[1] : g.keys[0]) * row_bytes : 0;
-            const uint32_t off = d_mine < p.c.stride ? static_cast<uint32_t>(row_of(n) % kHalf * row_bytes + d_mine * kElement) : kOutside;
-            ki[n].load(__builtin_amdgcn_make_buffer_rsrc(p.c.k + row * row_bytes, 0, bytes, kBufferWord3), off);
-            vi[n].load(__builtin_amdgcn_make_buffer_rsrc(p.c.v + row * row_bytes, 0, bytes, kBufferWord3), off);
+            const int j = k0 + t * kTile + kHalf * half_of(n), i = max(min(j, (k1 - 1) & -kHalf), 0);
+            const uint32_t entry = fastdiv(static_cast<uint32_t>(i), p.c.page_div);
+            g.page[n] = table[entry];
+            g.slot[n] = i - static_cast<int>(entry) * p.c.page_size;
+            g.keys[n] = max(min(k1 - j, kHalf), 0);
         }
-        if constexpr (DT == MIMIR_KV_I8) {
-            if (wave < 4) {  // the keys' of both halves, then the values'
-                const int u = wave % 2;
-                const bool has = u ? there(g, 1) : there(g, 0);
-                const int64_t row = (static_cast<int64_t>(has ? (u ? g.page[1] : g.page[0]) : 0) * p.c.kv_heads + w.head) * p.c.page_size +
-                                    (u ? g.slot[1] : g.slot[0]);
-                const int bytes = has ? 4 * (u ? g.keys[1] : g.keys[0]) : 0;
-                scale = buffer_f1(buffer_of((wave < 2 ? p.c.k_scale : p.c.v_scale) + row, bytes), static_cast<uint32_t>(4 * (lane % kHalf)));
-            }
+        return g;
+    };
+    RowItem<DT> ki[kItems], vi[kItems];
+    float scale[kItems];
+    const int scales = wave % kMovers;  // 8-bit: 0, the keys' scales are this wave's to move, 1, the values'
+    const auto load = [&](const Halves& g) {
+        if (!mover) return;
+#pragma unroll
+        for (int n = 0; n < kItems; ++n) {
+            const bool has = static_cast<uint32_t>(g.page[n]) < pages;
+            const int64_t row = (has ? g.page[n] : 0) * page_rows + head_rows + g.slot[n];
+            const int keys = has ? g.keys[n] : 0;
+            const int64_t at = row * row_bytes;
+            ki[n].load(__builtin_amdgcn_make_buffer_rsrc(p.c.k + at, 0, keys * row_bytes, kBufferWord3), off);
+            vi[n].load(__builtin_amdgcn_make_buffer_rsrc(p.c.v + at, 0, keys * row_bytes, kBufferWord3), off);
+            if constexpr (DT == MIMIR_KV_I8)
+                if (scales < 2)
+                    scale[n] = buffer_f1(buffer_of((scales ? p.c.v_scale : p.c.k_scale) + row, 4 * keys), static_cast<uint32_t>(4 * (lane % kHalf)));
         }
     };
     const auto stash = [&](char* key_buf, char* value_buf) {
+        if (!mover) return;
 #pragma unroll
         for (int n = 0; n < kItems; ++n) {
-            const int row = row_of(n);
-            if (row >= kTile || d_mine >= DP) continue;
-            ki[n].stash(key_buf + row * Tile::kKeyRow + 2 * d_mine, Tile::kKeyPlane);
-            vi[n].stash(value_buf + row * Tile::kValueRow + 2 * d_mine, Tile::kValuePlane);
+            if (d_mine < DP) {
+                ki[n].stash(key_buf + row_of(n) * Tile::kKeyRow + 2 * d_mine, Tile::kKeyPlane);
+                vi[n].stash(value_buf + row_of(n) * Tile::kValueRow + 2 * d_mine, Tile::kValuePlane);
+            }
+            if constexpr (DT == MIMIR_KV_I8)
+                if (scales < 2 && lane < kHalf)
+                    reinterpret_cast<float*>(key_buf + Tile::kScalesAt)[scales * kTile + half_of(n) * kHalf + lane] = scale[n];
         }
-        if constexpr (DT == MIMIR_KV_I8)
-            if (wave < 4 && lane < kHalf) reinterpret_cast<float*>(key_buf + Tile::kScalesAt)[wave * kHalf + lane] = scale;
     };
+
+    Halves to{};  // of the tile after the one in registers, which is after the one in LDS
+    if (tiles > 0) {
+        load(find(0));
+        to = find(1);
+    }
+    // This lane's query values, times scale * log2(e).
+    Split8 q[kC];
+    {
+        const float* row = q_row(min(my_row, w.row0 + w.rows - 1)) + 8 * hf;
+        const int left = p.c.head_dim - 8 * hf;  // of the row from there on
+        if (p.c.head_dim % 4 == 0) {
+            f4u x[kC][2];
+#pragma unroll
+            for (int c = 0; c < kC; ++c)
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+                    x[c][i] = 16 * c + 4 * i < left ? reinterpret_cast<const f4u*>(row + 16 * c)[i] : f4u{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int c = 0; c < kC; ++c) {
+                const f4u a = x[c][0] * p.qscale, b = x[c][1] * p.qscale;
+                const float y[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+                q[c] = split8(y);
+            }
+        } else {
+#pragma unroll
+            for (int c = 0; c < kC; ++c) {
+                float x[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[e] = 16 * c + e < left ? row[16 * c + e] * p.qscale : 0.f;
+                q[c] = split8(x);
+            }
+        }
+    }
 
     f16v o[kDb];
 #pragma unroll
     for (int d = 0; d < kDb; ++d) o[d] = f16v{};
     float m_run = -1e30f, l_run = 0.f;
 
-    Pages g0{}, g1{}, g2{};  // of the tile in LDS, the one in registers, the next
     if (tiles > 0) {
-        g0 = find(0);
-        load(g0);
-        g1 = find(1);
         stash(lds, values);
-        load(g1);
-        g2 = find(2);
+        load(to);
+        to = find(2);
     }
     __syncthreads();
     // A lane's part of a transposed read: key 4 hf + (lane % 16) / 4, dimensions
@@ -302,7 +327,7 @@ __global__ __launch_bounds__(WAVES * kWave, (WAVES / 4 * BlockShape<DT, DP, WAVE
         }
         if (t < tiles) {  // past the last tile the stash rewrites buffers that are not read again
             stash(next, v_next);
-            load(g2);
+            load(to);
         }
         if (active) {
             if constexpr (DT == MIMIR_KV_I8) {
@@ -313,11 +338,12 @@ __global__ __launch_bounds__(WAVES * kWave, (WAVES / 4 * BlockShape<DT, DP, WAVE
                     for (int e = 0; e < 4; ++e) s[r + e] *= x[e];
                 }
             }
-            if (!there(g0, 0) || !there(g0, 1) || __any(key + kTile > my_end)) {
+            if (holes || key + kTile > first_end) {
+                const bool first = !holes || there(key), second = !holes || there(key + kHalf);
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
                     const int j = key + 8 * (r / 4) + 4 * hf + r % 4;
-                    s[r] = j < my_end && there(g0, r / 8) ? s[r] : -INFINITY;
+                    s[r] = j < my_end && (r < 8 ? first : second) ? s[r] : -INFINITY;
                 }
             }
             float top = s[0];
@@ -348,9 +374,7 @@ __global__ __launch_bounds__(WAVES * kWave, (WAVES / 4 * BlockShape<DT, DP, WAVE
             }
             if (!late) weigh(v_cur);
         }
-        g0 = g1;
-        g1 = g2;
-        g2 = find(t + 3);
+        to = find(t + 3);
         char* const v_free = kStagger ? v_old : v_cur;
         v_old = v_cur;
         v_cur = v_next;

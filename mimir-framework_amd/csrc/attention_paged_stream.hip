@@ -161,10 +161,20 @@ __global__ __launch_bounds__(kStreamWaves * kWave, stream_waves(DT, DP, TILES)) 
         const float* row = q_row(my_row[n]);
 #pragma unroll
         for (int i = 0; i < kOwn; ++i)
+            if (p.c.head_dim % 4 == 0) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const int d = K::dim(wave + i * kStreamWaves, hg, e);
-                qx[n][i][e] = d < p.c.head_dim ? row[d] : 0.f;
+                for (int e = 0; e < 8; e += 4) {
+                    const int d = K::dim(wave + i * kStreamWaves, hg, e);
+                    const f4u x = d < p.c.head_dim ? *reinterpret_cast<const f4u*>(row + d) : f4u{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) qx[n][i][e + u] = x[u];
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const int d = K::dim(wave + i * kStreamWaves, hg, e);
+                    qx[n][i][e] = d < p.c.head_dim ? row[d] : 0.f;
+                }
             }
     }
 

@@ -50,6 +50,7 @@ struct PagedRuns {
     float* part;
     uint32_t runs;
     uint32_t extra;      // what a block costs besides its keys, in keys
+    uint32_t slack;      // how much longer a run may be for all to be of one block
     uint32_t grain;      // blocks are cut at multiples of this many keys, a power of two
     int32_t block_rows;
     int32_t part_rows;   // rows of a block that `part` has room for
@@ -183,7 +184,7 @@ struct PagedWalk {
     }
     // With fewer blocks than half the runs, a block's cost may be rounded up to whole
     // runs: a second part costs its run a way in and out.  With these runs if there are
-    // enough, or somewhat longer ones, if that is not longer than such a part.  The total.
+    // enough, or somewhat longer ones (by `slack`, or half).  The total.
     __device__ __forceinline__ uint64_t set_apart(const PagedArgs& p, const PagedRuns& a, uint64_t total, PagedCost cost) {
         const int lane = static_cast<int>(threadIdx.x % kWave);
         const uint64_t each = cost.base + static_cast<uint64_t>(cost.slope) * cost.blocks;  // the sequence's last block's
@@ -194,7 +195,7 @@ struct PagedWalk {
         if (lane_of(lanes_up_to(whole * count), kWave - 1) > a.runs) {
             const uint64_t most = lane_of(lanes_up_to(each * count), kWave - 1), left = a.runs - all;
             const uint64_t longer = uniform(quotient(most + left - 1, left));
-            if (longer > run + a.extra) return total;
+            if (longer > run + min(static_cast<uint64_t>(a.slack), run / 2)) return total;
             run = max(run, longer);
             whole = quotient(each + run - 1, run);
         }
@@ -325,7 +326,20 @@ __device__ __forceinline__ u4 bytes_bf16(uint32_t lo, uint32_t hi) {
     return r;
 }
 
-// Element d of a cache row (index `at` among the rows of the type's buffer).
+// Elements d .. d + 3 (d a multiple of 4) of a cache row (index `at` among the rows of
+// the type's buffer), and element d alone.
+template <int DT>
+__device__ __forceinline__ f4 elements(const char* base, int64_t at, int stride, int d) {
+    const int64_t i = at * stride + d;
+    if constexpr (DT == MIMIR_KV_F32) return *reinterpret_cast<const f4*>(base + 4 * i);
+    if constexpr (DT == MIMIR_KV_BF16) {
+        const u2 x = *reinterpret_cast<const u2*>(base + 2 * i);
+        const u4 w{x[0] << 16, x[0] & 0xffff0000u, x[1] << 16, x[1] & 0xffff0000u};
+        return __builtin_bit_cast(f4, w);
+    }
+    const uint32_t x = *reinterpret_cast<const uint32_t*>(base + i);
+    return f4{byte_float(x, 0), byte_float(x, 1), byte_float(x, 2), byte_float(x, 3)};
+}
 template <int DT>
 __device__ __forceinline__ float element(const char* base, int64_t at, int stride, int d) {
     const int64_t i = at * stride + d;
@@ -337,43 +351,69 @@ __device__ __forceinline__ float element(const char* base, int64_t at, int strid
 
 constexpr int kRowChunks = kKvMaxDim / kWave;
 
-// One query row over keys j0 .. j1 - 1 by one wave, lane l holding dimensions l + 64 c.
-// Leaves the sums (without the division) and the running max (base-2 units) and sum.
+// One query row over keys j0 .. j1 - 1 by one wave: 64 keys at a time, a lane each for
+// the scores; then lane l has dimensions l + 64 c of the sums.  Leaves those (without
+// the division) and the running max (base-2 units) and sum.
 template <int DT>
 __device__ __forceinline__ void row_over_keys(const PagedArgs& a, int s, int kv_head, const float* q, int j0, int j1,
                                               float* acc, float* m_out, float* l_out) {
-    const int lane = threadIdx.x % kWave;
-    float x[kRowChunks];
+    const int lane = threadIdx.x % kWave, d_all = a.c.head_dim;
 #pragma unroll
-    for (int c = 0; c < kRowChunks; ++c) {
-        const int d = lane + c * kWave;
-        x[c] = d < a.c.head_dim ? q[d] * a.qscale : 0.f;
-        acc[c] = 0.f;
-    }
+    for (int c = 0; c < kRowChunks; ++c) acc[c] = 0.f;
     float m = -1e30f, l = 0.f;
-    for (int j = j0; j < j1; ++j) {
-        const auto [page, slot] = kv_slot(a.b, a.c.pages, a.c.page_div, s, j);
-        if (page < 0) continue;
-        const int64_t at = (static_cast<int64_t>(page) * a.c.kv_heads + kv_head) * a.c.page_size + slot;
-        float part = 0.f;
+    for (int j = j0; j < j1; j += kWave) {
+        const KvSlot own = j + lane < j1 ? kv_slot(a.b, a.c.pages, a.c.page_div, s, j + lane) : KvSlot{-1, 0};
+        const bool has = own.page >= 0;
+        const int64_t at = (static_cast<int64_t>(has ? own.page : 0) * a.c.kv_heads + kv_head) * a.c.page_size + own.slot;
+        float score = 0.f;
+#pragma unroll 4
+        for (int d = 0; d < d_all; d += 4) {
+            const f4 k = elements<DT>(a.c.k, at, a.c.stride, d);
 #pragma unroll
-        for (int c = 0; c < kRowChunks; ++c) {
-            const int d = lane + c * kWave;
-            if (d < a.c.head_dim) part += x[c] * element<DT>(a.c.k, at, a.c.stride, d);
+            for (int e = 0; e < 4; ++e)
+                if (d + e < d_all) score += q[d + e] * a.qscale * k[e];
         }
-        float score = wave_sum(part);
         if constexpr (DT == MIMIR_KV_I8) score *= a.c.k_scale[at];
-        const float m_new = fmaxf(m, score);
+        if (!has) score = -INFINITY;
+        const float m_new = fmaxf(m, wave_max(score));
         const float alpha = __builtin_amdgcn_exp2f(m - m_new);
-        const float p = __builtin_amdgcn_exp2f(score - m_new);
+        const float p = has ? __builtin_amdgcn_exp2f(score - m_new) : 0.f;
         m = m_new;
-        l = l * alpha + p;
-        const float w = DT == MIMIR_KV_I8 ? p * a.c.v_scale[at] : p;
+        l = l * alpha + wave_sum(p);
+        const float weight = DT == MIMIR_KV_I8 ? p * a.c.v_scale[at] : p;
+#pragma unroll
+        for (int c = 0; c < kRowChunks; ++c) acc[c] *= alpha;
+        uint64_t left = __ballot(has);
+        while (left) {
+            constexpr int kAhead = 8;
+            float w[kAhead], v[kAhead][kRowChunks];
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) {
+                const bool any = left != 0;
+                const int i = any ? __builtin_ctzll(left) : 0;
+                const auto row = static_cast<int64_t>(lane_of(static_cast<uint64_t>(at), i));
+                w[u] = __builtin_bit_cast(float, lane_of(__builtin_bit_cast(uint32_t, weight), i));
+#pragma unroll
+                for (int c = 0; c < kRowChunks; ++c) {
+                    const int d = lane + c * kWave;
+                    v[u][c] = any && d < d_all ? element<DT>(a.c.v, row, a.c.stride, d) : 0.f;
+                }
+                if (!any) w[u] = 0.f;
+                left &= left - 1;
+            }
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u)
+#pragma unroll
+                for (int c = 0; c < kRowChunks; ++c) acc[c] += w[u] * v[u][c];
+        }
+        // What is NaN stays NaN: a row that is all NaN is done.
+        bool nan = true;
 #pragma unroll
         for (int c = 0; c < kRowChunks; ++c) {
-            const int d = lane + c * kWave;
-            if (d < a.c.head_dim) acc[c] = acc[c] * alpha + w * element<DT>(a.c.v, at, a.c.stride, d);
+            if (l != l) acc[c] = l;
+            nan = nan && (acc[c] != acc[c] || lane + c * kWave >= d_all);
         }
+        if (__all(nan)) break;
     }
     *m_out = m;
     *l_out = l;

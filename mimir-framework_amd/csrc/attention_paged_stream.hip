@@ -466,6 +466,7 @@ int mimir::paged_stream_launch(mimir_ctx* ctx, const PagedArgs& p, int dtype, in
     const int tiles = rows > kRows && !wide && rows == static_cast<int64_t>(p.b.max_new) * p.group ? 2 : 1;
     PagedRuns a{};
     a.extra = 2 * kStep;  // the queries, the first keys' way in, the sums' way out
+    a.slack = a.extra;
     a.grain = kStep;
     a.block_rows = kRows * tiles;
     a.least_rows = 1;

@@ -308,3 +308,34 @@ def test_agrees_with_the_whole_sequence_core(ctx):
                   heads, d, True)
     _, tol = attention64(q, k, v, 0, True, float(np.float32(1.0) / np.sqrt(np.float32(d))))
     assert (np.abs(got - out.numpy().reshape(got.shape)) <= 2 * tol).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("lens", [[(1, 1500)], [(60, 1500)]])
+def test_nan_in_some_dimensions_and_late_keys(ctx, dtype, lens):
+    """A value that is NaN in one dimension reaches that dimension alone, a key's NaN
+    all of the rows that see it; wherever the rows' keys are cut."""
+    d = 64
+    (n, m), = lens
+    q, kv = case(19, dtype, lens, 1, 4, d)
+    k, v = kv[0]
+    if dtype != "i8":
+        v[300, 0, 9] = np.nan
+    p = Paged(ctx, dtype, lens, 1, d, 16)
+    fill(p, kv)
+    sc = float(np.float32(1.0) / np.sqrt(np.float32(d)))
+    vz = v.copy()
+    vz[300, 0, 9] = 0 if dtype != "i8" else vz[300, 0, 9]
+    want, tol = attention64(q, held(k, dtype), held(vz, dtype), m - n, True, sc)
+    got = attend(ctx, p, q)
+    ok = np.ones(got.shape, bool)
+    if dtype != "i8":
+        ok[:, :, 9] = False
+        assert np.isnan(got[:, :, 9]).all()
+    assert (np.abs(got - want) <= tol)[ok].all()
+    k[m - 1, 0, 3] = np.nan
+    fill(p, kv)
+    got = attend(ctx, p, q)
+    ok[n - 1] = False
+    assert (np.abs(got - want) <= tol)[ok].all()
+    assert np.isnan(got[n - 1]).all()

@@ -26,18 +26,16 @@ constexpr int64_t kStreamRows = 64, kStreamBeside = 32;
 // lanes hold a row, four dimensions each.  ONE: the whole workgroup takes a row at a
 // time, its groups of lanes every so many of the runs (a long sequence's block may have
 // hundreds); else each group a row of its own.  The block's first run, whose descriptor
-// this is, kept what it begins, the others what they go on with.  `parts` workgroups
-// for each descriptor.
+// is the workgroup's, kept what it begins, the others what they go on with.  `parts`
+// workgroups for each descriptor.
 template <int LPR, bool ONE>
-__global__ __launch_bounds__(kBlock) void paged_join(PagedArgs p, PagedRuns a, uint32_t parts) {
+__device__ __forceinline__ void join_rows(const PagedArgs& p, const PagedRuns& a, uint32_t parts, uint32_t block, f4 (*share)[LPR], f2* stats) {
     constexpr int kAhead = 4, kGroups = kBlock / LPR, kEach = ONE ? kGroups : 1, kRowsOf = ONE ? 1 : kGroups;
-    __shared__ f4 share[kGroups][LPR];
-    __shared__ f2 stats[kGroups];
-    const uint32_t first = blockIdx.x / parts;
+    const uint32_t first = block / parts;
     const PagedShared s = a.shared[first];
     if (s.runs <= 1) return;
     const int lane = threadIdx.x % LPR, group = threadIdx.x / LPR, d = p.c.head_dim;
-    for (int row0 = static_cast<int>(blockIdx.x % parts) * kRowsOf; row0 < s.rows; row0 += static_cast<int>(parts) * kRowsOf) {
+    for (int row0 = static_cast<int>(block % parts) * kRowsOf; row0 < s.rows; row0 += static_cast<int>(parts) * kRowsOf) {
         const int row = row0 + (ONE ? 0 : group);
         const bool mine = row < s.rows;
         float m = -1e30f, l = 0.f;
@@ -95,41 +93,55 @@ __global__ __launch_bounds__(kBlock) void paged_join(PagedArgs p, PagedRuns a, u
     }
 }
 
+// Of one launch's blocks, and of another's behind them.
 template <int LPR>
-void launch_join(const PagedArgs& p, const PagedRuns& a, hipStream_t s) {
+__global__ __launch_bounds__(kBlock) void paged_join(PagedArgs p, PagedRuns a, uint32_t parts_a, PagedRuns b, uint32_t parts_b) {
+    constexpr int kGroups = kBlock / LPR;
+    __shared__ f4 share[kGroups][LPR];
+    __shared__ f2 stats[kGroups];
+    const uint32_t of_a = a.runs * parts_a;
+    const bool first = blockIdx.x < of_a;
+    const PagedRuns& r = first ? a : b;
+    const uint32_t parts = first ? parts_a : parts_b, block = first ? blockIdx.x : blockIdx.x - of_a;
+    if (r.many) join_rows<LPR, true>(p, r, parts, block, share, stats);
+    else join_rows<LPR, false>(p, r, parts, block, share, stats);
+}
+
+template <int LPR>
+void launch_join(const PagedArgs& p, const PagedRuns& a, const PagedRuns& b, hipStream_t s) {
     constexpr int kRowsOf = kBlock / LPR;
-    if (a.many) {
-        const unsigned parts = static_cast<unsigned>(std::min(a.part_rows, 8));
-        paged_join<LPR, true><<<a.runs * parts, kBlock, 0, s>>>(p, a, parts);
-    } else {
-        const unsigned parts = static_cast<unsigned>((a.part_rows + kRowsOf - 1) / kRowsOf);
-        paged_join<LPR, false><<<a.runs * parts, kBlock, 0, s>>>(p, a, parts);
-    }
+    const auto parts = [](const PagedRuns& x) {
+        return static_cast<uint32_t>(x.many ? std::min(x.part_rows, 8) : (x.part_rows + kRowsOf - 1) / kRowsOf);
+    };
+    paged_join<LPR><<<a.runs * parts(a) + b.runs * parts(b), kBlock, 0, s>>>(p, a, parts(a), b, parts(b));
+}
+
+// Joins the blocks that several runs had keys of; a launch that cut none has no runs.
+int join(mimir_ctx* ctx, const PagedArgs& p, const PagedRuns& a, const PagedRuns& b) {
+    if (a.runs + b.runs == 0) return MIMIR_OK;
+    if (p.c.head_dim <= 128) launch_join<32>(p, a, b, ctx->stream);
+    else launch_join<64>(p, a, b, ctx->stream);
+    return launched(ctx, "paged_join");
 }
 
 }  // namespace
 
-int64_t mimir::paged_runs(mimir_ctx* ctx, const PagedArgs& p, PagedRuns* a, int64_t runs, int64_t blocks, bool split) {
+int64_t mimir::paged_runs(mimir_ctx* ctx, const PagedArgs& p, PagedRuns* a, int64_t runs, int64_t blocks, bool split, bool beside) {
     // No more than keep to the least length of a run (PagedWalk), by the longest costs.
     const int64_t cost = a->extra + static_cast<int64_t>(p.b.max_len) + (p.causal ? (a->block_rows + p.group - 1) / p.group : 0);
-    runs = std::max<int64_t>(1, std::min(runs, blocks * cost / (a->extra + a->grain) + 1));
+    if (blocks < 1 << 24) runs = std::max<int64_t>(1, std::min(runs, blocks * cost / (a->extra + a->grain) + 1));
     a->apart = p.b.sequences <= kWave;
     a->many = a->part_rows <= 32 && runs > 4 * blocks;
-    const int64_t floats = runs * 2 * paged_part_floats(a->part_rows, p.c.head_dim);
-    const int64_t bytes = runs * static_cast<int64_t>(sizeof(PagedShared)) + floats * 4;
-    char* work = split && bytes <= static_cast<int64_t>(kPagedWorkBytes) ? paged_work(ctx) : nullptr;
+    constexpr size_t kAlone = kPagedWorkBytes - kPagedBesideBytes;
+    const int64_t bytes = runs * static_cast<int64_t>(sizeof(PagedShared)) + runs * 2 * paged_part_floats(a->part_rows, p.c.head_dim) * 4;
+    if (!split || bytes > static_cast<int64_t>(beside ? kPagedBesideBytes : kAlone)) return blocks;
+    char* work = paged_work(ctx);
     if (!work) return blocks;
+    if (beside) work += kAlone;
     a->shared = reinterpret_cast<PagedShared*>(work);
     a->part = reinterpret_cast<float*>(work + runs * sizeof(PagedShared));
     a->runs = static_cast<uint32_t>(runs);
     return runs;
-}
-
-int mimir::paged_join_launch(mimir_ctx* ctx, const PagedArgs& p, const PagedRuns& a) {
-    if (!a.part) return MIMIR_OK;
-    if (p.c.head_dim <= 128) launch_join<32>(p, a, ctx->stream);
-    else launch_join<64>(p, a, ctx->stream);
-    return launched(ctx, "paged_join");
 }
 
 extern "C" int mimir_attention_paged_fwd(mimir_ctx* ctx, const mimir_kv_cache* cache, const mimir_kv_batch* batch,
@@ -164,8 +176,14 @@ extern "C" int mimir_attention_paged_fwd(mimir_ctx* ctx, const mimir_kv_cache* c
     // tokens (or whose rows would suffice for that) has the second alone, which takes any.
     const int64_t rows = static_cast<int64_t>(a.b.max_new) * a.group;
     MIMIR_REQUIRE(ctx, rows <= INT32_MAX, "%s: %lld query rows of a head", what, (long long)rows);
-    if (rows <= kStreamRows || a.c.stride > kPagedBlockStride) return paged_stream_launch(ctx, a, cache->dtype, INT32_MAX);
-    if (a.b.sequences * static_cast<int64_t>(a.b.max_new) <= a.b.tokens) return paged_block_launch(ctx, a, cache->dtype, 1);
-    if (int st = paged_stream_launch(ctx, a, cache->dtype, kStreamBeside)) return st;
-    return paged_block_launch(ctx, a, cache->dtype, kStreamBeside + 1);
+    PagedRuns few{}, others{};
+    if (rows <= kStreamRows || a.c.stride > kPagedBlockStride) {
+        if (int st = paged_stream_launch(ctx, a, cache->dtype, INT32_MAX, false, &few)) return st;
+    } else {
+        const bool both = a.b.sequences * static_cast<int64_t>(a.b.max_new) > a.b.tokens;
+        if (both)
+            if (int st = paged_stream_launch(ctx, a, cache->dtype, kStreamBeside, true, &few)) return st;
+        if (int st = paged_block_launch(ctx, a, cache->dtype, both ? kStreamBeside + 1 : 1, &others)) return st;
+    }
+    return join(ctx, a, few, others);
 }

@@ -421,17 +421,15 @@ __device__ __forceinline__ void row_over_keys(const PagedArgs& a, int s, int kv_
 
 // The host's side (attention_paged_stream.hip, attention_paged_block.hip): sequences
 // of up to `most_rows` query rows a key / value head, and of `least_rows` on.
-int paged_stream_launch(mimir_ctx* ctx, const PagedArgs& p, int dtype, int64_t most_rows);
-int paged_block_launch(mimir_ctx* ctx, const PagedArgs& p, int dtype, int64_t least_rows);
+// What is left to join is in `left` (no runs: nothing).  beside: another launch follows.
+int paged_stream_launch(mimir_ctx* ctx, const PagedArgs& p, int dtype, int64_t most_rows, bool beside, PagedRuns* left);
+int paged_block_launch(mimir_ctx* ctx, const PagedArgs& p, int dtype, int64_t least_rows, PagedRuns* left);
 
 // The widest heads (padded) of the block kernel: its queries' terms are registers.
 constexpr int kPagedBlockStride = 128;
 
-// Joins the blocks that several runs had keys of.
-int paged_join_launch(mimir_ctx* ctx, const PagedArgs& p, const PagedRuns& a);
-
 // Sets up `a` for at most `runs` workgroups in the workspace, or for one per block
 // (`blocks` of them) where that is not to be had or `split` says not to; the grid.
-int64_t paged_runs(mimir_ctx* ctx, const PagedArgs& p, PagedRuns* a, int64_t runs, int64_t blocks, bool split);
+int64_t paged_runs(mimir_ctx* ctx, const PagedArgs& p, PagedRuns* a, int64_t runs, int64_t blocks, bool split, bool beside);
 
 }  // namespace mimir

@@ -99,370 +99,370 @@ __global__ __launch_bounds__(WAVES * kWave, (WAVES / 4 * BlockShape<DT, DP, WAVE
     const uint32_t at = a.runs % kXcds == 0 && gridDim.x == a.runs ? blockIdx.x % kXcds * (a.runs / kXcds) + blockIdx.x / kXcds : blockIdx.x;
     const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave);
     for (PagedWalk walk(p, a, at, &chunk); walk.more();) {
-    int tid = static_cast<int>(threadIdx.x);
-    asm volatile("" : "+v"(tid));  // what follows from it is computed for each block, not held in registers across them
-    const int lane = tid % kWave;
-    const PagedPiece w = walk.next(p, a);
-    if (w.rows <= 0) return;
-    const int k0 = w.k0, k1 = w.k1;
-    const int li = lane % 32, hf = lane / 32;
-    const int wave_rows = min(w.rows - wave * kTile, kTile);  // below 1: a wave that only moves tiles
-    const bool in = li < wave_rows;
-    const int my_row = w.row0 + wave * kTile + max(0, min(li, wave_rows - 1));
-    const int my_end = min(row_end(p, w.seq, min(my_row, w.row0 + w.rows - 1)), k1);
-    const int first_end = uniform(my_end);  // the wave's first row's, none sees fewer
-    const int wave_end = wave_rows > 0 ? min(k1, row_end(p, w.seq, w.row0 + wave * kTile + wave_rows - 1)) : k0;
-    const auto q_row = [&](int row) { return p.q + paged_row(p, p.ld_q, w.seq.first, w.head, row); };
-    const PagedPart part(a, p.c.head_dim, walk.index, w.begins);
-    // Row of the block: its output, or where its sums are kept.
-    const auto out_row = [&](int row) {
-        return w.whole ? p.out + paged_row(p, p.ld_out, w.seq.first, w.head, w.row0 + row)
-                       : part.sums(row);
-    };
+        int tid = static_cast<int>(threadIdx.x);
+        asm volatile("" : "+v"(tid));  // what follows from it is computed for each block, not held in registers across them
+        const int lane = tid % kWave;
+        const PagedPiece w = walk.next(p, a);
+        if (w.rows <= 0) return;
+        const int k0 = w.k0, k1 = w.k1;
+        const int li = lane % 32, hf = lane / 32;
+        const int wave_rows = min(w.rows - wave * kTile, kTile);  // below 1: a wave that only moves tiles
+        const bool in = li < wave_rows;
+        const int my_row = w.row0 + wave * kTile + max(0, min(li, wave_rows - 1));
+        const int my_end = min(row_end(p, w.seq, min(my_row, w.row0 + w.rows - 1)), k1);
+        const int first_end = uniform(my_end);  // the wave's first row's, none sees fewer
+        const int wave_end = wave_rows > 0 ? min(k1, row_end(p, w.seq, w.row0 + wave * kTile + wave_rows - 1)) : k0;
+        const auto q_row = [&](int row) { return p.q + paged_row(p, p.ld_q, w.seq.first, w.head, row); };
+        const PagedPart part(a, p.c.head_dim, walk.index, w.begins);
+        // Row of the block: its output, or where its sums are kept.
+        const auto out_row = [&](int row) {
+            return w.whole ? p.out + paged_row(p, p.ld_out, w.seq.first, w.head, w.row0 + row)
+                           : part.sums(row);
+        };
 
-    // Tiles in, one item (eight dimensions of a key) at a time.
-    const int tiles = (k1 - k0 + kTile - 1) / kTile;
-    const scalar_i32 table = (scalar_i32)(p.b.page_table + w.s * p.b.ld_pages);
-    const int row_bytes = p.c.stride * kElement;
-    const auto pages = static_cast<uint32_t>(p.c.pages);
-    const auto entry_of = [&](int j) { return fastdiv(static_cast<uint32_t>(max(min(j, (k1 - 1) & -kHalf), 0)), p.c.page_div); };
-    const auto there = [&](int j) { return static_cast<uint32_t>(table[entry_of(j)]) < pages; };
-    // Whether a page of these keys is none.
-    bool holes = false;
-    if (tiles > 0) {
-        const int32_t* entries = p.b.page_table + w.s * p.b.ld_pages;
-        const auto last = static_cast<int>(fastdiv(static_cast<uint32_t>(k1 - 1), p.c.page_div));
-        for (int e = static_cast<int>(fastdiv(static_cast<uint32_t>(k0), p.c.page_div)) + lane; e <= last; e += kWave)
-            holes = holes || static_cast<uint32_t>(entries[e]) >= pages;
-        holes = __any(holes);
-    }
-    // A thread's items: eight dimensions of a row.  An item's rows are, for a wave, of
-    // one half of the tile; what lies past a row's dimensions or the half's keys reads
-    // as zeros.
-    constexpr int kLanes = DP == 64 ? 8 : 16;
-    constexpr int kItems = (kTile * kLanes + kThreads - 1) / kThreads;
-    static_assert(kWave / kLanes <= kHalf && kHalf % (kWave / kLanes) == 0, "a wave's rows in one half");
-    static_assert(kItems == 1 || (kItems == 2 && kThreads == kHalf * kLanes), "an item a half");
-    constexpr int kMovers = kItems == 2 ? WAVES : kHalf * kLanes / kWave;  // waves that share a half
-    const int d_mine = 8 * (tid % kLanes);
-    const auto row_of = [&](int n) { return (tid + n * kThreads) / kLanes; };
-    const auto half_of = [&](int n) { return kItems == 2 ? n : wave / kMovers; };
-    const uint32_t off = d_mine < p.c.stride ? static_cast<uint32_t>(row_of(0) % kHalf * row_bytes + d_mine * kElement) : kOutside;
-    const int64_t page_rows = static_cast<int64_t>(p.c.kv_heads) * p.c.page_size, head_rows = static_cast<int64_t>(w.head) * p.c.page_size;
-    const bool mover = kItems == 2 || half_of(0) < 2;
-    // Where an item's half stands, and how many of its keys are there.
-    struct Halves {
-        int page[kItems], slot[kItems], keys[kItems];
-    };
-    const auto find = [&](int t) {
-        Halves g;
-#pragma unroll
-        for (int n = 0; n < kItems; ++n) {
-            const int j = k0 + t * kTile + kHalf * half_of(n), i = max(min(j, (k1 - 1) & -kHalf), 0);
-            const uint32_t entry = fastdiv(static_cast<uint32_t>(i), p.c.page_div);
-            g.page[n] = table[entry];
-            g.slot[n] = i - static_cast<int>(entry) * p.c.page_size;
-            g.keys[n] = max(min(k1 - j, kHalf), 0);
+        // Tiles in, one item (eight dimensions of a key) at a time.
+        const int tiles = (k1 - k0 + kTile - 1) / kTile;
+        const scalar_i32 table = (scalar_i32)(p.b.page_table + w.s * p.b.ld_pages);
+        const int row_bytes = p.c.stride * kElement;
+        const auto pages = static_cast<uint32_t>(p.c.pages);
+        const auto entry_of = [&](int j) { return fastdiv(static_cast<uint32_t>(max(min(j, (k1 - 1) & -kHalf), 0)), p.c.page_div); };
+        const auto there = [&](int j) { return static_cast<uint32_t>(table[entry_of(j)]) < pages; };
+        // Whether a page of these keys is none.
+        bool holes = false;
+        if (tiles > 0) {
+            const int32_t* entries = p.b.page_table + w.s * p.b.ld_pages;
+            const auto last = static_cast<int>(fastdiv(static_cast<uint32_t>(k1 - 1), p.c.page_div));
+            for (int e = static_cast<int>(fastdiv(static_cast<uint32_t>(k0), p.c.page_div)) + lane; e <= last; e += kWave)
+                holes = holes || static_cast<uint32_t>(entries[e]) >= pages;
+            holes = __any(holes);
         }
-        return g;
-    };
-    RowItem<DT> ki[kItems], vi[kItems];
-    float scale[kItems];
-    const int scales = wave % kMovers;  // 8-bit: 0, the keys' scales are this wave's to move, 1, the values'
-    const auto load = [&](const Halves& g) {
-        if (!mover) return;
+        // A thread's items: eight dimensions of a row.  An item's rows are, for a wave, of
+        // one half of the tile; what lies past a row's dimensions or the half's keys reads
+        // as zeros.
+        constexpr int kLanes = DP == 64 ? 8 : 16;
+        constexpr int kItems = (kTile * kLanes + kThreads - 1) / kThreads;
+        static_assert(kWave / kLanes <= kHalf && kHalf % (kWave / kLanes) == 0, "a wave's rows in one half");
+        static_assert(kItems == 1 || (kItems == 2 && kThreads == kHalf * kLanes), "an item a half");
+        constexpr int kMovers = kItems == 2 ? WAVES : kHalf * kLanes / kWave;  // waves that share a half
+        const int d_mine = 8 * (tid % kLanes);
+        const auto row_of = [&](int n) { return (tid + n * kThreads) / kLanes; };
+        const auto half_of = [&](int n) { return kItems == 2 ? n : wave / kMovers; };
+        const uint32_t off = d_mine < p.c.stride ? static_cast<uint32_t>(row_of(0) % kHalf * row_bytes + d_mine * kElement) : kOutside;
+        const int64_t page_rows = static_cast<int64_t>(p.c.kv_heads) * p.c.page_size, head_rows = static_cast<int64_t>(w.head) * p.c.page_size;
+        const bool mover = kItems == 2 || half_of(0) < 2;
+        // Where an item's half stands, and how many of its keys are there.
+        struct Halves {
+            int page[kItems], slot[kItems], keys[kItems];
+        };
+        const auto find = [&](int t) {
+            Halves g;
 #pragma unroll
-        for (int n = 0; n < kItems; ++n) {
-            const bool has = static_cast<uint32_t>(g.page[n]) < pages;
-            const int64_t row = (has ? g.page[n] : 0) * page_rows + head_rows + g.slot[n];
-            const int keys = has ? g.keys[n] : 0;
-            const int64_t at = row * row_bytes;
-            ki[n].load(__builtin_amdgcn_make_buffer_rsrc(p.c.k + at, 0, keys * row_bytes, kBufferWord3), off);
-            vi[n].load(__builtin_amdgcn_make_buffer_rsrc(p.c.v + at, 0, keys * row_bytes, kBufferWord3), off);
-            if constexpr (DT == MIMIR_KV_I8)
-                if (scales < 2)
-                    scale[n] = buffer_f1(buffer_of((scales ? p.c.v_scale : p.c.k_scale) + row, 4 * keys), static_cast<uint32_t>(4 * (lane % kHalf)));
-        }
-    };
-    const auto stash = [&](char* key_buf, char* value_buf) {
-        if (!mover) return;
-#pragma unroll
-        for (int n = 0; n < kItems; ++n) {
-            if (d_mine < DP) {
-                ki[n].stash(key_buf + row_of(n) * Tile::kKeyRow + 2 * d_mine, Tile::kKeyPlane);
-                vi[n].stash(value_buf + row_of(n) * Tile::kValueRow + 2 * d_mine, Tile::kValuePlane);
+            for (int n = 0; n < kItems; ++n) {
+                const int j = k0 + t * kTile + kHalf * half_of(n), i = max(min(j, (k1 - 1) & -kHalf), 0);
+                const uint32_t entry = fastdiv(static_cast<uint32_t>(i), p.c.page_div);
+                g.page[n] = table[entry];
+                g.slot[n] = i - static_cast<int>(entry) * p.c.page_size;
+                g.keys[n] = max(min(k1 - j, kHalf), 0);
             }
-            if constexpr (DT == MIMIR_KV_I8)
-                if (scales < 2 && lane < kHalf)
-                    reinterpret_cast<float*>(key_buf + Tile::kScalesAt)[scales * kTile + half_of(n) * kHalf + lane] = scale[n];
-        }
-    };
-
-    Halves to{};  // of the tile after the one in registers, which is after the one in LDS
-    if (tiles > 0) {
-        load(find(0));
-        to = find(1);
-    }
-    // This lane's query values, times scale * log2(e).
-    Split8 q[kC];
-    {
-        const float* row = q_row(min(my_row, w.row0 + w.rows - 1)) + 8 * hf;
-        const int left = p.c.head_dim - 8 * hf;  // of the row from there on
-        if (p.c.head_dim % 4 == 0) {
-            f4u x[kC][2];
+            return g;
+        };
+        RowItem<DT> ki[kItems], vi[kItems];
+        float scale[kItems];
+        const int scales = wave % kMovers;  // 8-bit: 0, the keys' scales are this wave's to move, 1, the values'
+        const auto load = [&](const Halves& g) {
+            if (!mover) return;
 #pragma unroll
-            for (int c = 0; c < kC; ++c)
-#pragma unroll
-                for (int i = 0; i < 2; ++i)
-                    x[c][i] = 16 * c + 4 * i < left ? reinterpret_cast<const f4u*>(row + 16 * c)[i] : f4u{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int c = 0; c < kC; ++c) {
-                const f4u a = x[c][0] * p.qscale, b = x[c][1] * p.qscale;
-                const float y[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
-                q[c] = split8(y);
-            }
-        } else {
-#pragma unroll
-            for (int c = 0; c < kC; ++c) {
-                float x[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) x[e] = 16 * c + e < left ? row[16 * c + e] * p.qscale : 0.f;
-                q[c] = split8(x);
-            }
-        }
-    }
-
-    f16v o[kDb];
-#pragma unroll
-    for (int d = 0; d < kDb; ++d) o[d] = f16v{};
-    float m_run = -1e30f, l_run = 0.f;
-
-    if (tiles > 0) {
-        stash(lds, values);
-        load(to);
-        to = find(2);
-    }
-    __syncthreads();
-    // A lane's part of a transposed read: key 4 hf + (lane % 16) / 4, dimensions
-    // 16 (lane / 16 % 2) + 4 (lane % 4) on.
-    const int v_lane = (4 * hf + lane % 16 / 4) * Tile::kValueRow + (lane / 16 % 2 * 16 + 4 * (lane % 4)) * 2;
-    f16v s;  // scores of a tile, then its weights
-    // o += V^T P^T over a tile's keys.  Values are read one operand ahead of their
-    // products, and the second half's weights are split beside the first half's.
-    const auto weigh = [&](const char* buf) {
-        const auto read = [&](int i, u4* v) {
-            const char* const at = buf + v_lane + 16 * (i / kDb) * Tile::kValueRow + 64 * (i % kDb);
-#pragma unroll
-            for (int n = 0; n < Tile::kPlanes; ++n) {
-                const u2 x0 = __builtin_bit_cast(u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(at + n * Tile::kValuePlane)));
-                const u2 x1 = __builtin_bit_cast(
-                    u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(at + n * Tile::kValuePlane + 8 * Tile::kValueRow)));
-                v[n] = u4{x0[0], x0[1], x1[0], x1[1]};
+            for (int n = 0; n < kItems; ++n) {
+                const bool has = static_cast<uint32_t>(g.page[n]) < pages;
+                const int64_t row = (has ? g.page[n] : 0) * page_rows + head_rows + g.slot[n];
+                const int keys = has ? g.keys[n] : 0;
+                const int64_t at = row * row_bytes;
+                ki[n].load(__builtin_amdgcn_make_buffer_rsrc(p.c.k + at, 0, keys * row_bytes, kBufferWord3), off);
+                vi[n].load(__builtin_amdgcn_make_buffer_rsrc(p.c.v + at, 0, keys * row_bytes, kBufferWord3), off);
+                if constexpr (DT == MIMIR_KV_I8)
+                    if (scales < 2)
+                        scale[n] = buffer_f1(buffer_of((scales ? p.c.v_scale : p.c.k_scale) + row, 4 * keys), static_cast<uint32_t>(4 * (lane % kHalf)));
             }
         };
-        const auto split = [&](int c) {
-            float x[8];
+        const auto stash = [&](char* key_buf, char* value_buf) {
+            if (!mover) return;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = s[8 * c + e];
-            return split8(x);
+            for (int n = 0; n < kItems; ++n) {
+                if (d_mine < DP) {
+                    ki[n].stash(key_buf + row_of(n) * Tile::kKeyRow + 2 * d_mine, Tile::kKeyPlane);
+                    vi[n].stash(value_buf + row_of(n) * Tile::kValueRow + 2 * d_mine, Tile::kValuePlane);
+                }
+                if constexpr (DT == MIMIR_KV_I8)
+                    if (scales < 2 && lane < kHalf)
+                        reinterpret_cast<float*>(key_buf + Tile::kScalesAt)[scales * kTile + half_of(n) * kHalf + lane] = scale[n];
+            }
         };
-        __builtin_amdgcn_s_setprio(1);
-        u4 v[2][Tile::kPlanes];
-        read(0, v[0]);
-        Split8 pw = split(0), pn;
-#pragma unroll
-        for (int i = 0; i < 2 * kDb; ++i) {
-            if (i + 1 < 2 * kDb) read(i + 1, v[(i + 1) % 2]);
-            if (i == 0) pn = split(1);
-            if (i == kDb) pw = pn;
-            o[i % kDb] = mfma_planes<Tile::kPlanes>(v[i % 2], pw, o[i % kDb]);
+
+        Halves to{};  // of the tile after the one in registers, which is after the one in LDS
+        if (tiles > 0) {
+            load(find(0));
+            to = find(1);
         }
-        if constexpr (Tile::kPlanes == 1) {
-            __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
-            __builtin_amdgcn_sched_group_barrier(0x002, 44, 0);
+        // This lane's query values, times scale * log2(e).
+        Split8 q[kC];
+        {
+            const float* row = q_row(min(my_row, w.row0 + w.rows - 1)) + 8 * hf;
+            const int left = p.c.head_dim - 8 * hf;  // of the row from there on
+            if (p.c.head_dim % 4 == 0) {
+                f4u x[kC][2];
 #pragma unroll
-            for (int i = 0; i < 2 * kDb; ++i) {
-                __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+                for (int c = 0; c < kC; ++c)
 #pragma unroll
-                for (int n = 0; n < 3; ++n) {
-                    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-                    if (i < kDb) __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);
+                    for (int i = 0; i < 2; ++i)
+                        x[c][i] = 16 * c + 4 * i < left ? reinterpret_cast<const f4u*>(row + 16 * c)[i] : f4u{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int c = 0; c < kC; ++c) {
+                    const f4u a = x[c][0] * p.qscale, b = x[c][1] * p.qscale;
+                    const float y[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+                    q[c] = split8(y);
+                }
+            } else {
+#pragma unroll
+                for (int c = 0; c < kC; ++c) {
+                    float x[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) x[e] = 16 * c + e < left ? row[16 * c + e] * p.qscale : 0.f;
+                    q[c] = split8(x);
                 }
             }
         }
-        __builtin_amdgcn_s_setprio(0);
-    };
-    const bool late = kStagger && wave >= WAVES / 2;
-    char *v_old = values, *v_cur = values, *v_next = values + Tile::kValueBytes;
-    for (int t = 0; t < tiles + (kStagger ? 1 : 0); ++t) {
-        const char* cur = lds + (t & 1) * Tile::kKeyBytes;
-        char* const next = lds + ((t + 1) & 1) * Tile::kKeyBytes;
-        const int key = k0 + t * kTile;
-        if (kStagger && late && t > 0 && key - kTile < wave_end) weigh(v_old);
-        const bool active = key < wave_end;
-        if (active) {
-            const auto read = [&](int c, u4* k) {
+
+        f16v o[kDb];
 #pragma unroll
-                for (int n = 0; n < Tile::kPlanes; ++n)
-                    k[n] = *reinterpret_cast<const u4*>(cur + n * Tile::kKeyPlane + li * Tile::kKeyRow + 32 * c + 16 * hf);
+        for (int d = 0; d < kDb; ++d) o[d] = f16v{};
+        float m_run = -1e30f, l_run = 0.f;
+
+        if (tiles > 0) {
+            stash(lds, values);
+            load(to);
+            to = find(2);
+        }
+        __syncthreads();
+        // A lane's part of a transposed read: key 4 hf + (lane % 16) / 4, dimensions
+        // 16 (lane / 16 % 2) + 4 (lane % 4) on.
+        const int v_lane = (4 * hf + lane % 16 / 4) * Tile::kValueRow + (lane / 16 % 2 * 16 + 4 * (lane % 4)) * 2;
+        f16v s;  // scores of a tile, then its weights
+        // o += V^T P^T over a tile's keys.  Values are read one operand ahead of their
+        // products, and the second half's weights are split beside the first half's.
+        const auto weigh = [&](const char* buf) {
+            const auto read = [&](int i, u4* v) {
+                const char* const at = buf + v_lane + 16 * (i / kDb) * Tile::kValueRow + 64 * (i % kDb);
+#pragma unroll
+                for (int n = 0; n < Tile::kPlanes; ++n) {
+                    const u2 x0 = __builtin_bit_cast(u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(at + n * Tile::kValuePlane)));
+                    const u2 x1 = __builtin_bit_cast(
+                        u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(at + n * Tile::kValuePlane + 8 * Tile::kValueRow)));
+                    v[n] = u4{x0[0], x0[1], x1[0], x1[1]};
+                }
             };
-            s = f16v{};
-            __builtin_amdgcn_s_setprio(1);
-            u4 k[2][Tile::kPlanes];
-            read(0, k[0]);
+            const auto split = [&](int c) {
+                float x[8];
 #pragma unroll
-            for (int c = 0; c < kC; ++c) {
-                if (c + 1 < kC) read(c + 1, k[(c + 1) % 2]);
-                s = mfma_planes<Tile::kPlanes>(k[c % 2], q[c], s);
+                for (int e = 0; e < 8; ++e) x[e] = s[8 * c + e];
+                return split8(x);
+            };
+            __builtin_amdgcn_s_setprio(1);
+            u4 v[2][Tile::kPlanes];
+            read(0, v[0]);
+            Split8 pw = split(0), pn;
+#pragma unroll
+            for (int i = 0; i < 2 * kDb; ++i) {
+                if (i + 1 < 2 * kDb) read(i + 1, v[(i + 1) % 2]);
+                if (i == 0) pn = split(1);
+                if (i == kDb) pw = pn;
+                o[i % kDb] = mfma_planes<Tile::kPlanes>(v[i % 2], pw, o[i % kDb]);
             }
             if constexpr (Tile::kPlanes == 1) {
-                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+                __builtin_amdgcn_sched_group_barrier(0x002, 44, 0);
 #pragma unroll
-                for (int c = 0; c < kC; ++c) {
-                    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-                    __builtin_amdgcn_sched_group_barrier(0x008, 3, 0);
+                for (int i = 0; i < 2 * kDb; ++i) {
+                    __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+#pragma unroll
+                    for (int n = 0; n < 3; ++n) {
+                        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                        if (i < kDb) __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);
+                    }
                 }
             }
             __builtin_amdgcn_s_setprio(0);
-        }
-        if (t < tiles) {  // past the last tile the stash rewrites buffers that are not read again
-            stash(next, v_next);
-            load(to);
-        }
-        if (active) {
-            if constexpr (DT == MIMIR_KV_I8) {
+        };
+        const bool late = kStagger && wave >= WAVES / 2;
+        char *v_old = values, *v_cur = values, *v_next = values + Tile::kValueBytes;
+        for (int t = 0; t < tiles + (kStagger ? 1 : 0); ++t) {
+            const char* cur = lds + (t & 1) * Tile::kKeyBytes;
+            char* const next = lds + ((t + 1) & 1) * Tile::kKeyBytes;
+            const int key = k0 + t * kTile;
+            if (kStagger && late && t > 0 && key - kTile < wave_end) weigh(v_old);
+            const bool active = key < wave_end;
+            if (active) {
+                const auto read = [&](int c, u4* k) {
 #pragma unroll
-                for (int r = 0; r < 16; r += 4) {
-                    const f4 x = *reinterpret_cast<const f4*>(cur + Tile::kScalesAt + (2 * r + 4 * hf) * 4);
+                    for (int n = 0; n < Tile::kPlanes; ++n)
+                        k[n] = *reinterpret_cast<const u4*>(cur + n * Tile::kKeyPlane + li * Tile::kKeyRow + 32 * c + 16 * hf);
+                };
+                s = f16v{};
+                __builtin_amdgcn_s_setprio(1);
+                u4 k[2][Tile::kPlanes];
+                read(0, k[0]);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) s[r + e] *= x[e];
+                for (int c = 0; c < kC; ++c) {
+                    if (c + 1 < kC) read(c + 1, k[(c + 1) % 2]);
+                    s = mfma_planes<Tile::kPlanes>(k[c % 2], q[c], s);
                 }
+                if constexpr (Tile::kPlanes == 1) {
+                    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+#pragma unroll
+                    for (int c = 0; c < kC; ++c) {
+                        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+                        __builtin_amdgcn_sched_group_barrier(0x008, 3, 0);
+                    }
+                }
+                __builtin_amdgcn_s_setprio(0);
             }
-            if (holes || key + kTile > first_end) {
-                const bool first = !holes || there(key), second = !holes || there(key + kHalf);
+            if (t < tiles) {  // past the last tile the stash rewrites buffers that are not read again
+                stash(next, v_next);
+                load(to);
+            }
+            if (active) {
+                if constexpr (DT == MIMIR_KV_I8) {
+#pragma unroll
+                    for (int r = 0; r < 16; r += 4) {
+                        const f4 x = *reinterpret_cast<const f4*>(cur + Tile::kScalesAt + (2 * r + 4 * hf) * 4);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) s[r + e] *= x[e];
+                    }
+                }
+                if (holes || key + kTile > first_end) {
+                    const bool first = !holes || there(key), second = !holes || there(key + kHalf);
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const int j = key + 8 * (r / 4) + 4 * hf + r % 4;
+                        s[r] = j < my_end && (r < 8 ? first : second) ? s[r] : -INFINITY;
+                    }
+                }
+                float top = s[0];
+#pragma unroll
+                for (int r = 1; r < 16; ++r) top = fmaxf(top, s[r]);
+                if (__any(top > m_run + kPagedSlack)) {
+                    const float m_new = fmaxf(m_run, fmaxf(top, __shfl_xor(top, 32)));
+                    const float f = __builtin_amdgcn_exp2f(m_run - m_new);
+                    m_run = m_new;
+                    l_run *= f;
+#pragma unroll
+                    for (int d = 0; d < kDb; ++d) o[d] *= f;
+                }
+                float sum = 0.f;
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
-                    const int j = key + 8 * (r / 4) + 4 * hf + r % 4;
-                    s[r] = j < my_end && (r < 8 ? first : second) ? s[r] : -INFINITY;
+                    s[r] = __builtin_amdgcn_exp2f(s[r] - m_run);
+                    sum += s[r];
                 }
-            }
-            float top = s[0];
+                l_run += sum;
+                if constexpr (DT == MIMIR_KV_I8) {
 #pragma unroll
-            for (int r = 1; r < 16; ++r) top = fmaxf(top, s[r]);
-            if (__any(top > m_run + kPagedSlack)) {
-                const float m_new = fmaxf(m_run, fmaxf(top, __shfl_xor(top, 32)));
-                const float f = __builtin_amdgcn_exp2f(m_run - m_new);
-                m_run = m_new;
-                l_run *= f;
+                    for (int r = 0; r < 16; r += 4) {
+                        const f4 x = *reinterpret_cast<const f4*>(cur + Tile::kScalesAt + (kTile + 2 * r + 4 * hf) * 4);
 #pragma unroll
-                for (int d = 0; d < kDb; ++d) o[d] *= f;
-            }
-            float sum = 0.f;
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                s[r] = __builtin_amdgcn_exp2f(s[r] - m_run);
-                sum += s[r];
-            }
-            l_run += sum;
-            if constexpr (DT == MIMIR_KV_I8) {
-#pragma unroll
-                for (int r = 0; r < 16; r += 4) {
-                    const f4 x = *reinterpret_cast<const f4*>(cur + Tile::kScalesAt + (kTile + 2 * r + 4 * hf) * 4);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) s[r + e] *= x[e];
+                        for (int e = 0; e < 4; ++e) s[r + e] *= x[e];
+                    }
                 }
+                if (!late) weigh(v_cur);
             }
-            if (!late) weigh(v_cur);
+            to = find(t + 3);
+            char* const v_free = kStagger ? v_old : v_cur;
+            v_old = v_cur;
+            v_cur = v_next;
+            v_next = kStagger && t == 0 ? values + 2 * Tile::kValueBytes : v_free;
+            __syncthreads();
         }
-        to = find(t + 3);
-        char* const v_free = kStagger ? v_old : v_cur;
-        v_old = v_cur;
-        v_cur = v_next;
-        v_next = kStagger && t == 0 ? values + 2 * Tile::kValueBytes : v_free;
-        __syncthreads();
-    }
 
-    // The wave's rows out: lane (li, hf) holds dimensions 32 d + 8 (r / 4) + 4 hf + r % 4.
-    if (wave_rows <= 0) continue;
-    const float l_tot = l_run + __shfl_xor(l_run, 32);
-    const int row = my_row - w.row0, d_all = p.c.head_dim;
-    float* const out = out_row(row);
-    const float inv = w.whole ? 1.0f / (l_tot + 1e-9f) : 1.0f;
-    const bool vec = d_all % 4 == 0 && (!w.whole || ((reinterpret_cast<uintptr_t>(p.out) & 15) == 0 && p.ld_out % 4 == 0));
-    float check = l_tot - l_tot;
+        // The wave's rows out: lane (li, hf) holds dimensions 32 d + 8 (r / 4) + 4 hf + r % 4.
+        if (wave_rows <= 0) continue;
+        const float l_tot = l_run + __shfl_xor(l_run, 32);
+        const int row = my_row - w.row0, d_all = p.c.head_dim;
+        float* const out = out_row(row);
+        const float inv = w.whole ? 1.0f / (l_tot + 1e-9f) : 1.0f;
+        const bool vec = d_all % 4 == 0 && (!w.whole || ((reinterpret_cast<uintptr_t>(p.out) & 15) == 0 && p.ld_out % 4 == 0));
+        float check = l_tot - l_tot;
 #pragma unroll
-    for (int d = 0; d < kDb; ++d)
+        for (int d = 0; d < kDb; ++d)
 #pragma unroll
-        for (int r = 0; r < 16; r += 4) {
-            const int d0 = 32 * d + 8 * (r / 4) + 4 * hf;
-            const f4 x{o[d][r] * inv, o[d][r + 1] * inv, o[d][r + 2] * inv, o[d][r + 3] * inv};
+            for (int r = 0; r < 16; r += 4) {
+                const int d0 = 32 * d + 8 * (r / 4) + 4 * hf;
+                const f4 x{o[d][r] * inv, o[d][r + 1] * inv, o[d][r + 2] * inv, o[d][r + 3] * inv};
 #pragma unroll
-            for (int e = 0; e < 4; ++e) check += x[e] - x[e];
-            if (!in) continue;
-            if (vec) {
-                if (d0 < d_all) *reinterpret_cast<f4*>(out + d0) = x;
-            } else {
+                for (int e = 0; e < 4; ++e) check += x[e] - x[e];
+                if (!in) continue;
+                if (vec) {
+                    if (d0 < d_all) *reinterpret_cast<f4*>(out + d0) = x;
+                } else {
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (d0 + e < d_all) out[d0 + e] = x[e];
+                    for (int e = 0; e < 4; ++e)
+                        if (d0 + e < d_all) out[d0 + e] = x[e];
+                }
             }
-        }
-    if (!w.whole && in && hf == 0) *part.stat(row) = f2{m_run, l_tot};
-    // Rows that came out NaN or infinite, again in fp32 (as paged_stream).
-    const uint64_t ballot = __ballot(check != check && in);
-    for (uint32_t bad = static_cast<uint32_t>(ballot | ballot >> 32); bad; bad &= bad - 1) {
-        const int r = wave * kTile + __builtin_ctz(bad), full = w.row0 + r;
-        float acc[kRowChunks], m, l;
-        row_over_keys<DT>(p, w.s, w.head, q_row(full), k0, min(k1, row_end(p, w.seq, full)), acc, &m, &l);
-        float* const to = out_row(r);
-        const float f = w.whole ? 1.0f / (l + 1e-9f) : 1.0f;
+        if (!w.whole && in && hf == 0) *part.stat(row) = f2{m_run, l_tot};
+        // Rows that came out NaN or infinite, again in fp32 (as paged_stream).
+        const uint64_t ballot = __ballot(check != check && in);
+        for (uint32_t bad = static_cast<uint32_t>(ballot | ballot >> 32); bad; bad &= bad - 1) {
+            const int r = wave * kTile + __builtin_ctz(bad), full = w.row0 + r;
+            float acc[kRowChunks], m, l;
+            row_over_keys<DT>(p, w.s, w.head, q_row(full), k0, min(k1, row_end(p, w.seq, full)), acc, &m, &l);
+            float* const to = out_row(r);
+            const float f = w.whole ? 1.0f / (l + 1e-9f) : 1.0f;
 #pragma unroll
-        for (int c = 0; c < kRowChunks; ++c)
-            if (lane + c * kWave < d_all) to[lane + c * kWave] = acc[c] * f;
-        if (!w.whole && lane == 0) *part.stat(r) = f2{m, l};
-    }
+            for (int c = 0; c < kRowChunks; ++c)
+                if (lane + c * kWave < d_all) to[lane + c * kWave] = acc[c] * f;
+            if (!w.whole && lane == 0) *part.stat(r) = f2{m, l};
+        }
     }
 }
 
 template <int DT, int DP, int WAVES>
-int launch(mimir_ctx* ctx, const PagedArgs& p, PagedRuns a) {
+int launch(mimir_ctx* ctx, const PagedArgs& p, PagedRuns a, PagedRuns* left) {
     a.block_rows = a.part_rows = WAVES * kTile;
     const int64_t rows = static_cast<int64_t>(p.b.max_new) * p.group;
     a.row_blocks = static_cast<int32_t>((rows + a.block_rows - 1) / a.block_rows);
     const int64_t blocks = static_cast<int64_t>(p.b.sequences) * p.c.kv_heads * a.row_blocks;
     const int64_t runs = ctx->tune.paged_runs > 0 ? ctx->tune.paged_runs : 256 * BlockShape<DT, DP, WAVES>::kResident;
-    const int64_t grid = paged_runs(ctx, p, &a, runs, blocks, true);
+    const int64_t grid = paged_runs(ctx, p, &a, runs, blocks, true, false);
     MIMIR_REQUIRE(ctx, dispatch_fits(grid, WAVES * kWave), "paged attention: grid of %lld workgroups exceeds the limit",
                   (long long)grid);
     paged_block<DT, DP, WAVES><<<static_cast<unsigned>(grid), WAVES * kWave, 0, ctx->stream>>>(p, a);
-    if (int st = launched(ctx, "paged_block")) return st;
-    return paged_join_launch(ctx, p, a);
+    *left = a;
+    return launched(ctx, "paged_block");
 }
 
 template <int DT, int DP>
-int launch_waves(mimir_ctx* ctx, const PagedArgs& p, const PagedRuns& a) {
+int launch_waves(mimir_ctx* ctx, const PagedArgs& p, const PagedRuns& a, PagedRuns* left) {
     int waves = static_cast<int64_t>(p.b.max_new) * p.group <= 4 * kTile ? 4 : 8;
     if (ctx->tune.attn_waves == 4 || ctx->tune.attn_waves == 8) waves = ctx->tune.attn_waves;
-    return waves == 4 ? launch<DT, DP, 4>(ctx, p, a) : launch<DT, DP, 8>(ctx, p, a);
+    return waves == 4 ? launch<DT, DP, 4>(ctx, p, a, left) : launch<DT, DP, 8>(ctx, p, a, left);
 }
 
 template <int DT>
-int launch_dim(mimir_ctx* ctx, const PagedArgs& p, const PagedRuns& a) {
-    if (p.c.stride <= 64) return launch_waves<DT, 64>(ctx, p, a);
-    if (p.c.stride <= 96) return launch_waves<DT, 96>(ctx, p, a);
-    return launch_waves<DT, 128>(ctx, p, a);
+int launch_dim(mimir_ctx* ctx, const PagedArgs& p, const PagedRuns& a, PagedRuns* left) {
+    if (p.c.stride <= 64) return launch_waves<DT, 64>(ctx, p, a, left);
+    if (p.c.stride <= 96) return launch_waves<DT, 96>(ctx, p, a, left);
+    return launch_waves<DT, 128>(ctx, p, a, left);
 }
 
 }  // namespace
 
-int mimir::paged_block_launch(mimir_ctx* ctx, const PagedArgs& p, int dtype, int64_t least_rows) {
+int mimir::paged_block_launch(mimir_ctx* ctx, const PagedArgs& p, int dtype, int64_t least_rows, PagedRuns* left) {
     PagedRuns a{};
     a.extra = 4 * kTile;
     a.slack = 8 * kTile;
     a.grain = kTile;
     a.least_rows = static_cast<int32_t>(least_rows);
     a.most_rows = INT32_MAX;
-    if (dtype == MIMIR_KV_F32) return launch_dim<MIMIR_KV_F32>(ctx, p, a);
-    if (dtype == MIMIR_KV_BF16) return launch_dim<MIMIR_KV_BF16>(ctx, p, a);
-    return launch_dim<MIMIR_KV_I8>(ctx, p, a);
+    if (dtype == MIMIR_KV_F32) return launch_dim<MIMIR_KV_F32>(ctx, p, a, left);
+    if (dtype == MIMIR_KV_BF16) return launch_dim<MIMIR_KV_BF16>(ctx, p, a, left);
+    return launch_dim<MIMIR_KV_I8>(ctx, p, a, left);
 }

@@ -140,296 +140,296 @@ __global__ __launch_bounds__(kStreamWaves * kWave, stream_waves(DT, DP, TILES)) 
     __shared__ PagedChunk chunk;
     const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave);
     for (PagedWalk walk(p, a, blockIdx.x, &chunk); walk.more();) {
-    int tid = static_cast<int>(threadIdx.x);
-    asm volatile("" : "+v"(tid));  // what follows from it is computed for each block, not held in registers across them
-    const int lane = tid % kWave, li = lane % 16, hg = lane / 16;
-    const PagedPiece w = walk.next(p, a);
-    if (w.rows <= 0) return;
-    const int k0 = w.k0, k1 = w.k1;
-    int my_row[R], my_end[R];
-#pragma unroll
-    for (int n = 0; n < R; ++n) {
-        my_row[n] = w.row0 + min(kRows * n + li, w.rows - 1);
-        my_end[n] = min(row_end(p, w.seq, my_row[n]), k1);
-    }
-    const auto q_row = [&](int row) { return p.q + paged_row(p, p.ld_q, w.seq.first, w.head, row); };
-    // The queries' loads go out ahead of the first keys', their terms follow those.
-    constexpr int kOwn = (kSteps + kStreamWaves - 1) / kStreamWaves;
-    float qx[R][kOwn][8];
-#pragma unroll
-    for (int n = 0; n < R; ++n) {
-        const float* row = q_row(my_row[n]);
-#pragma unroll
-        for (int i = 0; i < kOwn; ++i)
-            if (p.c.head_dim % 4 == 0) {
-#pragma unroll
-                for (int e = 0; e < 8; e += 4) {
-                    const int d = K::dim(wave + i * kStreamWaves, hg, e);
-                    const f4u x = d < p.c.head_dim ? *reinterpret_cast<const f4u*>(row + d) : f4u{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                    for (int u = 0; u < 4; ++u) qx[n][i][e + u] = x[u];
-                }
-            } else {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const int d = K::dim(wave + i * kStreamWaves, hg, e);
-                    qx[n][i][e] = d < p.c.head_dim ? row[d] : 0.f;
-                }
-            }
-    }
-
-    // Where the halves of a step stand; one without a page (or past the keys) takes
-    // the first page's address, and its keys count as unseen.
-    struct Step {
-        int page[H], slot[H];
-        __device__ __forceinline__ bool has(int u, const KvView& c) const { return page[u] >= 0 && page[u] < c.pages; }
-        // Row of the cache.
-        __device__ __forceinline__ int64_t at(int u, const KvView& c, int head) const {
-            return (static_cast<int64_t>(has(u, c) ? page[u] : 0) * c.kv_heads + head) * c.page_size + slot[u];
-        }
-    };
-    // The table through scalar loads: a vector load's wait would be one for the keys
-    // and values in flight before it too.
-    const scalar_i32 table = (scalar_i32)(p.b.page_table + w.s * p.b.ld_pages);
-    const auto find = [&](int key) {
-        Step st;
-#pragma unroll
-        for (int u = 0; u < H; ++u) {
-            const int j = key + kHalf * u;
-            const int i = min(j, (k1 - 1) & -kHalf);
-            const uint32_t entry = fastdiv(static_cast<uint32_t>(i), p.c.page_div);
-            st.page[u] = j < k1 ? table[entry] : -1;
-            st.slot[u] = i - static_cast<int>(entry) * p.c.page_size;
-        }
-        return st;
-    };
-    const int row_bytes = p.c.stride * K::kBytes;
-    // A half's rows; `keys` of them are there, the others read as zeros.
-    const auto half_rows = [&](char* base, int64_t at, int keys) {
-        return __builtin_amdgcn_make_buffer_rsrc(base + at * row_bytes, 0, keys * row_bytes, kBufferWord3);
-    };
-    uint32_t k_off[K::kVecs];
-#pragma unroll
-    for (int v = 0; v < K::kVecs; ++v)
-        k_off[v] = static_cast<uint32_t>((li * p.c.stride + min(K::first(v, hg), p.c.stride - 16 / K::kBytes)) * K::kBytes);
-    const uint32_t v_off = static_cast<uint32_t>((4 * hg * p.c.stride + min(li * ND, p.c.stride - ND)) * K::kBytes);
-
-    u4 kr[H][K::kVecs];
-    Values<DT, ND> vr[H / 2];
-    f4 ks[H], vs[H];
-    const auto load_k = [&](const Step& st) {
-#pragma unroll
-        for (int u = 0; u < H; ++u) {
-            const int64_t at = st.at(u, p.c, w.head);
-            const __amdgpu_buffer_rsrc_t rows = half_rows(p.c.k, at, kHalf);
-#pragma unroll
-            for (int v = 0; v < K::kVecs; ++v) kr[u][v] = __builtin_amdgcn_raw_buffer_load_b128(rows, k_off[v], 0, kNt);
-            if constexpr (DT == MIMIR_KV_I8) ks[u] = *reinterpret_cast<const f4*>(p.c.k_scale + at + 4 * hg);
-        }
-    };
-    const auto load_v = [&](const Step& st, int key_of) {
-#pragma unroll
-        for (int u = 0; u < H; ++u) {
-            const int64_t at = st.at(u, p.c, w.head);
-            const int keys = st.has(u, p.c) ? min(k1 - (key_of + kHalf * u), kHalf) : 0;
-            const __amdgpu_buffer_rsrc_t rows = half_rows(p.c.v, at, keys);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) vr[u / 2].load(4 * (u % 2) + e, rows, v_off, e * row_bytes);
-            if constexpr (DT == MIMIR_KV_I8) vs[u] = buffer_f4(buffer_of(p.c.v_scale + at, 4 * keys), static_cast<uint32_t>(16 * hg));
-        }
-    };
-
-    f4r o[R][ND];
-    float m_run[R], l_run[R];  // the max is the row's, the sum this lane's share
-#pragma unroll
-    for (int n = 0; n < R; ++n) {
-        m_run[n] = -1e30f;
-        l_run[n] = 0.f;
-#pragma unroll
-        for (int t = 0; t < ND; ++t) o[n][t] = f4r{0.f, 0.f, 0.f, 0.f};
-    }
-
-    constexpr int kKeys = kHalf * H, kStep = kKeys * kStreamWaves;
-    int key = k0 + wave * kKeys;
-    Step st{}, nx{}, after{};  // this step's, and the next two's, found a step ahead of their loads
-    if (key < k1) {
-        st = find(key);
-        load_k(st);
-        load_v(st, key);
-        nx = find(key + kStep);
-    }
-    __syncthreads();  // the last block's sums and flags are read
-    if (tid == 0) bad = 0;
-#pragma unroll
-    for (int i = 0; i < kOwn; ++i) {
-        const int c = wave + i * kStreamWaves;
-        if (c >= kSteps) break;
+        int tid = static_cast<int>(threadIdx.x);
+        asm volatile("" : "+v"(tid));  // what follows from it is computed for each block, not held in registers across them
+        const int lane = tid % kWave, li = lane % 16, hg = lane / 16;
+        const PagedPiece w = walk.next(p, a);
+        if (w.rows <= 0) return;
+        const int k0 = w.k0, k1 = w.k1;
+        int my_row[R], my_end[R];
 #pragma unroll
         for (int n = 0; n < R; ++n) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) qx[n][i][e] *= p.qscale;
-            const Split8 x = split8(qx[n][i]);
-            u4* const to = q_lds + 3 * (n * kSteps + c) * kWave + lane;
-            to[0] = x.h;
-            to[kWave] = x.m;
-            to[2 * kWave] = x.l;
+            my_row[n] = w.row0 + min(kRows * n + li, w.rows - 1);
+            my_end[n] = min(row_end(p, w.seq, my_row[n]), k1);
         }
-    }
-    __syncthreads();
-    // One step.  more: the next one's loads are issued in between, K's once the scores
-    // have read this one's, V's at the end; compiled apart from the last step, so that
-    // the waits for loads in flight count them.
-    const auto step = [&](auto more) {
-        int at = lane;
-        asm volatile("" : "+v"(at));  // read here in each step, not held in registers across them
-        const u4* const mine = q_lds + at;
-        f4r s[R][H];
+        const auto q_row = [&](int row) { return p.q + paged_row(p, p.ld_q, w.seq.first, w.head, row); };
+        // The queries' loads go out ahead of the first keys', their terms follow those.
+        constexpr int kOwn = (kSteps + kStreamWaves - 1) / kStreamWaves;
+        float qx[R][kOwn][8];
 #pragma unroll
-        for (int n = 0; n < R; ++n)
+        for (int n = 0; n < R; ++n) {
+            const float* row = q_row(my_row[n]);
 #pragma unroll
-            for (int u = 0; u < H; ++u) s[n][u] = f4r{0.f, 0.f, 0.f, 0.f};
+            for (int i = 0; i < kOwn; ++i)
+                if (p.c.head_dim % 4 == 0) {
 #pragma unroll
-        for (int c = 0; c < kSteps; ++c) {
-            typename K::Operand k[H];
+                    for (int e = 0; e < 8; e += 4) {
+                        const int d = K::dim(wave + i * kStreamWaves, hg, e);
+                        const f4u x = d < p.c.head_dim ? *reinterpret_cast<const f4u*>(row + d) : f4u{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int u = 0; u < H; ++u) k[u] = K::operand(kr[u], c);
+                        for (int u = 0; u < 4; ++u) qx[n][i][e + u] = x[u];
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const int d = K::dim(wave + i * kStreamWaves, hg, e);
+                        qx[n][i][e] = d < p.c.head_dim ? row[d] : 0.f;
+                    }
+                }
+        }
+
+        // Where the halves of a step stand; one without a page (or past the keys) takes
+        // the first page's address, and its keys count as unseen.
+        struct Step {
+            int page[H], slot[H];
+            __device__ __forceinline__ bool has(int u, const KvView& c) const { return page[u] >= 0 && page[u] < c.pages; }
+            // Row of the cache.
+            __device__ __forceinline__ int64_t at(int u, const KvView& c, int head) const {
+                return (static_cast<int64_t>(has(u, c) ? page[u] : 0) * c.kv_heads + head) * c.page_size + slot[u];
+            }
+        };
+        // The table through scalar loads: a vector load's wait would be one for the keys
+        // and values in flight before it too.
+        const scalar_i32 table = (scalar_i32)(p.b.page_table + w.s * p.b.ld_pages);
+        const auto find = [&](int key) {
+            Step st;
+#pragma unroll
+            for (int u = 0; u < H; ++u) {
+                const int j = key + kHalf * u;
+                const int i = min(j, (k1 - 1) & -kHalf);
+                const uint32_t entry = fastdiv(static_cast<uint32_t>(i), p.c.page_div);
+                st.page[u] = j < k1 ? table[entry] : -1;
+                st.slot[u] = i - static_cast<int>(entry) * p.c.page_size;
+            }
+            return st;
+        };
+        const int row_bytes = p.c.stride * K::kBytes;
+        // A half's rows; `keys` of them are there, the others read as zeros.
+        const auto half_rows = [&](char* base, int64_t at, int keys) {
+            return __builtin_amdgcn_make_buffer_rsrc(base + at * row_bytes, 0, keys * row_bytes, kBufferWord3);
+        };
+        uint32_t k_off[K::kVecs];
+#pragma unroll
+        for (int v = 0; v < K::kVecs; ++v)
+            k_off[v] = static_cast<uint32_t>((li * p.c.stride + min(K::first(v, hg), p.c.stride - 16 / K::kBytes)) * K::kBytes);
+        const uint32_t v_off = static_cast<uint32_t>((4 * hg * p.c.stride + min(li * ND, p.c.stride - ND)) * K::kBytes);
+
+        u4 kr[H][K::kVecs];
+        Values<DT, ND> vr[H / 2];
+        f4 ks[H], vs[H];
+        const auto load_k = [&](const Step& st) {
+#pragma unroll
+            for (int u = 0; u < H; ++u) {
+                const int64_t at = st.at(u, p.c, w.head);
+                const __amdgpu_buffer_rsrc_t rows = half_rows(p.c.k, at, kHalf);
+#pragma unroll
+                for (int v = 0; v < K::kVecs; ++v) kr[u][v] = __builtin_amdgcn_raw_buffer_load_b128(rows, k_off[v], 0, kNt);
+                if constexpr (DT == MIMIR_KV_I8) ks[u] = *reinterpret_cast<const f4*>(p.c.k_scale + at + 4 * hg);
+            }
+        };
+        const auto load_v = [&](const Step& st, int key_of) {
+#pragma unroll
+            for (int u = 0; u < H; ++u) {
+                const int64_t at = st.at(u, p.c, w.head);
+                const int keys = st.has(u, p.c) ? min(k1 - (key_of + kHalf * u), kHalf) : 0;
+                const __amdgpu_buffer_rsrc_t rows = half_rows(p.c.v, at, keys);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) vr[u / 2].load(4 * (u % 2) + e, rows, v_off, e * row_bytes);
+                if constexpr (DT == MIMIR_KV_I8) vs[u] = buffer_f4(buffer_of(p.c.v_scale + at, 4 * keys), static_cast<uint32_t>(16 * hg));
+            }
+        };
+
+        f4r o[R][ND];
+        float m_run[R], l_run[R];  // the max is the row's, the sum this lane's share
+#pragma unroll
+        for (int n = 0; n < R; ++n) {
+            m_run[n] = -1e30f;
+            l_run[n] = 0.f;
+#pragma unroll
+            for (int t = 0; t < ND; ++t) o[n][t] = f4r{0.f, 0.f, 0.f, 0.f};
+        }
+
+        constexpr int kKeys = kHalf * H, kStep = kKeys * kStreamWaves;
+        int key = k0 + wave * kKeys;
+        Step st{}, nx{}, after{};  // this step's, and the next two's, found a step ahead of their loads
+        if (key < k1) {
+            st = find(key);
+            load_k(st);
+            load_v(st, key);
+            nx = find(key + kStep);
+        }
+        __syncthreads();  // the last block's sums and flags are read
+        if (tid == 0) bad = 0;
+#pragma unroll
+        for (int i = 0; i < kOwn; ++i) {
+            const int c = wave + i * kStreamWaves;
+            if (c >= kSteps) break;
 #pragma unroll
             for (int n = 0; n < R; ++n) {
-                const u4* const x = mine + 3 * (n * kSteps + c) * kWave;
-                const Split8 q{x[0], x[kWave], x[2 * kWave]};
 #pragma unroll
-                for (int u = 0; u < H; ++u) s[n][u] = mfma16_split(k[u], q, s[n][u]);
+                for (int e = 0; e < 8; ++e) qx[n][i][e] *= p.qscale;
+                const Split8 x = split8(qx[n][i]);
+                u4* const to = q_lds + 3 * (n * kSteps + c) * kWave + lane;
+                to[0] = x.h;
+                to[kWave] = x.m;
+                to[2 * kWave] = x.l;
             }
-            if constexpr (DT == MIMIR_KV_F32) __builtin_amdgcn_sched_barrier(0);  // few terms at a time
         }
-        if constexpr (DT == MIMIR_KV_I8) {
+        __syncthreads();
+        // One step.  more: the next one's loads are issued in between, K's once the scores
+        // have read this one's, V's at the end; compiled apart from the last step, so that
+        // the waits for loads in flight count them.
+        const auto step = [&](auto more) {
+            int at = lane;
+            asm volatile("" : "+v"(at));  // read here in each step, not held in registers across them
+            const u4* const mine = q_lds + at;
+            f4r s[R][H];
 #pragma unroll
             for (int n = 0; n < R; ++n)
 #pragma unroll
-                for (int u = 0; u < H; ++u)
+                for (int u = 0; u < H; ++u) s[n][u] = f4r{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) s[n][u][r] *= ks[u][r];
-        }
-        if constexpr (decltype(more)::value) {
-            load_k(nx);
-            after = find(key + 2 * kStep);  // here, where no LDS read waits for it
-        }
+            for (int c = 0; c < kSteps; ++c) {
+                typename K::Operand k[H];
+#pragma unroll
+                for (int u = 0; u < H; ++u) k[u] = K::operand(kr[u], c);
+#pragma unroll
+                for (int n = 0; n < R; ++n) {
+                    const u4* const x = mine + 3 * (n * kSteps + c) * kWave;
+                    const Split8 q{x[0], x[kWave], x[2 * kWave]};
+#pragma unroll
+                    for (int u = 0; u < H; ++u) s[n][u] = mfma16_split(k[u], q, s[n][u]);
+                }
+                if constexpr (DT == MIMIR_KV_F32) __builtin_amdgcn_sched_barrier(0);  // few terms at a time
+            }
+            if constexpr (DT == MIMIR_KV_I8) {
+#pragma unroll
+                for (int n = 0; n < R; ++n)
+#pragma unroll
+                    for (int u = 0; u < H; ++u)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) s[n][u][r] *= ks[u][r];
+            }
+            if constexpr (decltype(more)::value) {
+                load_k(nx);
+                after = find(key + 2 * kStep);  // here, where no LDS read waits for it
+            }
 
-        bool holes = false;
+            bool holes = false;
 #pragma unroll
-        for (int u = 0; u < H; ++u) holes = holes || !st.has(u, p.c);
-        Split8 pw[R][H / 2];
+            for (int u = 0; u < H; ++u) holes = holes || !st.has(u, p.c);
+            Split8 pw[R][H / 2];
 #pragma unroll
-        for (int n = 0; n < R; ++n) {
-            float x[4 * H];
+            for (int n = 0; n < R; ++n) {
+                float x[4 * H];
 #pragma unroll
-            for (int e = 0; e < 4 * H; ++e) x[e] = s[n][e / 4][e % 4];
-            // Rows whose keys end inside the step, and halves that are not there: the
-            // weights are 0 (and values of keys that no row sees were read as zeros).
-            if (holes || __any(key + kKeys > my_end[n])) {
+                for (int e = 0; e < 4 * H; ++e) x[e] = s[n][e / 4][e % 4];
+                // Rows whose keys end inside the step, and halves that are not there: the
+                // weights are 0 (and values of keys that no row sees were read as zeros).
+                if (holes || __any(key + kKeys > my_end[n])) {
+#pragma unroll
+                    for (int e = 0; e < 4 * H; ++e) {
+                        const int u = e / 4, j = key + kHalf * u + 4 * hg + e % 4;
+                        x[e] = st.has(u, p.c) && j < my_end[n] ? x[e] : -INFINITY;
+                    }
+                }
+                float top = x[0];
+#pragma unroll
+                for (int e = 1; e < 4 * H; ++e) top = fmaxf(top, x[e]);
+                if (__any(top > m_run[n] + kPagedSlack)) {
+                    top = fmaxf(top, __shfl_xor(top, 16));
+                    top = fmaxf(top, __shfl_xor(top, 32));
+                    const float m_new = fmaxf(m_run[n], top);
+                    const float f = __builtin_amdgcn_exp2f(m_run[n] - m_new);
+                    m_run[n] = m_new;
+                    l_run[n] *= f;
+#pragma unroll
+                    for (int t = 0; t < ND; ++t) o[n][t] *= f;
+                }
 #pragma unroll
                 for (int e = 0; e < 4 * H; ++e) {
-                    const int u = e / 4, j = key + kHalf * u + 4 * hg + e % 4;
-                    x[e] = st.has(u, p.c) && j < my_end[n] ? x[e] : -INFINITY;
+                    x[e] = __builtin_amdgcn_exp2f(x[e] - m_run[n]);
+                    l_run[n] += x[e];
+                    if constexpr (DT == MIMIR_KV_I8) x[e] *= vs[e / 4][e % 4];
                 }
-            }
-            float top = x[0];
 #pragma unroll
-            for (int e = 1; e < 4 * H; ++e) top = fmaxf(top, x[e]);
-            if (__any(top > m_run[n] + kPagedSlack)) {
-                top = fmaxf(top, __shfl_xor(top, 16));
-                top = fmaxf(top, __shfl_xor(top, 32));
-                const float m_new = fmaxf(m_run[n], top);
-                const float f = __builtin_amdgcn_exp2f(m_run[n] - m_new);
-                m_run[n] = m_new;
-                l_run[n] *= f;
-#pragma unroll
-                for (int t = 0; t < ND; ++t) o[n][t] *= f;
+                for (int h = 0; h < H / 2; ++h) pw[n][h] = split8(x + 8 * h);
             }
 #pragma unroll
-            for (int e = 0; e < 4 * H; ++e) {
-                x[e] = __builtin_amdgcn_exp2f(x[e] - m_run[n]);
-                l_run[n] += x[e];
-                if constexpr (DT == MIMIR_KV_I8) x[e] *= vs[e / 4][e % 4];
-            }
+            for (int h = 0; h < H / 2; ++h)
 #pragma unroll
-            for (int h = 0; h < H / 2; ++h) pw[n][h] = split8(x + 8 * h);
+                for (int t = 0; t < ND; ++t) {
+                    const auto v = vr[h].operand(t);
+#pragma unroll
+                    for (int n = 0; n < R; ++n) o[n][t] = mfma16_split(v, pw[n][h], o[n][t]);
+                    if constexpr (DT == MIMIR_KV_F32)
+                        if (t % 2 == 1) __builtin_amdgcn_sched_barrier(0);
+                }
+            if constexpr (decltype(more)::value) load_v(nx, key + kStep);
+        };
+        for (; key + kStep < k1; key += kStep) {
+            step(std::true_type{});
+            st = nx;
+            nx = after;
         }
-#pragma unroll
-        for (int h = 0; h < H / 2; ++h)
-#pragma unroll
-            for (int t = 0; t < ND; ++t) {
-                const auto v = vr[h].operand(t);
-#pragma unroll
-                for (int n = 0; n < R; ++n) o[n][t] = mfma16_split(v, pw[n][h], o[n][t]);
-                if constexpr (DT == MIMIR_KV_F32)
-                    if (t % 2 == 1) __builtin_amdgcn_sched_barrier(0);
-            }
-        if constexpr (decltype(more)::value) load_v(nx, key + kStep);
-    };
-    for (; key + kStep < k1; key += kStep) {
-        step(std::true_type{});
-        st = nx;
-        nx = after;
-    }
-    if (key < k1) step(std::false_type{});
+        if (key < k1) step(std::false_type{});
 
-    // The waves' shares of the rows.  Lane (li, hg) holds dimensions (4 hg + r) ND + t.
-    __syncthreads();
+        // The waves' shares of the rows.  Lane (li, hg) holds dimensions (4 hg + r) ND + t.
+        __syncthreads();
 #pragma unroll
-    for (int n = 0; n < R; ++n) {
-        l_run[n] += __shfl_xor(l_run[n], 16);
-        l_run[n] += __shfl_xor(l_run[n], 32);
-        float* const to = share[wave][kRows * n + li];
+        for (int n = 0; n < R; ++n) {
+            l_run[n] += __shfl_xor(l_run[n], 16);
+            l_run[n] += __shfl_xor(l_run[n], 32);
+            float* const to = share[wave][kRows * n + li];
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
+            for (int r = 0; r < 4; ++r)
 #pragma unroll
-            for (int t = 0; t < ND; ++t) to[(4 * hg + r) * ND + t] = o[n][t][r];
-        if (hg == 0) {
-            to[DP] = m_run[n];
-            to[DP + 1] = l_run[n];
+                for (int t = 0; t < ND; ++t) to[(4 * hg + r) * ND + t] = o[n][t][r];
+            if (hg == 0) {
+                to[DP] = m_run[n];
+                to[DP + 1] = l_run[n];
+            }
         }
-    }
-    __syncthreads();
-    const auto out_row = [&](int row) { return p.out + paged_row(p, p.ld_out, w.seq.first, w.head, w.row0 + row); };
-    const PagedPart part(a, p.c.head_dim, walk.index, w.begins);
-    for (int x = tid; x < w.rows * p.c.head_dim; x += kStreamWaves * kWave) {
-        const int row = x / p.c.head_dim, d = x % p.c.head_dim;
-        float m = share[0][row][DP];
+        __syncthreads();
+        const auto out_row = [&](int row) { return p.out + paged_row(p, p.ld_out, w.seq.first, w.head, w.row0 + row); };
+        const PagedPart part(a, p.c.head_dim, walk.index, w.begins);
+        for (int x = tid; x < w.rows * p.c.head_dim; x += kStreamWaves * kWave) {
+            const int row = x / p.c.head_dim, d = x % p.c.head_dim;
+            float m = share[0][row][DP];
 #pragma unroll
-        for (int v = 1; v < kStreamWaves; ++v) m = fmaxf(m, share[v][row][DP]);
-        float l = 0.f, sum = 0.f;
+            for (int v = 1; v < kStreamWaves; ++v) m = fmaxf(m, share[v][row][DP]);
+            float l = 0.f, sum = 0.f;
 #pragma unroll
-        for (int v = 0; v < kStreamWaves; ++v) {
-            const float f = __builtin_amdgcn_exp2f(share[v][row][DP] - m);
-            l += share[v][row][DP + 1] * f;
-            sum += share[v][row][d] * f;
+            for (int v = 0; v < kStreamWaves; ++v) {
+                const float f = __builtin_amdgcn_exp2f(share[v][row][DP] - m);
+                l += share[v][row][DP + 1] * f;
+                sum += share[v][row][d] * f;
+            }
+            if (!(fabsf(sum) < INFINITY) || !(l < INFINITY)) atomicOr(&bad, 1u << row);
+            if (w.whole) {
+                out_row(row)[d] = sum * (1.0f / (l + 1e-9f));
+            } else {
+                part.sums(row)[d] = sum;
+                if (d == 0) *part.stat(row) = f2{m, l};
+            }
         }
-        if (!(fabsf(sum) < INFINITY) || !(l < INFINITY)) atomicOr(&bad, 1u << row);
-        if (w.whole) {
-            out_row(row)[d] = sum * (1.0f / (l + 1e-9f));
-        } else {
-            part.sums(row)[d] = sum;
-            if (d == 0) *part.stat(row) = f2{m, l};
-        }
-    }
-    __syncthreads();
-    // Rows that came out NaN or infinite, again in fp32: an operand had no bf16 split
-    // (split.hpp), or a value that the row does not see is not finite.
-    if (bad == 0) continue;
-    for (int row = wave; row < w.rows; row += kStreamWaves) {
-        if (!(bad >> row & 1)) continue;
-        float acc[kRowChunks], m, l;
-        row_over_keys<DT>(p, w.s, w.head, q_row(w.row0 + row), k0, min(k1, row_end(p, w.seq, w.row0 + row)), acc, &m, &l);
-        const float inv = w.whole ? 1.0f / (l + 1e-9f) : 1.0f;
-        float* out = w.whole ? out_row(row) : part.sums(row);
+        __syncthreads();
+        // Rows that came out NaN or infinite, again in fp32: an operand had no bf16 split
+        // (split.hpp), or a value that the row does not see is not finite.
+        if (bad == 0) continue;
+        for (int row = wave; row < w.rows; row += kStreamWaves) {
+            if (!(bad >> row & 1)) continue;
+            float acc[kRowChunks], m, l;
+            row_over_keys<DT>(p, w.s, w.head, q_row(w.row0 + row), k0, min(k1, row_end(p, w.seq, w.row0 + row)), acc, &m, &l);
+            const float inv = w.whole ? 1.0f / (l + 1e-9f) : 1.0f;
+            float* out = w.whole ? out_row(row) : part.sums(row);
 #pragma unroll
-        for (int c = 0; c < kRowChunks; ++c) {
-            const int d = lane + c * kWave;
-            if (d < p.c.head_dim) out[d] = acc[c] * inv;
+            for (int c = 0; c < kRowChunks; ++c) {
+                const int d = lane + c * kWave;
+                if (d < p.c.head_dim) out[d] = acc[c] * inv;
+            }
+            if (!w.whole && lane == 0) *part.stat(row) = f2{m, l};
         }
-        if (!w.whole && lane == 0) *part.stat(row) = f2{m, l};
-    }
     }
 }
 
@@ -456,14 +456,14 @@ int64_t stream_resident(int dtype, int stride, int tiles) {
 
 }  // namespace
 
-int mimir::paged_stream_launch(mimir_ctx* ctx, const PagedArgs& p, int dtype, int64_t most_rows) {
+int mimir::paged_stream_launch(mimir_ctx* ctx, const PagedArgs& p, int dtype, int64_t most_rows, bool beside, PagedRuns* left) {
     constexpr uint32_t kStep = 2 * kHalf * kStreamWaves;
     const int64_t rows = std::min(static_cast<int64_t>(p.b.max_new) * p.group, most_rows);
     // A sequence's second tile shares the first one's keys, unless other sequences have more rows
     // than this kernel takes: then single tokens are what most have.  (For wide fp32
     // heads two tiles are more than the registers hold.)
     const bool wide = dtype == MIMIR_KV_F32 && p.c.stride > 128;
-    const int tiles = rows > kRows && !wide && rows == static_cast<int64_t>(p.b.max_new) * p.group ? 2 : 1;
+    const int tiles = rows > kRows && !wide && !beside ? 2 : 1;
     PagedRuns a{};
     a.extra = 2 * kStep;  // the queries, the first keys' way in, the sums' way out
     a.slack = a.extra;
@@ -477,12 +477,12 @@ int mimir::paged_stream_launch(mimir_ctx* ctx, const PagedArgs& p, int dtype, in
     const int64_t runs = ctx->tune.paged_runs > 0 ? ctx->tune.paged_runs : stream_resident(dtype, p.c.stride, tiles);
     // Blocks of up to eight steps are not worth a join: 500 and 1000 keys x 8 heads of one sequence whole / cut, us:
     // 10 / 16, 14 / 17; 2000, 29 / 18.
-    const int64_t grid = paged_runs(ctx, p, &a, runs, blocks, p.b.max_len > static_cast<int64_t>(8 * kStep));
+    const int64_t grid = paged_runs(ctx, p, &a, runs, blocks, p.b.max_len > static_cast<int64_t>(8 * kStep), beside);
     MIMIR_REQUIRE(ctx, dispatch_fits(grid, kStreamWaves * kWave), "paged attention: grid of %lld workgroups exceeds the limit",
                   (long long)grid);
     if (dtype == MIMIR_KV_F32) launch_tiles<MIMIR_KV_F32>(p, a, tiles, static_cast<unsigned>(grid), ctx->stream);
     else if (dtype == MIMIR_KV_BF16) launch_tiles<MIMIR_KV_BF16>(p, a, tiles, static_cast<unsigned>(grid), ctx->stream);
     else launch_tiles<MIMIR_KV_I8>(p, a, tiles, static_cast<unsigned>(grid), ctx->stream);
-    if (int st = launched(ctx, "paged_stream")) return st;
-    return paged_join_launch(ctx, p, a);
+    *left = a;
+    return launched(ctx, "paged_stream");
 }

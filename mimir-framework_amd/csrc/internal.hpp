@@ -149,8 +149,10 @@ constexpr size_t kFixedWorkBytes = sizeof(float) * 256 * 256 * 130;
 // workgroup per query block.
 float* fixed_work(mimir_ctx* ctx);
 // What attention over a paged cache keeps of blocks that two workgroups share: two of
-// 256 rows of 128 dimensions for each of 256, and which they are.
-constexpr size_t kPagedWorkBytes = sizeof(float) * 256 * 2 * 256 * 130 + 64 * 1024;
+// 256 rows of 128 dimensions for each of 256, and which they are; behind them, for a
+// launch beside that one, two of 16 rows for each of 512.
+constexpr size_t kPagedBesideBytes = sizeof(float) * 512 * 2 * 16 * 130 + 64 * 1024;
+constexpr size_t kPagedWorkBytes = sizeof(float) * 256 * 2 * 256 * 130 + 64 * 1024 + kPagedBesideBytes;
 char* paged_work(mimir_ctx* ctx);
 bool attention_decode_applies(int64_t bh, int64_t q_len, int64_t kv_len, int64_t head_dim, bool causal);
 int attention_decode_launch(mimir_ctx* ctx, const float* q, int64_t ld_q, const float* k, const float* v, int64_t ld_kv,

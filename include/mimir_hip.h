@@ -462,8 +462,12 @@ int mimir_kv_read(mimir_ctx* ctx, const mimir_kv_cache* cache, const mimir_kv_ba
  * keys are in the cache already (mimir_kv_append).  fp32 precision as
  * mimir_attention_fwd, of the values that the cache's entries stand for.  A token
  * without keys gets zeros; what stands in keys that a token does not see does not
- * reach it.  out must not overlap q.  Uses the context's 33 MiB workspace
- * as mimir_attention_fwd does. */
+ * reach it.  out must not overlap q (out == q is refused).  The results of a row
+ * depend on its own sequence and on how the batch's work is dealt out, which its
+ * lengths and bounds decide: the same call gives the same bits.  Sums that
+ * workgroups share go through a workspace of the context (74 MiB, made by the first
+ * call that may need it, under capture too, and kept): graphs captured on one
+ * context are replayed one after the other. */
 int mimir_attention_paged_fwd(mimir_ctx* ctx, const mimir_kv_cache* cache, const mimir_kv_batch* batch, const float* q,
                               int64_t ld_q, float* out, int64_t ld_out, int64_t q_heads, float scale, int causal);
 

@@ -161,6 +161,7 @@ extern "C" int mimir_attention_paged_fwd(mimir_ctx* ctx, const mimir_kv_cache* c
     if (batch->tokens == 0 || batch->sequences == 0 || batch->max_new == 0) return MIMIR_OK;
     if (cache->pages == 0) a.b.max_len = 0;  // no keys, and no memory to point at
     MIMIR_REQUIRE(ctx, q && out, "%s: null pointer", what);
+    MIMIR_REQUIRE(ctx, q != out, "%s: out must not be q", what);
     MIMIR_ENTER(ctx);
     a.q = q;
     a.out = out;

@@ -1,6 +1,35 @@
 // attention_paged_stream.hip -- attention over a paged cache for few query rows per
 // key / value head (single tokens, a few of them, and the heads that share keys):
 // keys and values straight to registers.
+//
+// A wave takes 32 keys at a time, its workgroup's four waves side by side (a step of
+// 128), against 16 query rows, or twice 16 that share the keys' way in.
+// - Scores: S^T = K Q^T by v_mfma_f32_16x16x32_bf16, keys as rows.  Lane (li, hg)
+//   supplies key li's slots and query li's, 8 of 32 dimensions each; which dimensions
+//   a slot stands for is free as long as both sides agree, so a lane loads 16 bytes
+//   of a key at a time whatever the type (Kind).  It receives the scores of row li
+//   and the keys 4 hg + {0..3} of both halves: its softmax is its own, the max alone
+//   is shared with the other three lanes of the row, and only when it has grown by
+//   more than kPagedSlack.
+// - Output: O^T = V^T P^T over the 32 keys in that order, so the weights feed it as
+//   they are; a lane loads the same keys' values, ND dimensions each (Values).
+// - Entries of bf16 and 8 bits are exact in one bf16 term, fp32 ones take three, as
+//   the queries and weights do: 3 or 6 MFMAs for a product of fp32 precision.  The
+//   8-bit scales multiply scores and weights instead of elements.
+// - The queries' terms are in LDS (registers they would not fit beside two steps of
+//   keys); the four waves' sums are brought to one max there at the end.
+//
+// Loads: buffer loads without a bounds check in the code (the descriptor of a half of
+// 16 keys ends with its keys, what lies behind reads as zero), non-temporal: nothing
+// is read twice.  The next step's keys are asked for when the scores have read this
+// one's, its values at the end; page numbers two steps ahead through scalar loads.
+//
+// Bound by memory: 64 sequences x 4096 keys x 8 heads of 128, bf16, 162 us = 6.6 TB/s
+// (a copy: 6.4); 8-bit 5.4 TB/s, 64 bytes a lane and step in flight being half as
+// many (64 keys a step: no change; fewer instructions: within 10% without any
+// arithmetic); fp32, 2048 keys, 5.7 TB/s.  One sequence of 131002 keys 92 us =
+// 5.8 TB/s, of them 7 us the join.  Short ones by latency: 101 keys 7 us, a step
+// about 1.1 us, the lengths, pages, keys and sums one after the other.
 #include "attention_paged.hpp"
 
 #include <math.h>

@@ -4,8 +4,10 @@
 // Bound by HBM: q, k and v are read once and written once, in the cache's type.
 // LPR lanes hold a head row, eight elements each (two vectors, kvcache.hpp
 // unit_place), so that the largest absolute value of an 8-bit row is a few lane
-// exchanges away and nothing is read twice.  A workgroup takes rows of one token, whose sequence its waves search in
-// token_start while the row is on its way.
+// exchanges away and nothing is read twice.  A workgroup takes rows of one token, whose
+// sequence its waves search in token_start while the row is on its way.  Prompts of
+// 9270 tokens x 32 + 2 x 8 heads of 128 into an 8-bit cache and read back (500 MB): 68
+// and 17 us, 85 in turn = 5.9 TB/s; steps of 48 tokens 4 and 3, launch to launch 9.5.
 //
 // Numerics.  Rotation in double, rounded once (rotate_pair).  An 8-bit code is the
 // exact quotient x * 127 / max rounded to nearest even: the fp32 quotient is off by

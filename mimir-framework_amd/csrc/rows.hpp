@@ -64,7 +64,7 @@ struct Tuning {
     RowShape lnbwd{0, 0, 0};  // LayerNorm backward
     int lnbwd_grid = 0;       // its persistent grid (workgroups)
     int chain_streamed = 0;   // chain=0: the runtime streams every layer's output (no kept outputs)
-    int attn_waves = 0;       // attention forward: waves per workgroup (4, 8; 0: measured default)
+    int attn_waves = 0;       // attention forward, paged attention of many rows: waves per workgroup (4, 8; 0: measured default)
     int attn_splits = 0;      // attention forward: splits of the keys (0: measured default)
     int decode_splits = 0;    // attention_decode: workgroups per (sequence, head) (0: measured default)
     int paged_runs = 0;       // paged attention: workgroups that the work is dealt to (0: measured default)

@@ -187,6 +187,30 @@ inline void attention(Context& c, const float* q, int64_t ld_q, const float* k, 
             "Attention");
 }
 
+// Serving: packed tokens of several sequences, each at its own position, and their cache
+// of pages (mimir_kv_cache, mimir_kv_batch).
+inline void rope_rows(Context& c, const float* q, int64_t ld_q, float* q_out, int64_t ld_q_out, int64_t q_heads,
+                      const float* k, int64_t ld_k, float* k_out, int64_t ld_k_out, int64_t k_heads, int64_t tokens,
+                      int64_t head_dim, const int32_t* positions, const mimir_rope& rope) {
+    c.check(mimir_rope_rows_fwd(c.get(), q, ld_q, q_out, ld_q_out, q_heads, k, ld_k, k_out, ld_k_out, k_heads, tokens,
+                                head_dim, positions, &rope),
+            "RoPE rows");
+}
+inline void kv_append(Context& c, const mimir_kv_cache& cache, const mimir_kv_batch& batch, const float* k,
+                      const float* v, int64_t ld_kv, const mimir_rope* rope = nullptr, const float* q = nullptr,
+                      int64_t ld_q = 0, float* q_out = nullptr, int64_t ld_q_out = 0, int64_t q_heads = 0) {
+    c.check(mimir_kv_append(c.get(), &cache, &batch, k, v, ld_kv, rope, q, ld_q, q_out, ld_q_out, q_heads), "KV append");
+}
+inline void kv_read(Context& c, const mimir_kv_cache& cache, const mimir_kv_batch& batch, float* k_out, float* v_out,
+                    int64_t ld_out) {
+    c.check(mimir_kv_read(c.get(), &cache, &batch, k_out, v_out, ld_out), "KV read");
+}
+inline void attention_paged(Context& c, const mimir_kv_cache& cache, const mimir_kv_batch& batch, const float* q,
+                            int64_t ld_q, float* out, int64_t ld_out, int64_t q_heads, float scale, bool causal) {
+    c.check(mimir_attention_paged_fwd(c.get(), &cache, &batch, q, ld_q, out, ld_out, q_heads, scale, causal ? 1 : 0),
+            "paged attention");
+}
+
 }  // namespace device
 
 namespace detail {

@@ -190,6 +190,7 @@ int main() {
     BAD(attend(f, 32, f + 1, 32, 0, 1.f));
     BAD(attend(f, 32, f + 1, 32, 4, NAN));
     BAD(attend(f, 32, f + 1, 32, 4, INFINITY));
+    BAD(attend(f, 32, f, 32, 4, 1.f));  // in place
     BAD(attend(nullptr, 32, f + 1, 32, 4, 1.f));
     BAD(attend(f, 32, nullptr, 32, 4, 1.f));
 

@@ -4,6 +4,9 @@ other streams and contexts beside; and attention over batches that are dealt to 
 workgroups in every way (many sequences, few, two tiles of rows, cut anywhere),
 caches past 2^32 bytes and the longest context that a call may have."""
 import ctypes
+import os
+import shutil
+import subprocess
 import threading
 
 import numpy as np
@@ -121,18 +124,22 @@ def test_captured_and_replayed_with_other_lengths(dtype, longest, news, lens):
         junk = ctx.empty((tokens, heads * d))
         rng = np.random.default_rng(4)
         whole = [rng.standard_normal((longest, w)).astype(np.float32) for _ in range(3)]
-        # The whole sequences are in both caches.
-        filler_a, filler_b = ctx.empty((3 * longest, w)), other.empty((3 * longest, w))
-        for layer, filler in ((a, filler_a), (b, filler_b)):
-            layer.ctx.upload(filler, np.concatenate(whole))
-            layer.ctx.upload(layer.start, (np.arange(4) * longest).astype(np.int32))
-            layer.ctx.upload(layer.len, np.full(3, longest, np.int32))
-            batch = M.KVBatch(layer.start, layer.len, layer.table, 3, 3 * longest, layer.per, longest, longest)
-            layer.ctx.kv_append(layer.cache, batch, filler.offset(heads * d), filler.offset((heads + kh) * d), ld_kv=w)
+        fillers = [c.to_device(np.concatenate(whole)) for c in (ctx, other)]
+
+        def whole_sequences(pages):
+            """In both caches, in these pages."""
+            for layer, filler in zip((a, b), fillers):
+                layer.ctx.upload(layer.table, pages)
+                layer.ctx.upload(layer.start, (np.arange(4) * longest).astype(np.int32))
+                layer.ctx.upload(layer.len, np.full(3, longest, np.int32))
+                batch = M.KVBatch(layer.start, layer.len, layer.table, 3, 3 * longest, layer.per, longest, longest)
+                layer.ctx.kv_append(layer.cache, batch, filler.offset(heads * d), filler.offset((heads + kh) * d), ld_kv=w)
+
         graph = Graph(ctx, lambda: a.run(out_a, tokens, most))
         try:
             for turn, (n, m) in enumerate(zip(news * 2, lens * 2)):
                 rows = rng.standard_normal((tokens, w)).astype(np.float32)
+                whole_sequences(rng.permutation(3 * a.per).astype(np.int32).reshape(3, a.per))
                 for layer, out in ((a, out_a), (b, out_b)):
                     layer.set(n, m, rows)
                     layer.ctx.fill(out, -3.0)
@@ -334,3 +341,13 @@ def test_the_longest_context(ctx, dtype):
     mag = (weight @ np.abs(v[:, 0].astype(np.float64)) / weight.sum(1, keepdims=True))[None]
     tol = tol + 2 * (1 << 15) * U * mag
     assert (np.abs(out.numpy().reshape(want.shape) - want) <= tol).all()
+
+
+@pytest.mark.skipif(shutil.which("g++") is None, reason="g++ not available")
+def test_cpp_adapter(tmp_path):
+    here, lib = os.path.dirname(os.path.abspath(__file__)), os.path.dirname(M.LIB_PATH)
+    exe = tmp_path / "test_serving_device"
+    subprocess.run(["g++", "-O1", "-std=c++17", "-Wall", "-Werror", "-pthread", f"-I{here}/../include", "-o", str(exe),
+                    os.path.join(here, "cpp", "test_serving_device.cpp"), f"-L{lib}", "-lmimir_hip", f"-Wl,-rpath,{lib}"], check=True)
+    r = subprocess.run([str(exe)], capture_output=True, text=True, timeout=100)
+    assert r.returncode == 0 and r.stdout.strip() == "0 failures", r.stdout + r.stderr

@@ -120,7 +120,7 @@ __device__ __forceinline__ uint64_t paged_chunk(const PagedArgs& p, const PagedR
         *cost = paged_cost(p, a, seq);
     }
     const uint64_t sum = lanes_up_to(cost->ahead(cost->blocks) * static_cast<uint32_t>(p.c.kv_heads));
-    if (chunk && threadIdx.x < kWave) {
+    if (threadIdx.x < kWave) {
         chunk->sum[lane] = sum;
         chunk->seq[lane] = seq;
         chunk->cost[lane] = *cost;
@@ -174,15 +174,34 @@ struct PagedWalk {
             end = run = 1;
             return;
         }
-        PagedCost cost, other;
-        uint64_t total = lane_of(paged_chunk(p, a, 0, chunk, &cost), kWave - 1);
-        for (int b = kWave; b < p.b.sequences; b += kWave) total += lane_of(paged_chunk(p, a, b, nullptr, &other), kWave - 1);
+        PagedCost cost;
+        const int lane = static_cast<int>(threadIdx.x % kWave), each = (p.b.sequences + kWave - 1) / kWave;
+        uint64_t mine = 0, sum;  // costs of a lane's sequences, up to them
+        if (each <= 1) {
+            sum = paged_chunk(p, a, 0, chunk, &cost);
+        } else {
+#pragma unroll 4
+            for (int i = 0; i < each; ++i) {
+                const int s = lane * each + i;
+                if (s >= p.b.sequences) break;
+                const PagedCost one = paged_cost(p, a, kv_sequence(p.b, s));
+                mine += one.ahead(one.blocks) * static_cast<uint32_t>(p.c.kv_heads);
+            }
+            sum = lanes_up_to(mine);
+        }
+        uint64_t total = lane_of(sum, kWave - 1);
         run = uniform(max(quotient(total + a.runs - 1, a.runs), static_cast<uint64_t>(a.extra + a.grain)));
         if (a.apart) total = set_apart(p, a, total, cost);
         from = uniform(min(total, run * index));
         end = uniform(min(total, from + run));
         // A run of nothing begins no block; the others say so as they end.
         if (from >= end && threadIdx.x == 0) a.shared[index].runs = 0;
+        if (each > 1 && from < end) {  // the chunk from the sequences of the lane on that the run begins in
+            const int at = __builtin_ctzll(__ballot(sum > from));
+            base = uniform(at * each);
+            before = uniform(lane_of(sum, at) - lane_of(mine, at));
+            paged_chunk(p, a, base, chunk, &cost);
+        }
         __syncthreads();
     }
     // With fewer blocks than half the runs, a block's cost may be rounded up to whole

@@ -351,3 +351,52 @@ def test_cpp_adapter(tmp_path):
                     os.path.join(here, "cpp", "test_serving_device.cpp"), f"-L{lib}", "-lmimir_hip", f"-Wl,-rpath,{lib}"], check=True)
     r = subprocess.run([str(exe)], capture_output=True, text=True, timeout=100)
     assert r.returncode == 0 and r.stdout.strip() == "0 failures", r.stdout + r.stderr
+
+
+@pytest.mark.parametrize("seed,count", [(0, 64), (1, 65), (2, 4095), (3, 4096), (4, 4200), (5, 9000)])
+def test_tokens_of_thousands_of_sequences(ctx, seed, count):
+    """Which sequence a token is of, by what is written and read back: runs of sequences
+    without new tokens, several tokens, rows behind the last one."""
+    rng = np.random.default_rng(seed)
+    n = rng.choice([0, 1, 1, 2, 5], size=count)
+    hole = int(rng.integers(0, max(1, count - 200)))
+    n[hole:hole + 150] = 0
+    kh, d, page = 1, 4, 16
+    start = np.concatenate([[0], np.cumsum(n)]).astype(np.int32)
+    tokens = int(start[-1]) + 3
+    table = rng.permutation(count).astype(np.int32)
+    up = ctx.to_device
+    cache = M.KVCache(ctx, "f32", count, page, kh, d)
+    try:
+        x = np.arange(tokens * d, dtype=np.float32).reshape(tokens, d)
+        kv_len = np.maximum(n, rng.integers(0, 17, count)).astype(np.int32)
+        batch = M.KVBatch(up(start), up(kv_len), up(table), count, tokens, 1, 5, page)
+        ctx.kv_append(cache, batch, up(x), up(-x))
+        k = cache.k.numpy().reshape(count, page, stride_of(d))
+        for s in range(count):
+            got = k[table[s], kv_len[s] - n[s]:kv_len[s], :d]
+            np.testing.assert_array_equal(got, x[start[s]:start[s + 1]])
+        ko, vo = (up(np.full((tokens, d), -9.0, np.float32)) for _ in range(2))
+        ctx.kv_read(cache, batch, ko, vo)
+        np.testing.assert_array_equal(ko.numpy()[:-3], x[:-3])
+        np.testing.assert_array_equal(vo.numpy()[:-3], -x[:-3])
+        assert (ko.numpy()[-3:] == -9).all() and (vo.numpy()[-3:] == -9).all()
+    finally:
+        cache.close()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_runs_over_thousands_of_sequences(ctx, dtype):
+    """Most without new tokens, in stretches; lengths from 1 to 1400."""
+    rng = np.random.default_rng(40)
+    count, d = 4500, 16
+    n = np.zeros(count, int)
+    n[rng.choice(count, 300, replace=False)] = rng.integers(1, 3, 300)
+    n[1000:1130] = 1
+    lens = [(int(x), int(x + rng.integers(0, 1400 if i % 7 == 0 else 30))) if x else (0, 5) for i, x in enumerate(n)]
+    q, kv = case(41, dtype, lens, 1, 2, d)
+    p = Paged(ctx, dtype, lens, 1, d, 16, max_len=1500)
+    p.table = np.pad(p.table, ((0, 0), (0, 10)), constant_values=-1)
+    p.ld = p.table.shape[1]
+    fill(p, kv)
+    check(attend(ctx, p, q), p, q, kv)

@@ -127,9 +127,9 @@ int join(mimir_ctx* ctx, const PagedArgs& p, const PagedRuns& a, const PagedRuns
 }  // namespace
 
 int64_t mimir::paged_runs(mimir_ctx* ctx, const PagedArgs& p, PagedRuns* a, int64_t runs, int64_t blocks, bool split, bool beside) {
-    // No more than keep to the least length of a run (PagedWalk), by the longest costs.
+    // No more than keep to the least length of a run (PagedWalk), by the longest costs, each block's last one shorter.
     const int64_t cost = a->extra + static_cast<int64_t>(p.b.max_len) + (p.causal ? (a->block_rows + p.group - 1) / p.group : 0);
-    if (blocks < 1 << 24) runs = std::max<int64_t>(1, std::min(runs, blocks * cost / (a->extra + a->grain) + 1));
+    if (blocks < 1 << 24) runs = std::max<int64_t>(1, std::min(runs, blocks * (cost / (a->extra + a->grain) + 1)));
     a->apart = p.b.sequences <= kWave;
     a->many = a->part_rows <= 32 && runs > 4 * blocks;
     constexpr size_t kAlone = kPagedWorkBytes - kPagedBesideBytes;
@@ -174,14 +174,16 @@ extern "C" int mimir_attention_paged_fwd(mimir_ctx* ctx, const mimir_kv_cache* c
     a.group_div = make_fastdiv(static_cast<uint32_t>(a.group));
     // Sequences with few query rows of a key / value head stream their keys, the others'
     // keys go through LDS, by a launch each.  A batch whose sequences all have max_new
-    // tokens (or whose rows would suffice for that) has the second alone, which takes any.
+    // tokens (or whose rows would suffice for that) has the second alone, which takes any;
+    // so has one of short contexts (chunks of up to 91 tokens beside single ones, up to 100
+    // keys before them, 19 sequences: 42 us, by two launches 53).
     const int64_t rows = static_cast<int64_t>(a.b.max_new) * a.group;
     MIMIR_REQUIRE(ctx, rows <= INT32_MAX, "%s: %lld query rows of a head", what, (long long)rows);
     PagedRuns few{}, others{};
     if (rows <= kStreamRows || a.c.stride > kPagedBlockStride) {
         if (int st = paged_stream_launch(ctx, a, cache->dtype, INT32_MAX, false, &few)) return st;
     } else {
-        const bool both = a.b.sequences * static_cast<int64_t>(a.b.max_new) > a.b.tokens;
+        const bool both = a.b.sequences * static_cast<int64_t>(a.b.max_new) > a.b.tokens && a.b.max_len > kWholeLen;
         if (both)
             if (int st = paged_stream_launch(ctx, a, cache->dtype, kStreamBeside, true, &few)) return st;
         if (int st = paged_block_launch(ctx, a, cache->dtype, both ? kStreamBeside + 1 : 1, &others)) return st;

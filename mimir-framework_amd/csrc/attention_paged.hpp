@@ -447,6 +447,12 @@ __device__ __forceinline__ void row_over_keys(const PagedArgs& a, int s, int kv_
 int paged_stream_launch(mimir_ctx* ctx, const PagedArgs& p, int dtype, int64_t most_rows, bool beside, PagedRuns* left);
 int paged_block_launch(mimir_ctx* ctx, const PagedArgs& p, int dtype, int64_t least_rows, PagedRuns* left);
 
+// Contexts that the block kernel has whole, by workgroups of four waves: one prompt of
+// 250 tokens, 32 heads of 128, bf16: 32 us cut and joined, 29 whole by eight waves, 24 by
+// four; 64 of up to 102 57, 37 and 35.  (Up to 512: 12 prompts of 400, heads of 64, 78 and
+// 63, but 49 sequences of 315 or single tokens 64 and 79.)
+constexpr int kWholeLen = 256;
+
 // The widest heads (padded) of the block kernel: its queries' terms are registers.
 constexpr int kPagedBlockStride = 128;
 

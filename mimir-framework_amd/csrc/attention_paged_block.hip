@@ -455,7 +455,7 @@ int launch(mimir_ctx* ctx, const PagedArgs& p, PagedRuns a, PagedRuns* left) {
     a.row_blocks = static_cast<int32_t>((rows + a.block_rows - 1) / a.block_rows);
     const int64_t blocks = static_cast<int64_t>(p.b.sequences) * p.c.kv_heads * a.row_blocks;
     const int64_t runs = ctx->tune.paged_runs > 0 ? ctx->tune.paged_runs : 256 * BlockShape<DT, DP, WAVES>::kResident;
-    const int64_t grid = paged_runs(ctx, p, &a, runs, blocks, true, false);
+    const int64_t grid = paged_runs(ctx, p, &a, runs, blocks, p.b.max_len > kWholeLen, false);
     MIMIR_REQUIRE(ctx, dispatch_fits(grid, WAVES * kWave), "paged attention: grid of %lld workgroups exceeds the limit",
                   (long long)grid);
     paged_block<DT, DP, WAVES><<<static_cast<unsigned>(grid), WAVES * kWave, 0, ctx->stream>>>(p, a);
@@ -465,7 +465,7 @@ int launch(mimir_ctx* ctx, const PagedArgs& p, PagedRuns a, PagedRuns* left) {
 
 template <int DT, int DP>
 int launch_waves(mimir_ctx* ctx, const PagedArgs& p, const PagedRuns& a, PagedRuns* left) {
-    int waves = static_cast<int64_t>(p.b.max_new) * p.group <= 4 * kTile ? 4 : 8;
+    int waves = static_cast<int64_t>(p.b.max_new) * p.group <= 4 * kTile || p.b.max_len <= kWholeLen ? 4 : 8;
     if (ctx->tune.attn_waves == 4 || ctx->tune.attn_waves == 8) waves = ctx->tune.attn_waves;
     return waves == 4 ? launch<DT, DP, 4>(ctx, p, a, left) : launch<DT, DP, 8>(ctx, p, a, left);
 }

@@ -504,9 +504,12 @@ int mimir::paged_stream_launch(mimir_ctx* ctx, const PagedArgs& p, int dtype, in
     a.row_blocks = static_cast<int32_t>((rows + a.block_rows - 1) / a.block_rows);
     const int64_t blocks = static_cast<int64_t>(p.b.sequences) * p.c.kv_heads * a.row_blocks;
     const int64_t runs = ctx->tune.paged_runs > 0 ? ctx->tune.paged_runs : stream_resident(dtype, p.c.stride, tiles);
-    // Blocks of up to eight steps are not worth a join: 500 and 1000 keys x 8 heads of one sequence whole / cut, us:
-    // 10 / 16, 14 / 17; 2000, 29 / 18.
-    const int64_t grid = paged_runs(ctx, p, &a, runs, blocks, p.b.max_len > static_cast<int64_t>(8 * kStep), beside);
+    // Short blocks are not worth a join, by the bytes of one where they do not fill the GPU.  Whole / cut, us, two
+    // sequences x 8 heads: bf16 heads of 128, 500 keys 10 / 14, 1000 18 / 16; fp32 500 23 / 21, 1000 41 / 28; fp32
+    // heads of 256 500 57 / 42; 32 sequences, fp32 heads of 128 and 256, 500 keys 30 / 34, 70 / 74.
+    const int64_t key_bytes = 2 * static_cast<int64_t>(p.c.stride) * kv_element_bytes(dtype);
+    const bool whole = p.b.max_len <= static_cast<int64_t>(8 * kStep) && (p.b.max_len * key_bytes <= 448 * 1024 || 2 * blocks >= runs);
+    const int64_t grid = paged_runs(ctx, p, &a, runs, blocks, !whole, beside);
     MIMIR_REQUIRE(ctx, dispatch_fits(grid, kStreamWaves * kWave), "paged attention: grid of %lld workgroups exceeds the limit",
                   (long long)grid);
     if (dtype == MIMIR_KV_F32) launch_tiles<MIMIR_KV_F32>(p, a, tiles, static_cast<unsigned>(grid), ctx->stream);

@@ -19,8 +19,10 @@ namespace {
 // those beside longer ones.  Where the block kernel would take as long (40 to 64 rows,
 // stream / block, us): 32 sequences x 3000 keys x 4 heads of 128, bf16 90-98 / 86-88,
 // 8-bit 76-82 / 92-93, fp32 162-167 / 181-185; one of 30000 x 8 heads, 64 rows, bf16
-// 62 / 86, 8-bit 58 / 88, fp32 111 / 141.  Beside longer ones it has 16 rows a block.
-constexpr int64_t kStreamRows = 64, kStreamBeside = 32;
+// 62 / 86, 8-bit 58 / 88, fp32 111 / 141.  Beside longer ones it has 16 rows a block, and
+// so it has of fp32 heads over 128, which are the block kernel's from there on (32
+// sequences x 3000 keys x 4 heads of 256, 32 rows 369 / 173, 64 720 / 234).
+constexpr int64_t kStreamRows = 64, kStreamBeside = 32, kStreamWide = 16;
 
 // The shares of a block's rows: each brought to one max, added up and divided.  LPR
 // lanes hold a row, four dimensions each.  ONE: the whole workgroup takes a row at a
@@ -175,18 +177,22 @@ extern "C" int mimir_attention_paged_fwd(mimir_ctx* ctx, const mimir_kv_cache* c
     // Sequences with few query rows of a key / value head stream their keys, the others'
     // keys go through LDS, by a launch each.  A batch whose sequences all have max_new
     // tokens (or whose rows would suffice for that) has the second alone, which takes any;
-    // so has one of short contexts (chunks of up to 91 tokens beside single ones, up to 100
-    // keys before them, 19 sequences: 42 us, by two launches 53).
+    // so has one of short contexts that is one round of workgroups or little more (chunks of
+    // up to 91 tokens beside single ones, up to 100 keys before them, 19 sequences x 8
+    // heads: 42 us, by two launches 53; 64 sequences x 8 heads, bf16 45, by two 38; 84 x 8,
+    // fp32, of whose streaming workgroups a compute unit holds one, 84 and 96).
     const int64_t rows = static_cast<int64_t>(a.b.max_new) * a.group;
     MIMIR_REQUIRE(ctx, rows <= INT32_MAX, "%s: %lld query rows of a head", what, (long long)rows);
     PagedRuns few{}, others{};
-    if (rows <= kStreamRows || a.c.stride > kPagedBlockStride) {
+    const int64_t pairs = cache->dtype == MIMIR_KV_F32 && a.c.stride > 64 ? 1024 : 256;
+    const int64_t streamed = cache->dtype == MIMIR_KV_F32 && a.c.stride > 128 ? kStreamWide : kStreamRows;
+    if (rows <= streamed) {
         if (int st = paged_stream_launch(ctx, a, cache->dtype, INT32_MAX, false, &few)) return st;
     } else {
-        const bool both = a.b.sequences * static_cast<int64_t>(a.b.max_new) > a.b.tokens && a.b.max_len > kWholeLen;
+        const bool both = a.b.sequences * static_cast<int64_t>(a.b.max_new) > a.b.tokens && (a.b.max_len > kWholeLen || static_cast<int64_t>(a.b.sequences) * a.c.kv_heads > pairs);
         if (both)
-            if (int st = paged_stream_launch(ctx, a, cache->dtype, kStreamBeside, true, &few)) return st;
-        if (int st = paged_block_launch(ctx, a, cache->dtype, both ? kStreamBeside + 1 : 1, &others)) return st;
+            if (int st = paged_stream_launch(ctx, a, cache->dtype, std::min(streamed, kStreamBeside), true, &few)) return st;
+        if (int st = paged_block_launch(ctx, a, cache->dtype, both ? std::min(streamed, kStreamBeside) + 1 : 1, &others)) return st;
     }
     return join(ctx, a, few, others);
 }

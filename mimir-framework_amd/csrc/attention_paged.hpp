@@ -453,9 +453,6 @@ int paged_block_launch(mimir_ctx* ctx, const PagedArgs& p, int dtype, int64_t le
 // 63, but 49 sequences of 315 or single tokens 64 and 79.)
 constexpr int kWholeLen = 256;
 
-// The widest heads (padded) of the block kernel: its queries' terms are registers.
-constexpr int kPagedBlockStride = 128;
-
 // Sets up `a` for at most `runs` workgroups in the workspace, or for one per block
 // (`blocks` of them) where that is not to be had or `split` says not to; the grid.
 int64_t paged_runs(mimir_ctx* ctx, const PagedArgs& p, PagedRuns* a, int64_t runs, int64_t blocks, bool split, bool beside);

@@ -12,6 +12,11 @@
 //   read (ds_read_b64_tr_b16), in the order of keys that the scores come out in.
 // - Tile t is computed while t + 1 goes from registers to LDS and t + 2 comes from
 //   memory; one barrier a tile.
+// - Heads over 128: a row's queries and sums would not fit one wave's registers, so two
+//   waves (fp32: four) share 32 rows, a half (a quarter) of the dimensions each.  Their
+//   scores meet in LDS, in one order for all, and each wave does the row's softmax.
+//   Keys and values have one buffer each: a tile's values come in beside its scores'
+//   products, the next one's keys after them; two barriers a tile.
 // - Causal: a wave passes over tiles behind its last row's keys.  Rows' ends inside a
 //   tile, and pages that are none, are looked at only where there are any.
 //
@@ -23,7 +28,10 @@
 // Measured on the way: a lane's query row in loads of 4 bytes instead of 16 cost 12 us
 // a block, page numbers looked at for each tile instead of once a block 6 us of 219,
 // and waves that all multiply the values in the tile they were scored in 7% of the
-// whole.  Two accumulators in turns for the scores: no change.
+// whole.  Two accumulators in turns for the scores: no change.  Heads of 256, 4 prompts of
+// 1440 tokens, 8 heads, by streamed blocks of 16 (fp32) or 32 rows and by these: fp32 1243
+// and 321 us, bf16 392 and 172, 8-bit 343 and 196; 512 tokens over 4512 keys, 16 heads on
+// 4, fp32 995 and 280, bf16 235 and 131, 8-bit 159 and 149.
 #include "attention_paged.hpp"
 
 #include <math.h>
@@ -100,8 +108,14 @@ __device__ __forceinline__ f16v mfma_planes(const u4* a, const Split8& b, f16v c
 template <int DT, int DP, int WAVES>
 struct BlockShape {
     using Tile = BlockTile<DT, DP>;
+    // Waves that share 32 rows, a part of the dimensions each: where a row's queries and
+    // sums would not fit one's registers.
+    static constexpr int kShare = DP == 256 ? (DT == MIMIR_KV_F32 ? 4 : 2) : 1;
+    static constexpr int kDims = DP / kShare, kRows = WAVES / kShare * kTile;
     static constexpr int kValueBufs = WAVES == 8 ? 3 : 2;
-    static constexpr int kBytes = 2 * Tile::kKeyBytes + kValueBufs * Tile::kValueBytes;
+    static constexpr int kParts = WAVES * kWave * 16 * 4;  // scores of the dimensions of each wave
+    static constexpr int kBytes = kShare == 1 ? 2 * Tile::kKeyBytes + kValueBufs * Tile::kValueBytes
+                                              : Tile::kKeyBytes + Tile::kValueBytes + kParts;
     static constexpr int kResident = WAVES == 8 || kBytes + sizeof(PagedChunk) > 80 * 1024 ? 1 : 2;
 };
 
@@ -109,19 +123,22 @@ template <int DT, int DP, int WAVES>
 __global__ __launch_bounds__(WAVES * kWave, (WAVES / 4 * BlockShape<DT, DP, WAVES>::kResident)) void paged_block(PagedArgs p, PagedRuns a) {
     using Tile = BlockTile<DT, DP>;
     using Shape = BlockShape<DT, DP, WAVES>;
-    constexpr int kThreads = WAVES * kWave, kC = DP / 16, kDb = DP / 32;
+    constexpr int kThreads = WAVES * kWave, kC = Shape::kDims / 16, kDb = Shape::kDims / 32;
+    constexpr bool kShared = Shape::kShare > 1;
     constexpr int kElement = DT == MIMIR_KV_F32 ? 4 : DT == MIMIR_KV_BF16 ? 2 : 1;
     // Eight waves: the second four, which share the SIMDs with the first, multiply a
     // tile's values one tile later, so that one's softmax runs beside the other's products;
     // the values stay that much longer.
-    constexpr bool kStagger = WAVES == 8;
+    constexpr bool kStagger = WAVES == 8 && !kShared;
     __shared__ __attribute__((aligned(16))) char lds[Shape::kBytes];
-    char* const values = lds + 2 * Tile::kKeyBytes;
+    char* const values = lds + (kShared ? 1 : 2) * Tile::kKeyBytes;
     __shared__ PagedChunk chunk;
+    __shared__ uint32_t bad[WAVES];  // shared: the rows that came out NaN or infinite of each wave
 
     // Each XCD takes runs that follow each other, whose keys it has in its L2.
     const uint32_t at = a.runs % kXcds == 0 && gridDim.x == a.runs ? blockIdx.x % kXcds * (a.runs / kXcds) + blockIdx.x / kXcds : blockIdx.x;
     const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave);
+    const int group = wave / Shape::kShare, d_wave = wave % Shape::kShare * Shape::kDims;  // its rows, its dimensions
     for (PagedWalk walk(p, a, at, &chunk); walk.more();) {
         int tid = static_cast<int>(threadIdx.x);
         asm volatile("" : "+v"(tid));  // what follows from it is computed for each block, not held in registers across them
@@ -130,12 +147,12 @@ __global__ __launch_bounds__(WAVES * kWave, (WAVES / 4 * BlockShape<DT, DP, WAVE
         if (w.rows <= 0) return;
         const int k0 = w.k0, k1 = w.k1;
         const int li = lane % 32, hf = lane / 32;
-        const int wave_rows = min(w.rows - wave * kTile, kTile);  // below 1: a wave that only moves tiles
+        const int wave_rows = min(w.rows - group * kTile, kTile);  // below 1: a wave that only moves tiles
         const bool in = li < wave_rows;
-        const int my_row = w.row0 + wave * kTile + max(0, min(li, wave_rows - 1));
+        const int my_row = w.row0 + group * kTile + max(0, min(li, wave_rows - 1));
         const int my_end = min(row_end(p, w.seq, min(my_row, w.row0 + w.rows - 1)), k1);
         const int first_end = uniform(my_end);  // the wave's first row's, none sees fewer
-        const int wave_end = wave_rows > 0 ? min(k1, row_end(p, w.seq, w.row0 + wave * kTile + wave_rows - 1)) : k0;
+        const int wave_end = wave_rows > 0 ? min(k1, row_end(p, w.seq, w.row0 + group * kTile + wave_rows - 1)) : k0;
         const auto q_row = [&](int row) { return p.q + paged_row(p, p.ld_q, w.seq.first, w.head, row); };
         const PagedPart part(a, p.c.head_dim, walk.index, w.begins);
         // Row of the block: its output, or where its sums are kept.
@@ -163,7 +180,7 @@ __global__ __launch_bounds__(WAVES * kWave, (WAVES / 4 * BlockShape<DT, DP, WAVE
         // A thread's items: eight dimensions of a row.  An item's rows are, for a wave, of
         // one half of the tile; what lies past a row's dimensions or the half's keys reads
         // as zeros.
-        constexpr int kLanes = DP == 64 ? 8 : 16;
+        constexpr int kLanes = DP == 64 ? 8 : DP == 256 ? 32 : 16;
         constexpr int kItems = (kTile * kLanes + kThreads - 1) / kThreads;
         static_assert(kWave / kLanes <= kHalf && kHalf % (kWave / kLanes) == 0, "a wave's rows in one half");
         static_assert(kItems == 1 || (kItems == 2 && kThreads == kHalf * kLanes), "an item a half");
@@ -193,7 +210,7 @@ __global__ __launch_bounds__(WAVES * kWave, (WAVES / 4 * BlockShape<DT, DP, WAVE
         RowItem<DT> ki[kItems], vi[kItems];
         float scale[kItems];
         const int scales = wave % kMovers;  // 8-bit: 0, the keys' scales are this wave's to move, 1, the values'
-        const auto load = [&](const Halves& g) {
+        const auto load = [&](const Halves& g, bool keys_too, bool values_too) {
             if (!mover) return;
 #pragma unroll
             for (int n = 0; n < kItems; ++n) {
@@ -201,37 +218,38 @@ __global__ __launch_bounds__(WAVES * kWave, (WAVES / 4 * BlockShape<DT, DP, WAVE
                 const int64_t row = (has ? g.page[n] : 0) * page_rows + head_rows + g.slot[n];
                 const int keys = has ? g.keys[n] : 0;
                 const int64_t at = row * row_bytes;
-                ki[n].load(__builtin_amdgcn_make_buffer_rsrc(p.c.k + at, 0, keys * row_bytes, kBufferWord3), off);
-                vi[n].load(__builtin_amdgcn_make_buffer_rsrc(p.c.v + at, 0, keys * row_bytes, kBufferWord3), off);
+                if (keys_too) ki[n].load(__builtin_amdgcn_make_buffer_rsrc(p.c.k + at, 0, keys * row_bytes, kBufferWord3), off);
+                if (values_too) vi[n].load(__builtin_amdgcn_make_buffer_rsrc(p.c.v + at, 0, keys * row_bytes, kBufferWord3), off);
                 if constexpr (DT == MIMIR_KV_I8)
-                    if (scales < 2)
+                    if (scales < 2 && (scales ? values_too : keys_too))
                         scale[n] = buffer_f1(buffer_of((scales ? p.c.v_scale : p.c.k_scale) + row, 4 * keys), static_cast<uint32_t>(4 * (lane % kHalf)));
             }
         };
-        const auto stash = [&](char* key_buf, char* value_buf) {
+        // Both kinds' scales stand beside the keys.
+        const auto stash = [&](char* key_buf, char* value_buf, bool keys_too, bool values_too) {
             if (!mover) return;
 #pragma unroll
             for (int n = 0; n < kItems; ++n) {
                 if (d_mine < DP) {
-                    ki[n].stash(key_buf + row_of(n) * Tile::kKeyRow + 2 * d_mine, Tile::kKeyPlane);
-                    vi[n].stash(value_buf + row_of(n) * Tile::kValueRow + 2 * d_mine, Tile::kValuePlane);
+                    if (keys_too) ki[n].stash(key_buf + row_of(n) * Tile::kKeyRow + 2 * d_mine, Tile::kKeyPlane);
+                    if (values_too) vi[n].stash(value_buf + row_of(n) * Tile::kValueRow + 2 * d_mine, Tile::kValuePlane);
                 }
                 if constexpr (DT == MIMIR_KV_I8)
-                    if (scales < 2 && lane < kHalf)
+                    if (scales < 2 && (scales ? values_too : keys_too) && lane < kHalf)
                         reinterpret_cast<float*>(key_buf + Tile::kScalesAt)[scales * kTile + half_of(n) * kHalf + lane] = scale[n];
             }
         };
 
         Halves to{};  // of the tile after the one in registers, which is after the one in LDS
         if (tiles > 0) {
-            load(find(0));
+            load(find(0), true, true);
             to = find(1);
         }
         // This lane's query values, times scale * log2(e).
         Split8 q[kC];
         {
-            const float* row = q_row(min(my_row, w.row0 + w.rows - 1)) + 8 * hf;
-            const int left = p.c.head_dim - 8 * hf;  // of the row from there on
+            const float* row = q_row(min(my_row, w.row0 + w.rows - 1)) + d_wave + 8 * hf;
+            const int left = p.c.head_dim - d_wave - 8 * hf;  // of the row from there on
             if (p.c.head_dim % 4 == 0) {
                 f4u x[kC][2];
 #pragma unroll
@@ -261,15 +279,17 @@ __global__ __launch_bounds__(WAVES * kWave, (WAVES / 4 * BlockShape<DT, DP, WAVE
         for (int d = 0; d < kDb; ++d) o[d] = f16v{};
         float m_run = -1e30f, l_run = 0.f;
 
+        Halves later{};  // shared: the values follow a tile behind the keys
         if (tiles > 0) {
-            stash(lds, values);
-            load(to);
+            stash(lds, values, true, !kShared);
+            load(to, true, !kShared);
+            later = to;
             to = find(2);
         }
         __syncthreads();
         // A lane's part of a transposed read: key 4 hf + (lane % 16) / 4, dimensions
         // 16 (lane / 16 % 2) + 4 (lane % 4) on.
-        const int v_lane = (4 * hf + lane % 16 / 4) * Tile::kValueRow + (lane / 16 % 2 * 16 + 4 * (lane % 4)) * 2;
+        const int v_lane = (4 * hf + lane % 16 / 4) * Tile::kValueRow + (d_wave + lane / 16 % 2 * 16 + 4 * (lane % 4)) * 2;
         f16v s;  // scores of a tile, then its weights
         // o += V^T P^T over a tile's keys.  Values are read one operand ahead of their
         // products, and the second half's weights are split beside the first half's.
@@ -316,98 +336,137 @@ __global__ __launch_bounds__(WAVES * kWave, (WAVES / 4 * BlockShape<DT, DP, WAVE
             }
             __builtin_amdgcn_s_setprio(0);
         };
-        const bool late = kStagger && wave >= WAVES / 2;
-        char *v_old = values, *v_cur = values, *v_next = values + Tile::kValueBytes;
-        for (int t = 0; t < tiles + (kStagger ? 1 : 0); ++t) {
-            const char* cur = lds + (t & 1) * Tile::kKeyBytes;
-            char* const next = lds + ((t + 1) & 1) * Tile::kKeyBytes;
-            const int key = k0 + t * kTile;
-            if (kStagger && late && t > 0 && key - kTile < wave_end) weigh(v_old);
-            const bool active = key < wave_end;
-            if (active) {
-                const auto read = [&](int c, u4* k) {
+        // S^T = K Q^T over the wave's dimensions, 8-bit: times the keys' scales.
+        const auto scores = [&](const char* cur) {
+            const auto read = [&](int c, u4* k) {
 #pragma unroll
-                    for (int n = 0; n < Tile::kPlanes; ++n)
-                        k[n] = *reinterpret_cast<const u4*>(cur + n * Tile::kKeyPlane + li * Tile::kKeyRow + 32 * c + 16 * hf);
-                };
-                s = f16v{};
-                __builtin_amdgcn_s_setprio(1);
-                u4 k[2][Tile::kPlanes];
-                read(0, k[0]);
+                for (int n = 0; n < Tile::kPlanes; ++n)
+                    k[n] = *reinterpret_cast<const u4*>(cur + n * Tile::kKeyPlane + li * Tile::kKeyRow + 2 * d_wave + 32 * c + 16 * hf);
+            };
+            s = f16v{};
+            __builtin_amdgcn_s_setprio(1);
+            u4 k[2][Tile::kPlanes];
+            read(0, k[0]);
+#pragma unroll
+            for (int c = 0; c < kC; ++c) {
+                if (c + 1 < kC) read(c + 1, k[(c + 1) % 2]);
+                s = mfma_planes<Tile::kPlanes>(k[c % 2], q[c], s);
+            }
+            if constexpr (Tile::kPlanes == 1) {
+                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
 #pragma unroll
                 for (int c = 0; c < kC; ++c) {
-                    if (c + 1 < kC) read(c + 1, k[(c + 1) % 2]);
-                    s = mfma_planes<Tile::kPlanes>(k[c % 2], q[c], s);
-                }
-                if constexpr (Tile::kPlanes == 1) {
                     __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-#pragma unroll
-                    for (int c = 0; c < kC; ++c) {
-                        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-                        __builtin_amdgcn_sched_group_barrier(0x008, 3, 0);
-                    }
+                    __builtin_amdgcn_sched_group_barrier(0x008, 3, 0);
                 }
-                __builtin_amdgcn_s_setprio(0);
             }
-            if (t < tiles) {  // past the last tile the stash rewrites buffers that are not read again
-                stash(next, v_next);
-                load(to);
+            __builtin_amdgcn_s_setprio(0);
+        };
+        const auto scaled = [&](const char* of) {  // the keys' or the values' scales
+            if constexpr (DT == MIMIR_KV_I8) {
+#pragma unroll
+                for (int r = 0; r < 16; r += 4) {
+                    const f4 x = *reinterpret_cast<const f4*>(of + (2 * r + 4 * hf) * 4);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[r + e] *= x[e];
+                }
             }
-            if (active) {
-                if constexpr (DT == MIMIR_KV_I8) {
-#pragma unroll
-                    for (int r = 0; r < 16; r += 4) {
-                        const f4 x = *reinterpret_cast<const f4*>(cur + Tile::kScalesAt + (2 * r + 4 * hf) * 4);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) s[r + e] *= x[e];
-                    }
-                }
-                if (holes || key + kTile > first_end) {
-                    const bool first = !holes || there(key), second = !holes || there(key + kHalf);
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        const int j = key + 8 * (r / 4) + 4 * hf + r % 4;
-                        s[r] = j < my_end && (r < 8 ? first : second) ? s[r] : -INFINITY;
-                    }
-                }
-                float top = s[0];
-#pragma unroll
-                for (int r = 1; r < 16; ++r) top = fmaxf(top, s[r]);
-                if (__any(top > m_run + kPagedSlack)) {
-                    const float m_new = fmaxf(m_run, fmaxf(top, __shfl_xor(top, 32)));
-                    const float f = __builtin_amdgcn_exp2f(m_run - m_new);
-                    m_run = m_new;
-                    l_run *= f;
-#pragma unroll
-                    for (int d = 0; d < kDb; ++d) o[d] *= f;
-                }
-                float sum = 0.f;
+        };
+        // Scores of the tile from `key` on to weights.
+        const auto soften = [&](int key, const char* cur) {
+            if (holes || key + kTile > first_end) {
+                const bool first = !holes || there(key), second = !holes || there(key + kHalf);
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
-                    s[r] = __builtin_amdgcn_exp2f(s[r] - m_run);
-                    sum += s[r];
+                    const int j = key + 8 * (r / 4) + 4 * hf + r % 4;
+                    s[r] = j < my_end && (r < 8 ? first : second) ? s[r] : -INFINITY;
                 }
-                l_run += sum;
-                if constexpr (DT == MIMIR_KV_I8) {
-#pragma unroll
-                    for (int r = 0; r < 16; r += 4) {
-                        const f4 x = *reinterpret_cast<const f4*>(cur + Tile::kScalesAt + (kTile + 2 * r + 4 * hf) * 4);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) s[r + e] *= x[e];
-                    }
-                }
-                if (!late) weigh(v_cur);
             }
-            to = find(t + 3);
-            char* const v_free = kStagger ? v_old : v_cur;
-            v_old = v_cur;
-            v_cur = v_next;
-            v_next = kStagger && t == 0 ? values + 2 * Tile::kValueBytes : v_free;
-            __syncthreads();
+            float top = s[0];
+#pragma unroll
+            for (int r = 1; r < 16; ++r) top = fmaxf(top, s[r]);
+            if (__any(top > m_run + kPagedSlack)) {
+                const float m_new = fmaxf(m_run, fmaxf(top, __shfl_xor(top, 32)));
+                const float f = __builtin_amdgcn_exp2f(m_run - m_new);
+                m_run = m_new;
+                l_run *= f;
+#pragma unroll
+                for (int d = 0; d < kDb; ++d) o[d] *= f;
+            }
+            float sum = 0.f;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                s[r] = __builtin_amdgcn_exp2f(s[r] - m_run);
+                sum += s[r];
+            }
+            l_run += sum;
+            scaled(cur + Tile::kScalesAt + kTile * 4);
+        };
+        if constexpr (kShared) {
+            // One buffer each: a tile's values come in beside its scores' products, the next
+            // tile's keys when all waves have those.
+            f4* const parts = reinterpret_cast<f4*>(values + Tile::kValueBytes);  // [wave][four scores][lane]
+            for (int t = 0; t < tiles; ++t) {
+                const int key = k0 + t * kTile;
+                const bool active = key < wave_end;
+                stash(lds, values, false, true);
+                load(later, false, true);
+                if (active) {
+                    scores(lds);
+                    scaled(lds + Tile::kScalesAt);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) parts[(4 * wave + r) * kWave + lane] = f4{s[4 * r], s[4 * r + 1], s[4 * r + 2], s[4 * r + 3]};
+                }
+                __syncthreads();
+                stash(lds, values, true, false);
+                load(to, true, false);
+                if (active) {
+                    s = f16v{};
+#pragma unroll
+                    for (int g = 0; g < Shape::kShare; ++g)  // in one order for all
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            const f4 x = parts[(4 * (group * Shape::kShare + g) + r) * kWave + lane];
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) s[4 * r + e] += x[e];
+                        }
+                    soften(key, lds);
+                    weigh(values);
+                }
+                later = to;
+                to = find(t + 3);
+                __syncthreads();
+            }
+        } else {
+            const bool late = kStagger && wave >= WAVES / 2;
+            char *v_old = values, *v_cur = values, *v_next = values + Tile::kValueBytes;
+            for (int t = 0; t < tiles + (kStagger ? 1 : 0); ++t) {
+                const char* cur = lds + (t & 1) * Tile::kKeyBytes;
+                char* const next = lds + ((t + 1) & 1) * Tile::kKeyBytes;
+                const int key = k0 + t * kTile;
+                if (kStagger && late && t > 0 && key - kTile < wave_end) weigh(v_old);
+                const bool active = key < wave_end;
+                if (active) scores(cur);
+                if (t < tiles) {  // past the last tile the stash rewrites buffers that are not read again
+                    stash(next, v_next, true, true);
+                    load(to, true, true);
+                }
+                if (active) {
+                    scaled(cur + Tile::kScalesAt);
+                    soften(key, cur);
+                    if (!late) weigh(v_cur);
+                }
+                to = find(t + 3);
+                char* const v_free = kStagger ? v_old : v_cur;
+                v_old = v_cur;
+                v_cur = v_next;
+                v_next = kStagger && t == 0 ? values + 2 * Tile::kValueBytes : v_free;
+                __syncthreads();
+            }
         }
 
-        // The wave's rows out: lane (li, hf) holds dimensions 32 d + 8 (r / 4) + 4 hf + r % 4.
-        if (wave_rows <= 0) continue;
+        // The wave's rows out: lane (li, hf) holds dimensions 32 d + 8 (r / 4) + 4 hf + r % 4 of its own.
+        if (!kShared && wave_rows <= 0) continue;
         const float l_tot = l_run + __shfl_xor(l_run, 32);
         const int row = my_row - w.row0, d_all = p.c.head_dim;
         float* const out = out_row(row);
@@ -418,7 +477,7 @@ __global__ __launch_bounds__(WAVES * kWave, (WAVES / 4 * BlockShape<DT, DP, WAVE
         for (int d = 0; d < kDb; ++d)
 #pragma unroll
             for (int r = 0; r < 16; r += 4) {
-                const int d0 = 32 * d + 8 * (r / 4) + 4 * hf;
+                const int d0 = d_wave + 32 * d + 8 * (r / 4) + 4 * hf;
                 const f4 x{o[d][r] * inv, o[d][r + 1] * inv, o[d][r + 2] * inv, o[d][r + 3] * inv};
 #pragma unroll
                 for (int e = 0; e < 4; ++e) check += x[e] - x[e];
@@ -431,11 +490,19 @@ __global__ __launch_bounds__(WAVES * kWave, (WAVES / 4 * BlockShape<DT, DP, WAVE
                         if (d0 + e < d_all) out[d0 + e] = x[e];
                 }
             }
-        if (!w.whole && in && hf == 0) *part.stat(row) = f2{m_run, l_tot};
+        if (!w.whole && in && hf == 0 && d_wave == 0) *part.stat(row) = f2{m_run, l_tot};
         // Rows that came out NaN or infinite, again in fp32 (as paged_stream).
         const uint64_t ballot = __ballot(check != check && in);
-        for (uint32_t bad = static_cast<uint32_t>(ballot | ballot >> 32); bad; bad &= bad - 1) {
-            const int r = wave * kTile + __builtin_ctz(bad), full = w.row0 + r;
+        auto again = static_cast<uint32_t>(ballot | ballot >> 32);
+        if constexpr (kShared) {  // by the first of the waves, when all have written theirs
+            if (lane == 0) bad[wave] = again;
+            __syncthreads();
+            if (d_wave > 0) continue;
+#pragma unroll
+            for (int g = 1; g < Shape::kShare; ++g) again |= uniform(bad[wave + g]);
+        }
+        for (; again; again &= again - 1) {
+            const int r = group * kTile + __builtin_ctz(again), full = w.row0 + r;
             float acc[kRowChunks], m, l;
             row_over_keys<DT>(p, w.s, w.head, q_row(full), k0, min(k1, row_end(p, w.seq, full)), acc, &m, &l);
             float* const to = out_row(r);
@@ -450,7 +517,7 @@ __global__ __launch_bounds__(WAVES * kWave, (WAVES / 4 * BlockShape<DT, DP, WAVE
 
 template <int DT, int DP, int WAVES>
 int launch(mimir_ctx* ctx, const PagedArgs& p, PagedRuns a, PagedRuns* left) {
-    a.block_rows = a.part_rows = WAVES * kTile;
+    a.block_rows = a.part_rows = BlockShape<DT, DP, WAVES>::kRows;
     const int64_t rows = static_cast<int64_t>(p.b.max_new) * p.group;
     a.row_blocks = static_cast<int32_t>((rows + a.block_rows - 1) / a.block_rows);
     const int64_t blocks = static_cast<int64_t>(p.b.sequences) * p.c.kv_heads * a.row_blocks;
@@ -465,7 +532,12 @@ int launch(mimir_ctx* ctx, const PagedArgs& p, PagedRuns a, PagedRuns* left) {
 
 template <int DT, int DP>
 int launch_waves(mimir_ctx* ctx, const PagedArgs& p, const PagedRuns& a, PagedRuns* left) {
-    int waves = static_cast<int64_t>(p.b.max_new) * p.group <= 4 * kTile || p.b.max_len <= kWholeLen ? 4 : 8;
+    // Four for few rows and for short contexts; where a compute unit holds but one of four,
+    // only if those are one round (fp32 heads of 128, four / eight: one prompt of 250 tokens
+    // 38 / 44 us, 30 of up to 100 58 / 44).
+    const int64_t rows = static_cast<int64_t>(p.b.max_new) * p.group;
+    const int64_t blocks = static_cast<int64_t>(p.b.sequences) * p.c.kv_heads * ((rows + 4 * kTile - 1) / (4 * kTile));
+    int waves = rows <= 4 * kTile || (p.b.max_len <= kWholeLen && (BlockShape<DT, DP, 4>::kResident == 2 || blocks <= 256)) ? 4 : 8;
     if (ctx->tune.attn_waves == 4 || ctx->tune.attn_waves == 8) waves = ctx->tune.attn_waves;
     return waves == 4 ? launch<DT, DP, 4>(ctx, p, a, left) : launch<DT, DP, 8>(ctx, p, a, left);
 }
@@ -474,7 +546,8 @@ template <int DT>
 int launch_dim(mimir_ctx* ctx, const PagedArgs& p, const PagedRuns& a, PagedRuns* left) {
     if (p.c.stride <= 64) return launch_waves<DT, 64>(ctx, p, a, left);
     if (p.c.stride <= 96) return launch_waves<DT, 96>(ctx, p, a, left);
-    return launch_waves<DT, 128>(ctx, p, a, left);
+    if (p.c.stride <= 128) return launch_waves<DT, 128>(ctx, p, a, left);
+    return launch<DT, 256, 8>(ctx, p, a, left);
 }
 
 }  // namespace

@@ -489,10 +489,11 @@ int mimir::paged_stream_launch(mimir_ctx* ctx, const PagedArgs& p, int dtype, in
     constexpr uint32_t kStep = 2 * kHalf * kStreamWaves;
     const int64_t rows = std::min(static_cast<int64_t>(p.b.max_new) * p.group, most_rows);
     // A sequence's second tile shares the first one's keys, unless other sequences have more rows
-    // than this kernel takes: then single tokens are what most have.  (For wide fp32
-    // heads two tiles are more than the registers hold.)
-    const bool wide = dtype == MIMIR_KV_F32 && p.c.stride > 128;
-    const int tiles = rows > kRows && !wide && !beside ? 2 : 1;
+    // than this kernel takes: then single tokens are what most have.  (Wide fp32 heads,
+    // of which two tiles are more than the registers hold, come with one at most.)
+    const int tiles = rows > kRows && !beside ? 2 : 1;
+    MIMIR_REQUIRE(ctx, tiles == 1 || dtype != MIMIR_KV_F32 || p.c.stride <= 128, "paged attention: %lld rows of a wide head",
+                  (long long)rows);
     PagedRuns a{};
     a.extra = 2 * kStep;  // the queries, the first keys' way in, the sums' way out
     a.slack = a.extra;

@@ -400,3 +400,67 @@ def test_runs_over_thousands_of_sequences(ctx, dtype):
     p.ld = p.table.shape[1]
     fill(p, kv)
     check(attend(ctx, p, q), p, q, kv)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("lens,kh,heads,d,page", [
+    ([(65, 65)], 1, 1, 256, 16),
+    ([(128, 300)], 2, 2, 256, 48),
+    ([(129, 129), (1, 700), (33, 1200), (0, 9)], 1, 2, 256, 16),
+    ([(200, 1500), (70, 70)], 1, 3, 192, 32),
+    ([(90, 91)], 2, 4, 144, 16),
+    ([(100, 160)], 1, 1, 130, 16),
+    ([(67, 900)], 1, 2, 201, 64),
+    ([(80, 20), (300, 300)], 1, 1, 250, 16),
+])
+def test_wide_heads_of_many_rows(ctx, dtype, lens, kh, heads, d, page):
+    q, kv = case(d + page, dtype, lens, kh, heads, d)
+    p = Paged(ctx, dtype, lens, kh, d, page)
+    fill(p, kv)
+    check(attend(ctx, p, q), p, q, kv)
+    check(attend(ctx, p, q, causal=False, ld_extra=1, offset=3), p, q, kv, causal=False)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("tune", ["paged=1", "paged=7", "paged=256"])
+def test_wide_heads_dealt_to_any_number_of_workgroups(dtype, tune):
+    c = tuned_context(tune)
+    try:
+        lens = [(150, 700), (70, 640), (1, 1300)]
+        q, kv = case(50, dtype, lens, 1, 2, 256)
+        p = Paged(c, dtype, lens, 1, 256, 16)
+        fill(p, kv)
+        check(attend(c, p, q), p, q, kv)
+    finally:
+        c.close()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_wide_heads_holes_and_nan(ctx, dtype):
+    """Pages that are none, a NaN in one dimension, in a key that some rows see, and in
+    what no row sees (slots without tokens are NaN in every test)."""
+    lens, d, m = [(100, 500)], 256, 500
+    q, kv = case(51, dtype, lens, 1, 1, d)
+    k, v = kv[0]
+    p = Paged(ctx, dtype, lens, 1, d, 16)
+    fill(p, kv)
+    p.table[0, 3] = -1
+    keep = np.array([j for j in range(m) if j // 16 != 3])
+    got = attend(ctx, p, q, causal=False)
+    want, tol = attention64(q, held(k, dtype)[keep], held(v, dtype)[keep], 0, False, scale_of(d))
+    assert (np.abs(got - want) <= tol).all()
+    p = Paged(ctx, dtype, lens, 1, d, 16)
+    if dtype != "i8":
+        v[100, 0, 200] = np.nan
+    k[450, 0, 7] = np.nan
+    fill(p, kv)
+    got = attend(ctx, p, q)
+    vz = v.copy()
+    vz[100, 0, 200] = 0 if dtype != "i8" else vz[100, 0, 200]
+    want, tol = attention64(q[:50], held(k, dtype)[:450], held(vz, dtype)[:450], 400, True, scale_of(d))
+    ok = np.ones(want.shape, bool)
+    if dtype != "i8":
+        ok[:, :, 200] = False
+        assert np.isnan(got[:, :, 200]).all()
+    assert (np.abs(got[:50] - want) <= tol)[ok].all()
+    assert np.isnan(got[50:]).all()

@@ -31,7 +31,8 @@ constexpr int64_t kStreamRows = 64, kStreamBeside = 32, kStreamWide = 16;
 // is the workgroup's, kept what it begins, the others what they go on with.  `parts`
 // workgroups for each descriptor.
 template <int LPR, bool ONE>
-__device__ __forceinline__ void join_rows(const PagedArgs& p, const PagedRuns& a, uint32_t parts, uint32_t block, f4 (*share)[LPR], f2* stats) {
+__device__ __forceinline__ void join_rows(const PagedArgs& p, const PagedRuns& a, uint32_t parts, uint32_t block,
+                                          f4 (*share)[LPR], f2* stats) {
     constexpr int kAhead = 4, kGroups = kBlock / LPR, kEach = ONE ? kGroups : 1, kRowsOf = ONE ? 1 : kGroups;
     const uint32_t first = block / parts;
     const PagedShared s = a.shared[first];
@@ -135,7 +136,7 @@ int64_t mimir::paged_runs(mimir_ctx* ctx, const PagedArgs& p, PagedRuns* a, int6
     a->apart = p.b.sequences <= kWave;
     a->many = a->part_rows <= 32 && runs > 4 * blocks;
     constexpr size_t kAlone = kPagedWorkBytes - kPagedBesideBytes;
-    const int64_t bytes = runs * static_cast<int64_t>(sizeof(PagedShared)) + runs * 2 * paged_part_floats(a->part_rows, p.c.head_dim) * 4;
+    const int64_t bytes = runs * (static_cast<int64_t>(sizeof(PagedShared)) + 2 * 4 * paged_part_floats(a->part_rows, p.c.head_dim));
     if (!split || bytes > static_cast<int64_t>(beside ? kPagedBesideBytes : kAlone)) return blocks;
     char* work = paged_work(ctx);
     if (!work) return blocks;
@@ -189,7 +190,8 @@ extern "C" int mimir_attention_paged_fwd(mimir_ctx* ctx, const mimir_kv_cache* c
     if (rows <= streamed) {
         if (int st = paged_stream_launch(ctx, a, cache->dtype, INT32_MAX, false, &few)) return st;
     } else {
-        const bool both = a.b.sequences * static_cast<int64_t>(a.b.max_new) > a.b.tokens && (a.b.max_len > kWholeLen || static_cast<int64_t>(a.b.sequences) * a.c.kv_heads > pairs);
+        const int64_t sequences = a.b.sequences;
+        const bool both = sequences * a.b.max_new > a.b.tokens && (a.b.max_len > kWholeLen || sequences * a.c.kv_heads > pairs);
         if (both)
             if (int st = paged_stream_launch(ctx, a, cache->dtype, std::min(streamed, kStreamBeside), true, &few)) return st;
         if (int st = paged_block_launch(ctx, a, cache->dtype, both ? std::min(streamed, kStreamBeside) + 1 : 1, &others)) return st;

@@ -111,7 +111,8 @@ __device__ __forceinline__ uint64_t lanes_up_to(uint64_t sum) {
 
 // The costs of the sequences from `base` on up to the lane's; wave 0 writes them down.
 // The lane's own is left in `cost`.
-__device__ __forceinline__ uint64_t paged_chunk(const PagedArgs& p, const PagedRuns& a, int base, PagedChunk* chunk, PagedCost* cost) {
+__device__ __forceinline__ uint64_t paged_chunk(const PagedArgs& p, const PagedRuns& a, int base, PagedChunk* chunk,
+                                                PagedCost* cost) {
     const int lane = static_cast<int>(threadIdx.x % kWave);
     KvSequence seq{0, 0, 0};
     *cost = PagedCost{1, 0, 0};
@@ -130,7 +131,8 @@ __device__ __forceinline__ uint64_t paged_chunk(const PagedArgs& p, const PagedR
 
 // Keys that row `row` (of all its sequence's) sees.
 __device__ __forceinline__ int row_end(const PagedArgs& p, const KvSequence& q, int row) {
-    return p.causal ? min(max(q.len - q.n + static_cast<int>(fastdiv(static_cast<uint32_t>(row), p.group_div)) + 1, 0), q.len) : q.len;
+    if (!p.causal) return q.len;
+    return min(max(q.len - q.n + static_cast<int>(fastdiv(static_cast<uint32_t>(row), p.group_div)) + 1, 0), q.len);
 }
 
 // A run's part of a block.
@@ -243,7 +245,8 @@ struct PagedWalk {
             w.seq = kv_sequence(p.b, w.s);
             w.row0 = static_cast<int>(index % static_cast<uint32_t>(a.row_blocks)) * a.block_rows;
             const int64_t all = static_cast<int64_t>(w.seq.n) * p.group;
-            w.rows = all >= a.least_rows && all <= a.most_rows ? static_cast<int>(min(all - w.row0, static_cast<int64_t>(a.block_rows))) : 0;
+            const bool ours = all >= a.least_rows && all <= a.most_rows;
+            w.rows = ours ? static_cast<int>(min(all - w.row0, static_cast<int64_t>(a.block_rows))) : 0;
             w.k0 = 0;
             w.k1 = w.rows > 0 ? row_end(p, w.seq, w.row0 + w.rows - 1) : 0;
             w.whole = w.begins = true;
@@ -295,7 +298,8 @@ struct PagedWalk {
         w.begins = x0 == 0;
         w.whole = w.begins && x1 == all;
         if (threadIdx.x == 0 && w.begins && !w.whole)
-            a.shared[index] = PagedShared{static_cast<int32_t>(quotient(first + all - 1, run) - index) + 1, w.seq.first, w.row0, w.rows, w.head, {}};
+            a.shared[index] = PagedShared{static_cast<int32_t>(quotient(first + all - 1, run) - index) + 1, w.seq.first, w.row0,
+                                          w.rows, w.head, {}};
         from = uniform(first + x1);
         // None that a later run goes on with.
         if (threadIdx.x == 0 && from >= end && (w.whole || !w.begins)) a.shared[index].runs = 0;
@@ -306,7 +310,9 @@ struct PagedWalk {
 // Where a run keeps the sums of a block that it shares with others, the one that it
 // begins or goes on with: a max and a sum per row, then rows of head_dim sums from
 // 16-byte boundaries on.
-__host__ __device__ inline int64_t paged_part_stats(int part_rows) { return (2 * static_cast<int64_t>(part_rows) + 3) & ~int64_t{3}; }
+__host__ __device__ inline int64_t paged_part_stats(int part_rows) {
+    return (2 * static_cast<int64_t>(part_rows) + 3) & ~int64_t{3};
+}
 __host__ __device__ inline int64_t paged_part_stride(int head_dim) { return (head_dim + 3) & ~3; }
 __host__ __device__ inline int64_t paged_part_floats(int part_rows, int head_dim) {
     return paged_part_stats(part_rows) + part_rows * paged_part_stride(head_dim);

@@ -120,7 +120,8 @@ struct BlockShape {
 };
 
 template <int DT, int DP, int WAVES>
-__global__ __launch_bounds__(WAVES * kWave, (WAVES / 4 * BlockShape<DT, DP, WAVES>::kResident)) void paged_block(PagedArgs p, PagedRuns a) {
+__global__ __launch_bounds__(WAVES * kWave, (WAVES / 4 * BlockShape<DT, DP, WAVES>::kResident)) void paged_block(PagedArgs p,
+                                                                                                              PagedRuns a) {
     using Tile = BlockTile<DT, DP>;
     using Shape = BlockShape<DT, DP, WAVES>;
     constexpr int kThreads = WAVES * kWave, kC = Shape::kDims / 16, kDb = Shape::kDims / 32;
@@ -136,7 +137,8 @@ __global__ __launch_bounds__(WAVES * kWave, (WAVES / 4 * BlockShape<DT, DP, WAVE
     __shared__ uint32_t bad[WAVES];  // shared: the rows that came out NaN or infinite of each wave
 
     // Each XCD takes runs that follow each other, whose keys it has in its L2.
-    const uint32_t at = a.runs % kXcds == 0 && gridDim.x == a.runs ? blockIdx.x % kXcds * (a.runs / kXcds) + blockIdx.x / kXcds : blockIdx.x;
+    const bool dealt = a.runs % kXcds == 0 && gridDim.x == a.runs;
+    const uint32_t at = dealt ? blockIdx.x % kXcds * (a.runs / kXcds) + blockIdx.x / kXcds : blockIdx.x;
     const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave);
     const int group = wave / Shape::kShare, d_wave = wave % Shape::kShare * Shape::kDims;  // its rows, its dimensions
     for (PagedWalk walk(p, a, at, &chunk); walk.more();) {
@@ -166,8 +168,10 @@ __global__ __launch_bounds__(WAVES * kWave, (WAVES / 4 * BlockShape<DT, DP, WAVE
         const scalar_i32 table = (scalar_i32)(p.b.page_table + w.s * p.b.ld_pages);
         const int row_bytes = p.c.stride * kElement;
         const auto pages = static_cast<uint32_t>(p.c.pages);
-        const auto entry_of = [&](int j) { return fastdiv(static_cast<uint32_t>(max(min(j, (k1 - 1) & -kHalf), 0)), p.c.page_div); };
-        const auto there = [&](int j) { return static_cast<uint32_t>(table[entry_of(j)]) < pages; };
+        const auto there = [&](int j) {  // the half of a tile from key j on
+            const auto i = static_cast<uint32_t>(max(min(j, (k1 - 1) & -kHalf), 0));
+            return static_cast<uint32_t>(table[fastdiv(i, p.c.page_div)]) < pages;
+        };
         // Whether a page of these keys is none.
         bool holes = false;
         if (tiles > 0) {
@@ -188,8 +192,10 @@ __global__ __launch_bounds__(WAVES * kWave, (WAVES / 4 * BlockShape<DT, DP, WAVE
         const int d_mine = 8 * (tid % kLanes);
         const auto row_of = [&](int n) { return (tid + n * kThreads) / kLanes; };
         const auto half_of = [&](int n) { return kItems == 2 ? n : wave / kMovers; };
-        const uint32_t off = d_mine < p.c.stride ? static_cast<uint32_t>(row_of(0) % kHalf * row_bytes + d_mine * kElement) : kOutside;
-        const int64_t page_rows = static_cast<int64_t>(p.c.kv_heads) * p.c.page_size, head_rows = static_cast<int64_t>(w.head) * p.c.page_size;
+        const auto mine = static_cast<uint32_t>(row_of(0) % kHalf * row_bytes + d_mine * kElement);
+        const uint32_t off = d_mine < p.c.stride ? mine : kOutside;
+        const int64_t head_rows = static_cast<int64_t>(w.head) * p.c.page_size;
+        const int64_t page_rows = static_cast<int64_t>(p.c.kv_heads) * p.c.page_size;
         const bool mover = kItems == 2 || half_of(0) < 2;
         // Where an item's half stands, and how many of its keys are there.
         struct Halves {
@@ -222,7 +228,8 @@ __global__ __launch_bounds__(WAVES * kWave, (WAVES / 4 * BlockShape<DT, DP, WAVE
                 if (values_too) vi[n].load(__builtin_amdgcn_make_buffer_rsrc(p.c.v + at, 0, keys * row_bytes, kBufferWord3), off);
                 if constexpr (DT == MIMIR_KV_I8)
                     if (scales < 2 && (scales ? values_too : keys_too))
-                        scale[n] = buffer_f1(buffer_of((scales ? p.c.v_scale : p.c.k_scale) + row, 4 * keys), static_cast<uint32_t>(4 * (lane % kHalf)));
+                        scale[n] = buffer_f1(buffer_of((scales ? p.c.v_scale : p.c.k_scale) + row, 4 * keys),
+                                             static_cast<uint32_t>(4 * (lane % kHalf)));
             }
         };
         // Both kinds' scales stand beside the keys.
@@ -298,7 +305,8 @@ __global__ __launch_bounds__(WAVES * kWave, (WAVES / 4 * BlockShape<DT, DP, WAVE
                 const char* const at = buf + v_lane + 16 * (i / kDb) * Tile::kValueRow + 64 * (i % kDb);
 #pragma unroll
                 for (int n = 0; n < Tile::kPlanes; ++n) {
-                    const u2 x0 = __builtin_bit_cast(u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(at + n * Tile::kValuePlane)));
+                    const u2 x0 = __builtin_bit_cast(
+                        u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(at + n * Tile::kValuePlane)));
                     const u2 x1 = __builtin_bit_cast(
                         u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(at + n * Tile::kValuePlane + 8 * Tile::kValueRow)));
                     v[n] = u4{x0[0], x0[1], x1[0], x1[1]};
@@ -341,7 +349,8 @@ __global__ __launch_bounds__(WAVES * kWave, (WAVES / 4 * BlockShape<DT, DP, WAVE
             const auto read = [&](int c, u4* k) {
 #pragma unroll
                 for (int n = 0; n < Tile::kPlanes; ++n)
-                    k[n] = *reinterpret_cast<const u4*>(cur + n * Tile::kKeyPlane + li * Tile::kKeyRow + 2 * d_wave + 32 * c + 16 * hf);
+                    k[n] = *reinterpret_cast<const u4*>(cur + n * Tile::kKeyPlane + li * Tile::kKeyRow + 2 * d_wave + 32 * c +
+                                                        16 * hf);
             };
             s = f16v{};
             __builtin_amdgcn_s_setprio(1);
@@ -415,7 +424,8 @@ __global__ __launch_bounds__(WAVES * kWave, (WAVES / 4 * BlockShape<DT, DP, WAVE
                     scores(lds);
                     scaled(lds + Tile::kScalesAt);
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) parts[(4 * wave + r) * kWave + lane] = f4{s[4 * r], s[4 * r + 1], s[4 * r + 2], s[4 * r + 3]};
+                    for (int r = 0; r < 4; ++r)
+                        parts[(4 * wave + r) * kWave + lane] = f4{s[4 * r], s[4 * r + 1], s[4 * r + 2], s[4 * r + 3]};
                 }
                 __syncthreads();
                 stash(lds, values, true, false);

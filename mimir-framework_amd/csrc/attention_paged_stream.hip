@@ -264,7 +264,8 @@ __global__ __launch_bounds__(kStreamWaves * kWave, stream_waves(DT, DP, TILES)) 
                 const __amdgpu_buffer_rsrc_t rows = half_rows(p.c.v, at, keys);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) vr[u / 2].load(4 * (u % 2) + e, rows, v_off, e * row_bytes);
-                if constexpr (DT == MIMIR_KV_I8) vs[u] = buffer_f4(buffer_of(p.c.v_scale + at, 4 * keys), static_cast<uint32_t>(16 * hg));
+                if constexpr (DT == MIMIR_KV_I8)
+                    vs[u] = buffer_f4(buffer_of(p.c.v_scale + at, 4 * keys), static_cast<uint32_t>(16 * hg));
             }
         };
 
@@ -509,7 +510,8 @@ int mimir::paged_stream_launch(mimir_ctx* ctx, const PagedArgs& p, int dtype, in
     // sequences x 8 heads: bf16 heads of 128, 500 keys 10 / 14, 1000 18 / 16; fp32 500 23 / 21, 1000 41 / 28; fp32
     // heads of 256 500 57 / 42; 32 sequences, fp32 heads of 128 and 256, 500 keys 30 / 34, 70 / 74.
     const int64_t key_bytes = 2 * static_cast<int64_t>(p.c.stride) * kv_element_bytes(dtype);
-    const bool whole = p.b.max_len <= static_cast<int64_t>(8 * kStep) && (p.b.max_len * key_bytes <= 448 * 1024 || 2 * blocks >= runs);
+    const bool small = p.b.max_len * key_bytes <= 448 * 1024 || 2 * blocks >= runs;
+    const bool whole = small && p.b.max_len <= static_cast<int64_t>(8 * kStep);
     const int64_t grid = paged_runs(ctx, p, &a, runs, blocks, !whole, beside);
     MIMIR_REQUIRE(ctx, dispatch_fits(grid, kStreamWaves * kWave), "paged attention: grid of %lld workgroups exceeds the limit",
                   (long long)grid);

@@ -464,3 +464,39 @@ def test_wide_heads_holes_and_nan(ctx, dtype):
         assert np.isnan(got[:, :, 200]).all()
     assert (np.abs(got[:50] - want) <= tol)[ok].all()
     assert np.isnan(got[50:]).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,d", [(3, 64), (100, 64), (100, 256)])
+@pytest.mark.parametrize("pages", [0, 2])
+def test_no_keys_at_all(ctx, dtype, n, d, pages):
+    """A cache without pages, or a call whose bound is no keys: rows of zeros, nothing
+    written, rows read back as zeros."""
+    cache = M.KVCache(ctx, dtype, pages, 16, 1, d)
+    up = ctx.to_device
+    batch = M.KVBatch(up(np.array([0, n], np.int32)), up(np.array([n], np.int32)), None, 1, n, 0, n, 0)
+    try:
+        x = up(np.ones((n, d), np.float32))
+        out = up(np.full((n, 2 * d), 5.0, np.float32))
+        ctx.kv_append(cache, batch, x, x)
+        ctx.attention_paged(cache, batch, up(np.ones((n, 2 * d), np.float32)), out, 2)
+        assert not out.numpy().any()
+        back = up(np.full((n, d), 5.0, np.float32))
+        ctx.kv_read(cache, batch, back, None)
+        assert not back.numpy().any()
+    finally:
+        cache.close()
+
+
+def test_pages_that_two_sequences_share(ctx):
+    """A prefix that is in the cache once."""
+    d, page, m = 32, 16, 40000
+    q, kv = case(60, "bf16", [(1, m)], 1, 4, d)
+    p = Paged(ctx, "bf16", [(1, m), (1, 0)], 1, d, page)
+    fill(p, [kv[0], (kv[0][0][:0], kv[0][1][:0])])
+    p.table[1, :] = p.table[0, :]
+    p.kv_len = np.array([m, 1000], np.int32)
+    p.lens = [(1, m), (1, 1000)]
+    q2 = np.concatenate([q, q])
+    got = attend(ctx, p, q2)
+    check(got, p, q2, [kv[0], (kv[0][0][:1000], kv[0][1][:1000])])

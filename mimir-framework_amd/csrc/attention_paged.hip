@@ -132,7 +132,7 @@ int join(mimir_ctx* ctx, const PagedArgs& p, const PagedRuns& a, const PagedRuns
 int64_t mimir::paged_runs(mimir_ctx* ctx, const PagedArgs& p, PagedRuns* a, int64_t runs, int64_t blocks, bool split, bool beside) {
     // No more than keep to the least length of a run (PagedWalk), by the longest costs, each block's last one shorter.
     const int64_t cost = a->extra + static_cast<int64_t>(p.b.max_len) + (p.causal ? (a->block_rows + p.group - 1) / p.group : 0);
-    if (blocks < 1 << 24) runs = std::max<int64_t>(1, std::min(runs, blocks * (cost / (a->extra + a->grain) + 1)));
+    if (blocks < 1 << 24) runs = std::max<int64_t>(1, std::min(runs, blocks * (cost / a->least + 1)));
     a->apart = p.b.sequences <= kWave;
     a->many = a->part_rows <= 32 && runs > 4 * blocks;
     constexpr size_t kAlone = kPagedWorkBytes - kPagedBesideBytes;

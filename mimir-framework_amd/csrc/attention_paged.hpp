@@ -35,7 +35,7 @@ typedef const __attribute__((address_space(4))) int32_t* scalar_i32;
 // to the workgroups in equal runs, so that sequences of any lengths fill the GPU
 // evenly; a run may begin and end inside a block, whose parts paged_join adds up.
 // Every wave works out its run from the sequences' lengths, 64 of them at a time.
-// Sequences of 1 to 8191 keys, 64 of them x 8 heads, 8-bit: 112 us, with as many parts
+// Sequences of 1 to 8191 keys, 64 of them x 8 heads, 8-bit: 109 us, with as many parts
 // a sequence for all 210.  One sequence of 3000 keys: 20 us, with runs that end where
 // blocks do 16; chunks of 217 tokens of 3 sequences over 2700 to 3200 keys 94 and 92.
 
@@ -53,6 +53,7 @@ struct PagedRuns {
     float* part;
     uint32_t runs;
     uint32_t extra;      // what a block costs besides its keys, in keys
+    uint32_t least;      // length of a run at least
     uint32_t slack;      // how much longer a run may be for all to be of one block
     uint32_t grain;      // blocks are cut at multiples of this many keys, a power of two
     int32_t block_rows;
@@ -192,7 +193,7 @@ struct PagedWalk {
             sum = lanes_up_to(mine);
         }
         uint64_t total = lane_of(sum, kWave - 1);
-        run = uniform(max(quotient(total + a.runs - 1, a.runs), static_cast<uint64_t>(a.extra + a.grain)));
+        run = uniform(max(quotient(total + a.runs - 1, a.runs), static_cast<uint64_t>(a.least)));
         if (a.apart) total = set_apart(p, a, total, cost);
         from = uniform(min(total, run * index));
         end = uniform(min(total, from + run));

@@ -565,6 +565,7 @@ int launch_dim(mimir_ctx* ctx, const PagedArgs& p, const PagedRuns& a, PagedRuns
 int mimir::paged_block_launch(mimir_ctx* ctx, const PagedArgs& p, int dtype, int64_t least_rows, PagedRuns* left) {
     PagedRuns a{};
     a.extra = 4 * kTile;
+    a.least = 5 * kTile;
     a.slack = 8 * kTile;
     a.grain = kTile;
     a.least_rows = static_cast<int32_t>(least_rows);

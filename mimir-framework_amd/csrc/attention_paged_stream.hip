@@ -496,8 +496,13 @@ int mimir::paged_stream_launch(mimir_ctx* ctx, const PagedArgs& p, int dtype, in
     MIMIR_REQUIRE(ctx, tiles == 1 || dtype != MIMIR_KV_F32 || p.c.stride <= 128, "paged attention: %lld rows of a wide head",
                   (long long)rows);
     PagedRuns a{};
-    a.extra = 2 * kStep;  // the queries, the first keys' way in, the sums' way out
-    a.slack = a.extra;
+    // The queries, the first keys' way in, the sums' way out take as long whatever a key's bytes.  Two / three / four
+    // steps, 64 ragged sequences of up to 8191 keys, us: 8-bit heads of 128 115 / 109 / 109, of 64 75 / 67 / 64, bf16
+    // of 128, up to 4096, 96 / 97 / 99, fp32 209 / 214 / 217.
+    const int64_t key_bytes = 2 * static_cast<int64_t>(p.c.stride) * kv_element_bytes(dtype);
+    a.extra = (key_bytes >= 512 ? 2 : key_bytes >= 256 ? 3 : 4) * kStep;
+    a.least = 3 * kStep;
+    a.slack = 2 * kStep;
     a.grain = kStep;
     a.block_rows = kRows * tiles;
     a.least_rows = 1;
@@ -509,7 +514,6 @@ int mimir::paged_stream_launch(mimir_ctx* ctx, const PagedArgs& p, int dtype, in
     // Short blocks are not worth a join, by the bytes of one where they do not fill the GPU.  Whole / cut, us, two
     // sequences x 8 heads: bf16 heads of 128, 500 keys 10 / 14, 1000 18 / 16; fp32 500 23 / 21, 1000 41 / 28; fp32
     // heads of 256 500 57 / 42; 32 sequences, fp32 heads of 128 and 256, 500 keys 30 / 34, 70 / 74.
-    const int64_t key_bytes = 2 * static_cast<int64_t>(p.c.stride) * kv_element_bytes(dtype);
     const bool small = p.b.max_len * key_bytes <= 448 * 1024 || 2 * blocks >= runs;
     const bool whole = small && p.b.max_len <= static_cast<int64_t>(8 * kStep);
     const int64_t grid = paged_runs(ctx, p, &a, runs, blocks, !whole, beside);

@@ -450,7 +450,10 @@ __global__ __launch_bounds__(WAVES * kWave, (WAVES / 4 * BlockShape<DT, DP, WAVE
         } else {
             const bool late = kStagger && wave >= WAVES / 2;
             char *v_old = values, *v_cur = values, *v_next = values + Tile::kValueBytes;
-            for (int t = 0; t < tiles + (kStagger ? 1 : 0); ++t) {
+            // One more for the late waves; a block without keys has no turn: its sequence may
+            // have no page table to find a tile's page in.
+            const int turns = kStagger && tiles > 0 ? tiles + 1 : tiles;
+            for (int t = 0; t < turns; ++t) {
                 const char* cur = lds + (t & 1) * Tile::kKeyBytes;
                 char* const next = lds + ((t + 1) & 1) * Tile::kKeyBytes;
                 const int key = k0 + t * kTile;

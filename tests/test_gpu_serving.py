@@ -488,6 +488,45 @@ def test_no_keys_at_all(ctx, dtype, n, d, pages):
         cache.close()
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d", [64, 80, 128])
+@pytest.mark.parametrize("waves", [4, 8])
+@pytest.mark.parametrize("pages", [0, 2])
+def test_no_keys_and_no_page_table_by_waves(dtype, d, waves, pages):
+    """As above by each width of the kernel of many rows: eight waves take one turn more
+    than there are tiles, of which there are none."""
+    c = tuned_context(f"attnwaves={waves}")
+    try:
+        n, count = 140, 3
+        cache = M.KVCache(c, dtype, pages, 16, 1, d)
+        up = c.to_device
+        batch = M.KVBatch(up((np.arange(count + 1) * n).astype(np.int32)), up(np.zeros(count, np.int32)), None, count, count * n,
+                          0, n, 0)
+        out = up(np.full((count * n, d), 5.0, np.float32))
+        c.attention_paged(cache, batch, up(np.ones((count * n, d), np.float32)), out, 1)
+        assert not out.numpy().any()
+        cache.close()
+    finally:
+        c.close()
+
+
+@pytest.mark.parametrize("d", [100, 128])
+def test_no_keys_and_no_page_table_in_more_blocks_than_workgroups(ctx, d):
+    """fp32 heads of 97 to 128, more blocks of 128 rows than the GPU has compute units:
+    eight waves by the rule of sizes alone."""
+    n, count = 129, 150  # two blocks of 128 rows a sequence, 300 in all
+    cache = M.KVCache(ctx, "f32", 2, 16, 1, d)
+    try:
+        up = ctx.to_device
+        batch = M.KVBatch(up((np.arange(count + 1) * n).astype(np.int32)), up(np.zeros(count, np.int32)), None, count, count * n,
+                          0, n, 0)
+        out = up(np.full((count * n, d), 5.0, np.float32))
+        ctx.attention_paged(cache, batch, up(np.ones((count * n, d), np.float32)), out, 1)
+        assert not out.numpy().any()
+    finally:
+        cache.close()
+
+
 def test_pages_that_two_sequences_share(ctx):
     """A prefix that is in the cache once."""
     d, page, m = 32, 16, 40000

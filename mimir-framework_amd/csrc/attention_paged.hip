@@ -129,7 +129,9 @@ int join(mimir_ctx* ctx, const PagedArgs& p, const PagedRuns& a, const PagedRuns
 
 }  // namespace
 
-int64_t mimir::paged_runs(mimir_ctx* ctx, const PagedArgs& p, PagedRuns* a, int64_t runs, int64_t blocks, bool split, bool beside) {
+int64_t mimir::paged_runs(mimir_ctx* ctx, const PagedArgs& p, PagedRuns* a, int64_t runs, int64_t blocks, int threads, bool split,
+                          bool beside) {
+    split = split || !dispatch_fits(blocks, threads);
     // No more than keep to the least length of a run (PagedWalk), by the longest costs, each block's last one shorter.
     const int64_t cost = a->extra + static_cast<int64_t>(p.b.max_len) + (p.causal ? (a->block_rows + p.group - 1) / p.group : 0);
     if (blocks < 1 << 24) runs = std::max<int64_t>(1, std::min(runs, blocks * (cost / a->least + 1)));

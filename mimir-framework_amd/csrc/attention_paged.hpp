@@ -461,7 +461,10 @@ int paged_block_launch(mimir_ctx* ctx, const PagedArgs& p, int dtype, int64_t le
 constexpr int kWholeLen = 256;
 
 // Sets up `a` for at most `runs` workgroups in the workspace, or for one per block
-// (`blocks` of them) where that is not to be had or `split` says not to; the grid.
-int64_t paged_runs(mimir_ctx* ctx, const PagedArgs& p, PagedRuns* a, int64_t runs, int64_t blocks, bool split, bool beside);
+// (`blocks` of them) where that is not to be had or `split` says not to, which it may not
+// where so many do not fit a launch (of `threads` each): most are then of rows that max_new
+// allows and no sequence has.  The grid.
+int64_t paged_runs(mimir_ctx* ctx, const PagedArgs& p, PagedRuns* a, int64_t runs, int64_t blocks, int threads, bool split,
+                   bool beside);
 
 }  // namespace mimir

@@ -535,7 +535,7 @@ int launch(mimir_ctx* ctx, const PagedArgs& p, PagedRuns a, PagedRuns* left) {
     a.row_blocks = static_cast<int32_t>((rows + a.block_rows - 1) / a.block_rows);
     const int64_t blocks = static_cast<int64_t>(p.b.sequences) * p.c.kv_heads * a.row_blocks;
     const int64_t runs = ctx->tune.paged_runs > 0 ? ctx->tune.paged_runs : 256 * BlockShape<DT, DP, WAVES>::kResident;
-    const int64_t grid = paged_runs(ctx, p, &a, runs, blocks, p.b.max_len > kWholeLen, false);
+    const int64_t grid = paged_runs(ctx, p, &a, runs, blocks, WAVES * kWave, p.b.max_len > kWholeLen, false);
     MIMIR_REQUIRE(ctx, dispatch_fits(grid, WAVES * kWave), "paged attention: grid of %lld workgroups exceeds the limit",
                   (long long)grid);
     paged_block<DT, DP, WAVES><<<static_cast<unsigned>(grid), WAVES * kWave, 0, ctx->stream>>>(p, a);

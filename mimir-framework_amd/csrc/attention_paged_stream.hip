@@ -516,7 +516,7 @@ int mimir::paged_stream_launch(mimir_ctx* ctx, const PagedArgs& p, int dtype, in
     // heads of 256 500 57 / 42; 32 sequences, fp32 heads of 128 and 256, 500 keys 30 / 34, 70 / 74.
     const bool small = p.b.max_len * key_bytes <= 448 * 1024 || 2 * blocks >= runs;
     const bool whole = small && p.b.max_len <= static_cast<int64_t>(8 * kStep);
-    const int64_t grid = paged_runs(ctx, p, &a, runs, blocks, !whole, beside);
+    const int64_t grid = paged_runs(ctx, p, &a, runs, blocks, kStreamWaves * kWave, !whole, beside);
     MIMIR_REQUIRE(ctx, dispatch_fits(grid, kStreamWaves * kWave), "paged attention: grid of %lld workgroups exceeds the limit",
                   (long long)grid);
     if (dtype == MIMIR_KV_F32) launch_tiles<MIMIR_KV_F32>(p, a, tiles, static_cast<unsigned>(grid), ctx->stream);

@@ -332,8 +332,10 @@ int mimir::kv_batch(mimir_ctx* ctx, const char* what, const mimir_kv_cache* c, c
                   c->page_size);
     MIMIR_REQUIRE(ctx, b->sequences == 0 || (b->token_start && b->kv_len && (b->max_len == 0 || b->page_table)),
                   "%s: null batch array", what);
+    // No sequence has more rows than there are, whatever the bound.
     *out = KvBatch{b->token_start, b->kv_len, b->page_table, b->ld_pages, static_cast<int32_t>(b->sequences),
-                   static_cast<int32_t>(b->tokens), static_cast<int32_t>(b->max_new), static_cast<int32_t>(b->max_len)};
+                   static_cast<int32_t>(b->tokens), static_cast<int32_t>(std::min(b->max_new, b->tokens)),
+                   static_cast<int32_t>(b->max_len)};
     return MIMIR_OK;
 }
 

@@ -489,6 +489,32 @@ def test_no_keys_at_all(ctx, dtype, n, d, pages):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("count,max_new", [(3, 1 << 29), (3000, 3000), (3000, (1 << 30) - 1)])
+def test_bounds_far_above_what_sequences_have(ctx, dtype, count, max_new):
+    """A bound of new tokens that no launch of a workgroup per block would hold: single
+    tokens of a key each, whose rows are that key's value.  Its weight is 1 and the sum's
+    reciprocal too; the value is put together from up to three terms and scaled once, half
+    a step of fp32 each."""
+    kh, group, d, page = 16, 16, 16, 16
+    rng = np.random.default_rng(count)
+    v = rng.standard_normal((count, kh, d)).astype(np.float32)
+    cache = M.KVCache(ctx, dtype, count, page, kh, d)
+    try:
+        up = ctx.to_device
+        table = rng.permutation(count).astype(np.int32)
+        batch = M.KVBatch(up(np.arange(count + 1, dtype=np.int32)), up(np.ones(count, np.int32)), up(table), count, count, 1,
+                          max_new, page)
+        dv = up(v)
+        ctx.kv_append(cache, batch, dv, dv)
+        out = up(np.full((count, kh, group, d), 5.0, np.float32))
+        ctx.attention_paged(cache, batch, up(rng.standard_normal((count, kh * group * d)).astype(np.float32)), out, kh * group)
+        want = held(v, dtype)[:, :, None, :].astype(np.float64)
+        assert (np.abs(out.numpy() - want) <= 4 * U * np.abs(want)).all()
+    finally:
+        cache.close()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("d", [64, 80, 128])
 @pytest.mark.parametrize("waves", [4, 8])
 @pytest.mark.parametrize("pages", [0, 2])

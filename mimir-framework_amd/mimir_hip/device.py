@@ -424,6 +424,9 @@ class KVCache:
         self.c.k_scale, self.c.v_scale = _address(k_scale), _address(v_scale)
 
     def close(self):
+        """Frees the buffers that it made; calls with the cache are refused from then on."""
+        if self._own:
+            self.c.k = self.c.v = self.c.k_scale = self.c.v_scale = None
         for b in self._own:
             b.free()
         self._own = []

@@ -47,6 +47,35 @@ def test_null_context_is_einval():
     assert lib.mimir_rope_rows_bwd(None, None, 0, None, 0, 0, None, 0, None, 0, 0, 0, 8, None, rope, 0) == M.EINVAL
 
 
+class Room:
+    """A context's allocations without a GPU: `most` buffers, then MimirError."""
+
+    def __init__(self, most):
+        self.lib, self.most, self.held = M.load(), most, {}
+
+    def empty(self, shape, dtype=np.float32):
+        if len(self.held) == self.most:
+            raise M.MimirError(M.ENOMEM, "no room")
+        a = M.DeviceArray(self, 16 * (len(self.held) + 1), shape, dtype)
+        self.held[a.ptr] = a
+        return a
+
+    def free(self, a):
+        del self.held[a.ptr]
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "i8"])
+def test_a_closed_cache_is_refused(dtype):
+    """Its buffers are gone: no address of theirs is left for a call to take."""
+    room = Room(4)
+    cache = M.KVCache(room, dtype, 3, 16, 2, 20)
+    cache.close()
+    assert cache.c.k is None and cache.c.v is None and cache.c.k_scale is None and cache.c.v_scale is None
+    given = M.KVCache(room, dtype, 3, 16, 2, 20, 64, 128, 192, 256)
+    given.close()  # the program's own buffers stay its own
+    assert given.c.k == 64 and given.c.v == 128
+
+
 def frequencies(rot, theta, kind, factor, original_len, low, high):
     if kind == "base":
         theta = theta * factor ** (rot / (rot - 2))

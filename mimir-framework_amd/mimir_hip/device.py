@@ -413,9 +413,12 @@ class KVCache:
                 raise MimirError(EINVAL, f"KV cache: page_size {page_size}, kv_heads {kv_heads}, head_dim {head_dim}")
             rows = (pages, kv_heads, page_size)
             np_type = (np.float32, np.uint16, np.int8)[kind]
-            self._own = [ctx.empty(rows + (self.stride,), np_type) for _ in range(2)]
-            if kind == 2:
-                self._own += [ctx.empty(rows) for _ in range(2)]
+            try:
+                for shape, of in [(rows + (self.stride,), np_type)] * 2 + [(rows, np.float32)] * (2 if kind == 2 else 0):
+                    self._own.append(ctx.empty(shape, of))
+            except BaseException:  # no room for one of them: not the others either
+                self.close()
+                raise
             k, v, k_scale, v_scale = (self._own + [None, None])[:4]
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         if dtype != "i8":

@@ -64,6 +64,21 @@ class Room:
         del self.held[a.ptr]
 
 
+@pytest.mark.parametrize("dtype,buffers", [("f32", 2), ("bf16", 2), ("i8", 4)])
+def test_a_cache_without_room_keeps_nothing(dtype, buffers):
+    for most in range(buffers):
+        room = Room(most)
+        with pytest.raises(M.MimirError):
+            M.KVCache(room, dtype, 3, 16, 2, 20)
+        assert not room.held
+    room = Room(buffers)
+    cache = M.KVCache(room, dtype, 3, 16, 2, 20)
+    assert len(room.held) == buffers and cache.c.k == cache.k.ptr and cache.c.v_scale == (cache.v_scale.ptr if buffers == 4 else None)
+    cache.close()
+    cache.close()
+    assert not room.held
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "i8"])
 def test_a_closed_cache_is_refused(dtype):
     """Its buffers are gone: no address of theirs is left for a call to take."""

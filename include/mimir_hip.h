@@ -352,7 +352,9 @@ typedef struct mimir_rope_scaling {
 
 /* mimir_rope_table with scaled frequencies, for positions first .. first + rows - 1:
  * cos_tab / sin_tab are HOST arrays of rows * rot_dim / 2 floats, each value
- * computed in double and rounded once.  scaling NULL: NONE with magnitude 1. */
+ * computed in double and rounded once.  scaling NULL: NONE with magnitude 1.
+ * MIMIR_EINVAL, and nothing written, where an angle or the magnitude in fp32 would
+ * not be finite. */
 int mimir_rope_table_scaled(int64_t first, int64_t rows, int64_t rot_dim, double theta,
                             const mimir_rope_scaling* scaling, float* cos_tab, float* sin_tab);
 

@@ -191,7 +191,7 @@ int mimir_rope_table_scaled(int64_t first, int64_t rows, int64_t rot_dim, double
     const int64_t half = rot_dim / 2;
     const double d = static_cast<double>(rot_dim);
     const double base = z.kind == MIMIR_ROPE_SCALE_BASE ? theta * pow(z.factor, d / (d - 2.0)) : theta;
-    for (int64_t i = 0; i < half; ++i) {
+    const auto frequency = [&](int64_t i) {
         double f = 1.0 / pow(base, static_cast<double>(2 * i) / d);
         if (z.kind == MIMIR_ROPE_SCALE_LINEAR) f /= z.factor;
         if (z.kind == MIMIR_ROPE_SCALE_BY_PARTS) {
@@ -199,6 +199,17 @@ int mimir_rope_table_scaled(int64_t first, int64_t rows, int64_t rot_dim, double
             const double g = std::min(1.0, std::max(0.0, (turns - z.low) / (z.high - z.low)));
             f = (1.0 - g) * f / z.factor + g * f;
         }
+        return f;
+    };
+    // Nothing is written of a table that would have values which are no numbers.
+    if (rows > 0) {
+        if (first > INT64_MAX - rows || !std::isfinite(static_cast<float>(z.magnitude))) return MIMIR_EINVAL;
+        for (int64_t i = 0; i < half; ++i)
+            if (const double f = frequency(i); !std::isfinite(f) || !std::isfinite(static_cast<double>(first + rows - 1) * f))
+                return MIMIR_EINVAL;
+    }
+    for (int64_t i = 0; i < half; ++i) {
+        const double f = frequency(i);
         for (int64_t p = 0; p < rows; ++p) {
             const double a = static_cast<double>(first + p) * f;
             cos_tab[p * half + i] = static_cast<float>(cos(a) * z.magnitude);

@@ -2,6 +2,7 @@
 (tests/cpp/test_serving_args.cpp, with a context of a device that is not there),
 where a batch's tokens stand whatever its arrays hold (tests/cpp/test_kvindex.cpp),
 and the tables of scaled frequencies against their closed forms."""
+import ctypes
 import math
 import os
 import shutil
@@ -116,6 +117,26 @@ def test_scaled_tables(kind, rot, theta, first):
             a = (first + p) * f[i]
             for got, want in ((c[p, i], 1.2 * math.cos(a)), (s[p, i], 1.2 * math.sin(a))):
                 assert abs(float(got) - want) <= 2.0 ** -24 * 1.2 + 1.2 * 2.0 ** 17 * 4e-15
+
+
+@pytest.mark.parametrize("args", [
+    dict(kind="linear", factor=1e-320),                    # f / factor
+    dict(kind="linear", factor=1e-306, first=1 << 40),     # the angle
+    dict(kind="base", factor=1e-300, rot_dim=4),           # theta * factor^2
+    dict(kind="by_parts", factor=1e-320, original_len=8, low=1, high=2),
+    dict(theta=1e-320, rot_dim=64),
+    dict(magnitude=1e39),
+    dict(first=(1 << 63) - 2),                             # the last position
+])
+def test_tables_that_would_not_be_finite_are_refused(args):
+    lib = M.load()
+    how = dict(rot_dim=8, theta=1e4, kind="none", factor=1.0, original_len=1.0, low=1.0, high=32.0, magnitude=1.0, first=0) | args
+    c = np.full((5, how["rot_dim"] // 2), 7.0, np.float32)
+    z = M._lib.RopeScaling_C(M._lib.ROPE_SCALINGS.index(how["kind"]), how["factor"], how["original_len"], how["low"], how["high"],
+                             how["magnitude"])
+    at = c.ctypes.data_as(ctypes.c_void_p)
+    assert lib.mimir_rope_table_scaled(how["first"], 5, how["rot_dim"], how["theta"], ctypes.byref(z), at, at) == M.EINVAL
+    assert (c == 7).all()
 
 
 def test_unscaled_table_is_rope_table():

@@ -515,6 +515,23 @@ def test_bounds_far_above_what_sequences_have(ctx, dtype, count, max_new):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d", [64, 96, 128, 250])
+@pytest.mark.parametrize("waves", [4, 8])
+@pytest.mark.parametrize("lens", [[(140, 1300), (70, 900), (1, 300)], [(200, 250), (70, 90), (3, 3)]])
+def test_every_width_of_the_kernel_of_many_rows(dtype, d, waves, lens):
+    """Cut and joined, and whole: some of these hold a few registers in memory."""
+    c = tuned_context(f"attnwaves={waves}")
+    try:
+        q, kv = case(d + waves, dtype, lens, 1, 2, d)
+        p = Paged(c, dtype, lens, 1, d, 16)
+        fill(p, kv)
+        check(attend(c, p, q), p, q, kv)
+        check(attend(c, p, q, causal=False), p, q, kv, causal=False)
+    finally:
+        c.close()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("d", [64, 80, 128])
 @pytest.mark.parametrize("waves", [4, 8])
 @pytest.mark.parametrize("pages", [0, 2])

@@ -450,10 +450,7 @@ __global__ __launch_bounds__(WAVES * kWave, (WAVES / 4 * BlockShape<DT, DP, WAVE
         } else {
             const bool late = kStagger && wave >= WAVES / 2;
             char *v_old = values, *v_cur = values, *v_next = values + Tile::kValueBytes;
-            // One more for the late waves; a block without keys has no turn: its sequence may
-            // have no page table to find a tile's page in.
-            const int turns = kStagger && tiles > 0 ? tiles + 1 : tiles;
-            for (int t = 0; t < turns; ++t) {
+            for (int t = 0; t < tiles + (kStagger ? 1 : 0); ++t) {
                 const char* cur = lds + (t & 1) * Tile::kKeyBytes;
                 char* const next = lds + ((t + 1) & 1) * Tile::kKeyBytes;
                 const int key = k0 + t * kTile;
@@ -469,7 +466,9 @@ __global__ __launch_bounds__(WAVES * kWave, (WAVES / 4 * BlockShape<DT, DP, WAVE
                     soften(key, cur);
                     if (!late) weigh(v_cur);
                 }
-                to = find(t + 3);
+                // Not in the late waves' turn: it is a block's first where there are no keys, whose
+                // sequence may have no page table.
+                if (t < tiles) to = find(t + 3);
                 char* const v_free = kStagger ? v_old : v_cur;
                 v_old = v_cur;
                 v_cur = v_next;

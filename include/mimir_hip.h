@@ -425,9 +425,11 @@ int mimir_kv_cache_bytes(const mimir_kv_cache* cache, size_t* kv_bytes, size_t* 
  * page_size].  The arrays are DEVICE int32: they may change between two replays
  * of a captured graph, within the bounds that the call was made with.  No call
  * reads or writes outside the given buffers, whatever they hold: rows from
- * token_start[sequences] on are left as they are, tokens past max_new or
- * max_len are passed over, and a page outside [0, pages) holds no tokens (it is
- * not written; its keys are not attended; it reads as zeros), nor does a
+ * token_start[sequences] on are left as they are, and so are a sequence's new
+ * tokens after its first max_new, which then count as all of them; a kv_len[s]
+ * below 0 counts as 0 and one above max_len as max_len (both move the positions
+ * of the tokens that are left); and a page outside [0, pages) holds no tokens (it
+ * is not written; its keys are not attended; it reads as zeros), nor does a
  * position below 0.  A slot that two tokens of one call share is left with
  * either's row or a mixture. */
 typedef struct mimir_kv_batch {
@@ -437,7 +439,7 @@ typedef struct mimir_kv_batch {
     const int32_t* kv_len;      /* [sequences] */
     const int32_t* page_table;  /* [sequences][ld_pages] */
     int64_t ld_pages;
-    int64_t max_new;            /* no sequence has more new tokens */
+    int64_t max_new;            /* no sequence has more new tokens; may be far above what they have */
     int64_t max_len;            /* nor more cached ones; <= ld_pages * page_size */
 } mimir_kv_batch;
 

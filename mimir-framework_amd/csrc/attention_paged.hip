@@ -180,10 +180,16 @@ extern "C" int mimir_attention_paged_fwd(mimir_ctx* ctx, const mimir_kv_cache* c
     // Sequences with few query rows of a key / value head stream their keys, the others'
     // keys go through LDS, by a launch each.  A batch whose sequences all have max_new
     // tokens (or whose rows would suffice for that) has the second alone, which takes any;
-    // so has one of short contexts that is one round of workgroups or little more (chunks of
-    // up to 91 tokens beside single ones, up to 100 keys before them, 19 sequences x 8
-    // heads: 42 us, by two launches 53; 64 sequences x 8 heads, bf16 45, by two 38; 84 x 8,
-    // fp32, of whose streaming workgroups a compute unit holds one, 84 and 96).
+    // so has one of short contexts with up to 256 (sequence, key / value head) pairs, or, of
+    // fp32 heads over 64, of whose streaming workgroups a compute unit holds one, 1024.  One
+    // launch / two, us, chunks of 91 tokens beside single ones, up to 100 keys before them,
+    // sequences x 8 heads.  One chunk: bf16 heads of 128, 256 pairs 21 / 29, 512 27 / 36, 1024
+    // 43 / 45, 1792 68 / 61; 8-bit 25 / 33, 31 / 39, 47 / 48, 76 / 62; fp32 38 / 57, 69 / 77,
+    // 124 / 114, 209 / 171; fp32 heads of 64 19 / 28, 25 / 35, 38 / 43, 61 / 60, of 256 49 / 54,
+    // 85 / 75, 153 / 133, 255 / 221.  A chunk to seven single tokens: bf16 28 / 36, 40 / 46,
+    // 61 / 69, 100 / 105; fp32 50 / 59, 86 / 89, 150 / 160, 257 / 272, heads of 96 35 / 54,
+    // 47 / 77, 73 / 130, 119 / 209.  (So the sides meet between 500 and 1800 pairs, by the
+    // type and by how many chunks there are: 256 is on the low side, 1024 within it.)
     const int64_t rows = static_cast<int64_t>(a.b.max_new) * a.group;
     MIMIR_REQUIRE(ctx, rows <= INT32_MAX, "%s: %lld query rows of a head", what, (long long)rows);
     PagedRuns few{}, others{};

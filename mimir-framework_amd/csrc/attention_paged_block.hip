@@ -20,11 +20,17 @@
 // - Causal: a wave passes over tiles behind its last row's keys.  Rows' ends inside a
 //   tile, and pages that are none, are looked at only where there are any.
 //
-// Bound by the matrix cores, at the power that they draw (as attention.hip): 512
-// tokens of one sequence over 8812 keys, 32 heads on 8 of 128, bf16, 201 to 212 us =
+// 512 tokens of one sequence over 8812 keys, 32 heads on 8 of 128, bf16, 201 to 212 us =
 // 340 to 357 TFLOP/s of fp32 work, 1020 to 1070 of bf16 MFMAs, which are busy 46% of
 // the cycles at 2.1 GHz beside 5.4 VALU operations each; a library product of 8192 x
-// 8192 bf16 runs at 1390.  fp32 prompts (4 of up to 2048, 16 heads) 243 to 253 us.
+// 8192 bf16 runs at 1390.  Prompts (4 of up to 2048, 16 heads): fp32 240 to 253 us, bf16
+// 156, 8-bit 163; heads of 64 135, 101, 113.
+// What the other half of the cycles goes to has not been taken apart.  In the built code
+// each load of a tile stands in a loop over lanes (a descriptor's length, at most the keys
+// of a half, is a vector value to the compiler), which cuts the tile's instructions into
+// pieces that are not scheduled together; 167 to 212 scalar values are kept in vector
+// registers' lanes, and 1 to 11 vector registers of the instances of 128 and 256
+// dimensions (fp32: 96 and 128) in memory.
 // Measured on the way: a lane's query row in loads of 4 bytes instead of 16 cost 12 us
 // a block, page numbers looked at for each tile instead of once a block 6 us of 219,
 // and waves that all multiply the values in the tile they were scored in 7% of the

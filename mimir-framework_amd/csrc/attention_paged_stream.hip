@@ -17,7 +17,9 @@
 //   the queries and weights do: 3 or 6 MFMAs for a product of fp32 precision.  The
 //   8-bit scales multiply scores and weights instead of elements.
 // - The queries' terms are in LDS (registers they would not fit beside two steps of
-//   keys); the four waves' sums are brought to one max there at the end.
+//   keys); the four waves' sums are brought to one max there at the end.  No instance
+//   keeps vector registers in memory: a form that did (fp32 heads of 256, 100 bytes a
+//   lane) gave wrong scores, of which the cause was not found.
 //
 // Loads: buffer loads without a bounds check in the code (the descriptor of a half of
 // 16 keys ends with its keys, what lies behind reads as zero), non-temporal: nothing

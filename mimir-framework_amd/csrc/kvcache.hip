@@ -1,10 +1,12 @@
 // kvcache.hip -- the paged key/value cache: new tokens' keys and values written
 // into their pages (keys and queries rotated on the way), and read back.
 //
-// Bound by HBM: q, k and v are read once and written once, in the cache's type.
+// Bound by HBM: q, k and v are read from it once and written once, in the cache's type.
 // LPR lanes hold a head row, eight elements each (two vectors, kvcache.hpp
 // unit_place), so that the largest absolute value of an 8-bit row is a few lane
-// exchanges away and nothing is read twice.  A workgroup takes rows of one token, whose
+// exchanges away.  Of a row with fewer elements than that (unrotated heads of 80 have 10
+// units for 16 lanes) the lanes behind the last unit load and store vectors of its second
+// half once more, the same values to the same places.  A workgroup takes rows of one token, whose
 // sequence its waves search in token_start while the row is on its way.  Prompts of
 // 9270 tokens x 32 + 2 x 8 heads of 128 into an 8-bit cache and read back (500 MB): 68
 // and 17 us, 85 in turn = 5.9 TB/s; steps of 48 tokens 4 and 3, launch to launch 9.5.
@@ -80,7 +82,9 @@ __device__ __forceinline__ void put(char* row, int at, const float* x) {
 }
 
 // W: elements per vector, 4 where every row of q, k, v and q_out is whole 16-byte
-// vectors; UN units of 2 W elements per lane.  A workgroup has rows of one token:
+// vectors and half the rotated part too; UN units of 2 W elements per lane.  (Of one
+// element, 128 of 128 dimensions rotated and 124, prompts of 9270 tokens x 32 + 2 x 8
+// heads written and read back: fp32 99 and 128 us, bf16 90 and 119, 8-bit 86 and 118.)  A workgroup has rows of one token:
 // several tokens each kept fewer loads in flight (prompts of 9270 tokens x 48 heads of
 // 128, 8-bit: 91 us written and read back, with two 94, four 101, eight 123).
 template <int DT, int LPR, int W, bool KEEP>

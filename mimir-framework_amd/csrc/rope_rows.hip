@@ -70,7 +70,10 @@ struct Half {
     }
 };
 
-// W: elements per half of a slot, 4 where every row is whole 16-byte vectors.  A
+// W: elements per half of a slot, 4 where every row is whole 16-byte vectors and the
+// rotated part a multiple of 8, else 1 for all of a row (8192 tokens x 40 heads of 128, of
+// which 128 dimensions are rotated 48 us, 124 63; heads of 96 39 us = 6.5 TB/s, of 100 54
+// = 4.9 TB/s, of 99 57 = 4.6 TB/s; the same inputs each time, in part from the caches).  A
 // thread has one slot: 8192 tokens x 40 heads of 128 take 58 us = 5.8 TB/s (a copy of
 // as many bytes 53), with two slots a thread 61, four 61, eight 89.  The loads leave
 // their lines in the caches, where the projection before may have put them (4099

@@ -552,6 +552,51 @@ int mimir_embedding_f32ids_bwd(mimir_ctx* ctx, const float* ids, int64_t n_ids, 
                                int32_t padding_idx);
 
 /* ---------------------------------------------------------------------------
+ * Training: the loss of a model's last layer, gated products with their backward,
+ * gradients' norm and clipping.  No counterpart in the reference, whose trainer
+ * computes these on the host.  Device pointers, stream order.
+ * ------------------------------------------------------------------------- */
+
+/* Element types of these calls' matrices. */
+#define MIMIR_NUM_F32 0
+#define MIMIR_NUM_BF16 1
+
+/* Softmax cross entropy of the linear layer z = x w^T over a vocabulary, without z in
+ * memory: x [tokens][dim] (row stride ld_x elements), w [vocab][dim] (ld_w; an
+ * embedding table's layout), both of `type`, targets [tokens].
+ *   lse[i] = log sum_v exp z[i][v],  loss[i] = lse[i] - z[i][targets[i]]
+ *   mean[0] = sum of loss / max(count, 1),  mean[1] = count
+ * over the tokens that count: those whose target lies in [0, vocab).  Of the others
+ * loss and lse are 0, and what stands in their rows of x reaches nothing.  fp32
+ * products are as exact as fp32 arithmetic (three bf16 terms an operand, fp32 sums),
+ * bf16 ones exact with fp32 sums; the exponentials' sums are fp32, and
+ * exponentials below 2^-126 count as 0.  An infinity, a
+ * NaN or a magnitude above 3.38e38 in x (of a token that counts) or w may give NaN in
+ * whatever it is summed into.  mean may be NULL.  tokens and vocab up to 2^24, dim up
+ * to 2^18.  Scratch (the context's): x's rows again (fp32: 6 bytes an element), 8
+ * bytes for each token and 128 rows of w, and, for fp32 or rows that are no 16-byte
+ * multiples, up to 512 MiB of w's rows. */
+int mimir_linear_cross_entropy_fwd(mimir_ctx* ctx, int type, const void* x, int64_t ld_x, const void* w, int64_t ld_w,
+                                   const int32_t* targets, int64_t tokens, int64_t dim, int64_t vocab, float* loss,
+                                   float* lse, float* mean);
+
+/* Its gradients, from the forward's lse:
+ *   G[i][v] = g[i] (exp(z[i][v] - lse[i]) - [v == targets[i]]), 0 where i does not count
+ *   g[i] = scale * (dloss ? dloss[i] : 1) / (mean ? max(mean[1], 1) : 1)
+ *   dx = G w, dw = G^T x, written, or added to where accumulate_x / accumulate_w
+ * So dloss NULL with the forward's mean gives the gradient of the mean loss, and dloss
+ * without mean that of any function of the losses.  dx [tokens][dim] and dw
+ * [vocab][dim] have `type` (either may be NULL) and are rounded once; for bf16, G is
+ * held in bf16 in between (with at most 128 tokens as two bf16 terms).  dx may be x
+ * with the same stride; dw must not overlap the other buffers.  The same call gives the same bits.  Scratch:
+ * x's rows again, up to 512 MiB (at least 256 rows of w) for G and w's rows, and fp32
+ * sums of dx where the vocabulary is taken in pieces or there are few tokens. */
+int mimir_linear_cross_entropy_bwd(mimir_ctx* ctx, int type, const void* x, int64_t ld_x, const void* w, int64_t ld_w,
+                                   const int32_t* targets, int64_t tokens, int64_t dim, int64_t vocab, const float* lse,
+                                   const float* dloss, const float* mean, float scale, void* dx, int64_t ld_dx,
+                                   int accumulate_x, void* dw, int64_t ld_dw, int accumulate_w);
+
+/* ---------------------------------------------------------------------------
  * Device-resident runtime: a named tensor store and a layer runner with the
  * routing of the reference's Model::forwardPassNamed (Model.cpp:1352-1408,
  * forwardPassView Model.cpp:4621-6824) for the layer types of this path.

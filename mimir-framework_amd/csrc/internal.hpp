@@ -54,6 +54,9 @@ struct mimir_ctx {
     // (kept allocated) rather than freed; the retired buffers are freed when
     // the last graph goes.
     int graph_pins = 0;
+    // A call was captured whose scratch a graph of the program holds (matrix.hip):
+    // one pin for the context's life.
+    bool captured = false;
     std::vector<void*> retired;
 };
 

@@ -1,0 +1,529 @@
+// linear_ce.hip -- softmax cross entropy of a linear layer over a large vocabulary,
+// and its gradients, without the logits in memory.
+//
+//   z_iv = x_i . w_v,  lse_i = log sum_v exp z_iv,  loss_i = lse_i - z_i,t(i)
+//   G_iv = g_i (exp(z_iv - lse_i) - [v = t(i)]),  dx = G w,  dw (+)= G^T x
+//
+// The reference has no loss on the device side of this path: its trainer hands
+// Model::backwardPass a loss gradient (Model.cpp:7307-9153); this makes the one for
+// a model's last layer.
+//
+// Forward: the product z = w x^T of matrix.hpp, 256 or 128 of the vocabulary by as
+// many tokens a workgroup.  A lane has one token's logits in its registers, so the
+// tile's maximum and sum of exp(z - maximum) cost one exchange between half waves
+// and one through LDS; they go to part[tile][token] (8 bytes for 256 logits), and
+// ce_finish joins them.
+//
+// Backward: the same product again for a piece of the vocabulary, whose epilogue
+// writes G in bf16 (three planes for fp32 operands), then the two products with G.
+// The logits again cost a third of what the gradients' products do; keeping
+// exp(z - m) instead would take tokens x vocab values and the row factors, which are
+// known when the last piece is, could not go into dw's sums.  G without its common
+// factor (scale, and 1 / count for the mean): the factor is applied to the fp32 sums.
+// Rounding G to bf16 beside bf16 operands is off by 2^-8 relative at most a term, as
+// rounding a layer's output gradient is, and averages out in the sums.
+//
+// Tokens without a target take no part: x's counted rows are gathered first, so the
+// products run over those alone, and what stands in the others reaches nothing.
+#include "matrix.hpp"
+
+#include <algorithm>
+
+using namespace mimir;
+
+namespace {
+
+constexpr float kLog2e = 1.44269504088896340736f;
+// Below any logit that counts, and finite times log2 e: the maximum of nothing.
+constexpr float kLowest = -2.0e38f;
+
+// --- the counted rows --------------------------------------------------------------
+
+struct GatherArgs {
+    const void* x;
+    int64_t ld_x;
+    const int32_t* target;
+    int64_t tokens, dim, vocab;
+    uint16_t* dst;       // planes of [tokens][ld_dst]
+    int64_t ld_dst, plane;
+    int32_t* row;        // [tokens]: the token of each gathered row
+    int32_t* count;
+    float* zero_a;       // of tokens without a target: loss and lse, or null
+    float* zero_b;
+    void* dx;            // their gradient's rows are zeroed, or null
+    int64_t ld_dx;
+};
+
+constexpr int kGatherRows = 8;
+
+// Eight tokens a workgroup, two rows a wave's turn.  How many rows before its own
+// count is found by reading the targets before them (a few KB, in L2).
+template <bool BF16, bool VEC>
+__global__ __launch_bounds__(kBlock) void gather_rows(GatherArgs a) {
+    __shared__ int before[kBlock / kWave];
+    const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+    const int64_t t0 = static_cast<int64_t>(blockIdx.x) * kGatherRows;
+    const auto counts = [&](int64_t t) {
+        const int32_t v = a.target[t];
+        return v >= 0 && v < a.vocab;
+    };
+    int mine = 0;
+    for (int64_t t = threadIdx.x; t < t0; t += kBlock) mine += counts(t) ? 1 : 0;
+#pragma unroll
+    for (int s = 1; s < kWave; s *= 2) mine += __shfl_xor(mine, s);
+    if (lane == 0) before[wave] = mine;
+    __syncthreads();
+    int at = 0;
+#pragma unroll
+    for (int w = 0; w < kBlock / kWave; ++w) at += before[w];
+
+    for (int i = 0; i < kGatherRows; ++i) {
+        const int64_t t = t0 + i;
+        if (t >= a.tokens) break;
+        const bool in = counts(t);
+        if (i % (kBlock / kWave) == wave) {
+            if (in) {
+                if (lane == 0) a.row[at] = static_cast<int32_t>(t);
+                for (int64_t c = 8 * lane; c < a.ld_dst; c += 8 * kWave)
+                    mat_stage8<BF16, VEC>(a.x, t * a.ld_x + c, a.dim - c, a.dst + at * a.ld_dst + c, a.plane);
+            } else {
+                if (lane == 0 && a.zero_a) a.zero_a[t] = 0.0f, a.zero_b[t] = 0.0f;
+                if (a.dx)
+                    for (int64_t c = lane; c < a.dim; c += kWave) {
+                        if (BF16) static_cast<uint16_t*>(a.dx)[t * a.ld_dx + c] = 0;
+                        else static_cast<float*>(a.dx)[t * a.ld_dx + c] = 0.0f;
+                    }
+            }
+        }
+        at += in ? 1 : 0;
+    }
+    if (t0 + kGatherRows >= a.tokens && threadIdx.x == 0) *a.count = at;
+}
+
+// --- forward -----------------------------------------------------------------------
+
+// (max, sum of exp2((z - max) log2 e)) of two sets; an empty one is (-infinity, 0).
+__device__ __forceinline__ f2 join(f2 a, f2 b) {
+    const float m = fmaxf(fmaxf(a[0], b[0]), kLowest);
+    return f2{m, a[1] * __builtin_amdgcn_exp2f((a[0] - m) * kLog2e) + b[1] * __builtin_amdgcn_exp2f((b[0] - m) * kLog2e)};
+}
+
+struct CeStats {
+    const int32_t* target;
+    const int32_t* row;
+    f2* part;            // [tile][tokens]
+    float* logit;        // [tokens]: the target's
+    int64_t tokens, first;  // first: the piece's first vocabulary row
+    int32_t tile0;          // and tile
+
+    template <class S>
+    __device__ __forceinline__ void run(const MatAt& at, MatAcc<S>& acc, char* lds) const {
+        f2* red = reinterpret_cast<f2*>(lds);
+        const bool whole = at.m0 + S::kM <= at.m;
+#pragma unroll
+        for (int j = 0; j < S::kBn; ++j) {
+            const int32_t n = at.n0 + acc.n_of(j);
+            const int64_t target = n < at.n ? target_of(n) - first - at.m0 : -1;
+            float m = -__builtin_inff(), hit = 0.0f;
+            bool has = false;
+#pragma unroll
+            for (int i = 0; i < S::kBm; ++i)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const float z = whole || at.m0 + acc.m_of(i, r) < at.m ? acc.c[i][j][r] : -__builtin_inff();
+                    acc.c[i][j][r] = z;
+                    if (acc.m_of(i, r) == target) hit = z, has = true;
+                    m = fmaxf(m, z);
+                }
+            if (has) logit[n] = hit;
+            const float top = fmaxf(m, kLowest) * kLog2e;
+            float s = 0.0f;
+#pragma unroll
+            for (int i = 0; i < S::kBm; ++i)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s += __builtin_amdgcn_exp2f(__builtin_fmaf(acc.c[i][j][r], kLog2e, -top));
+            f2 v = join(f2{m, s}, f2{__shfl_xor(m, 32), __shfl_xor(s, 32)});
+            if (threadIdx.x % kWave < 32) red[acc.wm * S::kN + acc.n_of(j)] = v;
+        }
+        __syncthreads();
+        for (int c = threadIdx.x; c < S::kN; c += S::kThreads) {
+            if (at.n0 + c >= at.n) continue;
+            f2 v = red[c];
+#pragma unroll
+            for (int w = 1; w < S::kWaveM; ++w) v = join(v, red[w * S::kN + c]);
+            part[(tile0 + at.tile_m) * tokens + at.n0 + c] = v;
+        }
+    }
+    __device__ __forceinline__ int64_t target_of(int32_t n) const { return target[row[n]]; }
+};
+
+constexpr int kFinishTokens = 32;
+
+// 32 tokens a workgroup, eight threads a token over the tiles.
+__global__ __launch_bounds__(kBlock) void ce_finish(const f2* part, int64_t tokens, int32_t tiles, const float* logit,
+                                                    const int32_t* row, const int32_t* count, float* loss, float* lse) {
+    constexpr int kParts = kBlock / kFinishTokens;
+    __shared__ f2 red[kParts][kFinishTokens];
+    const int t = threadIdx.x % kFinishTokens, p = threadIdx.x / kFinishTokens;
+    const int64_t n = static_cast<int64_t>(blockIdx.x) * kFinishTokens + t;
+    const bool in = n < *count;
+    f2 v{-__builtin_inff(), 0.0f};
+    if (in)
+        for (int32_t i = p; i < tiles; i += kParts) v = join(v, part[i * tokens + n]);
+    red[p][t] = v;
+    __syncthreads();
+    if (p || !in) return;
+#pragma unroll
+    for (int w = 1; w < kParts; ++w) v = join(v, red[w][t]);
+    const float l = v[0] + logf(v[1]);
+    loss[row[n]] = l - logit[n];
+    lse[row[n]] = l;
+}
+
+// {sum / max(count, 1), count}: one workgroup, sums in 64 bits in a fixed order.
+__global__ __launch_bounds__(1024) void ce_mean(const float* loss, int64_t tokens, const int32_t* count, float* mean) {
+    __shared__ double red[1024 / kWave];
+    double s = 0.0;
+    for (int64_t t = threadIdx.x; t < tokens; t += 1024) s += loss[t];
+#pragma unroll
+    for (int d = 1; d < kWave; d *= 2) s += __shfl_xor(s, d);
+    if (threadIdx.x % kWave == 0) red[threadIdx.x / kWave] = s;
+    __syncthreads();
+    if (threadIdx.x) return;
+    for (int w = 1; w < 1024 / kWave; ++w) s += red[w];
+    mean[0] = static_cast<float>(s / (*count > 0 ? *count : 1));
+    mean[1] = static_cast<float>(*count);
+}
+
+// --- backward ----------------------------------------------------------------------
+
+// G of a piece of the vocabulary, PG planes of [n][ld], zeros from m on to ld.
+template <int PG>
+struct CeGrad {
+    const int32_t* target;
+    const int32_t* row;
+    const float* lse;
+    const float* dloss;  // null: 1
+    uint16_t* g;
+    int64_t ld, plane, first;
+
+    template <class S>
+    __device__ __forceinline__ void run(const MatAt& at, MatAcc<S>& acc, char*) const {
+#pragma unroll
+        for (int j = 0; j < S::kBn; ++j) {
+            const int32_t n = at.n0 + acc.n_of(j);
+            if (n >= at.n) continue;
+            const int32_t t = row[n];
+            const int64_t hit = target[t] - first - at.m0;
+            const float base = lse[t] * kLog2e, w = dloss ? dloss[t] : 1.0f;
+#pragma unroll
+            for (int i = 0; i < S::kBm; ++i)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const int32_t m = acc.m_of(i, 4 * q);
+                    if (at.m0 + m >= ld) continue;
+                    float v[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(acc.c[i][j][4 * q + e], kLog2e, -base));
+                        v[e] = at.m0 + m + e < at.m ? (p - (m + e == hit ? 1.0f : 0.0f)) * w : 0.0f;
+                    }
+                    uint16_t* to = g + n * ld + at.m0 + m;
+#pragma unroll
+                    for (int p = 0; p < PG; ++p) {
+                        const u2 x{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])};
+                        *reinterpret_cast<u2*>(to + p * plane) = x;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            v[e] -= __builtin_bit_cast(float, e % 2 ? x[e / 2] & 0xffff0000u : x[e / 2] << 16);
+                    }
+                }
+        }
+    }
+};
+
+// --- the work's parts ----------------------------------------------------------------
+
+struct Plan {
+    int64_t ld, ld_g, piece;     // columns of x's and w's planes, of G's; the piece's rows of w
+    int p, pg;                   // planes of x and w, of G
+    bool w_direct;
+    int splits;                  // of dx's contraction
+    size_t x, row, count, logit, part, w, g, partial, total;
+};
+
+constexpr int64_t kPieceBytes = int64_t{512} << 20;
+constexpr int64_t kTileM = 128;  // the smaller shape's: how many partial results a token has at most
+
+int64_t tiles_of(int64_t m, int64_t n, int64_t bm, int64_t bn) { return (m + bm - 1) / bm * ((n + bn - 1) / bn); }
+
+// Few tokens: the products' time is the weights' bytes, and G takes a second plane.
+constexpr int64_t kTwoPlaneTokens = 128;
+
+Plan plan_of(const Tuning& tune, int type, const void* w, int64_t ld_w, int64_t tokens, int64_t dim, int64_t vocab, bool back) {
+    Plan p{};
+    p.ld = mat_round(dim, 8);
+    p.p = type == MIMIR_NUM_BF16 ? 1 : 3;
+    p.pg = p.p == 3 ? 3 : tokens <= kTwoPlaneTokens ? 2 : 1;
+    p.w_direct = type == MIMIR_NUM_BF16 && mat_direct(w, ld_w, dim);
+    const int64_t of_row = (back ? tokens * p.pg * 2 : 0) + (p.w_direct ? 0 : p.ld * p.p * 2);
+    if (tune.mat_piece > 0) p.piece = mat_round(tune.mat_piece, 8);
+    else p.piece = of_row ? std::max<int64_t>(256, kPieceBytes / of_row / 256 * 256) : vocab;
+    p.piece = std::min({p.piece, mat_round(vocab, 8), int64_t{1} << 19});  // G's rows are within the operands' strides
+    p.ld_g = mat_round(p.piece, 8);
+    size_t at = 0;
+    const auto take = [&](size_t bytes) {
+        const size_t was = at;
+        at += (bytes + 255) / 256 * 256;
+        return was;
+    };
+    p.x = take(static_cast<size_t>(p.p * tokens * p.ld * 2));
+    p.row = take(static_cast<size_t>(tokens * 4));
+    p.count = take(4);
+    p.w = take(p.w_direct ? 0 : static_cast<size_t>(p.p * p.piece * p.ld * 2));
+    if (back) {
+        p.g = take(static_cast<size_t>(p.pg * tokens * p.ld_g * 2));
+        // Few tiles: the contraction over the piece is dealt to several workgroups.
+        const int64_t tiles = tiles_of(dim, tokens, 128, p.p == 3 ? 64 : 128), steps = p.piece / 64;
+        p.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(512 / std::max<int64_t>(tiles, 1), steps / 8)));
+        const bool partial = p.splits > 1 || p.piece < vocab;
+        p.partial = take(partial ? static_cast<size_t>(p.splits * tokens * mat_round(dim, 4) * 4) : 0);
+    } else {
+        p.logit = take(static_cast<size_t>(tokens * 4));
+        p.part = take(static_cast<size_t>((vocab + kTileM - 1) / kTileM * tokens * 8));
+    }
+    p.total = at;
+    return p;
+}
+
+struct Call {
+    int type;
+    const void* x;
+    int64_t ld_x;
+    const void* w;
+    int64_t ld_w;
+    const int32_t* target;
+    int64_t tokens, dim, vocab;
+};
+
+int check(mimir_ctx* ctx, const char* what, const Call& c) {
+    MIMIR_REQUIRE(ctx, c.type == MIMIR_NUM_F32 || c.type == MIMIR_NUM_BF16, "%s: type %d", what, c.type);
+    constexpr int64_t kMost = int64_t{1} << 24;
+    MIMIR_REQUIRE(ctx, c.tokens >= 0 && c.tokens <= kMost && c.dim >= 1 && c.dim <= (1 << 18) && c.vocab >= 1 && c.vocab <= kMost,
+                  "%s: tokens=%lld (0 to 2^24) dim=%lld (1 to 2^18) vocab=%lld (1 to 2^24)", what, (long long)c.tokens,
+                  (long long)c.dim, (long long)c.vocab);
+    MIMIR_REQUIRE(ctx, c.ld_x >= c.dim && c.ld_w >= c.dim, "%s: row strides (%lld, %lld) below dim", what, (long long)c.ld_x,
+                  (long long)c.ld_w);
+    return MIMIR_OK;
+}
+
+const char* rows_at(const Call& c, int64_t first) {
+    return static_cast<const char*>(c.w) + first * c.ld_w * (c.type == MIMIR_NUM_BF16 ? 2 : 4);
+}
+
+template <bool BF16>
+int gather(mimir_ctx* ctx, const Call& c, const GatherArgs& a) {
+    const bool vec = aligned16(c.x) && c.ld_x % (BF16 ? 8 : 4) == 0;
+    const auto grid = static_cast<unsigned>((c.tokens + kGatherRows - 1) / kGatherRows);
+    if (grid == 0) return MIMIR_OK;
+    if (vec) gather_rows<BF16, true><<<grid, kBlock, 0, ctx->stream>>>(a);
+    else gather_rows<BF16, false><<<grid, kBlock, 0, ctx->stream>>>(a);
+    return launched(ctx, "gather_rows");
+}
+
+// The piece's rows of w as an operand, from `first` on.
+int weights(mimir_ctx* ctx, const Call& c, const Plan& p, char* work, int64_t first, int64_t rows, MatOperand* out) {
+    if (p.w_direct) {
+        *out = MatOperand{reinterpret_cast<const uint16_t*>(rows_at(c, first)), c.ld_w, 0};
+        return MIMIR_OK;
+    }
+    auto* dst = reinterpret_cast<uint16_t*>(work + p.w);
+    *out = MatOperand{dst, p.ld, p.piece * p.ld};
+    return mat_stage(ctx, c.type, rows_at(c, first), rows, c.dim, c.ld_w, dst, p.ld, p.piece * p.ld);
+}
+
+MatArgs args_of(const MatOperand& a, const MatOperand& b, int64_t m, int64_t n, int64_t k) {
+    MatArgs g{};
+    g.a[0] = a;
+    g.b[0] = b;
+    g.m = static_cast<int32_t>(m);
+    g.n = static_cast<int32_t>(n);
+    g.k = static_cast<int32_t>(k);
+    g.segments = g.batches = g.splits = 1;
+    return g;
+}
+
+template <int P>
+int forward(mimir_ctx* ctx, const Call& c, const Plan& p, char* work, float* loss, float* lse) {
+    const MatOperand x{reinterpret_cast<const uint16_t*>(work + p.x), p.ld, c.tokens * p.ld};
+    auto* row = reinterpret_cast<int32_t*>(work + p.row);
+    auto* count = reinterpret_cast<int32_t*>(work + p.count);
+    CeStats e{c.target, row, reinterpret_cast<f2*>(work + p.part), reinterpret_cast<float*>(work + p.logit), c.tokens, 0, 0};
+    for (int64_t first = 0; first < c.vocab; first += p.piece) {
+        const int64_t rows = std::min(p.piece, c.vocab - first);
+        MatOperand w;
+        if (int st = weights(ctx, c, p, work, first, rows, &w)) return st;
+        MatArgs g = args_of(w, x, rows, c.tokens, c.dim);
+        g.n_dev = count;
+        e.first = first;
+        using B = MatBig<P, P, kRows, kRows>;
+        using S = MatSmall<P, P, kRows, kRows>;
+        const bool big = mat_fills<B>(ctx, g);
+        const int st = big ? mat_launch<B>(ctx, "cross entropy statistics", g, e) : mat_launch<S>(ctx, "cross entropy statistics", g, e);
+        if (st) return st;
+        e.tile0 += static_cast<int32_t>((rows + (big ? B::kM : S::kM) - 1) / (big ? B::kM : S::kM));
+    }
+    ce_finish<<<static_cast<unsigned>((c.tokens + kFinishTokens - 1) / kFinishTokens), kBlock, 0, ctx->stream>>>(
+        e.part, c.tokens, e.tile0, e.logit, row, count, loss, lse);
+    return launched(ctx, "ce_finish");
+}
+
+struct Gradients {
+    const float* lse;
+    const float* dloss;
+    const float* mean;
+    float scale;
+    void* dx;
+    int64_t ld_dx;
+    void* dw;
+    int64_t ld_dw;
+    int accumulate_x, accumulate_w;
+};
+
+// P planes of x and w, PG of G.
+template <int P, int PG>
+int backward(mimir_ctx* ctx, const Call& c, const Plan& p, char* work, const Gradients& d) {
+    const MatOperand x{reinterpret_cast<const uint16_t*>(work + p.x), p.ld, c.tokens * p.ld};
+    const MatOperand gr{reinterpret_cast<const uint16_t*>(work + p.g), p.ld_g, c.tokens * p.ld_g};
+    auto* row = reinterpret_cast<int32_t*>(work + p.row);
+    auto* count = reinterpret_cast<int32_t*>(work + p.count);
+    const int bf16 = c.type == MIMIR_NUM_BF16;
+    const int64_t size = bf16 ? 2 : 4;
+    const auto vec = [&](const void* q, int64_t ld) { return ld % 4 == 0 && reinterpret_cast<uintptr_t>(q) % (4 * size) == 0; };
+    MatOut ox{};
+    ox.out[0] = d.dx;
+    ox.ld = d.ld_dx;
+    ox.row = row;
+    ox.partial = reinterpret_cast<float*>(work + p.partial);
+    ox.ld_partial = mat_round(c.dim, 4);
+    ox.slice = c.tokens * ox.ld_partial;
+    ox.count = d.mean ? d.mean + 1 : nullptr;
+    ox.alpha = d.scale;
+    ox.bf16 = bf16;
+    ox.accumulate = d.accumulate_x;
+    ox.vec = vec(d.dx, d.ld_dx);
+    MatOut ow = ox;
+    ow.row = nullptr;
+    ow.partial = nullptr;
+    ow.ld = d.ld_dw;
+    ow.accumulate = d.accumulate_w;
+    ow.last = 1;
+    CeGrad<PG> e{c.target, row, d.lse, d.dloss, reinterpret_cast<uint16_t*>(work + p.g), p.ld_g, c.tokens * p.ld_g, 0};
+
+    for (int64_t first = 0; first < c.vocab; first += p.piece) {
+        const int64_t rows = std::min(p.piece, c.vocab - first);
+        MatOperand w;
+        if (int st = weights(ctx, c, p, work, first, rows, &w)) return st;
+        MatArgs g = args_of(w, x, rows, c.tokens, c.dim);
+        g.n_dev = count;
+        e.first = first;
+        using BG = MatBig<P, P, kRows, kRows>;
+        using SG = MatSmall<P, P, kRows, kRows>;
+        int st = mat_fills<BG>(ctx, g) ? mat_launch<BG>(ctx, "cross entropy gradient", g, e)
+                                               : mat_launch<SG>(ctx, "cross entropy gradient", g, e);
+        if (st) return st;
+        if (d.dx) {
+            g = args_of(w, gr, c.dim, c.tokens, rows);
+            g.n_dev = count;
+            g.splits = p.splits;
+            ox.read_partial = first > 0;
+            ox.last = p.splits == 1 && first + rows >= c.vocab;
+            using SX = MatSmall<P, PG, kCols, kRows>;
+            if constexpr (P == PG) {
+                using BX = MatBig<P, PG, kCols, kRows>;
+                st = p.splits == 1 && mat_fills<BX>(ctx, g) ? mat_launch<BX>(ctx, "cross entropy dx", g, ox)
+                                                                    : mat_launch<SX>(ctx, "cross entropy dx", g, ox);
+            } else {
+                st = mat_launch<SX>(ctx, "cross entropy dx", g, ox);
+            }
+            if (st) return st;
+        }
+        if (d.dw) {
+            g = args_of(x, gr, c.dim, rows, c.tokens);
+            if (c.tokens > 0) g.k_dev = count;
+            ow.out[0] = static_cast<char*>(d.dw) + first * d.ld_dw * size;
+            ow.vec = vec(ow.out[0], d.ld_dw);
+            using SW = MatSmall<P, PG, kCols, kCols>;
+            if constexpr (P == PG) {
+                using BW = MatBig<P, PG, kCols, kCols>;
+                st = mat_fills<BW>(ctx, g) ? mat_launch<BW>(ctx, "cross entropy dw", g, ow)
+                                                   : mat_launch<SW>(ctx, "cross entropy dw", g, ow);
+            } else {
+                st = mat_launch<SW>(ctx, "cross entropy dw", g, ow);
+            }
+            if (st) return st;
+        }
+    }
+    if (!d.dx || p.splits == 1) return MIMIR_OK;
+    ox.last = 1;
+    return mat_join(ctx, ox, c.tokens, c.dim, count, p.splits);
+}
+
+}  // namespace
+
+extern "C" {
+
+int mimir_linear_cross_entropy_fwd(mimir_ctx* ctx, int type, const void* x, int64_t ld_x, const void* w, int64_t ld_w,
+                                   const int32_t* targets, int64_t tokens, int64_t dim, int64_t vocab, float* loss, float* lse,
+                                   float* mean) {
+    if (!ctx) return MIMIR_EINVAL;
+    const char* what = "linear cross entropy";
+    const Call c{type, x, ld_x, w, ld_w, targets, tokens, dim, vocab};
+    if (int st = check(ctx, what, c)) return st;
+    MIMIR_REQUIRE(ctx, tokens == 0 || (x && w && targets && loss && lse), "%s: null pointer", what);
+    if (tokens == 0 && !mean) return MIMIR_OK;
+    MIMIR_ENTER(ctx);
+    const Plan p = plan_of(ctx->tune, type, w, ld_w, tokens, dim, vocab, false);
+    char* work;
+    if (int st = mat_scratch(ctx, p.total, &work)) return st;
+    auto* count = reinterpret_cast<int32_t*>(work + p.count);
+    if (tokens > 0) {
+        const GatherArgs a{x, ld_x, targets, tokens, dim, vocab, reinterpret_cast<uint16_t*>(work + p.x), p.ld, tokens * p.ld,
+                           reinterpret_cast<int32_t*>(work + p.row), count, loss, lse, nullptr, 0};
+        int st = type == MIMIR_NUM_BF16 ? gather<true>(ctx, c, a) : gather<false>(ctx, c, a);
+        if (!st) st = p.p == 1 ? forward<1>(ctx, c, p, work, loss, lse) : forward<3>(ctx, c, p, work, loss, lse);
+        if (st || !mean) return st;
+        ce_mean<<<1, 1024, 0, ctx->stream>>>(loss, tokens, count, mean);
+        return launched(ctx, "ce_mean");
+    }
+    return mimir_fill_f32(ctx, mean, 2, 0.0f);
+}
+
+int mimir_linear_cross_entropy_bwd(mimir_ctx* ctx, int type, const void* x, int64_t ld_x, const void* w, int64_t ld_w,
+                                   const int32_t* targets, int64_t tokens, int64_t dim, int64_t vocab, const float* lse,
+                                   const float* dloss, const float* mean, float scale, void* dx, int64_t ld_dx, int accumulate_x,
+                                   void* dw, int64_t ld_dw, int accumulate_w) {
+    if (!ctx) return MIMIR_EINVAL;
+    const char* what = "linear cross entropy gradient";
+    const Call c{type, x, ld_x, w, ld_w, targets, tokens, dim, vocab};
+    if (int st = check(ctx, what, c)) return st;
+    MIMIR_REQUIRE(ctx, (!dx || ld_dx >= dim) && (!dw || ld_dw >= dim), "%s: gradient strides (%lld, %lld) below dim", what,
+                  (long long)ld_dx, (long long)ld_dw);
+    MIMIR_REQUIRE(ctx, tokens == 0 || (x && w && targets && lse), "%s: null pointer", what);
+    MIMIR_REQUIRE(ctx, !dw || dw != w, "%s: dw must not be w", what);
+    MIMIR_REQUIRE(ctx, dx != x || ld_dx == ld_x, "%s: dx in place needs equal strides", what);
+    if (!dx && !dw) return MIMIR_OK;
+    MIMIR_ENTER(ctx);
+    Plan p = plan_of(ctx->tune, type, w, ld_w, tokens, dim, vocab, true);
+    char* work;
+    if (int st = mat_scratch(ctx, p.total, &work)) return st;
+    auto* count = reinterpret_cast<int32_t*>(work + p.count);
+    const Gradients d{lse, dloss, mean, scale, dx, ld_dx, dw, ld_dw, accumulate_x ? 1 : 0, accumulate_w ? 1 : 0};
+    const GatherArgs a{x, ld_x, targets, tokens, dim, vocab, reinterpret_cast<uint16_t*>(work + p.x), p.ld, tokens * p.ld,
+                       reinterpret_cast<int32_t*>(work + p.row), count, nullptr, nullptr, accumulate_x ? nullptr : dx, ld_dx};
+    if (int st = type == MIMIR_NUM_BF16 ? gather<true>(ctx, c, a) : gather<false>(ctx, c, a)) return st;
+    if (p.p == 3) return backward<3, 3>(ctx, c, p, work, d);
+    return p.pg == 2 ? backward<1, 2>(ctx, c, p, work, d) : backward<1, 1>(ctx, c, p, work, d);
+}
+
+}  // extern "C"

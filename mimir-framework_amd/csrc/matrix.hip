@@ -1,0 +1,80 @@
+// matrix.hip -- what the products of matrix.hpp need beside themselves: operands
+// split or copied into planes of bf16, slices of a split contraction joined, scratch.
+#include "matrix.hpp"
+
+using namespace mimir;
+
+namespace {
+
+// Eight columns a thread: 32 bytes of fp32 read, 16 written to each of three planes.
+template <bool BF16, bool VEC>
+__global__ __launch_bounds__(kBlock) void stage_rows(const void* src, int64_t rows, int64_t cols, int64_t ld, uint16_t* dst,
+                                                      int64_t ld_dst, int64_t plane) {
+    const int64_t of_row = ld_dst / 8, total = rows * of_row, stride = static_cast<int64_t>(gridDim.x) * kBlock;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * kBlock + threadIdx.x; i < total; i += stride) {
+        const int64_t r = i / of_row, c = i % of_row * 8;
+        mat_stage8<BF16, VEC>(src, r * ld + c, cols - c, dst + r * ld_dst + c, plane);
+    }
+}
+
+__global__ __launch_bounds__(kBlock) void join_slices(MatOut o, int64_t n, int64_t m, const int32_t* n_dev, int splits) {
+    if (n_dev) n = min(n, static_cast<int64_t>(*n_dev));
+    const float by = o.factor();
+    const int64_t of_row = (m + 3) / 4, total = n * of_row, stride = static_cast<int64_t>(gridDim.x) * kBlock;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * kBlock + threadIdx.x; i < total; i += stride) {
+        const int64_t r = i / of_row, c = i % of_row * 4;
+        const float* p = o.partial + r * o.ld_partial + c;
+        f4 v{};
+        for (int s = 0; s < splits; ++s) v += *reinterpret_cast<const f4*>(p + s * o.slice);
+        o.put(0, r, static_cast<int32_t>(c), static_cast<int32_t>(m), v, by);
+    }
+}
+
+unsigned grid_of(int64_t items) {
+    const int64_t b = (items + kBlock - 1) / kBlock;
+    return static_cast<unsigned>(b < 1 ? 1 : b > 65536 ? 65536 : b);
+}
+
+}  // namespace
+
+int mimir::mat_stage(mimir_ctx* ctx, int type, const void* src, int64_t rows, int64_t cols, int64_t ld, uint16_t* dst,
+                     int64_t ld_dst, int64_t plane) {
+    const unsigned grid = grid_of(rows * (ld_dst / 8));
+    if (rows == 0) return MIMIR_OK;
+    if (type == MIMIR_NUM_BF16) {
+        if (aligned16(src) && ld % 8 == 0) stage_rows<true, true><<<grid, kBlock, 0, ctx->stream>>>(src, rows, cols, ld, dst, ld_dst, plane);
+        else stage_rows<true, false><<<grid, kBlock, 0, ctx->stream>>>(src, rows, cols, ld, dst, ld_dst, plane);
+    } else {
+        if (aligned16(src) && ld % 4 == 0) stage_rows<false, true><<<grid, kBlock, 0, ctx->stream>>>(src, rows, cols, ld, dst, ld_dst, plane);
+        else stage_rows<false, false><<<grid, kBlock, 0, ctx->stream>>>(src, rows, cols, ld, dst, ld_dst, plane);
+    }
+    return launched(ctx, "stage_rows");
+}
+
+int mimir::mat_join(mimir_ctx* ctx, const MatOut& o, int64_t n, int64_t m, const int32_t* n_dev, int splits) {
+    if (n == 0 || m == 0) return MIMIR_OK;
+    join_slices<<<grid_of(n * ((m + 3) / 4)), kBlock, 0, ctx->stream>>>(o, n, m, n_dev, splits);
+    return launched(ctx, "join_slices");
+}
+
+int mimir::mat_scratch(mimir_ctx* ctx, size_t bytes, char** out) {
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    const hipError_t e = hipStreamIsCapturing(ctx->stream, &status);
+    if (e != hipSuccess) return hip_fail(ctx, e, "hipStreamIsCapturing");
+    void* p = nullptr;
+    int st;
+    if (status == hipStreamCaptureStatusNone) {
+        st = ensure_scratch(ctx, bytes, &p);
+    } else {
+        // A graph will hold the scratch's address: nothing of it is freed before the
+        // context is.  An allocation is no part of the graph.
+        if (!ctx->captured) graph_pin(ctx);
+        ctx->captured = true;
+        hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
+        if (hipThreadExchangeStreamCaptureMode(&mode) != hipSuccess) return fail(ctx, MIMIR_EDEVICE, "hipThreadExchangeStreamCaptureMode");
+        st = ensure_scratch(ctx, bytes, &p);
+        (void)hipThreadExchangeStreamCaptureMode(&mode);
+    }
+    *out = static_cast<char*>(p);
+    return st;
+}

@@ -1,0 +1,474 @@
+// matrix.hpp -- the wide products of a training step (a linear layer's cross
+// entropy, linear_ce.hip, and the gated products of a feed-forward block,
+// gated_linear.hip) on the bf16 matrix cores, with what follows a product done
+// on its registers (an Epi).
+//
+//   C[n][m] = sum_k A(m, k) B(n, k)
+//
+// A and B are planes of bf16 in memory: one for bf16 values, three for fp32
+// (split.hpp: x = h + m + l, six products), two for a value held closer than
+// bf16 beside a bf16 operand.  An operand is kRows (element (r, k) at r * ld + k)
+// or kCols (at k * ld + r): a matrix has one layout for every product it is in,
+// and no transposed copy is made.
+//
+// A workgroup computes BM x BN of C, WGM x WGN waves of 32 x 32 blocks.  A step
+// takes BK of the contraction: its tiles go from memory to one of two LDS
+// buffers by buffer loads that write LDS, while the products of the step before
+// run from the other; one barrier a step.  Those loads put the 16 bytes of lane l
+// at 16 l of a wave's kilobyte, so the order that keeps reads off each other's
+// banks is made by what each lane asks for: 16-byte chunk c of row r stands at
+// chunk c ^ swizzle(r).  kRows operands are read in ds_read_b128, kCols ones four
+// values of four k at a time by ds_read_b64_tr_b16, which transposes them.  Both
+// give lane l row l % 32 and k = 8 (l / 32) .. + 7 of a 32 x 16 operand.
+//
+// A lane of the product holds one n (l % 32) and, in its 16 registers, m =
+// 8 (r / 4) + 4 (l / 32) + r % 4: reductions over m stay in registers, and four
+// values of one row of C[n][m] are stored at a time.
+//
+// Every load's row and k are compared with the operand's own (kOutside, which
+// reads zeros), so operands may end anywhere; a chunk of 8 lies within a row, ld
+// is a multiple of 8 and the operand 16-byte aligned.
+#pragma once
+
+#include "internal.hpp"
+#include "split.hpp"
+
+#include <type_traits>
+
+namespace mimir {
+
+enum : int { kRows = 0, kCols = 1 };
+
+struct MatOperand {
+    const uint16_t* p;
+    int64_t ld;     // elements between rows in memory
+    int64_t plane;  // elements between planes
+};
+
+struct MatArgs {
+    // With two segments the contraction runs over (a[0], b[0]), then (a[1], b[1]);
+    // with two batches, or a dual A, a[1] is the second's and b[1] is not read.
+    MatOperand a[2], b[2];
+    int32_t m, n, k;        // k of one segment
+    const int32_t* n_dev;   // not null: n is at most this
+    const int32_t* k_dev;   // not null: k is at most this
+    int32_t segments, batches, splits;
+};
+
+struct MatAt {
+    int32_t m0, n0, m, n;  // the tile's first, and the limits
+    int32_t batch, split, tile_m;
+};
+
+// Every workgroup runs it once; a workgroup of 64 * WGM * WGN threads.
+template <int BM, int BN, int WGM, int WGN, int BK, int PA, int PB, int KA, int KB, bool DUAL = false>
+struct MatShape {
+    static constexpr int kM = BM, kN = BN, kWaveM = WGM, kWaveN = WGN, kK = BK, kPa = PA, kPb = PB, kKindA = KA, kKindB = KB;
+    static constexpr bool kDual = DUAL;
+    static constexpr int kWaves = WGM * WGN, kThreads = kWave * kWaves;
+    static constexpr int kBm = BM / WGM / 32, kBn = BN / WGN / 32;  // 32 x 32 blocks of a wave
+    static constexpr int kSubs = DUAL ? 2 : 1, kSubRows = BM / kSubs, kSubBlocks = kBm / kSubs;
+    static constexpr int kPlaneA = BM * BK * 2, kPlaneB = BN * BK * 2;  // bytes
+    static constexpr int kStage = PA * kPlaneA + PB * kPlaneB;
+    static constexpr int kLds = 2 * kStage;
+    static_assert(kLds <= 160 * 1024 && kBm % kSubs == 0 && BK % 16 == 0);
+};
+
+// --- one operand's tile: R rows by BK --------------------------------------------
+
+template <int R, int BK, int KIND>
+__device__ __forceinline__ constexpr int mat_swizzle(int i) {
+    // kRows, of row i: rows of 128 bytes use eight places, rows of 64 bytes four for
+    // two rows.  kCols, of k i: four k's 64 bytes (32 values) in different banks.
+    if (KIND == kRows) return BK == 64 ? i & 7 : (i >> 1) & 3;
+    return R == 64 ? 4 * ((i >> 1) & 1) : 4 * (i & 3);
+}
+
+// LDS writes of 16 bytes a lane, behind each other from `lds` (uniform) on.  In asm:
+// the compiler would wait for a builtin's load before any later LDS read, since it
+// does not tell the two buffers apart.  The kernel waits itself (mat_landed); nothing
+// else in it uses m0, which no clobber list can name.
+__device__ __forceinline__ void load_to_lds(uint32_t lds, uint32_t voff, __amdgpu_buffer_rsrc_t rs, uint32_t soff) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+                 :
+                 : "s"(lds), "v"(voff), "s"(rs), "s"(soff)
+                 : "memory");
+}
+__device__ __forceinline__ void mat_landed() { asm volatile("s_waitcnt vmcnt(0)" : : : "memory"); }
+
+template <int R, int BK, int P, int KIND, int WAVES>
+struct MatTile {
+    static constexpr int kBytes = R * BK * 2;
+    static constexpr int kLoads = kBytes / 1024 / WAVES;  // of a wave, a plane
+    static_assert(kLoads >= 1 && kBytes % (1024 * WAVES) == 0);
+    static constexpr int kLanes = KIND == kRows ? BK / 8 : R / 8;  // 16-byte chunks of a row of the tile
+    static constexpr int kRowsOf = kWave / kLanes;                // rows of the tile in a wave's kilobyte
+    // kRows: every load has other rows, each at its own limit, and the same k.  kCols:
+    // every load has other k's and the same rows.
+    uint32_t off[KIND == kRows ? kLoads : 1];
+    int32_t k_mine;
+
+    __device__ __forceinline__ void init(int64_t ld, int32_t rows) {
+        const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+        const int r = lane / kLanes, slot = lane % kLanes;
+        if constexpr (KIND == kRows) {
+            const int chunk = slot ^ mat_swizzle<R, BK, KIND>(r);  // a kilobyte's rows are a multiple of the swizzle's
+            k_mine = 8 * chunk;
+#pragma unroll
+            for (int j = 0; j < kLoads; ++j) {
+                const int row = (j * WAVES + wave) * kRowsOf + r;
+                off[j] = row < rows ? static_cast<uint32_t>(row * ld * 2 + 16 * chunk) : kOutside;
+            }
+        } else {
+            k_mine = wave * kRowsOf + r;  // load j: + j * WAVES * kRowsOf, a multiple of the swizzle's four
+            const int chunk = slot ^ mat_swizzle<R, BK, KIND>(k_mine);
+            off[0] = 8 * chunk < rows ? static_cast<uint32_t>(k_mine * ld * 2 + 16 * chunk) : kOutside;
+        }
+    }
+    static_assert(KIND == kRows || (WAVES * kRowsOf) % 4 == 0 || kLoads == 1);
+    static_assert(KIND == kCols || kRowsOf % 8 == 0);
+
+    // k0 .. k0 + BK of the contraction, `left` of them inside it.  base: the tile's first row.
+    __device__ __forceinline__ void load(uint32_t lds, const MatOperand& o, const uint16_t* base, int32_t k0, int32_t left) const {
+        const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+            const uint16_t* at = base + p * o.plane + (KIND == kRows ? k0 : k0 * o.ld);
+            const __amdgpu_buffer_rsrc_t rs =
+                __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(at), 0, 0x7fffffff, kBufferWord3);
+#pragma unroll
+            for (int j = 0; j < kLoads; ++j) {
+                const uint32_t to = lds + p * kBytes + (j * WAVES + wave) * 1024;
+                if constexpr (KIND == kRows) {
+                    load_to_lds(to, left >= BK || k_mine < left ? off[j] : kOutside, rs, 0);
+                } else {
+                    constexpr int kNext = WAVES * kRowsOf;
+                    load_to_lds(to, left >= BK || k_mine + j * kNext < left ? off[0] : kOutside, rs,
+                                static_cast<uint32_t>(j * kNext * o.ld * 2));
+                }
+            }
+        }
+    }
+};
+
+typedef int16_t s4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s4* lds_tr;
+
+// A lane's part of a 32 x 16 operand in a tile.
+template <int R, int BK, int KIND>
+struct MatRead {
+    static constexpr int kBytes = R * BK * 2;
+
+    // Rows row0 .. + 31 (a multiple of 32), k 16 c .. + 15.
+    static __device__ __forceinline__ u4 get(const char* tile, int row0, int c, int p) {
+        const int lane = threadIdx.x % kWave, li = lane % 32, hf = lane / 32;
+        const char* base = tile + p * kBytes;
+        if constexpr (KIND == kRows) {
+            const int chunk = (2 * c + hf) ^ mat_swizzle<R, BK, KIND>(li);
+            return *reinterpret_cast<const u4*>(base + (row0 + li) * (BK * 2) + 16 * chunk);
+        } else {
+            const int q = lane % 16 / 4;                                   // k % 4
+            const int k = 16 * c + 8 * hf + q;
+            const int chunk = (row0 / 8 + 2 * (lane / 16 % 2) + lane % 4 / 2);
+            const char* a = base + k * (2 * R) + 16 * (chunk ^ mat_swizzle<R, BK, KIND>(k)) + 8 * (lane % 2);
+            const char* b = base + (k + 4) * (2 * R) + 16 * (chunk ^ mat_swizzle<R, BK, KIND>(k + 4)) + 8 * (lane % 2);
+            const u2 x = __builtin_bit_cast(u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_tr)a));
+            const u2 y = __builtin_bit_cast(u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_tr)b));
+            return u4{x[0], x[1], y[0], y[1]};
+        }
+    }
+};
+
+// --- the product ------------------------------------------------------------------
+
+constexpr int kMatXcds = 8;
+constexpr int kMatGroup = 4;  // n tiles that neighbours in the order share
+
+// Workgroup -> tile.  Workgroups go to the XCDs round-robin; each XCD takes a
+// contiguous run of the tiles that there are (n may be known on the device alone),
+// four n tiles beside each other for each m, so that the 32 tiles in flight on an
+// XCD read 8 tiles of A and 4 of B.
+template <class S>
+__device__ __forceinline__ bool mat_tile_of(const MatArgs& g, MatAt* at) {
+    at->m = g.m;
+    at->n = g.n_dev ? min(g.n, *g.n_dev) : g.n;
+    const uint32_t tiles_m = (g.m + S::kM / S::kSubs - 1) / (S::kM / S::kSubs), tiles_n = (at->n + S::kN - 1) / S::kN;
+    const uint32_t one = tiles_m * tiles_n, total = one * g.batches * g.splits;
+    const uint32_t per = (total + kMatXcds - 1) / kMatXcds;
+    const uint32_t i = (blockIdx.x % kMatXcds) * per + blockIdx.x / kMatXcds;
+    if (blockIdx.x / kMatXcds >= per || i >= total) return false;
+    const uint32_t r = i % one, z = i / one;
+    at->batch = z % g.batches;
+    at->split = z / g.batches;
+    const uint32_t group = r / (kMatGroup * tiles_m), first = group * kMatGroup, wide = min(tiles_n - first, uint32_t{kMatGroup});
+    const uint32_t in = r - group * kMatGroup * tiles_m;
+    at->tile_m = in / wide;
+    at->m0 = at->tile_m * (S::kM / S::kSubs);
+    at->n0 = (first + in % wide) * S::kN;
+    return true;
+}
+
+// A wave's blocks of C, and which they are.
+template <class S>
+struct MatAcc {
+    f16v c[S::kBm][S::kBn];
+    int wm, wn;  // the wave
+    // First row (m, within the tile or, dual, within its half) of block i, first column (n) of block j.
+    __device__ __forceinline__ int row(int i) const {
+        return wm * (S::kSubRows / S::kWaveM) + 32 * (i % S::kSubBlocks);
+    }
+    __device__ __forceinline__ int col(int j) const { return wn * (S::kN / S::kWaveN) + 32 * j; }
+    // m of register r of block i, within the tile.
+    __device__ __forceinline__ int m_of(int i, int r) const {
+        return row(i) + 8 * (r / 4) + 4 * (threadIdx.x % kWave / 32) + r % 4;
+    }
+    __device__ __forceinline__ int n_of(int j) const { return col(j) + threadIdx.x % 32; }
+};
+
+template <class S, class Epi>
+__global__ __launch_bounds__(S::kThreads, S::kThreads == 512 ? 2 : 1) void mat_kernel(MatArgs g, Epi epi) {
+    __shared__ __attribute__((aligned(1024))) char lds[S::kLds];
+    MatAt at;
+    if (!mat_tile_of<S>(g, &at)) return;
+    const int32_t k = g.k_dev ? min(g.k, *g.k_dev) : g.k;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    MatAcc<S> acc;
+    acc.wm = wave / S::kWaveN;
+    acc.wn = wave % S::kWaveN;
+
+    using TileA = MatTile<S::kSubRows, S::kK, S::kPa, S::kKindA, S::kWaves>;
+    using TileB = MatTile<S::kN, S::kK, S::kPb, S::kKindB, S::kWaves>;
+    TileA ta;
+    TileB tb;
+    ta.init(g.a[0].ld, g.m - at.m0);
+    tb.init(g.b[0].ld, at.n - at.n0);
+    const auto first = [](const MatOperand& o, int kind, int32_t row) { return o.p + (kind == kRows ? row * o.ld : row); };
+
+    // Steps of this workgroup: the split's share of all segments' steps.
+    const int32_t of_one = (k + S::kK - 1) / S::kK, all = of_one * g.segments;
+    const int32_t begin = static_cast<int32_t>(static_cast<int64_t>(all) * at.split / g.splits);
+    const int32_t end = static_cast<int32_t>(static_cast<int64_t>(all) * (at.split + 1) / g.splits);
+    const uint32_t base = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)lds));
+    const auto load = [&](int32_t step, int buf) {
+        const int seg = g.segments > 1 && step >= of_one;
+        const int32_t k0 = (step - seg * of_one) * S::kK, left = k - k0;
+        const uint32_t to = base + buf * S::kStage;
+#pragma unroll
+        for (int s = 0; s < S::kSubs; ++s) {
+            const MatOperand& o = g.a[S::kDual ? s : g.segments > 1 ? seg : at.batch];
+            ta.load(to + s * S::kPa * TileA::kBytes, o, first(o, S::kKindA, at.m0), k0, left);
+        }
+        const MatOperand& o = g.b[seg];
+        tb.load(to + S::kPa * S::kPlaneA, o, first(o, S::kKindB, at.n0), k0, left);
+    };
+
+#pragma unroll
+    for (int i = 0; i < S::kBm; ++i)
+#pragma unroll
+        for (int j = 0; j < S::kBn; ++j) acc.c[i][j] = f16v{};
+    if (begin < end) load(begin, 0);
+    for (int32_t step = begin; step < end; ++step) {
+        const int buf = (step - begin) & 1;
+        mat_landed();
+        __syncthreads();
+        if (step + 1 < end) load(step + 1, buf ^ 1);
+        const char* la = lds + buf * S::kStage;
+        const char* lb = la + S::kPa * S::kPlaneA;
+#pragma unroll
+        for (int c = 0; c < S::kK / 16; ++c) {
+            u4 a[S::kBm][S::kPa], b[S::kBn][S::kPb];
+#pragma unroll
+            for (int p = 0; p < S::kPb; ++p)
+#pragma unroll
+                for (int j = 0; j < S::kBn; ++j) b[j][p] = MatRead<S::kN, S::kK, S::kKindB>::get(lb, acc.col(j), c, p);
+#pragma unroll
+            for (int p = 0; p < S::kPa; ++p)
+#pragma unroll
+                for (int i = 0; i < S::kBm; ++i)
+                    a[i][p] = MatRead<S::kSubRows, S::kK, S::kKindA>::get(
+                        la + (i / S::kSubBlocks) * S::kPa * TileA::kBytes, acc.row(i), c, p);
+            // The small products first (mfma_split's order where both have three planes).
+            constexpr int kLast = (S::kPa > S::kPb ? S::kPa : S::kPb) - 1;
+#pragma unroll
+            for (int sum = kLast; sum >= 0; --sum)
+#pragma unroll
+                for (int pa = S::kPa - 1; pa >= 0; --pa) {
+                    const int pb = sum - pa;
+                    if (pb < 0 || pb >= S::kPb) continue;
+#pragma unroll
+                    for (int i = 0; i < S::kBm; ++i)
+#pragma unroll
+                        for (int j = 0; j < S::kBn; ++j) acc.c[i][j] = mfma_bf16(a[i][pa], b[j][pb], acc.c[i][j]);
+                }
+        }
+    }
+    __syncthreads();  // the epilogue may use the LDS
+    epi.template run<S>(at, acc, lds);
+}
+
+template <class S>
+int64_t mat_tiles(const MatArgs& g) {
+    const int64_t tm = S::kM / S::kSubs;
+    return (g.m + tm - 1) / tm * ((g.n + S::kN - 1) / S::kN) * g.batches;
+}
+
+// The two shapes of a product with PA and PB planes: a CU's workgroup of eight waves
+// where such tiles fill most of the GPU, else four waves, two or more to a CU.
+template <int PA, int PB, int KA, int KB, bool DUAL = false>
+using MatBig = std::conditional_t<PA == 3, MatShape<256, 128, 4, 2, 32, 3, 3, KA, KB, DUAL>,
+                                  MatShape<256, 256, 2, 4, 64, PA, PB, KA, KB, DUAL>>;
+template <int PA, int PB, int KA, int KB, bool DUAL = false>
+using MatSmall = std::conditional_t<PA == 3, MatShape<128, 64, 2, 2, 32, 3, 3, KA, KB, DUAL>,
+                                    MatShape<128, 128, 2, 2, 64, PA, PB, KA, KB, DUAL>>;
+constexpr int64_t kMatBigTiles = 192;
+template <class S>
+bool mat_fills(const mimir_ctx* ctx, const MatArgs& g) {
+    return ctx->tune.mat_big >= 0 ? ctx->tune.mat_big == 1 : mat_tiles<S>(g) >= kMatBigTiles;
+}
+
+// The byte offsets within a tile fit 31 bits.
+inline bool mat_ld_fits(int64_t ld) { return ld < (int64_t{1} << 20); }
+
+template <class S, class Epi>
+int mat_launch(mimir_ctx* ctx, const char* what, const MatArgs& g, const Epi& epi) {
+    const int64_t total = mat_tiles<S>(g) * g.splits;
+    const int64_t grid = (total + kMatXcds - 1) / kMatXcds * kMatXcds;
+    if (total == 0) return MIMIR_OK;
+    MIMIR_REQUIRE(ctx, dispatch_fits(grid, S::kThreads), "%s: grid of %lld workgroups exceeds the limit", what, (long long)grid);
+    mat_kernel<S, Epi><<<static_cast<unsigned>(grid), S::kThreads, 0, ctx->stream>>>(g, epi);
+    return launched(ctx, what);
+}
+
+// --- C as a result -----------------------------------------------------------------
+
+// out[row(n)][m] (+)= alpha * sum, sum over the pieces and splits of the contraction
+// that fp32 slices hold (`partial`, one for each split, row n at n * ld_partial).
+// A lane has four m's of a row: one 16-byte (fp32) or 8-byte (bf16) store.
+struct MatOut {
+    void* out[2];             // of each batch
+    int64_t ld;
+    const int32_t* row;       // not null: the row of n
+    float* partial;           // [splits][n][ld_partial], not null if read or written
+    int64_t ld_partial, slice;
+    const float* count;       // not null: alpha is divided by max(count, 1)
+    float alpha;
+    int32_t bf16, accumulate;
+    int32_t read_partial;     // pieces before this one have left their sums
+    int32_t last;             // this piece's sums go to out, not to partial
+    int32_t vec;              // out and ld are multiples of four elements
+
+    __device__ __forceinline__ float factor() const { return count ? alpha / fmaxf(*count, 1.0f) : alpha; }
+    __device__ __forceinline__ void put(int batch, int64_t n, int32_t m, int32_t limit, f4 v, float by) const {
+        const int64_t r = row ? row[n] : n;
+        if (bf16) {
+            uint16_t* p = static_cast<uint16_t*>(out[batch]) + r * ld + m;
+            f4 old{};
+            if (vec && m + 4 <= limit) {
+                if (accumulate) {
+                    const u2 t = *reinterpret_cast<const u2*>(p);
+                    old = f4{__builtin_bit_cast(float, t[0] << 16), __builtin_bit_cast(float, t[0] & 0xffff0000u),
+                             __builtin_bit_cast(float, t[1] << 16), __builtin_bit_cast(float, t[1] & 0xffff0000u)};
+                }
+                v = v * by + old;
+                *reinterpret_cast<u2*>(p) = u2{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])};
+                return;
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (m + e < limit) {
+                    const float x = v[e] * by + (accumulate ? __builtin_bit_cast(float, static_cast<uint32_t>(p[e]) << 16) : 0.0f);
+                    p[e] = static_cast<uint16_t>(pack_bf16(x, x));
+                }
+            return;
+        }
+        float* p = static_cast<float*>(out[batch]) + r * ld + m;
+        if (vec && m + 4 <= limit) {
+            f4* q = reinterpret_cast<f4*>(p);
+            *q = accumulate ? v * by + *q : v * by;
+            return;
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (m + e < limit) p[e] = accumulate ? v[e] * by + p[e] : v[e] * by;
+    }
+
+    template <class S>
+    __device__ __forceinline__ void run(const MatAt& at, MatAcc<S>& acc, char*) const {
+        const float by = factor();
+#pragma unroll
+        for (int j = 0; j < S::kBn; ++j) {
+            const int32_t n = at.n0 + acc.n_of(j);
+            if (n >= at.n) continue;
+#pragma unroll
+            for (int i = 0; i < S::kBm; ++i)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const int32_t m = at.m0 + acc.m_of(i, 4 * q);
+                    if (m >= at.m) continue;
+                    f4 v{acc.c[i][j][4 * q], acc.c[i][j][4 * q + 1], acc.c[i][j][4 * q + 2], acc.c[i][j][4 * q + 3]};
+                    // ld_partial is a multiple of four: a whole vector, past m too.
+                    f4* p = reinterpret_cast<f4*>(partial + at.split * slice + n * ld_partial + m);
+                    if (read_partial) v += *p;
+                    if (last) put(at.batch, n, m, at.m, v, by);
+                    else *p = v;
+                }
+        }
+    }
+};
+
+// --- operands from a caller's matrices (matrix.hip) --------------------------------
+
+constexpr int64_t mat_round(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
+
+// Whether bf16 rows can be an operand as they are.
+inline bool mat_direct(const void* p, int64_t ld, int64_t cols) {
+    return aligned16(p) && ld % 8 == 0 && cols % 8 == 0 && mat_ld_fits(ld);
+}
+
+// Eight values from element `at` of src on, `left` of them in the row, to dst, `plane`
+// elements to the next plane.  VEC: 16-byte loads.
+template <bool BF16, bool VEC>
+__device__ __forceinline__ void mat_stage8(const void* src, int64_t at, int64_t left, uint16_t* dst, int64_t plane) {
+    if constexpr (BF16) {
+        const uint16_t* p = static_cast<const uint16_t*>(src) + at;
+        u4 v{};
+        if (VEC && left >= 8) {
+            v = *reinterpret_cast<const u4*>(p);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (e < left) v[e / 2] |= static_cast<uint32_t>(p[e]) << (16 * (e % 2));
+        }
+        *reinterpret_cast<u4*>(dst) = v;
+    } else {
+        const float* p = static_cast<const float*>(src) + at;
+        float x[8];
+        if (VEC && left >= 8) {
+            const f4 a = *reinterpret_cast<const f4*>(p), b = *reinterpret_cast<const f4*>(p + 4);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = a[e], x[4 + e] = b[e];
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = e < left ? p[e] : 0.0f;
+        }
+        const Split8 s = split8(x);
+        *reinterpret_cast<u4*>(dst) = s.h;
+        *reinterpret_cast<u4*>(dst + plane) = s.m;
+        *reinterpret_cast<u4*>(dst + 2 * plane) = s.l;
+    }
+}
+
+// dst [planes][.][ld_dst]: `rows` rows of `cols`, split into planes (fp32: three,
+// bf16: one), zeros up to ld_dst (a multiple of 8, at least cols).  plane: elements
+// between planes.
+int mat_stage(mimir_ctx* ctx, int type, const void* src, int64_t rows, int64_t cols, int64_t ld, uint16_t* dst, int64_t ld_dst,
+              int64_t plane);
+// The sum of `splits` slices into out (MatOut's fields say how), n_dev as MatArgs'.
+int mat_join(mimir_ctx* ctx, const MatOut& o, int64_t n, int64_t m, const int32_t* n_dev, int splits);
+
+// The context's scratch of at least `bytes`, also while its stream is being captured:
+// then the old one, which the graph or one before it may hold, is kept as long as the
+// context.
+int mat_scratch(mimir_ctx* ctx, size_t bytes, char** out);
+
+}  // namespace mimir

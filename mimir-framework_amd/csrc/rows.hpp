@@ -50,7 +50,7 @@ struct RowShape {
 //   MIMIR_TUNE="norm=1024x1x1024,layernorm=512x2x512,softmax=64x4x64,ew=1,gather=1024,rope=1,
 //               lnbwd=512x2x512,lnbwd_grid=512,chain=0,attnbwd_heads=4,attnbwd_blocks=2,
 //               embsort=0,embruns=0,emb1pass=0,blas=0,lnbwd_narrow=0,lrcpw=2,ewbs=128,
-//               lrapply=256x4,lrpart=256"
+//               lrapply=256x4,lrpart=256,matpiece=256,matbig=1"
 // Each entry selects among the compiled variants above; an entry that does
 // not fit a call (row too wide for it) is ignored for that call.  Unset, the
 // measured defaults apply.  Used for sweeps; results are identical.
@@ -78,6 +78,8 @@ struct Tuning {
                                 // in three (0)
     int blas_lt = -1;           // library products: hipBLASLt first (-1, 1) or rocBLAS only (0)
     int gemm = 0;               // matrix products: 128 (gemm_tile), 16 or 4 (waves of gemm_strip), 1 (library); 0: by size
+    int mat_piece = 0;          // wide products: rows of w, or hidden columns, of a piece (0: what 512 MiB hold)
+    int mat_big = -1;           // wide products: the larger tiles always (1), never (0) or where they fill the GPU (-1)
     int lnbwd_narrow = -1;      // LayerNorm backward, rows <= 64 floats: several rows per wave (-1, 1) or not (0)
     int lr_cpw = 0;             // long rows: 4096-float chunks per workgroup of the first pass (1, 2, 4; 0: measured default)
     int ew_bs = 0;              // workgroup size of the one-float4-per-thread streaming kernels (64 .. 1024; 0: default)
@@ -131,6 +133,8 @@ inline Tuning read_tuning() {
         else if (!std::strcmp(k, "emb1pass")) t.embed_bwd_onepass = std::atoi(v);
         else if (!std::strcmp(k, "blas")) t.blas_lt = std::atoi(v);
         else if (!std::strcmp(k, "gemm")) t.gemm = std::atoi(v);
+        else if (!std::strcmp(k, "matpiece")) t.mat_piece = std::atoi(v);
+        else if (!std::strcmp(k, "matbig")) t.mat_big = std::atoi(v);
         else if (!std::strcmp(k, "lnbwd_narrow")) t.lnbwd_narrow = std::atoi(v);
         else if (!std::strcmp(k, "lrcpw")) t.lr_cpw = std::atoi(v);
         else if (!std::strcmp(k, "ewbs")) t.ew_bs = std::atoi(v);

@@ -32,6 +32,8 @@ BRANCH_TYPES = ("NONE", "RESIDUAL", "SKIP_CONNECTION", "DENSE_CONNECTION", "ATTE
 # MIMIR_KV_* (element types of a key/value cache) and MIMIR_ROPE_SCALE_*, in order.
 KV_TYPES = ("f32", "bf16", "i8")
 ROPE_SCALINGS = ("none", "linear", "base", "by_parts")
+# MIMIR_NUM_* (element types of the training calls' matrices), in order.
+NUM_TYPES = ("f32", "bf16")
 MERGE_OPS = ("ADD", "MULTIPLY", "CONCATENATE", "MAX", "AVERAGE", "GATED", "ATTENTION_WEIGHTED")
 
 
@@ -162,6 +164,9 @@ SIGNATURES = {
     "mimir_add_bwd": (c_int, [_P, _P, c_int64, c_int64, _P, _P, c_int, c_int]),
     "mimir_embedding_bwd": (c_int, [_P, _P, c_int64, _P, _P, c_int64, c_int32, c_int32, c_int32]),
     "mimir_embedding_f32ids_bwd": (c_int, [_P, _P, c_int64, _P, _P, c_int64, c_int32, c_int32, c_int32]),
+    "mimir_linear_cross_entropy_fwd": (c_int, [_P, c_int, _P, c_int64, _P, c_int64, _P, c_int64, c_int64, c_int64, _P, _P, _P]),
+    "mimir_linear_cross_entropy_bwd": (c_int, [_P, c_int, _P, c_int64, _P, c_int64, _P, c_int64, c_int64, c_int64, _P, _P, _P,
+                                               c_float, _P, c_int64, c_int, _P, c_int64, c_int]),
     "mimir_store_create": (c_int, [_P, _PP]),
     "mimir_store_destroy": (c_int, [_P]),
     "mimir_store_clear": (c_int, [_P]),

@@ -78,6 +78,13 @@ def _ptr(x):
     raise TypeError(f"expected a DeviceArray or a device address, got {type(x)}")
 
 
+def _num(dtype):
+    """MIMIR_NUM_* of "f32" or "bf16"."""
+    if dtype not in _lib.NUM_TYPES:
+        raise ValueError(f"type {dtype!r}: one of {_lib.NUM_TYPES}")
+    return _lib.NUM_TYPES.index(dtype)
+
+
 class Context:
     """One HIP device + stream (``mimir_ctx``)."""
 
@@ -325,6 +332,24 @@ class Context:
         fn = self.lib.mimir_embedding_f32ids_bwd if float_ids else self.lib.mimir_embedding_bwd
         self.check(fn(self.handle, _ptr(ids), n_ids, _ptr(dy), _ptr(grad_table), table_len, vocab, dim,
                       padding_idx))
+
+
+    # -- training: the last layer's loss, gated products, gradients' norm ---------
+
+    def linear_cross_entropy(self, x, w, targets, tokens, dim, vocab, loss, lse, mean=None, dtype="f32", ld_x=None, ld_w=None):
+        """mimir_linear_cross_entropy_fwd: loss and lse of each token, mean = {mean
+        loss, tokens that count}; rows of x and w default to dim."""
+        self.check(self.lib.mimir_linear_cross_entropy_fwd(self.handle, _num(dtype), _ptr(x), ld_x or dim, _ptr(w), ld_w or dim,
+                                                           _ptr(targets), tokens, dim, vocab, _ptr(loss), _ptr(lse), _ptr(mean)))
+
+    def linear_cross_entropy_bwd(self, x, w, targets, lse, dloss, mean, dx, dw, tokens, dim, vocab, scale=1.0, dtype="f32",
+                                 ld_x=None, ld_w=None, ld_dx=None, ld_dw=None, accumulate_x=False, accumulate_w=False):
+        """mimir_linear_cross_entropy_bwd: dx and dw (either may be None); dloss None
+        and the forward's mean give the gradient of the mean loss."""
+        self.check(self.lib.mimir_linear_cross_entropy_bwd(
+            self.handle, _num(dtype), _ptr(x), ld_x or dim, _ptr(w), ld_w or dim, _ptr(targets), tokens, dim, vocab, _ptr(lse),
+            _ptr(dloss), _ptr(mean), float(scale), _ptr(dx), ld_dx or dim, int(bool(accumulate_x)), _ptr(dw), ld_dw or dim,
+            int(bool(accumulate_w))))
 
 
 class Event:

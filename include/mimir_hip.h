@@ -596,6 +596,59 @@ int mimir_linear_cross_entropy_bwd(mimir_ctx* ctx, int type, const void* x, int6
                                    const float* dloss, const float* mean, float scale, void* dx, int64_t ld_dx,
                                    int accumulate_x, void* dw, int64_t ld_dw, int accumulate_w);
 
+/* Activations of the gated products. */
+#define MIMIR_ACT_SILU 0 /* x / (1 + exp(-x)), mimir_silu_fwd's */
+#define MIMIR_ACT_GELU 1 /* the tanh form, mimir_gelu_fwd's */
+
+/* The gated products of a feed-forward block, y = act(x Wg) * (x Wu): x [tokens][dim]
+ * (row stride ld_x), Wg and Wu [dim][hidden] (both ld_w; input by output, as the
+ * attention layers' weights), y [tokens][hidden] (ld_y), all of `type`; y is rounded
+ * once.  Exactness and magnitudes as mimir_linear_cross_entropy_fwd's.  gate_up
+ * [tokens][2 * hidden], fp32, 16-byte aligned, gets x Wg then x Wu of each token for
+ * the backward (NULL: they are not written).  tokens up to 2^24, dim to 2^18, hidden to
+ * 2^20.  y must not overlap the inputs.  Scratch (the context's): fp32, or rows that
+ * are no 16-byte multiples: x again and up to 512 MiB of the weights' columns. */
+int mimir_gated_linear_fwd(mimir_ctx* ctx, int type, int act, const void* x, int64_t ld_x, const void* w_gate,
+                           const void* w_up, int64_t ld_w, int64_t tokens, int64_t dim, int64_t hidden, void* y,
+                           int64_t ld_y, float* gate_up);
+
+/* Its gradients from the forward's gate_up and dy [tokens][hidden] (ld_dy):
+ *   du = dy * act(gate), dg = dy * up * act'(gate)
+ *   dx = dg Wg^T + du Wu^T, dWg = x^T dg, dWu = x^T du
+ * dx [tokens][dim] (ld_dx) written, or added to where accumulate_x, and dWg, dWu
+ * [dim][hidden] (both ld_dw) likewise with accumulate_w; all of `type`, rounded once.
+ * dx, or dWg and dWu together, may be NULL.  For bf16, dg and du are held in bf16 in
+ * between (with at most 128 tokens as two bf16 terms).  Outputs must not overlap the
+ * inputs or one another.  The same call gives the same bits.  Scratch: as the
+ * forward's, up to 512 MiB (at least 256 columns) with dg and du, and fp32 sums where
+ * the columns are taken in pieces or there are few tiles. */
+int mimir_gated_linear_bwd(mimir_ctx* ctx, int type, int act, const void* x, int64_t ld_x, const void* w_gate,
+                           const void* w_up, int64_t ld_w, int64_t tokens, int64_t dim, int64_t hidden,
+                           const float* gate_up, const void* dy, int64_t ld_dy, void* dx, int64_t ld_dx,
+                           int accumulate_x, void* dw_gate, void* dw_up, int64_t ld_dw, int accumulate_w);
+
+/* One of many gradients: n contiguous elements of `type` (MIMIR_NUM_*) at `data`
+ * (aligned to their size), the clipped ones at `out`, which may be data. */
+typedef struct mimir_tensor {
+    const void* data;
+    void* out;
+    int64_t n;
+    int32_t type;
+} mimir_tensor;
+
+/* *norm (device) = sqrt of the sum of squares of all elements of `count` tensors (a
+ * HOST array, read within the call; up to 2^20), summed in 64 bits in an order that
+ * the list's sizes decide.  0 for no elements. */
+int mimir_grad_norm(mimir_ctx* ctx, const mimir_tensor* tensors, int64_t count, float* norm);
+
+/* out = data * min(1, max_norm / (norm + 1e-6)) of every tensor, norm as
+ * mimir_grad_norm's, written to *norm (device) unless NULL.  Where the factor is 1,
+ * tensors in place are left alone.  A NaN norm makes every element NaN, an infinite
+ * one finite elements 0.  max_norm >= 0.  No out may overlap another tensor.  The list
+ * is read within the call, so a captured call keeps the addresses.  Scratch: 16 KiB for
+ * each 96 tensors. */
+int mimir_grad_clip(mimir_ctx* ctx, const mimir_tensor* tensors, int64_t count, float max_norm, float* norm);
+
 /* ---------------------------------------------------------------------------
  * Device-resident runtime: a named tensor store and a layer runner with the
  * routing of the reference's Model::forwardPassNamed (Model.cpp:1352-1408,

@@ -248,14 +248,12 @@ struct Plan {
     int64_t ld, ld_g, piece;     // columns of x's and w's planes, of G's; the piece's rows of w
     int p, pg;                   // planes of x and w, of G
     bool w_direct;
-    int splits;                  // of dx's contraction
-    size_t x, row, count, logit, part, w, g, partial, total;
+    int splits_x, splits_w;      // of dx's contraction over a piece, of dw's over the tokens
+    size_t x, row, count, logit, part, w, g, partial, partial_w, total;
 };
 
 constexpr int64_t kPieceBytes = int64_t{512} << 20;
 constexpr int64_t kTileM = 128;  // the smaller shape's: how many partial results a token has at most
-
-int64_t tiles_of(int64_t m, int64_t n, int64_t bm, int64_t bn) { return (m + bm - 1) / bm * ((n + bn - 1) / bn); }
 
 // Few tokens: the products' time is the weights' bytes, and G takes a second plane.
 constexpr int64_t kTwoPlaneTokens = 128;
@@ -283,11 +281,14 @@ Plan plan_of(const Tuning& tune, int type, const void* w, int64_t ld_w, int64_t 
     p.w = take(p.w_direct ? 0 : static_cast<size_t>(p.p * p.piece * p.ld * 2));
     if (back) {
         p.g = take(static_cast<size_t>(p.pg * tokens * p.ld_g * 2));
-        // Few tiles: the contraction over the piece is dealt to several workgroups.
-        const int64_t tiles = tiles_of(dim, tokens, 128, p.p == 3 ? 64 : 128), steps = p.piece / 64;
-        p.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(512 / std::max<int64_t>(tiles, 1), steps / 8)));
-        const bool partial = p.splits > 1 || p.piece < vocab;
-        p.partial = take(partial ? static_cast<size_t>(p.splits * tokens * mat_round(dim, 4) * 4) : 0);
+        const auto splits = [&](int64_t m, int64_t n, int64_t k) {
+            return p.p == 3 ? mat_splits<MatSmall<3, 3, kCols, kRows>>(m, n, k, 1) : mat_splits<MatSmall<1, 1, kCols, kRows>>(m, n, k, 1);
+        };
+        const int64_t piece = std::min(p.piece, vocab), ld = mat_round(dim, 4);
+        p.splits_x = splits(dim, tokens, piece);
+        p.splits_w = splits(dim, piece, tokens);
+        p.partial = take(p.splits_x > 1 || p.piece < vocab ? static_cast<size_t>(p.splits_x * tokens * ld * 4) : 0);
+        p.partial_w = take(p.splits_w > 1 ? static_cast<size_t>(p.splits_w * piece * ld * 4) : 0);
     } else {
         p.logit = take(static_cast<size_t>(tokens * 4));
         p.part = take(static_cast<size_t>((vocab + kTileM - 1) / kTileM * tokens * 8));
@@ -414,7 +415,8 @@ int backward(mimir_ctx* ctx, const Call& c, const Plan& p, char* work, const Gra
     ox.vec = vec(d.dx, d.ld_dx);
     MatOut ow = ox;
     ow.row = nullptr;
-    ow.partial = nullptr;
+    ow.partial = reinterpret_cast<float*>(work + p.partial_w);
+    ow.slice = std::min(p.piece, c.vocab) * ow.ld_partial;
     ow.ld = d.ld_dw;
     ow.accumulate = d.accumulate_w;
     ow.last = 1;
@@ -435,17 +437,9 @@ int backward(mimir_ctx* ctx, const Call& c, const Plan& p, char* work, const Gra
         if (d.dx) {
             g = args_of(w, gr, c.dim, c.tokens, rows);
             g.n_dev = count;
-            g.splits = p.splits;
             ox.read_partial = first > 0;
-            ox.last = p.splits == 1 && first + rows >= c.vocab;
-            using SX = MatSmall<P, PG, kCols, kRows>;
-            if constexpr (P == PG) {
-                using BX = MatBig<P, PG, kCols, kRows>;
-                st = p.splits == 1 && mat_fills<BX>(ctx, g) ? mat_launch<BX>(ctx, "cross entropy dx", g, ox)
-                                                                    : mat_launch<SX>(ctx, "cross entropy dx", g, ox);
-            } else {
-                st = mat_launch<SX>(ctx, "cross entropy dx", g, ox);
-            }
+            ox.last = first + rows >= c.vocab;
+            st = mat_product<P, PG, kCols, kRows>(ctx, "cross entropy dx", g, ox, p.splits_x);
             if (st) return st;
         }
         if (d.dw) {
@@ -453,20 +447,11 @@ int backward(mimir_ctx* ctx, const Call& c, const Plan& p, char* work, const Gra
             if (c.tokens > 0) g.k_dev = count;
             ow.out[0] = static_cast<char*>(d.dw) + first * d.ld_dw * size;
             ow.vec = vec(ow.out[0], d.ld_dw);
-            using SW = MatSmall<P, PG, kCols, kCols>;
-            if constexpr (P == PG) {
-                using BW = MatBig<P, PG, kCols, kCols>;
-                st = mat_fills<BW>(ctx, g) ? mat_launch<BW>(ctx, "cross entropy dw", g, ow)
-                                                   : mat_launch<SW>(ctx, "cross entropy dw", g, ow);
-            } else {
-                st = mat_launch<SW>(ctx, "cross entropy dw", g, ow);
-            }
+            st = mat_product<P, PG, kCols, kCols>(ctx, "cross entropy dw", g, ow, p.splits_w);
             if (st) return st;
         }
     }
-    if (!d.dx || p.splits == 1) return MIMIR_OK;
-    ox.last = 1;
-    return mat_join(ctx, ox, c.tokens, c.dim, count, p.splits);
+    return MIMIR_OK;
 }
 
 }  // namespace

@@ -17,16 +17,16 @@ __global__ __launch_bounds__(kBlock) void stage_rows(const void* src, int64_t ro
     }
 }
 
-__global__ __launch_bounds__(kBlock) void join_slices(MatOut o, int64_t n, int64_t m, const int32_t* n_dev, int splits) {
-    if (n_dev) n = min(n, static_cast<int64_t>(*n_dev));
+__global__ __launch_bounds__(kBlock) void join_slices(MatOut o, MatArgs g) {
+    const int64_t n = g.n_dev ? min(g.n, *g.n_dev) : g.n;
     const float by = o.factor();
-    const int64_t of_row = (m + 3) / 4, total = n * of_row, stride = static_cast<int64_t>(gridDim.x) * kBlock;
-    for (int64_t i = static_cast<int64_t>(blockIdx.x) * kBlock + threadIdx.x; i < total; i += stride) {
-        const int64_t r = i / of_row, c = i % of_row * 4;
-        const float* p = o.partial + r * o.ld_partial + c;
+    const int64_t of_row = (g.m + 3) / 4, one = n * of_row, stride = static_cast<int64_t>(gridDim.x) * kBlock;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * kBlock + threadIdx.x; i < one * g.batches; i += stride) {
+        const int64_t batch = i / one, r = i % one / of_row, c = i % one % of_row * 4;
+        const float* p = o.partial + batch * o.slice + r * o.ld_partial + c;
         f4 v{};
-        for (int s = 0; s < splits; ++s) v += *reinterpret_cast<const f4*>(p + s * o.slice);
-        o.put(0, r, static_cast<int32_t>(c), static_cast<int32_t>(m), v, by);
+        for (int s = 0; s < g.splits; ++s) v += *reinterpret_cast<const f4*>(p + s * g.batches * o.slice);
+        o.put(static_cast<int>(batch), r, static_cast<int32_t>(c), g.m, v, by);
     }
 }
 
@@ -51,9 +51,9 @@ int mimir::mat_stage(mimir_ctx* ctx, int type, const void* src, int64_t rows, in
     return launched(ctx, "stage_rows");
 }
 
-int mimir::mat_join(mimir_ctx* ctx, const MatOut& o, int64_t n, int64_t m, const int32_t* n_dev, int splits) {
-    if (n == 0 || m == 0) return MIMIR_OK;
-    join_slices<<<grid_of(n * ((m + 3) / 4)), kBlock, 0, ctx->stream>>>(o, n, m, n_dev, splits);
+int mimir::mat_join(mimir_ctx* ctx, const MatOut& o, const MatArgs& g) {
+    if (g.n == 0 || g.m == 0) return MIMIR_OK;
+    join_slices<<<grid_of(static_cast<int64_t>(g.n) * ((g.m + 3) / 4) * g.batches), kBlock, 0, ctx->stream>>>(o, g);
     return launched(ctx, "join_slices");
 }
 

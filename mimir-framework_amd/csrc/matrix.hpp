@@ -33,6 +33,7 @@
 #include "internal.hpp"
 #include "split.hpp"
 
+#include <algorithm>
 #include <type_traits>
 
 namespace mimir {
@@ -58,6 +59,7 @@ struct MatArgs {
 struct MatAt {
     int32_t m0, n0, m, n;  // the tile's first, and the limits
     int32_t batch, split, tile_m;
+    int32_t slice;  // split * batches + batch
 };
 
 // Every workgroup runs it once; a workgroup of 64 * WGM * WGN threads.
@@ -200,6 +202,7 @@ __device__ __forceinline__ bool mat_tile_of(const MatArgs& g, MatAt* at) {
     const uint32_t r = i % one, z = i / one;
     at->batch = z % g.batches;
     at->split = z / g.batches;
+    at->slice = z;
     const uint32_t group = r / (kMatGroup * tiles_m), first = group * kMatGroup, wide = min(tiles_n - first, uint32_t{kMatGroup});
     const uint32_t in = r - group * kMatGroup * tiles_m;
     at->tile_m = in / wide;
@@ -342,13 +345,13 @@ int mat_launch(mimir_ctx* ctx, const char* what, const MatArgs& g, const Epi& ep
 // --- C as a result -----------------------------------------------------------------
 
 // out[row(n)][m] (+)= alpha * sum, sum over the pieces and splits of the contraction
-// that fp32 slices hold (`partial`, one for each split, row n at n * ld_partial).
+// that fp32 slices hold (`partial`, one for each split and batch, row n at n * ld_partial).
 // A lane has four m's of a row: one 16-byte (fp32) or 8-byte (bf16) store.
 struct MatOut {
     void* out[2];             // of each batch
     int64_t ld;
     const int32_t* row;       // not null: the row of n
-    float* partial;           // [splits][n][ld_partial], not null if read or written
+    float* partial;           // [splits][batches][n][ld_partial], not null if read or written
     int64_t ld_partial, slice;
     const float* count;       // not null: alpha is divided by max(count, 1)
     float alpha;
@@ -407,7 +410,7 @@ struct MatOut {
                     if (m >= at.m) continue;
                     f4 v{acc.c[i][j][4 * q], acc.c[i][j][4 * q + 1], acc.c[i][j][4 * q + 2], acc.c[i][j][4 * q + 3]};
                     // ld_partial is a multiple of four: a whole vector, past m too.
-                    f4* p = reinterpret_cast<f4*>(partial + at.split * slice + n * ld_partial + m);
+                    f4* p = reinterpret_cast<f4*>(partial + at.slice * slice + n * ld_partial + m);
                     if (read_partial) v += *p;
                     if (last) put(at.batch, n, m, at.m, v, by);
                     else *p = v;
@@ -463,8 +466,40 @@ __device__ __forceinline__ void mat_stage8(const void* src, int64_t at, int64_t 
 // between planes.
 int mat_stage(mimir_ctx* ctx, int type, const void* src, int64_t rows, int64_t cols, int64_t ld, uint16_t* dst, int64_t ld_dst,
               int64_t plane);
-// The sum of `splits` slices into out (MatOut's fields say how), n_dev as MatArgs'.
-int mat_join(mimir_ctx* ctx, const MatOut& o, int64_t n, int64_t m, const int32_t* n_dev, int splits);
+// The sum of the splits' slices into out (MatOut's fields say how) for a product of g.
+int mat_join(mimir_ctx* ctx, const MatOut& o, const MatArgs& g);
+
+// How many workgroups a contraction of `k` is dealt to where the tiles of C alone
+// leave CUs idle: about two for each CU, at least four steps each.
+template <class SMALL>
+int mat_splits(int64_t m, int64_t n, int64_t k, int64_t batches) {
+    const int64_t tiles = (m + SMALL::kM - 1) / SMALL::kM * ((n + SMALL::kN - 1) / SMALL::kN) * batches;
+    const int64_t steps = (k + SMALL::kK - 1) / SMALL::kK;
+    const int64_t s = std::min(512 / std::max<int64_t>(tiles, 1), steps / 4);
+    return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(s, 64)));
+}
+
+// C as a result, in the shape that fits, split `splits` ways.  o.last: these are the
+// contraction's last pieces.  PA, PB: planes.
+template <int PA, int PB, int KA, int KB>
+int mat_product(mimir_ctx* ctx, const char* what, MatArgs g, MatOut o, int splits) {
+    g.splits = splits;
+    const int32_t last = o.last;
+    if (splits > 1) o.last = 0;
+    int st = MIMIR_OK;
+    bool done = false;
+    if constexpr (PA == PB) {
+        using B = MatBig<PA, PB, KA, KB>;
+        if (splits == 1 && mat_fills<B>(ctx, g)) {
+            st = mat_launch<B>(ctx, what, g, o);
+            done = true;
+        }
+    }
+    if (!done) st = mat_launch<MatSmall<PA, PB, KA, KB>>(ctx, what, g, o);
+    if (st || splits == 1 || !last) return st;
+    o.last = 1;
+    return mat_join(ctx, o, g);
+}
 
 // The context's scratch of at least `bytes`, also while its stream is being captured:
 // then the old one, which the graph or one before it may hold, is kept as long as the

@@ -34,6 +34,8 @@ KV_TYPES = ("f32", "bf16", "i8")
 ROPE_SCALINGS = ("none", "linear", "base", "by_parts")
 # MIMIR_NUM_* (element types of the training calls' matrices), in order.
 NUM_TYPES = ("f32", "bf16")
+# MIMIR_ACT_*, in order.
+ACTIVATIONS = ("silu", "gelu")
 MERGE_OPS = ("ADD", "MULTIPLY", "CONCATENATE", "MAX", "AVERAGE", "GATED", "ATTENTION_WEIGHTED")
 
 
@@ -97,6 +99,11 @@ class KVBatch_C(Structure):
     """struct mimir_kv_batch."""
     _fields_ = [("sequences", c_int64), ("tokens", c_int64), ("token_start", c_void_p), ("kv_len", c_void_p),
                 ("page_table", c_void_p), ("ld_pages", c_int64), ("max_new", c_int64), ("max_len", c_int64)]
+
+
+class Tensor_C(Structure):
+    """struct mimir_tensor."""
+    _fields_ = [("data", c_void_p), ("out", c_void_p), ("n", c_int64), ("type", c_int32)]
 
 
 # name -> (restype, argtypes); mirrors include/mimir_hip.h one to one.
@@ -167,6 +174,11 @@ SIGNATURES = {
     "mimir_linear_cross_entropy_fwd": (c_int, [_P, c_int, _P, c_int64, _P, c_int64, _P, c_int64, c_int64, c_int64, _P, _P, _P]),
     "mimir_linear_cross_entropy_bwd": (c_int, [_P, c_int, _P, c_int64, _P, c_int64, _P, c_int64, c_int64, c_int64, _P, _P, _P,
                                                c_float, _P, c_int64, c_int, _P, c_int64, c_int]),
+    "mimir_gated_linear_fwd": (c_int, [_P, c_int, c_int, _P, c_int64, _P, _P, c_int64, c_int64, c_int64, c_int64, _P, c_int64, _P]),
+    "mimir_gated_linear_bwd": (c_int, [_P, c_int, c_int, _P, c_int64, _P, _P, c_int64, c_int64, c_int64, c_int64, _P, _P, c_int64,
+                                       _P, c_int64, c_int, _P, _P, c_int64, c_int]),
+    "mimir_grad_norm": (c_int, [_P, POINTER(Tensor_C), c_int64, _P]),
+    "mimir_grad_clip": (c_int, [_P, POINTER(Tensor_C), c_int64, c_float, _P]),
     "mimir_store_create": (c_int, [_P, _PP]),
     "mimir_store_destroy": (c_int, [_P]),
     "mimir_store_clear": (c_int, [_P]),

@@ -85,6 +85,13 @@ def _num(dtype):
     return _lib.NUM_TYPES.index(dtype)
 
 
+def _act(name):
+    """MIMIR_ACT_* of "silu" or "gelu"."""
+    if name not in _lib.ACTIVATIONS:
+        raise ValueError(f"activation {name!r}: one of {_lib.ACTIVATIONS}")
+    return _lib.ACTIVATIONS.index(name)
+
+
 class Context:
     """One HIP device + stream (``mimir_ctx``)."""
 
@@ -350,6 +357,46 @@ class Context:
             self.handle, _num(dtype), _ptr(x), ld_x or dim, _ptr(w), ld_w or dim, _ptr(targets), tokens, dim, vocab, _ptr(lse),
             _ptr(dloss), _ptr(mean), float(scale), _ptr(dx), ld_dx or dim, int(bool(accumulate_x)), _ptr(dw), ld_dw or dim,
             int(bool(accumulate_w))))
+
+    def gated_linear(self, x, w_gate, w_up, y, tokens, dim, hidden, act="silu", gate_up=None, dtype="f32", ld_x=None, ld_w=None,
+                     ld_y=None):
+        """mimir_gated_linear_fwd: y = act(x w_gate) * (x w_up); gate_up, if given,
+        keeps both products for gated_linear_bwd."""
+        self.check(self.lib.mimir_gated_linear_fwd(self.handle, _num(dtype), _act(act), _ptr(x), ld_x or dim, _ptr(w_gate),
+                                                   _ptr(w_up), ld_w or hidden, tokens, dim, hidden, _ptr(y), ld_y or hidden,
+                                                   _ptr(gate_up)))
+
+    def gated_linear_bwd(self, x, w_gate, w_up, gate_up, dy, dx, dw_gate, dw_up, tokens, dim, hidden, act="silu", dtype="f32",
+                         ld_x=None, ld_w=None, ld_dy=None, ld_dx=None, ld_dw=None, accumulate_x=False, accumulate_w=False):
+        """mimir_gated_linear_bwd: dx, dw_gate and dw_up (dx, or the latter two, may be None)."""
+        self.check(self.lib.mimir_gated_linear_bwd(
+            self.handle, _num(dtype), _act(act), _ptr(x), ld_x or dim, _ptr(w_gate), _ptr(w_up), ld_w or hidden, tokens, dim,
+            hidden, _ptr(gate_up), _ptr(dy), ld_dy or hidden, _ptr(dx), ld_dx or dim, int(bool(accumulate_x)), _ptr(dw_gate),
+            _ptr(dw_up), ld_dw or hidden, int(bool(accumulate_w))))
+
+    def grad_norm(self, tensors: "TensorList", norm):
+        """mimir_grad_norm: the 2-norm of all tensors' elements, to one device float."""
+        self.check(self.lib.mimir_grad_norm(self.handle, tensors.c, len(tensors), _ptr(norm)))
+
+    def grad_clip(self, tensors: "TensorList", max_norm, norm=None):
+        """mimir_grad_clip: every tensor times min(1, max_norm / (norm + 1e-6))."""
+        self.check(self.lib.mimir_grad_clip(self.handle, tensors.c, len(tensors), float(max_norm), _ptr(norm)))
+
+
+class TensorList:
+    """Gradients to be measured or clipped together (an array of ``mimir_tensor``):
+    (data, elements, "f32" or "bf16"[, out]) each; out defaults to data, in place."""
+
+    def __init__(self, tensors):
+        tensors = list(tensors)
+        self.c = (_lib.Tensor_C * max(1, len(tensors)))()
+        self.count = len(tensors)
+        for c, (data, n, dtype, *out) in zip(self.c, tensors):
+            c.data, c.n, c.type = _ptr(data), int(n), _num(dtype)
+            c.out = _ptr(out[0]) if out else c.data
+
+    def __len__(self):
+        return self.count
 
 
 class Event:

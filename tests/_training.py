@@ -103,3 +103,57 @@ def near(got, want, bound, what=""):
     if err.size and over.max() > 0:
         at = np.unravel_index(np.argmax(over), over.shape)
         raise AssertionError(f"{what}: {err[at]:.3g} off {want[at]:.6g} at {at}, bound {bound[at]:.3g}; {(over > 0).sum()} of {over.size} over")
+
+
+# --- gated products ----------------------------------------------------------
+
+def activation64(name, x):
+    """(act, act', the logistic's argument) in float64."""
+    if name == "silu":
+        v, dv = x, np.ones_like(x)
+    else:
+        k = 2 * np.sqrt(2 / np.pi)
+        v, dv = k * (x + 0.044715 * x ** 3), k * (1 + 3 * 0.044715 * x ** 2)
+    with np.errstate(over="ignore"):
+        s = 1 / (1 + np.exp(-v))
+        one_s = 1 / (1 + np.exp(v))
+    return x * s, s + x * s * one_s * dv, v
+
+
+def gated64(x, wg, wu, act, dtype):
+    """{y, bound, gate, up and what their products may be off by}."""
+    x, wg, wu = (np.asarray(a, np.float64) for a in (x, wg, wu))
+    gate, up = x @ wg, x @ wu
+    eg, eu = (np.abs(x) @ np.abs(w) * steps(x.shape[1]) * U for w in (wg, wu))
+    a, slope, v = activation64(act, gate)
+    # act' is at most 1.13 and act'' 1.6 of either form; the exponential's argument rounds a few times (6 U |v|), the
+    # function, the reciprocal and the products a few more.
+    ea = 1.2 * eg + np.abs(a) * (10 + 6 * np.abs(v)) * U
+    half = UB if dtype == "bf16" else U
+    y = a * up
+    ey = ea * np.abs(up) + (np.abs(a) + ea) * eu + 2 * U * np.abs(y) + 1.01 * half * np.abs(y) + 2.0 ** -126
+    s = np.abs(slope) + np.abs(slope - a / np.where(gate == 0, 1, gate))
+    es = 1.7 * eg + s * (12 + 6 * np.abs(v)) * U
+    return dict(y=y, ey=ey, gate=gate, up=up, eg=eg, eu=eu, a=a, ea=ea, slope=slope, es=es)
+
+
+def gated_bwd64(x, wg, wu, dy, c, dtype):
+    """{name: (value, bound)} of dx, dwg, dwu from gated64's c."""
+    x, wg, wu, dy = (np.asarray(a, np.float64) for a in (x, wg, wu, dy))
+    n, d = x.shape
+    du, dg = dy * c["a"], dy * c["up"] * c["slope"]
+    edu = np.abs(dy) * c["ea"] + 2 * U * np.abs(du)
+    edg = np.abs(dy) * (c["eu"] * (np.abs(c["slope"]) + c["es"]) + np.abs(c["up"]) * c["es"]) + 3 * U * np.abs(dg)
+    if dtype == "bf16":
+        r = 1.01 * (UB * UB if n <= 128 else UB)
+        edu, edg = edu + r * np.abs(du), edg + r * np.abs(dg)
+    half = UB if dtype == "bf16" else U
+    adu, adg = np.abs(du) + edu, np.abs(dg) + edg
+    out = {}
+    k = steps(2 * wg.shape[1]) + 70
+    dx = dg @ wg.T + du @ wu.T
+    out["dx"] = dx, 1.05 * (edg @ np.abs(wg).T + edu @ np.abs(wu).T + (adg @ np.abs(wg).T + adu @ np.abs(wu).T) * k * U + 1.01 * half * np.abs(dx)) + 2.0 ** -120
+    for name, g, e, a in (("dwg", dg, edg, adg), ("dwu", du, edu, adu)):
+        w = x.T @ g
+        out[name] = w, 1.05 * (np.abs(x).T @ e + np.abs(x).T @ a * (steps(n) + 70) * U + 1.01 * half * np.abs(w)) + 2.0 ** -120
+    return out

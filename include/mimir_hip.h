@@ -604,7 +604,7 @@ int mimir_linear_cross_entropy_bwd(mimir_ctx* ctx, int type, const void* x, int6
  * (row stride ld_x), Wg and Wu [dim][hidden] (both ld_w; input by output, as the
  * attention layers' weights), y [tokens][hidden] (ld_y), all of `type`; y is rounded
  * once.  Exactness and magnitudes as mimir_linear_cross_entropy_fwd's.  gate_up
- * [tokens][2 * hidden], fp32, 16-byte aligned, gets x Wg then x Wu of each token for
+ * [tokens][2 * hidden], fp32, gets x Wg then x Wu of each token for
  * the backward (NULL: they are not written).  tokens up to 2^24, dim to 2^18, hidden to
  * 2^20.  y must not overlap the inputs.  Scratch (the context's): fp32, or rows that
  * are no 16-byte multiples: x again and up to 512 MiB of the weights' columns. */

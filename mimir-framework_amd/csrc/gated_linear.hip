@@ -74,9 +74,9 @@ struct GatedOut {
                     y.put(0, n, m, at.m, v, 1.0f);
                     if (!gate_up) continue;
                     float* to = gate_up + n * 2 * hidden + m;
-                    if (hidden % 4 == 0) {
-                        *reinterpret_cast<f4*>(to) = g;
-                        *reinterpret_cast<f4*>(to + hidden) = u;
+                    if (m + 4 <= at.m) {
+                        *reinterpret_cast<f4u*>(to) = g;
+                        *reinterpret_cast<f4u*>(to + hidden) = u;
                     } else {
 #pragma unroll
                         for (int e = 0; e < 4; ++e)
@@ -99,7 +99,7 @@ struct GradArgs {
 };
 
 // Eight columns a thread; columns from `cols` on are zeros.
-template <int ACT, bool BF16, int PG, bool VEC>
+template <int ACT, bool BF16, int PG>
 __global__ __launch_bounds__(kBlock) void gated_grad(GradArgs a) {
     const int64_t of_row = a.cols_out / 8, total = a.tokens * of_row, stride = static_cast<int64_t>(gridDim.x) * kBlock;
     for (int64_t i = static_cast<int64_t>(blockIdx.x) * kBlock + threadIdx.x; i < total; i += stride) {
@@ -107,22 +107,23 @@ __global__ __launch_bounds__(kBlock) void gated_grad(GradArgs a) {
         const float* gp = a.gate_up + t * 2 * a.hidden + c;
         const float* up = gp + a.hidden;
         float g[8], u[8], d[8];
-        if (VEC && left >= 8) {
+        if (left >= 8) {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const f4 x = ld4<true>(gp + 4 * h), y = ld4<true>(up + 4 * h);
+                const f4u x = __builtin_nontemporal_load(reinterpret_cast<const f4u*>(gp + 4 * h));
+                const f4u y = __builtin_nontemporal_load(reinterpret_cast<const f4u*>(up + 4 * h));
 #pragma unroll
                 for (int e = 0; e < 4; ++e) g[4 * h + e] = x[e], u[4 * h + e] = y[e];
             }
             if constexpr (BF16) {
-                const u4 x = *reinterpret_cast<const u4*>(static_cast<const uint16_t*>(a.dy) + t * a.ld_dy + c);
+                const u4e x = *reinterpret_cast<const u4e*>(static_cast<const uint16_t*>(a.dy) + t * a.ld_dy + c);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) d[e] = __builtin_bit_cast(float, e % 2 ? x[e / 2] & 0xffff0000u : x[e / 2] << 16);
             } else {
                 const float* p = static_cast<const float*>(a.dy) + t * a.ld_dy + c;
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    const f4 x = ld4<true>(p + 4 * h);
+                    const f4u x = __builtin_nontemporal_load(reinterpret_cast<const f4u*>(p + 4 * h));
 #pragma unroll
                     for (int e = 0; e < 4; ++e) d[4 * h + e] = x[e];
                 }
@@ -261,8 +262,6 @@ MatArgs args_of(int64_t m, int64_t n, int64_t k) {
     return g;
 }
 
-bool vec4(const void* p, int64_t ld, int bf16) { return ld % 4 == 0 && reinterpret_cast<uintptr_t>(p) % (bf16 ? 8 : 16) == 0; }
-
 template <int P, int ACT>
 int forward(mimir_ctx* ctx, const Call& c, const Plan& p, char* work, void* y, int64_t ld_y, float* gate_up) {
     MatOperand x;
@@ -277,7 +276,6 @@ int forward(mimir_ctx* ctx, const Call& c, const Plan& p, char* work, void* y, i
         e.y.out[0] = static_cast<char*>(y) + first * (bf16 ? 2 : 4);
         e.y.ld = ld_y;
         e.y.bf16 = bf16;
-        e.y.vec = vec4(e.y.out[0], ld_y, bf16);
         e.gate_up = gate_up ? gate_up + first : nullptr;
         e.hidden = c.hidden;
         using B = MatBig<P, P, kCols, kRows, true>;
@@ -317,7 +315,6 @@ int backward(mimir_ctx* ctx, const Call& c, const Plan& p, char* work, const Gra
     ox.alpha = 1.0f;
     ox.bf16 = bf16;
     ox.accumulate = d.accumulate_x;
-    ox.vec = vec4(d.dx, d.ld_dx, bf16);
     MatOut ow = ox;
     ow.partial = reinterpret_cast<float*>(work + p.partial_w);
     ow.ld_partial = mat_round(std::min(p.piece, c.hidden), 4);
@@ -330,11 +327,9 @@ int backward(mimir_ctx* ctx, const Call& c, const Plan& p, char* work, const Gra
         const GradArgs a{d.gate_up ? d.gate_up + first : nullptr, c.hidden, static_cast<const char*>(d.dy) + first * size, d.ld_dy,
                          planes, c.tokens, cols, p.piece, plane};
         if (c.tokens > 0) {
-            const bool vec = c.hidden % 4 == 0 && d.ld_dy % 8 == 0 && aligned16(a.gate_up) && aligned16(a.dy);
             const int64_t blocks = (c.tokens * (p.piece / 8) + kBlock - 1) / kBlock;
             const auto grid = static_cast<unsigned>(std::min<int64_t>(blocks, 1 << 16));
-            if (vec) gated_grad<ACT, P == 1, PG, true><<<grid, kBlock, 0, ctx->stream>>>(a);
-            else gated_grad<ACT, P == 1, PG, false><<<grid, kBlock, 0, ctx->stream>>>(a);
+            gated_grad<ACT, P == 1, PG><<<grid, kBlock, 0, ctx->stream>>>(a);
             if (int st = launched(ctx, "gated_grad")) return st;
         }
         const MatOperand dg{planes, ld_g, plane}, du{planes + p.piece, ld_g, plane};
@@ -355,7 +350,6 @@ int backward(mimir_ctx* ctx, const Call& c, const Plan& p, char* work, const Gra
             g.b[0] = x;
             g.batches = 2;
             for (int i = 0; i < 2; ++i) ow.out[i] = static_cast<char*>(d.dw[i]) + first * size;
-            ow.vec = vec4(ow.out[0], d.ld_dw, bf16) && vec4(ow.out[1], d.ld_dw, bf16);
             if (int st = mat_product<PG, P, kCols, kCols>(ctx, "gated dw", g, ow, p.splits_w)) return st;
         }
     }
@@ -376,7 +370,6 @@ int mimir_gated_linear_fwd(mimir_ctx* ctx, int type, int act, const void* x, int
     if (tokens == 0) return MIMIR_OK;
     MIMIR_REQUIRE(ctx, x && w_gate && w_up && y, "%s: null pointer", what);
     MIMIR_REQUIRE(ctx, y != x, "%s: y must not be x", what);
-    MIMIR_REQUIRE(ctx, aligned16(gate_up), "%s: gate_up must be 16-byte aligned", what);
     MIMIR_ENTER(ctx);
     const Plan p = plan_of(ctx->tune, c, false);
     char* work;
@@ -399,7 +392,6 @@ int mimir_gated_linear_bwd(mimir_ctx* ctx, int type, int act, const void* x, int
                   (long long)ld_dx, (long long)ld_dw);
     if (!dx && !dw_gate) return MIMIR_OK;
     MIMIR_REQUIRE(ctx, tokens == 0 || (x && w_gate && w_up && gate_up && dy), "%s: null pointer", what);
-    MIMIR_REQUIRE(ctx, aligned16(gate_up), "%s: gate_up must be 16-byte aligned", what);
     MIMIR_REQUIRE(ctx, !dx || (dx != x && dx != dy && dx != w_gate && dx != w_up), "%s: dx must not be an input", what);
     MIMIR_REQUIRE(ctx, !dw_gate || (dw_gate != w_gate && dw_gate != w_up && dw_up != w_gate && dw_up != w_up && dw_gate != dw_up),
                   "%s: dw_gate and dw_up must be buffers of their own", what);

@@ -56,6 +56,22 @@ __device__ __forceinline__ float bf16_at(uint32_t pair, int high) {
     return __builtin_bit_cast(float, high ? pair & 0xffff0000u : pair << 16);
 }
 
+// f(element, vector) for the workgroup's vectors of `wide` elements of p[0, n): the N of
+// a whole chunk are loaded before the first is used.
+template <int N, class V, class T, class F>
+__device__ __forceinline__ void with_vectors(const T* p, int wide, int64_t n, F&& f) {
+    const int64_t first = wide * threadIdx.x, next = wide * kBlock;
+    if (n == kChunk) {
+        V v[N];
+#pragma unroll
+        for (int j = 0; j < N; ++j) v[j] = *reinterpret_cast<const V*>(p + first + j * next);
+#pragma unroll
+        for (int j = 0; j < N; ++j) f(first + j * next, v[j]);
+        return;
+    }
+    for (int64_t i = first; i < n; i += next) f(i, *reinterpret_cast<const V*>(p + i));
+}
+
 __device__ __forceinline__ double block_sum64(double v, double* lds) {
 #pragma unroll
     for (int d = 1; d < kWave; d *= 2) v += __shfl_xor(v, d);
@@ -80,22 +96,20 @@ __global__ __launch_bounds__(kBlock) void norm_sums(List l, double* sums) {
             const uint16_t* p = static_cast<const uint16_t*>(l.in[k.tensor]) + k.at;
             if (vec) {
                 done = k.n / 8 * 8;
-                for (int64_t i = 8 * threadIdx.x; i < done; i += 8 * kBlock) {
-                    const u4 v = *reinterpret_cast<const u4*>(p + i);
+                with_vectors<4, u4>(p, 8, done, [&](int64_t, u4 v) {
 #pragma unroll
                     for (int e = 0; e < 8; ++e) s[e % 4] += square(bf16_at(v[e / 2], e % 2));
-                }
+                });
             }
             for (int64_t i = done + threadIdx.x; i < k.n; i += kBlock) s[0] += square(bf16_at(p[i], 0));
         } else {
             const float* p = static_cast<const float*>(l.in[k.tensor]) + k.at;
             if (vec) {
                 done = k.n / 4 * 4;
-                for (int64_t i = 4 * threadIdx.x; i < done; i += 4 * kBlock) {
-                    const f4 v = *reinterpret_cast<const f4*>(p + i);
+                with_vectors<8, f4>(p, 4, done, [&](int64_t, f4 v) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) s[e] += square(v[e]);
-                }
+                });
             }
             for (int64_t i = done + threadIdx.x; i < k.n; i += kBlock) s[0] += square(p[i]);
         }
@@ -136,13 +150,12 @@ __global__ __launch_bounds__(kBlock) void clip(List l, const double* sums, int32
             uint16_t* q = static_cast<uint16_t*>(l.out[k.tensor]) + k.at;
             if (vec) {
                 done = k.n / 8 * 8;
-                for (int64_t i = 8 * threadIdx.x; i < done; i += 8 * kBlock) {
-                    const u4 v = *reinterpret_cast<const u4*>(p + i);
+                with_vectors<4, u4>(p, 8, done, [&](int64_t i, u4 v) {
                     u4 y;
 #pragma unroll
                     for (int e = 0; e < 4; ++e) y[e] = pack_bf16(bf16_at(v[e], 0) * by * after, bf16_at(v[e], 1) * by * after);
-                    *reinterpret_cast<u4*>(q + i) = y;
-                }
+                    st_stream(q + i, y);
+                });
             }
             for (int64_t i = done + threadIdx.x; i < k.n; i += kBlock) {
                 const float y = bf16_at(p[i], 0) * by * after;
@@ -153,8 +166,7 @@ __global__ __launch_bounds__(kBlock) void clip(List l, const double* sums, int32
             float* q = static_cast<float*>(l.out[k.tensor]) + k.at;
             if (vec) {
                 done = k.n / 4 * 4;
-                for (int64_t i = 4 * threadIdx.x; i < done; i += 4 * kBlock)
-                    *reinterpret_cast<f4*>(q + i) = *reinterpret_cast<const f4*>(p + i) * by * after;
+                with_vectors<8, f4>(p, 4, done, [&](int64_t i, f4 v) { st_stream(q + i, v * by * after); });
             }
             for (int64_t i = done + threadIdx.x; i < k.n; i += kBlock) q[i] = p[i] * by * after;
         }

@@ -47,28 +47,30 @@ struct GatherArgs {
     uint16_t* dst;       // planes of [tokens][ld_dst]
     int64_t ld_dst, plane;
     int32_t* row;        // [tokens]: the token of each gathered row
-    int32_t* count;
+    int32_t* count;      // and a counter for ce_finish, zeroed
     float* zero_a;       // of tokens without a target: loss and lse, or null
     float* zero_b;
     void* dx;            // their gradient's rows are zeroed, or null
     int64_t ld_dx;
 };
 
-constexpr int kGatherRows = 8;
+constexpr int kGatherRows = kBlock / kWave;
 
-// Eight tokens a workgroup, two rows a wave's turn.  How many rows before its own
-// count is found by reading the targets before them (a few KB, in L2).
-template <bool BF16, bool VEC>
+// Four tokens a workgroup, one a wave.  How many rows before its own count is found by
+// reading the targets before them (a few KB, in L2).
+template <bool BF16>
 __global__ __launch_bounds__(kBlock) void gather_rows(GatherArgs a) {
     __shared__ int before[kBlock / kWave];
     const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-    const int64_t t0 = static_cast<int64_t>(blockIdx.x) * kGatherRows;
-    const auto counts = [&](int64_t t) {
-        const int32_t v = a.target[t];
-        return v >= 0 && v < a.vocab;
-    };
+    const int64_t t0 = static_cast<int64_t>(blockIdx.x) * kGatherRows, t = t0 + wave;
+    const auto counts = [&](int64_t i) { return static_cast<uint32_t>(a.target[i]) < static_cast<uint32_t>(a.vocab); };
     int mine = 0;
-    for (int64_t t = threadIdx.x; t < t0; t += kBlock) mine += counts(t) ? 1 : 0;
+    for (int64_t i = threadIdx.x; i < t0; i += 4 * kBlock) {
+        bool is[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) is[e] = i + e * kBlock < t0 && counts(i + e * kBlock);
+        mine += is[0] + is[1] + is[2] + is[3];
+    }
 #pragma unroll
     for (int s = 1; s < kWave; s *= 2) mine += __shfl_xor(mine, s);
     if (lane == 0) before[wave] = mine;
@@ -76,28 +78,28 @@ __global__ __launch_bounds__(kBlock) void gather_rows(GatherArgs a) {
     int at = 0;
 #pragma unroll
     for (int w = 0; w < kBlock / kWave; ++w) at += before[w];
-
-    for (int i = 0; i < kGatherRows; ++i) {
-        const int64_t t = t0 + i;
-        if (t >= a.tokens) break;
-        const bool in = counts(t);
-        if (i % (kBlock / kWave) == wave) {
-            if (in) {
-                if (lane == 0) a.row[at] = static_cast<int32_t>(t);
-                for (int64_t c = 8 * lane; c < a.ld_dst; c += 8 * kWave)
-                    mat_stage8<BF16, VEC>(a.x, t * a.ld_x + c, a.dim - c, a.dst + at * a.ld_dst + c, a.plane);
-            } else {
-                if (lane == 0 && a.zero_a) a.zero_a[t] = 0.0f, a.zero_b[t] = 0.0f;
-                if (a.dx)
-                    for (int64_t c = lane; c < a.dim; c += kWave) {
-                        if (BF16) static_cast<uint16_t*>(a.dx)[t * a.ld_dx + c] = 0;
-                        else static_cast<float*>(a.dx)[t * a.ld_dx + c] = 0.0f;
-                    }
-            }
-        }
-        at += in ? 1 : 0;
+    const bool last = t0 + kGatherRows >= a.tokens;
+    if (last && threadIdx.x == 0) {
+        int all = at;
+        for (int64_t i = t0; i < a.tokens; ++i) all += counts(i) ? 1 : 0;
+        a.count[0] = all;
+        a.count[1] = 0;  // ce_finish's workgroups that are done
     }
-    if (t0 + kGatherRows >= a.tokens && threadIdx.x == 0) *a.count = at;
+    if (t >= a.tokens) return;
+    for (int64_t i = t0; i < t; ++i) at += counts(i) ? 1 : 0;
+    if (counts(t)) {
+        if (lane == 0) a.row[at] = static_cast<int32_t>(t);
+#pragma unroll 4
+        for (int64_t c = 8 * lane; c < a.ld_dst; c += 8 * kWave)
+            mat_stage8<BF16>(a.x, t * a.ld_x + c, a.dim - c, a.dst + at * a.ld_dst + c, a.plane);
+        return;
+    }
+    if (lane == 0 && a.zero_a) a.zero_a[t] = 0.0f, a.zero_b[t] = 0.0f;
+    if (!a.dx) return;
+    for (int64_t c = lane; c < a.dim; c += kWave) {
+        if (BF16) static_cast<uint16_t*>(a.dx)[t * a.ld_dx + c] = 0;
+        else static_cast<float*>(a.dx)[t * a.ld_dx + c] = 0.0f;
+    }
 }
 
 // --- forward -----------------------------------------------------------------------
@@ -159,39 +161,59 @@ struct CeStats {
 
 constexpr int kFinishTokens = 32;
 
-// 32 tokens a workgroup, eight threads a token over the tiles.
+// 32 tokens a workgroup, eight threads a token over the tiles.  The workgroup that is
+// done last adds up all of them for the mean, in a fixed order and 64 bits.
 __global__ __launch_bounds__(kBlock) void ce_finish(const f2* part, int64_t tokens, int32_t tiles, const float* logit,
-                                                    const int32_t* row, const int32_t* count, float* loss, float* lse) {
-    constexpr int kParts = kBlock / kFinishTokens;
+                                                    const int32_t* row, int32_t* count, float* loss, float* lse, double* sums,
+                                                    float* mean) {
+    constexpr int kParts = kBlock / kFinishTokens, kTogether = 4;
     __shared__ f2 red[kParts][kFinishTokens];
+    __shared__ double wave_sums[kBlock / kWave];
+    __shared__ bool last;
     const int t = threadIdx.x % kFinishTokens, p = threadIdx.x / kFinishTokens;
     const int64_t n = static_cast<int64_t>(blockIdx.x) * kFinishTokens + t;
     const bool in = n < *count;
     f2 v{-__builtin_inff(), 0.0f};
     if (in)
-        for (int32_t i = p; i < tiles; i += kParts) v = join(v, part[i * tokens + n]);
+        for (int32_t i = p; i < tiles; i += kTogether * kParts) {
+            f2 x[kTogether];
+#pragma unroll
+            for (int e = 0; e < kTogether; ++e)
+                x[e] = i + e * kParts < tiles ? part[(i + e * kParts) * tokens + n] : f2{-__builtin_inff(), 0.0f};
+            v = join(v, join(join(x[0], x[1]), join(x[2], x[3])));
+        }
     red[p][t] = v;
     __syncthreads();
-    if (p || !in) return;
+    double sum = 0.0;
+    if (p == 0 && in) {
 #pragma unroll
-    for (int w = 1; w < kParts; ++w) v = join(v, red[w][t]);
-    const float l = v[0] + logf(v[1]);
-    loss[row[n]] = l - logit[n];
-    lse[row[n]] = l;
-}
-
-// {sum / max(count, 1), count}: one workgroup, sums in 64 bits in a fixed order.
-__global__ __launch_bounds__(1024) void ce_mean(const float* loss, int64_t tokens, const int32_t* count, float* mean) {
-    __shared__ double red[1024 / kWave];
-    double s = 0.0;
-    for (int64_t t = threadIdx.x; t < tokens; t += 1024) s += loss[t];
+        for (int w = 1; w < kParts; ++w) v = join(v, red[w][t]);
+        const float l = v[0] + logf(v[1]), own = l - logit[n];
+        loss[row[n]] = own;
+        lse[row[n]] = l;
+        sum = own;
+    }
+    if (!mean) return;
+    if (threadIdx.x < kWave) {
 #pragma unroll
-    for (int d = 1; d < kWave; d *= 2) s += __shfl_xor(s, d);
-    if (threadIdx.x % kWave == 0) red[threadIdx.x / kWave] = s;
+        for (int d = 1; d < kFinishTokens; d *= 2) sum += __shfl_xor(sum, d);
+        if (threadIdx.x == 0) {
+            __hip_atomic_store(sums + blockIdx.x, sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            last = __hip_atomic_fetch_add(count + 1, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == static_cast<int>(gridDim.x) - 1;
+        }
+    }
+    __syncthreads();
+    if (!last) return;
+    sum = 0.0;
+    for (uint32_t i = threadIdx.x; i < gridDim.x; i += kBlock)
+        sum += __hip_atomic_load(sums + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+#pragma unroll
+    for (int d = 1; d < kWave; d *= 2) sum += __shfl_xor(sum, d);
+    if (threadIdx.x % kWave == 0) wave_sums[threadIdx.x / kWave] = sum;
     __syncthreads();
     if (threadIdx.x) return;
-    for (int w = 1; w < 1024 / kWave; ++w) s += red[w];
-    mean[0] = static_cast<float>(s / (*count > 0 ? *count : 1));
+    for (int w = 1; w < kBlock / kWave; ++w) sum += wave_sums[w];
+    mean[0] = static_cast<float>(sum / (*count > 0 ? *count : 1));
     mean[1] = static_cast<float>(*count);
 }
 
@@ -249,7 +271,7 @@ struct Plan {
     int p, pg;                   // planes of x and w, of G
     bool w_direct;
     int splits_x, splits_w;      // of dx's contraction over a piece, of dw's over the tokens
-    size_t x, row, count, logit, part, w, g, partial, partial_w, total;
+    size_t x, row, count, logit, sums, part, w, g, partial, partial_w, total;
 };
 
 constexpr int64_t kPieceBytes = int64_t{512} << 20;
@@ -277,7 +299,7 @@ Plan plan_of(const Tuning& tune, int type, const void* w, int64_t ld_w, int64_t 
     };
     p.x = take(static_cast<size_t>(p.p * tokens * p.ld * 2));
     p.row = take(static_cast<size_t>(tokens * 4));
-    p.count = take(4);
+    p.count = take(8);
     p.w = take(p.w_direct ? 0 : static_cast<size_t>(p.p * p.piece * p.ld * 2));
     if (back) {
         p.g = take(static_cast<size_t>(p.pg * tokens * p.ld_g * 2));
@@ -291,6 +313,7 @@ Plan plan_of(const Tuning& tune, int type, const void* w, int64_t ld_w, int64_t 
         p.partial_w = take(p.splits_w > 1 ? static_cast<size_t>(p.splits_w * piece * ld * 4) : 0);
     } else {
         p.logit = take(static_cast<size_t>(tokens * 4));
+        p.sums = take(static_cast<size_t>((tokens + kFinishTokens - 1) / kFinishTokens * 8));
         p.part = take(static_cast<size_t>((vocab + kTileM - 1) / kTileM * tokens * 8));
     }
     p.total = at;
@@ -322,13 +345,11 @@ const char* rows_at(const Call& c, int64_t first) {
     return static_cast<const char*>(c.w) + first * c.ld_w * (c.type == MIMIR_NUM_BF16 ? 2 : 4);
 }
 
-template <bool BF16>
 int gather(mimir_ctx* ctx, const Call& c, const GatherArgs& a) {
-    const bool vec = aligned16(c.x) && c.ld_x % (BF16 ? 8 : 4) == 0;
     const auto grid = static_cast<unsigned>((c.tokens + kGatherRows - 1) / kGatherRows);
     if (grid == 0) return MIMIR_OK;
-    if (vec) gather_rows<BF16, true><<<grid, kBlock, 0, ctx->stream>>>(a);
-    else gather_rows<BF16, false><<<grid, kBlock, 0, ctx->stream>>>(a);
+    if (c.type == MIMIR_NUM_BF16) gather_rows<true><<<grid, kBlock, 0, ctx->stream>>>(a);
+    else gather_rows<false><<<grid, kBlock, 0, ctx->stream>>>(a);
     return launched(ctx, "gather_rows");
 }
 
@@ -355,7 +376,7 @@ MatArgs args_of(const MatOperand& a, const MatOperand& b, int64_t m, int64_t n, 
 }
 
 template <int P>
-int forward(mimir_ctx* ctx, const Call& c, const Plan& p, char* work, float* loss, float* lse) {
+int forward(mimir_ctx* ctx, const Call& c, const Plan& p, char* work, float* loss, float* lse, float* mean) {
     const MatOperand x{reinterpret_cast<const uint16_t*>(work + p.x), p.ld, c.tokens * p.ld};
     auto* row = reinterpret_cast<int32_t*>(work + p.row);
     auto* count = reinterpret_cast<int32_t*>(work + p.count);
@@ -375,7 +396,7 @@ int forward(mimir_ctx* ctx, const Call& c, const Plan& p, char* work, float* los
         e.tile0 += static_cast<int32_t>((rows + (big ? B::kM : S::kM) - 1) / (big ? B::kM : S::kM));
     }
     ce_finish<<<static_cast<unsigned>((c.tokens + kFinishTokens - 1) / kFinishTokens), kBlock, 0, ctx->stream>>>(
-        e.part, c.tokens, e.tile0, e.logit, row, count, loss, lse);
+        e.part, c.tokens, e.tile0, e.logit, row, count, loss, lse, reinterpret_cast<double*>(work + p.sums), mean);
     return launched(ctx, "ce_finish");
 }
 
@@ -400,7 +421,6 @@ int backward(mimir_ctx* ctx, const Call& c, const Plan& p, char* work, const Gra
     auto* count = reinterpret_cast<int32_t*>(work + p.count);
     const int bf16 = c.type == MIMIR_NUM_BF16;
     const int64_t size = bf16 ? 2 : 4;
-    const auto vec = [&](const void* q, int64_t ld) { return ld % 4 == 0 && reinterpret_cast<uintptr_t>(q) % (4 * size) == 0; };
     MatOut ox{};
     ox.out[0] = d.dx;
     ox.ld = d.ld_dx;
@@ -412,7 +432,6 @@ int backward(mimir_ctx* ctx, const Call& c, const Plan& p, char* work, const Gra
     ox.alpha = d.scale;
     ox.bf16 = bf16;
     ox.accumulate = d.accumulate_x;
-    ox.vec = vec(d.dx, d.ld_dx);
     MatOut ow = ox;
     ow.row = nullptr;
     ow.partial = reinterpret_cast<float*>(work + p.partial_w);
@@ -446,7 +465,6 @@ int backward(mimir_ctx* ctx, const Call& c, const Plan& p, char* work, const Gra
             g = args_of(x, gr, c.dim, rows, c.tokens);
             if (c.tokens > 0) g.k_dev = count;
             ow.out[0] = static_cast<char*>(d.dw) + first * d.ld_dw * size;
-            ow.vec = vec(ow.out[0], d.ld_dw);
             st = mat_product<P, PG, kCols, kCols>(ctx, "cross entropy dw", g, ow, p.splits_w);
             if (st) return st;
         }
@@ -472,16 +490,11 @@ int mimir_linear_cross_entropy_fwd(mimir_ctx* ctx, int type, const void* x, int6
     char* work;
     if (int st = mat_scratch(ctx, p.total, &work)) return st;
     auto* count = reinterpret_cast<int32_t*>(work + p.count);
-    if (tokens > 0) {
-        const GatherArgs a{x, ld_x, targets, tokens, dim, vocab, reinterpret_cast<uint16_t*>(work + p.x), p.ld, tokens * p.ld,
-                           reinterpret_cast<int32_t*>(work + p.row), count, loss, lse, nullptr, 0};
-        int st = type == MIMIR_NUM_BF16 ? gather<true>(ctx, c, a) : gather<false>(ctx, c, a);
-        if (!st) st = p.p == 1 ? forward<1>(ctx, c, p, work, loss, lse) : forward<3>(ctx, c, p, work, loss, lse);
-        if (st || !mean) return st;
-        ce_mean<<<1, 1024, 0, ctx->stream>>>(loss, tokens, count, mean);
-        return launched(ctx, "ce_mean");
-    }
-    return mimir_fill_f32(ctx, mean, 2, 0.0f);
+    if (tokens == 0) return mimir_fill_f32(ctx, mean, 2, 0.0f);
+    const GatherArgs a{x, ld_x, targets, tokens, dim, vocab, reinterpret_cast<uint16_t*>(work + p.x), p.ld, tokens * p.ld,
+                       reinterpret_cast<int32_t*>(work + p.row), count, loss, lse, nullptr, 0};
+    if (int st = gather(ctx, c, a)) return st;
+    return p.p == 1 ? forward<1>(ctx, c, p, work, loss, lse, mean) : forward<3>(ctx, c, p, work, loss, lse, mean);
 }
 
 int mimir_linear_cross_entropy_bwd(mimir_ctx* ctx, int type, const void* x, int64_t ld_x, const void* w, int64_t ld_w,
@@ -506,7 +519,7 @@ int mimir_linear_cross_entropy_bwd(mimir_ctx* ctx, int type, const void* x, int6
     const Gradients d{lse, dloss, mean, scale, dx, ld_dx, dw, ld_dw, accumulate_x ? 1 : 0, accumulate_w ? 1 : 0};
     const GatherArgs a{x, ld_x, targets, tokens, dim, vocab, reinterpret_cast<uint16_t*>(work + p.x), p.ld, tokens * p.ld,
                        reinterpret_cast<int32_t*>(work + p.row), count, nullptr, nullptr, accumulate_x ? nullptr : dx, ld_dx};
-    if (int st = type == MIMIR_NUM_BF16 ? gather<true>(ctx, c, a) : gather<false>(ctx, c, a)) return st;
+    if (int st = gather(ctx, c, a)) return st;
     if (p.p == 3) return backward<3, 3>(ctx, c, p, work, d);
     return p.pg == 2 ? backward<1, 2>(ctx, c, p, work, d) : backward<1, 1>(ctx, c, p, work, d);
 }

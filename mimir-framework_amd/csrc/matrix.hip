@@ -7,13 +7,13 @@ using namespace mimir;
 namespace {
 
 // Eight columns a thread: 32 bytes of fp32 read, 16 written to each of three planes.
-template <bool BF16, bool VEC>
+template <bool BF16>
 __global__ __launch_bounds__(kBlock) void stage_rows(const void* src, int64_t rows, int64_t cols, int64_t ld, uint16_t* dst,
                                                       int64_t ld_dst, int64_t plane) {
     const int64_t of_row = ld_dst / 8, total = rows * of_row, stride = static_cast<int64_t>(gridDim.x) * kBlock;
     for (int64_t i = static_cast<int64_t>(blockIdx.x) * kBlock + threadIdx.x; i < total; i += stride) {
         const int64_t r = i / of_row, c = i % of_row * 8;
-        mat_stage8<BF16, VEC>(src, r * ld + c, cols - c, dst + r * ld_dst + c, plane);
+        mat_stage8<BF16>(src, r * ld + c, cols - c, dst + r * ld_dst + c, plane);
     }
 }
 
@@ -41,13 +41,8 @@ int mimir::mat_stage(mimir_ctx* ctx, int type, const void* src, int64_t rows, in
                      int64_t ld_dst, int64_t plane) {
     const unsigned grid = grid_of(rows * (ld_dst / 8));
     if (rows == 0) return MIMIR_OK;
-    if (type == MIMIR_NUM_BF16) {
-        if (aligned16(src) && ld % 8 == 0) stage_rows<true, true><<<grid, kBlock, 0, ctx->stream>>>(src, rows, cols, ld, dst, ld_dst, plane);
-        else stage_rows<true, false><<<grid, kBlock, 0, ctx->stream>>>(src, rows, cols, ld, dst, ld_dst, plane);
-    } else {
-        if (aligned16(src) && ld % 4 == 0) stage_rows<false, true><<<grid, kBlock, 0, ctx->stream>>>(src, rows, cols, ld, dst, ld_dst, plane);
-        else stage_rows<false, false><<<grid, kBlock, 0, ctx->stream>>>(src, rows, cols, ld, dst, ld_dst, plane);
-    }
+    if (type == MIMIR_NUM_BF16) stage_rows<true><<<grid, kBlock, 0, ctx->stream>>>(src, rows, cols, ld, dst, ld_dst, plane);
+    else stage_rows<false><<<grid, kBlock, 0, ctx->stream>>>(src, rows, cols, ld, dst, ld_dst, plane);
     return launched(ctx, "stage_rows");
 }
 

@@ -63,16 +63,17 @@ struct MatAt {
 };
 
 // Every workgroup runs it once; a workgroup of 64 * WGM * WGN threads.
-template <int BM, int BN, int WGM, int WGN, int BK, int PA, int PB, int KA, int KB, bool DUAL = false>
+template <int BM, int BN, int WGM, int WGN, int BK, int STAGES, int PA, int PB, int KA, int KB, bool DUAL = false>
 struct MatShape {
     static constexpr int kM = BM, kN = BN, kWaveM = WGM, kWaveN = WGN, kK = BK, kPa = PA, kPb = PB, kKindA = KA, kKindB = KB;
     static constexpr bool kDual = DUAL;
+    static constexpr int kStages = STAGES;
     static constexpr int kWaves = WGM * WGN, kThreads = kWave * kWaves;
     static constexpr int kBm = BM / WGM / 32, kBn = BN / WGN / 32;  // 32 x 32 blocks of a wave
     static constexpr int kSubs = DUAL ? 2 : 1, kSubRows = BM / kSubs, kSubBlocks = kBm / kSubs;
     static constexpr int kPlaneA = BM * BK * 2, kPlaneB = BN * BK * 2;  // bytes
     static constexpr int kStage = PA * kPlaneA + PB * kPlaneB;
-    static constexpr int kLds = 2 * kStage;
+    static constexpr int kLds = STAGES * kStage;
     static_assert(kLds <= 160 * 1024 && kBm % kSubs == 0 && BK % 16 == 0);
 };
 
@@ -80,9 +81,9 @@ struct MatShape {
 
 template <int R, int BK, int KIND>
 __device__ __forceinline__ constexpr int mat_swizzle(int i) {
-    // kRows, of row i: rows of 128 bytes use eight places, rows of 64 bytes four for
-    // two rows.  kCols, of k i: four k's 64 bytes (32 values) in different banks.
-    if (KIND == kRows) return BK == 64 ? i & 7 : (i >> 1) & 3;
+    // kRows, of row i: 16 rows' same chunk in the 16 places of the 64 banks.  kCols, of k
+    // i: four k's 64 bytes (32 values) in different banks.
+    if (KIND == kRows) return BK == 64 ? (i >> 1) & 7 : (i >> 2) & 3;
     return R == 64 ? 4 * ((i >> 1) & 1) : 4 * (i & 3);
 }
 
@@ -96,7 +97,12 @@ __device__ __forceinline__ void load_to_lds(uint32_t lds, uint32_t voff, __amdgp
                  : "s"(lds), "v"(voff), "s"(rs), "s"(soff)
                  : "memory");
 }
-__device__ __forceinline__ void mat_landed() { asm volatile("s_waitcnt vmcnt(0)" : : : "memory"); }
+// All but the last N of the wave's loads are there.
+template <int N>
+__device__ __forceinline__ void mat_landed() {
+    static_assert(N < 64);
+    asm volatile("s_waitcnt vmcnt(%0)" : : "n"(N) : "memory");
+}
 
 template <int R, int BK, int P, int KIND, int WAVES>
 struct MatTile {
@@ -114,7 +120,8 @@ struct MatTile {
         const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
         const int r = lane / kLanes, slot = lane % kLanes;
         if constexpr (KIND == kRows) {
-            const int chunk = slot ^ mat_swizzle<R, BK, KIND>(r);  // a kilobyte's rows are a multiple of the swizzle's
+            // Loads are WAVES * kRowsOf rows apart, a multiple of the swizzle's 16.
+            const int chunk = slot ^ mat_swizzle<R, BK, KIND>(wave * kRowsOf + r);
             k_mine = 8 * chunk;
 #pragma unroll
             for (int j = 0; j < kLoads; ++j) {
@@ -128,30 +135,46 @@ struct MatTile {
         }
     }
     static_assert(KIND == kRows || (WAVES * kRowsOf) % 4 == 0 || kLoads == 1);
-    static_assert(KIND == kCols || kRowsOf % 8 == 0);
+    static_assert(KIND == kCols || (WAVES * kRowsOf) % 16 == 0);
 
-    // k0 .. k0 + BK of the contraction, `left` of them inside it.  base: the tile's first row.
-    __device__ __forceinline__ void load(uint32_t lds, const MatOperand& o, const uint16_t* base, int32_t k0, int32_t left) const {
-        const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    // A step from `at` (bytes; the tile's first row, the step's first k) on, `left` of its
+    // k inside the contraction, for wave `wave` (uniform).
+    __device__ __forceinline__ void load(uint32_t lds, uint64_t at, int64_t plane, uint32_t next, int32_t left, uint32_t wave) const {
+        constexpr int kNext = WAVES * kRowsOf;  // kCols: k's from one load to the next, `next` bytes
 #pragma unroll
         for (int p = 0; p < P; ++p) {
-            const uint16_t* at = base + p * o.plane + (KIND == kRows ? k0 : k0 * o.ld);
-            const __amdgpu_buffer_rsrc_t rs =
-                __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(at), 0, 0x7fffffff, kBufferWord3);
+            const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
+                reinterpret_cast<void*>(at + p * plane), 0, 0x7fffffff, kBufferWord3);
+            const uint32_t to = lds + p * kBytes + wave * 1024;
+            if (left >= BK) {
 #pragma unroll
-            for (int j = 0; j < kLoads; ++j) {
-                const uint32_t to = lds + p * kBytes + (j * WAVES + wave) * 1024;
-                if constexpr (KIND == kRows) {
-                    load_to_lds(to, left >= BK || k_mine < left ? off[j] : kOutside, rs, 0);
-                } else {
-                    constexpr int kNext = WAVES * kRowsOf;
-                    load_to_lds(to, left >= BK || k_mine + j * kNext < left ? off[0] : kOutside, rs,
-                                static_cast<uint32_t>(j * kNext * o.ld * 2));
-                }
+                for (int j = 0; j < kLoads; ++j)
+                    load_to_lds(to + j * WAVES * 1024, off[KIND == kRows ? j : 0], rs, KIND == kRows ? 0 : j * next);
+            } else {
+#pragma unroll
+                for (int j = 0; j < kLoads; ++j)
+                    load_to_lds(to + j * WAVES * 1024,
+                                k_mine + (KIND == kRows ? 0 : j * kNext) < left ? off[KIND == kRows ? j : 0] : kOutside, rs,
+                                KIND == kRows ? 0 : j * next);
             }
         }
     }
+    // Bytes from one load of a step to the next (kCols).
+    static __device__ __forceinline__ uint32_t next_of(int64_t ld) { return static_cast<uint32_t>(WAVES * kRowsOf * ld * 2); }
 };
+
+// Where the next step of an operand is, in registers: a step's loads are issued without
+// a look at the kernel's arguments, whose latency the matrix cores would wait out.
+struct MatStream {
+    uint64_t at;
+    int64_t step, plane;  // bytes
+};
+
+template <int KIND, int BK>
+__device__ __forceinline__ MatStream mat_stream(const MatOperand& o, int32_t row0, int32_t k0) {
+    const int64_t first = KIND == kRows ? row0 * o.ld + k0 : k0 * o.ld + row0;
+    return MatStream{reinterpret_cast<uint64_t>(o.p) + 2 * first, KIND == kRows ? 2 * BK : 2 * BK * o.ld, 2 * o.plane};
+}
 
 typedef int16_t s4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s4* lds_tr;
@@ -193,7 +216,7 @@ constexpr int kMatGroup = 4;  // n tiles that neighbours in the order share
 template <class S>
 __device__ __forceinline__ bool mat_tile_of(const MatArgs& g, MatAt* at) {
     at->m = g.m;
-    at->n = g.n_dev ? min(g.n, *g.n_dev) : g.n;
+    at->n = g.n_dev ? __builtin_amdgcn_readfirstlane(min(g.n, *g.n_dev)) : g.n;
     const uint32_t tiles_m = (g.m + S::kM / S::kSubs - 1) / (S::kM / S::kSubs), tiles_n = (at->n + S::kN - 1) / S::kN;
     const uint32_t one = tiles_m * tiles_n, total = one * g.batches * g.splits;
     const uint32_t per = (total + kMatXcds - 1) / kMatXcds;
@@ -228,12 +251,32 @@ struct MatAcc {
     __device__ __forceinline__ int n_of(int j) const { return col(j) + threadIdx.x % 32; }
 };
 
+// Every wave's LDS reads before it are done and every wave's landed loads can be read
+// after it; loads still out stay out (__syncthreads would wait for them).
+__device__ __forceinline__ void mat_barrier() {
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" : : : "memory");
+}
+
+// Reads spread between the products of the chunk before.
+template <class S>
+__device__ __forceinline__ void mat_interleave() {
+    constexpr int kPairs = S::kPa == 3 ? 6 : S::kPa + S::kPb - 1;
+    constexpr int kReads = S::kPa * S::kBm * (S::kKindA == kCols ? 2 : 1) + S::kPb * S::kBn * (S::kKindB == kCols ? 2 : 1);
+    constexpr int kMfma = kPairs * S::kBm * S::kBn;
+    constexpr int kEach = (kReads + kMfma - 1) / kMfma;
+#pragma unroll
+    for (int i = 0; i < kMfma; ++i) {
+        if (i * kEach < kReads) __builtin_amdgcn_sched_group_barrier(0x100, kEach, 0);
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    }
+}
+
 template <class S, class Epi>
 __global__ __launch_bounds__(S::kThreads, S::kThreads == 512 ? 2 : 1) void mat_kernel(MatArgs g, Epi epi) {
     __shared__ __attribute__((aligned(1024))) char lds[S::kLds];
     MatAt at;
     if (!mat_tile_of<S>(g, &at)) return;
-    const int32_t k = g.k_dev ? min(g.k, *g.k_dev) : g.k;
+    const int32_t k = g.k_dev ? __builtin_amdgcn_readfirstlane(min(g.k, *g.k_dev)) : g.k;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     MatAcc<S> acc;
     acc.wm = wave / S::kWaveN;
@@ -245,65 +288,108 @@ __global__ __launch_bounds__(S::kThreads, S::kThreads == 512 ? 2 : 1) void mat_k
     TileB tb;
     ta.init(g.a[0].ld, g.m - at.m0);
     tb.init(g.b[0].ld, at.n - at.n0);
-    const auto first = [](const MatOperand& o, int kind, int32_t row) { return o.p + (kind == kRows ? row * o.ld : row); };
-
     // Steps of this workgroup: the split's share of all segments' steps.
     const int32_t of_one = (k + S::kK - 1) / S::kK, all = of_one * g.segments;
     const int32_t begin = static_cast<int32_t>(static_cast<int64_t>(all) * at.split / g.splits);
     const int32_t end = static_cast<int32_t>(static_cast<int64_t>(all) * (at.split + 1) / g.splits);
     const uint32_t base = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)lds));
-    const auto load = [&](int32_t step, int buf) {
-        const int seg = g.segments > 1 && step >= of_one;
-        const int32_t k0 = (step - seg * of_one) * S::kK, left = k - k0;
+    const uint32_t next_a = __builtin_amdgcn_readfirstlane(TileA::next_of(g.a[0].ld));
+    const uint32_t next_b = __builtin_amdgcn_readfirstlane(TileB::next_of(g.b[0].ld));
+    MatStream sa[S::kSubs], sb;
+    int32_t fetched = begin, left = 0, until = 0;  // the next step to load; its k's left; the segment's end
+    const auto seek = [&]() {
+        const int seg = g.segments > 1 && fetched >= of_one;
+        const int32_t k0 = (fetched - seg * of_one) * S::kK;
+        until = (seg + 1) * of_one;
+        left = k - k0;
+#pragma unroll
+        for (int s = 0; s < S::kSubs; ++s)
+            sa[s] = mat_stream<S::kKindA, S::kK>(g.a[S::kDual ? s : g.segments > 1 ? seg : at.batch], at.m0, k0);
+        sb = mat_stream<S::kKindB, S::kK>(g.b[seg], at.n0, k0);
+    };
+    const auto load = [&](int buf) {
         const uint32_t to = base + buf * S::kStage;
 #pragma unroll
         for (int s = 0; s < S::kSubs; ++s) {
-            const MatOperand& o = g.a[S::kDual ? s : g.segments > 1 ? seg : at.batch];
-            ta.load(to + s * S::kPa * TileA::kBytes, o, first(o, S::kKindA, at.m0), k0, left);
+            ta.load(to + s * S::kPa * TileA::kBytes, sa[s].at, sa[s].plane, next_a, left, wave);
+            sa[s].at += sa[s].step;
         }
-        const MatOperand& o = g.b[seg];
-        tb.load(to + S::kPa * S::kPlaneA, o, first(o, S::kKindB, at.n0), k0, left);
+        tb.load(to + S::kPa * S::kPlaneA, sb.at, sb.plane, next_b, left, wave);
+        sb.at += sb.step;
+        left -= S::kK;
+        if (++fetched == until && fetched < end) seek();
     };
 
 #pragma unroll
     for (int i = 0; i < S::kBm; ++i)
 #pragma unroll
         for (int j = 0; j < S::kBn; ++j) acc.c[i][j] = f16v{};
-    if (begin < end) load(begin, 0);
-    for (int32_t step = begin; step < end; ++step) {
-        const int buf = (step - begin) & 1;
-        mat_landed();
-        __syncthreads();
-        if (step + 1 < end) load(step + 1, buf ^ 1);
+    // Operands of 16 of the contraction, read one ahead of their products.
+    u4 a[2][S::kBm][S::kPa], b[2][S::kBn][S::kPb];
+    const auto read = [&](int buf, int c, int to) {
         const char* la = lds + buf * S::kStage;
         const char* lb = la + S::kPa * S::kPlaneA;
 #pragma unroll
-        for (int c = 0; c < S::kK / 16; ++c) {
-            u4 a[S::kBm][S::kPa], b[S::kBn][S::kPb];
+        for (int p = 0; p < S::kPb; ++p)
 #pragma unroll
-            for (int p = 0; p < S::kPb; ++p)
+            for (int j = 0; j < S::kBn; ++j) b[to][j][p] = MatRead<S::kN, S::kK, S::kKindB>::get(lb, acc.col(j), c, p);
 #pragma unroll
-                for (int j = 0; j < S::kBn; ++j) b[j][p] = MatRead<S::kN, S::kK, S::kKindB>::get(lb, acc.col(j), c, p);
+        for (int p = 0; p < S::kPa; ++p)
 #pragma unroll
-            for (int p = 0; p < S::kPa; ++p)
+            for (int i = 0; i < S::kBm; ++i)
+                a[to][i][p] = MatRead<S::kSubRows, S::kK, S::kKindA>::get(la + (i / S::kSubBlocks) * S::kPa * TileA::kBytes,
+                                                                          acc.row(i), c, p);
+    };
+    // The small products first (mfma_split's order where both have three planes).
+    const auto multiply = [&](int at) {
+        constexpr int kLast = (S::kPa > S::kPb ? S::kPa : S::kPb) - 1;
+#pragma unroll
+        for (int sum = kLast; sum >= 0; --sum)
+#pragma unroll
+            for (int pa = S::kPa - 1; pa >= 0; --pa) {
+                const int pb = sum - pa;
+                if (pb < 0 || pb >= S::kPb) continue;
 #pragma unroll
                 for (int i = 0; i < S::kBm; ++i)
-                    a[i][p] = MatRead<S::kSubRows, S::kK, S::kKindA>::get(
-                        la + (i / S::kSubBlocks) * S::kPa * TileA::kBytes, acc.row(i), c, p);
-            // The small products first (mfma_split's order where both have three planes).
-            constexpr int kLast = (S::kPa > S::kPb ? S::kPa : S::kPb) - 1;
 #pragma unroll
-            for (int sum = kLast; sum >= 0; --sum)
+                    for (int j = 0; j < S::kBn; ++j) acc.c[i][j] = mfma_bf16(a[at][i][pa], b[at][j][pb], acc.c[i][j]);
+            }
+    };
+    constexpr int kChunks = S::kK / 16;
+    static_assert(kChunks % 2 == 0);
+    // Loads are kStages - 1 steps ahead of the products.  Those of a step are complete
+    // once only the later steps' are out.
+    constexpr int kAhead = S::kStages - 1;
+    constexpr int kLater = (S::kStages - 2) * (S::kPa * S::kSubs * TileA::kLoads + S::kPb * TileB::kLoads);
+    if (begin < end) {
+        seek();
+        for (int i = 0; i < kAhead && begin + i < end; ++i) load(i);
+        if (begin + kAhead <= end) mat_landed<kLater>();
+        else mat_landed<0>();
+        mat_barrier();
+        read(0, 0, 0);
+    }
+    int buf = 0;
+    for (int32_t step = begin; step < end; ++step) {
+        if (S::kStages == 2 && fetched < end) load(buf ^ 1);
+        const int next = buf + 1 < S::kStages ? buf + 1 : 0;
 #pragma unroll
-                for (int pa = S::kPa - 1; pa >= 0; --pa) {
-                    const int pb = sum - pa;
-                    if (pb < 0 || pb >= S::kPb) continue;
-#pragma unroll
-                    for (int i = 0; i < S::kBm; ++i)
-#pragma unroll
-                        for (int j = 0; j < S::kBn; ++j) acc.c[i][j] = mfma_bf16(a[i][pa], b[j][pb], acc.c[i][j]);
-                }
+        for (int c = 0; c < kChunks; ++c) {
+            if (c + 1 < kChunks) {
+                read(buf, c + 1, (c + 1) & 1);
+            } else if (step + 1 < end) {
+                if (step + kAhead < end) mat_landed<kLater>();
+                else mat_landed<0>();
+                mat_barrier();
+                read(next, 0, 0);
+            }
+            multiply(c & 1);
+            mat_interleave<S>();
+            // Behind the first products, which run meanwhile.  The buffer is the step
+            // before's, which every wave has read (the last barrier).
+            if (S::kStages > 2 && c == 0 && fetched < end) load(buf ? buf - 1 : S::kStages - 1);
         }
+        buf = next;
     }
     __syncthreads();  // the epilogue may use the LDS
     epi.template run<S>(at, acc, lds);
@@ -318,11 +404,11 @@ int64_t mat_tiles(const MatArgs& g) {
 // The two shapes of a product with PA and PB planes: a CU's workgroup of eight waves
 // where such tiles fill most of the GPU, else four waves, two or more to a CU.
 template <int PA, int PB, int KA, int KB, bool DUAL = false>
-using MatBig = std::conditional_t<PA == 3, MatShape<256, 128, 4, 2, 32, 3, 3, KA, KB, DUAL>,
-                                  MatShape<256, 256, 2, 4, 64, PA, PB, KA, KB, DUAL>>;
+using MatBig = std::conditional_t<PA == 3, MatShape<256, 128, 4, 2, 32, 2, 3, 3, KA, KB, DUAL>,
+                                  MatShape<256, 256, 2, 4, 64, 2, PA, PB, KA, KB, DUAL>>;
 template <int PA, int PB, int KA, int KB, bool DUAL = false>
-using MatSmall = std::conditional_t<PA == 3, MatShape<128, 64, 2, 2, 32, 3, 3, KA, KB, DUAL>,
-                                    MatShape<128, 128, 2, 2, 64, PA, PB, KA, KB, DUAL>>;
+using MatSmall = std::conditional_t<PA == 3, MatShape<128, 64, 2, 2, 32, 2, 3, 3, KA, KB, DUAL>,
+                                    MatShape<128, 128, 2, 2, 64, 2, PA, PB, KA, KB, DUAL>>;
 constexpr int64_t kMatBigTiles = 192;
 template <class S>
 bool mat_fills(const mimir_ctx* ctx, const MatArgs& g) {
@@ -342,6 +428,11 @@ int mat_launch(mimir_ctx* ctx, const char* what, const MatArgs& g, const Epi& ep
     return launched(ctx, what);
 }
 
+// Vectors at an address that is a multiple of their elements' size: gfx950 loads and
+// stores them as it does aligned ones.
+typedef uint32_t u4e __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t u2e __attribute__((ext_vector_type(2), aligned(2)));
+
 // --- C as a result -----------------------------------------------------------------
 
 // out[row(n)][m] (+)= alpha * sum, sum over the pieces and splits of the contraction
@@ -358,7 +449,6 @@ struct MatOut {
     int32_t bf16, accumulate;
     int32_t read_partial;     // pieces before this one have left their sums
     int32_t last;             // this piece's sums go to out, not to partial
-    int32_t vec;              // out and ld are multiples of four elements
 
     __device__ __forceinline__ float factor() const { return count ? alpha / fmaxf(*count, 1.0f) : alpha; }
     __device__ __forceinline__ void put(int batch, int64_t n, int32_t m, int32_t limit, f4 v, float by) const {
@@ -366,14 +456,14 @@ struct MatOut {
         if (bf16) {
             uint16_t* p = static_cast<uint16_t*>(out[batch]) + r * ld + m;
             f4 old{};
-            if (vec && m + 4 <= limit) {
+            if (m + 4 <= limit) {
                 if (accumulate) {
-                    const u2 t = *reinterpret_cast<const u2*>(p);
+                    const u2e t = *reinterpret_cast<const u2e*>(p);
                     old = f4{__builtin_bit_cast(float, t[0] << 16), __builtin_bit_cast(float, t[0] & 0xffff0000u),
                              __builtin_bit_cast(float, t[1] << 16), __builtin_bit_cast(float, t[1] & 0xffff0000u)};
                 }
                 v = v * by + old;
-                *reinterpret_cast<u2*>(p) = u2{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])};
+                *reinterpret_cast<u2e*>(p) = u2e{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])};
                 return;
             }
 #pragma unroll
@@ -385,8 +475,8 @@ struct MatOut {
             return;
         }
         float* p = static_cast<float*>(out[batch]) + r * ld + m;
-        if (vec && m + 4 <= limit) {
-            f4* q = reinterpret_cast<f4*>(p);
+        if (m + 4 <= limit) {
+            f4u* q = reinterpret_cast<f4u*>(p);
             *q = accumulate ? v * by + *q : v * by;
             return;
         }
@@ -429,14 +519,14 @@ inline bool mat_direct(const void* p, int64_t ld, int64_t cols) {
 }
 
 // Eight values from element `at` of src on, `left` of them in the row, to dst, `plane`
-// elements to the next plane.  VEC: 16-byte loads.
-template <bool BF16, bool VEC>
+// elements to the next plane.
+template <bool BF16>
 __device__ __forceinline__ void mat_stage8(const void* src, int64_t at, int64_t left, uint16_t* dst, int64_t plane) {
     if constexpr (BF16) {
         const uint16_t* p = static_cast<const uint16_t*>(src) + at;
         u4 v{};
-        if (VEC && left >= 8) {
-            v = *reinterpret_cast<const u4*>(p);
+        if (left >= 8) {
+            v = *reinterpret_cast<const u4e*>(p);
         } else {
 #pragma unroll
             for (int e = 0; e < 8; ++e)
@@ -446,8 +536,8 @@ __device__ __forceinline__ void mat_stage8(const void* src, int64_t at, int64_t 
     } else {
         const float* p = static_cast<const float*>(src) + at;
         float x[8];
-        if (VEC && left >= 8) {
-            const f4 a = *reinterpret_cast<const f4*>(p), b = *reinterpret_cast<const f4*>(p + 4);
+        if (left >= 8) {
+            const f4u a = *reinterpret_cast<const f4u*>(p), b = *reinterpret_cast<const f4u*>(p + 4);
 #pragma unroll
             for (int e = 0; e < 4; ++e) x[e] = a[e], x[4 + e] = b[e];
         } else {

@@ -286,6 +286,27 @@ int forward(mimir_ctx* ctx, const Call& c, const Plan& p, char* work, void* y, i
     return MIMIR_OK;
 }
 
+// Few tokens, operands that can be read as they are: one launch.
+bool few_applies(const Call& c) {
+    const bool fp32 = c.type == MIMIR_NUM_F32;
+    return c.tokens <= kFewN && few_direct(fp32, c.x, c.ld_x, c.dim) && few_direct(fp32, c.w[0], c.ld_w, c.hidden) &&
+           few_direct(fp32, c.w[1], c.ld_w, c.hidden);
+}
+
+template <bool FP32, int ACT>
+int forward_few(mimir_ctx* ctx, const Call& c, void* y, int64_t ld_y, float* gate_up) {
+    MatArgs g = args_of(c.hidden, c.tokens, c.dim);
+    for (int i = 0; i < 2; ++i) g.a[i] = MatOperand{static_cast<const uint16_t*>(c.w[i]), c.ld_w, 0};
+    g.b[0] = MatOperand{static_cast<const uint16_t*>(c.x), c.ld_x, 0};
+    GatedOut<ACT> e{};
+    e.y.out[0] = y;
+    e.y.ld = ld_y;
+    e.y.bf16 = !FP32;
+    e.gate_up = gate_up;
+    e.hidden = c.hidden;
+    return few_launch<4, 2, 3, FP32, kCols, true>(ctx, "gated products", g, e);
+}
+
 struct Gradients {
     const float* gate_up;
     const void* dy;
@@ -371,6 +392,10 @@ int mimir_gated_linear_fwd(mimir_ctx* ctx, int type, int act, const void* x, int
     MIMIR_REQUIRE(ctx, x && w_gate && w_up && y, "%s: null pointer", what);
     MIMIR_REQUIRE(ctx, y != x, "%s: y must not be x", what);
     MIMIR_ENTER(ctx);
+    if (few_applies(c)) {
+        if (type == MIMIR_NUM_F32) return act == kSilu ? forward_few<true, kSilu>(ctx, c, y, ld_y, gate_up) : forward_few<true, kGelu>(ctx, c, y, ld_y, gate_up);
+        return act == kSilu ? forward_few<false, kSilu>(ctx, c, y, ld_y, gate_up) : forward_few<false, kGelu>(ctx, c, y, ld_y, gate_up);
+    }
     const Plan p = plan_of(ctx->tune, c, false);
     char* work;
     if (int st = mat_scratch(ctx, p.total, &work)) return st;

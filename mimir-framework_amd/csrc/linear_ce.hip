@@ -112,7 +112,7 @@ __device__ __forceinline__ f2 join(f2 a, f2 b) {
 
 struct CeStats {
     const int32_t* target;
-    const int32_t* row;
+    const int32_t* row;  // null: n itself
     f2* part;            // [tile][tokens]
     float* logit;        // [tokens]: the target's
     int64_t tokens, first;  // first: the piece's first vocabulary row
@@ -156,65 +156,93 @@ struct CeStats {
             part[(tile0 + at.tile_m) * tokens + at.n0 + c] = v;
         }
     }
-    __device__ __forceinline__ int64_t target_of(int32_t n) const { return target[row[n]]; }
+    __device__ __forceinline__ int64_t target_of(int32_t n) const { return target[row ? row[n] : n]; }
 };
 
 constexpr int kFinishTokens = 32;
 
-// 32 tokens a workgroup, eight threads a token over the tiles.  The workgroup that is
-// done last adds up all of them for the mean, in a fixed order and 64 bits.
-__global__ __launch_bounds__(kBlock) void ce_finish(const f2* part, int64_t tokens, int32_t tiles, const float* logit,
-                                                    const int32_t* row, int32_t* count, float* loss, float* lse, double* sums,
-                                                    float* mean) {
-    constexpr int kParts = kBlock / kFinishTokens, kTogether = 4;
+struct FinishArgs {
+    const f2* part;
+    int64_t tokens;
+    int32_t tiles;
+    const float* logit;
+    const int32_t* row;     // of the gathered tokens, *count of them; null: all tokens, one workgroup
+    int32_t* count;         // and the counter of workgroups that are done
+    const int32_t* target;  // row null
+    int64_t vocab;
+    float* loss;
+    float* lse;
+    double* sums;           // one for each workgroup
+    float* mean;            // or null
+};
+
+// 32 tokens a workgroup, THREADS / 32 threads a token over the tiles.  The workgroup
+// that is done last adds up all of them for the mean, in a fixed order and 64 bits.
+template <int THREADS>
+__global__ __launch_bounds__(THREADS) void ce_finish(FinishArgs a) {
+    constexpr int kParts = THREADS / kFinishTokens, kTogether = 4;
     __shared__ f2 red[kParts][kFinishTokens];
-    __shared__ double wave_sums[kBlock / kWave];
+    __shared__ double wave_sums[THREADS / kWave];
     __shared__ bool last;
     const int t = threadIdx.x % kFinishTokens, p = threadIdx.x / kFinishTokens;
     const int64_t n = static_cast<int64_t>(blockIdx.x) * kFinishTokens + t;
-    const bool in = n < *count;
+    const int64_t limit = a.row ? *a.count : a.tokens;
+    const bool in = n < limit && (a.row || static_cast<uint32_t>(a.target[n]) < static_cast<uint32_t>(a.vocab));
     f2 v{-__builtin_inff(), 0.0f};
     if (in)
-        for (int32_t i = p; i < tiles; i += kTogether * kParts) {
+        for (int32_t i = p; i < a.tiles; i += kTogether * kParts) {
             f2 x[kTogether];
 #pragma unroll
             for (int e = 0; e < kTogether; ++e)
-                x[e] = i + e * kParts < tiles ? part[(i + e * kParts) * tokens + n] : f2{-__builtin_inff(), 0.0f};
+                x[e] = i + e * kParts < a.tiles ? a.part[(i + e * kParts) * a.tokens + n] : f2{-__builtin_inff(), 0.0f};
             v = join(v, join(join(x[0], x[1]), join(x[2], x[3])));
         }
     red[p][t] = v;
     __syncthreads();
     double sum = 0.0;
-    if (p == 0 && in) {
+    if (p == 0 && n < limit) {
+        float l = 0.0f, own = 0.0f;
+        if (in) {
 #pragma unroll
-        for (int w = 1; w < kParts; ++w) v = join(v, red[w][t]);
-        const float l = v[0] + logf(v[1]), own = l - logit[n];
-        loss[row[n]] = own;
-        lse[row[n]] = l;
-        sum = own;
+            for (int w = 1; w < kParts; ++w) v = join(v, red[w][t]);
+            l = v[0] + logf(v[1]);
+            own = l - a.logit[n];
+            sum = own;
+        }
+        const int64_t to = a.row ? a.row[n] : n;
+        a.loss[to] = own;
+        a.lse[to] = l;
     }
-    if (!mean) return;
+    if (!a.mean) return;
+    int32_t count = a.row ? static_cast<int32_t>(limit) : 0;
     if (threadIdx.x < kWave) {
+        if (!a.row) count = __popcll(__ballot(p == 0 && in));
 #pragma unroll
         for (int d = 1; d < kFinishTokens; d *= 2) sum += __shfl_xor(sum, d);
         if (threadIdx.x == 0) {
-            __hip_atomic_store(sums + blockIdx.x, sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            last = __hip_atomic_fetch_add(count + 1, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == static_cast<int>(gridDim.x) - 1;
+            last = !a.row;
+            if (a.row) {
+                __hip_atomic_store(a.sums + blockIdx.x, sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                last = __hip_atomic_fetch_add(a.count + 1, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == static_cast<int>(gridDim.x) - 1;
+            }
         }
     }
     __syncthreads();
     if (!last) return;
-    sum = 0.0;
-    for (uint32_t i = threadIdx.x; i < gridDim.x; i += kBlock)
-        sum += __hip_atomic_load(sums + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (a.row) {
+        sum = 0.0;
+        for (uint32_t i = threadIdx.x; i < gridDim.x; i += THREADS)
+            sum += __hip_atomic_load(a.sums + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 #pragma unroll
-    for (int d = 1; d < kWave; d *= 2) sum += __shfl_xor(sum, d);
-    if (threadIdx.x % kWave == 0) wave_sums[threadIdx.x / kWave] = sum;
-    __syncthreads();
+        for (int d = 1; d < kWave; d *= 2) sum += __shfl_xor(sum, d);
+        if (threadIdx.x % kWave == 0) wave_sums[threadIdx.x / kWave] = sum;
+        __syncthreads();
+        for (int w = 1; w < THREADS / kWave; ++w)
+            if (threadIdx.x == 0) sum += wave_sums[w];
+    }
     if (threadIdx.x) return;
-    for (int w = 1; w < kBlock / kWave; ++w) sum += wave_sums[w];
-    mean[0] = static_cast<float>(sum / (*count > 0 ? *count : 1));
-    mean[1] = static_cast<float>(*count);
+    a.mean[0] = static_cast<float>(sum / (count > 0 ? count : 1));
+    a.mean[1] = static_cast<float>(count);
 }
 
 // --- backward ----------------------------------------------------------------------
@@ -395,8 +423,32 @@ int forward(mimir_ctx* ctx, const Call& c, const Plan& p, char* work, float* los
         if (st) return st;
         e.tile0 += static_cast<int32_t>((rows + (big ? B::kM : S::kM) - 1) / (big ? B::kM : S::kM));
     }
-    ce_finish<<<static_cast<unsigned>((c.tokens + kFinishTokens - 1) / kFinishTokens), kBlock, 0, ctx->stream>>>(
-        e.part, c.tokens, e.tile0, e.logit, row, count, loss, lse, reinterpret_cast<double*>(work + p.sums), mean);
+    const FinishArgs f{e.part, c.tokens, e.tile0, e.logit, row, count, nullptr, 0, loss, lse, reinterpret_cast<double*>(work + p.sums), mean};
+    ce_finish<kBlock><<<static_cast<unsigned>((c.tokens + kFinishTokens - 1) / kFinishTokens), kBlock, 0, ctx->stream>>>(f);
+    return launched(ctx, "ce_finish");
+}
+
+// Few tokens, operands that can be read as they are: no token is gathered and no operand
+// staged.
+constexpr int kFewBlocks = 2;
+
+bool few_applies(const Call& c) {
+    const bool fp32 = c.type == MIMIR_NUM_F32;
+    return c.tokens <= kFewN && few_direct(fp32, c.x, c.ld_x, c.dim) && few_direct(fp32, c.w, c.ld_w, c.dim);
+}
+
+template <bool FP32>
+int forward_few(mimir_ctx* ctx, const Call& c, float* loss, float* lse, float* mean) {
+    constexpr int64_t kRowsOf = 32 * kFewBlocks;
+    const int64_t tiles = (c.vocab + kRowsOf - 1) / kRowsOf;
+    char* work;
+    if (int st = mat_scratch(ctx, 256 + static_cast<size_t>(tiles * c.tokens * 8), &work)) return st;
+    const auto operand = [](const void* p, int64_t ld) { return MatOperand{static_cast<const uint16_t*>(p), ld, 0}; };
+    const MatArgs g = args_of(operand(c.w, c.ld_w), operand(c.x, c.ld_x), c.vocab, c.tokens, c.dim);
+    const CeStats e{c.target, nullptr, reinterpret_cast<f2*>(work + 256), reinterpret_cast<float*>(work), c.tokens, 0, 0};
+    if (int st = few_launch<4, kFewBlocks, 3, FP32, kRows, false>(ctx, "cross entropy statistics", g, e)) return st;
+    const FinishArgs f{e.part, c.tokens, static_cast<int32_t>(tiles), e.logit, nullptr, nullptr, c.target, c.vocab, loss, lse, nullptr, mean};
+    ce_finish<1024><<<1, 1024, 0, ctx->stream>>>(f);
     return launched(ctx, "ce_finish");
 }
 
@@ -486,6 +538,8 @@ int mimir_linear_cross_entropy_fwd(mimir_ctx* ctx, int type, const void* x, int6
     MIMIR_REQUIRE(ctx, tokens == 0 || (x && w && targets && loss && lse), "%s: null pointer", what);
     if (tokens == 0 && !mean) return MIMIR_OK;
     MIMIR_ENTER(ctx);
+    if (tokens > 0 && few_applies(c))
+        return type == MIMIR_NUM_F32 ? forward_few<true>(ctx, c, loss, lse, mean) : forward_few<false>(ctx, c, loss, lse, mean);
     const Plan p = plan_of(ctx->tune, type, w, ld_w, tokens, dim, vocab, false);
     char* work;
     if (int st = mat_scratch(ctx, p.total, &work)) return st;

@@ -433,6 +433,215 @@ int mat_launch(mimir_ctx* ctx, const char* what, const MatArgs& g, const Epi& ep
 typedef uint32_t u4e __attribute__((ext_vector_type(4), aligned(2)));
 typedef uint32_t u2e __attribute__((ext_vector_type(2), aligned(2)));
 
+// --- products of few tokens ---------------------------------------------------------
+//
+// Up to 32 n: the time is A's bytes (the weights').  Each wave of a workgroup has its
+// own share of the contraction and its own ring of LDS stages, filled as mat_kernel's
+// are, so nothing waits for another wave before the end, where the waves' sums meet in
+// LDS.  FP32: both operands are fp32 in memory and are split as they are read from LDS
+// (their planes would be three times the bytes on the way).  Of each wave's stages all
+// but one are on their way: 8 waves of 2 x 8 KB a CU are 33 MB in flight on the GPU.
+
+constexpr int kFewN = 32;
+
+// 32 rows of a raw fp32 operand, BK = 32: kRows 128 bytes a row, kCols 128 bytes a k.
+template <int KIND>
+__device__ __forceinline__ Split8 few_read32(const char* tile, int c) {
+    const int lane = threadIdx.x % kWave, li = lane % 32, hf = lane / 32;
+    float x[8];
+    if constexpr (KIND == kRows) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const f4 v = *reinterpret_cast<const f4*>(tile + li * 128 + 16 * ((4 * c + 2 * hf + h) ^ mat_swizzle<32, 64, kRows>(li)));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[4 * h + e] = v[e];
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = *reinterpret_cast<const float*>(tile + (16 * c + 8 * hf + e) * 128 + 4 * li);
+    }
+    return split8(x);
+}
+
+// The same of bf16, BK = 64: kCols 64 bytes a k.
+template <int KIND>
+__device__ __forceinline__ u4 few_read16(const char* tile, int c) {
+    if constexpr (KIND == kRows) {
+        return MatRead<32, 64, kRows>::get(tile, 0, c, 0);
+    } else {
+        const int lane = threadIdx.x % kWave;
+        const char* a = tile + (16 * c + 8 * (lane / 32) + lane % 16 / 4) * 64 + 32 * (lane / 16 % 2) + 8 * (lane % 4);
+        const u2 x = __builtin_bit_cast(u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_tr)a));
+        const u2 y = __builtin_bit_cast(u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_tr)(a + 4 * 64)));
+        return u4{x[0], x[1], y[0], y[1]};
+    }
+}
+
+// WAVES waves, BLOCKS blocks of 32 rows of A (DUAL: half of them of a[0], half of a[1]).
+template <int WAVES, int BLOCKS, int STAGES, bool FP32, int KA, bool DUAL>
+struct FewShape {
+    static constexpr int kM = 32 * BLOCKS, kN = kFewN, kWaveN = 1, kThreads = kWave * WAVES, kKindA = KA;
+    static constexpr bool kDual = DUAL;
+    static constexpr int kSubs = DUAL ? 2 : 1, kSubRows = kM / kSubs, kSubBlocks = 1;
+    // The epilogue: a block (DUAL: one of each) a wave.
+    static constexpr int kBm = kSubs, kBn = 1, kWaveM = BLOCKS / kSubs;
+    static constexpr int kK = FP32 ? 32 : 64;
+    static constexpr int kTile = 4096;  // bytes of 32 rows of kK
+    static constexpr int kStage = (BLOCKS + 1) * kTile, kRing = STAGES * kStage, kLds = WAVES * kRing;
+    static_assert(kLds <= 160 * 1024 && kWaveM <= WAVES && WAVES * BLOCKS * 4096 <= kLds);
+};
+
+template <int WAVES, int BLOCKS, int STAGES, bool FP32, int KA, bool DUAL, class Epi>
+__global__ __launch_bounds__(kWave* WAVES, 1) void few_kernel(MatArgs g, Epi epi) {
+    using S = FewShape<WAVES, BLOCKS, STAGES, FP32, KA, DUAL>;
+    constexpr int kSize = FP32 ? 4 : 2, kChunk = 16 / kSize;  // bytes of an element, elements of 16 bytes
+    __shared__ __attribute__((aligned(1024))) char lds[S::kLds];
+    const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    MatAt at{};
+    at.m = g.m;
+    at.n = g.n;
+    at.tile_m = blockIdx.x;
+    at.m0 = at.tile_m * (S::kM / S::kSubs);
+
+    // Rows of 128 bytes: eight lanes a row.  kCols bf16: 64 bytes of 32 values a k, four lanes.
+    constexpr bool kWide = KA == kRows || FP32;
+    constexpr int kLanesA = kWide ? 8 : 4, kRowsOfA = kWave / kLanesA, kLoads = S::kTile / 1024;
+    const int ra = lane / kLanesA, slot_a = lane % kLanesA, rb = lane / 8, slot_b = lane % 8;
+    uint32_t off_a[BLOCKS][KA == kRows ? kLoads : 1], off_b[kLoads];
+    int32_t k_a[KA == kRows ? kLoads : 1], k_b[kLoads];
+    const int64_t lda = g.a[0].ld * kSize, ldb = g.b[0].ld * kSize;  // bytes
+#pragma unroll
+    for (int j = 0; j < kLoads; ++j) {
+        const int row = j * 8 + rb, chunk = slot_b ^ mat_swizzle<32, 64, kRows>(row);
+        k_b[j] = kChunk * chunk;
+        off_b[j] = row < g.n ? static_cast<uint32_t>(row * ldb + 16 * chunk) : kOutside;
+    }
+#pragma unroll
+    for (int b = 0; b < BLOCKS; ++b) {
+        const int32_t rows = g.m - at.m0 - 32 * (DUAL ? b % (BLOCKS / 2) : b);  // of this block on
+        if constexpr (KA == kRows) {
+#pragma unroll
+            for (int j = 0; j < kLoads; ++j) {
+                const int row = j * 8 + ra, chunk = slot_a ^ mat_swizzle<32, 64, kRows>(row);
+                k_a[j] = kChunk * chunk;
+                off_a[b][j] = row < rows ? static_cast<uint32_t>(row * lda + 16 * chunk) : kOutside;
+            }
+        } else {
+            k_a[0] = ra;
+            off_a[b][0] = kChunk * slot_a < rows ? static_cast<uint32_t>(ra * lda + 16 * slot_a) : kOutside;
+        }
+    }
+
+    const int32_t all = (g.k + S::kK - 1) / S::kK;
+    const int32_t begin = static_cast<int32_t>(static_cast<int64_t>(all) * wave / WAVES);
+    const int32_t end = static_cast<int32_t>(static_cast<int64_t>(all) * (wave + 1) / WAVES);
+    const uint32_t base = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)lds)) + wave * S::kRing;
+    uint64_t pa[BLOCKS], pb = reinterpret_cast<uint64_t>(g.b[0].p) + int64_t{begin} * 128;
+    const int64_t step_a = KA == kRows ? 128 : S::kK * lda;
+#pragma unroll
+    for (int b = 0; b < BLOCKS; ++b) {
+        const MatOperand& o = g.a[DUAL ? b / (BLOCKS / 2) : 0];
+        const int64_t row = at.m0 + 32 * (DUAL ? b % (BLOCKS / 2) : b);
+        pa[b] = reinterpret_cast<uint64_t>(o.p) + (KA == kRows ? row * lda : row * kSize) + begin * step_a;
+    }
+    int32_t fetched = begin;
+    const auto load = [&](int stage) {
+        const int32_t left = g.k - fetched * S::kK;
+        const uint32_t to = base + stage * S::kStage;
+        const auto rsrc = [](uint64_t p) { return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(p), 0, 0x7fffffff, kBufferWord3); };
+#pragma unroll
+        for (int b = 0; b < BLOCKS; ++b) {
+            const auto rs = rsrc(pa[b]);
+#pragma unroll
+            for (int j = 0; j < kLoads; ++j) {
+                if constexpr (KA == kRows)
+                    load_to_lds(to + b * S::kTile + j * 1024, k_a[j] < left ? off_a[b][j] : kOutside, rs, 0);
+                else
+                    load_to_lds(to + b * S::kTile + j * 1024, k_a[0] + j * kRowsOfA < left ? off_a[b][0] : kOutside, rs,
+                                __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(j * kRowsOfA * lda)));
+            }
+            pa[b] += step_a;
+        }
+        const auto rs = rsrc(pb);
+#pragma unroll
+        for (int j = 0; j < kLoads; ++j) load_to_lds(to + BLOCKS * S::kTile + j * 1024, k_b[j] < left ? off_b[j] : kOutside, rs, 0);
+        pb += 128;
+        ++fetched;
+    };
+
+    f16v acc[BLOCKS];
+#pragma unroll
+    for (int b = 0; b < BLOCKS; ++b) acc[b] = f16v{};
+    constexpr int kLater = (STAGES - 2) * (BLOCKS + 1) * kLoads;
+    for (int i = 0; i < STAGES - 1 && fetched < end; ++i) load(i);
+    int buf = 0;
+    for (int32_t step = begin; step < end; ++step) {
+        if (step + STAGES - 1 <= end) mat_landed<kLater>();
+        else mat_landed<0>();
+        const char* tile = lds + wave * S::kRing + buf * S::kStage;
+        const char* tb = tile + BLOCKS * S::kTile;
+#pragma unroll
+        for (int c = 0; c < S::kK / 16; ++c) {
+            if constexpr (FP32) {
+                const Split8 x = few_read32<kRows>(tb, c);
+#pragma unroll
+                for (int b = 0; b < BLOCKS; ++b) acc[b] = mfma_split(few_read32<KA>(tile + b * S::kTile, c), x, acc[b]);
+            } else {
+                const u4 x = MatRead<32, 64, kRows>::get(tb, 0, c, 0);
+#pragma unroll
+                for (int b = 0; b < BLOCKS; ++b) acc[b] = mfma_bf16(few_read16<KA>(tile + b * S::kTile, c), x, acc[b]);
+            }
+        }
+        // The stage that was read is the next to be filled: its reads are in registers.
+        asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
+        if (fetched < end) load(buf ? buf - 1 : STAGES - 1);
+        buf = buf + 1 < STAGES ? buf + 1 : 0;
+    }
+    __syncthreads();
+    float* part = reinterpret_cast<float*>(lds);  // [wave][block][register][lane]
+#pragma unroll
+    for (int b = 0; b < BLOCKS; ++b)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) part[((wave * BLOCKS + b) * 16 + r) * kWave + lane] = acc[b][r];
+    __syncthreads();
+    MatAcc<S> sum;
+    sum.wm = wave;
+    sum.wn = 0;
+    if (wave < S::kWaveM) {
+#pragma unroll
+        for (int i = 0; i < S::kBm; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                float v = 0.0f;
+#pragma unroll
+                for (int w = 0; w < WAVES; ++w) v += part[((w * BLOCKS + i * S::kWaveM + wave) * 16 + r) * kWave + lane];
+                sum.c[i][0][r] = v;
+            }
+    } else {
+        at.n = 0;  // no part of the result
+#pragma unroll
+        for (int i = 0; i < S::kBm; ++i) sum.c[i][0] = f16v{};
+    }
+    __syncthreads();  // the epilogue may use the LDS
+    epi.template run<S>(at, sum, lds);
+}
+
+
+// Operands that few_kernel takes as they are: 16-byte chunks within rows.
+inline bool few_direct(bool fp32, const void* p, int64_t ld, int64_t cols) {
+    const int64_t of = fp32 ? 4 : 8;
+    return aligned16(p) && ld % of == 0 && cols % of == 0 && mat_ld_fits(ld);
+}
+
+template <int WAVES, int BLOCKS, int STAGES, bool FP32, int KA, bool DUAL, class Epi>
+int few_launch(mimir_ctx* ctx, const char* what, const MatArgs& g, const Epi& epi) {
+    constexpr int64_t kRowsOf = 32 * BLOCKS / (DUAL ? 2 : 1);
+    const int64_t grid = (g.m + kRowsOf - 1) / kRowsOf;
+    MIMIR_REQUIRE(ctx, dispatch_fits(grid, kWave * WAVES), "%s: grid of %lld workgroups exceeds the limit", what, (long long)grid);
+    few_kernel<WAVES, BLOCKS, STAGES, FP32, KA, DUAL, Epi><<<static_cast<unsigned>(grid), kWave * WAVES, 0, ctx->stream>>>(g, epi);
+    return launched(ctx, what);
+}
+
 // --- C as a result -----------------------------------------------------------------
 
 // out[row(n)][m] (+)= alpha * sum, sum over the pieces and splits of the contraction

@@ -57,30 +57,39 @@ struct GatedOut {
 #pragma unroll
         for (int j = 0; j < S::kBn; ++j) {
             const int32_t n = at.n0 + acc.n_of(j);
-            if (n >= at.n) continue;
+            const bool live = n < at.n;
 #pragma unroll
             for (int i = 0; i < S::kSubBlocks; ++i)
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const int32_t m = at.m0 + acc.m_of(i, 4 * q);
-                    if (m >= at.m) continue;
-                    f4 g, u, v;
+                for (int h = 0; h < 2; ++h) {
+                    f4 g[2], u[2];
+                    float v[8];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        g[e] = acc.c[i][j][4 * q + e];
-                        u[e] = acc.c[i + S::kSubBlocks][j][4 * q + e];
-                        v[e] = act1<ACT>(g[e]) * u[e];
+                    for (int e = 0; e < 8; ++e) {
+                        g[e / 4][e % 4] = acc.c[i][j][8 * h + e];
+                        u[e / 4][e % 4] = acc.c[i + S::kSubBlocks][j][8 * h + e];
+                        v[e] = act1<ACT>(acc.c[i][j][8 * h + e]) * acc.c[i + S::kSubBlocks][j][8 * h + e];
                     }
-                    y.put(0, n, m, at.m, v, 1.0f);
-                    if (!gate_up) continue;
-                    float* to = gate_up + n * 2 * hidden + m;
-                    if (m + 4 <= at.m) {
-                        *reinterpret_cast<f4u*>(to) = g;
-                        *reinterpret_cast<f4u*>(to + hidden) = u;
-                    } else {
+                    if (y.bf16) {
+                        const u4 x = mat_exchange(mat_pack8(v));
+                        if (live) y.put8(0, n, at.m0 + acc.m_of8(i, h), at.m, x);
+                    }
+                    if (!live) continue;
 #pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            if (m + e < at.m) to[e] = g[e], to[hidden + e] = u[e];
+                    for (int q = 0; q < 2; ++q) {
+                        const int32_t m = at.m0 + acc.m_of(i, 8 * h + 4 * q);
+                        if (m >= at.m) continue;
+                        if (!y.bf16) y.put(0, n, m, at.m, f4{v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]}, 1.0f);
+                        if (!gate_up) continue;
+                        float* to = gate_up + n * 2 * hidden + m;
+                        if (m + 4 <= at.m) {
+                            *reinterpret_cast<f4u*>(to) = g[q];
+                            *reinterpret_cast<f4u*>(to + hidden) = u[q];
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                if (m + e < at.m) to[e] = g[q][e], to[hidden + e] = u[q][e];
+                        }
                     }
                 }
         }
@@ -175,11 +184,11 @@ struct Plan {
     int p, pg;
     int64_t ld_x, piece, ld_w;  // columns of x's planes; a piece's columns of the weights, their planes' columns
     bool x_direct, w_direct;
-    int splits_x, splits_w;
+    MatDeal deal_x, deal_w;
     size_t x, w, g, partial, partial_w, total;
 };
 
-Plan plan_of(const Tuning& tune, const Call& c, bool back) {
+Plan plan_of(const mimir_ctx* ctx, const Call& c, bool back) {
     Plan p{};
     p.p = c.type == MIMIR_NUM_BF16 ? 1 : 3;
     p.pg = p.p == 3 ? 3 : c.tokens <= kTwoPlaneTokens ? 2 : 1;
@@ -187,7 +196,7 @@ Plan plan_of(const Tuning& tune, const Call& c, bool back) {
     p.w_direct = p.p == 1 && mat_direct(c.w[0], c.ld_w, c.hidden) && mat_direct(c.w[1], c.ld_w, c.hidden);
     p.ld_x = mat_round(c.dim, 8);
     const int64_t of_column = (back ? c.tokens * p.pg * 4 : 0) + (p.w_direct ? 0 : c.dim * p.p * 4);
-    if (tune.mat_piece > 0) p.piece = mat_round(tune.mat_piece, 8);
+    if (ctx->tune.mat_piece > 0) p.piece = mat_round(ctx->tune.mat_piece, 8);
     else p.piece = of_column ? std::max<int64_t>(256, kPieceBytes / of_column / 256 * 256) : c.hidden;
     p.piece = std::min({p.piece, mat_round(c.hidden, 8), int64_t{1} << 18});
     p.ld_w = p.piece;
@@ -202,14 +211,18 @@ Plan plan_of(const Tuning& tune, const Call& c, bool back) {
     if (back) {
         p.g = take(static_cast<size_t>(p.pg * c.tokens * 2 * p.piece * 2));
         const int64_t piece = std::min(p.piece, c.hidden);
-        const auto splits = [&](int64_t m, int64_t n, int64_t k, int64_t batches) {
-            return p.p == 3 ? mat_splits<MatSmall<3, 3, kRows, kRows>>(m, n, k, batches)
-                            : mat_splits<MatSmall<1, 1, kRows, kRows>>(m, n, k, batches);
-        };
-        p.splits_x = splits(c.dim, c.tokens, 2 * piece, 1);
-        p.splits_w = splits(piece, c.dim, c.tokens, 2);
-        p.partial = take(p.splits_x > 1 || p.piece < c.hidden ? static_cast<size_t>(p.splits_x * c.tokens * mat_round(c.dim, 4) * 4) : 0);
-        p.partial_w = take(p.splits_w > 1 ? static_cast<size_t>(2 * p.splits_w * c.dim * mat_round(piece, 4) * 4) : 0);
+        if (p.p == 3) {
+            p.deal_x = mat_deal<3, 3, kRows, kRows>(ctx, c.dim, c.tokens, 2 * piece, 1, p.piece < c.hidden);
+            p.deal_w = mat_deal<3, 3, kCols, kCols>(ctx, piece, c.dim, c.tokens, 2, false);
+        } else if (p.pg == 2) {
+            p.deal_x = mat_deal<1, 2, kRows, kRows>(ctx, c.dim, c.tokens, 2 * piece, 1, p.piece < c.hidden);
+            p.deal_w = mat_deal<2, 1, kCols, kCols>(ctx, piece, c.dim, c.tokens, 2, false);
+        } else {
+            p.deal_x = mat_deal<1, 1, kRows, kRows>(ctx, c.dim, c.tokens, 2 * piece, 1, p.piece < c.hidden);
+            p.deal_w = mat_deal<1, 1, kCols, kCols>(ctx, piece, c.dim, c.tokens, 2, false);
+        }
+        p.partial = take(p.deal_x.partial);
+        p.partial_w = take(p.deal_w.partial);
     }
     p.total = std::max<size_t>(at, 256);
     return p;
@@ -258,7 +271,7 @@ MatArgs args_of(int64_t m, int64_t n, int64_t k) {
     g.m = static_cast<int32_t>(m);
     g.n = static_cast<int32_t>(n);
     g.k = static_cast<int32_t>(k);
-    g.segments = g.batches = g.splits = 1;
+    g.segments = g.batches = 1;
     return g;
 }
 
@@ -332,14 +345,12 @@ int backward(mimir_ctx* ctx, const Call& c, const Plan& p, char* work, const Gra
     ox.ld = d.ld_dx;
     ox.partial = reinterpret_cast<float*>(work + p.partial);
     ox.ld_partial = mat_round(c.dim, 4);
-    ox.slice = c.tokens * ox.ld_partial;
     ox.alpha = 1.0f;
     ox.bf16 = bf16;
     ox.accumulate = d.accumulate_x;
     MatOut ow = ox;
     ow.partial = reinterpret_cast<float*>(work + p.partial_w);
     ow.ld_partial = mat_round(std::min(p.piece, c.hidden), 4);
-    ow.slice = c.dim * ow.ld_partial;
     ow.ld = d.ld_dw;
     ow.accumulate = d.accumulate_w;
     ow.last = 1;
@@ -362,7 +373,7 @@ int backward(mimir_ctx* ctx, const Call& c, const Plan& p, char* work, const Gra
             g.segments = 2;
             ox.read_partial = first > 0;
             ox.last = first + cols >= c.hidden;
-            if (int st = mat_product<P, PG, kRows, kRows>(ctx, "gated dx", g, ox, p.splits_x)) return st;
+            if (int st = mat_product<P, PG, kRows, kRows>(ctx, "gated dx", g, ox, p.deal_x)) return st;
         }
         if (d.dw[0]) {
             MatArgs g = args_of(cols, c.dim, c.tokens);
@@ -371,7 +382,7 @@ int backward(mimir_ctx* ctx, const Call& c, const Plan& p, char* work, const Gra
             g.b[0] = x;
             g.batches = 2;
             for (int i = 0; i < 2; ++i) ow.out[i] = static_cast<char*>(d.dw[i]) + first * size;
-            if (int st = mat_product<PG, P, kCols, kCols>(ctx, "gated dw", g, ow, p.splits_w)) return st;
+            if (int st = mat_product<PG, P, kCols, kCols>(ctx, "gated dw", g, ow, p.deal_w)) return st;
         }
     }
     return MIMIR_OK;
@@ -396,7 +407,7 @@ int mimir_gated_linear_fwd(mimir_ctx* ctx, int type, int act, const void* x, int
         if (type == MIMIR_NUM_F32) return act == kSilu ? forward_few<true, kSilu>(ctx, c, y, ld_y, gate_up) : forward_few<true, kGelu>(ctx, c, y, ld_y, gate_up);
         return act == kSilu ? forward_few<false, kSilu>(ctx, c, y, ld_y, gate_up) : forward_few<false, kGelu>(ctx, c, y, ld_y, gate_up);
     }
-    const Plan p = plan_of(ctx->tune, c, false);
+    const Plan p = plan_of(ctx, c, false);
     char* work;
     if (int st = mat_scratch(ctx, p.total, &work)) return st;
     if (p.p == 3) return act == kSilu ? forward<3, kSilu>(ctx, c, p, work, y, ld_y, gate_up) : forward<3, kGelu>(ctx, c, p, work, y, ld_y, gate_up);
@@ -422,7 +433,7 @@ int mimir_gated_linear_bwd(mimir_ctx* ctx, int type, int act, const void* x, int
                   "%s: dw_gate and dw_up must be buffers of their own", what);
     if (tokens == 0 && !dw_gate) return MIMIR_OK;
     MIMIR_ENTER(ctx);
-    const Plan p = plan_of(ctx->tune, c, true);
+    const Plan p = plan_of(ctx, c, true);
     char* work;
     if (int st = mat_scratch(ctx, p.total, &work)) return st;
     const Gradients d{gate_up, dy, ld_dy, tokens ? dx : nullptr, ld_dx, {dw_gate, dw_up}, ld_dw, accumulate_x ? 1 : 0, accumulate_w ? 1 : 0};

@@ -126,18 +126,29 @@ struct CeStats {
         for (int j = 0; j < S::kBn; ++j) {
             const int32_t n = at.n0 + acc.n_of(j);
             const int64_t target = n < at.n ? target_of(n) - first - at.m0 : -1;
-            float m = -__builtin_inff(), hit = 0.0f;
-            bool has = false;
+            // Few tiles hold any of their tokens' targets.
+            if (__any(target >= 0 && target < S::kM)) {
+                float hit = 0.0f;
+                bool has = false;
+#pragma unroll
+                for (int i = 0; i < S::kBm; ++i)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r)
+                        if (acc.m_of(i, r) == target) hit = acc.c[i][j][r], has = true;
+                if (has) logit[n] = hit;
+            }
+            if (!whole) {
+#pragma unroll
+                for (int i = 0; i < S::kBm; ++i)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r)
+                        if (at.m0 + acc.m_of(i, r) >= at.m) acc.c[i][j][r] = -__builtin_inff();
+            }
+            float m = -__builtin_inff();
 #pragma unroll
             for (int i = 0; i < S::kBm; ++i)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const float z = whole || at.m0 + acc.m_of(i, r) < at.m ? acc.c[i][j][r] : -__builtin_inff();
-                    acc.c[i][j][r] = z;
-                    if (acc.m_of(i, r) == target) hit = z, has = true;
-                    m = fmaxf(m, z);
-                }
-            if (has) logit[n] = hit;
+                for (int r = 0; r < 16; ++r) m = fmaxf(m, acc.c[i][j][r]);
             const float top = fmaxf(m, kLowest) * kLog2e;
             float s = 0.0f;
 #pragma unroll
@@ -262,30 +273,32 @@ struct CeGrad {
 #pragma unroll
         for (int j = 0; j < S::kBn; ++j) {
             const int32_t n = at.n0 + acc.n_of(j);
-            if (n >= at.n) continue;
-            const int32_t t = row[n];
-            const int64_t hit = target[t] - first - at.m0;
-            const float base = lse[t] * kLog2e, w = dloss ? dloss[t] : 1.0f;
+            const bool live = n < at.n;
+            const int32_t t = live ? row[n] : 0;
+            const int64_t hit = live ? target[t] - first - at.m0 : -1;
+            const float base = live ? lse[t] * kLog2e : 0.0f, w = live && dloss ? dloss[t] : 1.0f;
 #pragma unroll
             for (int i = 0; i < S::kBm; ++i)
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const int32_t m = acc.m_of(i, 4 * q);
-                    if (at.m0 + m >= ld) continue;
-                    float v[4];
+                for (int h = 0; h < 2; ++h) {
+                    float v[8];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(acc.c[i][j][4 * q + e], kLog2e, -base));
-                        v[e] = at.m0 + m + e < at.m ? (p - (m + e == hit ? 1.0f : 0.0f)) * w : 0.0f;
+                    for (int e = 0; e < 8; ++e) {
+                        const int32_t m = acc.m_of(i, 8 * h + e);
+                        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(acc.c[i][j][8 * h + e], kLog2e, -base));
+                        v[e] = at.m0 + m < at.m ? (p - (m == hit ? 1.0f : 0.0f)) * w : 0.0f;
                     }
-                    uint16_t* to = g + n * ld + at.m0 + m;
+                    const int32_t m = at.m0 + acc.m_of8(i, h);
+                    uint16_t* to = g + n * ld + m;
 #pragma unroll
                     for (int p = 0; p < PG; ++p) {
-                        const u2 x{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])};
-                        *reinterpret_cast<u2*>(to + p * plane) = x;
+                        const u4 x = mat_pack8(v);
+                        const u4 y = mat_exchange(x);  // every lane takes part
+                        if (live && m < ld) *reinterpret_cast<u4*>(to + p * plane) = y;
+                        if (p + 1 < PG)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            v[e] -= __builtin_bit_cast(float, e % 2 ? x[e / 2] & 0xffff0000u : x[e / 2] << 16);
+                            for (int e = 0; e < 8; ++e)
+                                v[e] -= __builtin_bit_cast(float, e % 2 ? x[e / 2] & 0xffff0000u : x[e / 2] << 16);
                     }
                 }
         }
@@ -298,7 +311,7 @@ struct Plan {
     int64_t ld, ld_g, piece;     // columns of x's and w's planes, of G's; the piece's rows of w
     int p, pg;                   // planes of x and w, of G
     bool w_direct;
-    int splits_x, splits_w;      // of dx's contraction over a piece, of dw's over the tokens
+    MatDeal deal_x, deal_w;      // dx's contraction over a piece, dw's over the tokens
     size_t x, row, count, logit, sums, part, w, g, partial, partial_w, total;
 };
 
@@ -308,14 +321,14 @@ constexpr int64_t kTileM = 128;  // the smaller shape's: how many partial result
 // Few tokens: the products' time is the weights' bytes, and G takes a second plane.
 constexpr int64_t kTwoPlaneTokens = 128;
 
-Plan plan_of(const Tuning& tune, int type, const void* w, int64_t ld_w, int64_t tokens, int64_t dim, int64_t vocab, bool back) {
+Plan plan_of(const mimir_ctx* ctx, int type, const void* w, int64_t ld_w, int64_t tokens, int64_t dim, int64_t vocab, bool back) {
     Plan p{};
     p.ld = mat_round(dim, 8);
     p.p = type == MIMIR_NUM_BF16 ? 1 : 3;
     p.pg = p.p == 3 ? 3 : tokens <= kTwoPlaneTokens ? 2 : 1;
     p.w_direct = type == MIMIR_NUM_BF16 && mat_direct(w, ld_w, dim);
     const int64_t of_row = (back ? tokens * p.pg * 2 : 0) + (p.w_direct ? 0 : p.ld * p.p * 2);
-    if (tune.mat_piece > 0) p.piece = mat_round(tune.mat_piece, 8);
+    if (ctx->tune.mat_piece > 0) p.piece = mat_round(ctx->tune.mat_piece, 8);
     else p.piece = of_row ? std::max<int64_t>(256, kPieceBytes / of_row / 256 * 256) : vocab;
     p.piece = std::min({p.piece, mat_round(vocab, 8), int64_t{1} << 19});  // G's rows are within the operands' strides
     p.ld_g = mat_round(p.piece, 8);
@@ -331,14 +344,19 @@ Plan plan_of(const Tuning& tune, int type, const void* w, int64_t ld_w, int64_t 
     p.w = take(p.w_direct ? 0 : static_cast<size_t>(p.p * p.piece * p.ld * 2));
     if (back) {
         p.g = take(static_cast<size_t>(p.pg * tokens * p.ld_g * 2));
-        const auto splits = [&](int64_t m, int64_t n, int64_t k) {
-            return p.p == 3 ? mat_splits<MatSmall<3, 3, kCols, kRows>>(m, n, k, 1) : mat_splits<MatSmall<1, 1, kCols, kRows>>(m, n, k, 1);
-        };
-        const int64_t piece = std::min(p.piece, vocab), ld = mat_round(dim, 4);
-        p.splits_x = splits(dim, tokens, piece);
-        p.splits_w = splits(dim, piece, tokens);
-        p.partial = take(p.splits_x > 1 || p.piece < vocab ? static_cast<size_t>(p.splits_x * tokens * ld * 4) : 0);
-        p.partial_w = take(p.splits_w > 1 ? static_cast<size_t>(p.splits_w * piece * ld * 4) : 0);
+        const int64_t piece = std::min(p.piece, vocab);
+        if (p.p == 3) {
+            p.deal_x = mat_deal<3, 3, kCols, kRows>(ctx, dim, tokens, piece, 1, p.piece < vocab);
+            p.deal_w = mat_deal<3, 3, kCols, kCols>(ctx, dim, piece, tokens, 1, false);
+        } else if (p.pg == 2) {
+            p.deal_x = mat_deal<1, 2, kCols, kRows>(ctx, dim, tokens, piece, 1, p.piece < vocab);
+            p.deal_w = mat_deal<1, 2, kCols, kCols>(ctx, dim, piece, tokens, 1, false);
+        } else {
+            p.deal_x = mat_deal<1, 1, kCols, kRows>(ctx, dim, tokens, piece, 1, p.piece < vocab);
+            p.deal_w = mat_deal<1, 1, kCols, kCols>(ctx, dim, piece, tokens, 1, false);
+        }
+        p.partial = take(p.deal_x.partial);
+        p.partial_w = take(p.deal_w.partial);
     } else {
         p.logit = take(static_cast<size_t>(tokens * 4));
         p.sums = take(static_cast<size_t>((tokens + kFinishTokens - 1) / kFinishTokens * 8));
@@ -399,7 +417,7 @@ MatArgs args_of(const MatOperand& a, const MatOperand& b, int64_t m, int64_t n, 
     g.m = static_cast<int32_t>(m);
     g.n = static_cast<int32_t>(n);
     g.k = static_cast<int32_t>(k);
-    g.segments = g.batches = g.splits = 1;
+    g.segments = g.batches = 1;
     return g;
 }
 
@@ -479,7 +497,6 @@ int backward(mimir_ctx* ctx, const Call& c, const Plan& p, char* work, const Gra
     ox.row = row;
     ox.partial = reinterpret_cast<float*>(work + p.partial);
     ox.ld_partial = mat_round(c.dim, 4);
-    ox.slice = c.tokens * ox.ld_partial;
     ox.count = d.mean ? d.mean + 1 : nullptr;
     ox.alpha = d.scale;
     ox.bf16 = bf16;
@@ -487,7 +504,6 @@ int backward(mimir_ctx* ctx, const Call& c, const Plan& p, char* work, const Gra
     MatOut ow = ox;
     ow.row = nullptr;
     ow.partial = reinterpret_cast<float*>(work + p.partial_w);
-    ow.slice = std::min(p.piece, c.vocab) * ow.ld_partial;
     ow.ld = d.ld_dw;
     ow.accumulate = d.accumulate_w;
     ow.last = 1;
@@ -510,14 +526,14 @@ int backward(mimir_ctx* ctx, const Call& c, const Plan& p, char* work, const Gra
             g.n_dev = count;
             ox.read_partial = first > 0;
             ox.last = first + rows >= c.vocab;
-            st = mat_product<P, PG, kCols, kRows>(ctx, "cross entropy dx", g, ox, p.splits_x);
+            st = mat_product<P, PG, kCols, kRows>(ctx, "cross entropy dx", g, ox, p.deal_x);
             if (st) return st;
         }
         if (d.dw) {
             g = args_of(x, gr, c.dim, rows, c.tokens);
             if (c.tokens > 0) g.k_dev = count;
             ow.out[0] = static_cast<char*>(d.dw) + first * d.ld_dw * size;
-            st = mat_product<P, PG, kCols, kCols>(ctx, "cross entropy dw", g, ow, p.splits_w);
+            st = mat_product<P, PG, kCols, kCols>(ctx, "cross entropy dw", g, ow, p.deal_w);
             if (st) return st;
         }
     }
@@ -540,7 +556,7 @@ int mimir_linear_cross_entropy_fwd(mimir_ctx* ctx, int type, const void* x, int6
     MIMIR_ENTER(ctx);
     if (tokens > 0 && few_applies(c))
         return type == MIMIR_NUM_F32 ? forward_few<true>(ctx, c, loss, lse, mean) : forward_few<false>(ctx, c, loss, lse, mean);
-    const Plan p = plan_of(ctx->tune, type, w, ld_w, tokens, dim, vocab, false);
+    const Plan p = plan_of(ctx, type, w, ld_w, tokens, dim, vocab, false);
     char* work;
     if (int st = mat_scratch(ctx, p.total, &work)) return st;
     auto* count = reinterpret_cast<int32_t*>(work + p.count);
@@ -566,7 +582,7 @@ int mimir_linear_cross_entropy_bwd(mimir_ctx* ctx, int type, const void* x, int6
     MIMIR_REQUIRE(ctx, dx != x || ld_dx == ld_x, "%s: dx in place needs equal strides", what);
     if (!dx && !dw) return MIMIR_OK;
     MIMIR_ENTER(ctx);
-    Plan p = plan_of(ctx->tune, type, w, ld_w, tokens, dim, vocab, true);
+    Plan p = plan_of(ctx, type, w, ld_w, tokens, dim, vocab, true);
     char* work;
     if (int st = mat_scratch(ctx, p.total, &work)) return st;
     auto* count = reinterpret_cast<int32_t*>(work + p.count);

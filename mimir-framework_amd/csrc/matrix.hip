@@ -17,15 +17,16 @@ __global__ __launch_bounds__(kBlock) void stage_rows(const void* src, int64_t ro
     }
 }
 
-__global__ __launch_bounds__(kBlock) void join_slices(MatOut o, MatArgs g) {
-    const int64_t n = g.n_dev ? min(g.n, *g.n_dev) : g.n;
+__global__ __launch_bounds__(kBlock) void join_slices(MatOut o, MatArgs g, int bm, int bn) {
+    const int64_t n = g.n_dev ? min(g.n, *g.n_dev) : g.n, slice = n * o.ld_partial;
+    const int32_t splits = g.splits_of(((g.m + bm - 1) / bm) * ((n + bn - 1) / bn));
     const float by = o.factor();
     const int64_t of_row = (g.m + 3) / 4, one = n * of_row, stride = static_cast<int64_t>(gridDim.x) * kBlock;
     for (int64_t i = static_cast<int64_t>(blockIdx.x) * kBlock + threadIdx.x; i < one * g.batches; i += stride) {
         const int64_t batch = i / one, r = i % one / of_row, c = i % one % of_row * 4;
-        const float* p = o.partial + batch * o.slice + r * o.ld_partial + c;
+        const float* p = o.partial + batch * slice + r * o.ld_partial + c;
         f4 v{};
-        for (int s = 0; s < g.splits; ++s) v += *reinterpret_cast<const f4*>(p + s * g.batches * o.slice);
+        for (int s = 0; s < splits; ++s) v += *reinterpret_cast<const f4*>(p + s * g.batches * slice);
         o.put(static_cast<int>(batch), r, static_cast<int32_t>(c), g.m, v, by);
     }
 }
@@ -46,9 +47,9 @@ int mimir::mat_stage(mimir_ctx* ctx, int type, const void* src, int64_t rows, in
     return launched(ctx, "stage_rows");
 }
 
-int mimir::mat_join(mimir_ctx* ctx, const MatOut& o, const MatArgs& g) {
+int mimir::mat_join(mimir_ctx* ctx, const MatOut& o, const MatArgs& g, int bm, int bn) {
     if (g.n == 0 || g.m == 0) return MIMIR_OK;
-    join_slices<<<grid_of(static_cast<int64_t>(g.n) * ((g.m + 3) / 4) * g.batches), kBlock, 0, ctx->stream>>>(o, g);
+    join_slices<<<grid_of(static_cast<int64_t>(g.n) * ((g.m + 3) / 4) * g.batches), kBlock, 0, ctx->stream>>>(o, g, bm, bn);
     return launched(ctx, "join_slices");
 }
 

@@ -53,12 +53,20 @@ struct MatArgs {
     int32_t m, n, k;        // k of one segment
     const int32_t* n_dev;   // not null: n is at most this
     const int32_t* k_dev;   // not null: k is at most this
-    int32_t segments, batches, splits;
+    int32_t segments, batches;
+    // How many ways the contraction is split: as many as leave the tiles' workgroups at
+    // `fill` (n may be known on the device alone), at most `splits`.  0: once.
+    int32_t fill, splits;
+
+    __host__ __device__ int32_t splits_of(int64_t tiles) const {
+        const int64_t s = fill / (tiles > 0 ? tiles * batches : 1);
+        return fill == 0 || s < 1 ? 1 : s < splits ? static_cast<int32_t>(s) : splits;
+    }
 };
 
 struct MatAt {
     int32_t m0, n0, m, n;  // the tile's first, and the limits
-    int32_t batch, split, tile_m;
+    int32_t batch, split, splits, tile_m;
     int32_t slice;  // split * batches + batch
 };
 
@@ -218,7 +226,9 @@ __device__ __forceinline__ bool mat_tile_of(const MatArgs& g, MatAt* at) {
     at->m = g.m;
     at->n = g.n_dev ? __builtin_amdgcn_readfirstlane(min(g.n, *g.n_dev)) : g.n;
     const uint32_t tiles_m = (g.m + S::kM / S::kSubs - 1) / (S::kM / S::kSubs), tiles_n = (at->n + S::kN - 1) / S::kN;
-    const uint32_t one = tiles_m * tiles_n, total = one * g.batches * g.splits;
+    const uint32_t one = tiles_m * tiles_n;
+    at->splits = g.splits_of(one);
+    const uint32_t total = one * g.batches * at->splits;
     const uint32_t per = (total + kMatXcds - 1) / kMatXcds;
     const uint32_t i = (blockIdx.x % kMatXcds) * per + blockIdx.x / kMatXcds;
     if (blockIdx.x / kMatXcds >= per || i >= total) return false;
@@ -248,6 +258,10 @@ struct MatAcc {
     __device__ __forceinline__ int m_of(int i, int r) const {
         return row(i) + 8 * (r / 4) + 4 * (threadIdx.x % kWave / 32) + r % 4;
     }
+    // First m of the eight that a lane has of registers 8 h .. + 7 after mat_exchange.
+    __device__ __forceinline__ int m_of8(int i, int h) const {
+        return row(i) + 16 * h + 8 * (threadIdx.x % kWave / 32);
+    }
     __device__ __forceinline__ int n_of(int j) const { return col(j) + threadIdx.x % 32; }
 };
 
@@ -255,6 +269,18 @@ struct MatAcc {
 // after it; loads still out stay out (__syncthreads would wait for them).
 __device__ __forceinline__ void mat_barrier() {
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" : : : "memory");
+}
+
+// Eight registers of a block as bf16, in their order.
+__device__ __forceinline__ u4 mat_pack8(const float* v) {
+    return u4{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7])};
+}
+// mat_pack8's values, four of them m 4 hf .. and four 8 + 4 hf .. of a row, as eight
+// consecutive ones: the half waves trade (hf: lane / 32).
+__device__ __forceinline__ u4 mat_exchange(u4 x) {
+    const auto a = __builtin_amdgcn_permlane32_swap(x[0], x[2], false, false);
+    const auto b = __builtin_amdgcn_permlane32_swap(x[1], x[3], false, false);
+    return u4{a[0], b[0], a[1], b[1]};
 }
 
 // Reads spread between the products of the chunk before.
@@ -290,8 +316,8 @@ __global__ __launch_bounds__(S::kThreads, S::kThreads == 512 ? 2 : 1) void mat_k
     tb.init(g.b[0].ld, at.n - at.n0);
     // Steps of this workgroup: the split's share of all segments' steps.
     const int32_t of_one = (k + S::kK - 1) / S::kK, all = of_one * g.segments;
-    const int32_t begin = static_cast<int32_t>(static_cast<int64_t>(all) * at.split / g.splits);
-    const int32_t end = static_cast<int32_t>(static_cast<int64_t>(all) * (at.split + 1) / g.splits);
+    const int32_t begin = static_cast<int32_t>(static_cast<int64_t>(all) * at.split / at.splits);
+    const int32_t end = static_cast<int32_t>(static_cast<int64_t>(all) * (at.split + 1) / at.splits);
     const uint32_t base = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)lds));
     const uint32_t next_a = __builtin_amdgcn_readfirstlane(TileA::next_of(g.a[0].ld));
     const uint32_t next_b = __builtin_amdgcn_readfirstlane(TileB::next_of(g.b[0].ld));
@@ -420,7 +446,8 @@ inline bool mat_ld_fits(int64_t ld) { return ld < (int64_t{1} << 20); }
 
 template <class S, class Epi>
 int mat_launch(mimir_ctx* ctx, const char* what, const MatArgs& g, const Epi& epi) {
-    const int64_t total = mat_tiles<S>(g) * g.splits;
+    // Fewer n than there may be have fewer tiles and more splits: `fill` workgroups at most.
+    const int64_t tiles = mat_tiles<S>(g), total = tiles ? std::max<int64_t>(tiles, g.fill) : 0;
     const int64_t grid = (total + kMatXcds - 1) / kMatXcds * kMatXcds;
     if (total == 0) return MIMIR_OK;
     MIMIR_REQUIRE(ctx, dispatch_fits(grid, S::kThreads), "%s: grid of %lld workgroups exceeds the limit", what, (long long)grid);
@@ -652,7 +679,7 @@ struct MatOut {
     int64_t ld;
     const int32_t* row;       // not null: the row of n
     float* partial;           // [splits][batches][n][ld_partial], not null if read or written
-    int64_t ld_partial, slice;
+    int64_t ld_partial;
     const float* count;       // not null: alpha is divided by max(count, 1)
     float alpha;
     int32_t bf16, accumulate;
@@ -694,13 +721,41 @@ struct MatOut {
             if (m + e < limit) p[e] = accumulate ? v[e] * by + p[e] : v[e] * by;
     }
 
+    // Eight consecutive bf16 of a row, nothing to add.
+    __device__ __forceinline__ void put8(int batch, int64_t n, int32_t m, int32_t limit, u4 v) const {
+        uint16_t* p = static_cast<uint16_t*>(out[batch]) + (row ? row[n] : n) * ld + m;
+        if (m + 8 <= limit) {
+            *reinterpret_cast<u4e*>(p) = v;
+            return;
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (m + e < limit) p[e] = static_cast<uint16_t>(v[e / 2] >> (16 * (e % 2)));
+    }
+
     template <class S>
     __device__ __forceinline__ void run(const MatAt& at, MatAcc<S>& acc, char*) const {
         const float by = factor();
+        const int64_t slice = at.n * ld_partial;
+        const bool plain = bf16 && last && !read_partial && !accumulate;
 #pragma unroll
         for (int j = 0; j < S::kBn; ++j) {
             const int32_t n = at.n0 + acc.n_of(j);
-            if (n >= at.n) continue;
+            const bool live = n < at.n;
+            if (plain) {
+#pragma unroll
+                for (int i = 0; i < S::kBm; ++i)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        float v[8];
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) v[e] = acc.c[i][j][8 * h + e] * by;
+                        const u4 x = mat_exchange(mat_pack8(v));
+                        if (live) put8(at.batch, n, at.m0 + acc.m_of8(i, h), at.m, x);
+                    }
+                continue;
+            }
+            if (!live) continue;
 #pragma unroll
             for (int i = 0; i < S::kBm; ++i)
 #pragma unroll
@@ -765,39 +820,71 @@ __device__ __forceinline__ void mat_stage8(const void* src, int64_t at, int64_t 
 // between planes.
 int mat_stage(mimir_ctx* ctx, int type, const void* src, int64_t rows, int64_t cols, int64_t ld, uint16_t* dst, int64_t ld_dst,
               int64_t plane);
-// The sum of the splits' slices into out (MatOut's fields say how) for a product of g.
-int mat_join(mimir_ctx* ctx, const MatOut& o, const MatArgs& g);
+// A product into MatOut: its shape, and how its contraction is dealt to workgroups where
+// the tiles of C alone leave CUs idle.
+struct MatDeal {
+    bool big;
+    int32_t fill, splits;
+    size_t partial;  // bytes of the slices
+};
 
-// How many workgroups a contraction of `k` is dealt to where the tiles of C alone
-// leave CUs idle: about two for each CU, at least four steps each.
-template <class SMALL>
-int mat_splits(int64_t m, int64_t n, int64_t k, int64_t batches) {
-    const int64_t tiles = (m + SMALL::kM - 1) / SMALL::kM * ((n + SMALL::kN - 1) / SMALL::kN) * batches;
-    const int64_t steps = (k + SMALL::kK - 1) / SMALL::kK;
-    const int64_t s = std::min(512 / std::max<int64_t>(tiles, 1), steps / 4);
-    return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(s, 64)));
+// The larger tiles where they fill the GPU, or, the contraction split, come to 1 for
+// each CU; else the smaller ones, split to 2 for each CU.  A split has at least 512 of
+// the contraction.  `more`: the sums go through fp32 slices whether split or not.
+template <class BIG, class SMALL, bool HAS_BIG>
+MatDeal mat_deal(const mimir_ctx* ctx, int64_t m, int64_t n, int64_t k, int64_t batches, bool more) {
+    constexpr int32_t kBigFill = 256, kSmallFill = 512;
+    constexpr int64_t kLeastK = 512;
+    const auto tiles = [&](int64_t bm, int64_t bn) { return (m + bm - 1) / bm * ((n + bn - 1) / bn) * batches; };
+    const int64_t big = tiles(BIG::kM, BIG::kN), most = std::max<int64_t>(1, k / kLeastK);
+    const int64_t big_most = std::max<int64_t>(1, kBigFill / std::max<int64_t>(big, 1));
+    MatDeal d{};
+    d.big = HAS_BIG && (ctx->tune.mat_big >= 0 ? ctx->tune.mat_big == 1 : big * std::min(most, big_most) >= kMatBigTiles);
+    d.fill = d.big ? kBigFill : kSmallFill;
+    d.splits = static_cast<int32_t>(std::min<int64_t>(most, 64));
+    const int64_t now = tiles(d.big ? BIG::kM : SMALL::kM, d.big ? BIG::kN : SMALL::kN);
+    // n on the device may be smaller than here: then there are more splits, but no more
+    // tiles' worth of sums than `fill`.
+    if (d.splits == 1 || now >= d.fill) d.splits = 1, d.fill = 0;
+    const int64_t ld = mat_round(m, 4);
+    if (d.splits > 1)
+        d.partial = sizeof(float) * static_cast<size_t>(d.fill * (d.big ? int64_t{BIG::kM} * BIG::kN : int64_t{SMALL::kM} * SMALL::kN) + 4);
+    if (more || d.splits > 1) d.partial = std::max(d.partial, sizeof(float) * static_cast<size_t>(n * ld * batches));
+    return d;
+}
+template <int PA, int PB, int KA, int KB>
+MatDeal mat_deal(const mimir_ctx* ctx, int64_t m, int64_t n, int64_t k, int64_t batches, bool more) {
+    using S = MatSmall<PA, PB, KA, KB>;
+    if constexpr (PA == PB) return mat_deal<MatBig<PA, PB, KA, KB>, S, true>(ctx, m, n, k, batches, more);
+    else return mat_deal<S, S, false>(ctx, m, n, k, batches, more);
 }
 
-// C as a result, in the shape that fits, split `splits` ways.  o.last: these are the
-// contraction's last pieces.  PA, PB: planes.
+// The sum of the splits' slices into out (MatOut's fields say how) for a product of g in
+// tiles of bm x bn.
+int mat_join(mimir_ctx* ctx, const MatOut& o, const MatArgs& g, int bm, int bn);
+
+// C as a result.  o.last: these are the contraction's last pieces.
 template <int PA, int PB, int KA, int KB>
-int mat_product(mimir_ctx* ctx, const char* what, MatArgs g, MatOut o, int splits) {
-    g.splits = splits;
+int mat_product(mimir_ctx* ctx, const char* what, MatArgs g, MatOut o, const MatDeal& d) {
+    g.splits = d.splits;
+    g.fill = d.fill;
     const int32_t last = o.last;
-    if (splits > 1) o.last = 0;
+    if (d.splits > 1) o.last = 0;
     int st = MIMIR_OK;
-    bool done = false;
+    using S = MatSmall<PA, PB, KA, KB>;
+    int bm = S::kM, bn = S::kN;
     if constexpr (PA == PB) {
         using B = MatBig<PA, PB, KA, KB>;
-        if (splits == 1 && mat_fills<B>(ctx, g)) {
+        if (d.big) {
+            bm = B::kM;
+            bn = B::kN;
             st = mat_launch<B>(ctx, what, g, o);
-            done = true;
         }
     }
-    if (!done) st = mat_launch<MatSmall<PA, PB, KA, KB>>(ctx, what, g, o);
-    if (st || splits == 1 || !last) return st;
+    if (!d.big) st = mat_launch<S>(ctx, what, g, o);
+    if (st || d.splits == 1 || !last) return st;
     o.last = 1;
-    return mat_join(ctx, o, g);
+    return mat_join(ctx, o, g, bm, bn);
 }
 
 // The context's scratch of at least `bytes`, also while its stream is being captured:

@@ -105,6 +105,7 @@ struct GradArgs {
     int64_t ld_dy;
     uint16_t* out;         // planes of [tokens][2 * cols_out]: dg, then du
     int64_t tokens, cols, cols_out, plane;
+    float* raw;            // also as they are, dg [tokens][cols] then du, or null
 };
 
 // Eight columns a thread; columns from `cols` on are zeros.
@@ -156,6 +157,15 @@ __global__ __launch_bounds__(kBlock) void gated_grad(GradArgs a) {
             du[e] = d[e] * s[0];
             dg[e] = d[e] * u[e] * s[1];
         }
+        if (PG == 3 && a.raw) {
+            float* to = a.raw + t * a.cols + c;
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                if (4 * h + 4 <= left) {
+                    *reinterpret_cast<f4u*>(to + 4 * h) = f4u{dg[4 * h], dg[4 * h + 1], dg[4 * h + 2], dg[4 * h + 3]};
+                    *reinterpret_cast<f4u*>(to + a.tokens * a.cols + 4 * h) = f4u{du[4 * h], du[4 * h + 1], du[4 * h + 2], du[4 * h + 3]};
+                }
+        }
         uint16_t* to = a.out + t * 2 * a.cols_out + c;
         const Split8 x = split8(dg), y = split8(du);
         const u4 xs[3] = {x.h, x.m, x.l}, ys[3] = {y.h, y.m, y.l};
@@ -183,10 +193,20 @@ struct Call {
 struct Plan {
     int p, pg;
     int64_t ld_x, piece, ld_w;  // columns of x's planes; a piece's columns of the weights, their planes' columns
-    bool x_direct, w_direct;
+    bool x_direct, w_direct, few;
     MatDeal deal_x, deal_w;
-    size_t x, w, g, partial, partial_w, total;
+    size_t x, w, g, raw, partial, partial_w, total;
 };
+
+// Few tokens, weights that can be read as they are.
+bool few_weights(const Call& c) {
+    const bool fp32 = c.type == MIMIR_NUM_F32;
+    return c.tokens <= kFewN && c.hidden <= (1 << 18) && few_direct(fp32, c.w[0], c.ld_w, c.hidden) &&
+           few_direct(fp32, c.w[1], c.ld_w, c.hidden);
+}
+// And their rows of x: the forward is one launch.
+bool few_applies(const Call& c) { return few_weights(c) && few_direct(c.type == MIMIR_NUM_F32, c.x, c.ld_x, c.dim); }
+
 
 Plan plan_of(const mimir_ctx* ctx, const Call& c, bool back) {
     Plan p{};
@@ -195,10 +215,12 @@ Plan plan_of(const mimir_ctx* ctx, const Call& c, bool back) {
     p.x_direct = p.p == 1 && mat_direct(c.x, c.ld_x, c.dim);
     p.w_direct = p.p == 1 && mat_direct(c.w[0], c.ld_w, c.hidden) && mat_direct(c.w[1], c.ld_w, c.hidden);
     p.ld_x = mat_round(c.dim, 8);
+    // fp32: the weights' planes would be five times their bytes on the way.
+    p.few = back && p.p == 3 && few_weights(c);
     const int64_t of_column = (back ? c.tokens * p.pg * 4 : 0) + (p.w_direct ? 0 : c.dim * p.p * 4);
     if (ctx->tune.mat_piece > 0) p.piece = mat_round(ctx->tune.mat_piece, 8);
     else p.piece = of_column ? std::max<int64_t>(256, kPieceBytes / of_column / 256 * 256) : c.hidden;
-    p.piece = std::min({p.piece, mat_round(c.hidden, 8), int64_t{1} << 18});
+    p.piece = std::min({p.few ? c.hidden + 8 : p.piece, mat_round(c.hidden, 8), int64_t{1} << 18});
     p.ld_w = p.piece;
     size_t at = 0;
     const auto take = [&](size_t bytes) {
@@ -207,7 +229,7 @@ Plan plan_of(const mimir_ctx* ctx, const Call& c, bool back) {
         return was;
     };
     p.x = take(p.x_direct ? 0 : static_cast<size_t>(p.p * c.tokens * p.ld_x * 2));
-    p.w = take(p.w_direct ? 0 : static_cast<size_t>(2 * p.p * c.dim * p.ld_w * 2));
+    p.w = take(p.w_direct || p.few ? 0 : static_cast<size_t>(2 * p.p * c.dim * p.ld_w * 2));
     if (back) {
         p.g = take(static_cast<size_t>(p.pg * c.tokens * 2 * p.piece * 2));
         const int64_t piece = std::min(p.piece, c.hidden);
@@ -220,6 +242,11 @@ Plan plan_of(const mimir_ctx* ctx, const Call& c, bool back) {
         } else {
             p.deal_x = mat_deal<1, 1, kRows, kRows>(ctx, c.dim, c.tokens, 2 * piece, 1, p.piece < c.hidden);
             p.deal_w = mat_deal<1, 1, kCols, kCols>(ctx, piece, c.dim, c.tokens, 2, false);
+        }
+        if (p.few) {
+            p.raw = take(static_cast<size_t>(2 * c.tokens * c.hidden * 4));
+            p.deal_x.splits = few_splits<true, kRows>(c.dim, c.hidden, 2);
+            p.deal_x.partial = static_cast<size_t>(2 * p.deal_x.splits * c.tokens * mat_round(c.dim, 4) * 4);
         }
         p.partial = take(p.deal_x.partial);
         p.partial_w = take(p.deal_w.partial);
@@ -271,7 +298,7 @@ MatArgs args_of(int64_t m, int64_t n, int64_t k) {
     g.m = static_cast<int32_t>(m);
     g.n = static_cast<int32_t>(n);
     g.k = static_cast<int32_t>(k);
-    g.segments = g.batches = 1;
+    g.segments = g.batches = g.splits = 1;
     return g;
 }
 
@@ -297,13 +324,6 @@ int forward(mimir_ctx* ctx, const Call& c, const Plan& p, char* work, void* y, i
         if (st) return st;
     }
     return MIMIR_OK;
-}
-
-// Few tokens, operands that can be read as they are: one launch.
-bool few_applies(const Call& c) {
-    const bool fp32 = c.type == MIMIR_NUM_F32;
-    return c.tokens <= kFewN && few_direct(fp32, c.x, c.ld_x, c.dim) && few_direct(fp32, c.w[0], c.ld_w, c.hidden) &&
-           few_direct(fp32, c.w[1], c.ld_w, c.hidden);
 }
 
 template <bool FP32, int ACT>
@@ -357,7 +377,7 @@ int backward(mimir_ctx* ctx, const Call& c, const Plan& p, char* work, const Gra
     for (int64_t first = 0; first < c.hidden; first += p.piece) {
         const int64_t cols = std::min(p.piece, c.hidden - first);
         const GradArgs a{d.gate_up ? d.gate_up + first : nullptr, c.hidden, static_cast<const char*>(d.dy) + first * size, d.ld_dy,
-                         planes, c.tokens, cols, p.piece, plane};
+                         planes, c.tokens, cols, p.piece, plane, p.few ? reinterpret_cast<float*>(work + p.raw) : nullptr};
         if (c.tokens > 0) {
             const int64_t blocks = (c.tokens * (p.piece / 8) + kBlock - 1) / kBlock;
             const auto grid = static_cast<unsigned>(std::min<int64_t>(blocks, 1 << 16));
@@ -367,13 +387,23 @@ int backward(mimir_ctx* ctx, const Call& c, const Plan& p, char* work, const Gra
         const MatOperand dg{planes, ld_g, plane}, du{planes + p.piece, ld_g, plane};
         if (d.dx) {
             MatArgs g = args_of(c.dim, c.tokens, cols);
-            if (int st = weights(ctx, c, p, work, first, cols, g.a)) return st;
-            g.b[0] = dg;
-            g.b[1] = du;
-            g.segments = 2;
             ox.read_partial = first > 0;
             ox.last = first + cols >= c.hidden;
-            if (int st = mat_product<P, PG, kRows, kRows>(ctx, "gated dx", g, ox, p.deal_x)) return st;
+            g.segments = 2;
+            int st = MIMIR_OK;
+            if (P == 3 && p.few) {
+                for (int i = 0; i < 2; ++i) {
+                    g.a[i] = MatOperand{static_cast<const uint16_t*>(c.w[i]), c.ld_w, 0};
+                    g.b[i] = MatOperand{reinterpret_cast<const uint16_t*>(a.raw + i * c.tokens * c.hidden), c.hidden, 0};
+                }
+                g.splits = p.deal_x.splits;
+                if constexpr (P == 3) st = few_product<true, kRows>(ctx, "gated dx", g, ox);
+            } else if (st = weights(ctx, c, p, work, first, cols, g.a); st == MIMIR_OK) {
+                g.b[0] = dg;
+                g.b[1] = du;
+                st = mat_product<P, PG, kRows, kRows>(ctx, "gated dx", g, ox, p.deal_x);
+            }
+            if (st) return st;
         }
         if (d.dw[0]) {
             MatArgs g = args_of(cols, c.dim, c.tokens);

@@ -46,6 +46,7 @@ struct GatherArgs {
     int64_t tokens, dim, vocab;
     uint16_t* dst;       // planes of [tokens][ld_dst]
     int64_t ld_dst, plane;
+    float* raw;          // the rows as they are [tokens][dim] too (fp32, dim a multiple of 4), or null
     int32_t* row;        // [tokens]: the token of each gathered row
     int32_t* count;      // and a counter for ce_finish, zeroed
     float* zero_a;       // of tokens without a target: loss and lse, or null
@@ -92,6 +93,8 @@ __global__ __launch_bounds__(kBlock) void gather_rows(GatherArgs a) {
 #pragma unroll 4
         for (int64_t c = 8 * lane; c < a.ld_dst; c += 8 * kWave)
             mat_stage8<BF16>(a.x, t * a.ld_x + c, a.dim - c, a.dst + at * a.ld_dst + c, a.plane);
+        if (!BF16 && a.raw)
+            for (int64_t c = lane; c < a.dim; c += kWave) a.raw[at * a.dim + c] = static_cast<const float*>(a.x)[t * a.ld_x + c];
         return;
     }
     if (lane == 0 && a.zero_a) a.zero_a[t] = 0.0f, a.zero_b[t] = 0.0f;
@@ -267,6 +270,8 @@ struct CeGrad {
     const float* dloss;  // null: 1
     uint16_t* g;
     int64_t ld, plane, first;
+    float* raw;          // G as it is too, [n][ld_raw], zeros from m on, or null
+    int64_t ld_raw;
 
     template <class S>
     __device__ __forceinline__ void run(const MatAt& at, MatAcc<S>& acc, char*) const {
@@ -288,6 +293,11 @@ struct CeGrad {
                         const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(acc.c[i][j][8 * h + e], kLog2e, -base));
                         v[e] = at.m0 + m < at.m ? (p - (m == hit ? 1.0f : 0.0f)) * w : 0.0f;
                     }
+                    if (PG == 3 && raw && live)
+#pragma unroll
+                        for (int q = 0; q < 2; ++q)
+                            if (const int32_t m = at.m0 + acc.m_of(i, 8 * h + 4 * q); m < ld_raw)
+                                *reinterpret_cast<f4*>(raw + n * ld_raw + m) = f4{v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]};
                     const int32_t m = at.m0 + acc.m_of8(i, h);
                     uint16_t* to = g + n * ld + m;
 #pragma unroll
@@ -310,11 +320,12 @@ struct CeGrad {
 struct Plan {
     int64_t ld, ld_g, piece;     // columns of x's and w's planes, of G's; the piece's rows of w
     int p, pg;                   // planes of x and w, of G
-    bool w_direct;
+    bool w_direct, few;
     MatDeal deal_x, deal_w;      // dx's contraction over a piece, dw's over the tokens
-    size_t x, row, count, logit, sums, part, w, g, partial, partial_w, total;
+    size_t x, raw_x, row, count, logit, sums, part, w, g, raw_g, partial, partial_w, total;
 };
 
+constexpr int kFewBlocks = 2;  // of 32 rows of w, a workgroup's with few tokens
 constexpr int64_t kPieceBytes = int64_t{512} << 20;
 constexpr int64_t kTileM = 128;  // the smaller shape's: how many partial results a token has at most
 
@@ -327,10 +338,12 @@ Plan plan_of(const mimir_ctx* ctx, int type, const void* w, int64_t ld_w, int64_
     p.p = type == MIMIR_NUM_BF16 ? 1 : 3;
     p.pg = p.p == 3 ? 3 : tokens <= kTwoPlaneTokens ? 2 : 1;
     p.w_direct = type == MIMIR_NUM_BF16 && mat_direct(w, ld_w, dim);
+    // Few tokens in fp32: w's planes would be five times its bytes on the way.
+    p.few = back && p.p == 3 && tokens <= kFewN && vocab <= (1 << 18) && few_direct(true, w, ld_w, dim);
     const int64_t of_row = (back ? tokens * p.pg * 2 : 0) + (p.w_direct ? 0 : p.ld * p.p * 2);
     if (ctx->tune.mat_piece > 0) p.piece = mat_round(ctx->tune.mat_piece, 8);
     else p.piece = of_row ? std::max<int64_t>(256, kPieceBytes / of_row / 256 * 256) : vocab;
-    p.piece = std::min({p.piece, mat_round(vocab, 8), int64_t{1} << 19});  // G's rows are within the operands' strides
+    p.piece = std::min({p.few ? vocab + 8 : p.piece, mat_round(vocab, 8), int64_t{1} << 19});  // G's rows are within the operands' strides
     p.ld_g = mat_round(p.piece, 8);
     size_t at = 0;
     const auto take = [&](size_t bytes) {
@@ -341,7 +354,7 @@ Plan plan_of(const mimir_ctx* ctx, int type, const void* w, int64_t ld_w, int64_
     p.x = take(static_cast<size_t>(p.p * tokens * p.ld * 2));
     p.row = take(static_cast<size_t>(tokens * 4));
     p.count = take(8);
-    p.w = take(p.w_direct ? 0 : static_cast<size_t>(p.p * p.piece * p.ld * 2));
+    p.w = take(p.w_direct || p.few ? 0 : static_cast<size_t>(p.p * p.piece * p.ld * 2));
     if (back) {
         p.g = take(static_cast<size_t>(p.pg * tokens * p.ld_g * 2));
         const int64_t piece = std::min(p.piece, vocab);
@@ -354,6 +367,12 @@ Plan plan_of(const mimir_ctx* ctx, int type, const void* w, int64_t ld_w, int64_
         } else {
             p.deal_x = mat_deal<1, 1, kCols, kRows>(ctx, dim, tokens, piece, 1, p.piece < vocab);
             p.deal_w = mat_deal<1, 1, kCols, kCols>(ctx, dim, piece, tokens, 1, false);
+        }
+        if (p.few) {
+            p.raw_x = take(static_cast<size_t>(tokens * dim * 4));
+            p.raw_g = take(static_cast<size_t>(tokens * mat_round(vocab, 4) * 4));
+            p.deal_x.splits = few_splits<true, kCols>(dim, vocab, 1);
+            p.deal_x.partial = static_cast<size_t>(p.deal_x.splits * tokens * mat_round(dim, 4) * 4);
         }
         p.partial = take(p.deal_x.partial);
         p.partial_w = take(p.deal_w.partial);
@@ -417,7 +436,7 @@ MatArgs args_of(const MatOperand& a, const MatOperand& b, int64_t m, int64_t n, 
     g.m = static_cast<int32_t>(m);
     g.n = static_cast<int32_t>(n);
     g.k = static_cast<int32_t>(k);
-    g.segments = g.batches = 1;
+    g.segments = g.batches = g.splits = 1;
     return g;
 }
 
@@ -448,8 +467,6 @@ int forward(mimir_ctx* ctx, const Call& c, const Plan& p, char* work, float* los
 
 // Few tokens, operands that can be read as they are: no token is gathered and no operand
 // staged.
-constexpr int kFewBlocks = 2;
-
 bool few_applies(const Call& c) {
     const bool fp32 = c.type == MIMIR_NUM_F32;
     return c.tokens <= kFewN && few_direct(fp32, c.x, c.ld_x, c.dim) && few_direct(fp32, c.w, c.ld_w, c.dim);
@@ -507,26 +524,41 @@ int backward(mimir_ctx* ctx, const Call& c, const Plan& p, char* work, const Gra
     ow.ld = d.ld_dw;
     ow.accumulate = d.accumulate_w;
     ow.last = 1;
-    CeGrad<PG> e{c.target, row, d.lse, d.dloss, reinterpret_cast<uint16_t*>(work + p.g), p.ld_g, c.tokens * p.ld_g, 0};
+    CeGrad<PG> e{c.target, row, d.lse, d.dloss, reinterpret_cast<uint16_t*>(work + p.g), p.ld_g, c.tokens * p.ld_g, 0,
+                 p.few ? reinterpret_cast<float*>(work + p.raw_g) : nullptr, mat_round(c.vocab, 4)};
+    const bool few = P == 3 && p.few;
+    const auto as_is = [](const void* q, int64_t ld) { return MatOperand{static_cast<const uint16_t*>(q), ld, 0}; };
 
     for (int64_t first = 0; first < c.vocab; first += p.piece) {
         const int64_t rows = std::min(p.piece, c.vocab - first);
-        MatOperand w;
-        if (int st = weights(ctx, c, p, work, first, rows, &w)) return st;
-        MatArgs g = args_of(w, x, rows, c.tokens, c.dim);
+        MatOperand w = as_is(c.w, c.ld_w);
+        if (!few)
+            if (int st = weights(ctx, c, p, work, first, rows, &w)) return st;
+        MatArgs g = args_of(w, few ? as_is(work + p.raw_x, c.dim) : x, rows, c.tokens, c.dim);
         g.n_dev = count;
         e.first = first;
         using BG = MatBig<P, P, kRows, kRows>;
         using SG = MatSmall<P, P, kRows, kRows>;
-        int st = mat_fills<BG>(ctx, g) ? mat_launch<BG>(ctx, "cross entropy gradient", g, e)
-                                               : mat_launch<SG>(ctx, "cross entropy gradient", g, e);
+        int st = MIMIR_OK;
+        if (!few) {
+            st = mat_fills<BG>(ctx, g) ? mat_launch<BG>(ctx, "cross entropy gradient", g, e)
+                                       : mat_launch<SG>(ctx, "cross entropy gradient", g, e);
+        } else if constexpr (P == 3) {
+            st = few_launch<4, kFewBlocks, 3, true, kRows, false>(ctx, "cross entropy gradient", g, e);
+        }
         if (st) return st;
         if (d.dx) {
             g = args_of(w, gr, c.dim, c.tokens, rows);
             g.n_dev = count;
             ox.read_partial = first > 0;
             ox.last = first + rows >= c.vocab;
-            st = mat_product<P, PG, kCols, kRows>(ctx, "cross entropy dx", g, ox, p.deal_x);
+            if (!few) {
+                st = mat_product<P, PG, kCols, kRows>(ctx, "cross entropy dx", g, ox, p.deal_x);
+            } else if constexpr (P == 3) {
+                g.b[0] = as_is(work + p.raw_g, mat_round(c.vocab, 4));
+                g.splits = p.deal_x.splits;
+                st = few_product<true, kCols>(ctx, "cross entropy dx", g, ox);
+            }
             if (st) return st;
         }
         if (d.dw) {
@@ -562,7 +594,7 @@ int mimir_linear_cross_entropy_fwd(mimir_ctx* ctx, int type, const void* x, int6
     auto* count = reinterpret_cast<int32_t*>(work + p.count);
     if (tokens == 0) return mimir_fill_f32(ctx, mean, 2, 0.0f);
     const GatherArgs a{x, ld_x, targets, tokens, dim, vocab, reinterpret_cast<uint16_t*>(work + p.x), p.ld, tokens * p.ld,
-                       reinterpret_cast<int32_t*>(work + p.row), count, loss, lse, nullptr, 0};
+                       nullptr, reinterpret_cast<int32_t*>(work + p.row), count, loss, lse, nullptr, 0};
     if (int st = gather(ctx, c, a)) return st;
     return p.p == 1 ? forward<1>(ctx, c, p, work, loss, lse, mean) : forward<3>(ctx, c, p, work, loss, lse, mean);
 }
@@ -588,7 +620,7 @@ int mimir_linear_cross_entropy_bwd(mimir_ctx* ctx, int type, const void* x, int6
     auto* count = reinterpret_cast<int32_t*>(work + p.count);
     const Gradients d{lse, dloss, mean, scale, dx, ld_dx, dw, ld_dw, accumulate_x ? 1 : 0, accumulate_w ? 1 : 0};
     const GatherArgs a{x, ld_x, targets, tokens, dim, vocab, reinterpret_cast<uint16_t*>(work + p.x), p.ld, tokens * p.ld,
-                       reinterpret_cast<int32_t*>(work + p.row), count, nullptr, nullptr, accumulate_x ? nullptr : dx, ld_dx};
+                       p.few ? reinterpret_cast<float*>(work + p.raw_x) : nullptr, reinterpret_cast<int32_t*>(work + p.row), count, nullptr, nullptr, accumulate_x ? nullptr : dx, ld_dx};
     if (int st = gather(ctx, c, a)) return st;
     if (p.p == 3) return backward<3, 3>(ctx, c, p, work, d);
     return p.pg == 2 ? backward<1, 2>(ctx, c, p, work, d) : backward<1, 1>(ctx, c, p, work, d);

@@ -350,6 +350,17 @@ __global__ __launch_bounds__(S::kThreads, S::kThreads == 512 ? 2 : 1) void mat_k
     for (int i = 0; i < S::kBm; ++i)
 #pragma unroll
         for (int j = 0; j < S::kBn; ++j) acc.c[i][j] = f16v{};
+    // Three planes: the five small products of a split have sums of their own, 2^-8 the
+    // size, so that the sum proper rounds once for 16 of the contraction and not six
+    // times (errors against float64 of sums of 1024: 1.2e-6 -> 0.5e-6).
+    constexpr bool kTwoSums = S::kPa == 3;
+    f16v low[kTwoSums ? S::kBm : 1][kTwoSums ? S::kBn : 1];
+    if constexpr (kTwoSums) {
+#pragma unroll
+        for (int i = 0; i < S::kBm; ++i)
+#pragma unroll
+            for (int j = 0; j < S::kBn; ++j) low[i][j] = f16v{};
+    }
     // Operands of 16 of the contraction, read one ahead of their products.
     u4 a[2][S::kBm][S::kPa], b[2][S::kBn][S::kPb];
     const auto read = [&](int buf, int c, int to) {
@@ -378,7 +389,10 @@ __global__ __launch_bounds__(S::kThreads, S::kThreads == 512 ? 2 : 1) void mat_k
 #pragma unroll
                 for (int i = 0; i < S::kBm; ++i)
 #pragma unroll
-                    for (int j = 0; j < S::kBn; ++j) acc.c[i][j] = mfma_bf16(a[at][i][pa], b[at][j][pb], acc.c[i][j]);
+                    for (int j = 0; j < S::kBn; ++j) {
+                        f16v& to = kTwoSums && sum > 0 ? low[kTwoSums ? i : 0][kTwoSums ? j : 0] : acc.c[i][j];
+                        to = mfma_bf16(a[at][i][pa], b[at][j][pb], to);
+                    }
             }
     };
     constexpr int kChunks = S::kK / 16;
@@ -416,6 +430,12 @@ __global__ __launch_bounds__(S::kThreads, S::kThreads == 512 ? 2 : 1) void mat_k
             if (S::kStages > 2 && c == 0 && fetched < end) load(buf ? buf - 1 : S::kStages - 1);
         }
         buf = next;
+    }
+    if constexpr (kTwoSums) {
+#pragma unroll
+        for (int i = 0; i < S::kBm; ++i)
+#pragma unroll
+            for (int j = 0; j < S::kBn; ++j) acc.c[i][j] += low[i][j];
     }
     __syncthreads();  // the epilogue may use the LDS
     epi.template run<S>(at, acc, lds);
@@ -462,7 +482,8 @@ typedef uint32_t u2e __attribute__((ext_vector_type(2), aligned(2)));
 
 // --- products of few tokens ---------------------------------------------------------
 //
-// Up to 32 n: the time is A's bytes (the weights').  Each wave of a workgroup has its
+// Up to 32 n: the time is A's bytes (the weights').  A workgroup has a tile of C, or
+// one of the slices of its contraction (MatOut's): of each segment, `splits`.  Each wave of a workgroup has its
 // own share of the contraction and its own ring of LDS stages, filled as mat_kernel's
 // are, so nothing waits for another wave before the end, where the waves' sums meet in
 // LDS.  FP32: both operands are fp32 in memory and are split as they are read from LDS
@@ -525,9 +546,12 @@ __global__ __launch_bounds__(kWave* WAVES, 1) void few_kernel(MatArgs g, Epi epi
     __shared__ __attribute__((aligned(1024))) char lds[S::kLds];
     const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     MatAt at{};
+    const uint32_t tiles = (g.m + S::kM / S::kSubs - 1) / (S::kM / S::kSubs);
     at.m = g.m;
-    at.n = g.n;
-    at.tile_m = blockIdx.x;
+    at.n = g.n_dev ? __builtin_amdgcn_readfirstlane(min(g.n, *g.n_dev)) : g.n;
+    at.tile_m = blockIdx.x % tiles;
+    at.slice = blockIdx.x / tiles;  // of the contraction: split of segment
+    const int seg = DUAL ? 0 : at.slice % g.segments;
     at.m0 = at.tile_m * (S::kM / S::kSubs);
 
     // Rows of 128 bytes: eight lanes a row.  kCols bf16: 64 bytes of 32 values a k, four lanes.
@@ -541,7 +565,7 @@ __global__ __launch_bounds__(kWave* WAVES, 1) void few_kernel(MatArgs g, Epi epi
     for (int j = 0; j < kLoads; ++j) {
         const int row = j * 8 + rb, chunk = slot_b ^ mat_swizzle<32, 64, kRows>(row);
         k_b[j] = kChunk * chunk;
-        off_b[j] = row < g.n ? static_cast<uint32_t>(row * ldb + 16 * chunk) : kOutside;
+        off_b[j] = row < at.n ? static_cast<uint32_t>(row * ldb + 16 * chunk) : kOutside;
     }
 #pragma unroll
     for (int b = 0; b < BLOCKS; ++b) {
@@ -559,15 +583,16 @@ __global__ __launch_bounds__(kWave* WAVES, 1) void few_kernel(MatArgs g, Epi epi
         }
     }
 
-    const int32_t all = (g.k + S::kK - 1) / S::kK;
-    const int32_t begin = static_cast<int32_t>(static_cast<int64_t>(all) * wave / WAVES);
-    const int32_t end = static_cast<int32_t>(static_cast<int64_t>(all) * (wave + 1) / WAVES);
+    // The wave's share of its segment's steps, `splits` workgroups to a tile.
+    const int32_t all = (g.k + S::kK - 1) / S::kK, parts = WAVES * g.splits, part_of = at.slice / g.segments * WAVES + wave;
+    const int32_t begin = static_cast<int32_t>(static_cast<int64_t>(all) * part_of / parts);
+    const int32_t end = static_cast<int32_t>(static_cast<int64_t>(all) * (part_of + 1) / parts);
     const uint32_t base = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)lds)) + wave * S::kRing;
-    uint64_t pa[BLOCKS], pb = reinterpret_cast<uint64_t>(g.b[0].p) + int64_t{begin} * 128;
+    uint64_t pa[BLOCKS], pb = reinterpret_cast<uint64_t>(g.b[seg].p) + int64_t{begin} * 128;
     const int64_t step_a = KA == kRows ? 128 : S::kK * lda;
 #pragma unroll
     for (int b = 0; b < BLOCKS; ++b) {
-        const MatOperand& o = g.a[DUAL ? b / (BLOCKS / 2) : 0];
+        const MatOperand& o = g.a[DUAL ? b / (BLOCKS / 2) : seg];
         const int64_t row = at.m0 + 32 * (DUAL ? b % (BLOCKS / 2) : b);
         pa[b] = reinterpret_cast<uint64_t>(o.p) + (KA == kRows ? row * lda : row * kSize) + begin * step_a;
     }
@@ -596,9 +621,13 @@ __global__ __launch_bounds__(kWave* WAVES, 1) void few_kernel(MatArgs g, Epi epi
         ++fetched;
     };
 
-    f16v acc[BLOCKS];
+    f16v acc[BLOCKS], low[FP32 ? BLOCKS : 1];  // low: as mat_kernel's
 #pragma unroll
     for (int b = 0; b < BLOCKS; ++b) acc[b] = f16v{};
+    if constexpr (FP32) {
+#pragma unroll
+        for (int b = 0; b < BLOCKS; ++b) low[b] = f16v{};
+    }
     constexpr int kLater = (STAGES - 2) * (BLOCKS + 1) * kLoads;
     for (int i = 0; i < STAGES - 1 && fetched < end; ++i) load(i);
     int buf = 0;
@@ -612,7 +641,15 @@ __global__ __launch_bounds__(kWave* WAVES, 1) void few_kernel(MatArgs g, Epi epi
             if constexpr (FP32) {
                 const Split8 x = few_read32<kRows>(tb, c);
 #pragma unroll
-                for (int b = 0; b < BLOCKS; ++b) acc[b] = mfma_split(few_read32<KA>(tile + b * S::kTile, c), x, acc[b]);
+                for (int b = 0; b < BLOCKS; ++b) {
+                    const Split8 y = few_read32<KA>(tile + b * S::kTile, c);
+                    low[b] = mfma_bf16(y.l, x.h, low[b]);
+                    low[b] = mfma_bf16(y.h, x.l, low[b]);
+                    low[b] = mfma_bf16(y.m, x.m, low[b]);
+                    low[b] = mfma_bf16(y.m, x.h, low[b]);
+                    low[b] = mfma_bf16(y.h, x.m, low[b]);
+                    acc[b] = mfma_bf16(y.h, x.h, acc[b]);
+                }
             } else {
                 const u4 x = MatRead<32, 64, kRows>::get(tb, 0, c, 0);
 #pragma unroll
@@ -623,6 +660,10 @@ __global__ __launch_bounds__(kWave* WAVES, 1) void few_kernel(MatArgs g, Epi epi
         asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
         if (fetched < end) load(buf ? buf - 1 : STAGES - 1);
         buf = buf + 1 < STAGES ? buf + 1 : 0;
+    }
+    if constexpr (FP32) {
+#pragma unroll
+        for (int b = 0; b < BLOCKS; ++b) acc[b] += low[b];
     }
     __syncthreads();
     float* part = reinterpret_cast<float*>(lds);  // [wave][block][register][lane]
@@ -663,7 +704,7 @@ inline bool few_direct(bool fp32, const void* p, int64_t ld, int64_t cols) {
 template <int WAVES, int BLOCKS, int STAGES, bool FP32, int KA, bool DUAL, class Epi>
 int few_launch(mimir_ctx* ctx, const char* what, const MatArgs& g, const Epi& epi) {
     constexpr int64_t kRowsOf = 32 * BLOCKS / (DUAL ? 2 : 1);
-    const int64_t grid = (g.m + kRowsOf - 1) / kRowsOf;
+    const int64_t grid = (g.m + kRowsOf - 1) / kRowsOf * g.segments * g.splits;
     MIMIR_REQUIRE(ctx, dispatch_fits(grid, kWave * WAVES), "%s: grid of %lld workgroups exceeds the limit", what, (long long)grid);
     few_kernel<WAVES, BLOCKS, STAGES, FP32, KA, DUAL, Epi><<<static_cast<unsigned>(grid), kWave * WAVES, 0, ctx->stream>>>(g, epi);
     return launched(ctx, what);
@@ -862,6 +903,26 @@ MatDeal mat_deal(const mimir_ctx* ctx, int64_t m, int64_t n, int64_t k, int64_t 
 // The sum of the splits' slices into out (MatOut's fields say how) for a product of g in
 // tiles of bm x bn.
 int mat_join(mimir_ctx* ctx, const MatOut& o, const MatArgs& g, int bm, int bn);
+
+// A product of few n into MatOut through slices: workgroups for about two for each CU,
+// each wave with at least four steps.
+template <bool FP32, int KA>
+int few_splits(int64_t m, int64_t k, int segments) {
+    const int64_t tiles = (m + 63) / 64 * segments, steps = (k + (FP32 ? 31 : 63)) / (FP32 ? 32 : 64);
+    return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({512 / std::max<int64_t>(tiles, 1), steps / 16, 64})));
+}
+template <bool FP32, int KA>
+int few_product(mimir_ctx* ctx, const char* what, MatArgs g, MatOut o) {
+    const int32_t last = o.last, splits = g.splits, segments = g.segments;
+    o.last = last && splits * segments == 1;
+    if (int st = few_launch<4, 2, 3, FP32, KA, false>(ctx, what, g, o)) return st;
+    if (!last || o.last) return MIMIR_OK;
+    o.last = 1;
+    g.splits = splits * segments;  // mat_join's: as many slices, whatever the tiles
+    g.segments = 1;
+    g.fill = INT32_MAX;
+    return mat_join(ctx, o, g, 1 << 24, 1 << 24);
+}
 
 // C as a result.  o.last: these are the contraction's last pieces.
 template <int PA, int PB, int KA, int KB>

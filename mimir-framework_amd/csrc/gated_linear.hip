@@ -96,6 +96,29 @@ struct GatedOut {
     }
 };
 
+// y from gate and up, eight columns a thread.
+struct ActArgs {
+    const float* gate_up;  // [tokens][2 * hidden]
+    int64_t tokens, hidden;
+    void* y;
+    int64_t ld_y;
+};
+template <int ACT, bool BF16>
+__global__ __launch_bounds__(kBlock) void gated_act(ActArgs a) {
+    const int64_t of_row = (a.hidden + 7) / 8, total = a.tokens * of_row, stride = static_cast<int64_t>(gridDim.x) * kBlock;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * kBlock + threadIdx.x; i < total; i += stride) {
+        const int64_t t = i / of_row, c = i % of_row * 8;
+        const float* gp = a.gate_up + t * 2 * a.hidden + c;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            if (c + e >= a.hidden) break;
+            const float v = act1<ACT>(gp[e]) * gp[a.hidden + e];
+            if (BF16) static_cast<uint16_t*>(a.y)[t * a.ld_y + c + e] = static_cast<uint16_t>(pack_bf16(v, v));
+            else static_cast<float*>(a.y)[t * a.ld_y + c + e] = v;
+        }
+    }
+}
+
 // --- backward ----------------------------------------------------------------------
 
 struct GradArgs {
@@ -194,6 +217,9 @@ struct Plan {
     int p, pg;
     int64_t ld_x, piece, ld_w;  // columns of x's planes; a piece's columns of the weights, their planes' columns
     bool x_direct, w_direct, few;
+    bool split;                 // forward: few tiles, so the contraction is dealt out and the activation a pass of its own
+    MatDeal deal_y;
+    size_t gate_up;
     MatDeal deal_x, deal_w;
     size_t x, w, g, raw, partial, partial_w, total;
 };
@@ -230,6 +256,18 @@ Plan plan_of(const mimir_ctx* ctx, const Call& c, bool back) {
     };
     p.x = take(p.x_direct ? 0 : static_cast<size_t>(p.p * c.tokens * p.ld_x * 2));
     p.w = take(p.w_direct || p.few ? 0 : static_cast<size_t>(2 * p.p * c.dim * p.ld_w * 2));
+    if (!back) {
+        // Tiles for less than half of the CUs, and a contraction that several can share.
+        constexpr int64_t kFewTiles = 128, kLongDim = 1024;
+        const int64_t tn = p.p == 3 ? 64 : 128, tiles = (c.hidden + 63) / 64 * ((c.tokens + tn - 1) / tn);
+        p.split = p.piece >= c.hidden && tiles < kFewTiles && c.dim >= kLongDim && ctx->tune.mat_big != 1;
+        if (p.split) {
+            p.deal_y = p.p == 3 ? mat_deal<3, 3, kCols, kRows>(ctx, c.hidden, c.tokens, c.dim, 2, false)
+                                : mat_deal<1, 1, kCols, kRows>(ctx, c.hidden, c.tokens, c.dim, 2, false);
+            p.partial = take(p.deal_y.partial);
+            p.gate_up = take(static_cast<size_t>(2 * c.tokens * c.hidden * 4));
+        }
+    }
     if (back) {
         p.g = take(static_cast<size_t>(p.pg * c.tokens * 2 * p.piece * 2));
         const int64_t piece = std::min(p.piece, c.hidden);
@@ -312,6 +350,23 @@ int forward(mimir_ctx* ctx, const Call& c, const Plan& p, char* work, void* y, i
         MatArgs g = args_of(cols, c.tokens, c.dim);
         if (int st = weights(ctx, c, p, work, first, cols, g.a)) return st;
         g.b[0] = x;
+        if (p.split) {
+            if (!gate_up) gate_up = reinterpret_cast<float*>(work + p.gate_up);
+            MatOut o{};
+            o.out[0] = gate_up;
+            o.out[1] = gate_up + c.hidden;
+            o.ld = 2 * c.hidden;
+            o.partial = reinterpret_cast<float*>(work + p.partial);
+            o.ld_partial = mat_round(c.hidden, 4);
+            o.alpha = 1.0f;
+            o.last = 1;
+            g.batches = 2;
+            if (int st = mat_product<P, P, kCols, kRows>(ctx, "gated products", g, o, p.deal_y)) return st;
+            const int64_t blocks = (c.tokens * ((c.hidden + 7) / 8) + kBlock - 1) / kBlock;
+            gated_act<ACT, P == 1><<<static_cast<unsigned>(std::min<int64_t>(blocks, 1 << 16)), kBlock, 0, ctx->stream>>>(
+                ActArgs{gate_up, c.tokens, c.hidden, y, ld_y});
+            return launched(ctx, "gated_act");
+        }
         GatedOut<ACT> e{};
         e.y.out[0] = static_cast<char*>(y) + first * (bf16 ? 2 : 4);
         e.y.ld = ld_y;

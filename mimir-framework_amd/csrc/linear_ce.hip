@@ -379,7 +379,8 @@ Plan plan_of(const mimir_ctx* ctx, int type, const void* w, int64_t ld_w, int64_
     } else {
         p.logit = take(static_cast<size_t>(tokens * 4));
         p.sums = take(static_cast<size_t>((tokens + kFinishTokens - 1) / kFinishTokens * 8));
-        p.part = take(static_cast<size_t>((vocab + kTileM - 1) / kTileM * tokens * 8));
+        const int64_t pieces = (vocab + p.piece - 1) / p.piece, tiles = (std::min(p.piece, vocab) + kTileM - 1) / kTileM;
+        p.part = take(static_cast<size_t>(pieces * tiles * tokens * 8));
     }
     p.total = at;
     return p;

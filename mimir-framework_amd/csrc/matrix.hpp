@@ -455,6 +455,13 @@ using MatBig = std::conditional_t<PA == 3, MatShape<256, 128, 4, 2, 32, 2, 3, 3,
 template <int PA, int PB, int KA, int KB, bool DUAL = false>
 using MatSmall = std::conditional_t<PA == 3, MatShape<128, 64, 2, 2, 32, 2, 3, 3, KA, KB, DUAL>,
                                     MatShape<128, 128, 2, 2, 64, 2, PA, PB, KA, KB, DUAL>>;
+// A contraction of a step or two is over before a workgroup's stores are: smaller
+// stages, so that more workgroups share a CU.
+// Measured, 9 tokens' dw of 32000 x 4096 bf16: 75 us, 154 with stages of 64.  Three
+// planes gain nothing by it (134 us against the larger tiles' 121 for 2 x 4096 x 11008).
+template <int PA, int PB, int KA, int KB>
+using MatThin = MatShape<128, 128, 2, 2, 32, 2, PA, PB, KA, KB>;
+constexpr int64_t kMatThinK = 64;
 constexpr int64_t kMatBigTiles = 192;
 template <class S>
 bool mat_fills(const mimir_ctx* ctx, const MatArgs& g) {
@@ -549,8 +556,13 @@ __global__ __launch_bounds__(kWave* WAVES, 1) void few_kernel(MatArgs g, Epi epi
     const uint32_t tiles = (g.m + S::kM / S::kSubs - 1) / (S::kM / S::kSubs);
     at.m = g.m;
     at.n = g.n_dev ? __builtin_amdgcn_readfirstlane(min(g.n, *g.n_dev)) : g.n;
-    at.tile_m = blockIdx.x % tiles;
-    at.slice = blockIdx.x / tiles;  // of the contraction: split of segment
+    // Neighbouring tiles on one XCD, as mat_tile_of deals them: kCols tiles are 128 bytes
+    // of each row, and their neighbours read the next.
+    const uint32_t total = gridDim.x, per = (total + kMatXcds - 1) / kMatXcds, full = total - (per - 1) * kMatXcds;
+    const uint32_t xcd = blockIdx.x % kMatXcds;  // the first `full` of them have `per` workgroups, the others one less
+    const uint32_t id = xcd * per - (xcd > full ? xcd - full : 0) + blockIdx.x / kMatXcds;
+    at.tile_m = id % tiles;
+    at.slice = id / tiles;  // of the contraction: split of segment
     const int seg = DUAL ? 0 : at.slice % g.segments;
     at.m0 = at.tile_m * (S::kM / S::kSubs);
 
@@ -864,7 +876,7 @@ int mat_stage(mimir_ctx* ctx, int type, const void* src, int64_t rows, int64_t c
 // A product into MatOut: its shape, and how its contraction is dealt to workgroups where
 // the tiles of C alone leave CUs idle.
 struct MatDeal {
-    bool big;
+    bool big, thin;
     int32_t fill, splits;
     size_t partial;  // bytes of the slices
 };
@@ -872,7 +884,7 @@ struct MatDeal {
 // The larger tiles where they fill the GPU, or, the contraction split, come to 1 for
 // each CU; else the smaller ones, split to 2 for each CU.  A split has at least 512 of
 // the contraction.  `more`: the sums go through fp32 slices whether split or not.
-template <class BIG, class SMALL, bool HAS_BIG>
+template <class BIG, class SMALL, bool HAS_BIG, bool HAS_THIN>
 MatDeal mat_deal(const mimir_ctx* ctx, int64_t m, int64_t n, int64_t k, int64_t batches, bool more) {
     constexpr int32_t kBigFill = 256, kSmallFill = 512;
     constexpr int64_t kLeastK = 512;
@@ -880,7 +892,8 @@ MatDeal mat_deal(const mimir_ctx* ctx, int64_t m, int64_t n, int64_t k, int64_t 
     const int64_t big = tiles(BIG::kM, BIG::kN), most = std::max<int64_t>(1, k / kLeastK);
     const int64_t big_most = std::max<int64_t>(1, kBigFill / std::max<int64_t>(big, 1));
     MatDeal d{};
-    d.big = HAS_BIG && (ctx->tune.mat_big >= 0 ? ctx->tune.mat_big == 1 : big * std::min(most, big_most) >= kMatBigTiles);
+    d.thin = HAS_THIN && k <= kMatThinK && ctx->tune.mat_big != 1;
+    d.big = HAS_BIG && !d.thin && (ctx->tune.mat_big >= 0 ? ctx->tune.mat_big == 1 : big * std::min(most, big_most) >= kMatBigTiles);
     d.fill = d.big ? kBigFill : kSmallFill;
     d.splits = static_cast<int32_t>(std::min<int64_t>(most, 64));
     const int64_t now = tiles(d.big ? BIG::kM : SMALL::kM, d.big ? BIG::kN : SMALL::kN);
@@ -896,8 +909,8 @@ MatDeal mat_deal(const mimir_ctx* ctx, int64_t m, int64_t n, int64_t k, int64_t 
 template <int PA, int PB, int KA, int KB>
 MatDeal mat_deal(const mimir_ctx* ctx, int64_t m, int64_t n, int64_t k, int64_t batches, bool more) {
     using S = MatSmall<PA, PB, KA, KB>;
-    if constexpr (PA == PB) return mat_deal<MatBig<PA, PB, KA, KB>, S, true>(ctx, m, n, k, batches, more);
-    else return mat_deal<S, S, false>(ctx, m, n, k, batches, more);
+    if constexpr (PA == PB) return mat_deal<MatBig<PA, PB, KA, KB>, S, true, PA != 3>(ctx, m, n, k, batches, more);
+    else return mat_deal<S, S, false, true>(ctx, m, n, k, batches, more);
 }
 
 // The sum of the splits' slices into out (MatOut's fields say how) for a product of g in
@@ -942,7 +955,9 @@ int mat_product(mimir_ctx* ctx, const char* what, MatArgs g, MatOut o, const Mat
             st = mat_launch<B>(ctx, what, g, o);
         }
     }
-    if (!d.big) st = mat_launch<S>(ctx, what, g, o);
+    if constexpr (PA != 3)
+        if (d.thin) st = mat_launch<MatThin<PA, PB, KA, KB>>(ctx, what, g, o);
+    if (!d.thin && !d.big) st = mat_launch<S>(ctx, what, g, o);
     if (st || d.splits == 1 || !last) return st;
     o.last = 1;
     return mat_join(ctx, o, g, bm, bn);

@@ -211,6 +211,44 @@ inline void attention_paged(Context& c, const mimir_kv_cache& cache, const mimir
             "paged attention");
 }
 
+// Training: the last layer's loss, gated products, gradients' norm and clipping
+// (mimir_hip.h; type MIMIR_NUM_*, act MIMIR_ACT_*).
+inline void linear_cross_entropy(Context& c, int type, const void* x, int64_t ld_x, const void* w, int64_t ld_w,
+                                 const int32_t* targets, int64_t tokens, int64_t dim, int64_t vocab, float* loss,
+                                 float* lse, float* mean = nullptr) {
+    c.check(mimir_linear_cross_entropy_fwd(c.get(), type, x, ld_x, w, ld_w, targets, tokens, dim, vocab, loss, lse, mean),
+            "linear cross entropy");
+}
+inline void linear_cross_entropy_bwd(Context& c, int type, const void* x, int64_t ld_x, const void* w, int64_t ld_w,
+                                     const int32_t* targets, int64_t tokens, int64_t dim, int64_t vocab, const float* lse,
+                                     const float* dloss, const float* mean, float scale, void* dx, int64_t ld_dx,
+                                     bool accumulate_x, void* dw, int64_t ld_dw, bool accumulate_w) {
+    c.check(mimir_linear_cross_entropy_bwd(c.get(), type, x, ld_x, w, ld_w, targets, tokens, dim, vocab, lse, dloss, mean,
+                                           scale, dx, ld_dx, accumulate_x ? 1 : 0, dw, ld_dw, accumulate_w ? 1 : 0),
+            "linear cross entropy gradient");
+}
+inline void gated_linear(Context& c, int type, int act, const void* x, int64_t ld_x, const void* w_gate, const void* w_up,
+                         int64_t ld_w, int64_t tokens, int64_t dim, int64_t hidden, void* y, int64_t ld_y,
+                         float* gate_up = nullptr) {
+    c.check(mimir_gated_linear_fwd(c.get(), type, act, x, ld_x, w_gate, w_up, ld_w, tokens, dim, hidden, y, ld_y, gate_up),
+            "gated products");
+}
+inline void gated_linear_bwd(Context& c, int type, int act, const void* x, int64_t ld_x, const void* w_gate,
+                             const void* w_up, int64_t ld_w, int64_t tokens, int64_t dim, int64_t hidden,
+                             const float* gate_up, const void* dy, int64_t ld_dy, void* dx, int64_t ld_dx,
+                             bool accumulate_x, void* dw_gate, void* dw_up, int64_t ld_dw, bool accumulate_w) {
+    c.check(mimir_gated_linear_bwd(c.get(), type, act, x, ld_x, w_gate, w_up, ld_w, tokens, dim, hidden, gate_up, dy, ld_dy,
+                                   dx, ld_dx, accumulate_x ? 1 : 0, dw_gate, dw_up, ld_dw, accumulate_w ? 1 : 0),
+            "gated products' gradient");
+}
+inline void grad_norm(Context& c, const std::vector<mimir_tensor>& tensors, float* norm) {
+    c.check(mimir_grad_norm(c.get(), tensors.data(), static_cast<int64_t>(tensors.size()), norm), "gradients' norm");
+}
+inline void grad_clip(Context& c, const std::vector<mimir_tensor>& tensors, float max_norm, float* norm = nullptr) {
+    c.check(mimir_grad_clip(c.get(), tensors.data(), static_cast<int64_t>(tensors.size()), max_norm, norm),
+            "gradients' clipping");
+}
+
 }  // namespace device
 
 namespace detail {

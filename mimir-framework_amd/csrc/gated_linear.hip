@@ -187,6 +187,10 @@ __global__ __launch_bounds__(kBlock) void gated_grad(GradArgs a) {
                 if (4 * h + 4 <= left) {
                     *reinterpret_cast<f4u*>(to + 4 * h) = f4u{dg[4 * h], dg[4 * h + 1], dg[4 * h + 2], dg[4 * h + 3]};
                     *reinterpret_cast<f4u*>(to + a.tokens * a.cols + 4 * h) = f4u{du[4 * h], du[4 * h + 1], du[4 * h + 2], du[4 * h + 3]};
+                } else {
+#pragma unroll
+                    for (int e = 4 * h; e < 4 * h + 3; ++e)
+                        if (e < left) to[e] = dg[e], to[a.tokens * a.cols + e] = du[e];
                 }
         }
         uint16_t* to = a.out + t * 2 * a.cols_out + c;
@@ -392,7 +396,7 @@ int forward_few(mimir_ctx* ctx, const Call& c, void* y, int64_t ld_y, float* gat
     e.y.bf16 = !FP32;
     e.gate_up = gate_up;
     e.hidden = c.hidden;
-    return few_launch<4, 2, 3, FP32, kCols, true>(ctx, "gated products", g, e);
+    return few_launch<FP32, kCols, true>(ctx, "gated products", g, e);
 }
 
 struct Gradients {

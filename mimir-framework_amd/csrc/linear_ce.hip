@@ -46,7 +46,7 @@ struct GatherArgs {
     int64_t tokens, dim, vocab;
     uint16_t* dst;       // planes of [tokens][ld_dst]
     int64_t ld_dst, plane;
-    float* raw;          // the rows as they are [tokens][dim] too (fp32, dim a multiple of 4), or null
+    float* raw;          // the rows as they are [tokens][dim] too (fp32), or null
     int32_t* row;        // [tokens]: the token of each gathered row
     int32_t* count;      // and a counter for ce_finish, zeroed
     float* zero_a;       // of tokens without a target: loss and lse, or null
@@ -325,7 +325,6 @@ struct Plan {
     size_t x, raw_x, row, count, logit, sums, part, w, g, raw_g, partial, partial_w, total;
 };
 
-constexpr int kFewBlocks = 2;  // of 32 rows of w, a workgroup's with few tokens
 constexpr int64_t kPieceBytes = int64_t{512} << 20;
 constexpr int64_t kTileM = 128;  // the smaller shape's: how many partial results a token has at most
 
@@ -482,7 +481,7 @@ int forward_few(mimir_ctx* ctx, const Call& c, float* loss, float* lse, float* m
     const auto operand = [](const void* p, int64_t ld) { return MatOperand{static_cast<const uint16_t*>(p), ld, 0}; };
     const MatArgs g = args_of(operand(c.w, c.ld_w), operand(c.x, c.ld_x), c.vocab, c.tokens, c.dim);
     const CeStats e{c.target, nullptr, reinterpret_cast<f2*>(work + 256), reinterpret_cast<float*>(work), c.tokens, 0, 0};
-    if (int st = few_launch<4, kFewBlocks, 3, FP32, kRows, false>(ctx, "cross entropy statistics", g, e)) return st;
+    if (int st = few_launch<FP32, kRows, false>(ctx, "cross entropy statistics", g, e)) return st;
     const FinishArgs f{e.part, c.tokens, static_cast<int32_t>(tiles), e.logit, nullptr, nullptr, c.target, c.vocab, loss, lse, nullptr, mean};
     ce_finish<1024><<<1, 1024, 0, ctx->stream>>>(f);
     return launched(ctx, "ce_finish");
@@ -545,7 +544,7 @@ int backward(mimir_ctx* ctx, const Call& c, const Plan& p, char* work, const Gra
             st = mat_fills<BG>(ctx, g) ? mat_launch<BG>(ctx, "cross entropy gradient", g, e)
                                        : mat_launch<SG>(ctx, "cross entropy gradient", g, e);
         } else if constexpr (P == 3) {
-            st = few_launch<4, kFewBlocks, 3, true, kRows, false>(ctx, "cross entropy gradient", g, e);
+            st = few_launch<true, kRows, false>(ctx, "cross entropy gradient", g, e);
         }
         if (st) return st;
         if (d.dx) {

@@ -494,28 +494,48 @@ typedef uint32_t u2e __attribute__((ext_vector_type(2), aligned(2)));
 // own share of the contraction and its own ring of LDS stages, filled as mat_kernel's
 // are, so nothing waits for another wave before the end, where the waves' sums meet in
 // LDS.  FP32: both operands are fp32 in memory and are split as they are read from LDS
-// (their planes would be three times the bytes on the way).  Of each wave's stages all
-// but one are on their way: 8 waves of 2 x 8 KB a CU are 33 MB in flight on the GPU.
+// (their planes would be five times the bytes on the way).  Of each wave's three stages
+// two are on their way: 4 waves of 2 x 8 KB of A a CU are 17 MB in flight on the GPU.
+// Measured: 32 x 4096 x 32000 bf16 43 us in the kernel, 6.1 TB/s; kCols operands, whose
+// tiles are 64 or 128 bytes of each row, 2.7 TB/s (5 x 4096 x 11008 fp32, both weights,
+// 134 us).
 
 constexpr int kFewN = 32;
 
 // 32 rows of a raw fp32 operand, BK = 32: kRows 128 bytes a row, kCols 128 bytes a k.
-template <int KIND>
-__device__ __forceinline__ Split8 few_read32(const char* tile, int c) {
+// Rows begin at any float.  Where a row ends inside a 16-byte chunk, the chunk's last
+// floats of the row were loaded, so that nothing behind it is read: they stand at the
+// chunk's end.  kRows, TAIL: `left` k's of the tile are inside.  kCols: the lane's column stands `shift` floats further (few_shift).
+template <int KIND, bool TAIL>
+__device__ __forceinline__ Split8 few_read32(const char* tile, int c, int left, int shift) {
     const int lane = threadIdx.x % kWave, li = lane % 32, hf = lane / 32;
     float x[8];
     if constexpr (KIND == kRows) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const f4 v = *reinterpret_cast<const f4*>(tile + li * 128 + 16 * ((4 * c + 2 * hf + h) ^ mat_swizzle<32, 64, kRows>(li)));
+            const int k = 16 * c + 8 * hf + 4 * h;
+            f4 v = *reinterpret_cast<const f4*>(tile + li * 128 + 16 * (k / 4 ^ mat_swizzle<32, 64, kRows>(li)));
+            if (TAIL && left % 4 && k < left && k + 4 > left) {
+                const int by = 4 - left % 4;
+                v = f4{by == 1 ? v[1] : by == 2 ? v[2] : v[3], by == 1 ? v[2] : by == 2 ? v[3] : 0.0f, by == 1 ? v[3] : 0.0f, 0.0f};
+            }
 #pragma unroll
             for (int e = 0; e < 4; ++e) x[4 * h + e] = v[e];
         }
     } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = *reinterpret_cast<const float*>(tile + (16 * c + 8 * hf + e) * 128 + 4 * li);
+        for (int e = 0; e < 8; ++e) x[e] = *reinterpret_cast<const float*>(tile + (16 * c + 8 * hf + e) * 128 + 4 * (li + shift));
     }
     return split8(x);
+}
+// Of the lane's column, `rows` columns left of the matrix: those in its last, cut chunk.
+__device__ __forceinline__ int few_shift(int32_t rows) {
+    const int li = threadIdx.x % 32;
+    return rows < 32 && rows % 4 && li < rows && li >= rows - rows % 4 ? 4 - rows % 4 : 0;
+}
+// Bytes that a load of the chunk from `at` on goes back where only `left` are left.
+__device__ __forceinline__ uint32_t few_back(int32_t at, int32_t left) {
+    return left - at < 4 ? 4 * (4 - (left - at)) : 0;
 }
 
 // The same of bf16, BK = 64: kCols 64 bytes a k.
@@ -550,6 +570,8 @@ template <int WAVES, int BLOCKS, int STAGES, bool FP32, int KA, bool DUAL, class
 __global__ __launch_bounds__(kWave* WAVES, 1) void few_kernel(MatArgs g, Epi epi) {
     using S = FewShape<WAVES, BLOCKS, STAGES, FP32, KA, DUAL>;
     constexpr int kSize = FP32 ? 4 : 2, kChunk = 16 / kSize;  // bytes of an element, elements of 16 bytes
+    // Offsets count from here before their row's step, so that those that go back stay positive.
+    constexpr int kBefore = FP32 ? 16 : 0;
     __shared__ __attribute__((aligned(1024))) char lds[S::kLds];
     const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     MatAt at{};
@@ -570,6 +592,7 @@ __global__ __launch_bounds__(kWave* WAVES, 1) void few_kernel(MatArgs g, Epi epi
     constexpr bool kWide = KA == kRows || FP32;
     constexpr int kLanesA = kWide ? 8 : 4, kRowsOfA = kWave / kLanesA, kLoads = S::kTile / 1024;
     const int ra = lane / kLanesA, slot_a = lane % kLanesA, rb = lane / 8, slot_b = lane % 8;
+    int shift[BLOCKS];  // kCols fp32: of the lane's column in each block
     uint32_t off_a[BLOCKS][KA == kRows ? kLoads : 1], off_b[kLoads];
     int32_t k_a[KA == kRows ? kLoads : 1], k_b[kLoads];
     const int64_t lda = g.a[0].ld * kSize, ldb = g.b[0].ld * kSize;  // bytes
@@ -577,21 +600,24 @@ __global__ __launch_bounds__(kWave* WAVES, 1) void few_kernel(MatArgs g, Epi epi
     for (int j = 0; j < kLoads; ++j) {
         const int row = j * 8 + rb, chunk = slot_b ^ mat_swizzle<32, 64, kRows>(row);
         k_b[j] = kChunk * chunk;
-        off_b[j] = row < at.n ? static_cast<uint32_t>(row * ldb + 16 * chunk) : kOutside;
+        off_b[j] = row < at.n ? static_cast<uint32_t>(row * ldb + 16 * chunk + kBefore) : kOutside;
     }
 #pragma unroll
     for (int b = 0; b < BLOCKS; ++b) {
         const int32_t rows = g.m - at.m0 - 32 * (DUAL ? b % (BLOCKS / 2) : b);  // of this block on
+        shift[b] = FP32 && KA == kCols ? few_shift(rows) : 0;
         if constexpr (KA == kRows) {
 #pragma unroll
             for (int j = 0; j < kLoads; ++j) {
                 const int row = j * 8 + ra, chunk = slot_a ^ mat_swizzle<32, 64, kRows>(row);
                 k_a[j] = kChunk * chunk;
-                off_a[b][j] = row < rows ? static_cast<uint32_t>(row * lda + 16 * chunk) : kOutside;
+                off_a[b][j] = row < rows ? static_cast<uint32_t>(row * lda + 16 * chunk + kBefore) : kOutside;
             }
         } else {
             k_a[0] = ra;
-            off_a[b][0] = kChunk * slot_a < rows ? static_cast<uint32_t>(ra * lda + 16 * slot_a) : kOutside;
+            off_a[b][0] = kChunk * slot_a < rows ? static_cast<uint32_t>(ra * lda + 16 * slot_a + kBefore) : kOutside;
+            if constexpr (FP32)
+                if (kChunk * slot_a < rows) off_a[b][0] -= few_back(kChunk * slot_a, rows);
         }
     }
 
@@ -612,14 +638,18 @@ __global__ __launch_bounds__(kWave* WAVES, 1) void few_kernel(MatArgs g, Epi epi
     const auto load = [&](int stage) {
         const int32_t left = g.k - fetched * S::kK;
         const uint32_t to = base + stage * S::kStage;
-        const auto rsrc = [](uint64_t p) { return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(p), 0, 0x7fffffff, kBufferWord3); };
+        const auto rsrc = [](uint64_t p) {
+            return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(p - kBefore), 0, 0x7fffffff, kBufferWord3);
+        };
+        // A chunk's offset in the last step, which its row may end in.
+        const auto tail = [&](uint32_t off, int32_t k) { return k < left && off != kOutside ? off - (FP32 ? few_back(k, left) : 0) : kOutside; };
 #pragma unroll
         for (int b = 0; b < BLOCKS; ++b) {
             const auto rs = rsrc(pa[b]);
 #pragma unroll
             for (int j = 0; j < kLoads; ++j) {
                 if constexpr (KA == kRows)
-                    load_to_lds(to + b * S::kTile + j * 1024, k_a[j] < left ? off_a[b][j] : kOutside, rs, 0);
+                    load_to_lds(to + b * S::kTile + j * 1024, left >= S::kK ? off_a[b][j] : tail(off_a[b][j], k_a[j]), rs, 0);
                 else
                     load_to_lds(to + b * S::kTile + j * 1024, k_a[0] + j * kRowsOfA < left ? off_a[b][0] : kOutside, rs,
                                 __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(j * kRowsOfA * lda)));
@@ -628,7 +658,8 @@ __global__ __launch_bounds__(kWave* WAVES, 1) void few_kernel(MatArgs g, Epi epi
         }
         const auto rs = rsrc(pb);
 #pragma unroll
-        for (int j = 0; j < kLoads; ++j) load_to_lds(to + BLOCKS * S::kTile + j * 1024, k_b[j] < left ? off_b[j] : kOutside, rs, 0);
+        for (int j = 0; j < kLoads; ++j)
+            load_to_lds(to + BLOCKS * S::kTile + j * 1024, left >= S::kK ? off_b[j] : tail(off_b[j], k_b[j]), rs, 0);
         pb += 128;
         ++fetched;
     };
@@ -648,26 +679,32 @@ __global__ __launch_bounds__(kWave* WAVES, 1) void few_kernel(MatArgs g, Epi epi
         else mat_landed<0>();
         const char* tile = lds + wave * S::kRing + buf * S::kStage;
         const char* tb = tile + BLOCKS * S::kTile;
+        const int32_t inside = g.k - step * S::kK;
+        const auto multiply = [&](auto tail) {
+            constexpr bool kTail = decltype(tail)::value;
 #pragma unroll
-        for (int c = 0; c < S::kK / 16; ++c) {
-            if constexpr (FP32) {
-                const Split8 x = few_read32<kRows>(tb, c);
+            for (int c = 0; c < S::kK / 16; ++c) {
+                if constexpr (FP32) {
+                    const Split8 x = few_read32<kRows, kTail>(tb, c, inside, 0);
 #pragma unroll
-                for (int b = 0; b < BLOCKS; ++b) {
-                    const Split8 y = few_read32<KA>(tile + b * S::kTile, c);
-                    low[b] = mfma_bf16(y.l, x.h, low[b]);
-                    low[b] = mfma_bf16(y.h, x.l, low[b]);
-                    low[b] = mfma_bf16(y.m, x.m, low[b]);
-                    low[b] = mfma_bf16(y.m, x.h, low[b]);
-                    low[b] = mfma_bf16(y.h, x.m, low[b]);
-                    acc[b] = mfma_bf16(y.h, x.h, acc[b]);
+                    for (int b = 0; b < BLOCKS; ++b) {
+                        const Split8 y = few_read32<KA, kTail>(tile + b * S::kTile, c, inside, KA == kCols ? shift[b] : 0);
+                        low[b] = mfma_bf16(y.l, x.h, low[b]);
+                        low[b] = mfma_bf16(y.h, x.l, low[b]);
+                        low[b] = mfma_bf16(y.m, x.m, low[b]);
+                        low[b] = mfma_bf16(y.m, x.h, low[b]);
+                        low[b] = mfma_bf16(y.h, x.m, low[b]);
+                        acc[b] = mfma_bf16(y.h, x.h, acc[b]);
+                    }
+                } else {
+                    const u4 x = MatRead<32, 64, kRows>::get(tb, 0, c, 0);
+#pragma unroll
+                    for (int b = 0; b < BLOCKS; ++b) acc[b] = mfma_bf16(few_read16<KA>(tile + b * S::kTile, c), x, acc[b]);
                 }
-            } else {
-                const u4 x = MatRead<32, 64, kRows>::get(tb, 0, c, 0);
-#pragma unroll
-                for (int b = 0; b < BLOCKS; ++b) acc[b] = mfma_bf16(few_read16<KA>(tile + b * S::kTile, c), x, acc[b]);
             }
-        }
+        };
+        if (FP32 && inside < S::kK) multiply(std::true_type{});
+        else multiply(std::false_type{});
         // The stage that was read is the next to be filled: its reads are in registers.
         asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
         if (fetched < end) load(buf ? buf - 1 : STAGES - 1);
@@ -707,18 +744,23 @@ __global__ __launch_bounds__(kWave* WAVES, 1) void few_kernel(MatArgs g, Epi epi
 }
 
 
-// Operands that few_kernel takes as they are: 16-byte chunks within rows.
+// Operands that few_kernel takes as they are: fp32 rows of at least a chunk, bf16 ones in
+// whole, aligned chunks.
 inline bool few_direct(bool fp32, const void* p, int64_t ld, int64_t cols) {
-    const int64_t of = fp32 ? 4 : 8;
-    return aligned16(p) && ld % of == 0 && cols % of == 0 && mat_ld_fits(ld);
+    if (fp32) return cols >= 4 && mat_ld_fits(ld);
+    return aligned16(p) && ld % 8 == 0 && cols % 8 == 0 && mat_ld_fits(ld);
 }
 
-template <int WAVES, int BLOCKS, int STAGES, bool FP32, int KA, bool DUAL, class Epi>
+// Four waves have a CU's LDS to themselves.  Two workgroups of two waves sharing it are
+// slower, also where tiles number a little more than the CUs (32 x 4096 x 32000 bf16, 500
+// tiles: 68 us against 55).
+constexpr int kFewBlocks = 2;
+template <bool FP32, int KA, bool DUAL, class Epi>
 int few_launch(mimir_ctx* ctx, const char* what, const MatArgs& g, const Epi& epi) {
-    constexpr int64_t kRowsOf = 32 * BLOCKS / (DUAL ? 2 : 1);
+    constexpr int64_t kRowsOf = 32 * kFewBlocks / (DUAL ? 2 : 1);
     const int64_t grid = (g.m + kRowsOf - 1) / kRowsOf * g.segments * g.splits;
-    MIMIR_REQUIRE(ctx, dispatch_fits(grid, kWave * WAVES), "%s: grid of %lld workgroups exceeds the limit", what, (long long)grid);
-    few_kernel<WAVES, BLOCKS, STAGES, FP32, KA, DUAL, Epi><<<static_cast<unsigned>(grid), kWave * WAVES, 0, ctx->stream>>>(g, epi);
+    MIMIR_REQUIRE(ctx, dispatch_fits(grid, 4 * kWave), "%s: grid of %lld workgroups exceeds the limit", what, (long long)grid);
+    few_kernel<4, kFewBlocks, 3, FP32, KA, DUAL, Epi><<<static_cast<unsigned>(grid), 4 * kWave, 0, ctx->stream>>>(g, epi);
     return launched(ctx, what);
 }
 
@@ -928,7 +970,7 @@ template <bool FP32, int KA>
 int few_product(mimir_ctx* ctx, const char* what, MatArgs g, MatOut o) {
     const int32_t last = o.last, splits = g.splits, segments = g.segments;
     o.last = last && splits * segments == 1;
-    if (int st = few_launch<4, 2, 3, FP32, KA, false>(ctx, what, g, o)) return st;
+    if (int st = few_launch<FP32, KA, false>(ctx, what, g, o)) return st;
     if (!last || o.last) return MIMIR_OK;
     o.last = 1;
     g.splits = splits * segments;  // mat_join's: as many slices, whatever the tiles

@@ -66,7 +66,7 @@ def hold(got, x, wg, wu, dy, act, dtype, start=None):
             near(got[name], want, bound, name)
 
 
-SIZES = [(1, 1, 1), (1, 8, 3), (7, 24, 72), (32, 296, 1000), (17, 1024, 40), (5, 2048, 64), (40, 1100, 70), (70, 2051, 129), (20, 8, 8), (31, 136, 36), (2, 5, 100), (3, 64, 257), (31, 33, 129), (32, 64, 128), (33, 65, 300), (65, 136, 520),
+SIZES = [(1, 1, 1), (1, 8, 3), (7, 24, 72), (32, 296, 1000), (17, 1024, 40), (5, 2048, 64), (40, 1100, 70), (70, 2051, 129), (20, 8, 8), (31, 136, 36), (9, 37, 71), (32, 1003, 335), (16, 30, 34), (4, 6, 5), (2, 5, 100), (3, 64, 257), (31, 33, 129), (32, 64, 128), (33, 65, 300), (65, 136, 520),
          (129, 100, 513), (300, 40, 77), (130, 1000, 264), (1000, 16, 24)]
 
 

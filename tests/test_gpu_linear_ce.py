@@ -78,7 +78,7 @@ def hold(got, x, w, target, dtype, weight=None, use_mean=True, scale=1.0, start=
 
 
 # tokens, dim, vocab
-SIZES = [(1, 1, 1), (1, 8, 2), (7, 24, 70), (32, 296, 1000), (17, 1024, 333), (5, 2048, 64), (20, 8, 3), (2, 5, 100), (3, 64, 257), (31, 33, 129), (32, 64, 128), (33, 65, 300), (65, 136, 1000),
+SIZES = [(1, 1, 1), (1, 8, 2), (7, 24, 70), (32, 296, 1000), (17, 1024, 333), (5, 2048, 64), (20, 8, 3), (9, 37, 71), (32, 1003, 335), (16, 30, 34), (4, 6, 5), (2, 5, 100), (3, 64, 257), (31, 33, 129), (32, 64, 128), (33, 65, 300), (65, 136, 1000),
          (129, 100, 513), (300, 40, 777), (130, 1000, 264)]
 
 

@@ -462,7 +462,11 @@ using MatSmall = std::conditional_t<PA == 3, MatShape<128, 64, 2, 2, 32, 2, 3, 3
 template <int PA, int PB, int KA, int KB>
 using MatThin = MatShape<128, 128, 2, 2, 32, 2, PA, PB, KA, KB>;
 constexpr int64_t kMatThinK = 64;
-constexpr int64_t kMatBigTiles = 192;
+// More than 128 larger tiles are one round of the GPU's CUs where four times as many
+// smaller ones are two rounds of two to a CU.  Measured (larger / smaller), us: fp32
+// 1024 x 1021 x 2752 gated, 176 tiles 76 / 85, its dw 72 / 80; 700 x 300 x 1500, 40 tiles 45 /
+// 31; bf16 1001 x 777 x 50001 statistics, 784 tiles 103 / 120.
+constexpr int64_t kMatBigTiles = 129;
 template <class S>
 bool mat_fills(const mimir_ctx* ctx, const MatArgs& g) {
     return ctx->tune.mat_big >= 0 ? ctx->tune.mat_big == 1 : mat_tiles<S>(g) >= kMatBigTiles;

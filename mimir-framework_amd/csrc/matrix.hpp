@@ -98,9 +98,11 @@ __device__ __forceinline__ constexpr int mat_swizzle(int i) {
 // LDS writes of 16 bytes a lane, behind each other from `lds` (uniform) on.  In asm:
 // the compiler would wait for a builtin's load before any later LDS read, since it
 // does not tell the two buffers apart.  The kernel waits itself (mat_landed); nothing
-// else in it uses m0, which no clobber list can name.
+// else in it uses m0, which no clobber list can name.  The s_nop: one wait state from m0
+// to the load, and five from a lane read that the compiler may have made for an operand
+// just before, which it does not keep apart from assembly.
 __device__ __forceinline__ void load_to_lds(uint32_t lds, uint32_t voff, __amdgpu_buffer_rsrc_t rs, uint32_t soff) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
                  :
                  : "s"(lds), "v"(voff), "s"(rs), "s"(soff)
                  : "memory");

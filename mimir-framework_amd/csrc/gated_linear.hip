@@ -16,6 +16,10 @@
 // tokens are few), then dx is one product over both weights' columns and dWg, dWu are
 // two batches of another.  The pass is bound by its bytes (20 or 12 a value beside
 // 4 or 12 written), the products by the matrix cores.
+//
+// Measured on MI355X, us: 2048 tokens x 4096 x 11008 bf16 forward 337 (1.10 PFLOP/s); 8192
+// tokens forward and backward 4267 (forward 1553, the pass 257 = 5.6 TB/s, dx 1218, both
+// weights' 1269); 1021 x 1024 x 2752 fp32 both 258; 7 tokens fp32 forward 16.9.
 #include "matrix.hpp"
 #include "pointwise.hpp"
 

@@ -85,6 +85,11 @@ int main() {
         OK(k.fwd());
         k.dw = nullptr;
         FINE(k.bwd());
+        k = Ce{};
+        k.tokens = 0;
+        k.x = k.dx = nullptr;  // no buffer in place of another
+        k.ld_dx = 9;
+        FINE(k.bwd());
     }
 
     // --- gated products

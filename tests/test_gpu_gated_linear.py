@@ -5,6 +5,7 @@ import numpy as np
 import pytest
 
 import mimir_hip as M
+from _serving import bf16_value
 from _training import Mat, UB, U, gated64, gated_bwd64, held, near
 
 pytestmark = pytest.mark.gpu
@@ -150,3 +151,24 @@ def test_same_bits_again(ctx, dtype):
     u, v = run(ctx, *a, "silu", dtype), run(ctx, *a, "silu", dtype)
     for name in u:
         assert np.array_equal(u[name], v[name]), name
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_rows_past_32_bits(ctx, dtype):
+    """gate_up of more than 2^31 values, y of more than 2^32 bytes in fp32: the last rows."""
+    tokens, dim, hidden, last = 70001, 8, 16384, 3
+    x, wg, wu, _ = make(3, tokens, dim, 1, dtype)
+    rng = np.random.default_rng(4)
+    wg, wu = (held(rng.standard_normal((dim, hidden)), dtype) for _ in range(2))
+    X, G, W = Mat(ctx, x, dtype), Mat(ctx, wg, dtype), Mat(ctx, wu, dtype)
+    y = ctx.empty(tokens * hidden, np.float32 if dtype == "f32" else np.uint16)
+    gu = ctx.empty(tokens * 2 * hidden)
+    ctx.gated_linear(X.ptr, G.ptr, W.ptr, y, tokens, dim, hidden, gate_up=gu, dtype=dtype)
+    c = gated64(x[-last:], wg, wu, "silu", dtype)
+    got = y.offset((tokens - last) * hidden, (last, hidden)).numpy()
+    near(bf16_value(got) if dtype == "bf16" else got, c["y"], c["ey"], "y")
+    keep = gu.offset((tokens - last) * 2 * hidden, (last, 2, hidden)).numpy()
+    near(keep[:, 0], c["gate"], c["eg"], "gate")
+    near(keep[:, 1], c["up"], c["eu"], "up")
+    y.free()
+    gu.free()

@@ -365,7 +365,6 @@ int forward(mimir_ctx* ctx, const Call& c, const Plan& p, char* work, void* y, i
             o.out[1] = gate_up + c.hidden;
             o.ld = 2 * c.hidden;
             o.partial = reinterpret_cast<float*>(work + p.partial);
-            o.ld_partial = mat_round(c.hidden, 4);
             o.alpha = 1.0f;
             o.last = 1;
             g.batches = 2;
@@ -427,13 +426,11 @@ int backward(mimir_ctx* ctx, const Call& c, const Plan& p, char* work, const Gra
     ox.out[0] = d.dx;
     ox.ld = d.ld_dx;
     ox.partial = reinterpret_cast<float*>(work + p.partial);
-    ox.ld_partial = mat_round(c.dim, 4);
     ox.alpha = 1.0f;
     ox.bf16 = bf16;
     ox.accumulate = d.accumulate_x;
     MatOut ow = ox;
     ow.partial = reinterpret_cast<float*>(work + p.partial_w);
-    ow.ld_partial = mat_round(std::min(p.piece, c.hidden), 4);
     ow.ld = d.ld_dw;
     ow.accumulate = d.accumulate_w;
     ow.last = 1;

@@ -517,7 +517,6 @@ int backward(mimir_ctx* ctx, const Call& c, const Plan& p, char* work, const Gra
     ox.ld = d.ld_dx;
     ox.row = row;
     ox.partial = reinterpret_cast<float*>(work + p.partial);
-    ox.ld_partial = mat_round(c.dim, 4);
     ox.count = d.mean ? d.mean + 1 : nullptr;
     ox.alpha = d.scale;
     ox.bf16 = bf16;

@@ -17,9 +17,9 @@ __global__ __launch_bounds__(kBlock) void stage_rows(const void* src, int64_t ro
     }
 }
 
-__global__ __launch_bounds__(kBlock) void join_slices(MatOut o, MatArgs g, int bm, int bn) {
+__global__ __launch_bounds__(kBlock) void join_slices(MatOut o, MatArgs g, MatTileSize tile) {
     const int64_t n = g.n_dev ? min(g.n, *g.n_dev) : g.n, slice = n * o.ld_partial;
-    const int32_t splits = g.splits_of(((g.m + bm - 1) / bm) * ((n + bn - 1) / bn));
+    const int32_t splits = g.splits_of(mat_tiles_of(tile, g.m, n, 1));
     const float by = o.factor();
     const int64_t of_row = (g.m + 3) / 4, one = n * of_row, stride = static_cast<int64_t>(gridDim.x) * kBlock;
     for (int64_t i = static_cast<int64_t>(blockIdx.x) * kBlock + threadIdx.x; i < one * g.batches; i += stride) {
@@ -47,9 +47,9 @@ int mimir::mat_stage(mimir_ctx* ctx, int type, const void* src, int64_t rows, in
     return launched(ctx, "stage_rows");
 }
 
-int mimir::mat_join(mimir_ctx* ctx, const MatOut& o, const MatArgs& g, int bm, int bn) {
+int mimir::mat_join(mimir_ctx* ctx, const MatOut& o, const MatArgs& g, MatTileSize tile) {
     if (g.n == 0 || g.m == 0) return MIMIR_OK;
-    join_slices<<<grid_of(static_cast<int64_t>(g.n) * ((g.m + 3) / 4) * g.batches), kBlock, 0, ctx->stream>>>(o, g, bm, bn);
+    join_slices<<<grid_of(static_cast<int64_t>(g.n) * ((g.m + 3) / 4) * g.batches), kBlock, 0, ctx->stream>>>(o, g, tile);
     return launched(ctx, "join_slices");
 }
 

@@ -39,6 +39,7 @@
 #pragma once
 
 #include "internal.hpp"
+#include "matdeal.hpp"
 #include "split.hpp"
 
 #include <algorithm>
@@ -62,14 +63,9 @@ struct MatArgs {
     const int32_t* n_dev;   // not null: n is at most this
     const int32_t* k_dev;   // not null: k is at most this
     int32_t segments, batches;
-    // How many ways the contraction is split: as many as leave the tiles' workgroups at
-    // `fill` (n may be known on the device alone), at most `splits`.  0: once.
-    int32_t fill, splits;
+    int32_t fill, splits;   // how the contraction is split (mat_splits; n may be known on the device alone)
 
-    __host__ __device__ int32_t splits_of(int64_t tiles) const {
-        const int64_t s = fill / (tiles > 0 ? tiles * batches : 1);
-        return fill == 0 || s < 1 ? 1 : s < splits ? static_cast<int32_t>(s) : splits;
-    }
+    __device__ __forceinline__ int32_t splits_of(int64_t tiles) const { return mat_splits(fill, splits, tiles * batches); }
 };
 
 struct MatAt {
@@ -788,7 +784,7 @@ struct MatOut {
     int64_t ld;
     const int32_t* row;       // not null: the row of n
     float* partial;           // [splits][batches][n][ld_partial], not null if read or written
-    int64_t ld_partial;
+    int64_t ld_partial;       // mat_slice_ld(m): mat_product and few_product set it
     const float* count;       // not null: alpha is divided by max(count, 1)
     float alpha;
     int32_t bf16, accumulate;
@@ -884,8 +880,6 @@ struct MatOut {
 
 // --- operands from a caller's matrices (matrix.hip) --------------------------------
 
-constexpr int64_t mat_round(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
-
 // Whether bf16 rows can be an operand as they are.
 inline bool mat_direct(const void* p, int64_t ld, int64_t cols) {
     return aligned16(p) && ld % 8 == 0 && cols % 8 == 0 && mat_ld_fits(ld);
@@ -929,38 +923,11 @@ __device__ __forceinline__ void mat_stage8(const void* src, int64_t at, int64_t 
 // between planes.
 int mat_stage(mimir_ctx* ctx, int type, const void* src, int64_t rows, int64_t cols, int64_t ld, uint16_t* dst, int64_t ld_dst,
               int64_t plane);
-// A product into MatOut: its shape, and how its contraction is dealt to workgroups where
-// the tiles of C alone leave CUs idle.
-struct MatDeal {
-    bool big, thin;
-    int32_t fill, splits;
-    size_t partial;  // bytes of the slices
-};
-
-// The larger tiles where they fill the GPU, or, the contraction split, come to 1 for
-// each CU; else the smaller ones, split to 2 for each CU.  A split has at least 512 of
-// the contraction.  `more`: the sums go through fp32 slices whether split or not.
+// mat_deal_of for the shapes of these planes and layouts.
 template <class BIG, class SMALL, bool HAS_BIG, bool HAS_THIN>
 MatDeal mat_deal(const mimir_ctx* ctx, int64_t m, int64_t n, int64_t k, int64_t batches, bool more) {
-    constexpr int32_t kBigFill = 256, kSmallFill = 512;
-    constexpr int64_t kLeastK = 512;
-    const auto tiles = [&](int64_t bm, int64_t bn) { return (m + bm - 1) / bm * ((n + bn - 1) / bn) * batches; };
-    const int64_t big = tiles(BIG::kM, BIG::kN), most = std::max<int64_t>(1, k / kLeastK);
-    const int64_t big_most = std::max<int64_t>(1, kBigFill / std::max<int64_t>(big, 1));
-    MatDeal d{};
-    d.thin = HAS_THIN && k <= kMatThinK && ctx->tune.mat_big != 1;
-    d.big = HAS_BIG && !d.thin && (ctx->tune.mat_big >= 0 ? ctx->tune.mat_big == 1 : big * std::min(most, big_most) >= kMatBigTiles);
-    d.fill = d.big ? kBigFill : kSmallFill;
-    d.splits = static_cast<int32_t>(std::min<int64_t>(most, 64));
-    const int64_t now = tiles(d.big ? BIG::kM : SMALL::kM, d.big ? BIG::kN : SMALL::kN);
-    // n on the device may be smaller than here: then there are more splits, but no more
-    // tiles' worth of sums than `fill`.
-    if (d.splits == 1 || now >= d.fill) d.splits = 1, d.fill = 0;
-    const int64_t ld = mat_round(m, 4);
-    if (d.splits > 1)
-        d.partial = sizeof(float) * static_cast<size_t>(d.fill * (d.big ? int64_t{BIG::kM} * BIG::kN : int64_t{SMALL::kM} * SMALL::kN) + 4);
-    if (more || d.splits > 1) d.partial = std::max(d.partial, sizeof(float) * static_cast<size_t>(n * ld * batches));
-    return d;
+    return mat_deal_of({{BIG::kM, BIG::kN}, {SMALL::kM, SMALL::kN}, HAS_BIG, HAS_THIN, kMatBigTiles, kMatThinK, ctx->tune.mat_big}, m, n, k,
+                       batches, more);
 }
 template <int PA, int PB, int KA, int KB>
 MatDeal mat_deal(const mimir_ctx* ctx, int64_t m, int64_t n, int64_t k, int64_t batches, bool more) {
@@ -970,8 +937,8 @@ MatDeal mat_deal(const mimir_ctx* ctx, int64_t m, int64_t n, int64_t k, int64_t 
 }
 
 // The sum of the splits' slices into out (MatOut's fields say how) for a product of g in
-// tiles of bm x bn.
-int mat_join(mimir_ctx* ctx, const MatOut& o, const MatArgs& g, int bm, int bn);
+// tiles of `tile`.
+int mat_join(mimir_ctx* ctx, const MatOut& o, const MatArgs& g, MatTileSize tile);
 
 // A product of few n into MatOut through slices: workgroups for about two for each CU,
 // each wave with at least four steps.
@@ -983,6 +950,7 @@ int few_splits(int64_t m, int64_t k, int segments) {
 template <bool FP32, int KA>
 int few_product(mimir_ctx* ctx, const char* what, MatArgs g, MatOut o) {
     const int32_t last = o.last, splits = g.splits, segments = g.segments;
+    o.ld_partial = mat_slice_ld(g.m);
     o.last = last && splits * segments == 1;
     if (int st = few_launch<FP32, KA, false>(ctx, what, g, o)) return st;
     if (!last || o.last) return MIMIR_OK;
@@ -990,7 +958,7 @@ int few_product(mimir_ctx* ctx, const char* what, MatArgs g, MatOut o) {
     g.splits = splits * segments;  // mat_join's: as many slices, whatever the tiles
     g.segments = 1;
     g.fill = INT32_MAX;
-    return mat_join(ctx, o, g, 1 << 24, 1 << 24);
+    return mat_join(ctx, o, g, MatTileSize{1 << 24, 1 << 24});
 }
 
 // C as a result.  o.last: these are the contraction's last pieces.
@@ -998,25 +966,26 @@ template <int PA, int PB, int KA, int KB>
 int mat_product(mimir_ctx* ctx, const char* what, MatArgs g, MatOut o, const MatDeal& d) {
     g.splits = d.splits;
     g.fill = d.fill;
+    o.ld_partial = mat_slice_ld(g.m);
     const int32_t last = o.last;
     if (d.splits > 1) o.last = 0;
     int st = MIMIR_OK;
     using S = MatSmall<PA, PB, KA, KB>;
-    int bm = S::kM, bn = S::kN;
+    MatTileSize tile{S::kM, S::kN};
     if constexpr (PA == PB) {
         using B = MatBig<PA, PB, KA, KB>;
-        if (d.big) {
-            bm = B::kM;
-            bn = B::kN;
-            st = mat_launch<B>(ctx, what, g, o);
-        }
+        if (d.big) tile = MatTileSize{B::kM, B::kN};
     }
+    MIMIR_REQUIRE(ctx, (o.last && !o.read_partial) || mat_slice_bytes(d, tile, g.m, g.n, g.batches) <= d.partial,
+                  "%s: %d x %d in %zu bytes of slices", what, g.m, g.n, d.partial);
+    if constexpr (PA == PB)
+        if (d.big) st = mat_launch<MatBig<PA, PB, KA, KB>>(ctx, what, g, o);
     if constexpr (PA != 3)
         if (d.thin) st = mat_launch<MatThin<PA, PB, KA, KB>>(ctx, what, g, o);
     if (!d.thin && !d.big) st = mat_launch<S>(ctx, what, g, o);
     if (st || d.splits == 1 || !last) return st;
     o.last = 1;
-    return mat_join(ctx, o, g, bm, bn);
+    return mat_join(ctx, o, g, tile);
 }
 
 // The context's scratch of at least `bytes`, also while its stream is being captured:

@@ -588,7 +588,8 @@ int mimir_linear_cross_entropy_fwd(mimir_ctx* ctx, int type, const void* x, int6
  * without mean that of any function of the losses.  dx [tokens][dim] and dw
  * [vocab][dim] have `type` (either may be NULL) and are rounded once; for bf16, G is
  * held in bf16 in between (with at most 128 tokens as two bf16 terms).  dx may be x
- * with the same stride; dw must not overlap the other buffers.  The same call gives the same bits.  Scratch:
+ * with the same stride; dw must not overlap the other buffers.  Without tokens the inputs
+ * may be NULL: dw is zeroed, or left as it is.  The same call gives the same bits.  Scratch:
  * x's rows again, up to 512 MiB (at least 256 rows of w) for G and w's rows, and fp32
  * sums of dx where the vocabulary is taken in pieces or there are few tokens. */
 int mimir_linear_cross_entropy_bwd(mimir_ctx* ctx, int type, const void* x, int64_t ld_x, const void* w, int64_t ld_w,
@@ -619,7 +620,8 @@ int mimir_gated_linear_fwd(mimir_ctx* ctx, int type, int act, const void* x, int
  * [dim][hidden] (both ld_dw) likewise with accumulate_w; all of `type`, rounded once.
  * dx, or dWg and dWu together, may be NULL.  For bf16, dg and du are held in bf16 in
  * between (with at most 128 tokens as two bf16 terms).  Outputs must not overlap the
- * inputs or one another.  The same call gives the same bits.  Scratch: as the
+ * inputs or one another.  Without tokens the inputs may be NULL: dWg and dWu are zeroed,
+ * or left as they are.  The same call gives the same bits.  Scratch: as the
  * forward's, up to 512 MiB (at least 256 columns) with dg and du, and fp32 sums where
  * the columns are taken in pieces or there are few tiles. */
 int mimir_gated_linear_bwd(mimir_ctx* ctx, int type, int act, const void* x, int64_t ld_x, const void* w_gate,

@@ -436,14 +436,12 @@ int backward(mimir_ctx* ctx, const Call& c, const Plan& p, char* work, const Gra
     ow.last = 1;
     for (int64_t first = 0; first < c.hidden; first += p.piece) {
         const int64_t cols = std::min(p.piece, c.hidden - first);
-        const GradArgs a{d.gate_up ? d.gate_up + first : nullptr, c.hidden, static_cast<const char*>(d.dy) + first * size, d.ld_dy,
+        const GradArgs a{d.gate_up + first, c.hidden, static_cast<const char*>(d.dy) + first * size, d.ld_dy,
                          planes, c.tokens, cols, p.piece, plane, p.few ? reinterpret_cast<float*>(work + p.raw) : nullptr};
-        if (c.tokens > 0) {
-            const int64_t blocks = (c.tokens * (p.piece / 8) + kBlock - 1) / kBlock;
-            const auto grid = static_cast<unsigned>(std::min<int64_t>(blocks, 1 << 16));
-            gated_grad<ACT, P == 1, PG><<<grid, kBlock, 0, ctx->stream>>>(a);
-            if (int st = launched(ctx, "gated_grad")) return st;
-        }
+        const int64_t blocks = (c.tokens * (p.piece / 8) + kBlock - 1) / kBlock;
+        const auto grid = static_cast<unsigned>(std::min<int64_t>(blocks, 1 << 16));
+        gated_grad<ACT, P == 1, PG><<<grid, kBlock, 0, ctx->stream>>>(a);
+        if (int st = launched(ctx, "gated_grad")) return st;
         const MatOperand dg{planes, ld_g, plane}, du{planes + p.piece, ld_g, plane};
         if (d.dx) {
             MatArgs g = args_of(c.dim, c.tokens, cols);
@@ -523,10 +521,15 @@ int mimir_gated_linear_bwd(mimir_ctx* ctx, int type, int act, const void* x, int
                   "%s: dw_gate and dw_up must be buffers of their own", what);
     if (tokens == 0 && !dw_gate) return MIMIR_OK;
     MIMIR_ENTER(ctx);
+    if (tokens == 0) {
+        if (accumulate_w) return MIMIR_OK;
+        if (int st = mat_zero(ctx, type, dw_gate, dim, hidden, ld_dw)) return st;
+        return mat_zero(ctx, type, dw_up, dim, hidden, ld_dw);
+    }
     const Plan p = plan_of(ctx, c, true);
     char* work;
     if (int st = mat_scratch(ctx, p.total, &work)) return st;
-    const Gradients d{gate_up, dy, ld_dy, tokens ? dx : nullptr, ld_dx, {dw_gate, dw_up}, ld_dw, accumulate_x ? 1 : 0, accumulate_w ? 1 : 0};
+    const Gradients d{gate_up, dy, ld_dy, dx, ld_dx, {dw_gate, dw_up}, ld_dw, accumulate_x ? 1 : 0, accumulate_w ? 1 : 0};
     const auto run = [&](auto a) {
         constexpr int ACT = decltype(a)::value;
         if (p.p == 3) return backward<3, 3, ACT>(ctx, c, p, work, d);

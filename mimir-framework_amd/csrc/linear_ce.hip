@@ -416,7 +416,6 @@ const char* rows_at(const Call& c, int64_t first) {
 
 int gather(mimir_ctx* ctx, const Call& c, const GatherArgs& a) {
     const auto grid = static_cast<unsigned>((c.tokens + kGatherRows - 1) / kGatherRows);
-    if (grid == 0) return MIMIR_OK;
     if (c.type == MIMIR_NUM_BF16) gather_rows<true><<<grid, kBlock, 0, ctx->stream>>>(a);
     else gather_rows<false><<<grid, kBlock, 0, ctx->stream>>>(a);
     return launched(ctx, "gather_rows");
@@ -566,7 +565,7 @@ int backward(mimir_ctx* ctx, const Call& c, const Plan& p, char* work, const Gra
         }
         if (d.dw) {
             g = args_of(x, gr, c.dim, rows, c.tokens);
-            if (c.tokens > 0) g.k_dev = count;
+            g.k_dev = count;
             ow.out[0] = static_cast<char*>(d.dw) + first * d.ld_dw * size;
             st = mat_product<P, PG, kCols, kCols>(ctx, "cross entropy dw", g, ow, p.deal_w);
             if (st) return st;
@@ -589,13 +588,13 @@ int mimir_linear_cross_entropy_fwd(mimir_ctx* ctx, int type, const void* x, int6
     MIMIR_REQUIRE(ctx, tokens == 0 || (x && w && targets && loss && lse), "%s: null pointer", what);
     if (tokens == 0 && !mean) return MIMIR_OK;
     MIMIR_ENTER(ctx);
-    if (tokens > 0 && few_applies(c))
+    if (tokens == 0) return mimir_fill_f32(ctx, mean, 2, 0.0f);
+    if (few_applies(c))
         return type == MIMIR_NUM_F32 ? forward_few<true>(ctx, c, loss, lse, mean) : forward_few<false>(ctx, c, loss, lse, mean);
     const Plan p = plan_of(ctx, type, w, ld_w, tokens, dim, vocab, false);
     char* work;
     if (int st = mat_scratch(ctx, p.total, &work)) return st;
     auto* count = reinterpret_cast<int32_t*>(work + p.count);
-    if (tokens == 0) return mimir_fill_f32(ctx, mean, 2, 0.0f);
     const GatherArgs a{x, ld_x, targets, tokens, dim, vocab, reinterpret_cast<uint16_t*>(work + p.x), p.ld, tokens * p.ld,
                        nullptr, reinterpret_cast<int32_t*>(work + p.row), count, loss, lse, nullptr, 0};
     if (int st = gather(ctx, c, a)) return st;
@@ -617,6 +616,8 @@ int mimir_linear_cross_entropy_bwd(mimir_ctx* ctx, int type, const void* x, int6
     MIMIR_REQUIRE(ctx, !dx || dx != x || ld_dx == ld_x, "%s: dx in place needs equal strides", what);
     if (!dx && !dw) return MIMIR_OK;
     MIMIR_ENTER(ctx);
+    // Without tokens no input is looked at (w may be null).
+    if (tokens == 0) return dw && !accumulate_w ? mat_zero(ctx, type, dw, vocab, dim, ld_dw) : MIMIR_OK;
     Plan p = plan_of(ctx, type, w, ld_w, tokens, dim, vocab, true);
     char* work;
     if (int st = mat_scratch(ctx, p.total, &work)) return st;

@@ -484,9 +484,7 @@ inline bool mat_ld_fits(int64_t ld) { return ld < (int64_t{1} << 20); }
 template <class S, class Epi>
 int mat_launch(mimir_ctx* ctx, const char* what, const MatArgs& g, const Epi& epi) {
     // Fewer n than there may be have fewer tiles and more splits: `fill` workgroups at most.
-    const int64_t tiles = mat_tiles<S>(g), total = tiles ? std::max<int64_t>(tiles, g.fill) : 0;
-    const int64_t grid = (total + kMatXcds - 1) / kMatXcds * kMatXcds;
-    if (total == 0) return MIMIR_OK;
+    const int64_t grid = mat_round(std::max<int64_t>(mat_tiles<S>(g), g.fill), kMatXcds);
     MIMIR_REQUIRE(ctx, dispatch_fits(grid, S::kThreads), "%s: grid of %lld workgroups exceeds the limit", what, (long long)grid);
     mat_kernel<S, Epi><<<static_cast<unsigned>(grid), S::kThreads, 0, ctx->stream>>>(g, epi);
     return launched(ctx, what);
@@ -923,6 +921,8 @@ __device__ __forceinline__ void mat_stage8(const void* src, int64_t at, int64_t 
 // between planes.
 int mat_stage(mimir_ctx* ctx, int type, const void* src, int64_t rows, int64_t cols, int64_t ld, uint16_t* dst, int64_t ld_dst,
               int64_t plane);
+// A matrix of zeros.
+int mat_zero(mimir_ctx* ctx, int type, void* p, int64_t rows, int64_t cols, int64_t ld);
 // mat_deal_of for the shapes of these planes and layouts.
 template <class BIG, class SMALL, bool HAS_BIG, bool HAS_THIN>
 MatDeal mat_deal(const mimir_ctx* ctx, int64_t m, int64_t n, int64_t k, int64_t batches, bool more) {

@@ -45,8 +45,9 @@ __device__ __forceinline__ f4 ld4(const float* p) {
 // the compiler does not count it in its waits, and a gfx9 wave's vmcnt is
 // in order, so a later wait for a load issued before such a store also
 // waits for the store: use it where every load precedes every store.  The data of a
-// store of more than 8 bytes may be overwritten from the second instruction after it
-// on: the compiler keeps to that for its own stores, and the s_nop for these.
+// store of more than 8 bytes may be overwritten by a vector instruction from two wait
+// states after it on: the compiler keeps to that for its own stores, and the s_nop for
+// these.
 enum : int { kStoreNt = 0, kStoreThrough = 1 };
 
 // A pointer into global memory (address space 1), so stores through it are
@@ -57,7 +58,7 @@ using gptr = __attribute__((address_space(1))) T*;
 template <int POL = kStoreNt>
 __device__ __forceinline__ void st_stream(void* p, u4 v) {
     if constexpr (POL == kStoreThrough) {
-        asm volatile("global_store_dwordx4 %0, %1, off sc1 nt\n\ts_nop 0" : : "v"(p), "v"(v) : "memory");
+        asm volatile("global_store_dwordx4 %0, %1, off sc1 nt\n\ts_nop 1" : : "v"(p), "v"(v) : "memory");
     } else {
         gptr<u4> g = (gptr<u4>)p;
         asm volatile("" : "+v"(g));

@@ -38,8 +38,13 @@ using namespace mimir;
 namespace {
 
 constexpr float kLog2e = 1.44269504088896340736f;
-// Below any logit that counts, and finite times log2 e: the maximum of nothing.
-constexpr float kLowest = -2.0e38f;
+// The maximum of nothing.
+constexpr float kLowest = -3.40282347e38f;
+
+// exp(z - m).  The difference first: z log2 e - m log2 e in one step is off by the rounding
+// of m log2 e, so that the maximum itself would not give 1, a sum could come out below 1
+// and a loss below 0, by more the larger the logits are.
+__device__ __forceinline__ float exp_from(float z, float m) { return __builtin_amdgcn_exp2f((z - m) * kLog2e); }
 
 // --- the counted rows --------------------------------------------------------------
 
@@ -111,10 +116,10 @@ __global__ __launch_bounds__(kBlock) void gather_rows(GatherArgs a) {
 
 // --- forward -----------------------------------------------------------------------
 
-// (max, sum of exp2((z - max) log2 e)) of two sets; an empty one is (-infinity, 0).
+// (max, sum of exp(z - max)) of two sets; an empty one is (-infinity, 0).
 __device__ __forceinline__ f2 join(f2 a, f2 b) {
     const float m = fmaxf(fmaxf(a[0], b[0]), kLowest);
-    return f2{m, a[1] * __builtin_amdgcn_exp2f((a[0] - m) * kLog2e) + b[1] * __builtin_amdgcn_exp2f((b[0] - m) * kLog2e)};
+    return f2{m, a[1] * exp_from(a[0], m) + b[1] * exp_from(b[0], m)};
 }
 
 struct CeStats {
@@ -156,12 +161,12 @@ struct CeStats {
             for (int i = 0; i < S::kBm; ++i)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) m = fmaxf(m, acc.c[i][j][r]);
-            const float top = fmaxf(m, kLowest) * kLog2e;
+            const float top = fmaxf(m, kLowest);
             float s = 0.0f;
 #pragma unroll
             for (int i = 0; i < S::kBm; ++i)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) s += __builtin_amdgcn_exp2f(__builtin_fmaf(acc.c[i][j][r], kLog2e, -top));
+                for (int r = 0; r < 16; ++r) s += exp_from(acc.c[i][j][r], top);
             f2 v = join(f2{m, s}, f2{__shfl_xor(m, 32), __shfl_xor(s, 32)});
             if (threadIdx.x % kWave < 32) red[acc.wm * S::kN + acc.n_of(j)] = v;
         }
@@ -285,7 +290,7 @@ struct CeGrad {
             const bool live = n < at.n;
             const int32_t t = live ? row[n] : 0;
             const int64_t hit = live ? target[t] - first - at.m0 : -1;
-            const float base = live ? lse[t] * kLog2e : 0.0f, w = live && dloss ? dloss[t] : 1.0f;
+            const float base = live ? lse[t] : 0.0f, w = live && dloss ? dloss[t] : 1.0f;
 #pragma unroll
             for (int i = 0; i < S::kBm; ++i)
 #pragma unroll
@@ -294,7 +299,7 @@ struct CeGrad {
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
                         const int32_t m = acc.m_of(i, 8 * h + e);
-                        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(acc.c[i][j][8 * h + e], kLog2e, -base));
+                        const float p = exp_from(acc.c[i][j][8 * h + e], base);
                         v[e] = at.m0 + m < at.m ? (p - (m == hit ? 1.0f : 0.0f)) * w : 0.0f;
                     }
                     if (PG == 3 && raw && live)

@@ -3,7 +3,7 @@ import numpy as np
 import pytest
 
 import mimir_hip as M
-from _training import Mat
+from _training import U, Mat, held
 
 pytestmark = pytest.mark.gpu
 
@@ -29,3 +29,46 @@ def test_no_tokens_no_inputs(ctx, dtype, dim, pad, offset):
         ctx.gated_linear_bwd(None, None, None, None, None, DX.ptr, A.ptr, B.ptr, 0, v, dim, dtype=dtype, ld_x=v, ld_w=dim + pad,
                              ld_dx=v, ld_dw=A.ld, accumulate_w=accumulate)
         assert (A.get() == (3 if accumulate else 0)).all() and (B.get() == A.get()).all() and (DX.get() == 3).all()
+
+
+@pytest.fixture(scope="module", params=["", "matbig=1,matpiece=264", "matbig=0,matpiece=136"], ids=["default", "big", "small"])
+def tuned(request):
+    """A context of its own: the shapes and pieces by rule, or forced."""
+    with pytest.MonkeyPatch.context() as mp:
+        mp.setenv("MIMIR_TUNE", request.param)
+        c = M.Context(0)
+    yield c
+    c.close()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("tokens,vocab", [(20, 700), (32, 64), (33, 500), (150, 900), (400, 5000)])
+def test_dominant_logits(tuned, tokens, vocab, dtype):
+    """Tokens are unit vectors, so logits are the weights' own values, exactly.  One of each token's is far above the
+    others: the sum is 1 plus what counts, the loss of that target is never below 0, and nothing but 0 where the others'
+    exponentials leave fp32; likewise the gradients."""
+    rng = np.random.default_rng(tokens)
+    dim = tokens
+    x = np.eye(tokens, dtype=np.float32)
+    top = held(rng.uniform(5, 3000, tokens) * np.where(rng.random(tokens) < 0.3, -1, 1), dtype)
+    # Half of the tokens' other logits are out of reach (exp of -150 is below 2^-149), half some tens below.
+    far = np.arange(tokens) % 2 == 0
+    gap = np.where(far, rng.uniform(160, 400, (vocab, tokens)), rng.uniform(2, 60, (vocab, tokens)))
+    w = held(top - gap, dtype)
+    target = rng.integers(0, vocab, tokens).astype(np.int32)
+    w[target, np.arange(tokens)] = top
+    assert (np.delete(w, 0, 0) <= top).all()
+    X, W, t = Mat(tuned, x, dtype), Mat(tuned, w, dtype), tuned.to_device(target)
+    loss, lse, mean = (tuned.empty(n) for n in (tokens, tokens, 2))
+    DX, DW = Mat(tuned, x, dtype), Mat(tuned, np.full(w.shape, 9.0), dtype)
+    tuned.linear_cross_entropy(X.ptr, W.ptr, t, tokens, dim, vocab, loss, lse, mean, dtype=dtype)
+    tuned.linear_cross_entropy_bwd(X.ptr, W.ptr, t, lse, None, None, DX.ptr, DW.ptr, tokens, dim, vocab, dtype=dtype)
+    loss, lse = loss.numpy(), lse.numpy()
+    assert (loss >= 0).all() and (lse >= top).all()
+    assert (loss[far] == 0).all() and (lse[far] == top[far]).all()
+    assert (DX.get()[far] == 0).all() and (DW.get()[:, far] == 0).all()
+    # The others: the exponentials' arguments are off by 3 U of a difference of at most 64 (with exp(-d) at most 1 / (e d)
+    # of it, so by 1.2 U), the function by a last place, sums by the number of their terms; lse rounds once.
+    z = w.astype(np.float64)
+    want = top + np.log(np.exp(z - top).sum(0))
+    assert (np.abs(lse - want) <= (5 + 140 + 4 * (vocab / 128 + 1) + 1.01 * np.abs(want)) * U).all()

@@ -72,3 +72,71 @@ def test_dominant_logits(tuned, tokens, vocab, dtype):
     z = w.astype(np.float64)
     want = top + np.log(np.exp(z - top).sum(0))
     assert (np.abs(lse - want) <= (5 + 140 + 4 * (vocab / 128 + 1) + 1.01 * np.abs(want)) * U).all()
+
+
+def plain_cross_entropy(x, w, target):
+    """(loss, lse) in float64, and which tokens count."""
+    ok = (target >= 0) & (target < len(w))
+    z = x.astype(np.float64) @ w.astype(np.float64).T
+    top = z.max(1)
+    lse = np.log(np.exp(z - top[:, None]).sum(1)) + top
+    return np.where(ok, lse - z[np.arange(len(z)), np.where(ok, target, 0)], 0), np.where(ok, lse, 0), ok
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("tokens", [8191, 8192, 8193, 16385, 70001])
+def test_many_tokens_gathered(ctx, tokens, dtype):
+    """Blocks of 8192 targets: all, none, some of them counting, the ends of blocks and of the batch."""
+    rng = np.random.default_rng(tokens)
+    dim, vocab = 8, 24
+    x, w = held(rng.standard_normal((tokens, dim)), dtype), held(rng.standard_normal((vocab, dim)), dtype)
+    target = rng.integers(0, vocab, tokens).astype(np.int32)
+    part = np.arange(tokens) // 4096
+    target[(part % 4 == 1) | ((part % 4 == 2) & (rng.random(tokens) < 0.5))] = -1
+    want, lses, ok = plain_cross_entropy(x, w, target)
+    x[~ok] = np.nan
+    X, W, t = Mat(ctx, x, dtype), Mat(ctx, w, dtype), ctx.to_device(target)
+    loss, lse, mean = (ctx.to_device(np.full(n, 5, np.float32)) for n in (tokens, tokens, 2))
+    ctx.linear_cross_entropy(X.ptr, W.ptr, t, tokens, dim, vocab, loss, lse, mean, dtype=dtype)
+    # |z| up to 20: sums of 8 products, exponentials and the sum of 24 of them are off by fewer than 100 U.
+    assert (np.abs(loss.numpy() - want) <= 100 * U * (1 + np.abs(lses))).all()
+    m = mean.numpy()
+    assert m[1] == ok.sum() and abs(m[0] - want.sum() / ok.sum()) <= 200 * U * (1 + want.sum() / ok.sum())
+    DX = Mat(ctx, np.full(x.shape, 9.0), dtype)
+    ctx.linear_cross_entropy_bwd(X.ptr, W.ptr, t, lse, None, mean, DX.ptr, None, tokens, dim, vocab, dtype=dtype)
+    prob = np.exp(np.where(ok[:, None], x, 0).astype(np.float64) @ w.astype(np.float64).T - lses[:, None])
+    g = prob.copy()
+    g[np.arange(tokens)[ok], target[ok]] -= 1
+    g, prob = (np.where(ok[:, None], v, 0) / ok.sum() for v in (g, prob))
+    # The exponentials are off by their arguments' errors (|z| up to 20), fewer than 150 U in all; G and the result round
+    # once each.
+    bound = (prob * 150 * U + np.abs(g) * (2 * 2.0 ** -8 if dtype == "bf16" else 20 * U)) @ np.abs(w.astype(np.float64)) * 1.1
+    assert (np.abs(DX.get() - g @ w.astype(np.float64)) <= bound).all() and (DX.get()[~ok] == 0).all()
+
+
+def test_time_is_linear_in_tokens(ctx):
+    """Eight times the tokens may take some eight times as long, not sixty."""
+    dim, vocab, most = 8, 16, 1 << 22
+    x, w, t = ctx.empty((most, dim)), ctx.empty((vocab, dim)), ctx.empty(most, np.int32)
+    loss, lse, mean, dx = ctx.empty(most), ctx.empty(most), ctx.empty(2), ctx.empty((most, dim))
+    ctx.fill(x, 0.5)
+    ctx.fill(w, 0.25)
+    ctx.upload(t, (np.arange(most) % 17 - 1).astype(np.int32))
+
+    def timed(n):
+        best = 1e9
+        for _ in range(4):
+            a, b = M.Event(ctx), M.Event(ctx)
+            a.record()
+            ctx.linear_cross_entropy(x, w, t, n, dim, vocab, loss, lse, mean)
+            ctx.linear_cross_entropy_bwd(x, w, t, lse, None, mean, dx, None, n, dim, vocab)
+            b.record()
+            ctx.sync()
+            best = min(best, a.elapsed_ms(b))
+        return best
+
+    small, large = timed(most // 8), timed(most)
+    count = (most - 1) // 17 * 16 + (most - 1) % 17  # every 17th token has no target, the first among them
+    assert mean.numpy()[1] == np.float32(count)
+    assert np.allclose(loss.numpy()[1:17], np.log(vocab), rtol=1e-6)
+    assert large < 24 * small, (small, large)

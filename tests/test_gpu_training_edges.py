@@ -140,3 +140,45 @@ def test_time_is_linear_in_tokens(ctx):
     assert mean.numpy()[1] == np.float32(count)
     assert np.allclose(loss.numpy()[1:17], np.log(vocab), rtol=1e-6)
     assert large < 24 * small, (small, large)
+
+
+@pytest.mark.parametrize("beside", [False, True])
+def test_clipping_of_thousands_of_tensors(ctx, beside):
+    """More launches than the clipping adds up the sums of by itself: 4000 tensors of one to some hundred elements."""
+    rng = np.random.default_rng(5)
+    sizes = rng.integers(0, 300, 4000)
+    start = np.concatenate([[0], np.cumsum(sizes)])
+    v = (rng.standard_normal(start[-1]) * np.repeat(10.0 ** rng.uniform(-2, 2, 4000), sizes)).astype(np.float32)
+    d = ctx.to_device(v)
+    out = ctx.to_device(np.zeros_like(v)) if beside else d
+    tensors = M.TensorList([(d.ptr + 4 * int(a), int(n), "f32", out.ptr + 4 * int(a)) for a, n in zip(start, sizes)])
+    norm = ctx.empty(2)
+    ctx.grad_norm(tensors, norm)
+    ctx.grad_clip(tensors, 2.5, norm.offset(1))
+    want = np.sqrt((v.astype(np.float64) ** 2).sum())
+    n = norm.numpy()
+    assert n[0] == n[1] and abs(n[0] - want) <= 1.01 * U * want
+    clipped = v * (2.5 / (want + 1e-6))
+    assert (np.abs(out.numpy() - clipped) <= 3.1 * U * np.abs(clipped)).all()
+
+
+def test_time_is_linear_in_tensors(ctx):
+    """Five times the tensors may take some five times as long, not fifteen."""
+    d, norm = ctx.empty(64 * 100000), ctx.empty(1)
+    ctx.fill(d, 0.5)
+
+    def timed(count):
+        tensors = M.TensorList([(d.ptr + 256 * i, 64, "f32") for i in range(count)])
+        best = 1e9
+        for _ in range(3):
+            a, b = M.Event(ctx), M.Event(ctx)
+            a.record()
+            ctx.grad_clip(tensors, 1e9, norm)
+            b.record()
+            ctx.sync()
+            best = min(best, a.elapsed_ms(b))
+        return best
+
+    small, large = timed(20000), timed(100000)
+    assert abs(norm.numpy()[0] - 0.5 * np.sqrt(64 * 100000)) < 1e-3
+    assert large < 9 * small, (small, large)

@@ -145,10 +145,11 @@ __global__ __launch_bounds__(kBlock) void clip(List l, const double* sums, int32
     const double n = sqrt(total_of(sums, count, lds));
     if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = static_cast<float>(n);
     const double ratio = static_cast<double>(max_norm) / (n + 1e-6);
-    // A NaN stays one.  A factor below fp32's normal values, of elements near its
-    // largest, goes in two: the first is 2^64 times it, with all its bits.
-    const float after = ratio < 0x1p-100 ? 0x1p-64f : 1.0f;
-    const float by = ratio > 1.0 ? 1.0f : static_cast<float>(ratio < 0x1p-100 ? ratio * 0x1p64 : ratio);
+    // A NaN stays one.  A factor that fp32 does not hold with all its bits, of elements
+    // near fp32's largest, multiplies in 64 bits.
+    const bool tiny = ratio < 0x1p-126;
+    const float by = ratio > 1.0 ? 1.0f : static_cast<float>(ratio);
+    const auto scaled = [&](float x) { return tiny ? static_cast<float>(static_cast<double>(x) * ratio) : x * by; };
     const int32_t chunks = l.first[l.count];
     for (int32_t c = chunks - 1 - static_cast<int32_t>(blockIdx.x); c >= 0; c -= gridDim.x) {
         const Chunk k = chunk_of(l, c);
@@ -163,12 +164,12 @@ __global__ __launch_bounds__(kBlock) void clip(List l, const double* sums, int32
                 with_vectors<4, u4>(p, 8, done, [&](int64_t i, u4 v) {
                     u4 y;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) y[e] = pack_bf16(bf16_at(v[e], 0) * by * after, bf16_at(v[e], 1) * by * after);
+                    for (int e = 0; e < 4; ++e) y[e] = pack_bf16(scaled(bf16_at(v[e], 0)), scaled(bf16_at(v[e], 1)));
                     st_stream(q + i, y);
                 });
             }
             for (int64_t i = done + threadIdx.x; i < k.n; i += kBlock) {
-                const float y = bf16_at(p[i], 0) * by * after;
+                const float y = scaled(bf16_at(p[i], 0));
                 q[i] = static_cast<uint16_t>(pack_bf16(y, y));
             }
         } else {
@@ -176,9 +177,9 @@ __global__ __launch_bounds__(kBlock) void clip(List l, const double* sums, int32
             float* q = static_cast<float*>(l.out[k.tensor]) + k.at;
             if (vec) {
                 done = k.n / 4 * 4;
-                with_vectors<8, f4>(p, 4, done, [&](int64_t i, f4 v) { st_stream(q + i, v * by * after); });
+                with_vectors<8, f4>(p, 4, done, [&](int64_t i, f4 v) { st_stream(q + i, f4{scaled(v[0]), scaled(v[1]), scaled(v[2]), scaled(v[3])}); });
             }
-            for (int64_t i = done + threadIdx.x; i < k.n; i += kBlock) q[i] = p[i] * by * after;
+            for (int64_t i = done + threadIdx.x; i < k.n; i += kBlock) q[i] = scaled(p[i]);
         }
     }
 }

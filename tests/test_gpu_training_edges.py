@@ -182,3 +182,20 @@ def test_time_is_linear_in_tensors(ctx):
     small, large = timed(20000), timed(100000)
     assert abs(norm.numpy()[0] - 0.5 * np.sqrt(64 * 100000)) < 1e-3
     assert large < 9 * small, (small, large)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("most,scale", [(1e-30, 1e38), (1e-38, 3e38), (1e-45, 3e38), (1e-20, 1e37), (3e-8, 1e30), (1e-38, 1e-37), (0.0, 1e38)])
+def test_clipping_by_tiny_factors(ctx, most, scale, kind):
+    """Factors far below fp32's range, of elements near its largest: the products are in it."""
+    rng = np.random.default_rng(6)
+    most = float(np.float32(most))
+    v = held((rng.uniform(0.3, 1, 5003) * scale * rng.choice([-1, 1], 5003)).astype(np.float32), kind)
+    m = Mat(ctx, v[None], kind)
+    ctx.grad_clip(M.TensorList([(m.ptr, v.size, kind)]), most)
+    norm = np.sqrt((v.astype(np.float64) ** 2).sum())
+    want = v.astype(np.float64) * (most / (norm + 1e-6))
+    # One rounding of the factor and one of the product; bf16 one more, and its subnormals' half step.
+    half = U * 2.01 + (1.001 * 2.0 ** -8 if kind == "bf16" else 0)
+    tiny = 2.0 ** -134 + 2.0 ** -150 if kind == "bf16" else 2.0 ** -150
+    assert (np.abs(m.get()[0] - want) <= half * np.abs(want) + tiny).all()

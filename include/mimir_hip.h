@@ -645,8 +645,9 @@ int mimir_grad_norm(mimir_ctx* ctx, const mimir_tensor* tensors, int64_t count, 
 
 /* out = data * min(1, max_norm / (norm + 1e-6)) of every tensor, norm as
  * mimir_grad_norm's, written to *norm (device) unless NULL.  Where the factor is 1,
- * tensors in place are left alone.  A NaN norm makes every element NaN, an infinite
- * one finite elements 0.  max_norm >= 0.  No out may overlap another tensor.  The list
+ * tensors in place are left alone.  A NaN among the elements makes every element NaN, an
+ * infinity makes the finite ones 0 and itself NaN.  max_norm >= 0; an infinite one clips
+ * nothing (but for a NaN).  No out may overlap another tensor.  The list
  * is read within the call, so a captured call keeps the addresses.  Scratch: 16 KiB for
  * each 96 tensors. */
 int mimir_grad_clip(mimir_ctx* ctx, const mimir_tensor* tensors, int64_t count, float max_norm, float* norm);

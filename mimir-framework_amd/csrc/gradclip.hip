@@ -144,7 +144,8 @@ __global__ __launch_bounds__(kBlock) void clip(List l, const double* sums, int32
     __shared__ double lds[kBlock / kWave];
     const double n = sqrt(total_of(sums, count, lds));
     if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = static_cast<float>(n);
-    const double ratio = static_cast<double>(max_norm) / (n + 1e-6);
+    // An infinite max_norm clips nothing, also where the norm is infinite.
+    const double ratio = isinf(max_norm) && !isnan(n) ? 2.0 : static_cast<double>(max_norm) / (n + 1e-6);
     // A NaN stays one.  A factor that fp32 does not hold with all its bits, of elements
     // near fp32's largest, multiplies in 64 bits.
     const bool tiny = ratio < 0x1p-126;

@@ -199,3 +199,17 @@ def test_clipping_by_tiny_factors(ctx, most, scale, kind):
     half = U * 2.01 + (1.001 * 2.0 ** -8 if kind == "bf16" else 0)
     tiny = 2.0 ** -134 + 2.0 ** -150 if kind == "bf16" else 2.0 ** -150
     assert (np.abs(m.get()[0] - want) <= half * np.abs(want) + tiny).all()
+
+
+@pytest.mark.parametrize("beside", [False, True])
+def test_infinite_bound_clips_nothing(ctx, beside):
+    for bad in (None, np.inf, -np.inf, np.nan):
+        v = np.linspace(-3, 5, 9000).astype(np.float32)
+        if bad is not None:
+            v[77] = bad
+        d = ctx.to_device(v)
+        out = ctx.to_device(np.zeros_like(v)) if beside else d
+        norm = ctx.empty(1)
+        ctx.grad_clip(M.TensorList([(d, v.size, "f32", out)]), np.inf, norm)
+        got = out.numpy()
+        assert np.isnan(got).all() if bad is np.nan else np.array_equal(got, v)

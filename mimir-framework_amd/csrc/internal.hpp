@@ -54,10 +54,12 @@ struct mimir_ctx {
     // (kept allocated) rather than freed; the retired buffers are freed when
     // the last graph goes.
     int graph_pins = 0;
-    // A call was captured whose scratch a graph of the program holds (matrix.hip):
-    // one pin for the context's life.
-    bool captured = false;
     std::vector<void*> retired;
+    // A graph of the program's own holds the address of the scratch (a captured call,
+    // matrix.hip).  The library does not see that graph end: such a scratch is kept, in
+    // `held` once it had to grow, as long as the context.
+    bool scratch_held = false;
+    std::vector<void*> held;
 };
 
 struct mimir_event {
@@ -108,8 +110,11 @@ inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 
 
 // Context scratch of at least `bytes` (runtime.hip).  Growing it waits for
 // the work already enqueued, which may still read the old buffer (or, while
-// captured graphs hold its address, retires the old buffer instead).
+// captured graphs hold its address, retires the old buffer instead, and keeps one that
+// a graph of the program's holds).
 int ensure_scratch(mimir_ctx* ctx, size_t bytes, void** out);
+// The same for a call that may be captured: then the scratch counts as held.
+int captured_scratch(mimir_ctx* ctx, size_t bytes, void** out);
 
 // Free a device buffer that enqueued work or captured graphs may still use:
 // retired while graphs are alive, else freed after the stream drains.

@@ -74,23 +74,8 @@ int mimir::mat_join(mimir_ctx* ctx, const MatOut& o, const MatArgs& g, MatTileSi
 }
 
 int mimir::mat_scratch(mimir_ctx* ctx, size_t bytes, char** out) {
-    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
-    const hipError_t e = hipStreamIsCapturing(ctx->stream, &status);
-    if (e != hipSuccess) return hip_fail(ctx, e, "hipStreamIsCapturing");
     void* p = nullptr;
-    int st;
-    if (status == hipStreamCaptureStatusNone) {
-        st = ensure_scratch(ctx, bytes, &p);
-    } else {
-        // A graph will hold the scratch's address: nothing of it is freed before the
-        // context is.  An allocation is no part of the graph.
-        if (!ctx->captured) graph_pin(ctx);
-        ctx->captured = true;
-        hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
-        if (hipThreadExchangeStreamCaptureMode(&mode) != hipSuccess) return fail(ctx, MIMIR_EDEVICE, "hipThreadExchangeStreamCaptureMode");
-        st = ensure_scratch(ctx, bytes, &p);
-        (void)hipThreadExchangeStreamCaptureMode(&mode);
-    }
+    const int st = captured_scratch(ctx, bytes, &p);
     *out = static_cast<char*>(p);
     return st;
 }

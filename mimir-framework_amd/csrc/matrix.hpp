@@ -988,9 +988,8 @@ int mat_product(mimir_ctx* ctx, const char* what, MatArgs g, MatOut o, const Mat
     return mat_join(ctx, o, g, tile);
 }
 
-// The context's scratch of at least `bytes`, also while its stream is being captured:
-// then the old one, which the graph or one before it may hold, is kept as long as the
-// context.
+// The context's scratch of at least `bytes`, also while its stream is being captured
+// (captured_scratch).
 int mat_scratch(mimir_ctx* ctx, size_t bytes, char** out);
 
 }  // namespace mimir

@@ -63,6 +63,15 @@ unsigned stride_grid(int64_t n) {
     return static_cast<unsigned>(b < 1 ? 1 : (b > 65536 ? 65536 : b));
 }
 
+// What enqueued work may still use, once that is done.
+int free_retired(mimir_ctx* ctx) {
+    hipError_t e = hipStreamSynchronize(ctx->stream);
+    if (e != hipSuccess) return hip_fail(ctx, e, "hipStreamSynchronize");
+    for (void* p : ctx->retired) (void)hipFree(p);
+    ctx->retired.clear();
+    return MIMIR_OK;
+}
+
 }  // namespace
 
 int mimir::retire_or_free(mimir_ctx* ctx, void* p) {
@@ -71,31 +80,34 @@ int mimir::retire_or_free(mimir_ctx* ctx, void* p) {
         ctx->retired.push_back(p);
         return MIMIR_OK;
     }
-    hipError_t e = hipStreamSynchronize(ctx->stream);
-    if (e != hipSuccess) return hip_fail(ctx, e, "hipStreamSynchronize");
-    (void)hipFree(p);
-    return MIMIR_OK;
+    ctx->retired.push_back(p);  // beside those that a capture left, if any
+    return free_retired(ctx);
 }
 
 void mimir::graph_pin(mimir_ctx* ctx) { ++ctx->graph_pins; }
 
 int mimir::graph_unpin(mimir_ctx* ctx) {
     if (--ctx->graph_pins > 0 || ctx->retired.empty()) return MIMIR_OK;
-    hipError_t e = hipStreamSynchronize(ctx->stream);
-    if (e != hipSuccess) return hip_fail(ctx, e, "hipStreamSynchronize");
-    for (void* p : ctx->retired) (void)hipFree(p);
-    ctx->retired.clear();
-    return MIMIR_OK;
+    return free_retired(ctx);
 }
 
 int mimir::ensure_scratch(mimir_ctx* ctx, size_t bytes, void** out) {
     if (bytes > ctx->scratch_bytes) {
+        size_t want = bytes < (size_t(1) << 20) ? (size_t(1) << 20) : bytes;
         if (ctx->scratch) {
-            if (int st = retire_or_free(ctx, ctx->scratch)) return st;
+            if (ctx->scratch_held) {
+                // By half at least, so that captures of larger and larger calls keep no
+                // more than some times the last one's.
+                const size_t half_more = ctx->scratch_bytes + ctx->scratch_bytes / 2;
+                if (half_more > want) want = half_more;
+                ctx->held.push_back(ctx->scratch);
+            } else if (int st = retire_or_free(ctx, ctx->scratch)) {
+                return st;
+            }
             ctx->scratch = nullptr;
             ctx->scratch_bytes = 0;
+            ctx->scratch_held = false;
         }
-        const size_t want = bytes < (size_t(1) << 20) ? (size_t(1) << 20) : bytes;
         hipError_t e = hipMalloc(&ctx->scratch, want);
         if (e != hipSuccess) {
             (void)hipGetLastError();
@@ -106,6 +118,26 @@ int mimir::ensure_scratch(mimir_ctx* ctx, size_t bytes, void** out) {
     }
     *out = ctx->scratch;
     return MIMIR_OK;
+}
+
+int mimir::captured_scratch(mimir_ctx* ctx, size_t bytes, void** out) {
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    const hipError_t e = hipStreamIsCapturing(ctx->stream, &status);
+    if (e != hipSuccess) return hip_fail(ctx, e, "hipStreamIsCapturing");
+    if (status == hipStreamCaptureStatusNone) return ensure_scratch(ctx, bytes, out);
+    // An allocation is no part of the graph.  A scratch that is too small and that no
+    // graph holds cannot be freed now, when the stream cannot be waited for.
+    if (bytes > ctx->scratch_bytes && ctx->scratch && !ctx->scratch_held) {
+        ctx->retired.push_back(ctx->scratch);
+        ctx->scratch = nullptr;
+        ctx->scratch_bytes = 0;
+    }
+    hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
+    if (hipThreadExchangeStreamCaptureMode(&mode) != hipSuccess) return fail(ctx, MIMIR_EDEVICE, "hipThreadExchangeStreamCaptureMode");
+    const int st = ensure_scratch(ctx, bytes, out);
+    (void)hipThreadExchangeStreamCaptureMode(&mode);
+    if (st == MIMIR_OK) ctx->scratch_held = true;
+    return st;
 }
 
 namespace {
@@ -171,6 +203,7 @@ int mimir_ctx_destroy(mimir_ctx* ctx) {
         if (ctx->fixed_work) (void)hipFree(ctx->fixed_work);
         if (ctx->paged_work) (void)hipFree(ctx->paged_work);
         for (void* p : ctx->retired) (void)hipFree(p);
+        for (void* p : ctx->held) (void)hipFree(p);
         (void)hipStreamDestroy(ctx->own_stream);
     }
     noalloc_scratch_release(ctx);  // after the stream drained (or could not be entered)

@@ -1,8 +1,11 @@
 """Calls of the training operators at the edges of what their documentation allows."""
+import ctypes
+
 import numpy as np
 import pytest
 
 import mimir_hip as M
+from _serving import Graph, Hip
 from _training import U, Mat, held
 
 pytestmark = pytest.mark.gpu
@@ -213,3 +216,70 @@ def test_infinite_bound_clips_nothing(ctx, beside):
         ctx.grad_clip(M.TensorList([(d, v.size, "f32", out)]), np.inf, norm)
         got = out.numpy()
         assert np.isnan(got).all() if bad is np.nan else np.array_equal(got, v)
+
+
+def test_scratch_after_a_capture_is_bounded():
+    """A captured call keeps the scratch that its graph holds; eager calls of more and more tokens after it leave no more
+    than that and their own behind, and the graph goes on giving its results."""
+    rng = np.random.default_rng(8)
+    dim, vocab, n, step = 64, 40, 50, 60000
+    with M.Context(0) as c:
+        hip = Hip(c)
+
+        def free_bytes():
+            c.sync()
+            free, total = ctypes.c_size_t(), ctypes.c_size_t()
+            hip("hipMemGetInfo", ctypes.byref(free), ctypes.byref(total))
+            return free.value
+
+        most = 20 * step
+        x, w = c.empty((most, dim)), c.to_device(rng.standard_normal((vocab, dim)).astype(np.float32))
+        c.fill(x, 0.125)
+        t = c.to_device((np.arange(most) % vocab).astype(np.int32))
+        loss, lse, mean = c.empty(most), c.empty(most), c.empty(2)
+        small = [c.to_device(rng.standard_normal((n, dim)).astype(np.float32)), c.empty(n), c.empty(n), c.empty(2)]
+        call = lambda: c.linear_cross_entropy(small[0], w, t, n, dim, vocab, *small[1:])  # noqa: E731
+        graphs = [Graph(c, call)]
+        graphs[0].launch()
+        want = small[1].numpy()
+        before, sizes = free_bytes(), []
+        for i in range(1, 21):
+            c.linear_cross_entropy(x, w, t, i * step, dim, vocab, loss, lse, mean)
+            assert mean.numpy()[1] == i * step
+            if i == 10:
+                graphs.append(Graph(c, call))
+            sizes.append(before - free_bytes())
+        # The rows' three planes alone, 6 bytes an element; the scratch of the second capture's time stays beside the
+        # last one, which is larger by half than it needs at most.  A buffer for each call would be ten times the last.
+        last = 6 * dim * most
+        assert last < sizes[-1] < 2.5 * last, sizes
+        for g in graphs * 2:
+            small[1].upload(np.zeros(n, np.float32))
+            g.launch()
+            c.linear_cross_entropy(x, w, t, 1000, dim, vocab, loss, lse, mean)
+            assert np.array_equal(small[1].numpy(), want)
+        for g in graphs:
+            g.close()
+
+
+def test_captures_that_grow(ctx):
+    """Captures of larger and larger calls, each the first of its size, replayed in any order."""
+    rng = np.random.default_rng(9)
+    dim, vocab = 72, 300
+    with M.Context(0) as c:
+        w = c.to_device((rng.standard_normal((vocab, dim)) / 8).astype(np.float32))
+        calls, graphs, wants = [], [], []
+        for n in (40, 700, 9000, 30000):
+            x, t = c.to_device(rng.standard_normal((n, dim)).astype(np.float32)), c.to_device(rng.integers(-1, vocab, n).astype(np.int32))
+            loss, lse, mean = c.empty(n), c.empty(n), c.empty(2)
+            calls.append((x, t, n, loss, lse, mean))
+            graphs.append(Graph(c, lambda: c.linear_cross_entropy(x, w, t, n, dim, vocab, loss, lse, mean)))
+        for x, t, n, loss, lse, mean in calls:
+            c.linear_cross_entropy(x, w, t, n, dim, vocab, loss, lse, mean)
+            wants.append(loss.numpy())
+        for i in (3, 0, 2, 1, 0, 3):
+            calls[i][3].upload(np.full(calls[i][2], 7, np.float32))
+            graphs[i].launch()
+            assert np.array_equal(calls[i][3].numpy(), wants[i]), i
+        for g in graphs:
+            g.close()

@@ -588,7 +588,7 @@ int mimir_linear_cross_entropy_fwd(mimir_ctx* ctx, int type, const void* x, int6
  * without mean that of any function of the losses.  dx [tokens][dim] and dw
  * [vocab][dim] have `type` (either may be NULL) and are rounded once; for bf16, G is
  * held in bf16 in between (with at most 128 tokens as two bf16 terms).  dx may be x
- * with the same stride; dw must not overlap the other buffers.  Without tokens the inputs
+ * with the same stride; they must not overlap any other buffer.  Without tokens the inputs
  * may be NULL: dw is zeroed, or left as it is.  The same call gives the same bits.  Scratch:
  * x's rows again, up to 512 MiB (at least 256 rows of w) for G and w's rows, and fp32
  * sums of dx where the vocabulary is taken in pieces or there are few tokens. */

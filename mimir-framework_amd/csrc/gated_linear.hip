@@ -489,7 +489,7 @@ int mimir_gated_linear_fwd(mimir_ctx* ctx, int type, int act, const void* x, int
     MIMIR_REQUIRE(ctx, ld_y >= hidden, "%s: row stride %lld below hidden", what, (long long)ld_y);
     if (tokens == 0) return MIMIR_OK;
     MIMIR_REQUIRE(ctx, x && w_gate && w_up && y, "%s: null pointer", what);
-    MIMIR_REQUIRE(ctx, y != x, "%s: y must not be x", what);
+    MIMIR_REQUIRE(ctx, mat_apart({y, gate_up}, {x, w_gate, w_up}), "%s: an output is an input or another output", what);
     MIMIR_ENTER(ctx);
     if (few_applies(c)) {
         if (type == MIMIR_NUM_F32) return act == kSilu ? forward_few<true, kSilu>(ctx, c, y, ld_y, gate_up) : forward_few<true, kGelu>(ctx, c, y, ld_y, gate_up);
@@ -516,9 +516,7 @@ int mimir_gated_linear_bwd(mimir_ctx* ctx, int type, int act, const void* x, int
                   (long long)ld_dx, (long long)ld_dw);
     if (!dx && !dw_gate) return MIMIR_OK;
     MIMIR_REQUIRE(ctx, tokens == 0 || (x && w_gate && w_up && gate_up && dy), "%s: null pointer", what);
-    MIMIR_REQUIRE(ctx, !dx || (dx != x && dx != dy && dx != w_gate && dx != w_up), "%s: dx must not be an input", what);
-    MIMIR_REQUIRE(ctx, !dw_gate || (dw_gate != w_gate && dw_gate != w_up && dw_up != w_gate && dw_up != w_up && dw_gate != dw_up),
-                  "%s: dw_gate and dw_up must be buffers of their own", what);
+    MIMIR_REQUIRE(ctx, mat_apart({dx, dw_gate, dw_up}, {x, w_gate, w_up, gate_up, dy}), "%s: an output is an input or another output", what);
     if (tokens == 0 && !dw_gate) return MIMIR_OK;
     MIMIR_ENTER(ctx);
     if (tokens == 0) {

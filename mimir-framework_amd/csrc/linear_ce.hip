@@ -629,6 +629,7 @@ int mimir_linear_cross_entropy_fwd(mimir_ctx* ctx, int type, const void* x, int6
     const Call c{type, x, ld_x, w, ld_w, targets, tokens, dim, vocab};
     if (int st = check(ctx, what, c)) return st;
     MIMIR_REQUIRE(ctx, tokens == 0 || (x && w && targets && loss && lse), "%s: null pointer", what);
+    MIMIR_REQUIRE(ctx, mat_apart({loss, lse, mean}, {x, w, targets}), "%s: an output is an input or another output", what);
     if (tokens == 0 && !mean) return MIMIR_OK;
     MIMIR_ENTER(ctx);
     if (tokens == 0) return mimir_fill_f32(ctx, mean, 2, 0.0f);
@@ -655,7 +656,8 @@ int mimir_linear_cross_entropy_bwd(mimir_ctx* ctx, int type, const void* x, int6
     MIMIR_REQUIRE(ctx, (!dx || ld_dx >= dim) && (!dw || ld_dw >= dim), "%s: gradient strides (%lld, %lld) below dim", what,
                   (long long)ld_dx, (long long)ld_dw);
     MIMIR_REQUIRE(ctx, tokens == 0 || (x && w && targets && lse), "%s: null pointer", what);
-    MIMIR_REQUIRE(ctx, !dw || dw != w, "%s: dw must not be w", what);
+    MIMIR_REQUIRE(ctx, mat_apart({dw}, {x, w, targets, lse, dloss, mean}) && mat_apart({dx, dw}, {w, targets, lse, dloss, mean}),
+                  "%s: dx may be x, and no other output an input", what);
     MIMIR_REQUIRE(ctx, !dx || dx != x || ld_dx == ld_x, "%s: dx in place needs equal strides", what);
     if (!dx && !dw) return MIMIR_OK;
     MIMIR_ENTER(ctx);

@@ -43,6 +43,7 @@
 #include "split.hpp"
 
 #include <algorithm>
+#include <initializer_list>
 #include <type_traits>
 
 namespace mimir {
@@ -986,6 +987,15 @@ int mat_product(mimir_ctx* ctx, const char* what, MatArgs g, MatOut o, const Mat
     if (st || d.splits == 1 || !last) return st;
     o.last = 1;
     return mat_join(ctx, o, g, tile);
+}
+
+// Whether no output is one of the inputs or another output.
+inline bool mat_apart(std::initializer_list<const void*> outputs, std::initializer_list<const void*> inputs) {
+    for (auto o = outputs.begin(); o != outputs.end(); ++o) {
+        if (!*o) continue;
+        if (std::find(inputs.begin(), inputs.end(), *o) != inputs.end() || std::find(o + 1, outputs.end(), *o) != outputs.end()) return false;
+    }
+    return true;
 }
 
 // The context's scratch of at least `bytes`, also while its stream is being captured

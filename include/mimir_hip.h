@@ -570,7 +570,8 @@ int mimir_embedding_f32ids_bwd(mimir_ctx* ctx, const float* ids, int64_t n_ids, 
  * loss and lse are 0, and what stands in their rows of x reaches nothing.  fp32
  * products are as exact as fp32 arithmetic (three bf16 terms an operand, fp32 sums),
  * bf16 ones exact with fp32 sums; the exponentials' sums are fp32, and
- * exponentials below 2^-126 count as 0.  An infinity, a
+ * exponentials below 2^-126 count as 0.  An fp32 value below 2^-110 keeps an absolute
+ * precision of 2^-134 in a product, so fewer than 24 bits.  An infinity, a
  * NaN or a magnitude above 3.38e38 in x (of a token that counts) or w may give NaN in
  * whatever it is summed into.  mean may be NULL.  tokens and vocab up to 2^24, dim up
  * to 2^18.  Scratch (the context's): x's rows again (fp32: 6 bytes an element), 8

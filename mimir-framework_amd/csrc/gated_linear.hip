@@ -291,7 +291,7 @@ Plan plan_of(const mimir_ctx* ctx, const Call& c, bool back) {
         }
         if (p.few) {
             p.raw = take(static_cast<size_t>(2 * c.tokens * c.hidden * 4));
-            p.deal_x.splits = few_splits<true, kRows>(c.dim, c.hidden, 2);
+            p.deal_x.splits = few_splits(c.dim, c.hidden, 2);
             p.deal_x.partial = static_cast<size_t>(2 * p.deal_x.splits * c.tokens * mat_round(c.dim, 4) * 4);
         }
         p.partial = take(p.deal_x.partial);
@@ -455,7 +455,7 @@ int backward(mimir_ctx* ctx, const Call& c, const Plan& p, char* work, const Gra
                     g.b[i] = MatOperand{reinterpret_cast<const uint16_t*>(a.raw + i * c.tokens * c.hidden), c.hidden, 0};
                 }
                 g.splits = p.deal_x.splits;
-                if constexpr (P == 3) st = few_product<true, kRows>(ctx, "gated dx", g, ox);
+                if constexpr (P == 3) st = few_product<kRows>(ctx, "gated dx", g, ox);
             } else if (st = weights(ctx, c, p, work, first, cols, g.a); st == MIMIR_OK) {
                 g.b[0] = dg;
                 g.b[1] = du;

@@ -408,7 +408,7 @@ Plan plan_of(const mimir_ctx* ctx, int type, const void* w, int64_t ld_w, int64_
         if (p.few) {
             p.raw_x = take(static_cast<size_t>(tokens * dim * 4));
             p.raw_g = take(static_cast<size_t>(tokens * mat_round(vocab, 4) * 4));
-            p.deal_x.splits = few_splits<true, kCols>(dim, vocab, 1);
+            p.deal_x.splits = few_splits(dim, vocab, 1);
             p.deal_x.partial = static_cast<size_t>(p.deal_x.splits * tokens * mat_round(dim, 4) * 4);
         }
         p.partial = take(p.deal_x.partial);
@@ -602,7 +602,7 @@ int backward(mimir_ctx* ctx, const Call& c, const Plan& p, char* work, const Gra
             } else if constexpr (P == 3) {
                 g.b[0] = as_is(work + p.raw_g, mat_round(c.vocab, 4));
                 g.splits = p.deal_x.splits;
-                st = few_product<true, kCols>(ctx, "cross entropy dx", g, ox);
+                st = few_product<kCols>(ctx, "cross entropy dx", g, ox);
             }
             if (st) return st;
         }

@@ -76,17 +76,16 @@ struct MatAt {
 };
 
 // Every workgroup runs it once; a workgroup of 64 * WGM * WGN threads.
-template <int BM, int BN, int WGM, int WGN, int BK, int STAGES, int PA, int PB, int KA, int KB, bool DUAL = false>
+template <int BM, int BN, int WGM, int WGN, int BK, int PA, int PB, int KA, int KB, bool DUAL = false>
 struct MatShape {
     static constexpr int kM = BM, kN = BN, kWaveM = WGM, kWaveN = WGN, kK = BK, kPa = PA, kPb = PB, kKindA = KA, kKindB = KB;
     static constexpr bool kDual = DUAL;
-    static constexpr int kStages = STAGES;
     static constexpr int kWaves = WGM * WGN, kThreads = kWave * kWaves;
     static constexpr int kBm = BM / WGM / 32, kBn = BN / WGN / 32;  // 32 x 32 blocks of a wave
     static constexpr int kSubs = DUAL ? 2 : 1, kSubRows = BM / kSubs, kSubBlocks = kBm / kSubs;
     static constexpr int kPlaneA = BM * BK * 2, kPlaneB = BN * BK * 2;  // bytes
     static constexpr int kStage = PA * kPlaneA + PB * kPlaneB;
-    static constexpr int kLds = STAGES * kStage;
+    static constexpr int kLds = 2 * kStage;
     static_assert(kLds <= 160 * 1024 && kBm % kSubs == 0 && BK % 16 == 0);
 };
 
@@ -404,39 +403,31 @@ __global__ __launch_bounds__(S::kThreads, S::kThreads == 512 ? 2 : 1) void mat_k
     };
     constexpr int kChunks = S::kK / 16;
     static_assert(kChunks % 2 == 0);
-    // Loads are kStages - 1 steps ahead of the products.  Those of a step are complete
-    // once only the later steps' are out.
-    constexpr int kAhead = S::kStages - 1;
-    constexpr int kLater = (S::kStages - 2) * (S::kPa * S::kSubs * TileA::kLoads + S::kPb * TileB::kLoads);
+    // Loads are a step ahead of the products.
     if (begin < end) {
         seek();
-        for (int i = 0; i < kAhead && begin + i < end; ++i) load(i);
-        if (begin + kAhead <= end) mat_landed<kLater>();
-        else mat_landed<0>();
+        load(0);
+        mat_landed<0>();
         mat_barrier();
         read(0, 0, 0);
     }
     int buf = 0;
     for (int32_t step = begin; step < end; ++step) {
-        if (S::kStages == 2 && fetched < end) load(buf ^ 1);
-        const int next = buf + 1 < S::kStages ? buf + 1 : 0;
+        // The buffer is the step before's, which every wave has read (the last barrier).
+        if (fetched < end) load(buf ^ 1);
 #pragma unroll
         for (int c = 0; c < kChunks; ++c) {
             if (c + 1 < kChunks) {
                 read(buf, c + 1, (c + 1) & 1);
             } else if (step + 1 < end) {
-                if (step + kAhead < end) mat_landed<kLater>();
-                else mat_landed<0>();
+                mat_landed<0>();
                 mat_barrier();
-                read(next, 0, 0);
+                read(buf ^ 1, 0, 0);
             }
             multiply(c & 1);
             mat_interleave<S>();
-            // Behind the first products, which run meanwhile.  The buffer is the step
-            // before's, which every wave has read (the last barrier).
-            if (S::kStages > 2 && c == 0 && fetched < end) load(buf ? buf - 1 : S::kStages - 1);
         }
-        buf = next;
+        buf ^= 1;
     }
     if constexpr (kTwoSums) {
 #pragma unroll
@@ -457,17 +448,17 @@ int64_t mat_tiles(const MatArgs& g) {
 // The two shapes of a product with PA and PB planes: a CU's workgroup of eight waves
 // where such tiles fill most of the GPU, else four waves, two or more to a CU.
 template <int PA, int PB, int KA, int KB, bool DUAL = false>
-using MatBig = std::conditional_t<PA == 3, MatShape<256, 128, 4, 2, 32, 2, 3, 3, KA, KB, DUAL>,
-                                  MatShape<256, 256, 2, 4, 64, 2, PA, PB, KA, KB, DUAL>>;
+using MatBig = std::conditional_t<PA == 3, MatShape<256, 128, 4, 2, 32, 3, 3, KA, KB, DUAL>,
+                                  MatShape<256, 256, 2, 4, 64, PA, PB, KA, KB, DUAL>>;
 template <int PA, int PB, int KA, int KB, bool DUAL = false>
-using MatSmall = std::conditional_t<PA == 3, MatShape<128, 64, 2, 2, 32, 2, 3, 3, KA, KB, DUAL>,
-                                    MatShape<128, 128, 2, 2, 64, 2, PA, PB, KA, KB, DUAL>>;
+using MatSmall = std::conditional_t<PA == 3, MatShape<128, 64, 2, 2, 32, 3, 3, KA, KB, DUAL>,
+                                    MatShape<128, 128, 2, 2, 64, PA, PB, KA, KB, DUAL>>;
 // A contraction of a step or two is over before a workgroup's stores are: smaller
 // stages, so that more workgroups share a CU.
 // Measured, 9 tokens' dw of 32000 x 4096 bf16: 75 us, 154 with stages of 64.  Three
 // planes gain nothing by it (134 us against the larger tiles' 121 for 2 x 4096 x 11008).
 template <int PA, int PB, int KA, int KB>
-using MatThin = MatShape<128, 128, 2, 2, 32, 2, PA, PB, KA, KB>;
+using MatThin = MatShape<128, 128, 2, 2, 32, PA, PB, KA, KB>;
 constexpr int64_t kMatThinK = 64;
 // More than 128 larger tiles are one round of the GPU's CUs where four times as many
 // smaller ones are two rounds of two to a CU.  Measured (larger / smaller), us: fp32
@@ -941,19 +932,18 @@ MatDeal mat_deal(const mimir_ctx* ctx, int64_t m, int64_t n, int64_t k, int64_t 
 // tiles of `tile`.
 int mat_join(mimir_ctx* ctx, const MatOut& o, const MatArgs& g, MatTileSize tile);
 
-// A product of few n into MatOut through slices: workgroups for about two for each CU,
-// each wave with at least four steps.
-template <bool FP32, int KA>
-int few_splits(int64_t m, int64_t k, int segments) {
-    const int64_t tiles = (m + 63) / 64 * segments, steps = (k + (FP32 ? 31 : 63)) / (FP32 ? 32 : 64);
+// An fp32 product of few n into MatOut through slices: workgroups for about two for each
+// CU, each wave with at least four steps of 32.
+inline int few_splits(int64_t m, int64_t k, int segments) {
+    const int64_t tiles = (m + 63) / 64 * segments, steps = (k + 31) / 32;
     return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({512 / std::max<int64_t>(tiles, 1), steps / 16, 64})));
 }
-template <bool FP32, int KA>
+template <int KA>
 int few_product(mimir_ctx* ctx, const char* what, MatArgs g, MatOut o) {
     const int32_t last = o.last, splits = g.splits, segments = g.segments;
     o.ld_partial = mat_slice_ld(g.m);
     o.last = last && splits * segments == 1;
-    if (int st = few_launch<FP32, KA, false>(ctx, what, g, o)) return st;
+    if (int st = few_launch<true, KA, false>(ctx, what, g, o)) return st;
     if (!last || o.last) return MIMIR_OK;
     o.last = 1;
     g.splits = splits * segments;  // mat_join's: as many slices, whatever the tiles

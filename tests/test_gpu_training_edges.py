@@ -7,6 +7,8 @@ import pytest
 import mimir_hip as M
 from _serving import Graph, Hip
 from _training import U, Mat, held
+from test_gpu_gated_linear import hold as hold_gated, make as make_gated, run as run_gated
+from test_gpu_linear_ce import hold as hold_ce, make as make_ce, run as run_ce
 
 pytestmark = pytest.mark.gpu
 
@@ -283,3 +285,28 @@ def test_captures_that_grow(ctx):
             assert np.array_equal(calls[i][3].numpy(), wants[i]), i
         for g in graphs:
             g.close()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("bad", [np.nan, np.inf])
+@pytest.mark.parametrize("tokens,masked", [(1, 1.0), (7, 0.5), (17, 1.0), (32, 0.4)])
+def test_few_tokens_without_target(tuned, tokens, masked, bad, dtype):
+    """As many tokens as take no gathering in the forward: rows that hold anything, targets outside the vocabulary."""
+    x, w, t = make_ce(tokens, tokens, 40, 300, dtype, masked)
+    t[0] = -1
+    none = t < 0
+    t[none] = np.resize(np.array([-1, -100, 300, 2 ** 31 - 1, -2 ** 31], np.int64), none.sum()).astype(np.int32)
+    x2 = x.copy()
+    x2[none] = bad
+    for kw in (dict(), dict(use_mean=False, weight=np.linspace(-1, 2, tokens), scale=0.5)):
+        hold_ce(run_ce(tuned, x2, w, t, dtype, **kw), x, w, t, dtype, **kw)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("tokens", [5, 40])
+def test_rows_far_apart(ctx, tokens, dtype):
+    """Row strides of 2^20 elements and more, which tiles do not take as they are."""
+    x, w, t = make_ce(tokens, tokens, 24, 70, dtype, 0.2)
+    hold_ce(run_ce(ctx, x, w, t, dtype, pad=(1 << 20) - 24 + 8 * (tokens == 5)), x, w, t, dtype)
+    a = make_gated(tokens, tokens, 24, 40, dtype)
+    hold_gated(run_gated(ctx, *a, "silu", dtype, pad=(1 << 20) - 24), *a, "silu", dtype)

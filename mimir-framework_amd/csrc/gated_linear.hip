@@ -265,10 +265,16 @@ Plan plan_of(const mimir_ctx* ctx, const Call& c, bool back) {
     p.x = take(p.x_direct ? 0 : static_cast<size_t>(p.p * c.tokens * p.ld_x * 2));
     p.w = take(p.w_direct || p.few ? 0 : static_cast<size_t>(2 * p.p * c.dim * p.ld_w * 2));
     if (!back) {
-        // Tiles for less than half of the CUs, and a contraction that several can share.
-        constexpr int64_t kFewTiles = 128, kLongDim = 1024;
+        // A contraction long enough that dealing it to several workgroups gains more than the
+        // second pass, of a launch and 16 bytes an element, takes.  The fewer the tiles, the
+        // more it gains, and fp32's six products a step gain more than bf16's one.  Measured,
+        // us, split / whole: fp32 dim 512, 16 to 258 tiles 36 to 56 / 32 to 49; 1024, 120 tiles
+        // 47 / 59, 172 64 / 65, 258 86 / 79; 2048, 250 tiles 133 / 155; 4096, 258 tiles 261 /
+        // 319, 344 709 / 708.  bf16 1024, 16 tiles 18 / 15, 125 30 / 19; 2048, 43 tiles 24 / 29,
+        // 86 31 to 35 / 30 to 32; 4096, 125 tiles 51 / 58, 172 66 / 64.
         const int64_t tn = p.p == 3 ? 64 : 128, tiles = (c.hidden + 63) / 64 * ((c.tokens + tn - 1) / tn);
-        p.split = p.piece >= c.hidden && tiles < kFewTiles && c.dim >= kLongDim && ctx->tune.mat_big != 1;
+        const int64_t least = p.p == 3 ? 1024 : 2048, most = std::min<int64_t>(c.dim / (p.p == 3 ? 8 : 32), 256);
+        p.split = p.piece >= c.hidden && tiles <= most && c.dim >= least && ctx->tune.mat_big != 1;
         if (p.split) {
             p.deal_y = p.p == 3 ? mat_deal<3, 3, kCols, kRows>(ctx, c.hidden, c.tokens, c.dim, 2, false)
                                 : mat_deal<1, 1, kCols, kRows>(ctx, c.hidden, c.tokens, c.dim, 2, false);

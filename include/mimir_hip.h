@@ -560,6 +560,11 @@ int mimir_embedding_f32ids_bwd(mimir_ctx* ctx, const float* ids, int64_t n_ids, 
 /* Element types of these calls' matrices. */
 #define MIMIR_NUM_F32 0
 #define MIMIR_NUM_BF16 1
+/* With MIMIR_NUM_BF16, in the `type` of a gradient (mimir_linear_cross_entropy_bwd,
+ * mimir_gated_linear_bwd): what it holds between its products is held in two bf16 terms
+ * (to 2^-16) with any number of tokens, not in one (2^-8) with more than 128.  The
+ * call takes two to three times as long. */
+#define MIMIR_NUM_TWO_TERMS 0x100
 
 /* Softmax cross entropy of the linear layer z = x w^T over a vocabulary, without z in
  * memory: x [tokens][dim] (row stride ld_x elements), w [vocab][dim] (ld_w; an
@@ -588,7 +593,8 @@ int mimir_linear_cross_entropy_fwd(mimir_ctx* ctx, int type, const void* x, int6
  * So dloss NULL with the forward's mean gives the gradient of the mean loss, and dloss
  * without mean that of any function of the losses.  dx [tokens][dim] and dw
  * [vocab][dim] have `type` (either may be NULL) and are rounded once; for bf16, G is
- * held in bf16 in between (with at most 128 tokens as two bf16 terms).  dx may be x
+ * held in bf16 in between (in two terms with at most 128 tokens, or where `type` has
+ * MIMIR_NUM_TWO_TERMS).  dx may be x
  * with the same stride; they must not overlap any other buffer.  Without tokens the inputs
  * may be NULL: dw is zeroed, or left as it is.  The same call gives the same bits.  Scratch:
  * x's rows again, up to 512 MiB (at least 256 rows of w) for G and w's rows, and fp32
@@ -620,7 +626,8 @@ int mimir_gated_linear_fwd(mimir_ctx* ctx, int type, int act, const void* x, int
  * dx [tokens][dim] (ld_dx) written, or added to where accumulate_x, and dWg, dWu
  * [dim][hidden] (both ld_dw) likewise with accumulate_w; all of `type`, rounded once.
  * dx, or dWg and dWu together, may be NULL.  For bf16, dg and du are held in bf16 in
- * between (with at most 128 tokens as two bf16 terms).  Outputs must not overlap the
+ * between (in two terms with at most 128 tokens, or where `type` has
+ * MIMIR_NUM_TWO_TERMS).  Outputs must not overlap the
  * inputs or one another.  Without tokens the inputs may be NULL: dWg and dWu are zeroed,
  * or left as they are.  The same call gives the same bits.  Scratch: as the
  * forward's, up to 512 MiB (at least 256 columns) with dg and du, and fp32 sums where

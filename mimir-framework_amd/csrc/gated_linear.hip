@@ -211,7 +211,11 @@ __global__ __launch_bounds__(kBlock) void gated_grad(GradArgs a) {
 // --- the work's parts --------------------------------------------------------------
 
 constexpr int64_t kPieceBytes = int64_t{512} << 20;
-constexpr int64_t kTwoPlaneTokens = 128;  // as linear_ce.hip's
+// As linear_ce.hip's.  Measured, gradients of 4096 x 11008 bf16: 64 tokens 148 us, 128 218
+// with two planes, 129 174 with one; the gradients' error is 1.4 times a single rounding's
+// with one, 1.0 with two.  With more tokens (MIMIR_NUM_TWO_TERMS) one / two: 129 173 / 269, 2048
+// 771 / 1817, 8192 2669 / 7624.
+constexpr int64_t kTwoPlaneTokens = 128;
 
 struct Call {
     int type, act;
@@ -242,10 +246,10 @@ bool few_weights(const Call& c) {
 bool few_applies(const Call& c) { return few_weights(c) && few_direct(c.type == MIMIR_NUM_F32, c.x, c.ld_x, c.dim); }
 
 
-Plan plan_of(const mimir_ctx* ctx, const Call& c, bool back) {
+Plan plan_of(const mimir_ctx* ctx, const Call& c, bool back, bool two_terms) {
     Plan p{};
     p.p = c.type == MIMIR_NUM_BF16 ? 1 : 3;
-    p.pg = p.p == 3 ? 3 : c.tokens <= kTwoPlaneTokens ? 2 : 1;
+    p.pg = p.p == 3 ? 3 : two_terms || c.tokens <= kTwoPlaneTokens ? 2 : 1;
     p.x_direct = p.p == 1 && mat_direct(c.x, c.ld_x, c.dim);
     p.w_direct = p.p == 1 && mat_direct(c.w[0], c.ld_w, c.hidden) && mat_direct(c.w[1], c.ld_w, c.hidden);
     p.ld_x = mat_round(c.dim, 8);
@@ -501,7 +505,7 @@ int mimir_gated_linear_fwd(mimir_ctx* ctx, int type, int act, const void* x, int
         if (type == MIMIR_NUM_F32) return act == kSilu ? forward_few<true, kSilu>(ctx, c, y, ld_y, gate_up) : forward_few<true, kGelu>(ctx, c, y, ld_y, gate_up);
         return act == kSilu ? forward_few<false, kSilu>(ctx, c, y, ld_y, gate_up) : forward_few<false, kGelu>(ctx, c, y, ld_y, gate_up);
     }
-    const Plan p = plan_of(ctx, c, false);
+    const Plan p = plan_of(ctx, c, false, false);
     char* work;
     if (int st = mat_scratch(ctx, p.total, &work)) return st;
     if (p.p == 3) return act == kSilu ? forward<3, kSilu>(ctx, c, p, work, y, ld_y, gate_up) : forward<3, kGelu>(ctx, c, p, work, y, ld_y, gate_up);
@@ -514,6 +518,8 @@ int mimir_gated_linear_bwd(mimir_ctx* ctx, int type, int act, const void* x, int
                            int accumulate_w) {
     if (!ctx) return MIMIR_EINVAL;
     const char* what = "gated products' gradient";
+    const bool two_terms = type == (MIMIR_NUM_BF16 | MIMIR_NUM_TWO_TERMS);
+    if (two_terms) type = MIMIR_NUM_BF16;
     const Call c{type, act, x, ld_x, {w_gate, w_up}, ld_w, tokens, dim, hidden};
     if (int st = check(ctx, what, c)) return st;
     MIMIR_REQUIRE(ctx, !dw_gate == !dw_up, "%s: dw_gate and dw_up go together", what);
@@ -530,7 +536,7 @@ int mimir_gated_linear_bwd(mimir_ctx* ctx, int type, int act, const void* x, int
         if (int st = mat_zero(ctx, type, dw_gate, dim, hidden, ld_dw)) return st;
         return mat_zero(ctx, type, dw_up, dim, hidden, ld_dw);
     }
-    const Plan p = plan_of(ctx, c, true);
+    const Plan p = plan_of(ctx, c, true, two_terms);
     char* work;
     if (int st = mat_scratch(ctx, p.total, &work)) return st;
     const Gradients d{gate_up, dy, ld_dy, dx, ld_dx, {dw_gate, dw_up}, ld_dw, accumulate_x ? 1 : 0, accumulate_w ? 1 : 0};

@@ -20,8 +20,9 @@
 // exp(z - m) instead would take tokens x vocab values and the row factors, which are
 // known when the last piece is, could not go into dw's sums.  G without its common
 // factor (scale, and 1 / count for the mean): the factor is applied to the fp32 sums.
-// Rounding G to bf16 beside bf16 operands is off by 2^-8 relative at most a term, as
-// rounding a layer's output gradient is, and averages out in the sums.
+// Rounding G to bf16 beside bf16 operands is off by 2^-8 of a term at most, as rounding a
+// layer's output gradient is, and averages out in the sums; two terms hold it to 2^-16
+// (few tokens, or where the caller asks for it).
 //
 // Tokens without a target take no part: x's counted rows are gathered first, so the
 // products run over those alone, and what stands in the others reaches nothing.
@@ -365,14 +366,20 @@ struct Plan {
 constexpr int64_t kPieceBytes = int64_t{512} << 20;
 constexpr int64_t kTileM = 128;  // the smaller shape's: how many partial results a token has at most
 
-// Few tokens: the products' time is the weights' bytes, and G takes a second plane.
+// G of bf16 operands takes a second plane where tokens are few: up to 64 the products' time
+// is the weights' bytes, and the fewer tokens a sum of dw runs over, the less its terms'
+// roundings average out.  Measured, both gradients, 4096 x 32000: 33 tokens 270 us, 64 279,
+// 128 384 with two planes, 129 290 with one.  With more tokens the caller chooses
+// (MIMIR_NUM_TWO_TERMS): 129 tokens 304 / 475 us with one / two, 2048 1443 / 3028, 8192
+// 5281 / 12372 (twice the products, in the smaller tiles).
 constexpr int64_t kTwoPlaneTokens = 128;
 
-Plan plan_of(const mimir_ctx* ctx, int type, const void* w, int64_t ld_w, int64_t tokens, int64_t dim, int64_t vocab, bool back) {
+Plan plan_of(const mimir_ctx* ctx, int type, const void* w, int64_t ld_w, int64_t tokens, int64_t dim, int64_t vocab, bool back,
+             bool two_terms) {
     Plan p{};
     p.ld = mat_round(dim, 8);
     p.p = type == MIMIR_NUM_BF16 ? 1 : 3;
-    p.pg = p.p == 3 ? 3 : tokens <= kTwoPlaneTokens ? 2 : 1;
+    p.pg = p.p == 3 ? 3 : two_terms || tokens <= kTwoPlaneTokens ? 2 : 1;
     p.w_direct = type == MIMIR_NUM_BF16 && mat_direct(w, ld_w, dim);
     // Few tokens in fp32: w's planes would be five times its bytes on the way.
     p.few = back && p.p == 3 && tokens <= kFewN && vocab <= (1 << 18) && few_direct(true, w, ld_w, dim);
@@ -635,7 +642,7 @@ int mimir_linear_cross_entropy_fwd(mimir_ctx* ctx, int type, const void* x, int6
     if (tokens == 0) return mimir_fill_f32(ctx, mean, 2, 0.0f);
     if (few_applies(c))
         return type == MIMIR_NUM_F32 ? forward_few<true>(ctx, c, loss, lse, mean) : forward_few<false>(ctx, c, loss, lse, mean);
-    const Plan p = plan_of(ctx, type, w, ld_w, tokens, dim, vocab, false);
+    const Plan p = plan_of(ctx, type, w, ld_w, tokens, dim, vocab, false, false);
     char* work;
     if (int st = mat_scratch(ctx, p.total, &work)) return st;
     auto* count = reinterpret_cast<int32_t*>(work + p.count);
@@ -651,6 +658,8 @@ int mimir_linear_cross_entropy_bwd(mimir_ctx* ctx, int type, const void* x, int6
                                    void* dw, int64_t ld_dw, int accumulate_w) {
     if (!ctx) return MIMIR_EINVAL;
     const char* what = "linear cross entropy gradient";
+    const bool two_terms = type == (MIMIR_NUM_BF16 | MIMIR_NUM_TWO_TERMS);
+    if (two_terms) type = MIMIR_NUM_BF16;
     const Call c{type, x, ld_x, w, ld_w, targets, tokens, dim, vocab};
     if (int st = check(ctx, what, c)) return st;
     MIMIR_REQUIRE(ctx, (!dx || ld_dx >= dim) && (!dw || ld_dw >= dim), "%s: gradient strides (%lld, %lld) below dim", what,
@@ -663,7 +672,7 @@ int mimir_linear_cross_entropy_bwd(mimir_ctx* ctx, int type, const void* x, int6
     MIMIR_ENTER(ctx);
     // Without tokens no input is looked at (w may be null).
     if (tokens == 0) return dw && !accumulate_w ? mat_zero(ctx, type, dw, vocab, dim, ld_dw) : MIMIR_OK;
-    Plan p = plan_of(ctx, type, w, ld_w, tokens, dim, vocab, true);
+    Plan p = plan_of(ctx, type, w, ld_w, tokens, dim, vocab, true, two_terms);
     char* work;
     if (int st = mat_scratch(ctx, p.total, &work)) return st;
     auto* count = reinterpret_cast<int32_t*>(work + p.count);

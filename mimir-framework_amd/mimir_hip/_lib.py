@@ -34,6 +34,7 @@ KV_TYPES = ("f32", "bf16", "i8")
 ROPE_SCALINGS = ("none", "linear", "base", "by_parts")
 # MIMIR_NUM_* (element types of the training calls' matrices), in order.
 NUM_TYPES = ("f32", "bf16")
+NUM_TWO_TERMS = 0x100  # MIMIR_NUM_TWO_TERMS
 # MIMIR_ACT_*, in order.
 ACTIVATIONS = ("silu", "gelu")
 MERGE_OPS = ("ADD", "MULTIPLY", "CONCATENATE", "MAX", "AVERAGE", "GATED", "ATTENTION_WEIGHTED")

@@ -85,6 +85,13 @@ def _num(dtype):
     return _lib.NUM_TYPES.index(dtype)
 
 
+def _num_bwd(dtype, two_terms):
+    """The same of a gradient, MIMIR_NUM_TWO_TERMS with it."""
+    if two_terms and dtype != "bf16":
+        raise ValueError(f"two_terms is for bf16, not {dtype!r}")
+    return _num(dtype) | (_lib.NUM_TWO_TERMS if two_terms else 0)
+
+
 def _act(name):
     """MIMIR_ACT_* of "silu" or "gelu"."""
     if name not in _lib.ACTIVATIONS:
@@ -350,11 +357,13 @@ class Context:
                                                            _ptr(targets), tokens, dim, vocab, _ptr(loss), _ptr(lse), _ptr(mean)))
 
     def linear_cross_entropy_bwd(self, x, w, targets, lse, dloss, mean, dx, dw, tokens, dim, vocab, scale=1.0, dtype="f32",
-                                 ld_x=None, ld_w=None, ld_dx=None, ld_dw=None, accumulate_x=False, accumulate_w=False):
+                                 ld_x=None, ld_w=None, ld_dx=None, ld_dw=None, accumulate_x=False, accumulate_w=False,
+                                 two_terms=False):
         """mimir_linear_cross_entropy_bwd: dx and dw (either may be None); dloss None
-        and the forward's mean give the gradient of the mean loss."""
+        and the forward's mean give the gradient of the mean loss; two_terms
+        (MIMIR_NUM_TWO_TERMS) for bf16 gradients rounded only once at the end."""
         self.check(self.lib.mimir_linear_cross_entropy_bwd(
-            self.handle, _num(dtype), _ptr(x), ld_x or dim, _ptr(w), ld_w or dim, _ptr(targets), tokens, dim, vocab, _ptr(lse),
+            self.handle, _num_bwd(dtype, two_terms), _ptr(x), ld_x or dim, _ptr(w), ld_w or dim, _ptr(targets), tokens, dim, vocab, _ptr(lse),
             _ptr(dloss), _ptr(mean), float(scale), _ptr(dx), ld_dx or dim, int(bool(accumulate_x)), _ptr(dw), ld_dw or dim,
             int(bool(accumulate_w))))
 
@@ -367,10 +376,12 @@ class Context:
                                                    _ptr(gate_up)))
 
     def gated_linear_bwd(self, x, w_gate, w_up, gate_up, dy, dx, dw_gate, dw_up, tokens, dim, hidden, act="silu", dtype="f32",
-                         ld_x=None, ld_w=None, ld_dy=None, ld_dx=None, ld_dw=None, accumulate_x=False, accumulate_w=False):
-        """mimir_gated_linear_bwd: dx, dw_gate and dw_up (dx, or the latter two, may be None)."""
+                         ld_x=None, ld_w=None, ld_dy=None, ld_dx=None, ld_dw=None, accumulate_x=False, accumulate_w=False,
+                         two_terms=False):
+        """mimir_gated_linear_bwd: dx, dw_gate and dw_up (dx, or the latter two, may be
+        None); two_terms as linear_cross_entropy_bwd's."""
         self.check(self.lib.mimir_gated_linear_bwd(
-            self.handle, _num(dtype), _act(act), _ptr(x), ld_x or dim, _ptr(w_gate), _ptr(w_up), ld_w or hidden, tokens, dim,
+            self.handle, _num_bwd(dtype, two_terms), _act(act), _ptr(x), ld_x or dim, _ptr(w_gate), _ptr(w_up), ld_w or hidden, tokens, dim,
             hidden, _ptr(gate_up), _ptr(dy), ld_dy or hidden, _ptr(dx), ld_dx or dim, int(bool(accumulate_x)), _ptr(dw_gate),
             _ptr(dw_up), ld_dw or hidden, int(bool(accumulate_w))))
 

@@ -48,6 +48,17 @@ int main() {
     expect(__LINE__, false, gated_bwd(7, 8, 9));
     for (int in : {1, 2, 3, 5, 6, 8, 9}) expect(__LINE__, true, gated_bwd(in, 8, 9));
     for (int in : {1, 2, 3, 5, 6, 7, 9}) expect(__LINE__, true, gated_bwd(7, in, 9)), expect(__LINE__, true, gated_bwd(7, 8, in == 9 ? 8 : in));
+    // Two terms: with bf16 in a gradient's type alone.
+    for (int type : {MIMIR_NUM_F32, MIMIR_NUM_BF16, 2})
+        for (int with : {0, MIMIR_NUM_TWO_TERMS}) {
+            const bool grad = type == 2 || (with && type != MIMIR_NUM_BF16), fwd = type == 2 || with;
+            expect(__LINE__, fwd, mimir_linear_cross_entropy_fwd(ctx, type | with, m[1], 4, m[2], 4, ids, 2, 4, 3, m[3], m[4], m[5]));
+            expect(__LINE__, grad, mimir_linear_cross_entropy_bwd(ctx, type | with, m[1], 4, m[2], 4, ids, 2, 4, 3, m[4], nullptr, nullptr,
+                                                                  1.0f, m[7], 4, 0, m[8], 4, 0));
+            expect(__LINE__, fwd, mimir_gated_linear_fwd(ctx, type | with, 0, m[1], 4, m[2], m[3], 5, 2, 4, 5, m[4], 5, m[5]));
+            expect(__LINE__, grad, mimir_gated_linear_bwd(ctx, type | with, 0, m[1], 4, m[2], m[3], 5, 2, 4, 5, m[5], m[6], 5, m[7], 4, 0,
+                                                          m[8], m[9], 5, 0));
+        }
     std::printf("training buffers: %d failures\n", failures);
     return failures != 0;
 }

@@ -461,9 +461,11 @@ template <int PA, int PB, int KA, int KB>
 using MatThin = MatShape<128, 128, 2, 2, 32, PA, PB, KA, KB>;
 constexpr int64_t kMatThinK = 64;
 // More than 128 larger tiles are one round of the GPU's CUs where four times as many
-// smaller ones are two rounds of two to a CU.  Measured (larger / smaller), us: fp32
-// 1024 x 1021 x 2752 gated, 176 tiles 76 / 85, its dw 72 / 80; 700 x 300 x 1500, 40 tiles 45 /
-// 31; bf16 1001 x 777 x 50001 statistics, 784 tiles 103 / 120.
+// smaller ones are two rounds of two to a CU; up to 128 they are one round of both.
+// Measured, a cross entropy's forward, us, larger / smaller tiles: bf16 512 x 4096 x 16384,
+// 128 larger tiles, 98 / 82, x 17000, 134 of them, 97 / 125; 64 x 4096 x 32000, 125, 104 / 81;
+// 1024 x 1024 x 8192, 128, 41 / 33, x 8500, 136, 42 / 46; fp32 512 x 2048 x 8192, 128, 163 /
+// 141, x 8500, 136, 165 / 204; 256 x 512 x 16384, 128, 63 / 56, x 17000, 134, 65 / 74.
 constexpr int64_t kMatBigTiles = 129;
 template <class S>
 bool mat_fills(const mimir_ctx* ctx, const MatArgs& g) {

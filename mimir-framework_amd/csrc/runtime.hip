@@ -93,7 +93,8 @@ int mimir::graph_unpin(mimir_ctx* ctx) {
 
 int mimir::ensure_scratch(mimir_ctx* ctx, size_t bytes, void** out) {
     if (bytes > ctx->scratch_bytes) {
-        size_t want = bytes < (size_t(1) << 20) ? (size_t(1) << 20) : bytes;
+        const size_t least = bytes < (size_t(1) << 20) ? (size_t(1) << 20) : bytes;
+        size_t want = least;
         if (ctx->scratch) {
             if (ctx->scratch_held) {
                 // By half at least, so that captures of larger and larger calls keep no
@@ -109,6 +110,10 @@ int mimir::ensure_scratch(mimir_ctx* ctx, size_t bytes, void** out) {
             ctx->scratch_held = false;
         }
         hipError_t e = hipMalloc(&ctx->scratch, want);
+        if (e != hipSuccess && want > least) {
+            (void)hipGetLastError();
+            e = hipMalloc(&ctx->scratch, want = least);
+        }
         if (e != hipSuccess) {
             (void)hipGetLastError();
             ctx->scratch = nullptr;

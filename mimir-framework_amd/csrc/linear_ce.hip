@@ -16,9 +16,10 @@
 //
 // Backward: the same product again for a piece of the vocabulary, whose epilogue
 // writes G in bf16 (three planes for fp32 operands), then the two products with G.
-// The logits again cost a third of what the gradients' products do; keeping
-// exp(z - m) instead would take tokens x vocab values and the row factors, which are
-// known when the last piece is, could not go into dw's sums.  G without its common
+// The logits again are a third of the backward's products: kept, they would be
+// tokens x vocab values of memory from the one call to the other.  (A single call for the
+// loss and its gradients could take the tokens in pieces and keep a piece's logits; with
+// two, a program has the loss first and weighs it.)  G without its common
 // factor (scale, and 1 / count for the mean): the factor is applied to the fp32 sums.
 // Rounding G to bf16 beside bf16 operands is off by 2^-8 of a term at most, as rounding a
 // layer's output gradient is, and averages out in the sums; two terms hold it to 2^-16
@@ -44,7 +45,8 @@ constexpr float kLowest = -3.40282347e38f;
 
 // exp(z - m).  The difference first: z log2 e - m log2 e in one step is off by the rounding
 // of m log2 e, so that the maximum itself would not give 1, a sum could come out below 1
-// and a loss below 0, by more the larger the logits are.
+// and a loss below 0, by more the larger the logits are.  (2048 tokens x 4096 x 32000 bf16
+// forward 461 us, 458 in one step.)
 __device__ __forceinline__ float exp_from(float z, float m) { return __builtin_amdgcn_exp2f((z - m) * kLog2e); }
 
 // --- the counted rows --------------------------------------------------------------

@@ -17,9 +17,10 @@
 // two batches of another.  The pass is bound by its bytes (20 or 12 a value beside
 // 4 or 12 written), the products by the matrix cores.
 //
-// Measured on MI355X, us: 2048 tokens x 4096 x 11008 bf16 forward 337 (1.10 PFLOP/s); 8192
-// tokens forward and backward 4267 (forward 1553, the pass 257 = 5.6 TB/s, dx 1218, both
-// weights' 1269); 1021 x 1024 x 2752 fp32 both 258; 7 tokens fp32 forward 16.9.
+// Measured on MI355X, us: 2048 tokens x 4096 x 11008 bf16 forward 335 (1.10 PFLOP/s); 8192
+// tokens forward and backward 4370 (forward 1562, the pass 258 = 5.6 TB/s, dx 1249, both
+// weights' 1300); 1021 x 1024 x 2752 fp32 both 258; 7 tokens fp32 forward 17.4; 8 tokens x
+// 4096 x 11008 forward 40 bf16 and 111 fp32, backward 106 and 210.
 #include "matrix.hpp"
 #include "pointwise.hpp"
 

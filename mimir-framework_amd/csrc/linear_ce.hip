@@ -28,9 +28,10 @@
 // Tokens without a target take no part: x's counted rows are gathered first, so the
 // products run over those alone, and what stands in the others reaches nothing.
 //
-// Measured on MI355X, us: 2048 tokens x 4096 x 32000 bf16 forward 453 (the product 447);
-// 8192 tokens forward and backward 7160 (products 1756, 1912, 1694, 1781); 32 tokens 55, the
-// weights' 262 MB at 6.1 TB/s in the kernel; 17 x 256 x 1000 fp32 10.5, two launches.
+// Measured on MI355X, us: 2048 tokens x 4096 x 32000 bf16 forward 461 to 472; 8192 tokens
+// forward and backward 7180 (products 1758, 1846, 1685, 1759); 32 tokens forward 55, the
+// weights' 262 MB at 6.2 TB/s in the kernel, backward 64 for G and 76 and 73 for dx and dw;
+// fp32 136, 116 and 177; 17 x 256 x 1000 fp32 10.7, two launches.
 #include "matrix.hpp"
 
 #include <algorithm>

@@ -30,12 +30,14 @@
 // is a multiple of 8 and the operand 16-byte aligned.
 //
 // Bound by the power of the matrix cores.  Measured on MI355X (bf16, 8192 tokens, 4096 x
-// 32000): with the cross entropy's statistics 1756 us = 1.22 PFLOP/s, gradients 1694 (A
-// across the contraction) and 1781 us (both); the library's product of this shape 1492 us.
-// 2048 tokens 447 us = 1.20, the library 445.  The matrix cores are busy 55 to 60% of the
+// 32000): with the cross entropy's statistics 1758 us = 1.22 PFLOP/s, with its gradient 1846,
+// the gradient's products 1685 (A across the contraction) and 1759 us (both); the library's
+// product of this shape 1492 us.  2048 tokens 440 to 475 us = 1.13 to 1.22, the library 445.
+// The matrix cores are busy 55 to 60% of the
 // cycles at 1.9 GHz; without its global loads the kernel takes 0.83, without its LDS reads
-// 0.90 of the time, at lower clocks the fuller they are.  fp32, 614 x 1024 x 32000: 222 to
-// 255 us = 158 to 181 TFLOP/s, where fp32 matrix instructions peak at 157.
+// 0.90 of the time, at lower clocks the fuller they are.  fp32, 614 x 1024 x 32000: 225 to
+// 260 us = 155 to 179 TFLOP/s, where fp32 matrix instructions peak at 157; with the cross
+// entropy's gradient, stored in three planes, 294.
 #pragma once
 
 #include "internal.hpp"
@@ -498,9 +500,10 @@ typedef uint32_t u2e __attribute__((ext_vector_type(2), aligned(2)));
 // LDS.  FP32: both operands are fp32 in memory and are split as they are read from LDS
 // (their planes would be five times the bytes on the way).  Of each wave's three stages
 // two are on their way: 4 waves of 2 x 8 KB of A a CU are 17 MB in flight on the GPU.
-// Measured: 32 x 4096 x 32000 bf16 43 us in the kernel, 6.1 TB/s; kCols operands, whose
-// tiles are 64 or 128 bytes of each row, 2.7 TB/s (5 x 4096 x 11008 fp32, both weights,
-// 134 us).
+// Measured: 32 x 4096 x 32000 bf16 42 us in the kernel, 6.2 TB/s (75 behind a step whose
+// gradients, as large, are on their way to memory); 17 x 4096 x 32000 fp32 128 us, 4.1 TB/s;
+// kCols operands, whose tiles are 64 or 128 bytes of each row, 8 x 4096 x 11008, both
+// weights: bf16 40 us = 4.5 TB/s, fp32 111 = 3.2.
 
 constexpr int kFewN = 32;
 

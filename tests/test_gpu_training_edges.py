@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 
 import mimir_hip as M
-from _serving import Graph, Hip
+from _serving import Graph, Hip, bf16_value
 from _training import U, Mat, held
 from test_gpu_gated_linear import hold as hold_gated, make as make_gated, run as run_gated
 from test_gpu_linear_ce import hold as hold_ce, make as make_ce, run as run_ce
@@ -310,3 +310,51 @@ def test_rows_far_apart(ctx, tokens, dtype):
     hold_ce(run_ce(ctx, x, w, t, dtype, pad=(1 << 20) - 24 + 8 * (tokens == 5)), x, w, t, dtype)
     a = make_gated(tokens, tokens, 24, 40, dtype)
     hold_gated(run_gated(ctx, *a, "silu", dtype, pad=(1 << 20) - 24), *a, "silu", dtype)
+
+
+class AmongNans(Mat):
+    """A matrix whose buffer holds NaN around and between its rows."""
+
+    FILL = np.float32(np.nan)
+
+    def get(self):
+        b = self.dev.numpy()
+        b = bf16_value(b) if self.dtype == "bf16" else b
+        rows, cols = self.shape
+        n = self.at + rows * self.ld
+        body = b[self.at:n].reshape(rows, self.ld)
+        assert np.isnan(b[:self.at]).all() and np.isnan(b[n:]).all() and np.isnan(body[:, cols:]).all()
+        return body[:, :cols].copy()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("pad,offset", [(0, 3), (8, 8), (5, 1), (1, 0)])
+@pytest.mark.parametrize("tokens,dim,vocab", [(5, 6, 70), (31, 37, 130), (17, 64, 257), (3, 1003, 65), (40, 48, 333), (150, 129, 300)])
+def test_nans_between_the_rows(tuned, monkeypatch, tokens, dim, vocab, pad, offset, dtype):
+    """Nothing around the rows is looked at: a product with a NaN would show, also one with 0."""
+    import test_gpu_gated_linear
+    import test_gpu_linear_ce
+    monkeypatch.setattr(test_gpu_linear_ce, "Mat", AmongNans)
+    monkeypatch.setattr(test_gpu_gated_linear, "Mat", AmongNans)
+    x, w, t = make_ce(tokens + dim, tokens, dim, vocab, dtype, 0.2)
+    hold_ce(run_ce(tuned, x, w, t, dtype, pad=pad, offset=offset), x, w, t, dtype)
+    a = make_gated(tokens + dim, tokens, dim, vocab, dtype)
+    hold_gated(run_gated(tuned, *a, "gelu", dtype, pad=pad, offset=offset), *a, "gelu", dtype)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("tokens,dim,vocab,masked", [(7, 24, 70, 0.5), (32, 1003, 335, 0.3), (2, 5, 100, 0.0), (20, 64, 3, 0.2), (45, 41, 333, 0.6), (130, 100, 513, 0.3), (300, 40, 777, 0.9)])
+def test_scratch_full_of_nans(tuned, tokens, dim, vocab, masked, dtype):
+    """What calls of NaN left in the scratch, in planes, sums, statistics and gradients, reaches no later call."""
+    for kind in ("f32", "bf16"):
+        nan = [np.full(s, np.nan, np.float32) for s in ((400, 1100), (900, 1100))]
+        X, W = Mat(tuned, nan[0], kind), Mat(tuned, nan[1], kind)
+        t, out = tuned.to_device(np.zeros(400, np.int32)), [tuned.empty(400), tuned.empty(400), tuned.empty(2)]
+        DX, DW = Mat(tuned, nan[0], kind), Mat(tuned, nan[1], kind)
+        tuned.linear_cross_entropy(X.ptr, W.ptr, t, 400, 1100, 900, *out, dtype=kind)
+        tuned.linear_cross_entropy_bwd(X.ptr, W.ptr, t, out[1], None, out[2], DX.ptr, DW.ptr, 400, 1100, 900, dtype=kind)
+        assert np.isnan(DX.get()).all()
+    x, w, t = make_ce(tokens + dim, tokens, dim, vocab, dtype, masked)
+    hold_ce(run_ce(tuned, x, w, t, dtype, pad=3), x, w, t, dtype)
+    a = make_gated(tokens + dim, tokens, dim, vocab, dtype)
+    hold_gated(run_gated(tuned, *a, "silu", dtype), *a, "silu", dtype)

@@ -80,8 +80,11 @@ int mimir::retire_or_free(mimir_ctx* ctx, void* p) {
         ctx->retired.push_back(p);
         return MIMIR_OK;
     }
-    ctx->retired.push_back(p);  // beside those that a capture left, if any
-    return free_retired(ctx);
+    // Those that a capture left go with it; where the stream cannot be waited for, p stays
+    // the caller's.
+    if (int st = free_retired(ctx)) return st;
+    (void)hipFree(p);
+    return MIMIR_OK;
 }
 
 void mimir::graph_pin(mimir_ctx* ctx) { ++ctx->graph_pins; }

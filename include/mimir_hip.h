@@ -563,7 +563,7 @@ int mimir_embedding_f32ids_bwd(mimir_ctx* ctx, const float* ids, int64_t n_ids, 
 /* With MIMIR_NUM_BF16, in the `type` of a gradient (mimir_linear_cross_entropy_bwd,
  * mimir_gated_linear_bwd): what it holds between its products is held in two bf16 terms
  * (to 2^-16) with any number of tokens, not in one (2^-8) with more than 128.  The
- * call takes two to three times as long. */
+ * call takes 1.3 to 3 times as long. */
 #define MIMIR_NUM_TWO_TERMS 0x100
 
 /* Softmax cross entropy of the linear layer z = x w^T over a vocabulary, without z in

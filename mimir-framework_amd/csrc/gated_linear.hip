@@ -212,9 +212,9 @@ __global__ __launch_bounds__(kBlock) void gated_grad(GradArgs a) {
 // --- the work's parts --------------------------------------------------------------
 
 constexpr int64_t kPieceBytes = int64_t{512} << 20;
-// As linear_ce.hip's.  Measured, gradients of 4096 x 11008 bf16: 64 tokens 148 us, 128 218
-// with two planes, 129 174 with one; the gradients' error is 1.4 times a single rounding's
-// with one, 1.0 with two.  With more tokens (MIMIR_NUM_TWO_TERMS) one / two: 129 173 / 269, 2048
+// As linear_ce.hip's.  Measured, gradients of 4096 x 11008 bf16: 64 tokens 147 us, 128 177
+// with two planes, 129 153 with one; the gradients' error is 1.4 times a single rounding's
+// with one, 1.0 with two.  With more tokens (MIMIR_NUM_TWO_TERMS) one / two: 129 156 / 223, 2048
 // 771 / 1817, 8192 2669 / 7624.
 constexpr int64_t kTwoPlaneTokens = 128;
 

@@ -371,9 +371,9 @@ constexpr int64_t kTileM = 128;  // the smaller shape's: how many partial result
 
 // G of bf16 operands takes a second plane where tokens are few: up to 64 the products' time
 // is the weights' bytes, and the fewer tokens a sum of dw runs over, the less its terms'
-// roundings average out.  Measured, both gradients, 4096 x 32000: 33 tokens 270 us, 64 279,
-// 128 384 with two planes, 129 290 with one.  With more tokens the caller chooses
-// (MIMIR_NUM_TWO_TERMS): 129 tokens 304 / 475 us with one / two, 2048 1443 / 3028, 8192
+// roundings average out.  Measured, both gradients, 4096 x 32000: 33 tokens 270 us, 64 284,
+// 128 322 with two planes, 129 286 with one.  With more tokens the caller chooses
+// (MIMIR_NUM_TWO_TERMS): 129 tokens 290 / 386 us with one / two, 2048 1443 / 3028, 8192
 // 5281 / 12372 (twice the products, in the smaller tiles).
 constexpr int64_t kTwoPlaneTokens = 128;
 

@@ -455,13 +455,16 @@ using MatBig = std::conditional_t<PA == 3, MatShape<256, 128, 4, 2, 32, 3, 3, KA
 template <int PA, int PB, int KA, int KB, bool DUAL = false>
 using MatSmall = std::conditional_t<PA == 3, MatShape<128, 64, 2, 2, 32, 3, 3, KA, KB, DUAL>,
                                     MatShape<128, 128, 2, 2, 64, PA, PB, KA, KB, DUAL>>;
-// A contraction of a step or two is over before a workgroup's stores are: smaller
+// A contraction of a few steps is over before a workgroup's stores are: smaller
 // stages, so that more workgroups share a CU.
-// Measured, 9 tokens' dw of 32000 x 4096 bf16: 75 us, 154 with stages of 64.  Three
-// planes gain nothing by it (134 us against the larger tiles' 121 for 2 x 4096 x 11008).
+// Measured, both gradients, us, these / the others: cross entropy bf16 4096 x 32000, 9
+// tokens' dw alone 75 / 154, 65 tokens 290 / 362, 128 322 / 383, 256 342 / 340, 400 452 / 435,
+// 512 499 / 465; gated 4096 x 11008, 65 tokens 152 / 207, 256 183 / 203, 512 266 / 268, 700
+// 345 / 333.  Three planes gain nothing by it (134 us against the larger tiles' 121 for 2 x
+// 4096 x 11008).
 template <int PA, int PB, int KA, int KB>
 using MatThin = MatShape<128, 128, 2, 2, 32, PA, PB, KA, KB>;
-constexpr int64_t kMatThinK = 64;
+constexpr int64_t kMatThinK = 256;
 // More than 128 larger tiles are one round of the GPU's CUs where four times as many
 // smaller ones are two rounds of two to a CU; up to 128 they are one round of both.
 // Measured, a cross entropy's forward, us, larger / smaller tiles: bf16 512 x 4096 x 16384,

@@ -29,9 +29,9 @@ static void pieces(const MatDealRule& r, int64_t tokens, int64_t dim, int64_t hi
 
 int main() {
     // The rules of the shapes in matrix.hpp: fp32, bf16, two planes beside one.
-    MatDealRule rules[] = {{{256, 128}, {128, 64}, true, false, 129, 64, -1},
-                           {{256, 256}, {128, 128}, true, true, 129, 64, -1},
-                           {{128, 128}, {128, 128}, false, true, 129, 64, -1}};
+    MatDealRule rules[] = {{{256, 128}, {128, 64}, true, false, 129, 256, -1},
+                           {{256, 256}, {128, 128}, true, true, 129, 256, -1},
+                           {{128, 128}, {128, 128}, false, true, 129, 256, -1}};
     // A short last piece behind a full one: 24 tiles where the room was made for 320.
     pieces(rules[0], 8192, 256, 5400, 5120, "fp32 8192 x 256 x 5400");
     pieces(rules[1], 131072, 1024, 1280, 1024, "bf16 131072 x 1024 x 1280");
